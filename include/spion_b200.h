@@ -37,6 +37,7 @@ enum {
 };
 
 enum { SPION_F32 = 0, SPION_BF16 = 1 };
+enum { SPION_F16 = 2, SPION_E4M3 = 3 };      /* the encoder's operators only: norms, 8-bit linear layers, optimizer */
 enum { SPION_CONV_DIAG = 0, SPION_CONV_BOX = 1 };
 enum { SPION_SELECT_PATHS = 0, SPION_SELECT_TOPK = 1 };
 enum { SPION_KIND_DENSE = 0, SPION_KIND_DENSE_KPM = 1, SPION_KIND_BLOCK = 2, SPION_KIND_BLOCK_KPM = 3 };
@@ -475,6 +476,23 @@ int spion_linear_prepare(int fp32);
 int spion_linear_status(int reset);
 /* Failure-path self-test that faults nothing, as spion_selftest_bounded_wait: the status word is set afterwards. */
 int spion_linear_selftest_bounded_wait(long long limit_cycles, void* cuda_stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Root-mean-square norm of [M, N] rows, with the addition of a residual before it: s = x + res (rounded to x's type), rstd = (mean s^2 + eps)^(-1/2),
+ * y = s w rstd.  Types: x SPION_F32, SPION_BF16 or SPION_F16; res of x's type, or 16 bits beside an fp32 x; y of x's type, 16 bits beside an fp32 x,
+ * or SPION_E4M3 with a scale per row (y = value * scale, the row's largest |y| at 448).  Row strides ldx, ldr (>= 0) and ldy (>= N) in elements; sum_out
+ * [M, N] (with res), may not overlap an input.  w [N] of any of the three types, or NULL (ones).  rstd [M] may be NULL.  norm == 0: rows to e4m3 as
+ * they are (y_type SPION_E4M3, no w, no res).  Any width; widths of a multiple of 8 with rows on 16-byte boundaries (32 for fp32) are faster. */
+int spion_rmsnorm_forward(const void* x, long long ldx, int x_type, const void* res, long long ldr, int res_type, const void* w, int w_type,
+                          void* sum_out, void* y, long long ldy, int y_type, float* scale, float* rstd, long long M, int N, float eps, int norm,
+                          void* cuda_stream);
+/* Its backward from s (rows lds apart), dy [M, N] (the type of y) and ds [M, N] (the type of s; may be NULL: the gradient of s from its other
+ * consumers): dx [M, N] in s's type and dres [M, N], the same in 16 bits (either may be NULL), dw [N] in w's type (may be NULL), summed in a fixed order.
+ * workspace: spion_rmsnorm_workspace_floats(M, N) floats (with dw). */
+long long spion_rmsnorm_workspace_floats(long long M, int N);
+int spion_rmsnorm_backward(const void* s, long long lds, int s_type, const void* dy, int dy_type, const void* ds, const void* w, int w_type,
+                           const float* rstd, void* dx, void* dres, int dres_type, void* dw, float* workspace, long long M, int N,
+                           void* cuda_stream);
 
 #ifdef __cplusplus
 }

@@ -13,7 +13,7 @@ LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib")
 # SPION_B200_LIBRARY names another build of the same library (e.g. one compiled with developer macros)
 LIB_PATH = os.environ.get("SPION_B200_LIBRARY") or os.path.join(LIB_DIR, "libspion_b200.so")
 
-F32, BF16 = 0, 1
+F32, BF16, F16, E4M3 = 0, 1, 2, 3
 CONV_DIAG, CONV_BOX = 0, 1
 SELECT_PATHS, SELECT_TOPK = 0, 1
 KIND_DENSE, KIND_DENSE_KPM, KIND_BLOCK, KIND_BLOCK_KPM = 0, 1, 2, 3
@@ -108,6 +108,11 @@ SIGNATURES = {
     "spion_linear_prepare": (c_int, [c_int]),
     "spion_linear_status": (c_int, [c_int]),
     "spion_linear_selftest_bounded_wait": (c_int, [c_longlong, c_void_p]),
+    "spion_rmsnorm_forward": (c_int, [c_void_p, c_longlong, c_int] * 2 + [c_void_p, c_int, c_void_p, c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_longlong,
+                                      c_int, ctypes.c_float, c_int, c_void_p]),
+    "spion_rmsnorm_workspace_floats": (c_longlong, [c_longlong, c_int]),
+    "spion_rmsnorm_backward": (c_int, [c_void_p, c_longlong, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                                       c_void_p, c_longlong, c_int, c_void_p]),
     "spion_static_scratch_capacity": (ctypes.c_size_t, []),
     "spion_attn_forward_static": (c_int, [c_void_p] * 9 + [c_int] * 6 + [c_void_p]),
 }

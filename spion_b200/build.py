@@ -6,7 +6,7 @@ Outputs (git-ignored, but shipped with the working tree):
     spion_b200/lib/libspion_b200.so        all kernels + the C ABI of include/spion_b200.h
     spion_b200/lib/{attn,attn_mask,block_attn,block_attn_mask}.so
                                            shims with the reference's own symbol names
-    spion_b200/lib/_torch_ops.so           autograd nodes of the Python modules (csrc/torch_ops.cpp)
+    spion_b200/lib/_torch_ops.so           autograd nodes of the Python modules (csrc/torch_ops.cpp, torch_encoder_ops.cpp)
 """
 from __future__ import annotations
 
@@ -76,18 +76,21 @@ def build_torch_ops(main, force: bool = False) -> str:
 
     import torch
     from torch.utils import cpp_extension
-    src = os.path.join(CSRC, "torch_ops.cpp")
+    srcs = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "torch_encoder_ops.cpp")]
     out = os.path.join(LIB, "_torch_ops.so")
-    header = os.path.join(os.path.dirname(HERE), "include", "spion_b200.h")
-    if not force and not _newer([src, header, main], out):
+    headers = [os.path.join(os.path.dirname(HERE), "include", "spion_b200.h"), os.path.join(CSRC, "torch_common.h")]
+    if not force and not _newer(srcs + headers + [main], out):
         return out
     inc = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")]
     tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    obj = os.path.join(OBJ, "torch_ops.o")
-    if force or _newer([src, header], obj):
-        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-w", "-DTORCH_EXTENSION_NAME=_torch_ops", "-DTORCH_API_INCLUDE_EXTENSION_H",
-              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + ["-I" + i for i in inc] + ["-c", src, "-o", obj])
-    _run(["g++", "-shared", obj, "-o", out, "-L" + LIB, "-lspion_b200", "-L" + tlib, "-ltorch_python", "-ltorch", "-ltorch_cpu",
+    objs = []
+    for src in srcs:
+        obj = os.path.join(OBJ, os.path.basename(src)[:-4] + ".o")
+        objs.append(obj)
+        if force or _newer([src] + headers, obj):
+            _run(["g++", "-O2", "-std=c++17", "-fPIC", "-w", "-DTORCH_EXTENSION_NAME=_torch_ops", "-DTORCH_API_INCLUDE_EXTENSION_H",
+                  f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + ["-I" + i for i in inc] + ["-c", src, "-o", obj])
+    _run(["g++", "-shared"] + objs + ["-o", out, "-L" + LIB, "-lspion_b200", "-L" + tlib, "-ltorch_python", "-ltorch", "-ltorch_cpu",
           "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
     return out
 
