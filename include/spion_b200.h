@@ -494,6 +494,25 @@ int spion_rmsnorm_backward(const void* s, long long lds, int s_type, const void*
                            const float* rstd, void* dx, void* dres, int dres_type, void* dw, float* workspace, long long M, int N,
                            void* cuda_stream);
 
+/* ------------------------------------------------------------------------------------------
+ * One AdamW step over many tensors: t += 1; g = clamp(g, -clip, clip); m = b1 m + (1 - b1) g; v = b2 v + (1 - b2) g^2;
+ * p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps).  Parameters and gradients of one type (SPION_F32, SPION_BF16, SPION_F16),
+ * contiguous; tensors may not overlap.  The moments of all tensors lie in one array each: a tensor's n values from place `at` on, a multiple of 256 (what
+ * fills the last block of 256 is left alone).  state_bits 32: fp32.  state_bits 8: m in e4m3, v in e5m2, and per block of 256 a scale each (powers of
+ * two, [places / 256]); rounded up or down at random, with bits that are a function of seed, step, `index` and the value's place in its tensor.  steps:
+ * device array, steps[index] counts the tensor's steps.  lr_dev: device scalar to read the rate from, or NULL: lr.  clip_value < 0: no clipping.  copy:
+ * receives p in copy_type (SPION_BF16 or SPION_F16), or NULL.  m and v on 32 bytes.  The table is read before the call returns. */
+typedef struct spion_adamw_tensor {
+  void* p;
+  const void* g;
+  void* copy;
+  long long n, at;
+  int index;
+} spion_adamw_tensor;
+int spion_adamw_step(const spion_adamw_tensor* host_tensors, int count, int type, int state_bits, void* m, void* v, float* m_scale,
+                     float* v_scale, float* steps, const float* lr_dev, double lr, double beta1, double beta2, double eps,
+                     double weight_decay, double clip_value, unsigned seed, int copy_type, void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif

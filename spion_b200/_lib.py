@@ -28,6 +28,11 @@ class Tokens(ctypes.Structure):
                 ("heads", c_int), ("head_dim", c_int), ("seq_len", c_int)]
 
 
+class AdamwTensor(ctypes.Structure):
+    """spion_adamw_tensor: a tensor of an optimizer step (see include/spion_b200.h)."""
+    _fields_ = [("p", c_void_p), ("g", c_void_p), ("copy", c_void_p), ("n", c_longlong), ("at", c_longlong), ("index", c_int)]
+
+
 # name -> (restype, argtypes); every symbol include/spion_b200.h declares
 SIGNATURES = {
     "spion_status_string": (ctypes.c_char_p, [c_int]),
@@ -113,6 +118,7 @@ SIGNATURES = {
     "spion_rmsnorm_workspace_floats": (c_longlong, [c_longlong, c_int]),
     "spion_rmsnorm_backward": (c_int, [c_void_p, c_longlong, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                        c_void_p, c_longlong, c_int, c_void_p]),
+    "spion_adamw_step": (c_int, [ctypes.POINTER(AdamwTensor), c_int, c_int, c_int] + [c_void_p] * 6 + [c_double] * 6 + [ctypes.c_uint, c_int, c_void_p]),
     "spion_static_scratch_capacity": (ctypes.c_size_t, []),
     "spion_attn_forward_static": (c_int, [c_void_p] * 9 + [c_int] * 6 + [c_void_p]),
 }

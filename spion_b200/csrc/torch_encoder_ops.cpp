@@ -1,6 +1,7 @@
-// Host path of the encoder's operators around the attention call: root-mean-square norm, rows in e4m3.  Each call checks what it is given, allocates
+// Host path of the encoder's operators around the attention call: root-mean-square norm, rows in e4m3,
+// the optimizer.  Each call checks what it is given, allocates
 // its results and calls the C ABI; the norm is an autograd node of its own.
-#include <cmath>
+#include <algorithm>
 #include <mutex>
 
 #include "torch_common.h"
@@ -245,6 +246,121 @@ Rows8 quantize_rows(const Tensor& x) {
   return q;
 }
 
+// ------------------------------------------------------------------------------------------------ AdamW
+struct Hyper { double lr, b1, b2, eps, wd, clip; unsigned seed; };
+
+// What one step changes is known to autograd's checks of saved tensors
+void changed(const Tensor& t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void check_flat(const char* op, const Tensor& t, const char* name, at::ScalarType type, int64_t least, const Tensor& like) {
+  check_plain(op, t, name);
+  same_device(op, t, like, name);
+  if (t.scalar_type() != type || !t.is_contiguous() || t.numel() < least)
+    refuse(op, std::string(name) + " has shape " + shape_of(t) + " and type " + c10::toString(t.scalar_type()) + ": " + std::to_string(least) +
+           " contiguous values of type " + c10::toString(type) + " are needed");
+}
+bool overlap(std::vector<std::pair<const char*, const char*>>& spans) {      // [begin, end)
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    if (spans[i].first < spans[i - 1].second) return true;
+  return false;
+}
+
+// grads: undefined where a tensor has none (it is left alone); copies: empty, or undefined where a tensor has none
+void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const Tensor& m, const Tensor& v, const Tensor& steps, const Tensor& m_scale,
+                const Tensor& v_scale, const Tensor& lr_dev, const std::vector<Tensor>& copies, const Hyper& h) {
+  const char* op = "adamw_step";
+  if (grads.size() != params.size()) refuse(op, std::to_string(params.size()) + " parameters and " + std::to_string(grads.size()) + " gradients");
+  if (!copies.empty() && copies.size() != params.size()) refuse(op, std::to_string(params.size()) + " parameters and " + std::to_string(copies.size()) + " copies");
+  if (params.empty()) return;
+  if (!(h.lr >= 0) && !lr_dev.defined()) refuse(op, "lr is " + std::to_string(h.lr));
+  if (!(h.b1 >= 0 && h.b1 < 1 && h.b2 >= 0 && h.b2 < 1)) refuse(op, "betas are " + std::to_string(h.b1) + ", " + std::to_string(h.b2));
+  if (!(h.eps >= 0) || !(h.wd >= 0)) refuse(op, "eps is " + std::to_string(h.eps) + ", weight_decay is " + std::to_string(h.wd));
+  const at::ScalarType type = params[0].scalar_type();
+  const Tensor& like = params[0];
+  check_plain(op, like, "a parameter");
+  if (!stream_type(type)) refuse(op, std::string("parameters have type ") + c10::toString(type) + "; fp32, bf16 and fp16 are served");
+  c10::cuda::CUDAGuard guard(like.device());
+  at::NoGradGuard no_grad;
+  std::vector<spion_adamw_tensor> table;
+  std::vector<Tensor> held;                                // gradients that had to be copied
+  std::vector<std::pair<const char*, const char*>> written;
+  table.reserve(params.size());
+  int64_t at = 0;
+  int copy_type = -1;
+  for (size_t i = 0; i < params.size(); ++i) {
+    const Tensor& t = params[i];
+    check_plain(op, t, "a parameter");
+    if (t.scalar_type() != type || t.device() != like.device() || !t.is_contiguous())
+      refuse(op, "parameter " + std::to_string(i) + " has type " + c10::toString(t.scalar_type()) + " on " + t.device().str() + " and strides that are " +
+             (t.is_contiguous() ? "" : "not ") + "contiguous; all are contiguous, of one type and on one device");
+    const int64_t n = t.numel(), begin = at;
+    at += (n + 255) / 256 * 256;
+    if (!grads[i].defined()) continue;
+    Tensor g = grads[i];
+    check_plain(op, g, "a gradient");
+    if (g.scalar_type() != type || g.device() != t.device() || g.sizes() != t.sizes())
+      refuse(op, "gradient " + std::to_string(i) + " has shape " + shape_of(g) + " and type " + c10::toString(g.scalar_type()) + " on " + g.device().str() +
+             ", its parameter " + shape_of(t) + ", " + c10::toString(type) + ", " + t.device().str());
+    if (!g.is_contiguous()) held.push_back(g = g.contiguous());
+    spion_adamw_tensor e = {t.data_ptr(), g.data_ptr(), nullptr, n, begin, (int)i};
+    if (!copies.empty() && copies[i].defined()) {
+      const Tensor& c = copies[i];
+      check_plain(op, c, "a copy");
+      if ((c.scalar_type() != at::kBFloat16 && c.scalar_type() != at::kHalf) || !c.is_contiguous() || c.sizes() != t.sizes() || c.device() != t.device())
+        refuse(op, "copy " + std::to_string(i) + " has shape " + shape_of(c) + " and type " + c10::toString(c.scalar_type()) +
+               ": contiguous, in 16 bits and of its parameter's shape and device is served");
+      const int ct = type_code(c.scalar_type());
+      if (copy_type >= 0 && ct != copy_type) refuse(op, "copies of two types");
+      copy_type = ct;
+      e.copy = c.data_ptr();
+      if (n) written.push_back({(const char*)e.copy, (const char*)e.copy + 2 * n});
+    }
+    if (n) written.push_back({(const char*)e.p, (const char*)e.p + n * t.element_size()});
+    table.push_back(e);
+  }
+  const bool bits8 = m_scale.defined();
+  if (bits8 != v_scale.defined()) refuse(op, "scales of one of the two moments are missing");
+  check_flat(op, m, "exp_avg", bits8 ? at::kFloat8_e4m3fn : at::kFloat, at, like);
+  check_flat(op, v, "exp_avg_sq", bits8 ? at::kFloat8_e5m2 : at::kFloat, at, like);
+  check_flat(op, steps, "steps", at::kFloat, (int64_t)params.size(), like);
+  if (bits8) {
+    check_flat(op, m_scale, "the scales of exp_avg", at::kFloat, at / 256, like);
+    check_flat(op, v_scale, "the scales of exp_avg_sq", at::kFloat, at / 256, like);
+  }
+  if (lr_dev.defined()) check_flat(op, lr_dev, "lr", at::kFloat, 1, like);
+  if (table.empty()) return;
+  for (const Tensor* t : {&m, &v, &steps, &m_scale, &v_scale})
+    if (t->defined() && t->numel()) written.push_back({(const char*)t->data_ptr(), (const char*)t->data_ptr() + t->numel() * t->element_size()});
+  if (overlap(written)) refuse(op, "two of the tensors that the step writes share memory");
+  check(spion_adamw_step(table.data(), (int)table.size(), type_code(type), bits8 ? 8 : 32, p(m), p(v), (float*)p(m_scale), (float*)p(v_scale), (float*)p(steps),
+                         pf(lr_dev), h.lr, h.b1, h.b2, h.eps, h.wd, h.clip, h.seed, copy_type, stream_of(like)), "spion_adamw_step");
+  for (const Tensor* t : {&m, &v, &steps, &m_scale, &v_scale}) changed(*t);
+  for (size_t i = 0; i < params.size(); ++i)
+    if (grads[i].defined()) {
+      changed(params[i]);
+      if (!copies.empty()) changed(copies[i]);
+    }
+}
+
+// A sequence of tensors and None, without the cost of a general conversion
+std::vector<Tensor> tensors(const py::object& list, const char* name) {
+  std::vector<Tensor> out;
+  if (list.is_none()) return out;
+  py::object fast = py::reinterpret_steal<py::object>(PySequence_Fast(list.ptr(), "a sequence of tensors is needed"));
+  if (!fast) throw py::error_already_set();
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(fast.ptr());
+  out.reserve(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* o = PySequence_Fast_GET_ITEM(fast.ptr(), i);
+    if (o == Py_None) out.emplace_back();
+    else if (THPVariable_Check(o)) out.push_back(THPVariable_Unpack(o));
+    else throw Failure(std::string("adamw_step: ") + name + " " + std::to_string(i) + " is not a tensor");
+  }
+  return out;
+}
+
 py::object or_none(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
 
 }  // namespace
@@ -275,6 +391,15 @@ void add_encoder_ops(py::module_& m) {
       r = quantize_rows(x);
     }
     return py::make_tuple(r.values, r.scales);
+  });
+  m.def("adamw_step", [](const py::object& params, const py::object& grads, const Tensor& exp_avg, const Tensor& exp_avg_sq, const Tensor& steps,
+                         const optional<Tensor>& m_scale, const optional<Tensor>& v_scale, const optional<Tensor>& lr_dev, const py::object& copies, double lr,
+                         double b1, double b2, double eps, double wd, double clip, uint64_t seed) {
+    const auto ps = tensors(params, "parameter"), gs = tensors(grads, "gradient"), cs = tensors(copies, "copy");
+    for (const Tensor& t : ps)
+      if (!t.defined()) throw Failure("adamw_step: a parameter is None");
+    adamw_step(ps, gs, exp_avg, exp_avg_sq, steps, m_scale.value_or(Tensor()), v_scale.value_or(Tensor()), lr_dev.value_or(Tensor()), cs,
+               Hyper{lr, b1, b2, eps, wd, clip, (unsigned)seed});
   });
 }
 

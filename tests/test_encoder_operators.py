@@ -41,3 +41,31 @@ def test_norm_arguments_at_the_c_boundary():
     assert backward(st=BF16, dt=F32) == -5
     assert L.spion_rmsnorm_workspace_floats(0, 8) == 0 and L.spion_rmsnorm_workspace_floats(3, 8) == 24
     assert L.spion_rmsnorm_workspace_floats(10 ** 9, 8) <= 8 * 2048
+
+
+def test_optimizer_arguments_at_the_c_boundary_and_in_the_module():
+    from spion_b200.optim import AdamW, adamw_step, places
+    L, d = _lib.lib, ctypes.c_void_p(4096)
+
+    def step(tensors=((4096, 4096, None, 10, 0, 0),), type=_lib.F32, bits=32, m=d, v=d, sm=None, sv=None, steps=d, lr=1e-3, b1=0.9, b2=0.99, eps=1e-8, wd=0.0,
+             copy_type=_lib.BF16):
+        table = (_lib.AdamwTensor * len(tensors))(*tensors)
+        return L.spion_adamw_step(table, len(tensors), type, bits, m, v, sm, sv, steps, None, lr, b1, b2, eps, wd, -1.0, 0, copy_type, None)
+
+    assert step(tensors=()) == 0
+    assert step(bits=16) == -1 and step(m=None) == -1 and step(v=None) == -1 and step(steps=None) == -1 and step(bits=8) == -1 and step(sm=d, sv=d) == -1
+    assert step(lr=-1.0) == -1 and step(b1=1.0) == -1 and step(b2=-0.1) == -1 and step(eps=float("nan")) == -1 and step(wd=-1.0) == -1
+    assert step(m=ctypes.c_void_p(4100)) == -1
+    assert step(tensors=((None, 4096, None, 10, 0, 0),)) == -1 and step(tensors=((4096, None, None, 10, 0, 0),)) == -1
+    assert step(tensors=((4096, 4096, None, -1, 0, 0),)) == -1 and step(tensors=((4096, 4096, None, 10, 100, 0),)) == -1
+    assert step(tensors=((4096, 4096, 4096, 10, 0, 0),), copy_type=_lib.F32) == -1
+    assert step(type=_lib.E4M3) == -5
+    w = torch.zeros(3)
+    with pytest.raises(SpionError, match="CUDA"):
+        adamw_step([w], [w], w, w, w)
+    with pytest.raises(SpionError, match="GPU"):
+        AdamW([torch.nn.Parameter(w)]).step()
+    for bad in (dict(state_bits=16), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1.0), dict(weight_decay=-0.1), dict(clip_value=-1.0)):
+        with pytest.raises(ValueError):
+            AdamW([torch.nn.Parameter(w)], **bad)
+    assert places([torch.zeros(1), torch.zeros(0), torch.zeros(257)]) == ([0, 256, 256], 768)
