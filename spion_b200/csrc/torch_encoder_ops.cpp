@@ -1,5 +1,5 @@
 // Host path of the encoder's operators around the attention call: root-mean-square norm, rows in e4m3,
-// the optimizer.  Each call checks what it is given, allocates
+// linear layer on them, optimizer.  Each call checks what it is given, allocates
 // its results and calls the C ABI; the norm is an autograd node of its own.
 #include <algorithm>
 #include <mutex>
@@ -246,6 +246,76 @@ Rows8 quantize_rows(const Tensor& x) {
   return q;
 }
 
+// ------------------------------------------------------------------------------------------------ linear layer on 8-bit rows
+// Rows of bytes as the products read them: on 16-byte boundaries (a copy where they lie otherwise), scales one after another.
+struct Operand8 {
+  Tensor values, scales;
+  int64_t M = 0, N = 0, ld = 0;
+  Operand8(const char* op, const Tensor& v, const Tensor& s, const char* name) {
+    check_plain(op, v, name);
+    check_plain(op, s, "a tensor of scales");
+    if (v.scalar_type() != at::kFloat8_e4m3fn || v.dim() < 1 || v.size(-1) < 1 || v.size(-1) > 0x7fffffff / 2)
+      refuse(op, std::string(name) + " has shape " + shape_of(v) + " and type " + c10::toString(v.scalar_type()) + ": rows of e4m3 are needed");
+    if (s.scalar_type() != at::kFloat || s.sizes() != v.sizes().slice(0, v.dim() - 1))
+      refuse(op, std::string(name) + " has shape " + shape_of(v) + ", its scales have " + shape_of(s) + " and type " + c10::toString(s.scalar_type()) +
+             ": an fp32 scale per row is needed");
+    same_device(op, s, v, "a tensor of scales");
+    const Rows r(v);
+    M = r.M; N = r.N;
+    values = r.t;
+    ld = M > 1 ? r.ld : (N + 15) / 16 * 16;
+    if (M > 0 && (((uintptr_t)values.data_ptr() | (uintptr_t)ld) % 16 != 0 || ld < N)) {
+      ld = (N + 15) / 16 * 16;
+      Tensor copy = empty_rows8(v, M, N);
+      copy.copy_(values);
+      values = copy;
+    }
+    scales = s.contiguous();
+  }
+};
+
+// x_scales undefined: x in floating point, its rows are quantised first
+Tensor linear_e4m3(const Tensor& x, const Tensor& x_scales, const Tensor& w, const Tensor& w_scales, const optional<Tensor>& bias,
+                   const optional<at::ScalarType>& out_type) {
+  const char* op = "linear_e4m3";
+  if (x.dim() < 1) refuse(op, "x has no dimension");
+  no_gradient(op, x);
+  if (x_scales.defined()) no_gradient(op, x_scales);
+  no_gradient(op, w); no_gradient(op, w_scales);
+  check_plain(op, x, "x");
+  c10::cuda::CUDAGuard guard(x.device());
+  Below below;
+  Tensor xv = x.detach(), xs = x_scales;
+  if (!xs.defined()) {
+    check_rows(op, x, "x");
+    const Rows8 q = quantize_rows(xv);
+    xv = q.values; xs = q.scales;
+  }
+  const at::ScalarType type = out_type.value_or(x_scales.defined() ? at::kBFloat16 : x.scalar_type());
+  if (!stream_type(type)) refuse(op, std::string("an output of type ") + c10::toString(type) + "; fp32, bf16 and fp16 are served");
+  if (w.dim() != 2) refuse(op, "the weights have shape " + shape_of(w) + ": [features out, features in] is needed");
+  const Operand8 a(op, xv, xs.detach(), "x"), b(op, w.detach(), w_scales.detach(), "w");
+  same_device(op, w, x, "w");
+  if (a.N != b.N) refuse(op, "x has rows of " + std::to_string(a.N) + " features, w of " + std::to_string(b.N));
+  if (b.M < 1 || b.M > 0x7fffffff / 2) refuse(op, "w has shape " + shape_of(w));
+  if (a.M > 0x7fffffff / 2) refuse(op, "x has shape " + shape_of(x));
+  Tensor bc;
+  if (bias.has_value()) {
+    no_gradient(op, *bias);
+    check_plain(op, *bias, "bias");
+    if (bias->dim() != 1 || bias->size(0) != b.M || !stream_type(bias->scalar_type()))
+      refuse(op, "bias has shape " + shape_of(*bias) + " and type " + c10::toString(bias->scalar_type()) + ", w has " + shape_of(w));
+    same_device(op, *bias, x, "bias");
+    bc = bias->detach().contiguous();
+  }
+  auto sizes = x.sizes().vec();
+  sizes.back() = b.M;
+  Tensor y = made(op, at::empty(sizes, x.options().dtype(type)));
+  check(spion_linear_e4m3(p(a.values), a.ld, pf(a.scales), p(b.values), b.ld, pf(b.scales), p(bc), bc.defined() ? type_code(bc.scalar_type()) : SPION_F32, p(y),
+                          b.M, type_code(type), a.M, (int)a.N, (int)b.M, stream_of(x)), "spion_linear_e4m3");
+  return y;
+}
+
 // ------------------------------------------------------------------------------------------------ AdamW
 struct Hyper { double lr, b1, b2, eps, wd, clip; unsigned seed; };
 
@@ -391,6 +461,11 @@ void add_encoder_ops(py::module_& m) {
       r = quantize_rows(x);
     }
     return py::make_tuple(r.values, r.scales);
+  });
+  m.def("linear_e4m3", [](const Tensor& x, const optional<Tensor>& x_scales, const Tensor& w, const Tensor& w_scales, const optional<Tensor>& bias,
+                          const optional<at::ScalarType>& type) {
+    py::gil_scoped_release nogil;
+    return linear_e4m3(x, x_scales.value_or(Tensor()), w, w_scales, bias, type);
   });
   m.def("adamw_step", [](const py::object& params, const py::object& grads, const Tensor& exp_avg, const Tensor& exp_avg_sq, const Tensor& steps,
                          const optional<Tensor>& m_scale, const optional<Tensor>& v_scale, const optional<Tensor>& lr_dev, const py::object& copies, double lr,

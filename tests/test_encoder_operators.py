@@ -69,3 +69,20 @@ def test_optimizer_arguments_at_the_c_boundary_and_in_the_module():
         with pytest.raises(ValueError):
             AdamW([torch.nn.Parameter(w)], **bad)
     assert places([torch.zeros(1), torch.zeros(0), torch.zeros(257)]) == ([0, 256, 256], 768)
+
+
+def test_8_bit_linear_arguments_at_the_c_boundary():
+    from spion_b200.quant import Rows8, linear_e4m3
+    L, d = _lib.lib, ctypes.c_void_p(4096)
+
+    def linear(x=d, ldx=16, sx=d, w=d, ldw=16, sw=d, bias=None, bt=_lib.F32, y=d, ldy=8, yt=_lib.BF16, T=4, K=10, N=8):
+        return L.spion_linear_e4m3(x, ldx, sx, w, ldw, sw, bias, bt, y, ldy, yt, T, K, N, None)
+
+    assert linear(T=0) == 0
+    assert linear(T=-1) == -1 and linear(K=0) == -1 and linear(N=0) == -1 and linear(ldy=7) == -1
+    assert linear(x=None) == -1 and linear(w=None) == -1 and linear(sx=None) == -1 and linear(sw=None) == -1 and linear(y=None) == -1
+    assert linear(ldx=17) == -1 and linear(ldw=24) == -1 and linear(K=17) == -1 and linear(x=ctypes.c_void_p(4097)) == -1
+    assert linear(bias=d, bt=_lib.E4M3) == -1 and linear(yt=_lib.E4M3) == -5 and linear(T=2 ** 31) == -2
+    x = torch.zeros(3, 16)
+    with pytest.raises(SpionError, match="CUDA"):
+        linear_e4m3(x, Rows8(x.to(torch.float8_e4m3fn), torch.ones(3)))
