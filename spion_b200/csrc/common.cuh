@@ -147,8 +147,9 @@ int sm_count();
 
 // linear.cu: status word of the linear layers on the current device, after the work of a stream
 int linear_status(int reset, cudaStream_t st);
-// linear_e4m3.cu: that of the layers on 8-bit operands (part of the former)
+// linear_e4m3.cu, rmsnorm.cu: those of the layers on 8-bit operands and of the norm's backward (reported with the former)
 int linear_e4m3_status(int reset, cudaStream_t st);
+int rmsnorm_status(int reset, cudaStream_t st);
 
 // Device memory of the contexts, from one pool per device that keeps up to 64 MB of what was given back, beside what is in use: mapping
 // and unmapping two or three megabytes took 2 to 4 ms of every context's life.  Freeing waits for the device, as cudaFree does (where it

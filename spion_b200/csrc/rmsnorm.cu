@@ -9,9 +9,14 @@
 // Statistics are fp32 sums.  The norm of a 16-bit stream is that of the rounded sum, which is what the next layer and the backward see.  The largest
 // |y| is the largest |s w| times rho, rounding included, because rounding keeps the order: sum and maximum take one reduction.
 //
-// Work split: rows of up to 256 values take 8 lanes (a warp has four rows), up to 1024 a warp, wider ones a CTA; a row that no register file holds is
-// read twice.  Pieces of eight elements where every row starts on the boundary of such a piece, single elements otherwise (odd widths).
+// Work split: rows of up to 256 values take 8 lanes (a warp has four rows or more), up to 1024 a warp, wider ones a CTA; a row that no register file holds
+// is read twice.  Pieces of eight elements where every row starts on the boundary of such a piece, single elements otherwise (odd widths).  The number of
+// threads of a row is a constant of each kernel, so a piece's place costs no arithmetic.
+#include <algorithm>
+#include <atomic>
+
 #include "rows.cuh"
+#include "tc_ptx.cuh"
 
 using namespace rows;
 
@@ -20,6 +25,9 @@ namespace {
 constexpr float SMALL = 0x1p-100f;        // what the scale of a row of zeros follows
 constexpr int CTA = 256;                  // threads of a CTA whose warps take rows of their own
 constexpr int MAX_PARTS = 1184;           // partial rows of a weight gradient: eight per multiprocessor of 148
+
+// Set by a bounded wait that gave up (the ring of the backward); launches of it after that leave at once until spion_linear_status has reported it.
+__device__ int g_rms_status;
 
 struct FwdArgs {
   const void* x; long long ldx;
@@ -33,12 +41,28 @@ struct FwdArgs {
   int norm;                               // 0: y = x
 };
 
-template <int VEC, int NV> __device__ __forceinline__ void load_weights(const void* p, int type, int N, int t, int tpr, float (&w)[NV * VEC]) {
+// (all loads first: a conversion beside its load would wait for it)
+template <class W, int VEC, int NV, int TPR> __device__ __forceinline__ void load_weights_of(const W* p, int N, int t, float (&w)[NV * VEC]) {
+  Piece<W, VEC> q[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (t + i * tpr) * VEC;
+    const int c = (t + i * TPR) * VEC;
+    if (c < N) q[i].load(p + c);
+    else q[i].zero();
+  }
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) w[i * VEC + e] = p == nullptr ? 1.f : c < N ? load_any(p, type, c + e) : 0.f;
+  for (int i = 0; i < NV * VEC; ++i) w[i] = q[i / VEC].at(i % VEC);
+}
+template <int VEC, int NV, int TPR> __device__ __forceinline__ void load_weights(const void* p, int type, int N, int t, float (&w)[NV * VEC]) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int i = 0; i < NV * VEC; ++i) w[i] = 1.f;
+  } else if (type == SPION_F32) {
+    load_weights_of<float, VEC, NV, TPR>(static_cast<const float*>(p), N, t, w);
+  } else if (type == SPION_BF16) {
+    load_weights_of<__nv_bfloat16, VEC, NV, TPR>(static_cast<const __nv_bfloat16*>(p), N, t, w);
+  } else {
+    load_weights_of<__half, VEC, NV, TPR>(static_cast<const __half*>(p), N, t, w);
   }
 }
 
@@ -51,80 +75,95 @@ __device__ __forceinline__ float row_scale(float top, float sum, float& scale) {
   return 448.f * __frcp_rn(a);
 }
 
-// SUB lanes to a row, 0: the CTA
-template <class S, class R, class Y, int VEC, int NV, int SUB, int THREADS>
-__global__ void __launch_bounds__(THREADS) k_rms_forward(const FwdArgs a) {
+// TPR threads to a row: 8 or 32 lanes of a warp, more: a CTA of that many.  Lanes take UR rows at a time, so that enough bytes are in flight.
+template <class S, class R, class Y, int VEC, int NV, int TPR, int UR>
+__global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR) k_rms_forward(const FwdArgs a) {
   constexpr bool Q = type_code<Y>() == SPION_E4M3;
+  constexpr int THREADS = TPR <= 32 ? CTA : TPR, RPC = THREADS / TPR, RPW = TPR <= 32 ? 32 / TPR : 1;      // rows of a CTA and of a warp
   __shared__ float2 part[2][32];
-  const int tpr = SUB ? SUB : (int)blockDim.x, t = SUB ? (int)threadIdx.x & (SUB - 1) : (int)threadIdx.x;
-  const int rpc = SUB ? (int)blockDim.x / SUB : 1, sub = SUB ? (int)(threadIdx.x & 31) / SUB : 0;
-  const S* const x = static_cast<const S*>(a.x);
-  const R* const r = static_cast<const R*>(a.r);
-  S* const s = static_cast<S*>(a.s);
-  Y* const y = static_cast<Y*>(a.y);
+  const int t = TPR <= 32 ? (int)threadIdx.x & (TPR - 1) : (int)threadIdx.x;
+  const S* const x = static_cast<const S*>(a.x) + t * VEC;
+  const R* const r = static_cast<const R*>(a.r) + t * VEC;
+  S* const s = static_cast<S*>(a.s) + t * VEC;
+  Y* const y = static_cast<Y*>(a.y) + t * VEC;
+  const int left = a.N - t * VEC;                        // piece i of the thread is in the row if i * TPR * VEC < left
   float w[NV * VEC];
-  load_weights<VEC, NV>(a.w, a.w_type, a.N, t, tpr, w);
+  load_weights<VEC, NV, TPR>(a.w, a.w_type, a.N, t, w);
   int buf = 0;
   const float over_n = 1.0f / a.N;
   // `first` is the same for all lanes of a warp: they leave the loop together
-  for (long long first = (long long)blockIdx.x * rpc + (SUB ? (threadIdx.x >> 5) * (32 / (SUB ? SUB : 32)) : 0); first < a.M;
-       first += (long long)gridDim.x * rpc) {
-    const long long row = first + sub;
-    const bool live = row < a.M;
-    Piece<S, VEC> px[NV];
-    Piece<R, VEC> pr[NV];
+  const int sub = TPR <= 32 ? (int)(threadIdx.x & 31) / TPR : 0;
+  for (long long first = (long long)blockIdx.x * RPC * UR + (TPR <= 32 ? (threadIdx.x >> 5) * RPW * UR : 0); first < a.M; first += (long long)gridDim.x * RPC * UR) {
+    Piece<S, VEC> px[UR][NV];
+    float v[UR][NV * VEC];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * tpr) * VEC;
-      if (live && c < a.N) px[i].load(x + row * a.ldx + c);
-      else px[i].zero();
+    for (int u = 0; u < UR; ++u) {
+      const long long row = first + u * RPW + sub;
+      const int here = row < a.M ? left : 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (i * TPR * VEC < here) px[u][i].load(x + row * a.ldx + i * TPR * VEC);
+        else px[u][i].zero();
     }
-    float v[NV * VEC];
-    if (r != nullptr) {
+    if (a.r != nullptr) {
+      Piece<R, VEC> pr[UR][NV];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = (t + i * tpr) * VEC;
-        if (live && c < a.N) pr[i].load(r + row * a.ldr + c);
-        else pr[i].zero();
+      for (int u = 0; u < UR; ++u) {
+        const long long row = first + u * RPW + sub;
+        const int here = row < a.M ? left : 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (i * TPR * VEC < here) pr[u][i].load(r + row * a.ldr + i * TPR * VEC);
+          else pr[u][i].zero();
       }
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = (t + i * tpr) * VEC;
-        float sum[VEC];
+      for (int u = 0; u < UR; ++u) {
+        const long long row = first + u * RPW + sub;
+        const int here = row < a.M ? left : 0;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          sum[e] = px[i].at(e) + pr[i].at(e);
-          v[i * VEC + e] = as_float(rounded<S>(sum[e]));
+        for (int i = 0; i < NV; ++i) {
+          float sum[VEC];
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            sum[e] = px[u][i].at(e) + pr[u][i].at(e);
+            v[u][i * VEC + e] = as_float(rounded<S>(sum[e]));
+          }
+          if (i * TPR * VEC < here) Out<S, VEC>::store(s + row * a.N + i * TPR * VEC, sum);
         }
-        if (live && c < a.N) Out<S, VEC>::store(s + row * a.N + c, sum);
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < NV * VEC; ++i) v[i] = px[i / VEC].at(i % VEC);
-    }
-    float sum = 0.f, top = 0.f;
+      for (int u = 0; u < UR; ++u)
 #pragma unroll
-    for (int i = 0; i < NV * VEC; ++i) {
-      sum = fmaf(v[i], v[i], sum);
-      v[i] *= w[i];
-      if (Q) top = fmaxf(top, fabsf(v[i]));
+        for (int i = 0; i < NV * VEC; ++i) v[u][i] = px[u][i / VEC].at(i % VEC);
     }
-    row_reduce<SUB, Q>(sum, top, part, buf);
-    const float rho = a.norm ? rsqrtf(fmaf(sum, over_n, a.eps)) : 1.f;
-    float f = rho;
-    if (Q) {
-      float scale;
-      f = row_scale(top * rho, a.norm ? top * rho : sum, scale);
-      if (t == 0 && live) a.scale[row] = scale;
-    }
-    if (t == 0 && live && a.rho != nullptr) a.rho[row] = rho;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * tpr) * VEC;
-      float o[VEC];
+    for (int u = 0; u < UR; ++u) {
+      const long long row = first + u * RPW + sub;
+      const int here = row < a.M ? left : 0;
+      float sum = 0.f, top = 0.f;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o[e] = Q ? v[i * VEC + e] * rho * f : v[i * VEC + e] * rho;
-      if (live && c < a.N) Out<Y, VEC>::store(y + row * a.ldy + c, o);
+      for (int i = 0; i < NV * VEC; ++i) {
+        sum = fmaf(v[u][i], v[u][i], sum);
+        v[u][i] *= w[i];
+        if (Q) top = fmaxf(top, fabsf(v[u][i]));
+      }
+      row_reduce<TPR, Q>(sum, top, part, buf);
+      const float rho = a.norm ? rsqrtf(fmaf(sum, over_n, a.eps)) : 1.f;
+      float f = 1.f;
+      if (Q) {
+        float scale;
+        f = row_scale(top * rho, a.norm ? top * rho : sum, scale);
+        if (t == 0 && row < a.M) a.scale[row] = scale;
+      }
+      if (t == 0 && row < a.M && a.rho != nullptr) a.rho[row] = rho;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        float o[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o[e] = Q ? v[u][i * VEC + e] * rho * f : v[u][i * VEC + e] * rho;
+        if (i * TPR * VEC < here) Out<Y, VEC>::store(y + row * a.ldy + i * TPR * VEC, o);
+      }
     }
   }
 }
@@ -141,6 +180,7 @@ __global__ void __launch_bounds__(512) k_rms_forward_wide(const FwdArgs a) {
     const S* const x = static_cast<const S*>(a.x) + row * a.ldx;
     Y* const y = static_cast<Y*>(a.y) + row * a.ldy;
     float sum = 0.f, top = 0.f;
+#pragma unroll 2
     for (int c = threadIdx.x * VEC; c < a.N; c += blockDim.x * VEC) {
       Piece<S, VEC> px;
       Piece<R, VEC> pr;
@@ -163,7 +203,7 @@ __global__ void __launch_bounds__(512) k_rms_forward_wide(const FwdArgs a) {
         if (Q) top = fmaxf(top, fabsf(v[e] * (a.w == nullptr ? 1.f : load_any(a.w, a.w_type, c + e))));
       }
     }
-    row_reduce<0, Q>(sum, top, part, buf);
+    row_reduce<512, Q>(sum, top, part, buf);
     const float rho = a.norm ? rsqrtf(fmaf(sum, 1.0f / a.N, a.eps)) : 1.f;
     float f = 1.f;
     if (Q) {
@@ -173,6 +213,7 @@ __global__ void __launch_bounds__(512) k_rms_forward_wide(const FwdArgs a) {
     }
     if (threadIdx.x == 0 && a.rho != nullptr) a.rho[row] = rho;
     const S* const from = r != nullptr ? s + row * a.N : x;                // this thread's own stores
+#pragma unroll 2
     for (int c = threadIdx.x * VEC; c < a.N; c += blockDim.x * VEC) {
       Piece<S, VEC> px;
       px.load(from + c);
@@ -199,104 +240,104 @@ struct BwdArgs {
   long long M; int N;
 };
 
-// Warps of a CTA leave their sums of a column side by side in shared memory and add them in order.
-template <class S, class D, int VEC, int NV, int SUB, int THREADS>
-__global__ void __launch_bounds__(THREADS) k_rms_backward(const BwdArgs a) {
-  next_may_start();                                                        // k_rms_dw
-  __shared__ float2 part[2][32];
-  constexpr int WIDTH = SUB ? SUB * NV * VEC : 1, GROUPS = SUB ? THREADS / SUB : 1;
-  constexpr int AT_ONCE = GROUPS < 8 ? GROUPS : 8;                         // groups of lanes whose sums are in shared memory together
-  __shared__ float sums[SUB ? AT_ONCE * WIDTH : 1];
-  const int tpr = SUB ? SUB : (int)blockDim.x, t = SUB ? (int)threadIdx.x & (SUB - 1) : (int)threadIdx.x;
-  const int rpc = SUB ? GROUPS : 1, sub = SUB ? (int)(threadIdx.x & 31) / SUB : 0;
-  const S* const s = static_cast<const S*>(a.s);
-  const D* const dy = static_cast<const D*>(a.dy);
-  const S* const ds = static_cast<const S*>(a.ds);
+// Both gradients of a row from registers.  `carry`: the sums of dy n, column by column.
+template <class S, class D, int VEC, int NV, int TPR>
+__device__ __forceinline__ void row_backward(const BwdArgs& a, long long row, int here, const Piece<S, VEC> (&ps)[NV], const Piece<D, VEC> (&pd)[NV],
+                                             const Piece<S, VEC> (&pk)[NV], float rho, float mean, const float (&w)[NV * VEC], int t) {
   S* const dx = static_cast<S*>(a.dx);
+  const float m = mean * rho;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float o[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) o[e] = fmaf(fmaf(-ps[i].at(e), m, pd[i].at(e) * w[i * VEC + e]), rho, pk[i].at(e));
+    if (i * TPR * VEC < here) {
+      const long long at = row * a.N + (t + i * TPR) * VEC;
+      if (dx != nullptr) Out<S, VEC>::store(dx + at, o);
+      if (a.dr != nullptr) {
+        if (a.dr_type == SPION_BF16) Out<__nv_bfloat16, VEC>::store(static_cast<__nv_bfloat16*>(a.dr) + at, o);
+        else Out<__half, VEC>::store(static_cast<__half*>(a.dr) + at, o);
+      }
+    }
+  }
+}
+
+// Rows through registers.  The groups of lanes of a CTA leave their sums of a column side by side in shared memory, where they are added in order.
+template <class S, class D, int VEC, int NV, int TPR, int UR>
+__global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR) k_rms_backward(const BwdArgs a) {
+  next_may_start();                                                        // k_rms_dw
+  constexpr int THREADS = TPR <= 32 ? CTA : TPR, RPC = THREADS / TPR, RPW = TPR <= 32 ? 32 / TPR : 1;
+  constexpr int WIDTH = TPR * NV * VEC, AT_ONCE = RPC < 8 ? RPC : 8;       // groups of lanes whose sums are in shared memory together
+  __shared__ float2 part[2][32];
+  __shared__ float sums[RPC > 1 ? AT_ONCE * WIDTH : 1];
+  const int t = TPR <= 32 ? (int)threadIdx.x & (TPR - 1) : (int)threadIdx.x, sub = TPR <= 32 ? (int)(threadIdx.x & 31) / TPR : 0;
+  const S* const s = static_cast<const S*>(a.s) + t * VEC;
+  const D* const dy = static_cast<const D*>(a.dy) + t * VEC;
+  const S* const ds = static_cast<const S*>(a.ds) + t * VEC;
+  const int left = a.N - t * VEC;
   float w[NV * VEC], acc[NV * VEC];
-  load_weights<VEC, NV>(a.w, a.w_type, a.N, t, tpr, w);
+  load_weights<VEC, NV, TPR>(a.w, a.w_type, a.N, t, w);
 #pragma unroll
   for (int i = 0; i < NV * VEC; ++i) acc[i] = 0.f;
   int buf = 0;
   const float over_n = 1.0f / a.N;
-  for (long long first = (long long)blockIdx.x * rpc + (SUB ? (threadIdx.x >> 5) * (32 / (SUB ? SUB : 32)) : 0); first < a.M;
-       first += (long long)gridDim.x * rpc) {
-    const long long row = first + sub;
-    const bool live = row < a.M;
-    Piece<S, VEC> ps[NV], pk[NV];
-    Piece<D, VEC> pd[NV];
-    const float rho = live ? a.rho[row] : 0.f;
+  for (long long first = (long long)blockIdx.x * RPC * UR + (TPR <= 32 ? (threadIdx.x >> 5) * RPW * UR : 0); first < a.M; first += (long long)gridDim.x * RPC * UR) {
+    Piece<S, VEC> ps[UR][NV], pk[UR][NV];
+    Piece<D, VEC> pd[UR][NV];
+    float rho[UR];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * tpr) * VEC;
-      if (live && c < a.N) ps[i].load(s + row * a.lds + c), pd[i].load(dy + row * a.N + c);
-      else ps[i].zero(), pd[i].zero();
-    }
-    if (ds != nullptr) {
+    for (int u = 0; u < UR; ++u) {
+      const long long row = first + u * RPW + sub;
+      const int here = row < a.M ? left : 0;
+      rho[u] = row < a.M ? a.rho[row] : 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = (t + i * tpr) * VEC;
-        if (live && c < a.N) pk[i].load(ds + row * a.N + c);
-        else pk[i].zero();
+        if (i * TPR * VEC < here) ps[u][i].load(s + row * a.lds + i * TPR * VEC), pd[u][i].load(dy + row * a.N + i * TPR * VEC);
+        else ps[u][i].zero(), pd[u][i].zero();
+        if (a.ds != nullptr && i * TPR * VEC < here) pk[u][i].load(ds + row * a.N + i * TPR * VEC);
+        else pk[u][i].zero();
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) pk[i].zero();
     }
-    float sum = 0.f, none = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV * VEC; ++i) {
-      const float n = ps[i / VEC].at(i % VEC) * rho, d = pd[i / VEC].at(i % VEC);
-      acc[i] = fmaf(d, n, acc[i]);
-      sum = fmaf(d * w[i], n, sum);
-    }
-    row_reduce<SUB, false>(sum, none, part, buf);
-    const float m = sum * over_n;
+    for (int u = 0; u < UR; ++u) {
+      const long long row = first + u * RPW + sub;
+      float sum = 0.f, none = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * tpr) * VEC;
-      float o[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float n = ps[i].at(e) * rho, g = pd[i].at(e) * w[i * VEC + e];
-        o[e] = fmaf(g - n * m, rho, pk[i].at(e));
+      for (int i = 0; i < NV * VEC; ++i) {
+        const float d = pd[u][i / VEC].at(i % VEC) * (ps[u][i / VEC].at(i % VEC) * rho[u]);
+        acc[i] += d;
+        sum = fmaf(d, w[i], sum);
       }
-      if (live && c < a.N) {
-        if (dx != nullptr) Out<S, VEC>::store(dx + row * a.N + c, o);
-        if (a.dr != nullptr) {
-          if (a.dr_type == SPION_BF16) Out<__nv_bfloat16, VEC>::store(static_cast<__nv_bfloat16*>(a.dr) + row * a.N + c, o);
-          else Out<__half, VEC>::store(static_cast<__half*>(a.dr) + row * a.N + c, o);
-        }
-      }
+      row_reduce<TPR, false>(sum, none, part, buf);
+      row_backward<S, D, VEC, NV, TPR>(a, row, row < a.M ? left : 0, ps[u], pd[u], pk[u], rho[u], sum * over_n, w, t);
     }
   }
   if (a.part == nullptr) return;
   float* const out = a.part + (long long)blockIdx.x * a.N;
-  if (SUB == 0) {
+  if (RPC == 1) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * tpr) * VEC;
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
-        if (c < a.N) out[c + e] = acc[i * VEC + e];
-    }
+        if (i * TPR * VEC < left) out[(t + i * TPR) * VEC + e] = acc[i * VEC + e];
     return;
   }
-  const int group = threadIdx.x / (SUB ? SUB : 1);
-  float total[(WIDTH + THREADS - 1) / THREADS];
+  constexpr int COLS = (WIDTH + THREADS - 1) / THREADS;
+  const int group = threadIdx.x / TPR;
+  float total[COLS];
 #pragma unroll
-  for (int k = 0; k < (WIDTH + THREADS - 1) / THREADS; ++k) total[k] = 0.f;
-  for (int g0 = 0; g0 < GROUPS; g0 += AT_ONCE) {
+  for (int k = 0; k < COLS; ++k) total[k] = 0.f;
+  for (int g0 = 0; g0 < RPC; g0 += AT_ONCE) {
     __syncthreads();
     if (group >= g0 && group < g0 + AT_ONCE) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) sums[(group - g0) * WIDTH + (t + i * tpr) * VEC + e] = acc[i * VEC + e];
+        for (int e = 0; e < VEC; ++e) sums[(group - g0) * WIDTH + (t + i * TPR) * VEC + e] = acc[i * VEC + e];
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < (WIDTH + THREADS - 1) / THREADS; ++k) {
+    for (int k = 0; k < COLS; ++k) {
       const int c = threadIdx.x + k * THREADS;
       if (c < WIDTH)
 #pragma unroll
@@ -304,10 +345,100 @@ __global__ void __launch_bounds__(THREADS) k_rms_backward(const BwdArgs a) {
     }
   }
 #pragma unroll
-  for (int k = 0; k < (WIDTH + THREADS - 1) / THREADS; ++k) {
+  for (int k = 0; k < COLS; ++k) {
     const int c = threadIdx.x + k * THREADS;
     if (c < WIDTH && c < a.N) out[c] = total[k];
   }
+}
+
+// Wide rows: a CTA takes its rows one after another out of a ring in shared memory that bulk copies fill several rows ahead, so that the row's sum, which
+// everything waits for, does not stop the loads.  The one barrier a row has for its sum also tells that all threads hold their pieces in registers: the
+// row's place in the ring is filled anew right after it.
+struct Ring { int stages; uint32_t stage, at_dy, at_ds; };                 // bytes
+constexpr uint32_t RING_BARS = 128;
+template <class S, class D, int NV, int TPR>
+__global__ void __launch_bounds__(TPR) k_rms_backward_ring(const BwdArgs a, const Ring ring) {
+  next_may_start();                                                        // k_rms_dw
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float2 part[2][32];
+  __shared__ int s_lost;
+  const int t = threadIdx.x, left = a.N - t * 8;
+  const uint32_t bars = tc::smem_u32(smem), rows0 = bars + RING_BARS;
+  const long long step = gridDim.x;
+  auto fill = [&](int st, long long row) {                                 // one thread
+    const uint32_t bytes = a.N * (uint32_t)sizeof(S), dbytes = a.N * (uint32_t)sizeof(D), at = rows0 + st * ring.stage, bar = bars + 8 * st;
+    tc::mbar_expect_tx(bar, bytes + dbytes + (a.ds != nullptr ? bytes : 0));
+    tc::bulk_load(at, static_cast<const S*>(a.s) + row * a.lds, bar, bytes);
+    tc::bulk_load(at + ring.at_dy, static_cast<const D*>(a.dy) + row * a.N, bar, dbytes);
+    if (a.ds != nullptr) tc::bulk_load(at + ring.at_ds, static_cast<const S*>(a.ds) + row * a.N, bar, bytes);
+  };
+  if (t == 0) {
+    s_lost = *reinterpret_cast<volatile int*>(&g_rms_status) != 0 ? -1 : 0;
+    for (int i = 0; i < ring.stages; ++i) tc::mbar_init(bars + 8 * i, 1);
+    tc::fence_barrier_init();
+    tc::fence_proxy_async();
+    for (int i = 0; i < ring.stages && s_lost == 0; ++i)
+      if (blockIdx.x + i * step < a.M) fill(i, blockIdx.x + i * step);
+  }
+  float w[NV * 8], acc[NV * 8];
+  load_weights<8, NV, TPR>(a.w, a.w_type, a.N, t, w);
+#pragma unroll
+  for (int i = 0; i < NV * 8; ++i) acc[i] = 0.f;
+  int buf = 0, st = 0, ph = 0;
+  const float over_n = 1.0f / a.N;
+  float rho = blockIdx.x < a.M ? a.rho[blockIdx.x] : 0.f;
+  __syncthreads();
+  if (s_lost != 0) return;
+  __syncthreads();
+  for (long long row = blockIdx.x; row < a.M; row += step) {
+    const float next = row + step < a.M ? a.rho[row + step] : 0.f;
+    if (!tc::mbar_wait(bars + 8 * st, ph)) s_lost = 1;                     // (bounded; the copies of this CTA end by themselves)
+    const uint8_t* const at = smem + RING_BARS + st * ring.stage;
+    Piece<S, 8> ps[NV], pk[NV];
+    Piece<D, 8> pd[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (t + i * TPR) * 8;
+      if (i * TPR * 8 < left) {
+        ps[i].load_shared(reinterpret_cast<const S*>(at) + c);
+        pd[i].load_shared(reinterpret_cast<const D*>(at + ring.at_dy) + c);
+      } else {
+        ps[i].zero(), pd[i].zero();
+      }
+      if (a.ds != nullptr && i * TPR * 8 < left) pk[i].load_shared(reinterpret_cast<const S*>(at + ring.at_ds) + c);
+      else pk[i].zero();
+    }
+    float sum = 0.f, none = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV * 8; ++i) {
+      const float d = pd[i / 8].at(i % 8) * (ps[i / 8].at(i % 8) * rho);
+      acc[i] += d;
+      sum = fmaf(d, w[i], sum);
+    }
+    row_reduce<TPR, false>(sum, none, part, buf);
+    if (s_lost) {                                                          // (every thread that set it did so before the barrier)
+      if (t == 0) {
+        atomicOr(&g_rms_status, 1);
+        for (int i = 0; i < ring.stages; ++i)                              // the copies under way end first, or this gives up again
+          if (row + (i - st + (i < st ? ring.stages : 0)) * step < a.M) tc::mbar_wait(bars + 8 * i, i < st ? ph ^ 1 : ph);
+      }
+      return;
+    }
+    if (t == 0 && row + ring.stages * step < a.M) fill(st, row + ring.stages * step);
+    row_backward<S, D, 8, NV, TPR>(a, row, left, ps, pd, pk, rho, sum * over_n, w, t);
+    rho = next;
+    if (++st == ring.stages) st = 0, ph ^= 1;
+  }
+  if (a.part == nullptr) return;
+  float* const out = a.part + (long long)blockIdx.x * a.N;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i * TPR * 8 < left) {
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = acc[i * 8 + e];
+      Out<float, 8>::store(out + (t + i * TPR) * 8, o);
+    }
 }
 
 // Rows that the registers do not hold: dx here, the weight gradient by columns (k_rms_columns).
@@ -321,6 +452,7 @@ __global__ void __launch_bounds__(512) k_rms_backward_wide(const BwdArgs a) {
     const S* const ds = a.ds == nullptr ? nullptr : static_cast<const S*>(a.ds) + row * a.N;
     const float rho = a.rho[row];
     float sum = 0.f, none = 0.f;
+#pragma unroll 2
     for (int c = threadIdx.x * VEC; c < a.N; c += blockDim.x * VEC) {
       Piece<S, VEC> ps;
       Piece<D, VEC> pd;
@@ -328,8 +460,9 @@ __global__ void __launch_bounds__(512) k_rms_backward_wide(const BwdArgs a) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) sum = fmaf(pd.at(e) * (a.w == nullptr ? 1.f : load_any(a.w, a.w_type, c + e)), ps.at(e) * rho, sum);
     }
-    row_reduce<0, false>(sum, none, part, buf);
+    row_reduce<512, false>(sum, none, part, buf);
     const float m = sum / a.N;
+#pragma unroll 2
     for (int c = threadIdx.x * VEC; c < a.N; c += blockDim.x * VEC) {
       Piece<S, VEC> ps, pk;
       Piece<D, VEC> pd;
@@ -368,8 +501,17 @@ __global__ void __launch_bounds__(1024) k_rms_dw(const float* part, int count, i
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float s = 0.f;
   wait_for_kernel_before();
-  if (c < N)
-    for (int r = warp; r < count; r += 32) s += part[(long long)r * N + c];
+  if (c < N) {
+    int r = warp;
+    for (; r + 7 * 32 < count; r += 8 * 32) {                              // eight loads at a time, added one after another
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = part[(long long)(r + 32 * k) * N + c];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += v[k];
+    }
+    for (; r < count; r += 32) s += part[(long long)r * N + c];
+  }
   sums[warp][lane] = s;
   __syncthreads();
   if (warp == 0 && c < N) {
@@ -389,31 +531,40 @@ int grid_of(long long M, int rows_per_cta, int threads) {
   const long long most = (long long)sm_count() * (2048 / threads), need = (M + rows_per_cta - 1) / rows_per_cta;
   return (int)(need < most ? need : most);
 }
-int threads_for(int pieces, int per_thread) { return ((pieces + per_thread - 1) / per_thread + 31) / 32 * 32; }
 
+template <class S, class R, class Y, int VEC, int NV, int TPR, int UR = 1> void launch_forward(const FwdArgs& a, cudaStream_t st) {
+  constexpr int THREADS = TPR <= 32 ? CTA : TPR;
+  k_rms_forward<S, R, Y, VEC, NV, TPR, UR><<<grid_of(a.M, THREADS / TPR * UR, THREADS), THREADS, 0, st>>>(a);
+}
 template <class S, class R, class Y>
 int forward(const FwdArgs& a, cudaStream_t st) {
   const bool vec = a.N % 8 == 0 && on_boundary(a.x, a.ldx, type_code<S>()) && on_boundary(a.r, a.ldr, type_code<R>()) &&
-                   on_boundary(a.s, a.N, type_code<S>()) && on_boundary(a.y, a.ldy, type_code<Y>());
-#define SPION_ROWS(VEC, NV, SUB, THREADS, threads) \
-  k_rms_forward<S, R, Y, VEC, NV, SUB, THREADS><<<grid_of(a.M, SUB ? (threads) / (SUB ? SUB : 1) : 1, threads), threads, 0, st>>>(a)
+                   on_boundary(a.s, a.N, type_code<S>()) && on_boundary(a.y, a.ldy, type_code<Y>()) && on_boundary(a.w, a.N, a.w_type);
+  const bool few = a.M <= sm_count();                    // as many threads as pieces
   if (vec) {
     const int n = a.N / 8;
-    if (n <= 8) SPION_ROWS(8, 1, 8, CTA, CTA);
-    else if (n <= 16) SPION_ROWS(8, 2, 8, CTA, CTA);
-    else if (n <= 32) SPION_ROWS(8, 4, 8, CTA, CTA);
-    else if (n <= 64) SPION_ROWS(8, 2, 32, CTA, CTA);
-    else if (n <= 128) SPION_ROWS(8, 4, 32, CTA, CTA);
-    else if (a.M <= sm_count() && n <= 1024) SPION_ROWS(8, 1, 0, 1024, threads_for(n, 1));       // few rows: as many threads as pieces
-    else if (n <= 2048) SPION_ROWS(8, 4, 0, 512, threads_for(n, 4));
+    if (n <= 8) launch_forward<S, R, Y, 8, 1, 8, 2>(a, st);
+    else if (n <= 16) launch_forward<S, R, Y, 8, 2, 8>(a, st);
+    else if (n <= 32) launch_forward<S, R, Y, 8, 4, 8>(a, st);
+    else if (n <= 64) launch_forward<S, R, Y, 8, 2, 32>(a, st);
+    else if (n <= 128) launch_forward<S, R, Y, 8, 4, 32>(a, st);
+    else if (few && n <= 256) launch_forward<S, R, Y, 8, 1, 256>(a, st);
+    else if (few && n <= 512) launch_forward<S, R, Y, 8, 1, 512>(a, st);
+    else if (few && n <= 1024) launch_forward<S, R, Y, 8, 1, 1024>(a, st);
+    else if (n <= 256) launch_forward<S, R, Y, 8, 4, 64>(a, st);
+    else if (n <= 512) launch_forward<S, R, Y, 8, 4, 128>(a, st);
+    else if (n <= 1024) launch_forward<S, R, Y, 8, 4, 256>(a, st);
+    else if (n <= 2048) launch_forward<S, R, Y, 8, 4, 512>(a, st);
     else k_rms_forward_wide<S, R, Y, 8><<<grid_of(a.M, 1, 512), 512, 0, st>>>(a);
   } else {
-    if (a.N <= 128) SPION_ROWS(1, 4, 32, CTA, CTA);
-    else if (a.N <= 512) SPION_ROWS(1, 16, 32, CTA, CTA);
-    else if (a.N <= 8192) SPION_ROWS(1, 16, 0, 512, threads_for(a.N, 16));
+    if (a.N <= 128) launch_forward<S, R, Y, 1, 4, 32, 2>(a, st);
+    else if (a.N <= 512) launch_forward<S, R, Y, 1, 16, 32>(a, st);
+    else if (a.N <= 1024) launch_forward<S, R, Y, 1, 16, 64>(a, st);
+    else if (a.N <= 2048) launch_forward<S, R, Y, 1, 16, 128>(a, st);
+    else if (a.N <= 4096) launch_forward<S, R, Y, 1, 16, 256>(a, st);
+    else if (a.N <= 8192) launch_forward<S, R, Y, 1, 16, 512>(a, st);
     else k_rms_forward_wide<S, R, Y, 1><<<grid_of(a.M, 1, 512), 512, 0, st>>>(a);
   }
-#undef SPION_ROWS
   SPION_LAUNCH_CHECK();
   return SPION_OK;
 }
@@ -427,33 +578,63 @@ template <class S, class R> int forward_out(const FwdArgs& a, int y_type, cudaSt
   return SPION_ERR_UNSUPPORTED;
 }
 
+// CTAs of a backward: what is resident at a time and no more, because every one of them leaves a partial row
+int parts_of(long long M, int rows_per_cta, int per_sm) {
+  const long long need = (M + rows_per_cta - 1) / rows_per_cta, most = std::min((long long)sm_count() * per_sm, (long long)MAX_PARTS);
+  return (int)(need < most ? need : most);
+}
+template <class S, class D, int VEC, int NV, int TPR, int UR = 1> int launch_backward(const BwdArgs& a, int per_sm, cudaStream_t st) {
+  constexpr int THREADS = TPR <= 32 ? CTA : TPR;
+  const int parts = parts_of(a.M, THREADS / TPR * UR, per_sm);
+  k_rms_backward<S, D, VEC, NV, TPR, UR><<<parts, THREADS, 0, st>>>(a);
+  return parts;
+}
+// 0: fewer than two rows fit
+template <class S, class D, int NV, int TPR> int launch_ring(const BwdArgs& a, int per_sm, cudaStream_t st) {
+  Ring r;
+  r.at_dy = a.N * (uint32_t)sizeof(S);
+  r.at_ds = r.at_dy + a.N * (uint32_t)sizeof(D);
+  r.stage = r.at_ds + (a.ds != nullptr ? a.N * (uint32_t)sizeof(S) : 0);
+  const uint32_t room = 200u * 1024 / per_sm - RING_BARS;
+  r.stages = (int)std::min(room / r.stage, 8u);
+  if (r.stages < 2) return 0;
+  const uint32_t smem = RING_BARS + r.stages * r.stage;
+  static std::atomic<uint64_t> ready{0};                                   // devices on which the kernel has its shared memory
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev >= 64 || !(ready.load() >> dev & 1)) {
+    if (cudaFuncSetAttribute(k_rms_backward_ring<S, D, NV, TPR>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) return 0;
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
+  const int parts = parts_of(a.M, 1, per_sm);
+  k_rms_backward_ring<S, D, NV, TPR><<<parts, TPR, smem, st>>>(a, r);
+  return parts;
+}
+
 template <class S, class D>
-int backward(BwdArgs a, void* dw, int dw_type, cudaStream_t st) {
+int backward(const BwdArgs& a, void* dw, int dw_type, cudaStream_t st) {
   const bool vec = a.N % 8 == 0 && on_boundary(a.s, a.lds, type_code<S>()) && on_boundary(a.dy, a.N, type_code<D>()) &&
-                   on_boundary(a.ds, a.N, type_code<S>()) && on_boundary(a.dx, a.N, type_code<S>()) && on_boundary(a.dr, a.N, a.dr_type);
+                   on_boundary(a.ds, a.N, type_code<S>()) && on_boundary(a.dx, a.N, type_code<S>()) && on_boundary(a.dr, a.N, a.dr_type) &&
+                   on_boundary(a.w, a.N, a.w_type) && on_boundary(a.part, a.N, SPION_F32);
   int parts = 0;
-  // what is resident at a time and no more: every CTA leaves a partial row
-#define SPION_ROWS(VEC, NV, SUB, THREADS, threads, per_sm)                                                                      \
-  do {                                                                                                                          \
-    const int rpc = SUB ? (threads) / (SUB ? SUB : 1) : 1;                                                                      \
-    const long long need = (a.M + rpc - 1) / rpc, most = (long long)sm_count() * (per_sm);                                      \
-    parts = (int)(need < most ? need : most);                                                                                   \
-    if (parts > MAX_PARTS) parts = MAX_PARTS;                                                                                   \
-    k_rms_backward<S, D, VEC, NV, SUB, THREADS><<<parts, threads, 0, st>>>(a);                                                  \
-  } while (0)
   if (vec) {
     const int n = a.N / 8;
-    if (n <= 8) SPION_ROWS(8, 1, 8, CTA, CTA, 6);
-    else if (n <= 16) SPION_ROWS(8, 2, 8, CTA, CTA, 3);
-    else if (n <= 64) SPION_ROWS(8, 2, 32, CTA, CTA, 3);
-    else if (n <= 1024) SPION_ROWS(8, 2, 0, 512, threads_for(n, 2), 1024 / threads_for(n, 2) < 8 ? 1024 / threads_for(n, 2) : 8);
-    else if (n <= 2048) SPION_ROWS(8, 2, 0, 1024, threads_for(n, 2), 1);
+    if (n <= 8) parts = launch_backward<S, D, 8, 1, 8, 2>(a, 4, st);
+    else if (n <= 16) parts = launch_backward<S, D, 8, 2, 8>(a, 3, st);
+    else if (n <= 64) parts = launch_backward<S, D, 8, 2, 32>(a, 3, st);
+    else if (n <= 128) parts = launch_ring<S, D, 1, 128>(a, 4, st);
+    else if (n <= 256) parts = launch_ring<S, D, 1, 256>(a, 4, st);
+    else if (n <= 512) parts = launch_ring<S, D, 1, 512>(a, 2, st);
+    else if (n <= 1024) parts = launch_ring<S, D, 1, 1024>(a, 1, st);
+    else if (n <= 2048) parts = launch_ring<S, D, 2, 1024>(a, 1, st);
   } else {
-    if (a.N <= 128) SPION_ROWS(1, 4, 32, CTA, CTA, 4);
-    else if (a.N <= 512) SPION_ROWS(1, 16, 32, CTA, CTA, 2);
-    else if (a.N <= 8192) SPION_ROWS(1, 16, 0, 512, threads_for(a.N, 16), 1024 / threads_for(a.N, 16) < 8 ? 1024 / threads_for(a.N, 16) : 8);
+    if (a.N <= 128) parts = launch_backward<S, D, 1, 4, 32, 2>(a, 4, st);
+    else if (a.N <= 512) parts = launch_backward<S, D, 1, 16, 32>(a, 2, st);
+    else if (a.N <= 1024) parts = launch_backward<S, D, 1, 16, 64>(a, 8, st);
+    else if (a.N <= 2048) parts = launch_backward<S, D, 1, 16, 128>(a, 4, st);
+    else if (a.N <= 4096) parts = launch_backward<S, D, 1, 16, 256>(a, 2, st);
+    else if (a.N <= 8192) parts = launch_backward<S, D, 1, 16, 512>(a, 1, st);
   }
-#undef SPION_ROWS
   if (parts == 0) {
     if (vec) k_rms_backward_wide<S, D, 8><<<grid_of(a.M, 1, 512), 512, 0, st>>>(a);
     else k_rms_backward_wide<S, D, 1><<<grid_of(a.M, 1, 512), 512, 0, st>>>(a);
@@ -472,6 +653,22 @@ int backward(BwdArgs a, void* dw, int dw_type, cudaStream_t st) {
 bool stream_type(int t) { return t == SPION_F32 || t == SPION_BF16 || t == SPION_F16; }
 
 }  // namespace
+
+// Status word of the norm's backward on the current device, after the work of a stream (linear.cu reports it with its own)
+int rmsnorm_status(int reset, cudaStream_t st) {
+  int v = 0;
+  SPION_CUDA_TRY(cudaMemcpyFromSymbolAsync(&v, g_rms_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
+  SPION_CUDA_TRY(cudaStreamSynchronize(st));
+  if (v == 0) return SPION_OK;
+  if (reset) {
+    void* word = nullptr;
+    SPION_CUDA_TRY(cudaGetSymbolAddress(&word, g_rms_status));
+    SPION_CUDA_TRY(cudaMemsetAsync(word, 0, sizeof(int), st));
+    SPION_CUDA_TRY(cudaStreamSynchronize(st));
+  }
+  fprintf(stderr, "spion_b200: status word of the root-mean-square norm = 0x%x (a bounded wait gave up)\n", v);
+  return SPION_ERR_TIMEOUT;
+}
 
 extern "C" {
 

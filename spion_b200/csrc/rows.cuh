@@ -57,6 +57,10 @@ template <> struct Piece<float, 8> {
     asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p) : "memory");
   }
+  __device__ __forceinline__ void load_shared(const float* p) {
+    const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+  }
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = 0;
@@ -66,6 +70,7 @@ template <> struct Piece<float, 8> {
 template <class T> struct Piece16 {
   uint4 q;
   __device__ __forceinline__ void load(const T* p) { q = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void load_shared(const T* p) { load(p); }
   __device__ __forceinline__ void zero() { q = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ uint32_t word(int i) const { return i < 2 ? q.x : i < 4 ? q.y : i < 6 ? q.z : q.w; }
 };
@@ -124,8 +129,8 @@ template <> struct Out<__nv_fp8_e4m3, 8> {
   }
 };
 
-// ---- sums and maxima over the threads of a row.  SUB lanes (a power of two up to 32), or with SUB == 0 all warps of the CTA, whose partial results
-// go through shared memory: `buf` alternates between two halves of `part`, so one barrier a row is enough.
+// ---- sums and maxima over the TPR threads of a row: lanes (a power of two up to 32), or all warps of the CTA, whose partial results go through shared
+// memory.  `buf` alternates between two halves of `part`, so one barrier a row is enough.
 template <int LANES> __device__ __forceinline__ float lane_sum(float v) {
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -136,16 +141,17 @@ template <int LANES> __device__ __forceinline__ float lane_max(float v) {
   for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-template <int SUB, bool MAX> __device__ __forceinline__ void row_reduce(float& sum, float& top, float2 (*part)[32], int& buf) {
-  sum = lane_sum<SUB == 0 ? 32 : SUB>(sum);
-  if (MAX) top = lane_max<SUB == 0 ? 32 : SUB>(top);
-  if (SUB != 0) return;
-  const int nw = blockDim.x >> 5;
+template <int TPR, bool MAX> __device__ __forceinline__ void row_reduce(float& sum, float& top, float2 (*part)[32], int& buf) {
+  constexpr int LANES = TPR < 32 ? TPR : 32, WARPS = TPR / 32;
+  sum = lane_sum<LANES>(sum);
+  if (MAX) top = lane_max<LANES>(top);
+  if (TPR <= 32) return;
   if ((threadIdx.x & 31) == 0) part[buf][threadIdx.x >> 5] = make_float2(sum, top);
   __syncthreads();
-  float2 t = (int)(threadIdx.x & 31) < nw ? part[buf][threadIdx.x & 31] : make_float2(0.f, 0.f);
-  sum = lane_sum<32>(t.x);
-  if (MAX) top = lane_max<32>(t.y);
+  const float2 t = (int)(threadIdx.x & 31) < WARPS ? part[buf][threadIdx.x & 31] : make_float2(0.f, 0.f);
+  constexpr int UP = WARPS <= 2 ? 2 : WARPS <= 4 ? 4 : WARPS <= 8 ? 8 : WARPS <= 16 ? 16 : 32;
+  sum = __shfl_sync(0xffffffffu, lane_sum<UP>(t.x), 0);
+  if (MAX) top = __shfl_sync(0xffffffffu, lane_max<UP>(t.y), 0);
   buf ^= 1;
 }
 
