@@ -44,14 +44,19 @@ void same_device(const char* op, const Tensor& t, const Tensor& like, const char
 
 // A tensor's rows over its last dimension as the kernels read them: rows a constant step apart, elements next to one another.
 struct Rows {
-  Tensor t;                              // [M, N]
+  Tensor t;
   int64_t M = 0, N = 0, ld = 0;
   explicit Rows(const Tensor& x) {
     N = x.size(-1);
     M = N ? x.numel() / N : 0;
+    ld = N;
+    if (x.is_contiguous()) {
+      t = x;
+      return;
+    }
     t = x.reshape({M, N});               // a view where the strides allow it
     if (N > 1 && t.stride(1) != 1) t = t.contiguous();
-    ld = M > 1 ? t.stride(0) : N;
+    if (M > 1) ld = t.stride(0);
   }
 };
 
@@ -267,7 +272,7 @@ struct Operand8 {
     if (M > 0 && (((uintptr_t)values.data_ptr() | (uintptr_t)ld) % 16 != 0 || ld < N)) {
       ld = (N + 15) / 16 * 16;
       Tensor copy = empty_rows8(v, M, N);
-      copy.copy_(values);
+      copy.copy_(values.view({M, N}));
       values = copy;
     }
     scales = s.contiguous();
