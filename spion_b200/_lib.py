@@ -119,7 +119,7 @@ SIGNATURES = {
     "spion_rmsnorm_backward": (c_int, [c_void_p, c_longlong, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
                                        c_void_p, c_longlong, c_int, c_void_p]),
     "spion_linear_e4m3": (c_int, [c_void_p, c_longlong, c_void_p] * 2 + [c_void_p, c_int, c_void_p, c_longlong, c_int, c_longlong, c_int, c_int, c_void_p]),
-    "spion_adamw_step": (c_int, [ctypes.POINTER(AdamwTensor), c_int, c_int, c_int] + [c_void_p] * 6 + [c_double] * 6 + [ctypes.c_uint, c_int, c_void_p]),
+    "spion_adamw_step": (c_int, [ctypes.POINTER(AdamwTensor), c_int, c_int, c_int] + [c_void_p] * 6 + [c_double] * 6 + [ctypes.c_uint, c_int, c_void_p, c_void_p]),
     "spion_static_scratch_capacity": (ctypes.c_size_t, []),
     "spion_attn_forward_static": (c_int, [c_void_p] * 9 + [c_int] * 6 + [c_void_p]),
 }

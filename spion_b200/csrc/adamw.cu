@@ -14,13 +14,16 @@
 // parameter: nothing is uploaded or kept between calls, and a captured step replays with the addresses it was captured with.
 #include <math.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "rows.cuh"
 
 using namespace rows;
 
 namespace {
 
-constexpr int BLOCK = 256, CTA = 256, CHUNK = 8 * BLOCK;       // values of a chunk: a block per warp
+constexpr int BLOCK = 256, CTA = 256;                           // values that share scales; threads
 constexpr int FEW = 64, MOST = 512;                             // tensors of a launch
 
 struct Tensor {
@@ -28,18 +31,15 @@ struct Tensor {
   const void* g;
   void* copy;                 // or null: p in 16 bits
   long long n, at;            // values, place of the first in the moments (a multiple of 256)
-  int index;                  // number of the tensor
 };
 struct Step {
   void *m, *v;
   float *m_scale, *v_scale;   // 8 bits: one per block
-  const float* steps;
-  const float* lr_dev;        // or null: lr
-  double lr, wd, log_b1, log_b2;
+  const float4* factors;      // of each tensor of the launch, from k_adamw_begin
   float b1, b2, c1, c2;       // betas and what is left of one
   float eps, clip;            // clip < 0: none
-  unsigned seed;
   int count, chunks, copy_type;
+  int span;                   // values of a chunk: one block per warp, or several where there are many
 };
 template <int MAX> struct Table {
   Step s;
@@ -96,77 +96,165 @@ __device__ __forceinline__ float lane_max_nan(float v) {
   for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-// the update's quotient: two units in the last place are lost beside a parameter that is many times as large
-__device__ __forceinline__ float root_of(float x) {
-  float r;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
+// The update's quotient: a few units in its last place are lost beside a parameter that is many times as large.  v below fp32's normal numbers counts as
+// zero; beside an eps of 2^-40 or more its root is nothing (FLUSH; other steps take the exact forms).
+template <bool FLUSH> __device__ __forceinline__ float quotient(float m, float v, float root_v, float eps) {
+  if (!FLUSH) return m / (sqrtf(v) * root_v + eps);
+  float r, q;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(r * root_v + eps));
+  return m * q;
 }
 // 2^(exponent of a - below); a >= 2^-100
 __device__ __forceinline__ float scale_of(float a, int below) { return __uint_as_float(((__float_as_uint(a) >> 23) - below) << 23); }
 __device__ __forceinline__ float over_scale(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }      // 1 / a power of two
 __device__ __forceinline__ float size_if_finite(float x) { return fabsf(x) <= 3.402823466e38f ? fabsf(x) : 0.f; }
 
-// The products and sums that the moments' codes depend on are rounded one by one, as written (no contraction).
-template <class P, int BITS, int MAX>
-__global__ void __launch_bounds__(CTA, BITS == 8 ? 3 : 4) k_adamw(const __grid_constant__ Table<MAX> a) {
-  next_may_start();                                                      // k_adamw_steps
-  __shared__ float s_factor[2];
+// What a lane has of a block of 256: eight values as they lie in memory.
+template <class P, int BITS> struct Lane {
+  Piece<P, 8> p, g;
+  typename std::conditional<BITS == 32, Piece<float, 8>, uint2>::type m, v;
+  float sm, sv;
+};
+// The step on eight values.  The products and sums that the moments' codes depend on are rounded one by one, as written (no contraction).
+// `place` + `stride` e: the values' places in their tensor.
+template <int BITS, bool FLUSH>
+__device__ __forceinline__ void update(const Step& s, const float4& f, float (&p)[8], float (&g)[8], float (&m)[8], float (&v)[8], float& sm, float& sv, uint2& cm, uint2& cv,
+                                       unsigned place, unsigned stride, unsigned key) {
+  if (s.clip >= 0.f)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = min_nan(max_nan(g[e], -s.clip), s.clip);      // NaN stays
+  float top_m = 0x1p-100f, top_v = 0x1p-100f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (BITS == 8) m[e] *= sm, v[e] *= sv;
+    m[e] = __fadd_rn(__fmul_rn(m[e], s.b1), __fmul_rn(g[e], s.c1));
+    v[e] = __fadd_rn(__fmul_rn(v[e], s.b2), __fmul_rn(__fmul_rn(g[e], g[e]), s.c2));
+    p[e] = p[e] * f.x - f.y * quotient<FLUSH>(m[e], v[e], f.z, s.eps);
+    if (BITS == 8) top_m = max_nan(top_m, fabsf(m[e])), top_v = max_nan(top_v, v[e]);
+  }
+  if (BITS == 32) return;
+  top_m = lane_max_nan(top_m);
+  top_v = lane_max_nan(top_v);
+  unsigned wm[8], wv[8];                                                 // codes in the top bytes
+  if (top_m < 0x1p14f && top_v < 0x1p28f) {                              // all finite, and scale and fit are one factor within fp32's range
+    sm = scale_of(top_m, 7), sv = scale_of(top_v, 14);
+    const float um = over_scale(sm) * FIT_E4M3, uv = over_scale(sv) * FIT_E5M2;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned r = mix((place + stride * e) ^ key);
+      wm[e] = code_e4m3(m[e] * um, r);
+      wv[e] = code_e5m2(v[e] > 0.f ? fmaxf(v[e] * uv, __uint_as_float(1u << 21)) : 0.f, r);      // never zero beside a first moment that is not
+    }
+  } else {
+    top_m = top_v = 0x1p-100f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top_m = fmaxf(top_m, size_if_finite(m[e])), top_v = fmaxf(top_v, size_if_finite(v[e]));
+    sm = scale_of(lane_max<32>(top_m), 7), sv = scale_of(lane_max<32>(top_v), 14);
+    const float um = over_scale(sm), uv = over_scale(sv);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned r = mix((place + stride * e) ^ key);
+      wm[e] = code_e4m3(m[e] * um * FIT_E4M3, r);
+      if (size_if_finite(m[e]) != fabsf(m[e])) wm[e] = 0x7fu << 24;      // an infinity is a NaN in e4m3
+      wv[e] = code_e5m2(v[e] > 0.f ? fmaxf(v[e] * uv * FIT_E5M2, __uint_as_float(1u << 21)) : 0.f, r);
+      if (size_if_finite(v[e]) != v[e]) wv[e] = (v[e] != v[e] ? 0x7fu : 0x7cu) << 24;
+    }
+  }
+  cm = make_uint2(top_bytes(wm[0], wm[1], wm[2], wm[3]), top_bytes(wm[4], wm[5], wm[6], wm[7]));
+  cv = make_uint2(top_bytes(wv[0], wv[1], wv[2], wv[3]), top_bytes(wv[4], wv[5], wv[6], wv[7]));
+}
+
+template <int BITS> constexpr int CTAS = BITS == 32 ? 4 : 4;              // resident on a multiprocessor
+template <class P, int BITS, bool FLUSH, int MAX>
+__global__ void __launch_bounds__(CTA, CTAS<BITS>) k_adamw(const __grid_constant__ Table<MAX> a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int i = 0;
-  float known = -1.f, lr_m = 0.f, root_v = 0.f;                          // the step that the factors are for
-  const float b1 = a.s.b1, b2 = a.s.b2, c1 = a.s.c1, c2 = a.s.c2;
-  const double lr = a.s.lr_dev != nullptr ? (double)*a.s.lr_dev : a.s.lr;
-  const float keep = (float)(1.0 - lr * a.s.wd);
   for (int chunk = blockIdx.x; chunk < a.s.chunks; chunk += gridDim.x) {
-    int lo = i, hi = a.s.count;                                          // the last tensor that begins at or before the chunk
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.chunk[mid] <= chunk) lo = mid;
-      else hi = mid;
+    if (i + 1 < a.s.count && a.chunk[i + 1] <= chunk) {
+      int hi = a.s.count;                                                // the last tensor that begins at or before the chunk
+      while (hi - i > 1) {
+        const int mid = (i + hi) >> 1;
+        if (a.chunk[mid] <= chunk) i = mid;
+        else hi = mid;
+      }
     }
-    i = lo;
     const Tensor& t = a.t[i];
-    const long long base = (long long)(chunk - a.chunk[i]) * CHUNK + warp * BLOCK;     // of the warp's block in its tensor
-    const float step = a.s.steps[t.index] + 1.f;
-    P* const p = static_cast<P*>(t.p) + base;
-    const P* const g = static_cast<const P*>(t.g) + base;
-    const long long left = t.n - base;                                   // may be none
-    const bool whole = left >= BLOCK && (((uintptr_t)p | (uintptr_t)g) & (8 * sizeof(P) - 1)) == 0 &&
-                       (t.copy == nullptr || ((uintptr_t)t.copy & 15) == 0);
-    // whole blocks on a boundary: a lane has values 8 lane .. 8 lane + 7, else values lane, lane + 32, ...
-    const int first = whole ? 8 * lane : lane, stride = whole ? 1 : 32;
-    const long long at = t.at + base;
-    float pv[8], gv[8], m[8], v[8];
-    if (whole) {
-      Piece<P, 8> pp, pg;
-      pp.load(p + first);
-      pg.load(g + first);
-      if (BITS == 32) {
-        Piece<float, 8> pm, pw;
-        pm.load(static_cast<const float*>(a.s.m) + at + first);
-        pw.load(static_cast<const float*>(a.s.v) + at + first);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m[e] = pm.at(e), v[e] = pw.at(e);
+    const bool boundary = (((uintptr_t)t.p | (uintptr_t)t.g) & (8 * sizeof(P) - 1)) == 0 && ((uintptr_t)t.copy & 15) == 0;
+    const long long begin = (long long)(chunk - a.chunk[i]) * a.s.span, end = min(t.n, begin + a.s.span);
+    float4 f;
+    unsigned key;
+    // k_adamw_begin has been started after everything that this step reads was written: only what it writes itself is waited for, with the first block
+    // of values on its way
+    auto begun = [&] {
+      wait_for_kernel_before();
+      f = __ldcg(a.s.factors + i);
+      key = mix(__float_as_uint(f.w) + (unsigned)(begin >> 32));
+    };
+    bool first = true;
+    long long base = begin + warp * BLOCK;
+    // whole blocks on a boundary: a lane has values 8 lane .. 8 lane + 7
+    for (; boundary && base + BLOCK <= end; base += CTA / 32 * BLOCK) {
+      const long long k = base + 8 * lane, at = t.at + k;
+      Lane<P, BITS> now;
+      now.p.load(static_cast<P*>(t.p) + k);
+      now.g.load(static_cast<const P*>(t.g) + k);
+      if constexpr (BITS == 32) {
+        now.m.load(static_cast<const float*>(a.s.m) + at);
+        now.v.load(static_cast<const float*>(a.s.v) + at);
       } else {
-        const uint2 cm = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.s.m) + at + first);
-        const uint2 cv = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.s.v) + at + first);
+        now.m = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.s.m) + at);
+        now.v = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.s.v) + at);
+        now.sm = a.s.m_scale[at / BLOCK];
+        now.sv = a.s.v_scale[at / BLOCK];
+      }
+      if (first) begun();
+      first = false;
+      float p[8], g[8], m[8], v[8], sm = now.sm, sv = now.sv;
+      uint2 cm, cv;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] = now.p.at(e), g[e] = now.g.at(e);
+      if constexpr (BITS == 32) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m[e] = now.m.at(e), v[e] = now.v.at(e);
+      } else {
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-          const unsigned wm = e < 4 ? cm.x : cm.y, wv = e < 4 ? cv.x : cv.y;
-          const float2 fm = from_e4m3x2(e & 2 ? wm >> 16 : wm & 0xffffu), fv = from_e5m2x2(wv, e & 2 ? 0x3424 : 0x1404);
+          const unsigned x = e < 4 ? now.m.x : now.m.y, y = e < 4 ? now.v.x : now.v.y;
+          const float2 fm = from_e4m3x2(e & 2 ? x >> 16 : x & 0xffffu), fv = from_e5m2x2(y, e & 2 ? 0x3424 : 0x1404);
           m[e] = fm.x, m[e + 1] = fm.y, v[e] = fv.x, v[e + 1] = fv.y;
         }
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) pv[e] = pp.at(e), gv[e] = pg.at(e);
-    } else {
+      update<BITS, FLUSH>(a.s, f, p, g, m, v, sm, sv, cm, cv, (unsigned)k, 1, key);
+      Out<P, 8>::store(static_cast<P*>(t.p) + k, p);
+      if constexpr (BITS == 32) {
+        Out<float, 8>::store(static_cast<float*>(a.s.m) + at, m);
+        Out<float, 8>::store(static_cast<float*>(a.s.v) + at, v);
+      } else {
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.s.m) + at) = cm;
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.s.v) + at) = cv;
+        if (lane == 0) a.s.m_scale[at / BLOCK] = sm, a.s.v_scale[at / BLOCK] = sv;
+      }
+      if (t.copy != nullptr) {
+        if (a.s.copy_type == SPION_BF16) Out<__nv_bfloat16, 8>::store(static_cast<__nv_bfloat16*>(t.copy) + k, p);
+        else Out<__half, 8>::store(static_cast<__half*>(t.copy) + k, p);
+      }
+    }
+    // a tensor's last block, and tensors that lie off the boundaries: a lane has values lane, lane + 32, ...
+    for (; base < end; base += CTA / 32 * BLOCK) {
+      const int left = (int)min(end - base, (long long)BLOCK);
+      const long long at = t.at + base;
+      P* const tp = static_cast<P*>(t.p) + base;
+      const P* const tg = static_cast<const P*>(t.g) + base;
+      float p[8], g[8], m[8], v[8], sm = 0.f, sv = 0.f;
+      uint2 cm, cv;
+      if (BITS == 8) sm = a.s.m_scale[at / BLOCK], sv = a.s.v_scale[at / BLOCK];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int k = first + 32 * e;
+        const int k = lane + 32 * e;
         const bool in = k < left;
-        pv[e] = in ? as_float(p[k]) : 0.f;
-        gv[e] = in ? as_float(g[k]) : 0.f;
+        p[e] = in ? as_float(tp[k]) : 0.f;
+        g[e] = in ? as_float(tg[k]) : 0.f;
         if (BITS == 32) {
           m[e] = in ? static_cast<const float*>(a.s.m)[at + k] : 0.f;
           v[e] = in ? static_cast<const float*>(a.s.v)[at + k] : 0.f;
@@ -175,84 +263,15 @@ __global__ void __launch_bounds__(CTA, BITS == 8 ? 3 : 4) k_adamw(const __grid_c
           v[e] = in ? from_e5m2(static_cast<const uint8_t*>(a.s.v)[at + k]) : 0.f;
         }
       }
-    }
-    float sm = 0.f, sv = 0.f;
-    if (BITS == 8 && left > 0) sm = a.s.m_scale[at / BLOCK], sv = a.s.v_scale[at / BLOCK];
-    if (step != known) {                                                 // (the same for the whole CTA)
-      __syncthreads();
-      if (threadIdx.x == 0) s_factor[0] = (float)(lr / -expm1((double)step * a.s.log_b1));
-      if (threadIdx.x == 32) s_factor[1] = (float)(1.0 / sqrt(-expm1((double)step * a.s.log_b2)));
-      __syncthreads();
-      lr_m = s_factor[0], root_v = s_factor[1];
-      known = step;
-    }
-    if (left <= 0) continue;
-    if (a.s.clip >= 0.f)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) gv[e] = min_nan(max_nan(gv[e], -a.s.clip), a.s.clip);      // NaN stays
-    float top_m = 0x1p-100f, top_v = 0x1p-100f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (BITS == 8) m[e] *= sm, v[e] *= sv;
-      m[e] = __fadd_rn(__fmul_rn(m[e], b1), __fmul_rn(gv[e], c1));
-      v[e] = __fadd_rn(__fmul_rn(v[e], b2), __fmul_rn(__fmul_rn(gv[e], gv[e]), c2));
-      pv[e] = pv[e] * keep - lr_m * __fdividef(m[e], root_of(v[e]) * root_v + a.s.eps);
-      if (BITS == 8) top_m = max_nan(top_m, fabsf(m[e])), top_v = max_nan(top_v, v[e]);
-    }
-    uint2 cm, cv;                                                        // codes, one to a byte
-    if (BITS == 8) {
-      top_m = lane_max_nan(top_m);
-      top_v = lane_max_nan(top_v);
-      const unsigned key = mix(mix(a.s.seed + mix((unsigned)step * 0x9E3779B1u + (unsigned)t.index)) + (unsigned)(base >> 32));
-      unsigned r[8], wm[8], wv[8];                                       // random bits; codes in the top bytes
-#pragma unroll
-      for (int e = 0; e < 8; ++e) r[e] = mix((unsigned)(base + first + stride * e) ^ key);
-      if (top_m < 0x1p14f && top_v < 0x1p28f) {                          // all finite, and scale and fit are one factor within fp32's range
-        sm = scale_of(top_m, 7), sv = scale_of(top_v, 14);
-        const float um = over_scale(sm) * FIT_E4M3, uv = over_scale(sv) * FIT_E5M2;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          wm[e] = code_e4m3(m[e] * um, r[e]);
-          // never zero beside a first moment that is not
-          wv[e] = code_e5m2(v[e] > 0.f ? fmaxf(v[e] * uv, __uint_as_float(1u << 21)) : 0.f, r[e]);
-        }
-      } else {
-        top_m = top_v = 0x1p-100f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top_m = fmaxf(top_m, size_if_finite(m[e])), top_v = fmaxf(top_v, size_if_finite(v[e]));
-        sm = scale_of(lane_max<32>(top_m), 7), sv = scale_of(lane_max<32>(top_v), 14);
-        const float um = over_scale(sm), uv = over_scale(sv);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          wm[e] = code_e4m3(m[e] * um * FIT_E4M3, r[e]);
-          if (size_if_finite(m[e]) != fabsf(m[e])) wm[e] = 0x7fu << 24;  // an infinity is a NaN in e4m3
-          wv[e] = code_e5m2(v[e] > 0.f ? fmaxf(v[e] * uv * FIT_E5M2, __uint_as_float(1u << 21)) : 0.f, r[e]);
-          if (size_if_finite(v[e]) != v[e]) wv[e] = (v[e] != v[e] ? 0x7fu : 0x7cu) << 24;
-        }
-      }
-      cm = make_uint2(top_bytes(wm[0], wm[1], wm[2], wm[3]), top_bytes(wm[4], wm[5], wm[6], wm[7]));
-      cv = make_uint2(top_bytes(wv[0], wv[1], wv[2], wv[3]), top_bytes(wv[4], wv[5], wv[6], wv[7]));
-      if (lane == 0) a.s.m_scale[at / BLOCK] = sm, a.s.v_scale[at / BLOCK] = sv;
-    }
-    if (whole) {
-      Out<P, 8>::store(p + first, pv);
-      if (BITS == 32) {
-        Out<float, 8>::store(static_cast<float*>(a.s.m) + at + first, m);
-        Out<float, 8>::store(static_cast<float*>(a.s.v) + at + first, v);
-      } else {
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.s.m) + at + first) = cm;
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.s.v) + at + first) = cv;
-      }
-      if (t.copy != nullptr) {
-        if (a.s.copy_type == SPION_BF16) Out<__nv_bfloat16, 8>::store(static_cast<__nv_bfloat16*>(t.copy) + base + first, pv);
-        else Out<__half, 8>::store(static_cast<__half*>(t.copy) + base + first, pv);
-      }
-    } else {
+      if (first) begun();
+      first = false;
+      update<BITS, FLUSH>(a.s, f, p, g, m, v, sm, sv, cm, cv, (unsigned)(base + lane), 32, key);
+      if (BITS == 8 && lane == 0) a.s.m_scale[at / BLOCK] = sm, a.s.v_scale[at / BLOCK] = sv;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int k = first + 32 * e;
+        const int k = lane + 32 * e;
         if (k >= left) continue;
-        p[k] = rounded<P>(pv[e]);
+        tp[k] = rounded<P>(p[e]);
         if (BITS == 32) {
           static_cast<float*>(a.s.m)[at + k] = m[e];
           static_cast<float*>(a.s.v)[at + k] = v[e];
@@ -260,54 +279,74 @@ __global__ void __launch_bounds__(CTA, BITS == 8 ? 3 : 4) k_adamw(const __grid_c
           static_cast<uint8_t*>(a.s.m)[at + k] = (uint8_t)((e < 4 ? cm.x : cm.y) >> (8 * (e & 3)));
           static_cast<uint8_t*>(a.s.v)[at + k] = (uint8_t)((e < 4 ? cv.x : cv.y) >> (8 * (e & 3)));
         }
-        if (t.copy != nullptr) store_any(t.copy, a.s.copy_type, base + k, pv[e]);
+        if (t.copy != nullptr) store_any(t.copy, a.s.copy_type, base + k, p[e]);
       }
     }
   }
 }
 
-// The counts go up when every CTA has read them.
-template <int MAX> struct Indices {
+// Counts go up, and what a tensor's values have in common is formed once: {what weight decay leaves, lr / (1 - b1^t), 1 / sqrt(1 - b2^t), random key}.
+struct Begin {
   float* steps;
+  float4* factors;
+  const float* lr_dev;        // or null: lr
+  double lr, wd, log_b1, log_b2;
+  unsigned seed;
   int count;
+};
+template <int MAX> struct Indices {
+  Begin b;
   int index[MAX];
 };
-template <int MAX> __global__ void __launch_bounds__(MAX) k_adamw_steps(const __grid_constant__ Indices<MAX> a) {
-  wait_for_kernel_before();
-  if ((int)threadIdx.x < a.count) a.steps[a.index[threadIdx.x]] += 1.f;
+template <int MAX> __global__ void __launch_bounds__(MAX) k_adamw_begin(const __grid_constant__ Indices<MAX> a) {
+  next_may_start();                                                      // k_adamw
+  if ((int)threadIdx.x >= a.b.count) return;
+  const int i = a.index[threadIdx.x];
+  const float step = a.b.steps[i] + 1.f;
+  const double lr = a.b.lr_dev != nullptr ? (double)*a.b.lr_dev : a.b.lr;
+  a.b.steps[i] = step;
+  a.b.factors[threadIdx.x] =
+      make_float4((float)(1.0 - lr * a.b.wd), (float)(lr / -expm1((double)step * a.b.log_b1)), (float)(1.0 / sqrt(-expm1((double)step * a.b.log_b2))),
+                  __uint_as_float(mix(a.b.seed + mix((unsigned)step * 0x9E3779B1u + (unsigned)i))));
 }
 
-template <class P, int BITS, int MAX>
-int launch(const Step& s, const spion_adamw_tensor* ts, int count, float* steps, cudaStream_t st) {
+template <class P, int BITS, bool FLUSH, int MAX>
+int launch(const Step& s, const Begin& b, const spion_adamw_tensor* ts, int count, cudaStream_t st) {
   Table<MAX> a;
   Indices<MAX> ix;
   a.s = s;
   a.s.count = 0;
-  ix.steps = steps;
-  ix.count = 0;
-  long long chunks = 0;
-  for (int i = 0; i < count; ++i) {
-    ix.index[ix.count++] = ts[i].index;
-    if (ts[i].n == 0) continue;
-    a.chunk[a.s.count] = (int)chunks;
-    a.t[a.s.count++] = Tensor{ts[i].p, ts[i].g, ts[i].copy, ts[i].n, ts[i].at, ts[i].index};
-    chunks += (ts[i].n + CHUNK - 1) / CHUNK;
-    if (chunks > 0x7fffffff) return SPION_ERR_SHAPE;
-  }
+  ix.b = b;
+  ix.b.count = 0;
+  // chunks of four blocks a warp where that leaves eight to every CTA: 75 million values in 8 bits SPAN4 us, one block a warp SPAN1
+  long long chunks = 0, total = 0;
+  for (int i = 0; i < count; ++i) total += ts[i].n;
+  const long long most = (long long)sm_count() * CTAS<BITS>;
+  a.s.span = CTA / 32 * BLOCK * (BITS == 8 && total >= most * 8 * 4 * (CTA / 32 * BLOCK) ? 4 : 1);
+  for (int full = 1; full >= 0; --full)                                  // tensors without values last: they have a count only
+    for (int i = 0; i < count; ++i) {
+      if ((ts[i].n > 0) != (full == 1)) continue;
+      ix.index[ix.b.count++] = ts[i].index;
+      if (full == 0) continue;
+      a.chunk[a.s.count] = (int)chunks;
+      a.t[a.s.count++] = Tensor{ts[i].p, ts[i].g, ts[i].copy, ts[i].n, ts[i].at};
+      chunks += (ts[i].n + a.s.span - 1) / a.s.span;
+      if (chunks > 0x7fffffff) return SPION_ERR_SHAPE;
+    }
   a.s.chunks = (int)chunks;
-  if (chunks > 0) {
-    const long long most = (long long)sm_count() * (BITS == 8 ? 3 : 4);
-    k_adamw<P, BITS, MAX><<<(int)(chunks < most ? chunks : most), CTA, 0, st>>>(a);
-    SPION_LAUNCH_CHECK();
-  }
-  SPION_CUDA_TRY(launch_after(k_adamw_steps<MAX>, dim3(1), dim3(MAX), 0, st, ix));
+  k_adamw_begin<MAX><<<1, MAX, 0, st>>>(ix);
+  SPION_LAUNCH_CHECK();
+  if (chunks > 0)
+    SPION_CUDA_TRY(launch_after(k_adamw<P, BITS, FLUSH, MAX>, dim3((unsigned)(chunks < most ? chunks : most)), dim3(CTA), 0, st, a));
   return SPION_OK;
 }
 template <class P, int BITS>
-int launches(const Step& s, const spion_adamw_tensor* ts, int count, float* steps, cudaStream_t st) {
+int launches(const Step& s, const Begin& b, const spion_adamw_tensor* ts, int count, cudaStream_t st) {
   for (int i = 0; i < count; i += MOST) {
     const int n = count - i < MOST ? count - i : MOST;
-    const int rc = n <= FEW ? launch<P, BITS, FEW>(s, ts + i, n, steps, st) : launch<P, BITS, MOST>(s, ts + i, n, steps, st);
+    const bool flush = s.eps >= 0x1p-40f;
+    const int rc = n > FEW ? flush ? launch<P, BITS, true, MOST>(s, b, ts + i, n, st) : launch<P, BITS, false, MOST>(s, b, ts + i, n, st)
+                           : flush ? launch<P, BITS, true, FEW>(s, b, ts + i, n, st) : launch<P, BITS, false, FEW>(s, b, ts + i, n, st);
     if (rc != SPION_OK) return rc;
   }
   return SPION_OK;
@@ -317,24 +356,25 @@ int launches(const Step& s, const spion_adamw_tensor* ts, int count, float* step
 
 extern "C" int spion_adamw_step(const spion_adamw_tensor* host_tensors, int count, int type, int state_bits, void* m, void* v, float* m_scale,
                                 float* v_scale, float* steps, const float* lr_dev, double lr, double beta1, double beta2, double eps,
-                                double weight_decay, double clip_value, unsigned seed, int copy_type, void* cuda_stream) {
+                                double weight_decay, double clip_value, unsigned seed, int copy_type, void* workspace, void* cuda_stream) {
   if (count < 0 || (state_bits != 8 && state_bits != 32)) return SPION_ERR_ARG;
   if (count == 0) return SPION_OK;
-  if (host_tensors == nullptr || m == nullptr || v == nullptr || steps == nullptr || (state_bits == 8) != (m_scale != nullptr && v_scale != nullptr))
+  if (host_tensors == nullptr || m == nullptr || v == nullptr || steps == nullptr || workspace == nullptr || (state_bits == 8) != (m_scale != nullptr && v_scale != nullptr))
     return SPION_ERR_ARG;
   if (!(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0 && weight_decay >= 0) || (lr_dev == nullptr && !(lr >= 0))) return SPION_ERR_ARG;
-  if (((uintptr_t)m | (uintptr_t)v) & 31) return SPION_ERR_ARG;
+  if (((uintptr_t)m | (uintptr_t)v) & 31 || (uintptr_t)workspace & 15) return SPION_ERR_ARG;
   for (int i = 0; i < count; ++i) {
     const spion_adamw_tensor& t = host_tensors[i];
     if (t.n < 0 || t.at < 0 || t.at % BLOCK || t.index < 0 || (t.n > 0 && (t.p == nullptr || t.g == nullptr))) return SPION_ERR_ARG;
     if (t.copy != nullptr && copy_type != SPION_BF16 && copy_type != SPION_F16) return SPION_ERR_ARG;
   }
-  const Step s = {m, v, m_scale, v_scale, steps, lr_dev, lr, weight_decay, log(beta1), log(beta2), (float)beta1, (float)beta2, (float)(1.0 - beta1),
-                  (float)(1.0 - beta2), (float)eps, clip_value >= 0 ? (float)clip_value : -1.f, seed, 0, 0, copy_type};
+  const Step s = {m, v, m_scale, v_scale, static_cast<const float4*>(workspace), (float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2),
+                  (float)eps, clip_value >= 0 ? (float)clip_value : -1.f, 0, 0, copy_type, 0};
+  const Begin b = {steps, static_cast<float4*>(workspace), lr_dev, lr, weight_decay, log(beta1), log(beta2), seed, 0};
   const cudaStream_t st = (cudaStream_t)cuda_stream;
-  if (type == SPION_F32) return state_bits == 8 ? launches<float, 8>(s, host_tensors, count, steps, st) : launches<float, 32>(s, host_tensors, count, steps, st);
+  if (type == SPION_F32) return state_bits == 8 ? launches<float, 8>(s, b, host_tensors, count, st) : launches<float, 32>(s, b, host_tensors, count, st);
   if (type == SPION_BF16)
-    return state_bits == 8 ? launches<__nv_bfloat16, 8>(s, host_tensors, count, steps, st) : launches<__nv_bfloat16, 32>(s, host_tensors, count, steps, st);
-  if (type == SPION_F16) return state_bits == 8 ? launches<__half, 8>(s, host_tensors, count, steps, st) : launches<__half, 32>(s, host_tensors, count, steps, st);
+    return state_bits == 8 ? launches<__nv_bfloat16, 8>(s, b, host_tensors, count, st) : launches<__nv_bfloat16, 32>(s, b, host_tensors, count, st);
+  if (type == SPION_F16) return state_bits == 8 ? launches<__half, 8>(s, b, host_tensors, count, st) : launches<__half, 32>(s, b, host_tensors, count, st);
   return SPION_ERR_UNSUPPORTED;
 }

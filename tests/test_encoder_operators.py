@@ -48,12 +48,12 @@ def test_optimizer_arguments_at_the_c_boundary_and_in_the_module():
     L, d = _lib.lib, ctypes.c_void_p(4096)
 
     def step(tensors=((4096, 4096, None, 10, 0, 0),), type=_lib.F32, bits=32, m=d, v=d, sm=None, sv=None, steps=d, lr=1e-3, b1=0.9, b2=0.99, eps=1e-8, wd=0.0,
-             copy_type=_lib.BF16):
+             copy_type=_lib.BF16, ws=d):
         table = (_lib.AdamwTensor * len(tensors))(*tensors)
-        return L.spion_adamw_step(table, len(tensors), type, bits, m, v, sm, sv, steps, None, lr, b1, b2, eps, wd, -1.0, 0, copy_type, None)
+        return L.spion_adamw_step(table, len(tensors), type, bits, m, v, sm, sv, steps, None, lr, b1, b2, eps, wd, -1.0, 0, copy_type, ws, None)
 
     assert step(tensors=()) == 0
-    assert step(bits=16) == -1 and step(m=None) == -1 and step(v=None) == -1 and step(steps=None) == -1 and step(bits=8) == -1 and step(sm=d, sv=d) == -1
+    assert step(bits=16) == -1 and step(m=None) == -1 and step(v=None) == -1 and step(steps=None) == -1 and step(ws=None) == -1 and step(bits=8) == -1 and step(sm=d, sv=d) == -1
     assert step(lr=-1.0) == -1 and step(b1=1.0) == -1 and step(b2=-0.1) == -1 and step(eps=float("nan")) == -1 and step(wd=-1.0) == -1
     assert step(m=ctypes.c_void_p(4100)) == -1
     assert step(tensors=((None, 4096, None, 10, 0, 0),)) == -1 and step(tensors=((4096, None, None, 10, 0, 0),)) == -1
