@@ -2,7 +2,7 @@
 // y in fp32, bf16 or fp16.
 //
 //   k_lin8        tcgen05 kind::f8f6f4, 128 tokens x BN features per tile, accumulators in tensor memory
-//   k_lin8_few    up to 32 tokens, where the weights are all there is to read: mma.sync on fragments that go from global memory to registers
+//   k_lin8_few    up to 8 tokens, where the weights are all there is to read: mma.sync on fragments that go through shared memory as they lie
 //
 // Products of two e4m3 numbers are exact in fp32 and are summed there.  The scales are applied to the sums, so operands stay as they lie in memory.
 #include <algorithm>
@@ -34,17 +34,20 @@ struct Lin8Maps { CUtensorMap x, w, y; };
 // ------------------------------------------------------------------------------------------------ tokens by the tile
 constexpr int L8_EPI = 8;                                 // warps that write results: two to each quarter of the tensor memory
 constexpr int L8_THREADS = 32 * (2 + L8_EPI);
-constexpr uint32_t L8_A = 128 * 128;                      // bytes of a chunk of tokens: 128 rows, 128 of the contraction
-constexpr uint32_t L8_RING = 192 * 1024;
-constexpr uint32_t L8_OUT = 4096;                         // per writing warp: results on their way out
-template <int BN> struct L8 {
-  static constexpr uint32_t STAGE = L8_A + BN * 128;
-  static constexpr int STAGES = L8_RING / STAGE;
-  static constexpr uint32_t BARS = L8_RING + L8_EPI * (L8_OUT + 256);      // 256: scale and bias of 32 features
+constexpr uint32_t L8_OUT = 4096;                         // results on their way out: 32 rows of up to 128 bytes
+// BK: bytes of the contraction in a chunk, 128, or 64 where there are no more: a box that is half outside of its matrix takes longer than a full one (131072
+// tokens of 64 features to 64: BK128 us, BK64).  CTAS: on a multiprocessor.  Two where the contraction is a chunk or two: a tile's latencies are most of
+// its time then.
+template <int BN, int BK, int CTAS> struct L8 {
+  static constexpr uint32_t A = 128 * BK, STAGE = A + BN * BK;
+  static constexpr int STAGES = CTAS == 1 ? 192 * 1024 / STAGE : 2, OUTS = CTAS == 2 && BK == 64 ? 2 : 1;      // stages; buffers of a writing warp
+  static constexpr uint32_t RING = STAGES * STAGE;
+  static constexpr uint32_t SCALES = RING + L8_EPI * OUTS * L8_OUT, BARS = SCALES + L8_EPI * 256;      // per warp: scale and bias of 32 features
   static constexpr uint32_t SMEM = BARS + 16 * STAGES + 64;
   static constexpr int ACC = 2 * BN;                      // tensor memory columns: two tiles
 };
-static_assert(L8<256>::SMEM <= 232448 && L8<128>::SMEM <= 232448 && L8<64>::SMEM <= 232448, "shared memory of a CTA");
+static_assert(L8<256, 128, 1>::SMEM <= 232448 && L8<128, 128, 1>::SMEM <= 232448 && L8<64, 128, 1>::SMEM <= 232448 &&
+              2 * (L8<128, 128, 2>::SMEM + 1024) <= 233472 && 2 * (L8<128, 64, 2>::SMEM + 1024) <= 233472 && 2 * L8<128, 128, 2>::ACC <= 512, "shared and tensor memory of a multiprocessor");
 
 // Tiles in groups of 16 rows of tiles, column by column inside a group: the CTAs that run at a time share their operands in L2.
 __device__ __forceinline__ void tile_at(const Lin8Args& a, int i, int& m, int& n) {
@@ -75,14 +78,14 @@ __device__ __forceinline__ void st_shared16(uint32_t a, uint32_t x, uint32_t y, 
 }
 
 // Warp 0 loads, warp 1 multiplies, the others write.  Every wait is bounded; whoever gives up leaves, and so do all that wait for it.
-template <int BN, class Y>
-__global__ void __launch_bounds__(L8_THREADS, 1) k_lin8(const __grid_constant__ Lin8Args a, const __grid_constant__ Lin8Maps maps) {
-  using C = L8<BN>;
+template <int BN, int BK, int CTAS, class Y>
+__global__ void __launch_bounds__(L8_THREADS, CTAS) k_lin8(const __grid_constant__ Lin8Args a, const __grid_constant__ Lin8Maps maps) {
+  using C = L8<BN, BK, CTAS>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t sbase = smem_u32(smem_raw);
   const uint32_t full = sbase + C::BARS, empty = full + 8 * C::STAGES, acc_full = empty + 8 * C::STAGES, acc_empty = acc_full + 16, slot = acc_empty + 16;
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int chunks = (a.K + 127) >> 7, tiles = a.tiles_m * a.tiles_n;
+  const int chunks = (a.K + BK - 1) / BK, tiles = a.tiles_m * a.tiles_n;
   volatile int& s_abort = *reinterpret_cast<int*>(smem_raw + (slot + 8 - sbase));
   if (warp == 0 && lane == 0) {
     s_abort = *reinterpret_cast<volatile int*>(&g_lin8_status);
@@ -114,8 +117,8 @@ __global__ void __launch_bounds__(L8_THREADS, 1) k_lin8(const __grid_constant__ 
             ok = mbar_wait(empty + 8 * st, ph);
             if (!ok) break;
             mbar_expect_tx(full + 8 * st, C::STAGE);
-            tma_load_2d(sbase + st * C::STAGE, &maps.x, full + 8 * st, c * 128, m * 128);
-            tma_load_2d(sbase + st * C::STAGE + L8_A, &maps.w, full + 8 * st, c * 128, n * BN);
+            tma_load_2d(sbase + st * C::STAGE, &maps.x, full + 8 * st, c * BK, m * 128);
+            tma_load_2d(sbase + st * C::STAGE + C::A, &maps.w, full + 8 * st, c * BK, n * BN);
             if (++st == C::STAGES) st = 0, ph ^= 1;
           }
         }
@@ -124,7 +127,8 @@ __global__ void __launch_bounds__(L8_THREADS, 1) k_lin8(const __grid_constant__ 
     } else if (warp == 1) {
       if (elect_one()) {
         constexpr uint32_t idesc = idesc_e4m3(128, BN);
-        const uint64_t a0 = make_smem_desc(sbase, 16, 1024, LAYOUT_SW128), b0 = make_smem_desc(sbase + L8_A, 16, 1024, LAYOUT_SW128);
+        constexpr uint32_t layout = BK == 128 ? LAYOUT_SW128 : LAYOUT_SW64;
+        const uint64_t a0 = make_smem_desc(sbase, 16, 8 * BK, layout), b0 = make_smem_desc(sbase + C::A, 16, 8 * BK, layout);
         int st = 0, ph = 0, buf = 0, acc_ph = 1;
         bool ok = true;
         for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
@@ -134,9 +138,9 @@ __global__ void __launch_bounds__(L8_THREADS, 1) k_lin8(const __grid_constant__ 
             ok = mbar_wait(full + 8 * st, ph);
             if (!ok) break;
             tc_fence_after();
-            const int left = a.K - c * 128;
+            const int left = a.K - c * BK;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < BK / 32; ++k)
               if (32 * k < left)
                 mma_e4m3(tmem + buf * BN, desc_advance(a0, st * C::STAGE + 32 * k), desc_advance(b0, st * C::STAGE + 32 * k), idesc, c > 0 || k > 0);
             mma_commit(empty + 8 * st);
@@ -150,86 +154,111 @@ __global__ void __launch_bounds__(L8_THREADS, 1) k_lin8(const __grid_constant__ 
       }
     } else {
       const int q = warp & 3, half = (warp - 2) >> 2, me = warp - 2;
-      const uint32_t out = sbase + L8_RING + me * L8_OUT;
-      float2* const sb = reinterpret_cast<float2*>(smem_raw + L8_RING + L8_EPI * L8_OUT + me * 256);
-      int buf = 0, ph = 0, turn = 0;
-      for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
+      constexpr bool WIDE = sizeof(Y) == 4;
+      constexpr int COLS = WIDE || BN == 64 ? 32 : 64, ROW = COLS * (int)sizeof(Y);      // features of a store: rows of 64 or 128 bytes
+      const uint32_t out = sbase + C::RING + me * C::OUTS * L8_OUT;
+      float2* const sb = reinterpret_cast<float2*>(smem_raw + C::SCALES + me * 256);
+      int buf = 0, ph = 0, turn = 0, scaled = -1;
+      float sx = 0.f, sw[BN / 64], b[BN / 64];
+      // the scales of a tile are read while the one before is written: their way from memory is as long as a small tile's time
+      auto row_scale = [&](int i) {
         int m, n;
+        if (i >= tiles) return 0.f;
         tile_at(a, i, m, n);
-        const int t = m * 128 + q * 32 + lane, c0 = n * BN + half * (BN / 2);
-        const float sx = t < a.T ? a.sx[t] : 0.f;
-        float sw[BN / 64], b[BN / 64];
+        const int t = m * 128 + q * 32 + lane;
+        return t < a.T ? a.sx[t] : 0.f;
+      };
+      auto column_scales = [&](int i) {
+        int m, n;
+        if (i >= tiles) return;
+        tile_at(a, i, m, n);
+        if (n == scaled) return;
+        scaled = n;
 #pragma unroll
         for (int g = 0; g < BN / 64; ++g) {
-          const int c = c0 + 32 * g + lane;
+          const int c = n * BN + half * (BN / 2) + 32 * g + lane;
           sw[g] = c < a.N ? a.sw[c] : 0.f;
           b[g] = c < a.N && a.bias != nullptr ? load_any(a.bias, a.bias_type, c) : 0.f;
         }
+      };
+      sx = row_scale(blockIdx.x);
+      column_scales(blockIdx.x);
+      for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
+        int m, n;
+        tile_at(a, i, m, n);
+        const int c0 = n * BN + half * (BN / 2);
+        const float next = row_scale(i + gridDim.x);
         if (!tc::warp_wait(acc_full + 8 * buf, ph, &g_lin8_status, ERR_MMA2_WAIT)) break;
         tc_fence_after();
 #pragma unroll
-        for (int g = 0; g < BN / 64; ++g) {
-          const int c = c0 + 32 * g;
-          uint32_t r[32];
-          tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + buf * BN + half * (BN / 2) + 32 * g, r);
-          sb[lane] = make_float2(sw[g], b[g]);
-          tmem_ld_wait();
-          if (g == BN / 64 - 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty + 8 * buf);
-          }
-          __syncwarp();
-          float v[32];
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float4 f = *reinterpret_cast<const float4*>(sb + e);
-            v[e] = fmaf(__uint_as_float(r[e]) * sx, f.x, f.y);
-            v[e + 1] = fmaf(__uint_as_float(r[e + 1]) * sx, f.z, f.w);
-          }
-          if (c >= a.N) { __syncwarp(); continue; }
-          constexpr bool WIDE = sizeof(Y) == 4;
-          const uint32_t tile = out + (WIDE ? 0 : (turn & 1) * 2048);
+        for (int g0 = 0; g0 < BN / 2; g0 += COLS) {
+          const int c = c0 + g0;
+          const uint32_t tile = out + turn * L8_OUT;
           if (a.staged) {                                // the bulk store that read this buffer last has done so
             if (lane == 0) {
-              if (WIDE) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+              if (C::OUTS == 1) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
               else asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
             }
             __syncwarp();
           }
-          if constexpr (WIDE) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              st_shared16(tile + lane * 128 + ((k ^ (lane & 7)) << 4), __float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]),
-                          __float_as_uint(v[4 * k + 2]), __float_as_uint(v[4 * k + 3]));
-          } else {
+          for (int g = g0; g < g0 + COLS; g += 32) {
+            uint32_t r[32];
+            tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + buf * BN + half * (BN / 2) + g, r);
+            __syncwarp();
+            sb[lane] = make_float2(sw[g / 32], b[g / 32]);
+            tmem_ld_wait();
+            if (g == BN / 2 - 32) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(acc_empty + 8 * buf);
+            }
+            __syncwarp();
+            float v[32];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              st_shared16(tile + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4), pack16(v[8 * k], v[8 * k + 1], Y()), pack16(v[8 * k + 2], v[8 * k + 3], Y()),
-                          pack16(v[8 * k + 4], v[8 * k + 5], Y()), pack16(v[8 * k + 6], v[8 * k + 7], Y()));
+            for (int e = 0; e < 32; e += 2) {
+              const float4 f = *reinterpret_cast<const float4*>(sb + e);
+              v[e] = fmaf(__uint_as_float(r[e]) * sx, f.x, f.y);
+              v[e + 1] = fmaf(__uint_as_float(r[e + 1]) * sx, f.z, f.w);
+            }
+            // pieces of 16 bytes in the swizzle of the store's map
+            const uint32_t row = tile + lane * ROW, turned = ROW == 128 ? lane & 7 : (lane >> 1) & 3;
+            if constexpr (WIDE) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                st_shared16(row + ((k ^ turned) << 4), __float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]),
+                            __float_as_uint(v[4 * k + 3]));
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                st_shared16(row + (((k + (g - g0) / 8) ^ turned) << 4), pack16(v[8 * k], v[8 * k + 1], Y()), pack16(v[8 * k + 2], v[8 * k + 3], Y()),
+                            pack16(v[8 * k + 4], v[8 * k + 5], Y()), pack16(v[8 * k + 6], v[8 * k + 7], Y()));
+            }
           }
           if (a.staged) {
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(&maps.y, tile, c, m * 128 + q * 32);
-              bulk_commit();
-            }
+            if (lane == 0 && c < a.N) tma_store_2d(&maps.y, tile, c, m * 128 + q * 32);
+            if (lane == 0) bulk_commit();
           } else {                                       // rows that start anywhere: lanes side by side along each
             __syncwarp();
             const uint8_t* const from = smem_raw + (tile - sbase);
-            Y* const y = static_cast<Y*>(a.y) + (long long)(m * 128 + q * 32) * a.ldy + c + lane;
             const int rows_here = min(32, a.T - (m * 128 + q * 32));
-            if (c + lane < a.N)
-              for (int row = 0; row < rows_here; ++row) {
-                const uint32_t at = WIDE ? row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4
-                                         : row * 64 + (((lane >> 3) ^ ((row >> 1) & 3)) << 4) + (lane & 7) * 2;
-                y[row * a.ldy] = *reinterpret_cast<const Y*>(from + at);
-              }
+            constexpr int PER = 16 / (int)sizeof(Y);     // elements of a piece
+#pragma unroll
+            for (int g = 0; g < COLS; g += 32) {
+              const int e = g + lane;
+              Y* const y = static_cast<Y*>(a.y) + (long long)(m * 128 + q * 32) * a.ldy + c + e;
+              if (c + e < a.N)
+                for (int r = 0; r < rows_here; ++r)
+                  y[r * a.ldy] = *reinterpret_cast<const Y*>(from + r * ROW + (((e / PER) ^ (ROW == 128 ? r & 7 : (r >> 1) & 3)) << 4) + e % PER * (int)sizeof(Y));
+            }
             __syncwarp();
           }
-          ++turn;
+          if (C::OUTS == 2) turn ^= 1;
         }
+        sx = next;
+        column_scales(i + gridDim.x);
         buf ^= 1;
         if (buf == 0) ph ^= 1;
       }
@@ -243,14 +272,15 @@ __global__ void __launch_bounds__(L8_THREADS, 1) k_lin8(const __grid_constant__ 
 }
 
 // ------------------------------------------------------------------------------------------------ few tokens
-constexpr int FEW_WARPS = 8, FEW_ROWS = 16, FEW_DEPTH = 4;
-__device__ __forceinline__ uint4 zero4() { return make_uint4(0, 0, 0, 0); }
-// sixteen bytes from place k of a row of K, zeros behind its end
-__device__ __forceinline__ uint4 load_row16(const uint8_t* row, int k, int K, bool in) {
-  if (!in || k >= K) return zero4();
-  if (k + 16 <= K) return *reinterpret_cast<const uint4*>(row + k);
+constexpr int FEW_WARPS = 8, FEW_ROWS = 16;
+constexpr int FEW_TOKENS = 8, FEW_CHUNK = 2048, FEW_LD = FEW_CHUNK + 64;      // bytes of a row at a time; rows in shared memory: eight lanes read two without conflict
+constexpr uint32_t FEW_STAGE = (FEW_ROWS + FEW_TOKENS) * FEW_LD, FEW_SMEM = 2 * FEW_STAGE + 64;
+// the last K % 16 bytes of a row
+__device__ __forceinline__ uint4 load_tail(bool in, const uint8_t* p, int count) {
   uint32_t w[4] = {0, 0, 0, 0};
-  for (int i = 0; i < K - k; ++i) w[i >> 2] |= (uint32_t)row[k + i] << (8 * (i & 3));
+#pragma unroll
+  for (int i = 0; i < 15; ++i)
+    if (in && i < count) w[i >> 2] |= (uint32_t)p[i] << (8 * (i & 3));
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 __device__ __forceinline__ void mma_16x8x32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -259,53 +289,77 @@ __device__ __forceinline__ void mma_16x8x32(float (&d)[4], uint32_t a0, uint32_t
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// A CTA has 16 features, its warps take every eighth piece of 64 of the contraction.  Four lanes read 64 bytes of a row side by side; which four of a lane's 16
-// bytes the product takes for which index of the contraction does not matter as long as tokens and weights agree, so a lane's words are used as they come.
-template <int NT, class Y>
+__device__ __forceinline__ void multiply(uint4 u, uint4 v, uint4 x, float (&d)[4]) {
+  mma_16x8x32(d, u.x, v.x, u.y, v.y, x.x, x.y);
+  mma_16x8x32(d, u.z, v.z, u.w, v.w, x.z, x.w);
+}
+// A CTA has 16 features.  Bulk copies bring 2048 bytes of each feature's and each token's row at a time, twice that is under way; the CTA's warps take every
+// eighth piece of 64.  Which four bytes of a lane's 16 the product takes for which index of the contraction does not matter as long as tokens and weights
+// agree, so a lane's words are used as they come.  Loads to registers instead were ordered one behind another by the compiler (one token, 4096 to 4096
+// features: FEWREG us, so FEWBULK).
+template <class Y>
 __global__ void __launch_bounds__(32 * FEW_WARPS) k_lin8_few(const __grid_constant__ Lin8Args a) {
-  __shared__ float part[FEW_WARPS][FEW_ROWS][8 * NT + 1];
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ float part[FEW_WARPS][FEW_ROWS][FEW_TOKENS + 1];
+  const uint32_t rows0 = smem_u32(smem_raw), bars = rows0 + 2 * FEW_STAGE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, k0 = (lane & 3) * 16;
-  const int n = blockIdx.x * FEW_ROWS + g;
-  const uint8_t* const w0 = a.w + (long long)n * a.ldw;
-  const uint8_t* const w1 = w0 + 8 * a.ldw;
-  const bool in0 = n < a.N, in1 = n + 8 < a.N;
-  float acc[NT][4];
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-  const int pieces = (a.K + 63) >> 6;
+  const int n0 = blockIdx.x * FEW_ROWS, whole = a.K & ~15, chunks = (whole + FEW_CHUNK - 1) / FEW_CHUNK;
+  const int features = min(FEW_ROWS, a.N - n0);
+  // rows that do not exist stay what is there: they meet no row that does
+  auto fill = [&](int c) {                               // one warp
+    const int st = c & 1, bytes = min(FEW_CHUNK, whole - c * FEW_CHUNK);
+    if (lane == 0) mbar_expect_tx(bars + 8 * st, (features + a.T) * (uint32_t)bytes);
+    __syncwarp();
+    const uint32_t to = rows0 + st * FEW_STAGE;
+    if (lane < features) bulk_load(to + lane * FEW_LD, a.w + (long long)(n0 + lane) * a.ldw + c * FEW_CHUNK, bars + 8 * st, bytes);
+    if (lane < a.T) bulk_load(to + (FEW_ROWS + lane) * FEW_LD, a.x + (long long)lane * a.ldx + c * FEW_CHUNK, bars + 8 * st, bytes);
+  };
+  if (threadIdx.x == 0) {
+    mbar_init(bars, 1);
+    mbar_init(bars + 8, 1);
+    fence_barrier_init();
+    fence_proxy_async();
+  }
+  const int lost = *reinterpret_cast<volatile int*>(&g_lin8_status);
   wait_for_kernel_before();
-  for (int p0 = warp; p0 < pieces; p0 += FEW_WARPS * FEW_DEPTH) {
-    uint4 u[FEW_DEPTH], v[FEW_DEPTH], x[FEW_DEPTH][NT];
-#pragma unroll
-    for (int d = 0; d < FEW_DEPTH; ++d) {
-      const int k = (p0 + d * FEW_WARPS) * 64 + k0;
-      u[d] = load_row16(w0, k, a.K, in0);
-      v[d] = load_row16(w1, k, a.K, in1);
-    }
-#pragma unroll
-    for (int d = 0; d < FEW_DEPTH; ++d) {
-      const int k = (p0 + d * FEW_WARPS) * 64 + k0;
-#pragma unroll
-      for (int j = 0; j < NT; ++j) x[d][j] = load_row16(a.x + (long long)(8 * j + g) * a.ldx, k, a.K, 8 * j + g < a.T);
-    }
-#pragma unroll
-    for (int d = 0; d < FEW_DEPTH; ++d)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        mma_16x8x32(acc[j], u[d].x, v[d].x, u[d].y, v[d].y, x[d][j].x, x[d][j].y);
-        mma_16x8x32(acc[j], u[d].z, v[d].z, u[d].w, v[d].w, x[d][j].z, x[d][j].w);
+  if (__syncthreads_or(lost)) return;
+  if (warp == 0)
+    for (int c = 0; c < min(chunks, 2); ++c) fill(c);
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int c = 0; c < chunks; ++c) {
+    const int st = c & 1, bytes = min(FEW_CHUNK, whole - c * FEW_CHUNK);
+    if (!__syncthreads_and(mbar_wait(bars + 8 * st, (c >> 1) & 1))) {
+      if (threadIdx.x == 0) {
+        report(&g_lin8_status, ERR_LOAD_WAIT);
+        if (c + 1 < chunks) mbar_wait(bars + 8 * (st ^ 1), ((c + 1) >> 1) & 1);      // the copies under way end first, or this gives up again
       }
+      return;
+    }
+    const uint8_t* const from = smem_raw + st * FEW_STAGE + g * FEW_LD + k0;
+#pragma unroll
+    for (int d = 0; d < FEW_CHUNK / 64 / FEW_WARPS; ++d) {
+      const int k = (warp + d * FEW_WARPS) * 64;
+      if (k >= bytes) break;
+      const bool in = k + k0 < bytes;
+      const uint4 none = make_uint4(0, 0, 0, 0);
+      const uint4 u = in ? *reinterpret_cast<const uint4*>(from + k) : none, v = in ? *reinterpret_cast<const uint4*>(from + 8 * FEW_LD + k) : none;
+      multiply(u, v, in ? *reinterpret_cast<const uint4*>(from + FEW_ROWS * FEW_LD + k) : none, acc);
+    }
+    if (c + 2 < chunks) {
+      __syncthreads();                                   // all warps are done with this half
+      if (warp == 0) fill(c + 2);
+    }
+  }
+  if (whole < a.K && warp == 0) {
+    const uint8_t* const w = a.w + (long long)(n0 + g) * a.ldw + whole;
+    const uint4 u = load_tail(g < features && k0 == 0, w, a.K - whole), v = load_tail(g + 8 < features && k0 == 0, w + 8 * a.ldw, a.K - whole);
+    multiply(u, v, load_tail(g < a.T && k0 == 0, a.x + (long long)g * a.ldx + whole, a.K - whole), acc);
   }
   const int t0 = 2 * (lane & 3);
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    part[warp][g][8 * j + t0] = acc[j][0], part[warp][g][8 * j + t0 + 1] = acc[j][1];
-    part[warp][g + 8][8 * j + t0] = acc[j][2], part[warp][g + 8][8 * j + t0 + 1] = acc[j][3];
-  }
+  part[warp][g][t0] = acc[0], part[warp][g][t0 + 1] = acc[1];
+  part[warp][g + 8][t0] = acc[2], part[warp][g + 8][t0 + 1] = acc[3];
   __syncthreads();
-  for (int i = threadIdx.x; i < FEW_ROWS * 8 * NT; i += 32 * FEW_WARPS) {
+  for (int i = threadIdx.x; i < FEW_ROWS * FEW_TOKENS; i += 32 * FEW_WARPS) {
     const int row = i & (FEW_ROWS - 1), t = i / FEW_ROWS, c = blockIdx.x * FEW_ROWS + row;
     if (t >= a.T || c >= a.N) continue;
     float s = 0.f;
@@ -348,7 +402,18 @@ int map_of(CUtensorMap* m, Encode encode, const void* base, int type, long long 
   return SPION_OK;
 }
 
-template <int BN, class Y> int launch_tiles(Lin8Args a, cudaStream_t st) {
+// once per kernel (the static of this instance) and device
+template <auto Kernel> int big_shared_memory_of(uint32_t bytes) {
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  SPION_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev >= 64 || !(ready.load() >> dev & 1)) {
+    SPION_CUDA_TRY(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
+  return SPION_OK;
+}
+template <int BN, int BK, int CTAS, class Y> int launch_tiles(Lin8Args a, cudaStream_t st) {
   Encode encode;
   int rc = encoder(&encode);
   if (rc != SPION_OK) return rc;
@@ -357,36 +422,34 @@ template <int BN, class Y> int launch_tiles(Lin8Args a, cudaStream_t st) {
   if ((long long)a.tiles_m * a.tiles_n > 0x7fffffff) return SPION_ERR_SHAPE;
   a.staged = ((uintptr_t)a.y % 16 == 0) && (a.ldy * (long long)sizeof(Y)) % 16 == 0;
   Lin8Maps maps;
-  if ((rc = map_of(&maps.x, encode, a.x, SPION_E4M3, a.K, a.T, a.ldx, 128, 128)) != SPION_OK) return rc;
-  if ((rc = map_of(&maps.w, encode, a.w, SPION_E4M3, a.K, a.N, a.ldw, 128, BN)) != SPION_OK) return rc;
+  if ((rc = map_of(&maps.x, encode, a.x, SPION_E4M3, a.K, a.T, a.ldx, BK, 128)) != SPION_OK) return rc;
+  if ((rc = map_of(&maps.w, encode, a.w, SPION_E4M3, a.K, a.N, a.ldw, BK, BN)) != SPION_OK) return rc;
   if (a.staged) {
-    if ((rc = map_of(&maps.y, encode, a.y, type_code<Y>(), a.N, a.T, a.ldy, 32, 32)) != SPION_OK) return rc;
+    if ((rc = map_of(&maps.y, encode, a.y, type_code<Y>(), a.N, a.T, a.ldy, sizeof(Y) == 4 || BN == 64 ? 32 : 64, 32)) != SPION_OK) return rc;
   } else {
     maps.y = maps.x;                                     // not used
   }
-  static std::atomic<uint64_t> ready{0};                 // devices on which the kernel has its shared memory
-  int dev = 0;
-  SPION_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev >= 64 || !(ready.load() >> dev & 1)) {
-    SPION_CUDA_TRY(cudaFuncSetAttribute(k_lin8<BN, Y>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L8<BN>::SMEM));
-    if (dev < 64) ready.fetch_or(1ull << dev);
-  }
+  if ((rc = big_shared_memory_of<k_lin8<BN, BK, CTAS, Y>>(L8<BN, BK, CTAS>::SMEM)) != SPION_OK) return rc;
   const int tiles = a.tiles_m * a.tiles_n;
-  SPION_CUDA_TRY(launch_after(k_lin8<BN, Y>, dim3(std::min(tiles, sm_count())), dim3(L8_THREADS), L8<BN>::SMEM, st, a, maps));
+  SPION_CUDA_TRY(launch_after(k_lin8<BN, BK, CTAS, Y>, dim3(std::min(tiles, sm_count() * CTAS)), dim3(L8_THREADS), L8<BN, BK, CTAS>::SMEM, st, a, maps));
+  return SPION_OK;
+}
+template <class Y> int launch_few(const Lin8Args& a, cudaStream_t st) {
+  const int rc = big_shared_memory_of<k_lin8_few<Y>>(FEW_SMEM);
+  if (rc != SPION_OK) return rc;
+  SPION_CUDA_TRY(launch_after(k_lin8_few<Y>, dim3((a.N + FEW_ROWS - 1) / FEW_ROWS), dim3(32 * FEW_WARPS), FEW_SMEM, st, a));
   return SPION_OK;
 }
 template <class Y> int launch_any(const Lin8Args& a, cudaStream_t st) {
-  if (a.T <= 32) {
-    const dim3 grid((a.N + FEW_ROWS - 1) / FEW_ROWS), block(32 * FEW_WARPS);
-    if (a.T <= 8) SPION_CUDA_TRY(launch_after(k_lin8_few<1, Y>, grid, block, 0, st, a));
-    else if (a.T <= 16) SPION_CUDA_TRY(launch_after(k_lin8_few<2, Y>, grid, block, 0, st, a));
-    else SPION_CUDA_TRY(launch_after(k_lin8_few<4, Y>, grid, block, 0, st, a));
-    return SPION_OK;
-  }
+  // 4096 to 4096 features, few / tiles: 8 tokens 6.1 us / 11.6, 16 tokens (twice the products) 10.4 / 11.6; 512 to 16384, 32 tokens 26 / 6.3: mma.sync is slow on
+  // 8-bit operands here, and what it does for more tokens outlasts the weights
+  if (a.T <= FEW_TOKENS) return launch_few<Y>(a, st);
   const long long rows_ = (a.T + 127) / 128, sms = sm_count();
-  if (a.N > 128 && rows_ * ((a.N + 255) / 256) >= sms) return launch_tiles<256, Y>(a, st);
-  if (a.N > 64 && rows_ * ((a.N + 127) / 128) >= sms) return launch_tiles<128, Y>(a, st);
-  return launch_tiles<64, Y>(a, st);
+  const bool wide = a.N > 64 && rows_ * ((a.N + 127) / 128) >= sms;
+  if (a.K <= 64) return wide ? launch_tiles<128, 64, 2, Y>(a, st) : launch_tiles<64, 64, 2, Y>(a, st);
+  if (a.K <= 256) return wide ? launch_tiles<128, 128, 2, Y>(a, st) : launch_tiles<64, 128, 2, Y>(a, st);
+  if (a.N > 128 && rows_ * ((a.N + 255) / 256) >= sms) return launch_tiles<256, 128, 1, Y>(a, st);
+  return wide ? launch_tiles<128, 128, 1, Y>(a, st) : launch_tiles<64, 128, 1, Y>(a, st);
 }
 
 }  // namespace

@@ -77,7 +77,7 @@ __device__ __forceinline__ float row_scale(float top, float sum, float& scale) {
 
 // TPR threads to a row: 8 or 32 lanes of a warp, more: a CTA of that many.  Lanes take UR rows at a time, so that enough bytes are in flight.
 template <class S, class R, class Y, int VEC, int NV, int TPR, int UR>
-__global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR) k_rms_forward(const FwdArgs a) {
+__global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR, VEC == 8 && TPR == 8 && NV * UR <= 2 ? 4 : 1) k_rms_forward(const FwdArgs a) {
   constexpr bool Q = type_code<Y>() == SPION_E4M3;
   constexpr int THREADS = TPR <= 32 ? CTA : TPR, RPC = THREADS / TPR, RPW = TPR <= 32 ? 32 / TPR : 1;      // rows of a CTA and of a warp
   __shared__ float2 part[2][32];
