@@ -101,6 +101,7 @@ class Attention(nn.Module):
             self.attn = Dense(config, attn_cpp, attn_handle)
 
         self.ff = Linear(self.num_head * self.head_dim, self.dim)
+        self.linear8 = None
         if torch.cuda.is_available():
             _lib.check(_lib.lib.spion_linear_prepare(int(self.native_dtype == torch.float32)), "spion_linear_prepare")
 
@@ -193,6 +194,22 @@ class Attention(nn.Module):
         attn_out = self.combine_heads(attn_out)
         out = linear(self.ff, attn_out)
         return out, attn
+
+    def quantize(self, on: bool = True):
+        """Keep the projections' weights in 8 bits beside those that train, as they are now, for ``forward_quantized``."""
+        from .quant import E4M3Linear
+        if on and not self.native:
+            raise _lib.SpionError("8-bit projections are served beside the native attention (config['native'])")
+        self.linear8 = [E4M3Linear(m, self.native_dtype) for m in (self.W_q, self.W_k, self.W_v, self.ff)] if on else None
+
+    def forward_quantized(self, X, mask, mat):
+        """``forward`` of the sparse phase with the projections on 8-bit operands.  X: ``Rows8`` [B, L, dim].  No gradients."""
+        if self.linear8 is None:
+            raise _lib.SpionError("quantize() comes first")
+        W_q, W_k, W_v, ff = self.linear8
+        with torch.autocast(device_type="cuda", enabled=False):
+            out, attn = self.block_attn(*(self.split_heads(W(X)) for W in (W_q, W_k, W_v)), mask.float(), mat)
+            return ff(self.combine_heads(out)), attn
 
     def reconstruct_for_blocksparse(self, config):
         num_batches = int(config["num_head"] * config["batch_size"])

@@ -43,9 +43,14 @@ def task_config(task: str, batch_size: int, native: bool = True, dtype: str = "f
 def make_norm(config, feeds_linear: bool):
     """LayerNorm of the encoder: the library's kernels when the configuration asks for the native path and the
     width is one they serve, else torch.nn.LayerNorm (what the reference uses).  feeds_linear: the output only
-    goes into linear layers, so under mixed precision it may be bf16 straight away."""
+    goes into linear layers, so under mixed precision it may be bf16 straight away.  ``config["norm"] = "rms"``: root-mean-square norm."""
     from .layernorm import SUPPORTED_WIDTHS, FusedLayerNorm
     dim = config["transformer_dim"]
+    if config.get("norm", "layer") == "rms":
+        from .rmsnorm import FusedRMSNorm
+        return FusedRMSNorm(dim, bf16_out=feeds_linear) if config.get("native") else nn.RMSNorm(dim, eps=1e-6)
+    if config.get("norm", "layer") != "layer":
+        raise ValueError(f"config['norm'] is {config['norm']!r}: 'layer' and 'rms' are served")
     if config.get("native") and config.get("fused_layernorm", True) and dim in SUPPORTED_WIDTHS:
         return FusedLayerNorm(dim, bf16_out=feeds_linear)
     return nn.LayerNorm(dim)
@@ -85,6 +90,7 @@ class TransformerLayer(nn.Module):
             from .layernorm import BiasGradLinear as Linear
         self.mlp_types = (Linear, nn.GELU, nn.Dropout, Linear, nn.Dropout)
         self.fuse_mlp = Linear is not nn.Linear
+        self.mlp8 = None
         self.mlpblock = nn.Sequential(Linear(dim, hid), nn.GELU(), nn.Dropout(p), Linear(hid, dim), nn.Dropout(p))
 
     def forward(self, X, mask, mat=None):
@@ -123,6 +129,35 @@ class TransformerLayer(nn.Module):
         X, nn_ = next_norm.add_norm(X, self.feed_forward(n2))
         return X, nn_, attn
 
+    def quantize(self, on: bool = True):
+        """Keep the layer's linear weights in 8 bits beside those that train, as they are now (see ``Classifier.quantize``)."""
+        from .quant import E4M3Linear
+        self.mha.quantize(on)
+        self.mlp8 = tuple(E4M3Linear(self.mlpblock[i], self.mha.native_dtype) for i in (0, 3)) if on else None
+
+    def forward_quantized(self, X, branch, mask, mat):
+        """The layer with its linear layers on 8-bit operands.  branch: what the layer before adds to X (None: nothing); returns X and what
+        this one adds to it."""
+        n1 = norm_rows8(self.norm1, X, branch)
+        if branch is not None:
+            X, n1 = n1
+        out, _ = self.mha.forward_quantized(n1, mask, mat)
+        X, n2 = norm_rows8(self.norm2, X, out)
+        lin1, lin2 = self.mlp8
+        return X, lin2(self.mlpblock[1](lin1(n2)))
+
+
+def norm_rows8(norm, x, res=None):
+    """``norm(x)`` in 8 bits, with ``res`` ``(x + res, norm(x + res))``: one kernel where the norm is the root-mean-square norm's."""
+    from .quant import quantize_rows
+    from .rmsnorm import FusedRMSNorm, rms_norm_e4m3
+    if isinstance(norm, FusedRMSNorm):
+        return rms_norm_e4m3(x, norm.weight, norm.eps, res)
+    if res is None:
+        return quantize_rows(norm(x))
+    s = x + res
+    return s, quantize_rows(norm(s))
+
 
 class Encoder(nn.Module):
     def __init__(self, config):
@@ -131,12 +166,19 @@ class Encoder(nn.Module):
         self.layers = nn.ModuleList(TransformerLayer(config) for _ in range(config["num_layers"]))
         self.norm = make_norm(config, False)
         from .layernorm import FusedLayerNorm
-        self.add_norm = bool(config.get("fused_add_norm", True)) and isinstance(self.norm, FusedLayerNorm)
+        from .rmsnorm import FusedRMSNorm
+        self.add_norm = bool(config.get("fused_add_norm", True)) and isinstance(self.norm, (FusedLayerNorm, FusedRMSNorm))
+        self.quantized = False
 
     def forward(self, ids, mask, mat_lst=None, is_attn=False):
         from .pattern import mean_attention_map
         X = self.embeddings(ids)
         maps = []
+        if self.quantized and mat_lst is not None and not self.training and not torch.is_grad_enabled():
+            branch = None
+            for i, layer in enumerate(self.layers):
+                X, branch = layer.forward_quantized(X, branch, mask, mat_lst[0][i])
+            return mask_rows(self.norm(X + branch), mask), maps
         if self.add_norm and mat_lst is not None:
             # sparse phase: residual additions inside the normalisation kernels
             Xn = self.layers[0].norm1(X)
@@ -170,6 +212,23 @@ class Classifier(nn.Module):
         dim, hid = config["transformer_dim"], config["transformer_hidden_dim"]
         self.head = nn.Sequential(nn.Linear(dim * (4 if self.dual else 1), hid), nn.ReLU(),
                                   nn.Linear(hid, config["num_classes"]))
+
+    def quantize(self, on: bool = True):
+        """Evaluate the sparse phase (``eval()``, no gradients) with the encoder's linear layers on 8-bit operands: weights as they are now, kept until
+        ``quantize(False)``; activations from norms that write 8 bits, or quantised by the layer."""
+        for layer in self.model.layers:
+            layer.quantize(on)
+        self.model.quantized = on
+
+    def scores(self, ids, mat_lst):
+        """Class scores of single- or dual-tower inputs in the sparse phase, without a loss."""
+        with torch.autocast(device_type="cuda", dtype=torch.bfloat16, enabled=self.amp):
+            if not self.dual:
+                t, _ = self.model(ids, (ids != 0).float(), mat_lst, False)
+                return self.head(sequence_means(t, t.shape[0])[0]).float()
+            towers = [torch.cat([ids[0], ids[1]], 0)] if self.batch_towers else list(ids)      # as in the sparse steps
+            x0, x1 = (m for x in towers for m in sequence_means(self.model(x, (x != 0).float(), mat_lst, False)[0], ids[0].shape[0]))
+            return self.head(torch.cat([x0, x1, x0 * x1, x0 - x1], dim=-1)).float()
 
     def forward(self, ids, label, mat_lst=None, is_attn=False):
         with torch.autocast(device_type="cuda", dtype=torch.bfloat16, enabled=self.amp):
@@ -205,8 +264,15 @@ class Trainer:
         torch.manual_seed(seed)                      # identical initial weights on every rank
         self.model = Classifier(config).to(self.device)
         self.bucket = dp.FlatGradBucket(self.model.parameters())
-        self.opt = torch.optim.AdamW(self.bucket.pieces(), lr=lr, weight_decay=0.0, capturable=True, fused=True)
-        self.bucket.state_by_parameter(self.opt)
+        # config["optimizer"] = "fused": the library's AdamW (clipping and the copies of the parameters inside), its moments in
+        # config["optimizer_state_bits"] bits
+        self.fused_opt = config.get("optimizer", "torch") == "fused"
+        if self.fused_opt:
+            from .optim import AdamW
+            self.opt = AdamW(self.bucket.params, lr=lr, weight_decay=0.0, state_bits=config.get("optimizer_state_bits", 32), clip_value=1.0, seed=seed)
+        else:
+            self.opt = torch.optim.AdamW(self.bucket.pieces(), lr=lr, weight_decay=0.0, capturable=True, fused=True)
+            self.bucket.state_by_parameter(self.opt)
         self.mat_lst = None
         self.patterns = None
         self._graph = None
@@ -217,6 +283,8 @@ class Trainer:
             ps = [p for m in self.model.modules() if isinstance(m, BiasGradLinear) for p in (m.weight, m.bias)]
             if ps:
                 self._shadow = (ps, register_shadows(ps))
+                if self.fused_opt:
+                    self.opt.write_copies(*self._shadow)
         self.allreduce_events = None     # set to a list to collect (start, end) CUDA events around the gradient all-reduce
 
     def step(self, ids, label, is_attn=False):
@@ -230,13 +298,36 @@ class Trainer:
             self.allreduce_events.append((e0, e1))
         else:
             self.bucket.allreduce_mean()
-        self.bucket.flat.clamp_(-1.0, 1.0)                              # clip_grad_value_ (main_conv_ff.py:186), all gradients at once
-        self.opt.step()
-        self._refresh_shadows()
+        self._update()
         return loss.detach(), maps
 
+    def _update(self):
+        if not self.fused_opt:
+            self.bucket.flat.clamp_(-1.0, 1.0)                          # clip_grad_value_ (main_conv_ff.py:186), all gradients at once
+        self.opt.step()
+        self._refresh_shadows()
+
+    def evaluate(self, ids, label):
+        """Mean loss and share of right answers of one batch in the sparse phase, without gradients or dropout.  ``config["eval_linear_bits"] = 8``:
+        with the encoder's linear layers on 8-bit operands."""
+        if self.mat_lst is None:
+            raise RuntimeError("evaluate after discover()")
+        eight = self.config.get("eval_linear_bits") == 8
+        training = self.model.training
+        self.model.eval()
+        try:
+            with torch.no_grad():
+                if eight:
+                    self.model.quantize()
+                scores = self.model.scores(ids, self.mat_lst)
+                return nn.functional.cross_entropy(scores, label), (scores.argmax(-1) == label).float().mean()
+        finally:
+            if eight:
+                self.model.quantize(False)
+            self.model.train(training)
+
     def _refresh_shadows(self):
-        if self._shadow is not None:
+        if self._shadow is not None and not self.fused_opt:
             from .layernorm import refresh_shadows
             refresh_shadows(*self._shadow)
 
@@ -275,9 +366,7 @@ class Trainer:
             self._g_loss = loss.detach()
         self._graph_opt = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self._graph_opt, capture_error_mode="thread_local"):
-            self.bucket.flat.clamp_(-1.0, 1.0)
-            self.opt.step()
-            self._refresh_shadows()
+            self._update()
         return self._graph
 
     def step_graph(self, ids, label):

@@ -29,29 +29,23 @@ def rms_norm_e4m3(x, weight, eps: float = 1e-6, res=None):
 class FusedRMSNorm(nn.Module):
     """Drop-in for ``nn.RMSNorm(dim)`` beside ``FusedLayerNorm``, with its ``add_norm``.
 
-    ``bf16_out=True``: under ``torch.autocast`` to bf16 the output of an fp32 stream is bf16 (the dtype the next linear layer casts its input to anyway).
-    ``e4m3_out``: the output is ``Rows8`` for 8-bit linear layers, in calls without gradients (see ``harness.Classifier.quantize``)."""
+    ``bf16_out=True``: under ``torch.autocast`` to bf16 the output of an fp32 stream is bf16 (the dtype the next linear layer casts its input to anyway)."""
 
     def __init__(self, dim: int, eps: float = 1e-6, bf16_out: bool = False):
         super().__init__()
         self.weight = nn.Parameter(torch.ones(dim))
         self.eps = eps
         self.bf16_out = bf16_out
-        self.e4m3_out = False
 
     def _type(self, x):
         bf16 = self.bf16_out and x.dtype == torch.float32 and torch.is_autocast_enabled() and torch.get_autocast_dtype("cuda") == torch.bfloat16
         return torch.bfloat16 if bf16 else None
 
     def forward(self, x):
-        if self.e4m3_out and not torch.is_grad_enabled():
-            return rms_norm_e4m3(x, self.weight, self.eps)
         return rms_norm(x, self.weight, self.eps, out_dtype=self._type(x))
 
     def add_norm(self, x, res):
         """``s = x + res`` and ``self(s)`` in one pass; returns ``(s, self(s))``."""
         if res.dtype != x.dtype and x.dtype != torch.float32:
             res = res.to(x.dtype)
-        if self.e4m3_out and not torch.is_grad_enabled():
-            return rms_norm_e4m3(x, self.weight, self.eps, res)
         return rms_norm(x, self.weight, self.eps, res, self._type(x))

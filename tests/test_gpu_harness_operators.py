@@ -1,0 +1,97 @@
+"""The encoder's operators together, as a training run uses them: root-mean-square norms, the fused AdamW step with moments in 32 and 8 bits, captured steps,
+and evaluation with the linear layers on 8-bit operands."""
+import numpy as np
+import pytest
+import torch
+
+from spion_b200 import synthetic
+
+pytestmark = pytest.mark.gpu
+
+
+def trainer(task="image", dtype="fp32", L=256, batch=4, **overrides):
+    from spion_b200 import harness
+    cfg = harness.task_config(task, batch, native=True, dtype=dtype)
+    cfg.update(max_seq_len=L, dropout_prob=0.0, attention_dropout=0.0, threshold=0.85, norm="rms", optimizer="fused")
+    cfg.update(overrides)
+    tr = harness.Trainer(cfg, lr=1e-3, seed=3)
+    ids = synthetic.token_ids(5, batch, L).cuda()
+    ids = (ids, synthetic.token_ids(6, batch, L).cuda()) if cfg["dual"] else ids
+    return tr, ids, synthetic.labels(5, batch, cfg["num_classes"]).cuda()
+
+
+def start(tr, ids, lab):
+    _, maps = tr.step(ids, lab, is_attn=True)
+    tr.discover(maps)
+
+
+def test_first_step_is_the_frameworks():
+    """The same gradients through both optimizers: a first step moves every parameter by at most lr, the quotient is some tens of units in its last place off
+    (test_gpu_optim.py: 16 u), and the parameter itself 3 u."""
+    a, ids, lab = trainer()
+    b, _, _ = trainer(optimizer="torch")
+    assert all(torch.equal(x, y) for x, y in zip(a.model.parameters(), b.model.parameters()))
+    start(a, ids, lab), start(b, ids, lab)
+    assert torch.equal(a.bucket.flat.clamp(-1, 1), b.bucket.flat)         # the fused step clips as it reads
+    for x, y in zip(a.model.parameters(), b.model.parameters()):
+        assert bool(((x - y).abs() <= 1e-3 * 32 * 2.0 ** -24 + 4 * 2.0 ** -24 * x.abs()).all())
+
+
+@pytest.mark.parametrize("task,dtype,L,bits", [("image", "fp32", 256, 32), ("image", "fp32", 256, 8), ("text", "bf16", 512, 8), ("retrieval", "bf16", 512, 32)])
+def test_training_then_evaluation(task, dtype, L, bits):
+    tr, ids, lab = trainer(task, dtype, L, batch=2, optimizer_state_bits=bits, eval_linear_bits=8)
+    start(tr, ids, lab)
+    losses = [float(tr.step(ids, lab)[0]) for _ in range(3)]
+    assert np.isfinite(losses).all()
+    if tr._shadow is not None:                                             # written by the optimizer's own pass
+        for p, c in zip(*tr._shadow):
+            assert torch.equal(c, p.detach().to(c.dtype))
+    before = [p.detach().clone() for p in tr.model.parameters()]
+    loss8, right8 = tr.evaluate(ids, lab)
+    tr.config["eval_linear_bits"] = 16
+    loss, right = tr.evaluate(ids, lab)
+    assert tr.model.training and all(torch.equal(a, b) for a, b in zip(before, tr.model.parameters()))
+    # Operands within 2^-4 each, errors of independent signs: a sum over 64 features or more is off by less than 2^-4 of its size, and six of them lead
+    # to scores of order one here
+    assert bool(torch.isfinite(loss8)) and abs(float(loss8 - loss)) < 0.25
+    assert 0 <= float(right8) <= 1 and 0 <= float(right) <= 1
+    again, _ = tr.evaluate(ids, lab)
+    assert float(again) == float(loss)
+    assert np.isfinite(float(tr.step(ids, lab)[0]))
+
+
+def test_evaluation_in_8_bits_with_layer_norm_and_without_a_pattern():
+    tr, ids, lab = trainer(norm="layer", optimizer="torch", eval_linear_bits=8)
+    with pytest.raises(RuntimeError, match="discover"):
+        tr.evaluate(ids, lab)
+    start(tr, ids, lab)
+    loss8, _ = tr.evaluate(ids, lab)
+    assert bool(torch.isfinite(loss8))
+    # quantised layers are for calls without gradients: a training step passes them by
+    tr.model.quantize()
+    loss, _ = tr.step(ids, lab)
+    tr.model.quantize(False)
+    assert np.isfinite(float(loss))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_steps(bits):
+    """Three steps and a captured one replayed three times are the same six steps: the same losses up to the order of sums that atomics may change, which
+    Adam's sign-like first steps can turn into lr per parameter and step."""
+    a, ids, lab = trainer(optimizer_state_bits=bits)
+    b, _, _ = trainer(optimizer_state_bits=bits)
+    start(a, ids, lab), start(b, ids, lab)
+    b.capture_sparse_step(ids, lab, warmup=3)
+    for _ in range(3):
+        a.step(ids, lab)
+    for _ in range(3):
+        want, _ = a.step(ids, lab)
+        got = b.step_graph(ids, lab)
+        assert abs(float(got) - float(want)) <= 1e-3 * max(1.0, abs(float(want)))
+    steps = [float(s["step"]) for s in b.opt.state.values()]
+    assert set(steps) == {7.0}
+
+
+def test_unknown_norm_is_refused():
+    with pytest.raises(ValueError, match="norm"):
+        trainer(norm="batch")
