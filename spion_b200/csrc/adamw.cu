@@ -81,20 +81,10 @@ __device__ __forceinline__ float2 from_e5m2x2(unsigned word, unsigned select) { 
 }
 __device__ __forceinline__ float from_e4m3(unsigned c) { return from_e4m3x2(c).x; }
 __device__ __forceinline__ float from_e5m2(unsigned c) { return from_e5m2x2(c, 0x1404).x; }
-__device__ __forceinline__ float max_nan(float a, float b) {             // NaN if either is
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
 __device__ __forceinline__ float min_nan(float a, float b) {
   float d;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
-}
-__device__ __forceinline__ float lane_max_nan(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
 }
 // The update's quotient: a few units in its last place are lost beside a parameter that is many times as large.  v below fp32's normal numbers counts as
 // zero; beside an eps of 2^-40 or more its root is nothing (FLUSH; other steps take the exact forms).
@@ -134,8 +124,8 @@ __device__ __forceinline__ void update(const Step& s, const float4& f, float (&p
     if (BITS == 8) top_m = max_nan(top_m, fabsf(m[e])), top_v = max_nan(top_v, v[e]);
   }
   if (BITS == 32) return;
-  top_m = lane_max_nan(top_m);
-  top_v = lane_max_nan(top_v);
+  top_m = lane_max_nan<32>(top_m);
+  top_v = lane_max_nan<32>(top_v);
   unsigned wm[8], wv[8];                                                 // codes in the top bytes
   if (top_m < 0x1p14f && top_v < 0x1p28f) {                              // all finite, and scale and fit are one factor within fp32's range
     sm = scale_of(top_m, 7), sv = scale_of(top_v, 14);

@@ -66,18 +66,18 @@ template <int VEC, int NV, int TPR> __device__ __forceinline__ void load_weights
   }
 }
 
-// e4m3: what y is multiplied with, and the row's scale.  A row with a NaN has the scale NaN (`sum` is NaN then), one with an infinity an infinite
-// scale and zeros beside NaN: no value of such a row comes back finite.
-__device__ __forceinline__ float row_scale(float top, float sum, float& scale) {
-  float a = top < SMALL ? SMALL : top;
-  if (sum != sum) a = sum;
-  scale = a / 448.f;
+// e4m3: what y is multiplied with, and the row's scale.  A row with a NaN has the scale NaN, one with an infinity an infinite scale and zeros beside
+// NaN: no value of such a row comes back finite.
+__device__ __forceinline__ float row_scale(float top, float& scale) {
+  const float a = top < SMALL ? SMALL : top;             // (NaN stays)
+  scale = a * (1.f / 448.f);
   return 448.f * __frcp_rn(a);
 }
 
 // TPR threads to a row: 8 or 32 lanes of a warp, more: a CTA of that many.  Lanes take UR rows at a time, so that enough bytes are in flight.
-template <class S, class R, class Y, int VEC, int NV, int TPR, int UR>
-__global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR, VEC == 8 && TPR == 8 && NV * UR <= 2 ? 4 : 1) k_rms_forward(const FwdArgs a) {
+// NORM false: rows to e4m3 as they are (131072 x 64 bf16: QNORM us with the sums and products of the norm left in, QPLAIN without).
+template <bool NORM, class S, class R, class Y, int VEC, int NV, int TPR, int UR>
+__global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR, VEC == 8 && TPR == 8 && NV <= 2 ? 4 : 1) k_rms_forward(const FwdArgs a) {
   constexpr bool Q = type_code<Y>() == SPION_E4M3;
   constexpr int THREADS = TPR <= 32 ? CTA : TPR, RPC = THREADS / TPR, RPW = TPR <= 32 ? 32 / TPR : 1;      // rows of a CTA and of a warp
   __shared__ float2 part[2][32];
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR, VEC == 8 && TPR == 8 &&
   Y* const y = static_cast<Y*>(a.y) + t * VEC;
   const int left = a.N - t * VEC;                        // piece i of the thread is in the row if i * TPR * VEC < left
   float w[NV * VEC];
-  load_weights<VEC, NV, TPR>(a.w, a.w_type, a.N, t, w);
+  if (NORM) load_weights<VEC, NV, TPR>(a.w, a.w_type, a.N, t, w);
   int buf = 0;
   const float over_n = 1.0f / a.N;
   // `first` is the same for all lanes of a warp: they leave the loop together
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR, VEC == 8 && TPR == 8 &&
         if (i * TPR * VEC < here) px[u][i].load(x + row * a.ldx + i * TPR * VEC);
         else px[u][i].zero();
     }
-    if (a.r != nullptr) {
+    if (NORM && a.r != nullptr) {
       Piece<R, VEC> pr[UR][NV];
 #pragma unroll
       for (int u = 0; u < UR; ++u) {
@@ -141,19 +141,27 @@ __global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR, VEC == 8 && TPR == 8 &&
     for (int u = 0; u < UR; ++u) {
       const long long row = first + u * RPW + sub;
       const int here = row < a.M ? left : 0;
-      float sum = 0.f, top = 0.f;
+      float sum = 0.f, top = 0.f, rho = 1.f, f = 1.f;
 #pragma unroll
       for (int i = 0; i < NV * VEC; ++i) {
-        sum = fmaf(v[u][i], v[u][i], sum);
-        v[u][i] *= w[i];
-        if (Q) top = fmaxf(top, fabsf(v[u][i]));
+        if (NORM) {
+          sum = fmaf(v[u][i], v[u][i], sum);
+          v[u][i] *= w[i];
+          if (Q) top = fmaxf(top, fabsf(v[u][i]));
+        } else {
+          top = max_nan(top, fabsf(v[u][i]));
+        }
       }
-      row_reduce<TPR, Q>(sum, top, part, buf);
-      const float rho = a.norm ? rsqrtf(fmaf(sum, over_n, a.eps)) : 1.f;
-      float f = 1.f;
+      if (NORM) {
+        row_reduce<TPR, Q>(sum, top, part, buf);
+        rho = rsqrtf(fmaf(sum, over_n, a.eps));
+        top *= rho;                                      // NaN where the sum is
+      } else {
+        row_max_nan<TPR>(top, part, buf);
+      }
       if (Q) {
         float scale;
-        f = row_scale(top * rho, a.norm ? top * rho : sum, scale);
+        f = row_scale(top, scale);
         if (t == 0 && row < a.M) a.scale[row] = scale;
       }
       if (t == 0 && row < a.M && a.rho != nullptr) a.rho[row] = rho;
@@ -161,7 +169,7 @@ __global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR, VEC == 8 && TPR == 8 &&
       for (int i = 0; i < NV; ++i) {
         float o[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) o[e] = Q ? v[u][i * VEC + e] * rho * f : v[u][i * VEC + e] * rho;
+        for (int e = 0; e < VEC; ++e) o[e] = !NORM ? v[u][i * VEC + e] * f : Q ? v[u][i * VEC + e] * rho * f : v[u][i * VEC + e] * rho;
         if (i * TPR * VEC < here) Out<Y, VEC>::store(y + row * a.ldy + i * TPR * VEC, o);
       }
     }
@@ -200,15 +208,19 @@ __global__ void __launch_bounds__(512) k_rms_forward_wide(const FwdArgs a) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         sum = fmaf(v[e], v[e], sum);
-        if (Q) top = fmaxf(top, fabsf(v[e] * (a.w == nullptr ? 1.f : load_any(a.w, a.w_type, c + e))));
+        if (Q) top = max_nan(top, fabsf(v[e] * (a.w == nullptr ? 1.f : load_any(a.w, a.w_type, c + e))));
       }
     }
-    row_reduce<512, Q>(sum, top, part, buf);
-    const float rho = a.norm ? rsqrtf(fmaf(sum, 1.0f / a.N, a.eps)) : 1.f;
-    float f = 1.f;
+    float rho = 1.f, f = 1.f;
+    if (a.norm) {
+      row_reduce<512, Q>(sum, top, part, buf);
+      rho = rsqrtf(fmaf(sum, 1.0f / a.N, a.eps));
+    } else {
+      row_max_nan<512>(top, part, buf);
+    }
     if (Q) {
       float scale;
-      f = row_scale(top * rho, a.norm ? top * rho : sum, scale);
+      f = row_scale(top * rho, scale);
       if (threadIdx.x == 0) a.scale[row] = scale;
     }
     if (threadIdx.x == 0 && a.rho != nullptr) a.rho[row] = rho;
@@ -264,7 +276,7 @@ __device__ __forceinline__ void row_backward(const BwdArgs& a, long long row, in
 
 // Rows through registers.  The groups of lanes of a CTA leave their sums of a column side by side in shared memory, where they are added in order.
 template <class S, class D, int VEC, int NV, int TPR, int UR>
-__global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR) k_rms_backward(const BwdArgs a) {
+__global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR, TPR <= 32 ? 2 : 512 / TPR) k_rms_backward(const BwdArgs a) {
   next_may_start();                                                        // k_rms_dw
   constexpr int THREADS = TPR <= 32 ? CTA : TPR, RPC = THREADS / TPR, RPW = TPR <= 32 ? 32 / TPR : 1;
   constexpr int WIDTH = TPR * NV * VEC, AT_ONCE = RPC < 8 ? RPC : 8;       // groups of lanes whose sums are in shared memory together
@@ -394,26 +406,26 @@ __global__ void __launch_bounds__(TPR) k_rms_backward_ring(const BwdArgs a, cons
     const float next = row + step < a.M ? a.rho[row + step] : 0.f;
     if (!tc::mbar_wait(bars + 8 * st, ph)) s_lost = 1;                     // (bounded; the copies of this CTA end by themselves)
     const uint8_t* const at = smem + RING_BARS + st * ring.stage;
-    Piece<S, 8> ps[NV], pk[NV];
-    Piece<D, 8> pd[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
+    auto piece = [&](int i, Piece<S, 8>& s, Piece<D, 8>& d, Piece<S, 8>& k) {
       const int c = (t + i * TPR) * 8;
-      if (i * TPR * 8 < left) {
-        ps[i].load_shared(reinterpret_cast<const S*>(at) + c);
-        pd[i].load_shared(reinterpret_cast<const D*>(at + ring.at_dy) + c);
-      } else {
-        ps[i].zero(), pd[i].zero();
-      }
-      if (a.ds != nullptr && i * TPR * 8 < left) pk[i].load_shared(reinterpret_cast<const S*>(at + ring.at_ds) + c);
-      else pk[i].zero();
-    }
+      s.zero(), d.zero(), k.zero();
+      if (i * TPR * 8 >= left) return;
+      s.load_shared(reinterpret_cast<const S*>(at) + c);
+      d.load_shared(reinterpret_cast<const D*>(at + ring.at_dy) + c);
+      if (a.ds != nullptr) k.load_shared(reinterpret_cast<const S*>(at + ring.at_ds) + c);
+    };
+    Piece<S, 8> ps[1], pk[1];
+    Piece<D, 8> pd[1];
     float sum = 0.f, none = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV * 8; ++i) {
-      const float d = pd[i / 8].at(i % 8) * (ps[i / 8].at(i % 8) * rho);
-      acc[i] += d;
-      sum = fmaf(d, w[i], sum);
+    for (int i = 0; i < NV; ++i) {
+      piece(i, ps[0], pd[0], pk[0]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = pd[0].at(e) * (ps[0].at(e) * rho);
+        acc[i * 8 + e] += d;
+        sum = fmaf(d, w[i * 8 + e], sum);
+      }
     }
     row_reduce<TPR, false>(sum, none, part, buf);
     if (s_lost) {                                                          // (every thread that set it did so before the barrier)
@@ -424,8 +436,25 @@ __global__ void __launch_bounds__(TPR) k_rms_backward_ring(const BwdArgs a, cons
       }
       return;
     }
-    if (t == 0 && row + ring.stages * step < a.M) fill(st, row + ring.stages * step);
-    row_backward<S, D, 8, NV, TPR>(a, row, left, ps, pd, pk, rho, sum * over_n, w, t);
+    const bool more = t == 0 && row + ring.stages * step < a.M;
+    if (NV == 1) {                                                         // the thread's piece is in registers
+      if (more) fill(st, row + ring.stages * step);
+      float w1[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w1[e] = w[e];
+      row_backward<S, D, 8, 1, TPR>(a, row, left, ps, pd, pk, rho, sum * over_n, w1, t);
+    } else {                                                               // several: read again, and the place is free a barrier later
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        piece(i, ps[0], pd[0], pk[0]);
+        float w1[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w1[e] = w[i * 8 + e];
+        row_backward<S, D, 8, 1, TPR>(a, row, left - i * TPR * 8, ps, pd, pk, rho, sum * over_n, w1, t + i * TPR);
+      }
+      __syncthreads();
+      if (more) fill(st, row + ring.stages * step);
+    }
     rho = next;
     if (++st == ring.stages) st = 0, ph ^= 1;
   }
@@ -501,17 +530,14 @@ __global__ void __launch_bounds__(1024) k_rms_dw(const float* part, int count, i
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float s = 0.f;
   wait_for_kernel_before();
-  if (c < N) {
-    int r = warp;
-    for (; r + 7 * 32 < count; r += 8 * 32) {                              // eight loads at a time, added one after another
+  if (c < N)
+    for (int r = warp; r < count; r += 8 * 32) {                           // eight loads at a time, added one after another
       float v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = part[(long long)(r + 32 * k) * N + c];
+      for (int k = 0; k < 8; ++k) v[k] = r + 32 * k < count ? part[(long long)(r + 32 * k) * N + c] : 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) s += v[k];
     }
-    for (; r < count; r += 32) s += part[(long long)r * N + c];
-  }
   sums[warp][lane] = s;
   __syncthreads();
   if (warp == 0 && c < N) {
@@ -532,37 +558,37 @@ int grid_of(long long M, int rows_per_cta, int threads) {
   return (int)(need < most ? need : most);
 }
 
-template <class S, class R, class Y, int VEC, int NV, int TPR, int UR = 1> void launch_forward(const FwdArgs& a, cudaStream_t st) {
+template <bool NORM, class S, class R, class Y, int VEC, int NV, int TPR, int UR = 1> void launch_forward(const FwdArgs& a, cudaStream_t st) {
   constexpr int THREADS = TPR <= 32 ? CTA : TPR;
-  k_rms_forward<S, R, Y, VEC, NV, TPR, UR><<<grid_of(a.M, THREADS / TPR * UR, THREADS), THREADS, 0, st>>>(a);
+  k_rms_forward<NORM, S, R, Y, VEC, NV, TPR, UR><<<grid_of(a.M, THREADS / TPR * UR, THREADS), THREADS, 0, st>>>(a);
 }
-template <class S, class R, class Y>
+template <class S, class R, class Y, bool NORM = true>
 int forward(const FwdArgs& a, cudaStream_t st) {
   const bool vec = a.N % 8 == 0 && on_boundary(a.x, a.ldx, type_code<S>()) && on_boundary(a.r, a.ldr, type_code<R>()) &&
                    on_boundary(a.s, a.N, type_code<S>()) && on_boundary(a.y, a.ldy, type_code<Y>()) && on_boundary(a.w, a.N, a.w_type);
   const bool few = a.M <= sm_count();                    // as many threads as pieces
   if (vec) {
     const int n = a.N / 8;
-    if (n <= 8) launch_forward<S, R, Y, 8, 1, 8, 2>(a, st);
-    else if (n <= 16) launch_forward<S, R, Y, 8, 2, 8>(a, st);
-    else if (n <= 32) launch_forward<S, R, Y, 8, 4, 8>(a, st);
-    else if (n <= 64) launch_forward<S, R, Y, 8, 2, 32>(a, st);
-    else if (n <= 128) launch_forward<S, R, Y, 8, 4, 32>(a, st);
-    else if (few && n <= 256) launch_forward<S, R, Y, 8, 1, 256>(a, st);
-    else if (few && n <= 512) launch_forward<S, R, Y, 8, 1, 512>(a, st);
-    else if (few && n <= 1024) launch_forward<S, R, Y, 8, 1, 1024>(a, st);
-    else if (n <= 256) launch_forward<S, R, Y, 8, 4, 64>(a, st);
-    else if (n <= 512) launch_forward<S, R, Y, 8, 4, 128>(a, st);
-    else if (n <= 1024) launch_forward<S, R, Y, 8, 4, 256>(a, st);
-    else if (n <= 2048) launch_forward<S, R, Y, 8, 4, 512>(a, st);
+    if (n <= 8) launch_forward<NORM, S, R, Y, 8, 1, 8, 2>(a, st);
+    else if (n <= 16) launch_forward<NORM, S, R, Y, 8, 2, 8>(a, st);
+    else if (n <= 32) launch_forward<NORM, S, R, Y, 8, 4, 8>(a, st);
+    else if (n <= 64) launch_forward<NORM, S, R, Y, 8, 2, 32>(a, st);
+    else if (n <= 128) launch_forward<NORM, S, R, Y, 8, 4, 32>(a, st);
+    else if (few && n <= 256) launch_forward<NORM, S, R, Y, 8, 1, 256>(a, st);
+    else if (few && n <= 512) launch_forward<NORM, S, R, Y, 8, 1, 512>(a, st);
+    else if (few && n <= 1024) launch_forward<NORM, S, R, Y, 8, 1, 1024>(a, st);
+    else if (n <= 256) launch_forward<NORM, S, R, Y, 8, 4, 64>(a, st);
+    else if (n <= 512) launch_forward<NORM, S, R, Y, 8, 4, 128>(a, st);
+    else if (n <= 1024) launch_forward<NORM, S, R, Y, 8, 4, 256>(a, st);
+    else if (n <= 2048) launch_forward<NORM, S, R, Y, 8, 4, 512>(a, st);
     else k_rms_forward_wide<S, R, Y, 8><<<grid_of(a.M, 1, 512), 512, 0, st>>>(a);
   } else {
-    if (a.N <= 128) launch_forward<S, R, Y, 1, 4, 32, 2>(a, st);
-    else if (a.N <= 512) launch_forward<S, R, Y, 1, 16, 32>(a, st);
-    else if (a.N <= 1024) launch_forward<S, R, Y, 1, 16, 64>(a, st);
-    else if (a.N <= 2048) launch_forward<S, R, Y, 1, 16, 128>(a, st);
-    else if (a.N <= 4096) launch_forward<S, R, Y, 1, 16, 256>(a, st);
-    else if (a.N <= 8192) launch_forward<S, R, Y, 1, 16, 512>(a, st);
+    if (a.N <= 128) launch_forward<NORM, S, R, Y, 1, 4, 32, 2>(a, st);
+    else if (a.N <= 512) launch_forward<NORM, S, R, Y, 1, 16, 32>(a, st);
+    else if (a.N <= 1024) launch_forward<NORM, S, R, Y, 1, 16, 64>(a, st);
+    else if (a.N <= 2048) launch_forward<NORM, S, R, Y, 1, 16, 128>(a, st);
+    else if (a.N <= 4096) launch_forward<NORM, S, R, Y, 1, 16, 256>(a, st);
+    else if (a.N <= 8192) launch_forward<NORM, S, R, Y, 1, 16, 512>(a, st);
     else k_rms_forward_wide<S, R, Y, 1><<<grid_of(a.M, 1, 512), 512, 0, st>>>(a);
   }
   SPION_LAUNCH_CHECK();
@@ -619,16 +645,16 @@ int backward(const BwdArgs& a, void* dw, int dw_type, cudaStream_t st) {
   int parts = 0;
   if (vec) {
     const int n = a.N / 8;
-    if (n <= 8) parts = launch_backward<S, D, 8, 1, 8, 2>(a, 4, st);
-    else if (n <= 16) parts = launch_backward<S, D, 8, 2, 8>(a, 3, st);
-    else if (n <= 64) parts = launch_backward<S, D, 8, 2, 32>(a, 3, st);
+    if (n <= 8) parts = launch_backward<S, D, 8, 1, 8, 2>(a, 2, st);
+    else if (n <= 16) parts = launch_backward<S, D, 8, 2, 8>(a, 2, st);
+    else if (n <= 64) parts = launch_backward<S, D, 8, 2, 32>(a, 2, st);
     else if (n <= 128) parts = launch_ring<S, D, 1, 128>(a, 4, st);
     else if (n <= 256) parts = launch_ring<S, D, 1, 256>(a, 4, st);
     else if (n <= 512) parts = launch_ring<S, D, 1, 512>(a, 2, st);
     else if (n <= 1024) parts = launch_ring<S, D, 1, 1024>(a, 1, st);
     else if (n <= 2048) parts = launch_ring<S, D, 2, 1024>(a, 1, st);
   } else {
-    if (a.N <= 128) parts = launch_backward<S, D, 1, 4, 32, 2>(a, 4, st);
+    if (a.N <= 128) parts = launch_backward<S, D, 1, 4, 32, 2>(a, 2, st);
     else if (a.N <= 512) parts = launch_backward<S, D, 1, 16, 32>(a, 2, st);
     else if (a.N <= 1024) parts = launch_backward<S, D, 1, 16, 64>(a, 8, st);
     else if (a.N <= 2048) parts = launch_backward<S, D, 1, 16, 128>(a, 4, st);
@@ -681,8 +707,13 @@ int spion_rmsnorm_forward(const void* x, long long ldx, int x_type, const void* 
   if (ldx < 0 || ldy < N || (res != nullptr && ldr < 0)) return SPION_ERR_ARG;
   if (!norm && (y_type != SPION_E4M3 || w != nullptr || res != nullptr)) return SPION_ERR_ARG;
   if (res == nullptr) res_type = x_type;
-  const FwdArgs a = {x, ldx, res, ldr, w, w_type, sum_out, y, ldy, scale, rstd, M, N, eps, norm};
   const cudaStream_t st = (cudaStream_t)cuda_stream;
+  const FwdArgs a = {x, ldx, res, ldr, w, w_type, sum_out, y, ldy, scale, rstd, M, N, eps, norm};
+  if (!norm) {
+    if (x_type == SPION_F32) return forward<float, float, __nv_fp8_e4m3, false>(a, st);
+    if (x_type == SPION_BF16) return forward<__nv_bfloat16, __nv_bfloat16, __nv_fp8_e4m3, false>(a, st);
+    return forward<__half, __half, __nv_fp8_e4m3, false>(a, st);
+  }
   if (x_type == SPION_F32) {
     if (res_type == SPION_F32) return forward_out<float, float>(a, y_type, st);
     if (res_type == SPION_BF16) return forward_out<float, __nv_bfloat16>(a, y_type, st);

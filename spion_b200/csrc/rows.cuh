@@ -155,4 +155,24 @@ template <int TPR, bool MAX> __device__ __forceinline__ void row_reduce(float& s
   buf ^= 1;
 }
 
+// the largest, NaN if one is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+template <int LANES> __device__ __forceinline__ float lane_max_nan(float v) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+template <int TPR> __device__ __forceinline__ void row_max_nan(float& top, float2 (*part)[32], int& buf) {
+  top = lane_max_nan<(TPR < 32 ? TPR : 32)>(top);
+  if (TPR <= 32) return;
+  if ((threadIdx.x & 31) == 0) part[buf][threadIdx.x >> 5].y = top;
+  __syncthreads();
+  top = lane_max_nan<32>((int)(threadIdx.x & 31) < TPR / 32 ? part[buf][threadIdx.x & 31].y : 0.f);
+  buf ^= 1;
+}
+
 }  // namespace rows
