@@ -15,9 +15,11 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "rows.cuh"
+#include "tc_ptx.cuh"
 
 using namespace rows;
 
@@ -155,22 +157,107 @@ __device__ __forceinline__ void update(const Step& s, const float4& f, float (&p
   cv = make_uint2(top_bytes(wv[0], wv[1], wv[2], wv[3]), top_bytes(wv[4], wv[5], wv[6], wv[7]));
 }
 
+// A whole block on its boundaries: a lane has values 8 lane .. 8 lane + 7.
+template <class P, int BITS, bool FLUSH>
+__device__ __forceinline__ void whole_block(const Step& s, const Tensor& t, const Lane<P, BITS>& now, long long base, int lane, const float4& f, unsigned key) {
+  const long long k = base + 8 * lane, at = t.at + k;
+  float p[8], g[8], m[8], v[8], sm = now.sm, sv = now.sv;
+  uint2 cm, cv;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) p[e] = now.p.at(e), g[e] = now.g.at(e);
+  if constexpr (BITS == 32) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m[e] = now.m.at(e), v[e] = now.v.at(e);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const unsigned x = e < 4 ? now.m.x : now.m.y, y = e < 4 ? now.v.x : now.v.y;
+      const float2 fm = from_e4m3x2(e & 2 ? x >> 16 : x & 0xffffu), fv = from_e5m2x2(y, e & 2 ? 0x3424 : 0x1404);
+      m[e] = fm.x, m[e + 1] = fm.y, v[e] = fv.x, v[e + 1] = fv.y;
+    }
+  }
+  update<BITS, FLUSH>(s, f, p, g, m, v, sm, sv, cm, cv, (unsigned)k, 1, key);
+  Out<P, 8>::store(static_cast<P*>(t.p) + k, p);
+  if constexpr (BITS == 32) {
+    Out<float, 8>::store(static_cast<float*>(s.m) + at, m);
+    Out<float, 8>::store(static_cast<float*>(s.v) + at, v);
+  } else {
+    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(s.m) + at) = cm;
+    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(s.v) + at) = cv;
+    if (lane == 0) s.m_scale[at / BLOCK] = sm, s.v_scale[at / BLOCK] = sv;
+  }
+  if (t.copy != nullptr) {
+    if (s.copy_type == SPION_BF16) Out<__nv_bfloat16, 8>::store(static_cast<__nv_bfloat16*>(t.copy) + k, p);
+    else Out<__half, 8>::store(static_cast<__half*>(t.copy) + k, p);
+  }
+}
+// A tensor's last block, and tensors that lie off the boundaries: a lane has values lane, lane + 32, ...  `begun` waits for the factors.
+template <class P, int BITS, bool FLUSH, class F>
+__device__ __forceinline__ void edge_block(const Step& s, const Tensor& t, long long base, long long end, int lane, float4& f, unsigned& key, F begun) {
+  const int left = (int)min(end - base, (long long)BLOCK);
+  const long long at = t.at + base;
+  P* const tp = static_cast<P*>(t.p) + base;
+  const P* const tg = static_cast<const P*>(t.g) + base;
+  float p[8], g[8], m[8], v[8], sm = 0.f, sv = 0.f;
+  uint2 cm, cv;
+  if (BITS == 8) sm = s.m_scale[at / BLOCK], sv = s.v_scale[at / BLOCK];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int k = lane + 32 * e;
+    const bool in = k < left;
+    p[e] = in ? as_float(tp[k]) : 0.f;
+    g[e] = in ? as_float(tg[k]) : 0.f;
+    if (BITS == 32) {
+      m[e] = in ? static_cast<const float*>(s.m)[at + k] : 0.f;
+      v[e] = in ? static_cast<const float*>(s.v)[at + k] : 0.f;
+    } else {
+      m[e] = in ? from_e4m3(static_cast<const uint8_t*>(s.m)[at + k]) : 0.f;
+      v[e] = in ? from_e5m2(static_cast<const uint8_t*>(s.v)[at + k]) : 0.f;
+    }
+  }
+  begun();
+  update<BITS, FLUSH>(s, f, p, g, m, v, sm, sv, cm, cv, (unsigned)(base + lane), 32, key);
+  if (BITS == 8 && lane == 0) s.m_scale[at / BLOCK] = sm, s.v_scale[at / BLOCK] = sv;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int k = lane + 32 * e;
+    if (k >= left) continue;
+    tp[k] = rounded<P>(p[e]);
+    if (BITS == 32) {
+      static_cast<float*>(s.m)[at + k] = m[e];
+      static_cast<float*>(s.v)[at + k] = v[e];
+    } else {
+      static_cast<uint8_t*>(s.m)[at + k] = (uint8_t)((e < 4 ? cm.x : cm.y) >> (8 * (e & 3)));
+      static_cast<uint8_t*>(s.v)[at + k] = (uint8_t)((e < 4 ? cv.x : cv.y) >> (8 * (e & 3)));
+    }
+    if (t.copy != nullptr) store_any(t.copy, s.copy_type, base + k, p[e]);
+  }
+}
+// the last tensor that begins at or before a chunk, from an earlier one
+template <int MAX> __device__ __forceinline__ int tensor_of(const Table<MAX>& a, int chunk, int i) {
+  if (i + 1 < a.s.count && a.chunk[i + 1] <= chunk) {
+    int hi = a.s.count;
+    while (hi - i > 1) {
+      const int mid = (i + hi) >> 1;
+      if (a.chunk[mid] <= chunk) i = mid;
+      else hi = mid;
+    }
+  }
+  return i;
+}
+template <class P> __device__ __forceinline__ bool on_boundaries(const Tensor& t) {
+  return (((uintptr_t)t.p | (uintptr_t)t.g) & (8 * sizeof(P) - 1)) == 0 && ((uintptr_t)t.copy & 15) == 0;
+}
+
 template <int BITS> constexpr int CTAS = BITS == 32 ? 4 : 4;              // resident on a multiprocessor
 template <class P, int BITS, bool FLUSH, int MAX>
 __global__ void __launch_bounds__(CTA, CTAS<BITS>) k_adamw(const __grid_constant__ Table<MAX> a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int i = 0;
   for (int chunk = blockIdx.x; chunk < a.s.chunks; chunk += gridDim.x) {
-    if (i + 1 < a.s.count && a.chunk[i + 1] <= chunk) {
-      int hi = a.s.count;                                                // the last tensor that begins at or before the chunk
-      while (hi - i > 1) {
-        const int mid = (i + hi) >> 1;
-        if (a.chunk[mid] <= chunk) i = mid;
-        else hi = mid;
-      }
-    }
+    i = tensor_of(a, chunk, i);
     const Tensor& t = a.t[i];
-    const bool boundary = (((uintptr_t)t.p | (uintptr_t)t.g) & (8 * sizeof(P) - 1)) == 0 && ((uintptr_t)t.copy & 15) == 0;
+    const bool boundary = on_boundaries<P>(t);
     const long long begin = (long long)(chunk - a.chunk[i]) * a.s.span, end = min(t.n, begin + a.s.span);
     float4 f;
     unsigned key;
@@ -183,7 +270,6 @@ __global__ void __launch_bounds__(CTA, CTAS<BITS>) k_adamw(const __grid_constant
     };
     bool first = true;
     long long base = begin + warp * BLOCK;
-    // whole blocks on a boundary: a lane has values 8 lane .. 8 lane + 7
     for (; boundary && base + BLOCK <= end; base += CTA / 32 * BLOCK) {
       const long long k = base + 8 * lane, at = t.at + k;
       Lane<P, BITS> now;
@@ -200,78 +286,98 @@ __global__ void __launch_bounds__(CTA, CTAS<BITS>) k_adamw(const __grid_constant
       }
       if (first) begun();
       first = false;
-      float p[8], g[8], m[8], v[8], sm = now.sm, sv = now.sv;
-      uint2 cm, cv;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) p[e] = now.p.at(e), g[e] = now.g.at(e);
-      if constexpr (BITS == 32) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m[e] = now.m.at(e), v[e] = now.v.at(e);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const unsigned x = e < 4 ? now.m.x : now.m.y, y = e < 4 ? now.v.x : now.v.y;
-          const float2 fm = from_e4m3x2(e & 2 ? x >> 16 : x & 0xffffu), fv = from_e5m2x2(y, e & 2 ? 0x3424 : 0x1404);
-          m[e] = fm.x, m[e + 1] = fm.y, v[e] = fv.x, v[e + 1] = fv.y;
-        }
-      }
-      update<BITS, FLUSH>(a.s, f, p, g, m, v, sm, sv, cm, cv, (unsigned)k, 1, key);
-      Out<P, 8>::store(static_cast<P*>(t.p) + k, p);
-      if constexpr (BITS == 32) {
-        Out<float, 8>::store(static_cast<float*>(a.s.m) + at, m);
-        Out<float, 8>::store(static_cast<float*>(a.s.v) + at, v);
-      } else {
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.s.m) + at) = cm;
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.s.v) + at) = cv;
-        if (lane == 0) a.s.m_scale[at / BLOCK] = sm, a.s.v_scale[at / BLOCK] = sv;
-      }
-      if (t.copy != nullptr) {
-        if (a.s.copy_type == SPION_BF16) Out<__nv_bfloat16, 8>::store(static_cast<__nv_bfloat16*>(t.copy) + k, p);
-        else Out<__half, 8>::store(static_cast<__half*>(t.copy) + k, p);
-      }
+      whole_block<P, BITS, FLUSH>(a.s, t, now, base, lane, f, key);
     }
-    // a tensor's last block, and tensors that lie off the boundaries: a lane has values lane, lane + 32, ...
     for (; base < end; base += CTA / 32 * BLOCK) {
-      const int left = (int)min(end - base, (long long)BLOCK);
-      const long long at = t.at + base;
-      P* const tp = static_cast<P*>(t.p) + base;
-      const P* const tg = static_cast<const P*>(t.g) + base;
-      float p[8], g[8], m[8], v[8], sm = 0.f, sv = 0.f;
-      uint2 cm, cv;
-      if (BITS == 8) sm = a.s.m_scale[at / BLOCK], sv = a.s.v_scale[at / BLOCK];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int k = lane + 32 * e;
-        const bool in = k < left;
-        p[e] = in ? as_float(tp[k]) : 0.f;
-        g[e] = in ? as_float(tg[k]) : 0.f;
-        if (BITS == 32) {
-          m[e] = in ? static_cast<const float*>(a.s.m)[at + k] : 0.f;
-          v[e] = in ? static_cast<const float*>(a.s.v)[at + k] : 0.f;
-        } else {
-          m[e] = in ? from_e4m3(static_cast<const uint8_t*>(a.s.m)[at + k]) : 0.f;
-          v[e] = in ? from_e5m2(static_cast<const uint8_t*>(a.s.v)[at + k]) : 0.f;
-        }
-      }
-      if (first) begun();
-      first = false;
-      update<BITS, FLUSH>(a.s, f, p, g, m, v, sm, sv, cm, cv, (unsigned)(base + lane), 32, key);
-      if (BITS == 8 && lane == 0) a.s.m_scale[at / BLOCK] = sm, a.s.v_scale[at / BLOCK] = sv;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int k = lane + 32 * e;
-        if (k >= left) continue;
-        tp[k] = rounded<P>(p[e]);
-        if (BITS == 32) {
-          static_cast<float*>(a.s.m)[at + k] = m[e];
-          static_cast<float*>(a.s.v)[at + k] = v[e];
-        } else {
-          static_cast<uint8_t*>(a.s.m)[at + k] = (uint8_t)((e < 4 ? cm.x : cm.y) >> (8 * (e & 3)));
-          static_cast<uint8_t*>(a.s.v)[at + k] = (uint8_t)((e < 4 ? cv.x : cv.y) >> (8 * (e & 3)));
-        }
-        if (t.copy != nullptr) store_any(t.copy, a.s.copy_type, base + k, p[e]);
-      }
+      edge_block<P, BITS, FLUSH>(a.s, t, base, end, lane, f, key, [&] {
+        if (first) begun();
+        first = false;
+      });
     }
+  }
+}
+
+// The same for many values with 8-bit moments, where a block's arithmetic takes as long as its way from memory: a warp of its own keeps three chunks of 2048
+// values under way to shared memory by bulk copies while eight warps work.  75 million fp32 values: RINGOFF us without, RINGON with it.
+constexpr int RING_STAGES = 3, RING_CTAS = 3, RING_CHUNK = CTA / 32 * BLOCK;
+template <class P> struct RingOf {
+  static constexpr uint32_t VALUES = RING_CHUNK * sizeof(P), STAGE = 2 * VALUES + 2 * RING_CHUNK, SMEM = RING_STAGES * STAGE + 64;
+};
+static_assert(RING_CTAS * (RingOf<float>::SMEM + 1024) <= 233472, "shared memory of a multiprocessor");
+// Set by a bounded wait that gave up; launches after it leave at once until spion_linear_status has reported it.
+__device__ int g_adamw_status;
+
+template <class P, bool FLUSH, int MAX>
+__global__ void __launch_bounds__(CTA + 32, RING_CTAS) k_adamw_ring(const __grid_constant__ Table<MAX> a) {
+  using R = RingOf<P>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint32_t rows0 = tc::smem_u32(smem), full = rows0 + RING_STAGES * R::STAGE, empty = full + 8 * RING_STAGES;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < RING_STAGES; ++i) tc::mbar_init(full + 8 * i, 1), tc::mbar_init(empty + 8 * i, CTA / 32);
+    tc::fence_barrier_init();
+    tc::fence_proxy_async();
+  }
+  if (__syncthreads_or(*reinterpret_cast<volatile int*>(&g_adamw_status))) return;
+  int i = 0, st = 0, ph = 0;
+  // a chunk goes through the ring if all of it is there and lies on the boundaries: both sides ask the same
+  auto copied = [&](const Tensor& t, long long begin) { return begin + RING_CHUNK <= t.n && on_boundaries<P>(t); };
+  if (warp == CTA / 32) {
+    if (lane != 0) return;
+    bool ok = true;
+    for (int chunk = blockIdx.x; chunk < a.s.chunks && ok; chunk += gridDim.x) {
+      i = tensor_of(a, chunk, i);
+      const Tensor& t = a.t[i];
+      const long long begin = (long long)(chunk - a.chunk[i]) * RING_CHUNK;
+      if (!copied(t, begin)) continue;
+      ok = tc::mbar_wait(empty + 8 * st, ph ^ 1);
+      if (!ok) break;
+      const uint32_t to = rows0 + st * R::STAGE, bar = full + 8 * st;
+      tc::mbar_expect_tx(bar, R::STAGE);
+      tc::bulk_load(to, static_cast<const P*>(t.p) + begin, bar, R::VALUES);
+      tc::bulk_load(to + R::VALUES, static_cast<const P*>(t.g) + begin, bar, R::VALUES);
+      tc::bulk_load(to + 2 * R::VALUES, static_cast<const uint8_t*>(a.s.m) + t.at + begin, bar, RING_CHUNK);
+      tc::bulk_load(to + 2 * R::VALUES + RING_CHUNK, static_cast<const uint8_t*>(a.s.v) + t.at + begin, bar, RING_CHUNK);
+      if (++st == RING_STAGES) st = 0, ph ^= 1;
+    }
+    if (!ok) atomicOr(&g_adamw_status, 1);
+    return;
+  }
+  bool waited = false;
+  for (int chunk = blockIdx.x; chunk < a.s.chunks; chunk += gridDim.x) {
+    i = tensor_of(a, chunk, i);
+    const Tensor& t = a.t[i];
+    const long long begin = (long long)(chunk - a.chunk[i]) * RING_CHUNK, base = begin + warp * BLOCK;
+    float4 f;
+    unsigned key;
+    auto begun = [&] {
+      if (!waited) wait_for_kernel_before();
+      waited = true;
+      f = __ldcg(a.s.factors + i);
+      key = mix(__float_as_uint(f.w) + (unsigned)(begin >> 32));
+    };
+    if (!copied(t, begin)) {
+      if (base < t.n) edge_block<P, 8, FLUSH>(a.s, t, base, t.n, lane, f, key, begun);
+      continue;
+    }
+    Lane<P, 8> now;
+    now.sm = a.s.m_scale[(t.at + base) / BLOCK];
+    now.sv = a.s.v_scale[(t.at + base) / BLOCK];
+    begun();
+    if (!__all_sync(0xffffffffu, tc::mbar_wait(full + 8 * st, ph))) {
+      if (lane == 0) atomicOr(&g_adamw_status, 2);
+      return;
+    }
+    const uint8_t* const from = smem + st * R::STAGE;
+    const int k = warp * BLOCK + 8 * lane;
+    now.p.load_shared(reinterpret_cast<const P*>(from) + k);
+    now.g.load_shared(reinterpret_cast<const P*>(from + R::VALUES) + k);
+    now.m = *reinterpret_cast<const uint2*>(from + 2 * R::VALUES + k);
+    now.v = *reinterpret_cast<const uint2*>(from + 2 * R::VALUES + RING_CHUNK + k);
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(empty + 8 * st);
+    whole_block<P, 8, FLUSH>(a.s, t, now, base, lane, f, key);
+    if (++st == RING_STAGES) st = 0, ph ^= 1;
   }
 }
 
@@ -308,11 +414,11 @@ int launch(const Step& s, const Begin& b, const spion_adamw_tensor* ts, int coun
   a.s.count = 0;
   ix.b = b;
   ix.b.count = 0;
-  // chunks of four blocks a warp where that leaves eight to every CTA: 75 million values in 8 bits SPAN4 us, one block a warp SPAN1
   long long chunks = 0, total = 0;
   for (int i = 0; i < count; ++i) total += ts[i].n;
-  const long long most = (long long)sm_count() * CTAS<BITS>;
-  a.s.span = CTA / 32 * BLOCK * (BITS == 8 && total >= most * 8 * 4 * (CTA / 32 * BLOCK) ? 4 : 1);
+  const bool ring = BITS == 8 && total >= (long long)sm_count() * RING_CTAS * RING_CHUNK * 8;      // eight chunks for each CTA
+  const long long most = (long long)sm_count() * (ring ? RING_CTAS : CTAS<BITS>);
+  a.s.span = CTA / 32 * BLOCK;
   for (int full = 1; full >= 0; --full)                                  // tensors without values last: they have a count only
     for (int i = 0; i < count; ++i) {
       if ((ts[i].n > 0) != (full == 1)) continue;
@@ -326,8 +432,21 @@ int launch(const Step& s, const Begin& b, const spion_adamw_tensor* ts, int coun
   a.s.chunks = (int)chunks;
   k_adamw_begin<MAX><<<1, MAX, 0, st>>>(ix);
   SPION_LAUNCH_CHECK();
-  if (chunks > 0)
-    SPION_CUDA_TRY(launch_after(k_adamw<P, BITS, FLUSH, MAX>, dim3((unsigned)(chunks < most ? chunks : most)), dim3(CTA), 0, st, a));
+  const dim3 grid((unsigned)(chunks < most ? chunks : most));
+  if constexpr (BITS == 8) {
+    if (ring) {
+      static std::atomic<uint64_t> ready{0};                               // devices on which the kernel has its shared memory
+      int dev = 0;
+      SPION_CUDA_TRY(cudaGetDevice(&dev));
+      if (dev >= 64 || !(ready.load() >> dev & 1)) {
+        SPION_CUDA_TRY(cudaFuncSetAttribute(k_adamw_ring<P, FLUSH, MAX>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RingOf<P>::SMEM));
+        if (dev < 64) ready.fetch_or(1ull << dev);
+      }
+      SPION_CUDA_TRY(launch_after(k_adamw_ring<P, FLUSH, MAX>, grid, dim3(CTA + 32), RingOf<P>::SMEM, st, a));
+      return SPION_OK;
+    }
+  }
+  if (chunks > 0) SPION_CUDA_TRY(launch_after(k_adamw<P, BITS, FLUSH, MAX>, grid, dim3(CTA), 0, st, a));
   return SPION_OK;
 }
 template <class P, int BITS>
@@ -343,6 +462,8 @@ int launches(const Step& s, const Begin& b, const spion_adamw_tensor* ts, int co
 }
 
 }  // namespace
+
+int adamw_status(int reset, cudaStream_t st) { return device_word_status(&g_adamw_status, "optimizer", reset, st); }
 
 extern "C" int spion_adamw_step(const spion_adamw_tensor* host_tensors, int count, int type, int state_bits, void* m, void* v, float* m_scale,
                                 float* v_scale, float* steps, const float* lr_dev, double lr, double beta1, double beta2, double eps,

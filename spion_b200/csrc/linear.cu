@@ -1609,8 +1609,10 @@ int linear_status(int reset, cudaStream_t st) {
   int v = 0;
   SPION_CUDA_TRY(cudaMemcpyFromSymbolAsync(&v, g_lin_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
   SPION_CUDA_TRY(cudaStreamSynchronize(st));
-  const int eight_bit = linear_e4m3_status(reset, st), norm = rmsnorm_status(reset, st);
-  if (v == 0) return eight_bit != SPION_OK ? eight_bit : norm;
+  int others = SPION_OK;
+  for (int rc : {linear_e4m3_status(reset, st), rmsnorm_status(reset, st), adamw_status(reset, st)})
+    if (others == SPION_OK) others = rc;
+  if (v == 0) return others;
   if (reset) {
     void* word = nullptr;
     SPION_CUDA_TRY(cudaGetSymbolAddress(&word, g_lin_status));

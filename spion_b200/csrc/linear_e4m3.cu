@@ -455,20 +455,7 @@ template <class Y> int launch_any(const Lin8Args& a, cudaStream_t st) {
 }  // namespace
 
 // Status word of these kernels on the current device, after the work of a stream (linear.cu reports it with its own)
-int linear_e4m3_status(int reset, cudaStream_t st) {
-  int v = 0;
-  SPION_CUDA_TRY(cudaMemcpyFromSymbolAsync(&v, g_lin8_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
-  SPION_CUDA_TRY(cudaStreamSynchronize(st));
-  if (v == 0) return SPION_OK;
-  if (reset) {
-    void* word = nullptr;
-    SPION_CUDA_TRY(cudaGetSymbolAddress(&word, g_lin8_status));
-    SPION_CUDA_TRY(cudaMemsetAsync(word, 0, sizeof(int), st));
-    SPION_CUDA_TRY(cudaStreamSynchronize(st));
-  }
-  fprintf(stderr, "spion_b200: status word of the 8-bit linear layers = 0x%x (a bounded wait gave up)\n", v);
-  return SPION_ERR_TIMEOUT;
-}
+int linear_e4m3_status(int reset, cudaStream_t st) { return device_word_status(&g_lin8_status, "8-bit linear layers", reset, st); }
 
 extern "C" int spion_linear_e4m3(const void* x, long long ldx, const float* x_scale, const void* w, long long ldw, const float* w_scale, const void* bias,
                                  int bias_type, void* y, long long ldy, int y_type, long long T, int K, int N, void* cuda_stream) {

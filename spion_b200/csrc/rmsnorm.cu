@@ -681,20 +681,7 @@ bool stream_type(int t) { return t == SPION_F32 || t == SPION_BF16 || t == SPION
 }  // namespace
 
 // Status word of the norm's backward on the current device, after the work of a stream (linear.cu reports it with its own)
-int rmsnorm_status(int reset, cudaStream_t st) {
-  int v = 0;
-  SPION_CUDA_TRY(cudaMemcpyFromSymbolAsync(&v, g_rms_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
-  SPION_CUDA_TRY(cudaStreamSynchronize(st));
-  if (v == 0) return SPION_OK;
-  if (reset) {
-    void* word = nullptr;
-    SPION_CUDA_TRY(cudaGetSymbolAddress(&word, g_rms_status));
-    SPION_CUDA_TRY(cudaMemsetAsync(word, 0, sizeof(int), st));
-    SPION_CUDA_TRY(cudaStreamSynchronize(st));
-  }
-  fprintf(stderr, "spion_b200: status word of the root-mean-square norm = 0x%x (a bounded wait gave up)\n", v);
-  return SPION_ERR_TIMEOUT;
-}
+int rmsnorm_status(int reset, cudaStream_t st) { return device_word_status(&g_rms_status, "root-mean-square norm", reset, st); }
 
 extern "C" {
 
