@@ -4,6 +4,10 @@
 //   k_lin8        tcgen05 kind::f8f6f4, 128 tokens x BN features per tile, accumulators in tensor memory
 //   k_lin8_few    up to 8 tokens, where the weights are all there is to read: mma.sync on fragments that go through shared memory as they lie
 //
+// Bound by the tensor cores where K and N are large (8192 x 4096 x 4096: 95 us, 2.9 PFLOP/s, the tensor pipe 83 % busy; by single CTAs of 128 x 256 105 us:
+// a pair reads half of the features' tile each, so a third less goes through shared memory and L2), by the passes over tokens and results where they are small
+// (131072 x 64 to 128: 10.8 us, 3.9 TB/s), by the weights for few tokens.
+//
 // Products of two e4m3 numbers are exact in fp32 and are summed there.  The scales are applied to the sums, so operands stay as they lie in memory.
 #include <algorithm>
 
@@ -36,18 +40,21 @@ constexpr int L8_EPI = 8;                                 // warps that write re
 constexpr int L8_THREADS = 32 * (2 + L8_EPI);
 constexpr uint32_t L8_OUT = 4096;                         // results on their way out: 32 rows of up to 128 bytes
 // BK: bytes of the contraction in a chunk, 128, or 64 where there are no more: a box that is half outside of its matrix takes longer than a full one (131072
-// tokens of 64 features to 64: BK128 us, BK64).  CTAS: on a multiprocessor.  Two where the contraction is a chunk or two: a tile's latencies are most of
+// tokens of 64 features to 64: 14.6 us, 12.3).  CTAS: on a multiprocessor.  Two where the contraction is a chunk or two: a tile's latencies are most of
 // its time then.
-template <int BN, int BK, int CTAS> struct L8 {
-  static constexpr uint32_t A = 128 * BK, STAGE = A + BN * BK;
+// PAIR: two CTAs of a cluster share a tile of 256 tokens; each brings its half of the tokens and of the features, one of them issues the products for both.
+template <int BN, int BK, int CTAS, bool PAIR> struct L8 {
+  static constexpr int FEATURES = PAIR ? BN / 2 : BN, TOKENS = PAIR ? 256 : 128;      // brought by a CTA; of a tile
+  static constexpr uint32_t A = 128 * BK, STAGE = A + FEATURES * BK;
   static constexpr int STAGES = CTAS == 1 ? 192 * 1024 / STAGE : 2, OUTS = CTAS == 2 && BK == 64 ? 2 : 1;      // stages; buffers of a writing warp
   static constexpr uint32_t RING = STAGES * STAGE;
   static constexpr uint32_t SCALES = RING + L8_EPI * OUTS * L8_OUT, BARS = SCALES + L8_EPI * 256;      // per warp: scale and bias of 32 features
   static constexpr uint32_t SMEM = BARS + 16 * STAGES + 64;
   static constexpr int ACC = 2 * BN;                      // tensor memory columns: two tiles
 };
-static_assert(L8<256, 128, 1>::SMEM <= 232448 && L8<128, 128, 1>::SMEM <= 232448 && L8<64, 128, 1>::SMEM <= 232448 &&
-              2 * (L8<128, 128, 2>::SMEM + 1024) <= 233472 && 2 * (L8<128, 64, 2>::SMEM + 1024) <= 233472 && 2 * L8<128, 128, 2>::ACC <= 512, "shared and tensor memory of a multiprocessor");
+static_assert(L8<256, 128, 1, true>::SMEM <= 232448 && L8<256, 128, 1, false>::SMEM <= 232448 && L8<128, 128, 1, false>::SMEM <= 232448 && L8<64, 128, 1, false>::SMEM <= 232448 &&
+              2 * (L8<128, 128, 2, false>::SMEM + 1024) <= 233472 && 2 * (L8<128, 64, 2, false>::SMEM + 1024) <= 233472 && 2 * L8<128, 128, 2, false>::ACC <= 512,
+              "shared and tensor memory of a multiprocessor");
 
 // Tiles in groups of 16 rows of tiles, column by column inside a group: the CTAs that run at a time share their operands in L2.
 __device__ __forceinline__ void tile_at(const Lin8Args& a, int i, int& m, int& n) {
@@ -77,31 +84,81 @@ __device__ __forceinline__ void st_shared16(uint32_t a, uint32_t x, uint32_t y, 
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+// ---- a pair of CTAs
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t in_leader(uint32_t addr) {          // the same place in the pair's first CTA
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ void pair_arrive(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void pair_tma_load_2d(uint32_t smem_dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(smem_dst), "l"((uint64_t)map), "r"(cluster_bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void pair_tmem_alloc(uint32_t smem_slot, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_slot), "r"(ncols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pair_tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// D: 128 rows in the tensor memory of each CTA; A and B: the same places of both CTAs' shared memory, half of the rows in each
+__device__ __forceinline__ void pair_mma_e4m3(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      :
+      : "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void pair_commit(uint32_t bar) {             // on both CTAs' barriers
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+
 // Warp 0 loads, warp 1 multiplies, the others write.  Every wait is bounded; whoever gives up leaves, and so do all that wait for it.
-template <int BN, int BK, int CTAS, class Y>
+// PAIR: both CTAs load and write, the first one's warp 1 multiplies for both.  Its `full` barriers count the bytes of both, its `acc_empty` the writing warps
+// of both; `empty` and `acc_full` are signalled in both.
+template <int BN, int BK, int CTAS, bool PAIR, class Y>
 __global__ void __launch_bounds__(L8_THREADS, CTAS) k_lin8(const __grid_constant__ Lin8Args a, const __grid_constant__ Lin8Maps maps) {
-  using C = L8<BN, BK, CTAS>;
+  using C = L8<BN, BK, CTAS, PAIR>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t sbase = smem_u32(smem_raw);
   const uint32_t full = sbase + C::BARS, empty = full + 8 * C::STAGES, acc_full = empty + 8 * C::STAGES, acc_empty = acc_full + 16, slot = acc_empty + 16;
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int chunks = (a.K + BK - 1) / BK, tiles = a.tiles_m * a.tiles_n;
   volatile int& s_abort = *reinterpret_cast<int*>(smem_raw + (slot + 8 - sbase));
+  const int rank = PAIR ? (int)cta_rank() : 0, first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
   if (warp == 0 && lane == 0) {
     s_abort = *reinterpret_cast<volatile int*>(&g_lin8_status);
     for (int i = 0; i < C::STAGES; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(acc_full + 8 * i, 1), mbar_init(acc_empty + 8 * i, L8_EPI);
+    for (int i = 0; i < 2; ++i) mbar_init(acc_full + 8 * i, 1), mbar_init(acc_empty + 8 * i, PAIR ? 2 * L8_EPI : L8_EPI);
     fence_barrier_init();
     fence_proxy_async();
     tma_prefetch_desc(&maps.x);
     tma_prefetch_desc(&maps.w);
   }
   if (warp == 1) {
-    tmem_alloc(slot, C::ACC);
-    tmem_relinquish();
+    if (PAIR) {
+      pair_tmem_alloc(slot, C::ACC);
+    } else {
+      tmem_alloc(slot, C::ACC);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<uint32_t*>(smem_raw + (slot - sbase));
   wait_for_kernel_before();                              // the operands of a call are often the results of the kernel before
@@ -110,28 +167,36 @@ __global__ void __launch_bounds__(L8_THREADS, CTAS) k_lin8(const __grid_constant
       if (elect_one()) {
         int st = 0, ph = 1;                              // a ring that has not been used yet is empty
         bool ok = true;
-        for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
+        for (int i = first; i < tiles && ok; i += step) {
           int m, n;
           tile_at(a, i, m, n);
           for (int c = 0; c < chunks && ok; ++c) {
             ok = mbar_wait(empty + 8 * st, ph);
             if (!ok) break;
-            mbar_expect_tx(full + 8 * st, C::STAGE);
-            tma_load_2d(sbase + st * C::STAGE, &maps.x, full + 8 * st, c * BK, m * 128);
-            tma_load_2d(sbase + st * C::STAGE + C::A, &maps.w, full + 8 * st, c * BK, n * BN);
+            const int row = m * C::TOKENS + rank * 128, col = n * BN + rank * C::FEATURES;
+            if (PAIR) {
+              if (rank == 0) mbar_expect_tx(full + 8 * st, 2 * C::STAGE);
+              const uint32_t bar = in_leader(full + 8 * st);
+              pair_tma_load_2d(sbase + st * C::STAGE, &maps.x, bar, c * BK, row);
+              pair_tma_load_2d(sbase + st * C::STAGE + C::A, &maps.w, bar, c * BK, col);
+            } else {
+              mbar_expect_tx(full + 8 * st, C::STAGE);
+              tma_load_2d(sbase + st * C::STAGE, &maps.x, full + 8 * st, c * BK, row);
+              tma_load_2d(sbase + st * C::STAGE + C::A, &maps.w, full + 8 * st, c * BK, col);
+            }
             if (++st == C::STAGES) st = 0, ph ^= 1;
           }
         }
         if (!ok) report(&g_lin8_status, ERR_LOAD_WAIT);
       }
     } else if (warp == 1) {
-      if (elect_one()) {
-        constexpr uint32_t idesc = idesc_e4m3(128, BN);
+      if (rank == 0 && elect_one()) {
+        constexpr uint32_t idesc = idesc_e4m3(C::TOKENS, BN);
         constexpr uint32_t layout = BK == 128 ? LAYOUT_SW128 : LAYOUT_SW64;
         const uint64_t a0 = make_smem_desc(sbase, 16, 8 * BK, layout), b0 = make_smem_desc(sbase + C::A, 16, 8 * BK, layout);
         int st = 0, ph = 0, buf = 0, acc_ph = 1;
         bool ok = true;
-        for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
+        for (int i = first; i < tiles && ok; i += step) {
           ok = mbar_wait(acc_empty + 8 * buf, acc_ph);
           tc_fence_after();
           for (int c = 0; c < chunks && ok; ++c) {
@@ -141,12 +206,19 @@ __global__ void __launch_bounds__(L8_THREADS, CTAS) k_lin8(const __grid_constant
             const int left = a.K - c * BK;
 #pragma unroll
             for (int k = 0; k < BK / 32; ++k)
-              if (32 * k < left)
-                mma_e4m3(tmem + buf * BN, desc_advance(a0, st * C::STAGE + 32 * k), desc_advance(b0, st * C::STAGE + 32 * k), idesc, c > 0 || k > 0);
-            mma_commit(empty + 8 * st);
+              if (32 * k < left) {
+                const uint64_t ad = desc_advance(a0, st * C::STAGE + 32 * k), bd = desc_advance(b0, st * C::STAGE + 32 * k);
+                if (PAIR) pair_mma_e4m3(tmem + buf * BN, ad, bd, idesc, c > 0 || k > 0);
+                else mma_e4m3(tmem + buf * BN, ad, bd, idesc, c > 0 || k > 0);
+              }
+            if (PAIR) pair_commit(empty + 8 * st);
+            else mma_commit(empty + 8 * st);
             if (++st == C::STAGES) st = 0, ph ^= 1;
           }
-          if (ok) mma_commit(acc_full + 8 * buf);
+          if (ok) {
+            if (PAIR) pair_commit(acc_full + 8 * buf);
+            else mma_commit(acc_full + 8 * buf);
+          }
           buf ^= 1;
           if (buf == 0) acc_ph ^= 1;
         }
@@ -165,7 +237,7 @@ __global__ void __launch_bounds__(L8_THREADS, CTAS) k_lin8(const __grid_constant
         int m, n;
         if (i >= tiles) return 0.f;
         tile_at(a, i, m, n);
-        const int t = m * 128 + q * 32 + lane;
+        const int t = m * C::TOKENS + rank * 128 + q * 32 + lane;
         return t < a.T ? a.sx[t] : 0.f;
       };
       auto column_scales = [&](int i) {
@@ -181,13 +253,13 @@ __global__ void __launch_bounds__(L8_THREADS, CTAS) k_lin8(const __grid_constant
           b[g] = c < a.N && a.bias != nullptr ? load_any(a.bias, a.bias_type, c) : 0.f;
         }
       };
-      sx = row_scale(blockIdx.x);
-      column_scales(blockIdx.x);
-      for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
+      sx = row_scale(first);
+      column_scales(first);
+      for (int i = first; i < tiles; i += step) {
         int m, n;
         tile_at(a, i, m, n);
-        const int c0 = n * BN + half * (BN / 2);
-        const float next = row_scale(i + gridDim.x);
+        const int c0 = n * BN + half * (BN / 2), row0 = m * C::TOKENS + rank * 128 + q * 32;
+        const float next = row_scale(i + step);
         if (!tc::warp_wait(acc_full + 8 * buf, ph, &g_lin8_status, ERR_MMA2_WAIT)) break;
         tc_fence_after();
 #pragma unroll
@@ -211,7 +283,10 @@ __global__ void __launch_bounds__(L8_THREADS, CTAS) k_lin8(const __grid_constant
             if (g == BN / 2 - 32) {
               tc_fence_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive(acc_empty + 8 * buf);
+              if (lane == 0) {
+                if (PAIR) pair_arrive(in_leader(acc_empty + 8 * buf));
+                else mbar_arrive(acc_empty + 8 * buf);
+              }
             }
             __syncwarp();
             float v[32];
@@ -238,17 +313,17 @@ __global__ void __launch_bounds__(L8_THREADS, CTAS) k_lin8(const __grid_constant
           if (a.staged) {
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0 && c < a.N) tma_store_2d(&maps.y, tile, c, m * 128 + q * 32);
+            if (lane == 0 && c < a.N && row0 < a.T) tma_store_2d(&maps.y, tile, c, row0);
             if (lane == 0) bulk_commit();
           } else {                                       // rows that start anywhere: lanes side by side along each
             __syncwarp();
             const uint8_t* const from = smem_raw + (tile - sbase);
-            const int rows_here = min(32, a.T - (m * 128 + q * 32));
+            const int rows_here = min(32, a.T - row0);
             constexpr int PER = 16 / (int)sizeof(Y);     // elements of a piece
 #pragma unroll
             for (int g = 0; g < COLS; g += 32) {
               const int e = g + lane;
-              Y* const y = static_cast<Y*>(a.y) + (long long)(m * 128 + q * 32) * a.ldy + c + e;
+              Y* const y = static_cast<Y*>(a.y) + (long long)row0 * a.ldy + c + e;
               if (c + e < a.N)
                 for (int r = 0; r < rows_here; ++r)
                   y[r * a.ldy] = *reinterpret_cast<const Y*>(from + r * ROW + (((e / PER) ^ (ROW == 128 ? r & 7 : (r >> 1) & 3)) << 4) + e % PER * (int)sizeof(Y));
@@ -258,7 +333,7 @@ __global__ void __launch_bounds__(L8_THREADS, CTAS) k_lin8(const __grid_constant
           if (C::OUTS == 2) turn ^= 1;
         }
         sx = next;
-        column_scales(i + gridDim.x);
+        column_scales(i + step);
         buf ^= 1;
         if (buf == 0) ph ^= 1;
       }
@@ -267,8 +342,12 @@ __global__ void __launch_bounds__(L8_THREADS, CTAS) k_lin8(const __grid_constant
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();                              // neither CTA's memory goes while the other may signal in it
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, C::ACC);
+  if (warp == 1) {
+    if (PAIR) pair_tmem_dealloc(tmem, C::ACC);
+    else tmem_dealloc(tmem, C::ACC);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ few tokens
@@ -296,7 +375,7 @@ __device__ __forceinline__ void multiply(uint4 u, uint4 v, uint4 x, float (&d)[4
 // A CTA has 16 features.  Bulk copies bring 2048 bytes of each feature's and each token's row at a time, twice that is under way; the CTA's warps take every
 // eighth piece of 64.  Which four bytes of a lane's 16 the product takes for which index of the contraction does not matter as long as tokens and weights
 // agree, so a lane's words are used as they come.  Loads to registers instead were ordered one behind another by the compiler (one token, 4096 to 4096
-// features: FEWREG us, so FEWBULK).
+// features, a graph of one call: 10.3 us, so 8.6; in a row of calls 5.5, 3.0 TB/s of weights, where launch and first bytes are most of the time).
 template <class Y>
 __global__ void __launch_bounds__(32 * FEW_WARPS) k_lin8_few(const __grid_constant__ Lin8Args a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -413,25 +492,49 @@ template <auto Kernel> int big_shared_memory_of(uint32_t bytes) {
   }
   return SPION_OK;
 }
-template <int BN, int BK, int CTAS, class Y> int launch_tiles(Lin8Args a, cudaStream_t st) {
+template <int BN, int BK, int CTAS, bool PAIR, class Y> int launch_tiles(Lin8Args a, cudaStream_t st) {
+  using C = L8<BN, BK, CTAS, PAIR>;
   Encode encode;
   int rc = encoder(&encode);
   if (rc != SPION_OK) return rc;
-  a.tiles_m = (a.T + 127) / 128;
+  a.tiles_m = (a.T + C::TOKENS - 1) / C::TOKENS;
   a.tiles_n = (a.N + BN - 1) / BN;
   if ((long long)a.tiles_m * a.tiles_n > 0x7fffffff) return SPION_ERR_SHAPE;
   a.staged = ((uintptr_t)a.y % 16 == 0) && (a.ldy * (long long)sizeof(Y)) % 16 == 0;
   Lin8Maps maps;
   if ((rc = map_of(&maps.x, encode, a.x, SPION_E4M3, a.K, a.T, a.ldx, BK, 128)) != SPION_OK) return rc;
-  if ((rc = map_of(&maps.w, encode, a.w, SPION_E4M3, a.K, a.N, a.ldw, BK, BN)) != SPION_OK) return rc;
+  if ((rc = map_of(&maps.w, encode, a.w, SPION_E4M3, a.K, a.N, a.ldw, BK, C::FEATURES)) != SPION_OK) return rc;
   if (a.staged) {
     if ((rc = map_of(&maps.y, encode, a.y, type_code<Y>(), a.N, a.T, a.ldy, sizeof(Y) == 4 || BN == 64 ? 32 : 64, 32)) != SPION_OK) return rc;
   } else {
     maps.y = maps.x;                                     // not used
   }
-  if ((rc = big_shared_memory_of<k_lin8<BN, BK, CTAS, Y>>(L8<BN, BK, CTAS>::SMEM)) != SPION_OK) return rc;
+  if ((rc = big_shared_memory_of<k_lin8<BN, BK, CTAS, PAIR, Y>>(C::SMEM)) != SPION_OK) return rc;
   const int tiles = a.tiles_m * a.tiles_n;
-  SPION_CUDA_TRY(launch_after(k_lin8<BN, BK, CTAS, Y>, dim3(std::min(tiles, sm_count() * CTAS)), dim3(L8_THREADS), L8<BN, BK, CTAS>::SMEM, st, a, maps));
+  if constexpr (PAIR) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.blockDim = dim3(L8_THREADS), cfg.dynamicSmemBytes = C::SMEM, cfg.stream = st, cfg.attrs = at;
+    // as many pairs as the device holds at a time (multiprocessors are paired inside their groups): the tiles are shared out evenly among those
+    static std::atomic<int> pairs[64];
+    int dev = 0;
+    SPION_CUDA_TRY(cudaGetDevice(&dev));
+    int n = dev < 64 ? pairs[dev].load() : 0;
+    if (n == 0) {
+      cfg.gridDim = dim3(2 * (sm_count() / 2)), cfg.numAttrs = 1;
+      SPION_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, k_lin8<BN, BK, CTAS, PAIR, Y>, &cfg));
+      if (n <= 0) return SPION_ERR_UNSUPPORTED;
+      if (dev < 64) pairs[dev].store(n);
+    }
+    cfg.gridDim = dim3(2 * std::min(tiles, n)), cfg.numAttrs = 2;
+    SPION_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_lin8<BN, BK, CTAS, PAIR, Y>, (const Lin8Args)a, (const Lin8Maps)maps));
+    return SPION_OK;
+  }
+  SPION_CUDA_TRY(launch_after(k_lin8<BN, BK, CTAS, PAIR, Y>, dim3(std::min(tiles, sm_count() * CTAS)), dim3(L8_THREADS), C::SMEM, st, a, maps));
   return SPION_OK;
 }
 template <class Y> int launch_few(const Lin8Args& a, cudaStream_t st) {
@@ -446,10 +549,10 @@ template <class Y> int launch_any(const Lin8Args& a, cudaStream_t st) {
   if (a.T <= FEW_TOKENS) return launch_few<Y>(a, st);
   const long long rows_ = (a.T + 127) / 128, sms = sm_count();
   const bool wide = a.N > 64 && rows_ * ((a.N + 127) / 128) >= sms;
-  if (a.K <= 64) return wide ? launch_tiles<128, 64, 2, Y>(a, st) : launch_tiles<64, 64, 2, Y>(a, st);
-  if (a.K <= 256) return wide ? launch_tiles<128, 128, 2, Y>(a, st) : launch_tiles<64, 128, 2, Y>(a, st);
-  if (a.N > 128 && rows_ * ((a.N + 255) / 256) >= sms) return launch_tiles<256, 128, 1, Y>(a, st);
-  return wide ? launch_tiles<128, 128, 1, Y>(a, st) : launch_tiles<64, 128, 1, Y>(a, st);
+  if (a.K <= 64) return wide ? launch_tiles<128, 64, 2, false, Y>(a, st) : launch_tiles<64, 64, 2, false, Y>(a, st);
+  if (a.K <= 256) return wide ? launch_tiles<128, 128, 2, false, Y>(a, st) : launch_tiles<64, 128, 2, false, Y>(a, st);
+  if (a.N > 128 && rows_ * ((a.N + 255) / 256) >= sms) return launch_tiles<256, 128, 1, true, Y>(a, st);
+  return wide ? launch_tiles<128, 128, 1, false, Y>(a, st) : launch_tiles<64, 128, 1, false, Y>(a, st);
 }
 
 }  // namespace
