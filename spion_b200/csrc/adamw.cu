@@ -26,7 +26,7 @@ using namespace rows;
 
 namespace {
 
-constexpr int BLOCK = 256, CTA = 256;                           // values that share scales; threads
+constexpr int BLOCK = 256, CTA = 256, CHUNK = CTA / 32 * BLOCK;  // values that share scales; threads; values that a CTA takes at a time, a block per warp
 constexpr int FEW = 64, MOST = 512;                             // tensors of a launch
 
 struct Tensor {
@@ -42,7 +42,6 @@ struct Step {
   float b1, b2, c1, c2;       // betas and what is left of one
   float eps, clip;            // clip < 0: none
   int count, chunks, copy_type;
-  int span;                   // values of a chunk: one block per warp, or several where there are many
 };
 template <int MAX> struct Table {
   Step s;
@@ -250,60 +249,53 @@ template <class P> __device__ __forceinline__ bool on_boundaries(const Tensor& t
   return (((uintptr_t)t.p | (uintptr_t)t.g) & (8 * sizeof(P) - 1)) == 0 && ((uintptr_t)t.copy & 15) == 0;
 }
 
-template <int BITS> constexpr int CTAS = BITS == 32 ? 4 : 4;              // resident on a multiprocessor
+constexpr int CTAS = 4;                                                  // resident on a multiprocessor
 template <class P, int BITS, bool FLUSH, int MAX>
-__global__ void __launch_bounds__(CTA, CTAS<BITS>) k_adamw(const __grid_constant__ Table<MAX> a) {
+__global__ void __launch_bounds__(CTA, CTAS) k_adamw(const __grid_constant__ Table<MAX> a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int i = 0;
   for (int chunk = blockIdx.x; chunk < a.s.chunks; chunk += gridDim.x) {
     i = tensor_of(a, chunk, i);
     const Tensor& t = a.t[i];
-    const bool boundary = on_boundaries<P>(t);
-    const long long begin = (long long)(chunk - a.chunk[i]) * a.s.span, end = min(t.n, begin + a.s.span);
+    const long long base = (long long)(chunk - a.chunk[i]) * CHUNK + warp * BLOCK;     // of the warp's block in its tensor
+    if (base >= t.n) continue;
     float4 f;
     unsigned key;
-    // k_adamw_begin has been started after everything that this step reads was written: only what it writes itself is waited for, with the first block
-    // of values on its way
+    // k_adamw_begin has been started after everything that this step reads was written: only what it writes itself is waited for, with the block's values
+    // on their way
     auto begun = [&] {
       wait_for_kernel_before();
       f = __ldcg(a.s.factors + i);
-      key = mix(__float_as_uint(f.w) + (unsigned)(begin >> 32));
+      key = mix(__float_as_uint(f.w) + (unsigned)(base >> 32));
     };
-    bool first = true;
-    long long base = begin + warp * BLOCK;
-    for (; boundary && base + BLOCK <= end; base += CTA / 32 * BLOCK) {
-      const long long k = base + 8 * lane, at = t.at + k;
-      Lane<P, BITS> now;
-      now.p.load(static_cast<P*>(t.p) + k);
-      now.g.load(static_cast<const P*>(t.g) + k);
-      if constexpr (BITS == 32) {
-        now.m.load(static_cast<const float*>(a.s.m) + at);
-        now.v.load(static_cast<const float*>(a.s.v) + at);
-      } else {
-        now.m = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.s.m) + at);
-        now.v = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.s.v) + at);
-        now.sm = a.s.m_scale[at / BLOCK];
-        now.sv = a.s.v_scale[at / BLOCK];
-      }
-      if (first) begun();
-      first = false;
-      whole_block<P, BITS, FLUSH>(a.s, t, now, base, lane, f, key);
+    if (base + BLOCK > t.n || !on_boundaries<P>(t)) {
+      edge_block<P, BITS, FLUSH>(a.s, t, base, t.n, lane, f, key, begun);
+      continue;
     }
-    for (; base < end; base += CTA / 32 * BLOCK) {
-      edge_block<P, BITS, FLUSH>(a.s, t, base, end, lane, f, key, [&] {
-        if (first) begun();
-        first = false;
-      });
+    const long long k = base + 8 * lane, at = t.at + k;
+    Lane<P, BITS> now;
+    now.p.load(static_cast<P*>(t.p) + k);
+    now.g.load(static_cast<const P*>(t.g) + k);
+    if constexpr (BITS == 32) {
+      now.m.load(static_cast<const float*>(a.s.m) + at);
+      now.v.load(static_cast<const float*>(a.s.v) + at);
+    } else {
+      now.m = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.s.m) + at);
+      now.v = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.s.v) + at);
+      now.sm = a.s.m_scale[at / BLOCK];
+      now.sv = a.s.v_scale[at / BLOCK];
     }
+    begun();
+    whole_block<P, BITS, FLUSH>(a.s, t, now, base, lane, f, key);
   }
 }
 
 // The same for many values with 8-bit moments, where a block's arithmetic takes as long as its way from memory: a warp of its own keeps three chunks of 2048
 // values under way to shared memory by bulk copies while eight warps work.  75 million fp32 values: 257 us without
 // it (4.6 TB/s; 70 instructions a value, two thirds of the issue slots), 214 with it (5.6 TB/s).
-constexpr int RING_STAGES = 3, RING_CTAS = 3, RING_CHUNK = CTA / 32 * BLOCK;
+constexpr int RING_STAGES = 3, RING_CTAS = 3;
 template <class P> struct RingOf {
-  static constexpr uint32_t VALUES = RING_CHUNK * sizeof(P), STAGE = 2 * VALUES + 2 * RING_CHUNK, SMEM = RING_STAGES * STAGE + 64;
+  static constexpr uint32_t VALUES = CHUNK * sizeof(P), STAGE = 2 * VALUES + 2 * CHUNK, SMEM = RING_STAGES * STAGE + 64;
 };
 static_assert(RING_CTAS * (RingOf<float>::SMEM + 1024) <= 233472, "shared memory of a multiprocessor");
 // Set by a bounded wait that gave up; launches after it leave at once until spion_linear_status has reported it.
@@ -323,14 +315,14 @@ __global__ void __launch_bounds__(CTA + 32, RING_CTAS) k_adamw_ring(const __grid
   if (__syncthreads_or(*reinterpret_cast<volatile int*>(&g_adamw_status))) return;
   int i = 0, st = 0, ph = 0;
   // a chunk goes through the ring if all of it is there and lies on the boundaries: both sides ask the same
-  auto copied = [&](const Tensor& t, long long begin) { return begin + RING_CHUNK <= t.n && on_boundaries<P>(t); };
+  auto copied = [&](const Tensor& t, long long begin) { return begin + CHUNK <= t.n && on_boundaries<P>(t); };
   if (warp == CTA / 32) {
     if (lane != 0) return;
     bool ok = true;
     for (int chunk = blockIdx.x; chunk < a.s.chunks && ok; chunk += gridDim.x) {
       i = tensor_of(a, chunk, i);
       const Tensor& t = a.t[i];
-      const long long begin = (long long)(chunk - a.chunk[i]) * RING_CHUNK;
+      const long long begin = (long long)(chunk - a.chunk[i]) * CHUNK;
       if (!copied(t, begin)) continue;
       ok = tc::mbar_wait(empty + 8 * st, ph ^ 1);
       if (!ok) break;
@@ -338,8 +330,8 @@ __global__ void __launch_bounds__(CTA + 32, RING_CTAS) k_adamw_ring(const __grid
       tc::mbar_expect_tx(bar, R::STAGE);
       tc::bulk_load(to, static_cast<const P*>(t.p) + begin, bar, R::VALUES);
       tc::bulk_load(to + R::VALUES, static_cast<const P*>(t.g) + begin, bar, R::VALUES);
-      tc::bulk_load(to + 2 * R::VALUES, static_cast<const uint8_t*>(a.s.m) + t.at + begin, bar, RING_CHUNK);
-      tc::bulk_load(to + 2 * R::VALUES + RING_CHUNK, static_cast<const uint8_t*>(a.s.v) + t.at + begin, bar, RING_CHUNK);
+      tc::bulk_load(to + 2 * R::VALUES, static_cast<const uint8_t*>(a.s.m) + t.at + begin, bar, CHUNK);
+      tc::bulk_load(to + 2 * R::VALUES + CHUNK, static_cast<const uint8_t*>(a.s.v) + t.at + begin, bar, CHUNK);
       if (++st == RING_STAGES) st = 0, ph ^= 1;
     }
     if (!ok) atomicOr(&g_adamw_status, 1);
@@ -349,7 +341,7 @@ __global__ void __launch_bounds__(CTA + 32, RING_CTAS) k_adamw_ring(const __grid
   for (int chunk = blockIdx.x; chunk < a.s.chunks; chunk += gridDim.x) {
     i = tensor_of(a, chunk, i);
     const Tensor& t = a.t[i];
-    const long long begin = (long long)(chunk - a.chunk[i]) * RING_CHUNK, base = begin + warp * BLOCK;
+    const long long begin = (long long)(chunk - a.chunk[i]) * CHUNK, base = begin + warp * BLOCK;
     float4 f;
     unsigned key;
     auto begun = [&] {
@@ -375,7 +367,7 @@ __global__ void __launch_bounds__(CTA + 32, RING_CTAS) k_adamw_ring(const __grid
     now.p.load_shared(reinterpret_cast<const P*>(from) + k);
     now.g.load_shared(reinterpret_cast<const P*>(from + R::VALUES) + k);
     now.m = *reinterpret_cast<const uint2*>(from + 2 * R::VALUES + k);
-    now.v = *reinterpret_cast<const uint2*>(from + 2 * R::VALUES + RING_CHUNK + k);
+    now.v = *reinterpret_cast<const uint2*>(from + 2 * R::VALUES + CHUNK + k);
     __syncwarp();
     if (lane == 0) tc::mbar_arrive(empty + 8 * st);
     whole_block<P, 8, FLUSH>(a.s, t, now, base, lane, f, key);
@@ -418,9 +410,8 @@ int launch(const Step& s, const Begin& b, const spion_adamw_tensor* ts, int coun
   ix.b.count = 0;
   long long chunks = 0, total = 0;
   for (int i = 0; i < count; ++i) total += ts[i].n;
-  const bool ring = BITS == 8 && total >= (long long)sm_count() * RING_CTAS * RING_CHUNK * 8;      // eight chunks for each CTA
-  const long long most = (long long)sm_count() * (ring ? RING_CTAS : CTAS<BITS>);
-  a.s.span = CTA / 32 * BLOCK;
+  const bool ring = BITS == 8 && total >= (long long)sm_count() * RING_CTAS * CHUNK * 8;      // eight chunks for each CTA
+  const long long most = (long long)sm_count() * (ring ? RING_CTAS : CTAS);
   for (int full = 1; full >= 0; --full)                                  // tensors without values last: they have a count only
     for (int i = 0; i < count; ++i) {
       if ((ts[i].n > 0) != (full == 1)) continue;
@@ -428,7 +419,7 @@ int launch(const Step& s, const Begin& b, const spion_adamw_tensor* ts, int coun
       if (full == 0) continue;
       a.chunk[a.s.count] = (int)chunks;
       a.t[a.s.count++] = Tensor{ts[i].p, ts[i].g, ts[i].copy, ts[i].n, ts[i].at};
-      chunks += (ts[i].n + a.s.span - 1) / a.s.span;
+      chunks += (ts[i].n + CHUNK - 1) / CHUNK;
       if (chunks > 0x7fffffff) return SPION_ERR_SHAPE;
     }
   a.s.chunks = (int)chunks;
@@ -482,7 +473,7 @@ extern "C" int spion_adamw_step(const spion_adamw_tensor* host_tensors, int coun
     if (t.copy != nullptr && copy_type != SPION_BF16 && copy_type != SPION_F16) return SPION_ERR_ARG;
   }
   const Step s = {m, v, m_scale, v_scale, static_cast<const float4*>(workspace), (float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2),
-                  (float)eps, clip_value >= 0 ? (float)clip_value : -1.f, 0, 0, copy_type, 0};
+                  (float)eps, clip_value >= 0 ? (float)clip_value : -1.f, 0, 0, copy_type};
   const Begin b = {steps, static_cast<float4*>(workspace), lr_dev, lr, weight_decay, log(beta1), log(beta2), seed, 0};
   const cudaStream_t st = (cudaStream_t)cuda_stream;
   if (type == SPION_F32) return state_bits == 8 ? launches<float, 8>(s, b, host_tensors, count, st) : launches<float, 32>(s, b, host_tensors, count, st);

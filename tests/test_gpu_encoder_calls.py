@@ -1,0 +1,138 @@
+"""Calls of the encoder's operators that are allowed and unusual: a process's first calls inside a capture, recomputed segments and hooks on saved tensors, calls on
+two streams at once, inference mode, tracing and transforms (refused)."""
+import subprocess
+import sys
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+FIRST = """
+import torch
+from spion_b200 import _lib
+from spion_b200.optim import adamw_step
+from spion_b200.quant import linear_e4m3, quantize_rows
+from spion_b200.rmsnorm import rms_norm
+torch.zeros(1, device="cuda")
+shapes = ((5, 64, 128), (8192, 1024, 1024), (40000, 64, 128), (300, 512, 96))
+xs = [torch.randn(T, K, device="cuda", requires_grad=True) for T, K, N in shapes] + [torch.randn(600, 2048, device="cuda", requires_grad=True)]
+ws = [torch.randn(N, K, device="cuda") for T, K, N in shapes]
+g = torch.ones(2048, device="cuda", requires_grad=True)
+p, d = torch.randn(8_000_000, device="cuda"), torch.randn(8_000_000, device="cuda")
+m, v = torch.zeros(8_000_000, device="cuda").to(torch.float8_e4m3fn), torch.zeros(8_000_000, device="cuda").to(torch.float8_e5m2)
+scales, steps = (torch.ones(31250, device="cuda"), torch.ones(31250, device="cuda")), torch.zeros(1, device="cuda")
+dy = torch.randn(600, 2048, device="cuda")
+
+def all_of_them():
+    out = [linear_e4m3(x.detach(), quantize_rows(w), out_dtype=torch.bfloat16) for x, w in zip(xs, ws)]
+    y = rms_norm(xs[-1], g)
+    out += [y.detach(), *torch.autograd.grad(y, (xs[-1], g), dy)]
+    adamw_step([p], [d], m, v, steps, scales=scales)
+    return out
+
+graph = torch.cuda.CUDAGraph()
+start = p.clone()
+with torch.cuda.graph(graph):
+    got = all_of_them()
+graph.replay()
+torch.cuda.synchronize()
+p_graph = p.clone()
+p.copy_(start)
+m.view(torch.uint8).zero_(); v.view(torch.uint8).zero_(); steps.zero_()
+scales[0].fill_(1); scales[1].fill_(1)
+for a, b in zip(got, all_of_them()):
+    assert torch.equal(a, b)
+assert torch.equal(p, p_graph) and not torch.equal(p, start)
+_lib.check(_lib.lib.spion_linear_status(0))
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    r = subprocess.run([sys.executable, "-c", FIRST], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+def test_recomputed_segments_and_hooks_on_saved_tensors():
+    from torch.utils.checkpoint import checkpoint
+
+    from spion_b200.rmsnorm import rms_norm
+    x, r = torch.randn(50, 192, device="cuda", requires_grad=True), torch.randn(50, 192, device="cuda", requires_grad=True)
+    w = torch.randn(192, device="cuda", requires_grad=True)
+
+    def f(x, r, w):
+        s, y = rms_norm(x, w, res=r)
+        return s * 0.5 + rms_norm(y, w)
+
+    want = torch.autograd.grad(f(x, r, w).square().sum(), (x, r, w))
+    got = torch.autograd.grad(checkpoint(f, x, r, w, use_reentrant=False).square().sum(), (x, r, w))
+    with torch.autograd.graph.save_on_cpu():
+        loss = f(x, r, w).square().sum()
+    hooked = torch.autograd.grad(loss, (x, r, w))
+    for a, b, c in zip(want, got, hooked):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_two_streams_at_once():
+    from spion_b200.optim import adamw_step
+    from spion_b200.quant import linear_e4m3, quantize_rows
+    from spion_b200.rmsnorm import rms_norm
+    x = torch.randn(8192, 1024, device="cuda")
+    q, w, g = quantize_rows(x), quantize_rows(torch.randn(2048, 1024, device="cuda")), torch.ones(1024, device="cuda")
+    n = 9_000_000
+
+    def state():
+        return (torch.ones(n, device="cuda"), torch.full((n,), 0.5, device="cuda"), torch.zeros(-(-n // 256) * 256, device="cuda"),
+                torch.zeros(-(-n // 256) * 256, device="cuda"), torch.zeros(1, device="cuda"))
+
+    want_y, want_n = linear_e4m3(q, w), rms_norm(x, g)
+    states = [state() for _ in range(3)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k] += [linear_e4m3(q, w), rms_norm(x, g)]
+                p, d, m, v, steps = states[k]
+                adamw_step([p], [d], m, v, steps)
+    torch.cuda.synchronize()
+    p, d, m, v, steps = states[2]
+    for _ in range(5):
+        adamw_step([p], [d], m, v, steps)
+    for k in range(2):
+        for i, t in enumerate(got[k]):
+            assert torch.equal(t, want_n if i % 2 else want_y)
+        assert torch.equal(states[k][0], p) and float(states[k][4]) == 5
+
+
+def test_inference_mode_and_what_is_refused():
+    from spion_b200._lib import SpionError
+    from spion_b200.quant import quantize_rows
+    from spion_b200.rmsnorm import rms_norm, rms_norm_e4m3
+    x, w = torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda")
+    with torch.inference_mode():
+        a, b = rms_norm(x, w), rms_norm_e4m3(x.clone(), w)
+    assert torch.equal(a, rms_norm(x, w)) and b.scales.shape == (4,)
+
+    def refused(call, match):
+        with pytest.raises(SpionError, match=match):
+            call()
+
+    refused(lambda: torch.func.vmap(lambda t: rms_norm(t, w))(x), "ordinary")
+    refused(lambda: torch.jit.trace(lambda t: rms_norm(t, w), (x,)), "ordinary")
+    refused(lambda: rms_norm_e4m3(x.clone().requires_grad_(), w), "gradient")
+    refused(lambda: rms_norm(x, w[:32]), "weight")
+    refused(lambda: rms_norm(x, w.double()), "weight")
+    refused(lambda: rms_norm(x.double(), w), "type")
+    refused(lambda: rms_norm(x, w, res=x[:2]), "res")
+    refused(lambda: rms_norm(x.half(), w, res=x), "res")
+    refused(lambda: rms_norm(x.half(), w, out_dtype=torch.float32), "output")
+    refused(lambda: rms_norm(x, w.cpu()), "CUDA")
+    refused(lambda: quantize_rows(x.to(torch.float8_e4m3fn)), "type")
+    refused(lambda: quantize_rows(torch.tensor(1.0, device="cuda")), "shape")
+    refused(lambda: quantize_rows(torch.empty(3, 0, device="cuda")), "shape")
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        refused(lambda: rms_norm(dual, w), "ordinary")
