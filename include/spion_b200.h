@@ -509,7 +509,7 @@ int spion_linear_e4m3(const void* x, long long ldx, const float* x_scale, const 
  * fills the last block of 256 is left alone).  state_bits 32: fp32.  state_bits 8: m in e4m3, v in e5m2, and per block of 256 a scale each (powers of
  * two, [places / 256]); rounded up or down at random, with bits that are a function of seed, step, `index` and the value's place in its tensor.  steps:
  * device array, steps[index] counts the tensor's steps.  lr_dev: device scalar to read the rate from, or NULL: lr.  clip_value < 0: no clipping.  copy:
- * receives p in copy_type (SPION_BF16 or SPION_F16), or NULL.  m and v on 32 bytes.  workspace: 16 * min(count, 512) bytes
+ * receives p in copy_type (SPION_BF16 or SPION_F16), or NULL.  m and v on 32 bytes.  workspace: 16 * min(count, 256) bytes
  * on 16, of the call's stream.  The table is read before the call returns. */
 typedef struct spion_adamw_tensor {
   void* p;

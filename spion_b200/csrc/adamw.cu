@@ -27,7 +27,7 @@ using namespace rows;
 namespace {
 
 constexpr int BLOCK = 256, CTA = 256, CHUNK = CTA / 32 * BLOCK;  // values that share scales; threads; values that a CTA takes at a time, a block per warp
-constexpr int FEW = 64, MOST = 512;                             // tensors of a launch
+constexpr int FEW = 64, MOST = 256;                             // tensors of a launch (a table of 512, 24 KB of parameters, cost 100 tensors 10 us on the host)
 
 struct Tensor {
   void* p;

@@ -81,7 +81,8 @@ __device__ __forceinline__ float row_scale(float top, float& scale) {
 // TPR threads to a row: 8 or 32 lanes of a warp, more: a CTA of that many.  Lanes take UR rows at a time, so that enough bytes are in flight.
 // NORM false: rows to e4m3 as they are (131072 x 64 bf16: 9.6 us with the sums and products of the norm left in, 8.7 without).
 template <bool NORM, class S, class R, class Y, int VEC, int NV, int TPR, int UR>
-__global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR, VEC == 8 && TPR == 8 && NV <= 2 ? 4 : 1) k_rms_forward(const FwdArgs a) {
+__global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR, VEC != 8 ? 1 : TPR == 8 && NV <= 2 ? 4 : TPR > 32 && NV == 4 ? 640 / TPR : 1) k_rms_forward(const FwdArgs a) {
+  next_may_start();                                                        // a linear layer on 8-bit rows prepares itself beside the last CTAs
   constexpr bool Q = type_code<Y>() == SPION_E4M3;
   constexpr int THREADS = TPR <= 32 ? CTA : TPR, RPC = THREADS / TPR, RPW = TPR <= 32 ? 32 / TPR : 1;      // rows of a CTA and of a warp
   __shared__ float2 part[2][32];

@@ -409,7 +409,7 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
   for (const Tensor* t : {&m, &v, &steps, &m_scale, &v_scale})
     if (t->defined() && t->numel()) written.push_back({(const char*)t->data_ptr(), (const char*)t->data_ptr() + t->numel() * t->element_size()});
   if (overlap(written)) refuse(op, "two of the tensors that the step writes share memory");
-  const Tensor ws = made(op, at::empty({4 * (int64_t)std::min<size_t>(table.size(), 512)}, like.options().dtype(at::kFloat)));
+  const Tensor ws = made(op, at::empty({4 * (int64_t)std::min<size_t>(table.size(), 256)}, like.options().dtype(at::kFloat)));
   check(spion_adamw_step(table.data(), (int)table.size(), type_code(type), bits8 ? 8 : 32, p(m), p(v), (float*)p(m_scale), (float*)p(v_scale), (float*)p(steps),
                          pf(lr_dev), h.lr, h.b1, h.b2, h.eps, h.wd, h.clip, h.seed, copy_type, p(ws), stream_of(like)),
         "spion_adamw_step");

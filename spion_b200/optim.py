@@ -62,7 +62,7 @@ class _Moments:
 
 
 class AdamW(torch.optim.Optimizer):
-    """``torch.optim.AdamW`` on the library's kernel: one launch per parameter group, type and device (512 tensors each).
+    """``torch.optim.AdamW`` on the library's kernel: one launch per parameter group, type and device (256 tensors each).
 
     ``state_bits=8``: moments in 8 bits with a scale per 256 values, 2 bytes a parameter instead of 8, rounded at random (repeatable: ``seed``).
     ``clip_value``: gradients are clipped to [-c, c] as they are read (``torch.nn.utils.clip_grad_value_``; ``.grad`` is left as it is).
