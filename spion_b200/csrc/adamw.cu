@@ -319,6 +319,7 @@ __global__ void __launch_bounds__(CTA + 32, RING_CTAS) k_adamw_ring(const __grid
   if (warp == CTA / 32) {
     if (lane != 0) return;
     bool ok = true;
+    long long fills = 0;
     for (int chunk = blockIdx.x; chunk < a.s.chunks && ok; chunk += gridDim.x) {
       i = tensor_of(a, chunk, i);
       const Tensor& t = a.t[i];
@@ -332,9 +333,13 @@ __global__ void __launch_bounds__(CTA + 32, RING_CTAS) k_adamw_ring(const __grid
       tc::bulk_load(to + R::VALUES, static_cast<const P*>(t.g) + begin, bar, R::VALUES);
       tc::bulk_load(to + 2 * R::VALUES, static_cast<const uint8_t*>(a.s.m) + t.at + begin, bar, CHUNK);
       tc::bulk_load(to + 2 * R::VALUES + CHUNK, static_cast<const uint8_t*>(a.s.v) + t.at + begin, bar, CHUNK);
+      ++fills;
       if (++st == RING_STAGES) st = 0, ph ^= 1;
     }
-    if (!ok) atomicOr(&g_adamw_status, 1);
+    if (!ok) {                                                             // the copies under way end first, or this gives up again
+      atomicOr(&g_adamw_status, 1);
+      for (long long j = fills > RING_STAGES ? fills - RING_STAGES : 0; j < fills; ++j) tc::mbar_wait(full + 8 * (int)(j % RING_STAGES), (int)(j / RING_STAGES) & 1);
+    }
     return;
   }
   bool waited = false;

@@ -166,6 +166,7 @@ __global__ void __launch_bounds__(L8_THREADS, CTAS) k_lin8(const __grid_constant
     if (warp == 0) {
       if (elect_one()) {
         int st = 0, ph = 1;                              // a ring that has not been used yet is empty
+        long long fills = 0;
         bool ok = true;
         for (int i = first; i < tiles && ok; i += step) {
           int m, n;
@@ -184,10 +185,15 @@ __global__ void __launch_bounds__(L8_THREADS, CTAS) k_lin8(const __grid_constant
               tma_load_2d(sbase + st * C::STAGE, &maps.x, full + 8 * st, c * BK, row);
               tma_load_2d(sbase + st * C::STAGE + C::A, &maps.w, full + 8 * st, c * BK, col);
             }
+            ++fills;
             if (++st == C::STAGES) st = 0, ph ^= 1;
           }
         }
-        if (!ok) report(&g_lin8_status, ERR_LOAD_WAIT);
+        if (!ok) {                                       // the copies under way end first (a pair's are counted in its first CTA), or this gives up again
+          report(&g_lin8_status, ERR_LOAD_WAIT);
+          for (long long j = fills > C::STAGES ? fills - C::STAGES : 0; j < fills && rank == 0; ++j)
+            mbar_wait(full + 8 * (int)(j % C::STAGES), (int)(j / C::STAGES) & 1);
+        }
       }
     } else if (warp == 1) {
       if (rank == 0 && elect_one()) {

@@ -14,7 +14,7 @@
 // threads of a row is a constant of each kernel, so a piece's place costs no arithmetic.
 //
 // Measured, of a copy's 6.54 TB/s: 32768 x 2048 bf16 + residual to e4m3 75 us (96 %); both directions: 131072 x 64 fp32 with bf16 branches 39 us (92 %), 8192 x
-// 4096 bf16 94 us (87 %), 4096 x 16384 bf16 181 us (90 %); by single elements 4099 x 769 fp32 21 us (37 %), 8192 x 2001 bf16 74 us (55 %): four and two bytes
+// 4096 bf16 89 us (92 %), 4096 x 16384 bf16 181 us (90 %); by single elements 4099 x 769 fp32 21 us (37 %), 8192 x 2001 bf16 74 us (55 %): four and two bytes
 // an access, and their addresses.  One row of 4096: 2.2 us, a launch.
 #include <algorithm>
 #include <atomic>
@@ -79,7 +79,7 @@ __device__ __forceinline__ float row_scale(float top, float& scale) {
 }
 
 // TPR threads to a row: 8 or 32 lanes of a warp, more: a CTA of that many.  Lanes take UR rows at a time, so that enough bytes are in flight.
-// NORM false: rows to e4m3 as they are (131072 x 64 bf16: 9.6 us with the sums and products of the norm left in, 8.7 without).
+// NORM false: rows to e4m3 as they are (131072 x 64 bf16: 9.6 us with the sums and products of the norm left in, 8.7 without, a launch among them: 6.5 in a row of calls).
 template <bool NORM, class S, class R, class Y, int VEC, int NV, int TPR, int UR>
 __global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR, VEC != 8 ? 1 : TPR == 8 && NV <= 2 ? 4 : TPR > 32 && NV == 4 ? 640 / TPR : 1) k_rms_forward(const FwdArgs a) {
   next_may_start();                                                        // a linear layer on 8-bit rows prepares itself beside the last CTAs
