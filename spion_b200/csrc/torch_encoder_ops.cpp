@@ -168,12 +168,12 @@ std::pair<Tensor, Tensor> rms_norm(const Tensor& x, const Tensor& w, double eps,
   Tensor s, y, rho;
   {
     Below below;
-    const Rows rx(x.detach());
-    const Tensor wc = w.detach().contiguous();
+    const Rows rx(x);
+    const Tensor wc = w.contiguous();
     y = made(op, at::empty(x.sizes(), x.options().dtype(type)));
     if (need) rho = at::empty({rx.M}, x.options().dtype(at::kFloat));
     if (res.has_value()) {
-      const Rows rr(res->detach());
+      const Rows rr(*res);
       s = at::empty(x.sizes(), x.options());
       check(spion_rmsnorm_forward(p(rx.t), rx.ld, type_code(x.scalar_type()), p(rr.t), rr.ld, type_code(res->scalar_type()), p(wc), type_code(wc.scalar_type()),
                                   p(s), p(y), rx.N, type_code(type), nullptr, (float*)p(rho), rx.M, (int)rx.N, (float)eps, 1, stream_of(x)),
@@ -220,13 +220,13 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_e4m3(const Tensor& x, const Tensor& 
   if (res.has_value()) no_gradient(op, *res);
   c10::cuda::CUDAGuard guard(x.device());
   Below below;
-  const Rows rx(x.detach());
-  const Tensor wc = w.detach().contiguous();
+  const Rows rx(x);
+  const Tensor wc = w.contiguous();
   const Rows8 q = empty_result(op, x, rx);
   Tensor s;
   const int64_t ld = (rx.N + 15) / 16 * 16;
   if (res.has_value()) {
-    const Rows rr(res->detach());
+    const Rows rr(*res);
     s = at::empty(x.sizes(), x.options());
     check(spion_rmsnorm_forward(p(rx.t), rx.ld, type_code(x.scalar_type()), p(rr.t), rr.ld, type_code(res->scalar_type()), p(wc), type_code(wc.scalar_type()), p(s),
                                 p(q.values), ld, SPION_E4M3, (float*)p(q.scales), nullptr, rx.M, (int)rx.N, (float)eps, 1, stream_of(x)),
@@ -244,7 +244,7 @@ Rows8 quantize_rows(const Tensor& x) {
   no_gradient(op, x);
   c10::cuda::CUDAGuard guard(x.device());
   Below below;
-  const Rows rx(x.detach());
+  const Rows rx(x);
   const Rows8 q = empty_result(op, x, rx);
   check(spion_rmsnorm_forward(p(rx.t), rx.ld, type_code(x.scalar_type()), nullptr, 0, 0, nullptr, 0, nullptr, p(q.values), (rx.N + 15) / 16 * 16, SPION_E4M3,
                               (float*)p(q.scales), nullptr, rx.M, (int)rx.N, 0.f, 0, stream_of(x)), "spion_rmsnorm_forward");
@@ -254,7 +254,9 @@ Rows8 quantize_rows(const Tensor& x) {
 // ------------------------------------------------------------------------------------------------ linear layer on 8-bit rows
 // Rows of bytes as the products read them: on 16-byte boundaries (a copy where they lie otherwise), scales one after another.
 struct Operand8 {
-  Tensor values, scales;
+  Tensor values, scales;                 // what keeps the memory
+  const void* p8 = nullptr;
+  const float* ps = nullptr;
   int64_t M = 0, N = 0, ld = 0;
   Operand8(const char* op, const Tensor& v, const Tensor& s, const char* name) {
     check_plain(op, v, name);
@@ -276,6 +278,22 @@ struct Operand8 {
       values = copy;
     }
     scales = s.contiguous();
+    p8 = p(values);
+    ps = pf(scales);
+  }
+  // rows in floating point, quantised here: scales and values in one piece of memory
+  Operand8(const char* op, const Tensor& x) {
+    check_rows(op, x, "x");
+    const Rows r(x);
+    M = r.M; N = r.N;
+    ld = (N + 15) / 16 * 16;
+    const int64_t at = (4 * M + 15) / 16 * 16;
+    values = made(op, at::empty({at + M * ld}, x.options().dtype(at::kByte)));
+    char* const base = (char*)p(values);
+    ps = (const float*)base;
+    p8 = base + at;
+    check(spion_rmsnorm_forward(p(r.t), r.ld, type_code(x.scalar_type()), nullptr, 0, 0, nullptr, 0, nullptr, base + at, ld, SPION_E4M3, (float*)base, nullptr, M, (int)N,
+                                0.f, 0, stream_of(x)), "spion_rmsnorm_forward");
   }
 };
 
@@ -283,27 +301,20 @@ struct Operand8 {
 Tensor linear_e4m3(const Tensor& x, const Tensor& x_scales, const Tensor& w, const Tensor& w_scales, const optional<Tensor>& bias,
                    const optional<at::ScalarType>& out_type) {
   const char* op = "linear_e4m3";
-  if (x.dim() < 1) refuse(op, "x has no dimension");
-  no_gradient(op, x);
-  if (x_scales.defined()) no_gradient(op, x_scales);
-  no_gradient(op, w); no_gradient(op, w_scales);
   check_plain(op, x, "x");
-  c10::cuda::CUDAGuard guard(x.device());
-  Below below;
-  Tensor xv = x.detach(), xs = x_scales;
-  if (!xs.defined()) {
-    check_rows(op, x, "x");
-    const Rows8 q = quantize_rows(xv);
-    xv = q.values; xs = q.scales;
-  }
+  if (x.dim() < 1) refuse(op, "x has no dimension");
+  no_gradient(op, x); no_gradient(op, w); no_gradient(op, w_scales);
+  if (x_scales.defined()) no_gradient(op, x_scales);
   const at::ScalarType type = out_type.value_or(x_scales.defined() ? at::kBFloat16 : x.scalar_type());
   if (!stream_type(type)) refuse(op, std::string("an output of type ") + c10::toString(type) + "; fp32, bf16 and fp16 are served");
   if (w.dim() != 2) refuse(op, "the weights have shape " + shape_of(w) + ": [features out, features in] is needed");
-  const Operand8 a(op, xv, xs.detach(), "x"), b(op, w.detach(), w_scales.detach(), "w");
+  if (w.size(0) < 1 || w.size(0) > 0x7fffffff / 2) refuse(op, "w has shape " + shape_of(w));
+  c10::cuda::CUDAGuard guard(x.device());
+  Below below;
+  const Operand8 b(op, w, w_scales, "w");
   same_device(op, w, x, "w");
-  if (a.N != b.N) refuse(op, "x has rows of " + std::to_string(a.N) + " features, w of " + std::to_string(b.N));
-  if (b.M < 1 || b.M > 0x7fffffff / 2) refuse(op, "w has shape " + shape_of(w));
-  if (a.M > 0x7fffffff / 2) refuse(op, "x has shape " + shape_of(x));
+  if (x.size(-1) != b.N) refuse(op, "x has rows of " + std::to_string(x.size(-1)) + " features, w of " + std::to_string(b.N));
+  if (x.numel() / x.size(-1) > 0x7fffffff / 2) refuse(op, "x has shape " + shape_of(x));
   Tensor bc;
   if (bias.has_value()) {
     no_gradient(op, *bias);
@@ -311,13 +322,14 @@ Tensor linear_e4m3(const Tensor& x, const Tensor& x_scales, const Tensor& w, con
     if (bias->dim() != 1 || bias->size(0) != b.M || !stream_type(bias->scalar_type()))
       refuse(op, "bias has shape " + shape_of(*bias) + " and type " + c10::toString(bias->scalar_type()) + ", w has " + shape_of(w));
     same_device(op, *bias, x, "bias");
-    bc = bias->detach().contiguous();
+    bc = bias->contiguous();
   }
+  const Operand8 a = x_scales.defined() ? Operand8(op, x, x_scales, "x") : Operand8(op, x);
   auto sizes = x.sizes().vec();
   sizes.back() = b.M;
   Tensor y = made(op, at::empty(sizes, x.options().dtype(type)));
-  check(spion_linear_e4m3(p(a.values), a.ld, pf(a.scales), p(b.values), b.ld, pf(b.scales), p(bc), bc.defined() ? type_code(bc.scalar_type()) : SPION_F32, p(y),
-                          b.M, type_code(type), a.M, (int)a.N, (int)b.M, stream_of(x)), "spion_linear_e4m3");
+  check(spion_linear_e4m3(a.p8, a.ld, a.ps, b.p8, b.ld, b.ps, p(bc), bc.defined() ? type_code(bc.scalar_type()) : SPION_F32, p(y), b.M, type_code(type), a.M,
+                          (int)a.N, (int)b.M, stream_of(x)), "spion_linear_e4m3");
   return y;
 }
 
@@ -336,7 +348,7 @@ void check_flat(const char* op, const Tensor& t, const char* name, at::ScalarTyp
            " contiguous values of type " + c10::toString(type) + " are needed");
 }
 bool overlap(std::vector<std::pair<const char*, const char*>>& spans) {      // [begin, end)
-  std::sort(spans.begin(), spans.end());
+  if (!std::is_sorted(spans.begin(), spans.end())) std::sort(spans.begin(), spans.end());
   for (size_t i = 1; i < spans.size(); ++i)
     if (spans[i].first < spans[i - 1].second) return true;
   return false;
@@ -362,6 +374,7 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
   std::vector<Tensor> held;                                // gradients that had to be copied
   std::vector<std::pair<const char*, const char*>> written;
   table.reserve(params.size());
+  written.reserve(params.size() + 8);
   int64_t at = 0;
   int copy_type = -1;
   for (size_t i = 0; i < params.size(); ++i) {
