@@ -553,6 +553,8 @@ template <class Y> int launch_any(const Lin8Args& a, cudaStream_t st) {
   // 4096 to 4096 features, few / tiles: 8 tokens 6.1 us / 11.6, 16 tokens (twice the products) 10.4 / 11.6; 512 to 16384, 32 tokens 26 / 6.3: mma.sync is slow on
   // 8-bit operands here, and what it does for more tokens outlasts the weights
   if (a.T <= FEW_TOKENS) return launch_few<Y>(a, st);
+  // The largest tile that leaves one to every multiprocessor.  Two small CTAs a multiprocessor up to 256 inner features, else pairs; two small / pairs: 65536 x
+  // 512 to 256 16.4 us / 18.2, to 1024 52.4 / 51.3, 32768 x 1024 to 1024 44.6 / 35.9, 16384 x 2048 to 2048 73 / 53.
   const long long rows_ = (a.T + 127) / 128, sms = sm_count();
   const bool wide = a.N > 64 && rows_ * ((a.N + 127) / 128) >= sms;
   if (a.K <= 64) return wide ? launch_tiles<128, 64, 2, false, Y>(a, st) : launch_tiles<64, 64, 2, false, Y>(a, st);

@@ -84,9 +84,12 @@ struct Below {                           // what happens inside is not recorded
   at::AutoDispatchBelowADInplaceOrView below;
   c10::impl::ExcludeDispatchKeyGuard no_autocast{c10::autocast_dispatch_keyset};
 };
-// Rows of bytes that start on 16: [.., N] of a buffer [M, N rounded up]
+// Rows of bytes start on 32, a sector of memory: tensor maps ask for 16, which costs them every box's rows a sector more (65536 x 272 to 256: 20.0 us, 65536 x
+// 288: 17.2; 112 and 96 14.7, 11.8).
+int64_t row8_stride(int64_t N) { return (N + 31) / 32 * 32; }
+// [.., N] of a buffer [M, N rounded up]
 Tensor empty_rows8(const Tensor& x, int64_t M, int64_t N) {
-  const int64_t ld = (N + 15) / 16 * 16;
+  const int64_t ld = row8_stride(N);
   Tensor t = at::empty({M, ld}, x.options().dtype(at::kFloat8_e4m3fn));
   return ld == N ? t : t.narrow(1, 0, N);
 }
@@ -224,7 +227,7 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_e4m3(const Tensor& x, const Tensor& 
   const Tensor wc = w.contiguous();
   const Rows8 q = empty_result(op, x, rx);
   Tensor s;
-  const int64_t ld = (rx.N + 15) / 16 * 16;
+  const int64_t ld = row8_stride(rx.N);
   if (res.has_value()) {
     const Rows rr(*res);
     s = at::empty(x.sizes(), x.options());
@@ -246,7 +249,7 @@ Rows8 quantize_rows(const Tensor& x) {
   Below below;
   const Rows rx(x);
   const Rows8 q = empty_result(op, x, rx);
-  check(spion_rmsnorm_forward(p(rx.t), rx.ld, type_code(x.scalar_type()), nullptr, 0, 0, nullptr, 0, nullptr, p(q.values), (rx.N + 15) / 16 * 16, SPION_E4M3,
+  check(spion_rmsnorm_forward(p(rx.t), rx.ld, type_code(x.scalar_type()), nullptr, 0, 0, nullptr, 0, nullptr, p(q.values), row8_stride(rx.N), SPION_E4M3,
                               (float*)p(q.scales), nullptr, rx.M, (int)rx.N, 0.f, 0, stream_of(x)), "spion_rmsnorm_forward");
   return q;
 }
@@ -270,9 +273,9 @@ struct Operand8 {
     const Rows r(v);
     M = r.M; N = r.N;
     values = r.t;
-    ld = M > 1 ? r.ld : (N + 15) / 16 * 16;
+    ld = M > 1 ? r.ld : row8_stride(N);
     if (M > 0 && (((uintptr_t)values.data_ptr() | (uintptr_t)ld) % 16 != 0 || ld < N)) {
-      ld = (N + 15) / 16 * 16;
+      ld = row8_stride(N);
       Tensor copy = empty_rows8(v, M, N);
       copy.copy_(values.view({M, N}));
       values = copy;
@@ -286,8 +289,8 @@ struct Operand8 {
     check_rows(op, x, "x");
     const Rows r(x);
     M = r.M; N = r.N;
-    ld = (N + 15) / 16 * 16;
-    const int64_t at = (4 * M + 15) / 16 * 16;
+    ld = row8_stride(N);
+    const int64_t at = (4 * M + 31) / 32 * 32;
     values = made(op, at::empty({at + M * ld}, x.options().dtype(at::kByte)));
     char* const base = (char*)p(values);
     ps = (const float*)base;

@@ -19,9 +19,9 @@ shapes = ((5, 64, 128), (8192, 1024, 1024), (40000, 64, 128), (300, 512, 96))
 xs = [torch.randn(T, K, device="cuda", requires_grad=True) for T, K, N in shapes] + [torch.randn(600, 2048, device="cuda", requires_grad=True)]
 ws = [torch.randn(N, K, device="cuda") for T, K, N in shapes]
 g = torch.ones(2048, device="cuda", requires_grad=True)
-p, d = torch.randn(8_000_000, device="cuda"), torch.randn(8_000_000, device="cuda")
-m, v = torch.zeros(8_000_000, device="cuda").to(torch.float8_e4m3fn), torch.zeros(8_000_000, device="cuda").to(torch.float8_e5m2)
-scales, steps = (torch.ones(31250, device="cuda"), torch.ones(31250, device="cuda")), torch.zeros(1, device="cuda")
+p, d = torch.randn(16_000_000, device="cuda"), torch.randn(16_000_000, device="cuda")
+m, v = torch.zeros(16_000_000, device="cuda").to(torch.float8_e4m3fn), torch.zeros(16_000_000, device="cuda").to(torch.float8_e5m2)
+scales, steps = (torch.ones(62500, device="cuda"), torch.ones(62500, device="cuda")), torch.zeros(1, device="cuda")
 dy = torch.randn(600, 2048, device="cuda")
 
 def all_of_them():
@@ -80,7 +80,7 @@ def test_two_streams_at_once():
     from spion_b200.rmsnorm import rms_norm
     x = torch.randn(8192, 1024, device="cuda")
     q, w, g = quantize_rows(x), quantize_rows(torch.randn(2048, 1024, device="cuda")), torch.ones(1024, device="cuda")
-    n = 9_000_000
+    n = 16_000_000
 
     def state():
         return (torch.ones(n, device="cuda"), torch.full((n,), 0.5, device="cuda"), torch.zeros(-(-n // 256) * 256, device="cuda"),

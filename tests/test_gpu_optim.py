@@ -176,13 +176,13 @@ def test_more_tensors_than_a_launch_takes(bits):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_many_values(dtype):
     """Enough of them for the kernel that copies ahead: tensors that end inside a chunk, small ones, one without a gradient; and tensors off their boundaries."""
-    check_step([3_000_001, 77, 2048, 4_600_000, 0, 5, 70_000], dtype, 8, clip=0.5, none=(6,))
-    check_step([7_400_003, 300], dtype, 8, offset=1)
+    check_step([6_000_001, 77, 2048, 9_200_000, 0, 5, 70_000], dtype, 8, clip=0.5, none=(6,))
+    check_step([14_800_003, 300], dtype, 8, offset=1)
 
 
 def test_values_that_are_not_finite_stay_where_they_are():
     from spion_b200.optim import adamw_step
-    for bits, n in ((32, 1000), (8, 1000), (8, 7_500_000)):
+    for bits, n in ((32, 1000), (8, 1000), (8, 15_000_000)):
         ps, gs, m, v, scales, _ = make([n], torch.float32, bits, 1)
         v.copy_(torch.where(torch.isfinite(v.float()), v.float(), 1.0).to(v.dtype))
         gs[0][10], gs[0][700] = float("nan"), float("inf")
