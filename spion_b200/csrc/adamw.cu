@@ -462,7 +462,10 @@ int launches(const Step& s, const Begin& b, const spion_adamw_tensor* ts, int co
 
 }  // namespace
 
-int adamw_status(int reset, cudaStream_t st) { return device_word_status(&g_adamw_status, "optimizer", reset, st); }
+int* adamw_status_word() {
+  void* word = nullptr;
+  return cudaGetSymbolAddress(&word, g_adamw_status) == cudaSuccess ? static_cast<int*>(word) : nullptr;
+}
 
 extern "C" int spion_adamw_step(const spion_adamw_tensor* host_tensors, int count, int type, int state_bits, void* m, void* v, float* m_scale,
                                 float* v_scale, float* steps, const float* lr_dev, double lr, double beta1, double beta2, double eps,

@@ -147,25 +147,11 @@ int sm_count();
 
 // linear.cu: status word of the linear layers on the current device, after the work of a stream
 int linear_status(int reset, cudaStream_t st);
-// linear_e4m3.cu, rmsnorm.cu, adamw.cu: those of the layers on 8-bit operands, of the norm's backward and of the optimizer (reported with the former)
-int linear_e4m3_status(int reset, cudaStream_t st);
-int rmsnorm_status(int reset, cudaStream_t st);
-int adamw_status(int reset, cudaStream_t st);
-// a status word (a __device__ int) on the current device, after the work of a stream
-template <class T> inline int device_word_status(T* symbol, const char* whose, int reset, cudaStream_t st) {
-  int v = 0;
-  void* word = nullptr;
-  SPION_CUDA_TRY(cudaGetSymbolAddress(&word, *symbol));
-  SPION_CUDA_TRY(cudaMemcpyAsync(&v, word, sizeof(int), cudaMemcpyDeviceToHost, st));
-  SPION_CUDA_TRY(cudaStreamSynchronize(st));
-  if (v == 0) return SPION_OK;
-  if (reset) {
-    SPION_CUDA_TRY(cudaMemsetAsync(word, 0, sizeof(int), st));
-    SPION_CUDA_TRY(cudaStreamSynchronize(st));
-  }
-  fprintf(stderr, "spion_b200: status word of the %s = 0x%x (a bounded wait gave up)\n", whose, v);
-  return SPION_ERR_TIMEOUT;
-}
+// linear_e4m3.cu, rmsnorm.cu, adamw.cu: where those of the layers on 8-bit operands, of the norm's backward and of the optimizer lie (null: the query failed);
+// reported with the former
+int* linear_e4m3_status_word();
+int* rmsnorm_status_word();
+int* adamw_status_word();
 
 // Device memory of the contexts, from one pool per device that keeps up to 64 MB of what was given back, beside what is in use: mapping
 // and unmapping two or three megabytes took 2 to 4 ms of every context's life.  Freeing waits for the device, as cudaFree does (where it

@@ -1606,21 +1606,26 @@ extern "C" int spion_linear_prepare(int fp32) {
 }
 
 int linear_status(int reset, cudaStream_t st) {
-  int v = 0;
-  SPION_CUDA_TRY(cudaMemcpyFromSymbolAsync(&v, g_lin_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
-  SPION_CUDA_TRY(cudaStreamSynchronize(st));
-  int others = SPION_OK;
-  for (int rc : {linear_e4m3_status(reset, st), rmsnorm_status(reset, st), adamw_status(reset, st)})
-    if (others == SPION_OK) others = rc;
-  if (v == 0) return others;
-  if (reset) {
-    void* word = nullptr;
-    SPION_CUDA_TRY(cudaGetSymbolAddress(&word, g_lin_status));
-    SPION_CUDA_TRY(cudaMemsetAsync(word, 0, sizeof(int), st));
-    SPION_CUDA_TRY(cudaStreamSynchronize(st));
+  static const char* const whose[] = {"linear layers", "8-bit linear layers", "root-mean-square norm", "optimizer"};
+  void* mine = nullptr;
+  SPION_CUDA_TRY(cudaGetSymbolAddress(&mine, g_lin_status));
+  int* const words[] = {static_cast<int*>(mine), linear_e4m3_status_word(), rmsnorm_status_word(), adamw_status_word()};
+  int v[4] = {0, 0, 0, 0}, rc = SPION_OK;
+  for (int i = 0; i < 4; ++i) {
+    if (words[i] == nullptr) return SPION_ERR_CUDA;
+    SPION_CUDA_TRY(cudaMemcpyAsync(&v[i], words[i], sizeof(int), cudaMemcpyDeviceToHost, st));
   }
-  fprintf(stderr, "spion_b200: status word of the linear layers = 0x%x (a bounded wait gave up)\n", v);
-  return SPION_ERR_TIMEOUT;
+  SPION_CUDA_TRY(cudaStreamSynchronize(st));
+  for (int i = 0; i < 4; ++i) {
+    if (v[i] == 0) continue;
+    if (reset) {
+      SPION_CUDA_TRY(cudaMemsetAsync(words[i], 0, sizeof(int), st));
+      SPION_CUDA_TRY(cudaStreamSynchronize(st));
+    }
+    fprintf(stderr, "spion_b200: status word of the %s = 0x%x (a bounded wait gave up)\n", whose[i], v[i]);
+    rc = SPION_ERR_TIMEOUT;
+  }
+  return rc;
 }
 
 extern "C" int spion_linear_status(int reset) {

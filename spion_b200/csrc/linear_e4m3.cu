@@ -565,8 +565,10 @@ template <class Y> int launch_any(const Lin8Args& a, cudaStream_t st) {
 
 }  // namespace
 
-// Status word of these kernels on the current device, after the work of a stream (linear.cu reports it with its own)
-int linear_e4m3_status(int reset, cudaStream_t st) { return device_word_status(&g_lin8_status, "8-bit linear layers", reset, st); }
+int* linear_e4m3_status_word() {
+  void* word = nullptr;
+  return cudaGetSymbolAddress(&word, g_lin8_status) == cudaSuccess ? static_cast<int*>(word) : nullptr;
+}
 
 extern "C" int spion_linear_e4m3(const void* x, long long ldx, const float* x_scale, const void* w, long long ldw, const float* w_scale, const void* bias,
                                  int bias_type, void* y, long long ldy, int y_type, long long T, int K, int N, void* cuda_stream) {

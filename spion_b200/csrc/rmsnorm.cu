@@ -685,8 +685,10 @@ bool stream_type(int t) { return t == SPION_F32 || t == SPION_BF16 || t == SPION
 
 }  // namespace
 
-// Status word of the norm's backward on the current device, after the work of a stream (linear.cu reports it with its own)
-int rmsnorm_status(int reset, cudaStream_t st) { return device_word_status(&g_rms_status, "root-mean-square norm", reset, st); }
+int* rmsnorm_status_word() {
+  void* word = nullptr;
+  return cudaGetSymbolAddress(&word, g_rms_status) == cudaSuccess ? static_cast<int*>(word) : nullptr;
+}
 
 extern "C" {
 
