@@ -65,6 +65,8 @@ def _load_shim(name, n_init, n_fwd, n_bwd, trailing_int):
 
 
 class Attention(nn.Module):
+    linear8 = None                                # the projections in 8 bits (quantize)
+
     def __init__(self, config, inference=False):
         super().__init__()
         self.inference = inference
@@ -101,7 +103,6 @@ class Attention(nn.Module):
             self.attn = Dense(config, attn_cpp, attn_handle)
 
         self.ff = Linear(self.num_head * self.head_dim, self.dim)
-        self.linear8 = None
         if torch.cuda.is_available():
             _lib.check(_lib.lib.spion_linear_prepare(int(self.native_dtype == torch.float32)), "spion_linear_prepare")
 

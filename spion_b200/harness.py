@@ -78,6 +78,8 @@ class Embeddings(nn.Module):
 
 
 class TransformerLayer(nn.Module):
+    mlp8 = None                                   # the feed-forward block's layers in 8 bits (quantize)
+
     def __init__(self, config):
         super().__init__()
         dim, hid, p = config["transformer_dim"], config["transformer_hidden_dim"], config["dropout_prob"]
@@ -90,7 +92,6 @@ class TransformerLayer(nn.Module):
             from .layernorm import BiasGradLinear as Linear
         self.mlp_types = (Linear, nn.GELU, nn.Dropout, Linear, nn.Dropout)
         self.fuse_mlp = Linear is not nn.Linear
-        self.mlp8 = None
         self.mlpblock = nn.Sequential(Linear(dim, hid), nn.GELU(), nn.Dropout(p), Linear(hid, dim), nn.Dropout(p))
 
     def forward(self, X, mask, mat=None):
@@ -160,6 +161,8 @@ def norm_rows8(norm, x, res=None):
 
 
 class Encoder(nn.Module):
+    quantized = False                             # evaluate on 8-bit operands (Classifier.quantize)
+
     def __init__(self, config):
         super().__init__()
         self.embeddings = Embeddings(config)
@@ -168,7 +171,6 @@ class Encoder(nn.Module):
         from .layernorm import FusedLayerNorm
         from .rmsnorm import FusedRMSNorm
         self.add_norm = bool(config.get("fused_add_norm", True)) and isinstance(self.norm, (FusedLayerNorm, FusedRMSNorm))
-        self.quantized = False
 
     def forward(self, ids, mask, mat_lst=None, is_attn=False):
         from .pattern import mean_attention_map

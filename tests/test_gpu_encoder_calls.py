@@ -74,6 +74,20 @@ def test_recomputed_segments_and_hooks_on_saved_tensors():
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
+def test_the_same_tensor_as_stream_and_residual():
+    from spion_b200.rmsnorm import rms_norm
+    for dtype in (torch.float32, torch.bfloat16):
+        x, w = torch.randn(30, 128, device="cuda", dtype=dtype, requires_grad=True), torch.ones(128, device="cuda", requires_grad=True)
+        z = x.detach().clone().requires_grad_()
+        s, y = rms_norm(x, w, res=x)
+        t, u = rms_norm(z, w, res=z.detach())
+        assert torch.equal(s, t) and torch.equal(y, u)
+        ds, dy = torch.randn_like(s), torch.randn_like(y)
+        one, = torch.autograd.grad((t, u), z, (ds, dy))
+        both, = torch.autograd.grad((s, y), x, (ds, dy))
+        assert torch.equal(both, one + one)
+
+
 def test_two_streams_at_once():
     from spion_b200.optim import adamw_step
     from spion_b200.quant import linear_e4m3, quantize_rows
