@@ -1,4 +1,4 @@
-// One AdamW step over many tensors in one launch (decoupled weight decay), with first and second moments in 32 or in 8 bits.
+// One AdamW step over many tensors in one launch, and a small one before it (decoupled weight decay), with first and second moments in 32 or in 8 bits.
 //
 //   t += 1;  g = clamp(g, -c, c);  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
 //   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)

@@ -1,6 +1,5 @@
-// Host path of the encoder's operators around the attention call: root-mean-square norm, rows in e4m3,
-// linear layer on them, optimizer.  Each call checks what it is given, allocates
-// its results and calls the C ABI; the norm is an autograd node of its own.
+// Host path of the encoder's operators around the attention call: root-mean-square norm, rows in e4m3, linear layer on them, optimizer.  Each call checks
+// what it is given, allocates its results and calls the C ABI; the norm is an autograd node of its own.
 #include <algorithm>
 #include <mutex>
 
