@@ -497,7 +497,7 @@ int spion_rmsnorm_backward(const void* s, long long lds, int s_type, const void*
 /* ------------------------------------------------------------------------------------------
  * Linear layer on 8-bit operands: y[t, n] = (sum_k x[t, k] w[n, k]) x_scale[t] w_scale[n] + bias[n].  x [T, K] and w [N, K] in e4m3, rows on 16-byte
  * boundaries (ldx, ldw multiples of 16, >= K; what lies between K and the next row is not read), scales fp32, bias (may be NULL) and y [T, N] SPION_F32,
- * SPION_BF16 or SPION_F16 (rows of y ldy >= N apart; on 16-byte boundaries they are written faster).  Sums in fp32.  A bounded wait that gives up is
+ * SPION_BF16 or SPION_F16 (rows of y ldy >= N apart; rows that begin and end on 16-byte boundaries are written faster).  Sums in fp32.  A bounded wait that gives up is
  * reported by spion_linear_status. */
 int spion_linear_e4m3(const void* x, long long ldx, const float* x_scale, const void* w, long long ldw, const float* w_scale, const void* bias,
                       int bias_type, void* y, long long ldy, int y_type, long long T, int K, int N, void* cuda_stream);

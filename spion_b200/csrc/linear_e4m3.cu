@@ -506,7 +506,8 @@ template <int BN, int BK, int CTAS, bool PAIR, class Y> int launch_tiles(Lin8Arg
   a.tiles_m = (a.T + C::TOKENS - 1) / C::TOKENS;
   a.tiles_n = (a.N + BN - 1) / BN;
   if ((long long)a.tiles_m * a.tiles_n > 0x7fffffff) return SPION_ERR_SHAPE;
-  a.staged = ((uintptr_t)a.y % 16 == 0) && (a.ldy * (long long)sizeof(Y)) % 16 == 0;
+  // (a store ends on a piece of 16 bytes: of a row that ends inside one it would write zeros behind the row)
+  a.staged = ((uintptr_t)a.y % 16 == 0) && (a.ldy * (long long)sizeof(Y)) % 16 == 0 && (a.N * (long long)sizeof(Y)) % 16 == 0;
   Lin8Maps maps;
   if ((rc = map_of(&maps.x, encode, a.x, SPION_E4M3, a.K, a.T, a.ldx, BK, 128)) != SPION_OK) return rc;
   if ((rc = map_of(&maps.w, encode, a.w, SPION_E4M3, a.K, a.N, a.ldw, BK, C::FEATURES)) != SPION_OK) return rc;

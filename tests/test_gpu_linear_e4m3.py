@@ -176,3 +176,23 @@ def test_what_it_refuses():
     refused("gradient", torch.randn(4, 64, device="cuda", requires_grad=True), w)
     refused("gradient", x, w, torch.zeros(20, device="cuda", requires_grad=True))
     refused("weights", x, Rows8(w.values[0], w.scales[0]))
+
+
+@pytest.mark.parametrize("T", [1, 7, 8, 9, 100, 128, 129, 257])
+@pytest.mark.parametrize("K,N", [(40, 50), (40, 64), (300, 130), (1000, 333), (512, 520)])
+def test_nothing_is_written_outside_of_the_result(T, K, N):
+    """Results into a larger matrix, rows further apart than they are long and from any element on: what lies around them stays."""
+    from spion_b200 import _lib
+    from spion_b200.quant import linear_e4m3
+    g = torch.Generator(device="cuda").manual_seed(T + K + N)
+    x, w = rows8(T, K, g), rows8(N, K, g)
+    for dtype, code in ((torch.float32, _lib.F32), (torch.bfloat16, _lib.BF16), (torch.float16, _lib.F16)):
+        want = linear_e4m3(x, w, out_dtype=dtype)
+        for ld, first in ((-(-N // 8) * 8 + 16, 64), (N + 3, 64), (N, 65), (N + 1, 3)):
+            buf = torch.full((first + (T + 2) * ld + 64,), 7.0, dtype=dtype, device="cuda")
+            expect = buf.clone()
+            expect[first:].as_strided((T, N), (ld, 1)).copy_(want)
+            _lib.check(_lib.lib.spion_linear_e4m3(x.values.data_ptr(), x.values.stride(0) if T > 1 else -(-K // 32) * 32, x.scales.data_ptr(), w.values.data_ptr(),
+                                                  w.values.stride(0), w.scales.data_ptr(), None, _lib.F32, buf[first:].data_ptr(), ld, code, T, K, N,
+                                                  torch.cuda.current_stream().cuda_stream))
+            assert torch.equal(buf, expect)
