@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR, VEC != 8 ? 1 : TPR == 8
         if (NORM) {
           sum = fmaf(v[u][i], v[u][i], sum);
           v[u][i] *= w[i];
-          if (Q) top = fmaxf(top, fabsf(v[u][i]));
+          if (Q) top = max_nan(top, fabsf(v[u][i]));      // (a NaN may be the weight's: the sum does not see it)
         } else {
           top = max_nan(top, fabsf(v[u][i]));
         }
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(TPR <= 32 ? CTA : TPR, VEC != 8 ? 1 : TPR == 8
       if (NORM) {
         row_reduce<TPR, Q>(sum, top, part, buf);
         rho = rsqrtf(fmaf(sum, over_n, a.eps));
-        top *= rho;                                      // NaN where the sum is
+        top *= rho;
       } else {
         row_max_nan<TPR>(top, part, buf);
       }

@@ -141,20 +141,6 @@ template <int LANES> __device__ __forceinline__ float lane_max(float v) {
   for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-template <int TPR, bool MAX> __device__ __forceinline__ void row_reduce(float& sum, float& top, float2 (*part)[32], int& buf) {
-  constexpr int LANES = TPR < 32 ? TPR : 32, WARPS = TPR / 32;
-  sum = lane_sum<LANES>(sum);
-  if (MAX) top = lane_max<LANES>(top);
-  if (TPR <= 32) return;
-  if ((threadIdx.x & 31) == 0) part[buf][threadIdx.x >> 5] = make_float2(sum, top);
-  __syncthreads();
-  const float2 t = (int)(threadIdx.x & 31) < WARPS ? part[buf][threadIdx.x & 31] : make_float2(0.f, 0.f);
-  constexpr int UP = WARPS <= 2 ? 2 : WARPS <= 4 ? 4 : WARPS <= 8 ? 8 : WARPS <= 16 ? 16 : 32;
-  sum = __shfl_sync(0xffffffffu, lane_sum<UP>(t.x), 0);
-  if (MAX) top = __shfl_sync(0xffffffffu, lane_max<UP>(t.y), 0);
-  buf ^= 1;
-}
-
 // the largest, NaN if one is
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
@@ -165,6 +151,19 @@ template <int LANES> __device__ __forceinline__ float lane_max_nan(float v) {
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
+}
+template <int TPR, bool MAX> __device__ __forceinline__ void row_reduce(float& sum, float& top, float2 (*part)[32], int& buf) {
+  constexpr int LANES = TPR < 32 ? TPR : 32, WARPS = TPR / 32;
+  sum = lane_sum<LANES>(sum);
+  if (MAX) top = lane_max_nan<LANES>(top);
+  if (TPR <= 32) return;
+  if ((threadIdx.x & 31) == 0) part[buf][threadIdx.x >> 5] = make_float2(sum, top);
+  __syncthreads();
+  const float2 t = (int)(threadIdx.x & 31) < WARPS ? part[buf][threadIdx.x & 31] : make_float2(0.f, 0.f);
+  constexpr int UP = WARPS <= 2 ? 2 : WARPS <= 4 ? 4 : WARPS <= 8 ? 8 : WARPS <= 16 ? 16 : 32;
+  sum = __shfl_sync(0xffffffffu, lane_sum<UP>(t.x), 0);
+  if (MAX) top = __shfl_sync(0xffffffffu, lane_max_nan<UP>(t.y), 0);
+  buf ^= 1;
 }
 template <int TPR> __device__ __forceinline__ void row_max_nan(float& top, float2 (*part)[32], int& buf) {
   top = lane_max_nan<(TPR < 32 ? TPR : 32)>(top);

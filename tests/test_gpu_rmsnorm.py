@@ -303,3 +303,26 @@ def test_module_beside_the_framework():
         assert s.dtype == torch.float32 and y.dtype == torch.bfloat16
     assert mod(x).dtype == torch.float32
     assert mod.add_norm(x.half(), x)[1].dtype == torch.float16
+
+
+@pytest.mark.parametrize("N", [1, 40, 64, 136, 333, 512, 1000, 2048, 4096, 5001, 16384, 17000, 20001])
+def test_weights_that_are_not_finite(N):
+    """A NaN of the weight, or an infinite weight times zero, is a NaN in every row: in 8 bits nothing of such a row comes back finite, in other types that
+    column alone.  An infinite y has an infinite scale, NaN in its place and zeros in the others, as the definition gives."""
+    from spion_b200.rmsnorm import rms_norm, rms_norm_e4m3
+    for M in (3, 300):
+        for bad in (float("nan"), float("inf"), -float("inf")):
+            x = torch.randn(M, N, device="cuda") + 3
+            w = torch.ones(N, device="cuda")
+            x[1, N // 2], w[N // 2] = 0, bad
+            for res in (None, torch.zeros_like(x)):
+                out = rms_norm_e4m3(x, w, EPS, res=res)
+                q = out if res is None else out[1]
+                y = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + EPS) * w
+                a = y.abs().amax(1)
+                want = (y * (448.0 / a)[:, None]).to(torch.float8_e4m3fn).float()
+                assert torch.equal(q.scales.isnan(), a.isnan()) and torch.equal(q.scales.isinf(), a.isinf()) and bool(a.isnan()[1])
+                assert torch.equal(q.values.float().nan_to_num(7.0), want.nan_to_num(7.0))
+                z = rms_norm(x, w, EPS, res=res)
+                z = z if res is None else z[1]
+                assert torch.equal(z.isnan(), y.isnan()) and torch.equal(z.isinf(), y.isinf())
