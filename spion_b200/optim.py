@@ -79,7 +79,7 @@ class AdamW(torch.optim.Optimizer):
         if clip_value is not None and not clip_value >= 0:
             raise ValueError(f"AdamW: clip_value is {clip_value}")
         self.state_bits, self.seed = state_bits, seed
-        self._moments, self._copies = {}, {}
+        self._moments, self._copies = [], {}             # of each group that has taken a step: its parameters, their arrays by type and device
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, clip_value=clip_value))
 
     def __getstate__(self):                     # copies of the optimizer keep their arrays (the base class would keep the views only)
@@ -90,26 +90,27 @@ class AdamW(torch.optim.Optimizer):
         for p, c in zip(params, copies, strict=True):
             self._copies[p] = c
 
-    def _sets(self, g, make=True):
-        """The moments of group number g, made at the first step (or when a state is loaded)."""
+    def _sets(self, g):
+        """The moments of group number g, made at its first step (or when a state is loaded).  They belong to its parameters, not to its place among the groups."""
         params = self.param_groups[g]["params"]
-        have = self._moments.get(g)
-        if have is None or sum(len(m.params) for m in have) != len(params):
-            if not make:
-                return []
-            if have is not None:
-                raise SpionError(f"AdamW: the parameters of group {g} have changed since its first step")
-            kinds = {}
-            for p in params:
-                if not p.is_cuda:
-                    raise SpionError("AdamW: a parameter is not on a GPU (there is no CPU path)")
-                kinds.setdefault((p.dtype, p.device), []).append(p)
-            if torch.cuda.is_current_stream_capturing():
-                raise SpionError("AdamW: take a step before one is captured (the moments would be made anew by every replay)")
-            have = self._moments[g] = [_Moments(ps, self.state_bits) for ps in kinds.values()]
-            for m in have:
-                for i, p in enumerate(m.params):
-                    self.state[p] = m.state_of(i)
+        ids = [id(p) for p in params]                    # (of tensors that self._moments keeps)
+        for held, have in self._moments:
+            if [id(p) for p in held] == ids:
+                return have
+        if any(p in self.state for p in params):
+            raise SpionError(f"AdamW: the parameters of group {g} have changed since its first step")
+        kinds = {}
+        for p in params:
+            if not p.is_cuda:
+                raise SpionError("AdamW: a parameter is not on a GPU (there is no CPU path)")
+            kinds.setdefault((p.dtype, p.device), []).append(p)
+        if torch.cuda.is_current_stream_capturing():
+            raise SpionError("AdamW: take a step before one is captured (the moments would be made anew by every replay)")
+        have = [_Moments(ps, self.state_bits) for ps in kinds.values()]
+        self._moments.append((list(params), have))
+        for m in have:
+            for i, p in enumerate(m.params):
+                self.state[p] = m.state_of(i)
         return have
 
     @torch.no_grad()

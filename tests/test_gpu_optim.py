@@ -384,3 +384,53 @@ def test_gradients_with_other_strides_and_another_stream():
     adamw_step([w], [torch.ones(8, device="cuda")], m, v, steps[:1])
     with pytest.raises(RuntimeError, match="modified"):
         y.backward()
+
+
+def test_steps_follow_the_parameter_groups():
+    """A group that leaves or moves takes its moments along; a parameter put in another's place starts anew, as torch's; groups mixed anew are refused."""
+    from spion_b200._lib import SpionError
+    from spion_b200.optim import AdamW
+    tensors = lambda: [torch.nn.Parameter(torch.full((300,), 1.0 + k, device="cuda")) for k in range(3)]      # noqa: E731
+
+    def both(call):
+        out = []
+        for make in (lambda ps: AdamW([{"params": [p]} for p in ps], lr=1e-2), lambda ps: torch.optim.AdamW([{"params": [p]} for p in ps], lr=1e-2)):
+            ps = tensors()
+            opt = make(ps)
+            for k in range(2):
+                for p in ps:
+                    p.grad = torch.full_like(p, 0.1 * (k + 1))
+                opt.step()
+            ps = call(opt, ps)
+            for p in ps:
+                p.grad = torch.full_like(p, -0.2)
+            opt.step()
+            out.append([p.detach().clone() for p in ps])
+        for a, b in zip(*out):
+            assert float((a - b).abs().max()) <= 3 * (32 * U * 1e-2 + 4 * U)
+
+    def removed(opt, ps):
+        del opt.param_groups[0]
+        return ps
+
+    def reordered(opt, ps):
+        opt.param_groups.reverse()
+        return ps
+
+    def replaced(opt, ps):
+        new = torch.nn.Parameter(torch.full((300,), 7.0, device="cuda"))
+        opt.param_groups[1]["params"] = [new]
+        return [*ps, new]
+
+    for change in (removed, reordered, replaced):
+        both(change)
+    ps = tensors()
+    opt = AdamW(ps)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    before = [p.detach().clone() for p in ps]
+    opt.param_groups[0]["params"] = [ps[0], torch.nn.Parameter(torch.zeros(300, device="cuda")), ps[2]]
+    with pytest.raises(SpionError, match="changed"):
+        opt.step()
+    assert all(torch.equal(p, b) for p, b in zip(ps, before))
