@@ -6,6 +6,8 @@ value and write 16-bit copies of the parameters (``layernorm.register_shadows``)
 """
 from __future__ import annotations
 
+from collections import defaultdict
+
 import torch
 
 from . import _ops
@@ -52,6 +54,15 @@ class _Moments:
         self.scales = tuple(torch.ones(total // BLOCK, device=dev) for _ in range(2)) if eight else None
         self.steps = torch.zeros(len(params), device=dev)
 
+    def __getstate__(self):                     # (torch does not pickle 8-bit floating-point types by themselves)
+        bytes_ = {k: self.__dict__[k].view(torch.uint8) for k in ("exp_avg", "exp_avg_sq") if self.bits == 8}
+        return self.__dict__ | bytes_
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        if self.bits == 8:
+            self.exp_avg, self.exp_avg_sq = self.exp_avg.view(torch.float8_e4m3fn), self.exp_avg_sq.view(torch.float8_e5m2)
+
     def state_of(self, i):
         p, at = self.params[i], self.at[i]
         s = {"step": self.steps[i], "exp_avg": self.exp_avg[at:at + p.numel()].view(p.shape), "exp_avg_sq": self.exp_avg_sq[at:at + p.numel()].view(p.shape)}
@@ -82,8 +93,17 @@ class AdamW(torch.optim.Optimizer):
         self._moments, self._copies = [], {}             # of each group that has taken a step: its parameters, their arrays by type and device
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, clip_value=clip_value))
 
-    def __getstate__(self):                     # copies of the optimizer keep their arrays (the base class would keep the views only)
-        return self.__dict__.copy()
+    def __getstate__(self):                     # what the base class keeps, with the arrays in place of their views
+        kept = super().__getstate__() | {k: self.__dict__[k] for k in ("state_bits", "seed", "_moments", "_copies")}
+        kept["state"] = defaultdict(dict)
+        return kept
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for _, sets in self._moments:
+            for m in sets:
+                for i, p in enumerate(m.params):
+                    self.state[p] = m.state_of(i)
 
     def write_copies(self, params, copies):
         """Every step also writes each of ``copies`` (16-bit, of its parameter's shape) for the parameter in ``params``."""

@@ -434,3 +434,30 @@ def test_steps_follow_the_parameter_groups():
     with pytest.raises(SpionError, match="changed"):
         opt.step()
     assert all(torch.equal(p, b) for p, b in zip(ps, before))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_copies_of_an_optimizer_that_has_a_scheduler(bits):
+    """A scheduler puts a step of its own into the optimizer's attributes: a copy has the class's, and steps its own parameters."""
+    import pickle
+
+    from spion_b200.optim import AdamW
+    a = small_model()
+    opt = AdamW(a.parameters(), lr=1e-2, state_bits=bits, seed=2)
+    scheduler = torch.optim.lr_scheduler.LambdaLR(opt, lambda k: 1.0)
+    gradients(a, 0)
+    opt.step()
+    scheduler.step()
+    copies = [copy.deepcopy((a, opt)), pickle.loads(pickle.dumps((a, opt)))]
+    before = [p.detach().clone() for p in a.parameters()]
+    for model, o in copies:
+        gradients(model, 1)
+        o.step()
+        assert all(torch.equal(p, b) for p, b in zip(a.parameters(), before))
+    gradients(a, 1)
+    opt.step()
+    want = opt.state_dict()["state"]
+    for model, o in copies:
+        assert all(torch.equal(p, q) for p, q in zip(a.parameters(), model.parameters()))
+        for i, s in o.state_dict()["state"].items():                      # what it keeps is what it steps on
+            assert all(torch.equal(s[k].float(), want[i][k].float()) for k in want[i])
