@@ -153,6 +153,10 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Moments are copied into the arrays that this optimizer keeps; they have to be of its ``state_bits``."""
+        state_dict = dict(state_dict)
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            other = hook(self, state_dict)
+            state_dict = state_dict if other is None else other
         groups, state = state_dict["param_groups"], state_dict["state"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("the optimizer state is not that of these parameter groups")
@@ -181,3 +185,5 @@ class AdamW(torch.optim.Optimizer):
                     dst.copy_(src)
         for mine, saved in zip(self.param_groups, groups):
             mine.update({k: v for k, v in saved.items() if k != "params" and k in mine})
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)

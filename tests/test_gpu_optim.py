@@ -461,3 +461,23 @@ def test_copies_of_an_optimizer_that_has_a_scheduler(bits):
         assert all(torch.equal(p, q) for p, q in zip(a.parameters(), model.parameters()))
         for i, s in o.state_dict()["state"].items():                      # what it keeps is what it steps on
             assert all(torch.equal(s[k].float(), want[i][k].float()) for k in want[i])
+
+
+def test_hooks_of_loading_a_state():
+    from spion_b200.optim import AdamW
+    a = small_model()
+    opt = AdamW(a.parameters())
+    gradients(a, 0)
+    opt.step()
+    saved, calls = copy.deepcopy(opt.state_dict()), []
+    saved["state"][0]["step"] = torch.tensor(5.0)
+
+    def before(o, state):
+        calls.append(("before", o is opt))
+        return {**state, "state": {**state["state"], 1: {**state["state"][1], "step": torch.tensor(9.0)}}}
+
+    opt.register_load_state_dict_pre_hook(before)
+    opt.register_load_state_dict_post_hook(lambda o: calls.append(("after", float(o.state[a[0].weight]["step"]))))
+    opt.load_state_dict(saved)
+    assert calls == [("before", True), ("after", 5.0)]
+    assert float(opt.state[a[0].bias]["step"]) == 9 and float(saved["state"][1]["step"]) == 1
