@@ -6,6 +6,7 @@ value and write 16-bit copies of the parameters (``layernorm.register_shadows``)
 """
 from __future__ import annotations
 
+import copy
 from collections import defaultdict
 
 import torch
@@ -14,6 +15,8 @@ from . import _ops
 from ._lib import SpionError
 
 BLOCK = 256
+# entries of torch.optim.AdamW's groups that say how it computes: a state is loaded without them
+_SWITCHES = ("amsgrad", "maximize", "foreach", "capturable", "differentiable", "fused", "decoupled_weight_decay")
 
 
 def places(tensors):
@@ -184,6 +187,6 @@ class AdamW(torch.optim.Optimizer):
                 else:
                     dst.copy_(src)
         for mine, saved in zip(self.param_groups, groups):
-            mine.update({k: v for k, v in saved.items() if k != "params" and k in mine})
+            mine.update({k: copy.deepcopy(v) for k, v in saved.items() if k != "params" and k not in _SWITCHES})
         for hook in self._optimizer_load_state_dict_post_hooks.values():
             hook(self)

@@ -481,3 +481,24 @@ def test_hooks_of_loading_a_state():
     opt.load_state_dict(saved)
     assert calls == [("before", True), ("after", 5.0)]
     assert float(opt.state[a[0].bias]["step"]) == 9 and float(saved["state"][1]["step"]) == 1
+
+
+def test_loaded_groups():
+    """Whatever a group carries is loaded with it (a scheduler's first rate), in tensors of this optimizer's own."""
+    from spion_b200.optim import AdamW
+    a, b = small_model(), small_model()
+    theirs = torch.optim.AdamW(a.parameters(), lr=torch.tensor(1e-2, device="cuda"), capturable=True)
+    torch.optim.lr_scheduler.LambdaLR(theirs, lambda k: 0.5)
+    gradients(a, 0)
+    theirs.step()
+    theirs.param_groups[0]["name"] = "all of them"
+    saved = theirs.state_dict()
+    mine = AdamW(b.parameters(), clip_value=3.0)
+    mine.load_state_dict(saved)
+    group = mine.param_groups[0]
+    assert group["name"] == "all of them" and float(group["initial_lr"]) == float(saved["param_groups"][0]["initial_lr"]) and group["clip_value"] == 3.0
+    assert float(group["lr"]) == float(theirs.param_groups[0]["lr"]) and group["lr"] is not theirs.param_groups[0]["lr"]
+    group["lr"].fill_(1.0)
+    assert float(theirs.param_groups[0]["lr"]) != 1.0
+    assert group["params"] == list(b.parameters())
+    torch.optim.lr_scheduler.LambdaLR(mine, lambda k: 0.5, last_epoch=3)   # asks for the first rate
