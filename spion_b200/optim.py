@@ -163,6 +163,12 @@ class AdamW(torch.optim.Optimizer):
         groups, state = state_dict["param_groups"], state_dict["state"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("the optimizer state is not that of these parameter groups")
+        for g in groups:
+            for k in ("amsgrad", "maximize"):
+                if g.get(k):
+                    raise ValueError(f"a state of AdamW with {k} cannot be continued: it is not served")
+            if g.get("weight_decay") and not g.get("decoupled_weight_decay", True):
+                raise ValueError("a state whose weight decay is not decoupled (Adam's) cannot be continued")
         want = {"step", "exp_avg", "exp_avg_sq"} | ({"exp_avg_scales", "exp_avg_sq_scales"} if self.state_bits == 8 else set())
         plan = []
         for g, saved in enumerate(groups):

@@ -86,3 +86,13 @@ def test_8_bit_linear_arguments_at_the_c_boundary():
     x = torch.zeros(3, 16)
     with pytest.raises(SpionError, match="CUDA"):
         linear_e4m3(x, Rows8(x.to(torch.float8_e4m3fn), torch.ones(3)))
+
+
+def test_states_of_other_algorithms_are_refused():
+    from spion_b200.optim import AdamW
+    w = torch.nn.Parameter(torch.zeros(3))
+    for kw, match in ((dict(amsgrad=True), "amsgrad"), (dict(maximize=True), "maximize")):
+        with pytest.raises(ValueError, match=match):
+            AdamW([w]).load_state_dict(torch.optim.AdamW([w], **kw).state_dict())
+    with pytest.raises(ValueError, match="decoupled"):
+        AdamW([w]).load_state_dict(torch.optim.Adam([w], weight_decay=0.1).state_dict())
