@@ -183,7 +183,9 @@ class AdamW(torch.optim.Optimizer):
                         plan.append((dst, None))
                         continue
                     src = torch.as_tensor(entry[k]) if k in entry and want <= set(entry) else None
-                    if src is None or src.shape != dst.shape or (k != "step" and src.dtype != dst.dtype):
+                    # (torch's moments of 16-bit parameters are in their type)
+                    types = (dst.dtype, torch.bfloat16, torch.float16) if self.state_bits == 32 else (dst.dtype,)
+                    if src is None or src.shape != dst.shape or (k != "step" and src.dtype not in types):
                         raise ValueError(f"the state of parameter {number} ({k}) is not that of an AdamW of {self.state_bits} bits and this shape")
                     plan.append((dst, src))
         with torch.no_grad():

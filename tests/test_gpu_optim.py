@@ -502,3 +502,27 @@ def test_loaded_groups():
     assert float(theirs.param_groups[0]["lr"]) != 1.0
     assert group["params"] == list(b.parameters())
     torch.optim.lr_scheduler.LambdaLR(mine, lambda k: 0.5, last_epoch=3)   # asks for the first rate
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_states_of_16_bit_parameters(dtype):
+    """torch keeps their moments in the parameter's type, this optimizer in fp32: each takes the other's, rounded where it is narrower."""
+    from spion_b200.optim import AdamW
+    a, b = small_model(dtype), small_model(dtype)
+    theirs, mine = torch.optim.AdamW(a.parameters()), AdamW(b.parameters())
+    gradients(a, 0)
+    theirs.step()
+    mine.load_state_dict(copy.deepcopy(theirs.state_dict()))
+    for p, q in zip(a.parameters(), b.parameters()):
+        for k in ("step", "exp_avg", "exp_avg_sq"):
+            x, y = mine.state[q][k], theirs.state[p][k]
+            assert x.dtype == torch.float32 and torch.equal(x, y.float().to(x.device))
+    gradients(b, 1)
+    mine.step()
+    theirs.load_state_dict(copy.deepcopy(mine.state_dict()))
+    for p, q in zip(a.parameters(), b.parameters()):
+        assert torch.equal(theirs.state[p]["exp_avg"], mine.state[q]["exp_avg"].to(dtype))
+    bad = copy.deepcopy(theirs.state_dict())
+    bad["state"][0]["exp_avg"] = bad["state"][0]["exp_avg"].int()
+    with pytest.raises(ValueError, match="exp_avg"):
+        mine.load_state_dict(bad)
