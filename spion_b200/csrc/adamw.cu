@@ -88,8 +88,9 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-// The update's quotient: a few units in its last place are lost beside a parameter that is many times as large.  v below fp32's normal numbers counts as
-// zero; beside an eps of 2^-40 or more its root is nothing (FLUSH; other steps take the exact forms).
+// The update's quotient: a few units in its last place are lost beside a parameter that is many times as large.  FLUSH: v below fp32's normal numbers, 2^-126,
+// counts as zero.  Its corrected root is at most 2^-63 / sqrt(1 - b2) at any step, 2^-24 of an eps of 2^-39 / sqrt(1 - b2) or more (b2 = 0.999: 5.8e-11);
+// steps with a smaller eps take the exact forms.
 template <bool FLUSH> __device__ __forceinline__ float quotient(float m, float v, float root_v, float eps) {
   if (!FLUSH) return m / (sqrtf(v) * root_v + eps);
   float r, q;
@@ -452,7 +453,7 @@ template <class P, int BITS>
 int launches(const Step& s, const Begin& b, const spion_adamw_tensor* ts, int count, cudaStream_t st) {
   for (int i = 0; i < count; i += MOST) {
     const int n = count - i < MOST ? count - i : MOST;
-    const bool flush = s.eps >= 0x1p-40f;
+    const bool flush = s.eps * sqrtf(s.c2) >= 0x1p-39f;
     const int rc = n > FEW ? flush ? launch<P, BITS, true, MOST>(s, b, ts + i, n, st) : launch<P, BITS, false, MOST>(s, b, ts + i, n, st)
                            : flush ? launch<P, BITS, true, FEW>(s, b, ts + i, n, st) : launch<P, BITS, false, FEW>(s, b, ts + i, n, st);
     if (rc != SPION_OK) return rc;

@@ -526,3 +526,25 @@ def test_states_of_16_bit_parameters(dtype):
     bad["state"][0]["exp_avg"] = bad["state"][0]["exp_avg"].int()
     with pytest.raises(ValueError, match="exp_avg"):
         mine.load_state_dict(bad)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-13, 2.0 ** -40, 1e-12, 2.0 ** -35, 1e-10, 1e-9])
+def test_small_eps_beside_small_second_moments(eps):
+    """Second moments on both sides of fp32's smallest normal number 2^-126, with the largest correction that b2 = 0.9999 has (100 at the first step): their roots
+    are what the update is divided by.  The bound is that of every other step; the numbers below 2^-126 are off by at most 2^-150, a root of 2^-126 and more
+    by 2^-25 of itself then, those of 2^-130 by 2^-21."""
+    from spion_b200.optim import adamw_step
+    n = 4096
+    g = np.exp(np.linspace(np.log(3e-18), np.log(1e-15), n))              # v from 2^-130 to 2^-113
+    for bits in (32, 8):
+        p, d = torch.zeros(n, device="cuda"), torch.from_numpy(g).float().cuda()
+        m, v = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+        scales = None
+        if bits == 8:
+            m, v, scales = m.to(torch.float8_e4m3fn), v.to(torch.float8_e5m2), (torch.ones(n // 256, device="cuda"), torch.ones(n // 256, device="cuda"))
+        hyper = dict(lr=1.0, betas=(0.9, 0.9999), eps=eps, weight_decay=0.0, clip_value=None)
+        adamw_step([p], [d], m, v, torch.zeros(1, device="cuda"), scales=scales, **hyper)
+        want = reference(np.zeros(n), d.double().cpu().numpy(), np.zeros(n), np.zeros(n), 0, 0, **hyper)
+        off = np.abs(p.double().cpu().numpy() - want["p"])
+        bound = want["err_p"] + np.abs(want["p"]) * np.minimum(2.0 ** -151 / want["v"], 1)
+        assert (off <= bound).all(), (off / bound).max()
