@@ -10,6 +10,8 @@ attention map, pattern discovery, then sparse steps -- and data parallelism from
 """
 from __future__ import annotations
 
+import contextlib
+
 import torch
 import torch.nn as nn
 
@@ -222,6 +224,23 @@ class Classifier(nn.Module):
             layer.quantize(on)
         self.model.quantized = on
 
+    @contextlib.contextmanager
+    def quantized_as(self, on: bool):
+        """Within the block the sparse phase is evaluated on 8-bit operands of the weights as they are now, or on none; what ``quantize`` has
+        left is put aside and comes back."""
+        encoder = self.model
+        was, kept = encoder.quantized, [(m.mha.linear8, m.mlp8) for m in encoder.layers]
+        try:
+            if on:
+                self.quantize()
+            else:
+                encoder.quantized = False
+            yield
+        finally:
+            encoder.quantized = was
+            for layer, (linear8, mlp8) in zip(encoder.layers, kept):
+                layer.mha.linear8, layer.mlp8 = linear8, mlp8
+
     def scores(self, ids, mat_lst):
         """Class scores of single- or dual-tower inputs in the sparse phase, without a loss."""
         with torch.autocast(device_type="cuda", dtype=torch.bfloat16, enabled=self.amp):
@@ -310,22 +329,18 @@ class Trainer:
         self._refresh_shadows()
 
     def evaluate(self, ids, label):
-        """Mean loss and share of right answers of one batch in the sparse phase, without gradients or dropout.  ``config["eval_linear_bits"] = 8``:
-        with the encoder's linear layers on 8-bit operands."""
+        """Mean loss and share of right answers of one batch in the sparse phase with the weights as they are now, without gradients or dropout.
+        ``config["eval_linear_bits"] = 8``: with the encoder's linear layers on 8-bit operands, quantised by the call; else on none, whatever
+        ``Classifier.quantize`` has left."""
         if self.mat_lst is None:
             raise RuntimeError("evaluate after discover()")
-        eight = self.config.get("eval_linear_bits") == 8
         training = self.model.training
         self.model.eval()
         try:
-            with torch.no_grad():
-                if eight:
-                    self.model.quantize()
+            with torch.no_grad(), self.model.quantized_as(self.config.get("eval_linear_bits") == 8):
                 scores = self.model.scores(ids, self.mat_lst)
                 return nn.functional.cross_entropy(scores, label), (scores.argmax(-1) == label).float().mean()
         finally:
-            if eight:
-                self.model.quantize(False)
             self.model.train(training)
 
     def _refresh_shadows(self):

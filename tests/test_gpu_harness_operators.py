@@ -95,3 +95,42 @@ def test_captured_steps(bits):
 def test_unknown_norm_is_refused():
     with pytest.raises(ValueError, match="norm"):
         trainer(norm="batch")
+
+
+def test_evaluation_leaves_what_was_quantised_as_it_was():
+    """quantize() keeps its weights until quantize(False), whatever is evaluated between; evaluate() is on what the configuration says and on the weights of
+    the moment."""
+    tr, ids, lab = trainer()
+    start(tr, ids, lab)
+    plain, _ = tr.evaluate(ids, lab)
+    tr.config["eval_linear_bits"] = 8
+    eight, _ = tr.evaluate(ids, lab)
+    assert float(eight) != float(plain)
+    layers = tr.model.model.layers
+    assert not tr.model.model.quantized and all(m.mha.linear8 is None and m.mlp8 is None for m in layers)
+    tr.model.quantize()
+    kept = [(m.mha.linear8, m.mlp8) for m in layers]
+    codes = [m.values.clone() for a, b in kept for m in (*a, *b)]
+    with torch.no_grad():
+        for p in tr.model.model.layers.parameters():
+            p.mul_(1.25)
+    with torch.no_grad():
+        tr.model.eval()
+        scores = tr.model.scores(ids, tr.mat_lst)
+        tr.model.train()
+    moved, _ = tr.evaluate(ids, lab)                                       # of the new weights
+    tr.config["eval_linear_bits"] = None
+    other, _ = tr.evaluate(ids, lab)                                       # not in 8 bits
+    tr.model.quantize(False)
+    assert float(tr.evaluate(ids, lab)[0]) == float(other)
+    tr.config["eval_linear_bits"] = 8
+    assert float(tr.evaluate(ids, lab)[0]) == float(moved) and float(moved) != float(eight)
+    tr.model.quantize()
+    for m, k in zip(layers, kept):
+        m.mha.linear8, m.mlp8 = k
+    tr.evaluate(ids, lab)
+    assert tr.model.model.quantized and all(m.mha.linear8 is a and m.mlp8 is b for m, (a, b) in zip(layers, kept))
+    assert all(torch.equal(m.values.view(torch.uint8), c.view(torch.uint8)) for m, c in zip([m for a, b in kept for m in (*a, *b)], codes))
+    with torch.no_grad():
+        tr.model.eval()
+        assert torch.equal(tr.model.scores(ids, tr.mat_lst), scores)
