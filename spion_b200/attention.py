@@ -201,12 +201,20 @@ class Attention(nn.Module):
         from .quant import E4M3Linear
         if on and not self.native:
             raise _lib.SpionError("8-bit projections are served beside the native attention (config['native'])")
+        if on:
+            self.check_for_8_bits()
         self.linear8 = [E4M3Linear(m, self.native_dtype) for m in (self.W_q, self.W_k, self.W_v, self.ff)] if on else None
+
+    def check_for_8_bits(self):
+        """``forward_quantized`` calls no forward of the projections nor of this module: refused where that would make a difference."""
+        if not (no_global_hooks() and untouched(self, (Attention,)) and all(untouched(self._modules.get(m), _PLAIN_LINEAR) for m in ("W_q", "W_k", "W_v", "ff"))):
+            raise _lib.SpionError("8-bit projections: the attention module or a projection is replaced or has a hook, which would be passed over")
 
     def forward_quantized(self, X, mask, mat):
         """``forward`` of the sparse phase with the projections on 8-bit operands.  X: ``Rows8`` [B, L, dim].  No gradients."""
         if self.linear8 is None:
             raise _lib.SpionError("quantize() comes first")
+        self.check_for_8_bits()
         W_q, W_k, W_v, ff = self.linear8
         with torch.autocast(device_type="cuda", enabled=False):
             out, attn = self.block_attn(*(self.split_heads(W(X)) for W in (W_q, W_k, W_v)), mask.float(), mat)

@@ -16,6 +16,7 @@ import torch
 import torch.nn as nn
 
 from . import dp
+from ._lib import SpionError
 from .attention import Attention, no_global_hooks, untouched
 from .layernorm import mask_rows, sequence_means
 from .pattern import discover_layers
@@ -112,14 +113,17 @@ class TransformerLayer(nn.Module):
                 return ops.mlp(*args)
         return self.mlpblock(n2)
 
-    def _mlp_is_plain(self) -> bool:
-        """The block is what __init__ made, nothing in it replaced or hooked, and no dropout of it is active."""
+    def _mlp_as_made(self) -> bool:
+        """The block is what __init__ made, nothing in it replaced or hooked."""
         block = self.mlpblock
-        if not (no_global_hooks() and untouched(block, (nn.Sequential,)) and len(block) == len(self.mlp_types)):
+        return no_global_hooks() and untouched(block, (nn.Sequential,)) and len(block) == len(self.mlp_types) \
+            and all(untouched(m, (t,)) for m, t in zip(block, self.mlp_types))
+
+    def _mlp_is_plain(self) -> bool:
+        """The block is as made, and no dropout of it is active."""
+        if not self._mlp_as_made():
             return False
-        if not all(untouched(m, (t,)) for m, t in zip(block, self.mlp_types)):
-            return False
-        lin1, act, drop1, lin2, drop2 = block
+        lin1, act, drop1, lin2, drop2 = self.mlpblock
         return act.approximate == "none" and lin1.bias is not None and lin2.bias is not None \
             and not any(d.training and d.p > 0 for d in (drop1, drop2))
 
@@ -135,12 +139,21 @@ class TransformerLayer(nn.Module):
     def quantize(self, on: bool = True):
         """Keep the layer's linear weights in 8 bits beside those that train, as they are now (see ``Classifier.quantize``)."""
         from .quant import E4M3Linear
+        if on:
+            self.check_for_8_bits()
         self.mha.quantize(on)
         self.mlp8 = tuple(E4M3Linear(self.mlpblock[i], self.mha.native_dtype) for i in (0, 3)) if on else None
+
+    def check_for_8_bits(self):
+        """``forward_quantized`` calls no forward of the linear layers, of the dropouts nor of what holds them: refused where that would make a difference."""
+        self.mha.check_for_8_bits()
+        if not (self._mlp_as_made() and untouched(self.dropout1, (nn.Dropout,))):
+            raise SpionError("8-bit feed-forward block: a module of it or the dropout before it is replaced or has a hook, which would be passed over")
 
     def forward_quantized(self, X, branch, mask, mat):
         """The layer with its linear layers on 8-bit operands.  branch: what the layer before adds to X (None: nothing); returns X and what
         this one adds to it."""
+        self.check_for_8_bits()
         n1 = norm_rows8(self.norm1, X, branch)
         if branch is not None:
             X, n1 = n1
@@ -151,10 +164,10 @@ class TransformerLayer(nn.Module):
 
 
 def norm_rows8(norm, x, res=None):
-    """``norm(x)`` in 8 bits, with ``res`` ``(x + res, norm(x + res))``: one kernel where the norm is the root-mean-square norm's."""
+    """``norm(x)`` in 8 bits, with ``res`` ``(x + res, norm(x + res))``: one kernel where the norm is the root-mean-square norm's and has no hook."""
     from .quant import quantize_rows
     from .rmsnorm import FusedRMSNorm, rms_norm_e4m3
-    if isinstance(norm, FusedRMSNorm):
+    if untouched(norm, (FusedRMSNorm,)) and no_global_hooks():
         return rms_norm_e4m3(x, norm.weight, norm.eps, res)
     if res is None:
         return quantize_rows(norm(x))
@@ -220,6 +233,8 @@ class Classifier(nn.Module):
     def quantize(self, on: bool = True):
         """Evaluate the sparse phase (``eval()``, no gradients) with the encoder's linear layers on 8-bit operands: weights as they are now, kept until
         ``quantize(False)``; activations from norms that write 8 bits, or quantised by the layer."""
+        for layer in self.model.layers if on else ():
+            layer.check_for_8_bits()                                  # all of them before the first is changed
         for layer in self.model.layers:
             layer.quantize(on)
         self.model.quantized = on

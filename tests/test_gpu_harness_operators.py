@@ -134,3 +134,52 @@ def test_evaluation_leaves_what_was_quantised_as_it_was():
     with torch.no_grad():
         tr.model.eval()
         assert torch.equal(tr.model.scores(ids, tr.mat_lst), scores)
+
+
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+def test_replaced_and_hooked_modules_of_an_8_bit_evaluation(norm):
+    """A norm that is hooked is called as a module; of linear layers, of the attention and of what lies between them an 8-bit evaluation calls no forward of their
+    own, so a hook or another module there is refused."""
+    from spion_b200._lib import SpionError
+    tr, ids, lab = trainer(norm=norm, eval_linear_bits=8)
+    start(tr, ids, lab)
+    want, _ = tr.evaluate(ids, lab)
+    layer, seen = tr.model.model.layers[1], []
+    hook = layer.norm2.register_forward_hook(lambda m, x, y: seen.append(y.shape))
+    got, _ = tr.evaluate(ids, lab)
+    hook.remove()
+    assert seen == [(4, 256, 64)] and abs(float(got) - float(want)) < 1e-2     # the same codes but for ties
+    hook = layer.norm1.register_forward_hook(lambda m, x, y: y * 2)            # a power of two: the same codes, other scales
+    doubled, _ = tr.evaluate(ids, lab)
+    hook.remove()
+    assert float(doubled) != float(want)
+
+    def refused():
+        with pytest.raises(SpionError, match="hook"):
+            tr.evaluate(ids, lab)
+        assert not tr.model.model.quantized and layer.mha.linear8 is None and layer.mlp8 is None and tr.model.training
+
+    for m in (layer.mha.W_q, layer.mha.W_k, layer.mha.W_v, layer.mha.ff, layer.mha, layer.mlpblock, layer.mlpblock[0], layer.mlpblock[3], layer.mlpblock[4], layer.dropout1):
+        hook = m.register_forward_hook(lambda m, x, y: None)
+        refused()
+        hook.remove()
+        hook = m.register_forward_pre_hook(lambda m, x: None)
+        refused()
+        hook.remove()
+    for owner, name in ((layer.mha, "W_k"), (layer.mha, "ff"), (layer.mlpblock, "0"), (layer.mlpblock, "2"), (layer, "dropout1")):
+        was = owner._modules[name]
+        owner._modules[name] = torch.nn.Identity()
+        refused()
+        owner._modules[name] = was
+    hook = torch.nn.modules.module.register_module_forward_hook(lambda m, x, y: None)
+    refused()
+    hook.remove()
+    tr.model.quantize()
+    hook = layer.mha.W_v.register_forward_hook(lambda m, x, y: None)           # hooked after it was quantised
+    with torch.no_grad(), pytest.raises(SpionError, match="hook"):
+        tr.model.eval()
+        tr.model.scores(ids, tr.mat_lst)
+    hook.remove()
+    tr.model.train()
+    tr.model.quantize(False)
+    assert float(tr.evaluate(ids, lab)[0]) == float(want)
