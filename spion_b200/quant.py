@@ -45,6 +45,15 @@ class E4M3Linear(nn.Module):
         self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().clone())
         self.in_features, self.out_features, self.out_dtype = linear.in_features, linear.out_features, out_dtype
 
+    def _apply(self, fn, recurse=True):
+        """A change of type (``half()``, ``to(dtype)``) is not one of the codes and their scales: they go to the device that it names."""
+        codes = {k: self._buffers[k] for k in ("values", "scales")}
+        super()._apply(fn, recurse)
+        for k, was in codes.items():
+            if self._buffers[k].dtype != was.dtype:
+                self._buffers[k] = was.to(self._buffers[k].device)
+        return self
+
     def forward(self, x):
         dtype = self.out_dtype
         if dtype is None and torch.is_autocast_enabled() and torch.get_autocast_dtype("cuda") == torch.bfloat16:

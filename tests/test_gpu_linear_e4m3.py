@@ -196,3 +196,17 @@ def test_nothing_is_written_outside_of_the_result(T, K, N):
                                                   w.values.stride(0), w.scales.data_ptr(), None, _lib.F32, buf[first:].data_ptr(), ld, code, T, K, N,
                                                   torch.cuda.current_stream().cuda_stream))
             assert torch.equal(buf, expect)
+
+
+def test_a_module_keeps_its_codes_when_its_type_is_changed():
+    from spion_b200.quant import E4M3Linear
+    lin = torch.nn.Linear(96, 40).cuda()
+    x = torch.randn(20, 96, device="cuda")
+    want = E4M3Linear(lin)(x)
+    for change in (lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.double().float(), lambda m: m.cpu().cuda(), lambda m: m.half().cpu().cuda().float()):
+        m = E4M3Linear(lin)
+        bias = m.bias.clone()
+        m = change(m)
+        assert m.values.dtype == torch.float8_e4m3fn and m.scales.dtype == torch.float32
+        m.bias = bias                                                      # (a type change of the bias is the caller's)
+        assert torch.equal(m(x), want)
