@@ -205,6 +205,12 @@ class Attention(nn.Module):
             self.check_for_8_bits()
         self.linear8 = [E4M3Linear(m, self.native_dtype) for m in (self.W_q, self.W_k, self.W_v, self.ff)] if on else None
 
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        for m in self.linear8 or ():                  # (no submodules: a state dict has the weights that they come from)
+            m._apply(fn)
+        return self
+
     def check_for_8_bits(self):
         """``forward_quantized`` calls no forward of the projections nor of this module: refused where that would make a difference."""
         if not (no_global_hooks() and untouched(self, (Attention,)) and all(untouched(self._modules.get(m), _PLAIN_LINEAR) for m in ("W_q", "W_k", "W_v", "ff"))):

@@ -144,6 +144,12 @@ class TransformerLayer(nn.Module):
         self.mha.quantize(on)
         self.mlp8 = tuple(E4M3Linear(self.mlpblock[i], self.mha.native_dtype) for i in (0, 3)) if on else None
 
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        for m in self.mlp8 or ():                     # (no submodules: a state dict has the weights that they come from)
+            m._apply(fn)
+        return self
+
     def check_for_8_bits(self):
         """``forward_quantized`` calls no forward of the linear layers, of the dropouts nor of what holds them: refused where that would make a difference."""
         self.mha.check_for_8_bits()

@@ -183,3 +183,16 @@ def test_replaced_and_hooked_modules_of_an_8_bit_evaluation(norm):
     tr.model.train()
     tr.model.quantize(False)
     assert float(tr.evaluate(ids, lab)[0]) == float(want)
+
+
+def test_8_bit_layers_go_where_their_model_goes():
+    tr, ids, lab = trainer()
+    start(tr, ids, lab)
+    keys = list(tr.model.state_dict())
+    tr.model.quantize()
+    assert list(tr.model.state_dict()) == keys
+    tr.model.to("cpu")
+    layers = [m for x in tr.model.model.layers for m in (*x.mha.linear8, *x.mlp8)]
+    assert all(t.device.type == "cpu" for m in layers for t in (m.values, m.scales, m.bias))
+    tr.model.to("cuda")
+    assert all(t.is_cuda for m in layers for t in (m.values, m.scales, m.bias))
