@@ -309,6 +309,11 @@ class Trainer:
         # config["optimizer"] = "fused": the library's AdamW (clipping and the copies of the parameters inside), its moments in
         # config["optimizer_state_bits"] bits
         self.fused_opt = config.get("optimizer", "torch") == "fused"
+        if config.get("optimizer", "torch") not in ("torch", "fused"):
+            raise ValueError(f"config['optimizer'] is {config['optimizer']!r}: 'torch' and 'fused' are served")
+        if not self.fused_opt and config.get("optimizer_state_bits", 32) != 32:
+            raise ValueError(f"config['optimizer_state_bits'] is {config['optimizer_state_bits']}: other than 32 with config['optimizer'] = 'fused' only")
+        self._evaluates_in_8_bits()
         if self.fused_opt:
             from .optim import AdamW
             self.opt = AdamW(self.bucket.params, lr=lr, weight_decay=0.0, state_bits=config.get("optimizer_state_bits", 32), clip_value=1.0, seed=seed)
@@ -349,16 +354,23 @@ class Trainer:
         self.opt.step()
         self._refresh_shadows()
 
+    def _evaluates_in_8_bits(self) -> bool:
+        bits = self.config.get("eval_linear_bits")
+        if bits not in (None, 8, 16, 32):
+            raise ValueError(f"config['eval_linear_bits'] is {bits}: 8, or 16, 32 and None for the layers as they are, are served")
+        return bits == 8
+
     def evaluate(self, ids, label):
         """Mean loss and share of right answers of one batch in the sparse phase with the weights as they are now, without gradients or dropout.
         ``config["eval_linear_bits"] = 8``: with the encoder's linear layers on 8-bit operands, quantised by the call; else on none, whatever
         ``Classifier.quantize`` has left."""
         if self.mat_lst is None:
             raise RuntimeError("evaluate after discover()")
+        eight = self._evaluates_in_8_bits()
         training = self.model.training
         self.model.eval()
         try:
-            with torch.no_grad(), self.model.quantized_as(self.config.get("eval_linear_bits") == 8):
+            with torch.no_grad(), self.model.quantized_as(eight):
                 scores = self.model.scores(ids, self.mat_lst)
                 return nn.functional.cross_entropy(scores, label), (scores.argmax(-1) == label).float().mean()
         finally:

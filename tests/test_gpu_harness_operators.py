@@ -196,3 +196,15 @@ def test_8_bit_layers_go_where_their_model_goes():
     assert all(t.device.type == "cpu" for m in layers for t in (m.values, m.scales, m.bias))
     tr.model.to("cuda")
     assert all(t.is_cuda for m in layers for t in (m.values, m.scales, m.bias))
+
+
+def test_unknown_optimizers_and_widths_are_refused():
+    for bad, match in ((dict(optimizer="adam8"), "optimizer"), (dict(optimizer="Fused"), "optimizer"), (dict(eval_linear_bits=4), "eval_linear_bits"),
+                       (dict(optimizer="torch", optimizer_state_bits=8), "optimizer_state_bits"), (dict(optimizer_state_bits=16), "state_bits")):
+        with pytest.raises(ValueError, match=match):
+            trainer(**bad)
+    tr, ids, lab = trainer(optimizer="torch")
+    start(tr, ids, lab)
+    tr.config["eval_linear_bits"] = 6
+    with pytest.raises(ValueError, match="eval_linear_bits"):
+        tr.evaluate(ids, lab)
