@@ -208,3 +208,96 @@ def test_unknown_optimizers_and_widths_are_refused():
     tr.config["eval_linear_bits"] = 6
     with pytest.raises(ValueError, match="eval_linear_bits"):
         tr.evaluate(ids, lab)
+
+
+def test_every_stage_of_an_8_bit_evaluation(monkeypatch):
+    """The encoder's pass on 8-bit operands, stage by stage: every value that a stage hands on is the next one's operand, in the place where it belongs, and each
+    stage is its formula on the operands that it got, in fp64.
+
+    Bounds, u = 2^-24: a linear layer as in test_gpu_linear_e4m3.py (U * (K / 8 + 16) of the sum of sizes, then a rounding to its type).  Rows in 8 bits: 2^-4 of
+    the value, half of the smallest step 2^-9 of the row's scale, and for the norm (K(N) / 2 + 8) u as in test_gpu_rmsnorm.py, 2^-7 more where the layer norm's
+    output was bf16 before."""
+    from spion_b200 import harness, quant
+    u = 2.0 ** -24
+    for norm, task, dtype, L in (("rms", "text", "fp32", 512), ("layer", "text", "bf16", 512), ("rms", "image", "bf16", 256), ("layer", "image", "fp32", 256)):
+        tr, ids, lab = trainer(task, dtype, L, batch=2, norm=norm)
+        ids = ids.clone()
+        ids[0, L - 100:], ids[1, 7:] = 0, 0                                # padding
+        start(tr, ids, lab)
+        encoder, linears, norms, attended = tr.model.model, [], [], []
+
+        def linear(x, w, bias=None, out_dtype=None, plain=quant.linear_e4m3):
+            y = plain(x, w, bias, out_dtype)
+            linears.append((x, w, bias, y))
+            return y
+
+        def rows8(m, x, res=None, plain=harness.norm_rows8):
+            y = plain(m, x, res)
+            norms.append((m, x, res, y))
+            return y
+
+        monkeypatch.setattr(quant, "linear_e4m3", linear)
+        monkeypatch.setattr(harness, "norm_rows8", rows8)
+        hooks = [x.mha.block_attn.register_forward_hook(lambda m, args, y: attended.append((m, args, y[0]))) for x in encoder.layers]
+        tr.model.eval()
+        mask = (ids != 0).float()
+        amp = lambda: torch.autocast("cuda", dtype=torch.bfloat16, enabled=tr.model.amp)      # noqa: E731
+        with torch.no_grad(), amp():
+            unquantised, _ = encoder(ids, mask, tr.mat_lst)
+            attended.clear()
+            tr.model.quantize()
+            out, _ = encoder(ids, mask, tr.mat_lst)
+            tr.model.quantize(False)
+            X = encoder.embeddings(ids)
+            again = [(m, args, m(*args)[0]) for m, args, _ in list(attended)]
+        [h.remove() for h in hooks]
+        monkeypatch.undo()
+        attended = attended[:len(encoder.layers)]
+        assert len(linears) == 6 * len(encoder.layers) and len(norms) == 2 * len(encoder.layers) and len(attended) == len(encoder.layers)
+
+        def check_linear(call, x, layer):
+            got, w, bias, y = call
+            assert got is x if isinstance(x, quant.Rows8) else torch.equal(got, x)
+            codes = quant.quantize_rows(layer.weight.detach())
+            assert torch.equal(w.values.view(torch.uint8), codes.values.view(torch.uint8)) and torch.equal(w.scales, codes.scales)
+            assert torch.equal(bias, layer.bias)
+            q = x if isinstance(x, quant.Rows8) else quant.quantize_rows(x)
+            A, B = q.values.double() * q.scales.double()[..., None], w.values.double() * w.scales.double()[:, None]
+            want, size = A @ B.t() + bias.double(), A.abs() @ B.abs().t() + bias.double().abs()
+            bound = size * u * (A.shape[-1] / 8 + 16) + want.abs() * torch.finfo(y.dtype).eps / 2 + 1e-38
+            assert bool(((y.double() - want).abs() <= bound).all())
+            return y
+
+        def check_rows(call, layer, x, res):
+            m, got, r, y = call
+            assert m is layer and (got is x or torch.equal(got, x)) and (r is res if res is None else torch.equal(r, res))
+            s, q = (x, y) if res is None else y
+            if res is not None:
+                want = x.double() + res.double()
+                assert bool(((s.double() - want).abs() <= want.abs() * 3 * u).all())
+            S = s.double()
+            if norm == "layer":
+                S = S - S.mean(-1, keepdim=True)
+            n = S / torch.sqrt((S * S).mean(-1, keepdim=True) + m.eps) * m.weight.double() + (m.bias.double() if norm == "layer" else 0)
+            rel = (64 / 2 + 64) * u + (2.0 ** -7 if norm == "layer" and dtype == "bf16" else 0)
+            size = n.abs() + (S.abs().amax(-1, keepdim=True) * 64 * u if norm == "layer" else 0)      # (differences of the mean: absolute errors)
+            off = (q.values.double() * q.scales.double()[..., None] - n).abs()
+            assert bool((off <= size * (2.0 ** -4 + 2 * rel) + q.scales.double()[..., None] * 2.0 ** -10 * 1.01 + 1e-6).all())
+            return s, q
+
+        branch = None
+        for i, layer in enumerate(encoder.layers):
+            lin, mha = linears[6 * i:6 * i + 6], layer.mha
+            X, n1 = check_rows(norms[2 * i], layer.norm1, X, branch)
+            heads = [mha.split_heads(check_linear(lin[k], n1, w)) for k, w in enumerate((mha.W_q, mha.W_k, mha.W_v))]
+            m, args, o = attended[i]
+            assert m is mha.block_attn and all(torch.equal(a, b) for a, b in zip(args, (*heads, mask, tr.mat_lst[0][i])))
+            assert torch.equal(again[i][2], o)
+            out1 = check_linear(lin[3], mha.combine_heads(o), mha.ff)
+            X, n2 = check_rows(norms[2 * i + 1], layer.norm2, X, out1)
+            hidden = check_linear(lin[4], n2, layer.mlpblock[0])
+            branch = check_linear(lin[5], torch.nn.functional.gelu(hidden), layer.mlpblock[3])
+        with torch.no_grad(), amp():
+            want = encoder.norm(X + branch) * mask[..., None]
+        assert torch.equal(out, want.to(out.dtype)) and not bool(out[mask == 0].any())
+        assert not torch.equal(out, unquantised)
