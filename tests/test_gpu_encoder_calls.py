@@ -150,3 +150,37 @@ def test_inference_mode_and_what_is_refused():
     with torch.autograd.forward_ad.dual_level():
         dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
         refused(lambda: rms_norm(dual, w), "ordinary")
+
+
+def test_the_rings_on_two_streams_at_once():
+    """The kernels that copy ahead: the optimizer's with 8-bit moments, the norm's backward."""
+    from spion_b200.optim import adamw_step
+    from spion_b200.rmsnorm import rms_norm
+    x, g = torch.randn(4096, 2048, device="cuda", requires_grad=True), torch.rand(2048, device="cuda", requires_grad=True)
+    dy, n = torch.randn(4096, 2048, device="cuda"), 16_000_000
+    start, d = torch.randn(n, device="cuda"), torch.randn(n, device="cuda")
+
+    def state():
+        return (start.clone(), torch.zeros(n, device="cuda").to(torch.float8_e4m3fn), torch.zeros(n, device="cuda").to(torch.float8_e5m2),
+                (torch.ones(n // 256, device="cuda"), torch.ones(n // 256, device="cuda")), torch.zeros(1, device="cuda"))
+
+    def step(s):
+        adamw_step([s[0]], [d], s[1], s[2], s[4], scales=s[3])
+
+    want = torch.autograd.grad(rms_norm(x, g), (x, g), dy)
+    states, streams, got = [state() for _ in range(3)], [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for s, stream in zip(states, streams):
+            with torch.cuda.stream(stream):
+                step(s)
+                got.append(torch.autograd.grad(rms_norm(x, g), (x, g), dy))
+    torch.cuda.synchronize()
+    for _ in range(4):
+        step(states[2])
+    for pair in got:
+        assert all(torch.equal(a, b) for a, b in zip(pair, want))
+    p, m, v, scales, _ = states[2]
+    for q, m1, v1, scales1, steps in states[:2]:
+        assert torch.equal(p, q) and torch.equal(m.view(torch.uint8), m1.view(torch.uint8)) and torch.equal(v.view(torch.uint8), v1.view(torch.uint8))
+        assert all(torch.equal(a, b) for a, b in zip(scales, scales1)) and float(steps) == 4
