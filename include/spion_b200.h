@@ -474,7 +474,8 @@ int spion_linear_prepare(int fp32);
 /* SPION_ERR_TIMEOUT when a bounded wait of these kernels has given up since the last reset (synchronises the device).  Until then
  * every call of them returns without writing its results. */
 int spion_linear_status(int reset);
-/* Failure-path self-test that faults nothing, as spion_selftest_bounded_wait: the status word is set afterwards. */
+/* Failure-path self-test that faults nothing, as spion_selftest_bounded_wait: the status words of the linear layers, of the 8-bit ones, of the norm and of
+ * the optimizer are set afterwards. */
 int spion_linear_selftest_bounded_wait(long long limit_cycles, void* cuda_stream);
 
 /* ------------------------------------------------------------------------------------------
@@ -509,7 +510,8 @@ int spion_linear_e4m3(const void* x, long long ldx, const float* x_scale, const 
  * fills the last block of 256 is left alone).  state_bits 32: fp32.  state_bits 8: m in e4m3, v in e5m2, and per block of 256 a scale each (powers of
  * two, [places / 256]); rounded up or down at random, with bits that are a function of seed, step, `index` and the value's place in its tensor.  steps:
  * device array, steps[index] counts the tensor's steps.  lr_dev: device scalar to read the rate from, or NULL: lr.  clip_value < 0: no clipping.  copy:
- * receives p in copy_type (SPION_BF16 or SPION_F16), or NULL.  m and v on 32 bytes.  workspace: 16 * min(count, 256) bytes
+ * receives p in copy_type (SPION_BF16 or SPION_F16), or NULL.  A bounded wait that gives up is reported by spion_linear_status; until then steps change
+ * nothing, counts included.  m and v on 32 bytes.  workspace: 16 * min(count, 256) bytes
  * on 16, of the call's stream.  The table is read before the call returns. */
 typedef struct spion_adamw_tensor {
   void* p;

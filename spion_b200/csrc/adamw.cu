@@ -250,10 +250,15 @@ template <class P> __device__ __forceinline__ bool on_boundaries(const Tensor& t
   return (((uintptr_t)t.p | (uintptr_t)t.g) & (8 * sizeof(P) - 1)) == 0 && ((uintptr_t)t.copy & 15) == 0;
 }
 
+// Set by a bounded wait of the ring below that gave up.  Until spion_linear_status has reported it all kernels of the optimizer leave at once: a step is whole or
+// nothing, counts included, but for the one whose wait it was.
+__device__ int g_adamw_status;
+
 constexpr int CTAS = 4;                                                  // resident on a multiprocessor
 template <class P, int BITS, bool FLUSH, int MAX>
 __global__ void __launch_bounds__(CTA, CTAS) k_adamw(const __grid_constant__ Table<MAX> a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lost = *reinterpret_cast<volatile int*>(&g_adamw_status);      // (on its way beside the first values)
   int i = 0;
   for (int chunk = blockIdx.x; chunk < a.s.chunks; chunk += gridDim.x) {
     i = tensor_of(a, chunk, i);
@@ -270,6 +275,7 @@ __global__ void __launch_bounds__(CTA, CTAS) k_adamw(const __grid_constant__ Tab
       key = mix(__float_as_uint(f.w) + (unsigned)(base >> 32));
     };
     if (base + BLOCK > t.n || !on_boundaries<P>(t)) {
+      if (lost != 0) return;
       edge_block<P, BITS, FLUSH>(a.s, t, base, t.n, lane, f, key, begun);
       continue;
     }
@@ -286,6 +292,7 @@ __global__ void __launch_bounds__(CTA, CTAS) k_adamw(const __grid_constant__ Tab
       now.sm = a.s.m_scale[at / BLOCK];
       now.sv = a.s.v_scale[at / BLOCK];
     }
+    if (lost != 0) return;
     begun();
     whole_block<P, BITS, FLUSH>(a.s, t, now, base, lane, f, key);
   }
@@ -299,9 +306,6 @@ template <class P> struct RingOf {
   static constexpr uint32_t VALUES = CHUNK * sizeof(P), STAGE = 2 * VALUES + 2 * CHUNK, SMEM = RING_STAGES * STAGE + 64;
 };
 static_assert(RING_CTAS * (RingOf<float>::SMEM + 1024) <= 233472, "shared memory of a multiprocessor");
-// Set by a bounded wait that gave up; launches after it leave at once until spion_linear_status has reported it.
-__device__ int g_adamw_status;
-
 template <class P, bool FLUSH, int MAX>
 __global__ void __launch_bounds__(CTA + 32, RING_CTAS) k_adamw_ring(const __grid_constant__ Table<MAX> a) {
   using R = RingOf<P>;
@@ -398,8 +402,10 @@ template <int MAX> __global__ void __launch_bounds__(MAX) k_adamw_begin(const __
   next_may_start();                                                      // k_adamw
   if ((int)threadIdx.x >= a.b.count) return;
   const int i = a.index[threadIdx.x];
+  const int lost = *reinterpret_cast<volatile int*>(&g_adamw_status);
   const float step = a.b.steps[i] + 1.f;
   const double lr = a.b.lr_dev != nullptr ? (double)*a.b.lr_dev : a.b.lr;
+  if (lost != 0) return;
   a.b.steps[i] = step;
   a.b.factors[threadIdx.x] =
       make_float4((float)(1.0 - lr * a.b.wd), (float)(lr / -expm1((double)step * a.b.log_b1)), (float)(1.0 / sqrt(-expm1((double)step * a.b.log_b2))),

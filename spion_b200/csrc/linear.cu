@@ -1634,7 +1634,8 @@ extern "C" int spion_linear_status(int reset) {
 }
 
 // One CTA waits, with a limit, on a barrier that nothing arrives on.
-__global__ void k_lin_wait_selftest(long long limit_cycles) {
+struct StatusWords { int* of[3]; };
+__global__ void k_lin_wait_selftest(long long limit_cycles, const StatusWords others) {
   __shared__ __align__(8) unsigned long long bar_storage;
   const uint32_t bar = smem_u32(&bar_storage);
   if (threadIdx.x == 0) {
@@ -1643,12 +1644,18 @@ __global__ void k_lin_wait_selftest(long long limit_cycles) {
   }
   __syncthreads();
   const bool ok = __syncthreads_and(mbar_wait_limit(bar, 0, limit_cycles));
-  if (!ok && threadIdx.x == 0) report(&g_lin_status, ERR_LOAD_WAIT);
+  if (!ok && threadIdx.x == 0) {
+    report(&g_lin_status, ERR_LOAD_WAIT);
+    for (int* word : others.of) report(word, ERR_LOAD_WAIT);
+  }
 }
 
 extern "C" int spion_linear_selftest_bounded_wait(long long limit_cycles, void* cuda_stream) {
   if (limit_cycles < 1 || limit_cycles > 2000000000LL) return SPION_ERR_ARG;
-  k_lin_wait_selftest<<<1, 128, 0, (cudaStream_t)cuda_stream>>>(limit_cycles);
+  const StatusWords others = {{linear_e4m3_status_word(), rmsnorm_status_word(), adamw_status_word()}};
+  for (int* word : others.of)
+    if (word == nullptr) return SPION_ERR_CUDA;
+  k_lin_wait_selftest<<<1, 128, 0, (cudaStream_t)cuda_stream>>>(limit_cycles, others);
   SPION_LAUNCH_CHECK();
   return SPION_OK;
 }

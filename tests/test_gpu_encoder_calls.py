@@ -184,3 +184,52 @@ def test_the_rings_on_two_streams_at_once():
     for q, m1, v1, scales1, steps in states[:2]:
         assert torch.equal(p, q) and torch.equal(m.view(torch.uint8), m1.view(torch.uint8)) and torch.equal(v.view(torch.uint8), v1.view(torch.uint8))
         assert all(torch.equal(a, b) for a, b in zip(scales, scales1)) and float(steps) == 4
+
+
+def test_a_wait_that_gave_up_leaves_nothing_half_done():
+    """The words that a bounded wait sets are set by the self-test of a short one.  Until they have been reported the optimizer leaves parameters, moments and counts
+    as they are and the 8-bit linear layer returns; after that all is as before."""
+    from spion_b200 import _lib
+    from spion_b200.optim import adamw_step
+    from spion_b200.quant import linear_e4m3, quantize_rows
+    g = torch.Generator(device="cuda").manual_seed(2)
+
+    def moments(n, bits):
+        at = -(-n // 256) * 256
+        m, v = torch.zeros(at, device="cuda"), torch.zeros(at, device="cuda")
+        if bits == 32:
+            return [m, v], None
+        return [m.to(torch.float8_e4m3fn), v.to(torch.float8_e5m2)], (torch.ones(at // 256, device="cuda"), torch.ones(at // 256, device="cuda"))
+
+    cases = []
+    for n, bits in ((16_000_001, 8), (5000, 8), (5000, 32)):
+        p, d = torch.randn(n, generator=g, device="cuda"), torch.randn(n, generator=g, device="cuda")
+        cases.append((p, d, *moments(n, bits), torch.zeros(1, device="cuda")))
+
+    def step():
+        for p, d, (m, v), scales, steps in cases:
+            adamw_step([p], [d], m, v, steps, scales=scales)
+
+    def state():
+        torch.cuda.synchronize()
+        return [t.clone().view(torch.uint8) for p, _, (m, v), scales, steps in cases for t in (p, m, v, steps, *(scales or ()))]
+
+    operands = [(quantize_rows(torch.randn(T, 512, generator=g, device="cuda")), quantize_rows(torch.randn(N, 512, generator=g, device="cuda")))
+                for T, N in ((4, 100), (700, 100), (20000, 1024))]
+    linears = lambda: [linear_e4m3(x, w) for x, w in operands]      # noqa: E731
+    step()
+    before, want = state(), linears()
+    assert _lib.lib.spion_linear_status(0) == 0
+    _lib.check(_lib.lib.spion_linear_selftest_bounded_wait(1000, torch.cuda.current_stream().cuda_stream))
+    try:
+        assert _lib.lib.spion_linear_status(0) != 0
+        step()
+        assert all(torch.equal(a, b) for a, b in zip(before, state()))
+        linears()
+        torch.cuda.synchronize()
+    finally:
+        assert _lib.lib.spion_linear_status(1) != 0 and _lib.lib.spion_linear_status(0) == 0
+    assert all(torch.equal(a, b) for a, b in zip(linears(), want))
+    step()
+    for (p, d, (m, v), scales, steps), first in zip(cases, (0, 6, 12)):
+        assert float(steps) == 2 and not torch.equal(p.view(torch.uint8), before[first])
