@@ -30,7 +30,8 @@ constexpr float SMALL = 0x1p-100f;        // what the scale of a row of zeros fo
 constexpr int CTA = 256;                  // threads of a CTA whose warps take rows of their own
 constexpr int MAX_PARTS = 1184;           // partial rows of a weight gradient: eight per multiprocessor of 148
 
-// Set by a bounded wait that gave up (the ring of the backward); launches of it after that leave at once until spion_linear_status has reported it.
+// Set by a bounded wait that gave up (the ring of the backward).  The gradients of the rows that its CTA had left are NaN then, and so are all of the launches
+// after it until spion_linear_status has reported it.
 __device__ int g_rms_status;
 
 struct FwdArgs {
@@ -382,6 +383,19 @@ __global__ void __launch_bounds__(TPR) k_rms_backward_ring(const BwdArgs a, cons
   const int t = threadIdx.x, left = a.N - t * 8;
   const uint32_t bars = tc::smem_u32(smem), rows0 = bars + RING_BARS;
   const long long step = gridDim.x;
+  auto give_up = [&](long long row) {                                      // what this CTA does not form is NaN, from this row on
+    float bad[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bad[e] = __int_as_float(0x7fffffff);
+    for (int c = t * 8; c < a.N; c += TPR * 8) {
+      for (long long r = row; r < a.M; r += step) {
+        if (a.dx != nullptr) Out<S, 8>::store(static_cast<S*>(a.dx) + r * a.N + c, bad);
+        if (a.dr != nullptr && a.dr_type == SPION_BF16) Out<__nv_bfloat16, 8>::store(static_cast<__nv_bfloat16*>(a.dr) + r * a.N + c, bad);
+        if (a.dr != nullptr && a.dr_type != SPION_BF16) Out<__half, 8>::store(static_cast<__half*>(a.dr) + r * a.N + c, bad);
+      }
+      if (a.part != nullptr) Out<float, 8>::store(a.part + (long long)blockIdx.x * a.N + c, bad);
+    }
+  };
   auto fill = [&](int st, long long row) {                                 // one thread
     const uint32_t bytes = a.N * (uint32_t)sizeof(S), dbytes = a.N * (uint32_t)sizeof(D), at = rows0 + st * ring.stage, bar = bars + 8 * st;
     tc::mbar_expect_tx(bar, bytes + dbytes + (a.ds != nullptr ? bytes : 0));
@@ -405,7 +419,7 @@ __global__ void __launch_bounds__(TPR) k_rms_backward_ring(const BwdArgs a, cons
   const float over_n = 1.0f / a.N;
   float rho = blockIdx.x < a.M ? a.rho[blockIdx.x] : 0.f;
   __syncthreads();
-  if (s_lost != 0) return;
+  if (s_lost != 0) return give_up(blockIdx.x);
   __syncthreads();
   for (long long row = blockIdx.x; row < a.M; row += step) {
     const float next = row + step < a.M ? a.rho[row + step] : 0.f;
@@ -439,7 +453,7 @@ __global__ void __launch_bounds__(TPR) k_rms_backward_ring(const BwdArgs a, cons
         for (int i = 0; i < ring.stages; ++i)                              // the copies under way end first, or this gives up again
           if (row + (i - st + (i < st ? ring.stages : 0)) * step < a.M) tc::mbar_wait(bars + 8 * i, i < st ? ph ^ 1 : ph);
       }
-      return;
+      return give_up(row);
     }
     const bool more = t == 0 && row + ring.stages * step < a.M;
     if (NV == 1) {                                                         // the thread's piece is in registers

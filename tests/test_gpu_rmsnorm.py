@@ -326,3 +326,33 @@ def test_weights_that_are_not_finite(N):
                 z = rms_norm(x, w, EPS, res=res)
                 z = z if res is None else z[1]
                 assert torch.equal(z.isnan(), y.isnan()) and torch.equal(z.isinf(), y.isinf())
+
+
+def test_gradients_after_a_wait_that_gave_up_are_nan():
+    """The word that a bounded wait of the backward's ring sets is set by the self-test of a short one: until it has been reported the gradients of that kernel are
+    NaN, not what their memory held; after that they are as before.  (The other kernels wait for nothing.)"""
+    from spion_b200 import _lib
+    from spion_b200.rmsnorm import rms_norm
+    g = torch.Generator(device="cuda").manual_seed(2)
+    calls = []
+    for M, N, stream, branch in ((600, 2048, "fp32", "bf16"), (3, 4096, "fp32", None), (200, 16384, "bf16", None), (5, 1024, "fp32", "fp16"), (300, 4000, "fp16", "fp16")):
+        x = torch.randn(M, N, generator=g, device="cuda").to(T[stream]).requires_grad_()
+        r = None if branch is None else torch.randn(M, N, generator=g, device="cuda").to(T[branch]).requires_grad_()
+        calls.append((x, r, torch.rand(N, generator=g, device="cuda", requires_grad=True), torch.randn(M, N, generator=g, device="cuda").to(T[stream])))
+
+    def gradients():
+        out = []
+        for x, r, w, dy in calls:
+            y = rms_norm(x, w, EPS, res=r)
+            out += torch.autograd.grad(y if r is None else y[1], (x, w) if r is None else (x, w, r), dy)
+        return out
+
+    want = gradients()
+    torch.cuda.synchronize()
+    assert all(bool(torch.isfinite(t).all()) for t in want) and _lib.lib.spion_linear_status(0) == 0
+    _lib.check(_lib.lib.spion_linear_selftest_bounded_wait(1000, torch.cuda.current_stream().cuda_stream))
+    try:
+        assert all(bool(t.isnan().all()) for t in gradients())
+    finally:
+        assert _lib.lib.spion_linear_status(1) != 0 and _lib.lib.spion_linear_status(0) == 0
+    assert all(torch.equal(a, b) for a, b in zip(gradients(), want))
