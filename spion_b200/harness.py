@@ -15,7 +15,7 @@ import contextlib
 import torch
 import torch.nn as nn
 
-from . import dp
+from . import _lib, dp
 from ._lib import SpionError
 from .attention import Attention, no_global_hooks, untouched
 from .layernorm import mask_rows, sequence_means
@@ -300,6 +300,8 @@ class Classifier(nn.Module):
 class Trainer:
     """dense step(s) -> discover -> sparse steps, with one flat-bucket all-reduce per step."""
 
+    status_every = 256               # steps after which a wait that gave up in a kernel ends the run
+
     def __init__(self, config, lr: float = 1e-4, device=None, seed: int = 0):
         self.config = config
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
@@ -333,6 +335,24 @@ class Trainer:
                 if self.fused_opt:
                     self.opt.write_copies(*self._shadow)
         self.allreduce_events = None     # set to a list to collect (start, end) CUDA events around the gradient all-reduce
+        self.steps = 0                   # taken, captured ones by their replays
+
+    def check_device_status(self) -> None:
+        """Raise if a bounded wait of a kernel has given up since it was last asked: results since then were not written.  Synchronises; under a
+        capture it asks nothing."""
+        if torch.cuda.is_current_stream_capturing():
+            return
+        with torch.cuda.device(self.device):
+            for m in self.model.modules():
+                if hasattr(m, "check_device_status"):
+                    m.check_device_status()
+            _lib.check(_lib.lib.spion_linear_status(1), "device status")
+
+    def _taken(self):
+        if not torch.cuda.is_current_stream_capturing():
+            self.steps += 1
+            if self.steps % self.status_every == 0:
+                self.check_device_status()
 
     def step(self, ids, label, is_attn=False):
         loss, maps = self.model(ids, label, self.mat_lst, is_attn)
@@ -346,6 +366,7 @@ class Trainer:
         else:
             self.bucket.allreduce_mean()
         self._update()
+        self._taken()
         return loss.detach(), maps
 
     def _update(self):
@@ -363,7 +384,7 @@ class Trainer:
     def evaluate(self, ids, label):
         """Mean loss and share of right answers of one batch in the sparse phase with the weights as they are now, without gradients or dropout.
         ``config["eval_linear_bits"] = 8``: with the encoder's linear layers on 8-bit operands, quantised by the call; else on none, whatever
-        ``Classifier.quantize`` has left."""
+        ``Classifier.quantize`` has left.  Synchronises, and raises if a kernel's wait gave up (``check_device_status``)."""
         if self.mat_lst is None:
             raise RuntimeError("evaluate after discover()")
         eight = self._evaluates_in_8_bits()
@@ -372,7 +393,9 @@ class Trainer:
         try:
             with torch.no_grad(), self.model.quantized_as(eight):
                 scores = self.model.scores(ids, self.mat_lst)
-                return nn.functional.cross_entropy(scores, label), (scores.argmax(-1) == label).float().mean()
+                out = nn.functional.cross_entropy(scores, label), (scores.argmax(-1) == label).float().mean()
+            self.check_device_status()
+            return out
         finally:
             self.model.train(training)
 
@@ -444,6 +467,7 @@ class Trainer:
                 ev[2].record()
             ev[3].record()
             self.allreduce_events.append(tuple(ev))
+        self._taken()
         return self._g_loss
 
     def discover(self, maps, threshold=None):

@@ -12,7 +12,7 @@ from collections import defaultdict
 import torch
 
 from . import _ops
-from ._lib import SpionError
+from ._lib import SpionError, check, lib
 
 BLOCK = 256
 # entries of torch.optim.AdamW's groups that say how it computes: a state is loaded without them
@@ -153,6 +153,20 @@ class AdamW(torch.optim.Optimizer):
                            copies=copies)
                 number += 1
         return loss
+
+    def check_device_status(self) -> None:
+        """Raise if a bounded wait of the library's kernels has given up since it was last asked (steps after that changed nothing).  Synchronises;
+        under a capture it asks nothing."""
+        if torch.cuda.is_current_stream_capturing():
+            return
+        for device in {p.device for held, _ in self._moments for p in held}:
+            with torch.cuda.device(device):
+                check(lib.spion_linear_status(1), "device status")
+
+    def state_dict(self):
+        """As the base class's; raises if steps have been left out (``check_device_status``)."""
+        self.check_device_status()
+        return super().state_dict()
 
     def load_state_dict(self, state_dict):
         """Moments are copied into the arrays that this optimizer keeps; they have to be of its ``state_bits``."""

@@ -301,3 +301,60 @@ def test_every_stage_of_an_8_bit_evaluation(monkeypatch):
             want = encoder.norm(X + branch) * mask[..., None]
         assert torch.equal(out, want.to(out.dtype)) and not bool(out[mask == 0].any())
         assert not torch.equal(out, unquantised)
+
+
+@pytest.mark.parametrize("optimizer", ["fused", "torch"])
+def test_a_wait_that_gave_up_ends_a_run(optimizer):
+    """Training whose kernels have left asks for the status by itself, and evaluation and the optimizer's state do: each raises once, then goes on."""
+    from spion_b200 import _lib
+    tr, ids, lab = trainer(optimizer=optimizer)
+    start(tr, ids, lab)
+    tr.step(ids, lab)
+    tr.check_device_status()
+
+    def lost():
+        _lib.check(_lib.lib.spion_linear_selftest_bounded_wait(1000, torch.cuda.current_stream().cuda_stream))
+
+    def raises(call):
+        lost()
+        with pytest.raises(_lib.SpionError, match="timed out"):
+            call()
+        tr.check_device_status()
+
+    raises(tr.check_device_status)
+    raises(lambda: tr.evaluate(ids, lab))
+    assert tr.model.training
+    if optimizer == "fused":
+        raises(tr.opt.state_dict)
+    assert np.isfinite(float(tr.evaluate(ids, lab)[0]))
+    tr.status_every = 3
+
+    def steps(call):
+        tr.steps = 0
+        call(), call()
+        with pytest.raises(_lib.SpionError, match="timed out"):
+            call()
+        tr.check_device_status()
+
+    lost()
+    steps(lambda: tr.step(ids, lab))
+    start_again, ids, lab = trainer(optimizer=optimizer)
+    start(start_again, ids, lab)
+    tr = start_again
+    tr.status_every = 3
+    tr.capture_sparse_step(ids, lab)
+    lost()
+    steps(lambda: tr.step_graph(ids, lab))
+    assert set(tr.opt.state_dict()["state"][0]) >= {"step", "exp_avg"}
+
+
+def test_an_evaluation_and_a_state_under_a_capture():
+    tr, ids, lab = trainer()
+    start(tr, ids, lab)
+    want, _ = tr.evaluate(ids, lab)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, _ = tr.evaluate(ids, lab)
+        state = tr.opt.state_dict()
+    graph.replay()
+    assert float(loss) == float(want) and len(state["state"]) == len(tr.bucket.params)
