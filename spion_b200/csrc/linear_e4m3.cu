@@ -40,7 +40,7 @@ constexpr int L8_EPI = 8;                                 // warps that write re
 constexpr int L8_THREADS = 32 * (2 + L8_EPI);
 constexpr uint32_t L8_OUT = 4096;                         // results on their way out: 32 rows of up to 128 bytes
 // BK: bytes of the contraction in a chunk, 128, or 64 where there are no more: a box that is half outside of its matrix takes longer than a full one (131072
-// tokens of 64 features to 64: 14.6 us, 12.3).  CTAS: on a multiprocessor.  Two where the contraction is a chunk or two: a tile's latencies are most of
+// tokens of 64 features to 64: 14.6 us, 12.3).  CTAS: on a multiprocessor.  Two where the contraction is a few chunks: a tile's latencies are most of
 // its time then.
 // PAIR: two CTAs of a cluster share a tile of 256 tokens; each brings its half of the tokens and of the features, one of them issues the products for both.
 template <int BN, int BK, int CTAS, bool PAIR> struct L8 {
@@ -554,13 +554,15 @@ template <class Y> int launch_any(const Lin8Args& a, cudaStream_t st) {
   // 4096 to 4096 features, few / tiles: 8 tokens 6.1 us / 11.6, 16 tokens (twice the products) 10.4 / 11.6; 512 to 16384, 32 tokens 26 / 6.3: mma.sync is slow on
   // 8-bit operands here, and what it does for more tokens outlasts the weights
   if (a.T <= FEW_TOKENS) return launch_few<Y>(a, st);
-  // The largest tile that leaves one to every multiprocessor.  Two small CTAs a multiprocessor up to 256 inner features, else pairs; two small / pairs: 65536 x
-  // 512 to 256 16.4 us / 18.2, to 1024 52.4 / 51.3, 32768 x 1024 to 1024 44.6 / 35.9, 16384 x 2048 to 2048 73 / 53.
+  // The largest tile that leaves one to every multiprocessor.  Pairs from more than 512 inner features on, two small CTAs a multiprocessor below; two small / pairs:
+  // 65536 x 256 to 256 13.4 us / 16.7, x 384 to 1024 43.1 / 49.1, x 512 to 256 18.6 / 19.8 and to 1024 49.3 / 50.7; 8192 x 640 to 4096 29.9 / 29.6, 32768 x 768 to
+  // 1024 35.4 / 30.8, x 1024 to 1024 42.9 / 33.8.  Where there are too few tiles of pairs, one CTA a multiprocessor from more than 256 on, two / one: 20000 x 320 to 64
+  // 5.5 / 6.1, 131072 x 512 to 64 17.7 / 17.1, 512 x 320 to 1024 3.9 / 3.7.
   const long long rows_ = (a.T + 127) / 128, sms = sm_count();
   const bool wide = a.N > 64 && rows_ * ((a.N + 127) / 128) >= sms;
   if (a.K <= 64) return wide ? launch_tiles<128, 64, 2, false, Y>(a, st) : launch_tiles<64, 64, 2, false, Y>(a, st);
   if (a.K <= 256) return wide ? launch_tiles<128, 128, 2, false, Y>(a, st) : launch_tiles<64, 128, 2, false, Y>(a, st);
-  if (a.N > 128 && rows_ * ((a.N + 255) / 256) >= sms) return launch_tiles<256, 128, 1, true, Y>(a, st);
+  if (a.N > 128 && rows_ * ((a.N + 255) / 256) >= sms) return a.K <= 512 ? launch_tiles<128, 128, 2, false, Y>(a, st) : launch_tiles<256, 128, 1, true, Y>(a, st);
   return wide ? launch_tiles<128, 128, 1, false, Y>(a, st) : launch_tiles<64, 128, 1, false, Y>(a, st);
 }
 
