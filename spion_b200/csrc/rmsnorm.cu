@@ -585,7 +585,9 @@ template <class S, class R, class Y, bool NORM = true>
 int forward(const FwdArgs& a, cudaStream_t st) {
   const bool vec = a.N % 8 == 0 && on_boundary(a.x, a.ldx, type_code<S>()) && on_boundary(a.r, a.ldr, type_code<R>()) &&
                    on_boundary(a.s, a.N, type_code<S>()) && on_boundary(a.y, a.ldy, type_code<Y>()) && on_boundary(a.w, a.N, a.w_type);
-  const bool few = a.M <= sm_count();                    // as many threads as pieces
+  // Where there is a multiprocessor to every row, a thread to a piece up to 4096 values.  That / four pieces a thread, us, one row, 148 rows: bf16 with a residual 2048 values
+  // 1.97 / 2.18, 2.05 / 2.26, 4096 2.35 / 2.27, 2.45 / 2.40 (to e4m3 2.31 / 2.35, 2.45 / 2.61, fp32 148 rows 2.81 / 3.38), 8192 3.08 / 2.69, 4.55 / 4.51.
+  const bool few = a.M <= sm_count();
   if (vec) {
     const int n = a.N / 8;
     if (n <= 8) launch_forward<NORM, S, R, Y, 8, 1, 8, 2>(a, st);
@@ -595,7 +597,6 @@ int forward(const FwdArgs& a, cudaStream_t st) {
     else if (n <= 128) launch_forward<NORM, S, R, Y, 8, 4, 32>(a, st);
     else if (few && n <= 256) launch_forward<NORM, S, R, Y, 8, 1, 256>(a, st);
     else if (few && n <= 512) launch_forward<NORM, S, R, Y, 8, 1, 512>(a, st);
-    else if (few && n <= 1024) launch_forward<NORM, S, R, Y, 8, 1, 1024>(a, st);
     else if (n <= 256) launch_forward<NORM, S, R, Y, 8, 4, 64>(a, st);
     else if (n <= 512) launch_forward<NORM, S, R, Y, 8, 4, 128>(a, st);
     else if (n <= 1024) launch_forward<NORM, S, R, Y, 8, 4, 256>(a, st);
