@@ -474,8 +474,8 @@ int spion_linear_prepare(int fp32);
 /* SPION_ERR_TIMEOUT when a bounded wait of these kernels has given up since the last reset (synchronises the device).  Until then
  * every call of them returns without writing its results. */
 int spion_linear_status(int reset);
-/* Failure-path self-test that faults nothing, as spion_selftest_bounded_wait: the status words of the linear layers, of the 8-bit ones, of the norm and of
- * the optimizer are set afterwards. */
+/* Failure-path self-test that faults nothing, as spion_selftest_bounded_wait: the status words of the linear layers, of the 8-bit ones and of the norm are set
+ * afterwards. */
 int spion_linear_selftest_bounded_wait(long long limit_cycles, void* cuda_stream);
 
 /* ------------------------------------------------------------------------------------------
@@ -489,6 +489,7 @@ int spion_rmsnorm_forward(const void* x, long long ldx, int x_type, const void* 
                           void* cuda_stream);
 /* Its backward from s (rows lds apart), dy [M, N] (the type of y) and ds [M, N] (the type of s; may be NULL: the gradient of s from its other
  * consumers): dx [M, N] in s's type and dres [M, N], the same in 16 bits (either may be NULL), dw [N] in w's type (may be NULL), summed in a fixed order.
+ * A bounded wait that gives up is reported by spion_linear_status: the gradients that it left, and those of later calls until then, are NaN.
  * workspace: spion_rmsnorm_workspace_floats(M, N) floats (with dw). */
 long long spion_rmsnorm_workspace_floats(long long M, int N);
 int spion_rmsnorm_backward(const void* s, long long lds, int s_type, const void* dy, int dy_type, const void* ds, const void* w, int w_type,
@@ -510,8 +511,8 @@ int spion_linear_e4m3(const void* x, long long ldx, const float* x_scale, const 
  * fills the last block of 256 is left alone).  state_bits 32: fp32.  state_bits 8: m in e4m3, v in e5m2, and per block of 256 a scale each (powers of
  * two, [places / 256]); rounded up or down at random, with bits that are a function of seed, step, `index` and the value's place in its tensor.  steps:
  * device array, steps[index] counts the tensor's steps.  lr_dev: device scalar to read the rate from, or NULL: lr.  clip_value < 0: no clipping.  copy:
- * receives p in copy_type (SPION_BF16 or SPION_F16), or NULL.  A bounded wait that gives up is reported by spion_linear_status; until then steps change
- * nothing, counts included.  m and v on 32 bytes.  workspace: 16 * min(count, 256) bytes
+ * receives p in copy_type (SPION_BF16 or SPION_F16), or NULL.  After a bounded wait of a linear layer or of the norm gave up a step changes nothing, counts
+ * included, until spion_linear_status has reported it.  m and v on 32 bytes.  workspace: 16 * min(count, 256) bytes
  * on 16, of the call's stream.  The table is read before the call returns. */
 typedef struct spion_adamw_tensor {
   void* p;

@@ -10,17 +10,15 @@
 // moment: the same bits on every run, nothing to store.  v is never rounded to zero, which would leave m / eps behind.
 //
 // Bound by the passes over parameters, gradients and moments: 28 bytes a value with 32-bit moments in fp32 (75 million values 337 us, 6.2 TB/s), 16 with
-// 8-bit ones, where the arithmetic of the codes is nearly as long (214 us; in bf16, 10 bytes a value, 216: that arithmetic).  A warp takes a block of
+// 8-bit ones, where the arithmetic of the codes is nearly as long (213 us; in bf16, 10 bytes a value, 205: that arithmetic; with bulk copies to shared memory
+// three chunks ahead 213 and 208, one tensor of 75 million 221 instead of 212, so there are none).  A warp takes a block of
 // 256 values at a time, eight to a lane in one access of each array, so the block's maxima stay in registers.  The table of tensors travels as a kernel
 // parameter: nothing is uploaded or kept between calls, and a captured step replays with the addresses it was captured with.
 #include <math.h>
 
-#include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include "rows.cuh"
-#include "tc_ptx.cuh"
 
 using namespace rows;
 
@@ -38,7 +36,7 @@ struct Tensor {
 struct Step {
   void *m, *v;
   float *m_scale, *v_scale;   // 8 bits: one per block
-  const float4* factors;      // of each tensor of the launch, from k_adamw_begin
+  const float4* factors;      // of each tensor of the launch, from k_adamw_begin; z < 0: nothing is to be changed
   float b1, b2, c1, c2;       // betas and what is left of one
   float eps, clip;            // clip < 0: none
   int count, chunks, copy_type;
@@ -217,6 +215,7 @@ __device__ __forceinline__ void edge_block(const Step& s, const Tensor& t, long 
     }
   }
   begun();
+  if (f.z < 0.f) return;
   update<BITS, FLUSH>(s, f, p, g, m, v, sm, sv, cm, cv, (unsigned)(base + lane), 32, key);
   if (BITS == 8 && lane == 0) s.m_scale[at / BLOCK] = sm, s.v_scale[at / BLOCK] = sv;
 #pragma unroll
@@ -250,15 +249,10 @@ template <class P> __device__ __forceinline__ bool on_boundaries(const Tensor& t
   return (((uintptr_t)t.p | (uintptr_t)t.g) & (8 * sizeof(P) - 1)) == 0 && ((uintptr_t)t.copy & 15) == 0;
 }
 
-// Set by a bounded wait of the ring below that gave up.  Until spion_linear_status has reported it all kernels of the optimizer leave at once: a step is whole or
-// nothing, counts included, but for the one whose wait it was.
-__device__ int g_adamw_status;
-
 constexpr int CTAS = 4;                                                  // resident on a multiprocessor
 template <class P, int BITS, bool FLUSH, int MAX>
 __global__ void __launch_bounds__(CTA, CTAS) k_adamw(const __grid_constant__ Table<MAX> a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int lost = *reinterpret_cast<volatile int*>(&g_adamw_status);      // (on its way beside the first values)
   int i = 0;
   for (int chunk = blockIdx.x; chunk < a.s.chunks; chunk += gridDim.x) {
     i = tensor_of(a, chunk, i);
@@ -275,7 +269,6 @@ __global__ void __launch_bounds__(CTA, CTAS) k_adamw(const __grid_constant__ Tab
       key = mix(__float_as_uint(f.w) + (unsigned)(base >> 32));
     };
     if (base + BLOCK > t.n || !on_boundaries<P>(t)) {
-      if (lost != 0) return;
       edge_block<P, BITS, FLUSH>(a.s, t, base, t.n, lane, f, key, begun);
       continue;
     }
@@ -292,96 +285,9 @@ __global__ void __launch_bounds__(CTA, CTAS) k_adamw(const __grid_constant__ Tab
       now.sm = a.s.m_scale[at / BLOCK];
       now.sv = a.s.v_scale[at / BLOCK];
     }
-    if (lost != 0) return;
     begun();
+    if (f.z < 0.f) return;
     whole_block<P, BITS, FLUSH>(a.s, t, now, base, lane, f, key);
-  }
-}
-
-// The same for many values with 8-bit moments, where a block's arithmetic takes as long as its way from memory: a warp of its own keeps three chunks of 2048
-// values under way to shared memory by bulk copies while eight warps work.  75 million fp32 values: 257 us without
-// it (4.6 TB/s; 70 instructions a value, two thirds of the issue slots), 214 with it (5.6 TB/s).
-constexpr int RING_STAGES = 3, RING_CTAS = 3;
-template <class P> struct RingOf {
-  static constexpr uint32_t VALUES = CHUNK * sizeof(P), STAGE = 2 * VALUES + 2 * CHUNK, SMEM = RING_STAGES * STAGE + 64;
-};
-static_assert(RING_CTAS * (RingOf<float>::SMEM + 1024) <= 233472, "shared memory of a multiprocessor");
-template <class P, bool FLUSH, int MAX>
-__global__ void __launch_bounds__(CTA + 32, RING_CTAS) k_adamw_ring(const __grid_constant__ Table<MAX> a) {
-  using R = RingOf<P>;
-  extern __shared__ __align__(128) uint8_t smem[];
-  const uint32_t rows0 = tc::smem_u32(smem), full = rows0 + RING_STAGES * R::STAGE, empty = full + 8 * RING_STAGES;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < RING_STAGES; ++i) tc::mbar_init(full + 8 * i, 1), tc::mbar_init(empty + 8 * i, CTA / 32);
-    tc::fence_barrier_init();
-    tc::fence_proxy_async();
-  }
-  if (__syncthreads_or(*reinterpret_cast<volatile int*>(&g_adamw_status))) return;
-  int i = 0, st = 0, ph = 0;
-  // a chunk goes through the ring if all of it is there and lies on the boundaries: both sides ask the same
-  auto copied = [&](const Tensor& t, long long begin) { return begin + CHUNK <= t.n && on_boundaries<P>(t); };
-  if (warp == CTA / 32) {
-    if (lane != 0) return;
-    bool ok = true;
-    long long fills = 0;
-    for (int chunk = blockIdx.x; chunk < a.s.chunks && ok; chunk += gridDim.x) {
-      i = tensor_of(a, chunk, i);
-      const Tensor& t = a.t[i];
-      const long long begin = (long long)(chunk - a.chunk[i]) * CHUNK;
-      if (!copied(t, begin)) continue;
-      ok = tc::mbar_wait(empty + 8 * st, ph ^ 1);
-      if (!ok) break;
-      const uint32_t to = rows0 + st * R::STAGE, bar = full + 8 * st;
-      tc::mbar_expect_tx(bar, R::STAGE);
-      tc::bulk_load(to, static_cast<const P*>(t.p) + begin, bar, R::VALUES);
-      tc::bulk_load(to + R::VALUES, static_cast<const P*>(t.g) + begin, bar, R::VALUES);
-      tc::bulk_load(to + 2 * R::VALUES, static_cast<const uint8_t*>(a.s.m) + t.at + begin, bar, CHUNK);
-      tc::bulk_load(to + 2 * R::VALUES + CHUNK, static_cast<const uint8_t*>(a.s.v) + t.at + begin, bar, CHUNK);
-      ++fills;
-      if (++st == RING_STAGES) st = 0, ph ^= 1;
-    }
-    if (!ok) {                                                             // the copies under way end first, or this gives up again
-      atomicOr(&g_adamw_status, 1);
-      for (long long j = fills > RING_STAGES ? fills - RING_STAGES : 0; j < fills; ++j) tc::mbar_wait(full + 8 * (int)(j % RING_STAGES), (int)(j / RING_STAGES) & 1);
-    }
-    return;
-  }
-  bool waited = false;
-  for (int chunk = blockIdx.x; chunk < a.s.chunks; chunk += gridDim.x) {
-    i = tensor_of(a, chunk, i);
-    const Tensor& t = a.t[i];
-    const long long begin = (long long)(chunk - a.chunk[i]) * CHUNK, base = begin + warp * BLOCK;
-    float4 f;
-    unsigned key;
-    auto begun = [&] {
-      if (!waited) wait_for_kernel_before();
-      waited = true;
-      f = __ldcg(a.s.factors + i);
-      key = mix(__float_as_uint(f.w) + (unsigned)(begin >> 32));
-    };
-    if (!copied(t, begin)) {
-      if (base < t.n) edge_block<P, 8, FLUSH>(a.s, t, base, t.n, lane, f, key, begun);
-      continue;
-    }
-    Lane<P, 8> now;
-    now.sm = a.s.m_scale[(t.at + base) / BLOCK];
-    now.sv = a.s.v_scale[(t.at + base) / BLOCK];
-    begun();
-    if (!__all_sync(0xffffffffu, tc::mbar_wait(full + 8 * st, ph))) {
-      if (lane == 0) atomicOr(&g_adamw_status, 2);
-      return;
-    }
-    const uint8_t* const from = smem + st * R::STAGE;
-    const int k = warp * BLOCK + 8 * lane;
-    now.p.load_shared(reinterpret_cast<const P*>(from) + k);
-    now.g.load_shared(reinterpret_cast<const P*>(from + R::VALUES) + k);
-    now.m = *reinterpret_cast<const uint2*>(from + 2 * R::VALUES + k);
-    now.v = *reinterpret_cast<const uint2*>(from + 2 * R::VALUES + CHUNK + k);
-    __syncwarp();
-    if (lane == 0) tc::mbar_arrive(empty + 8 * st);
-    whole_block<P, 8, FLUSH>(a.s, t, now, base, lane, f, key);
-    if (++st == RING_STAGES) st = 0, ph ^= 1;
   }
 }
 
@@ -393,6 +299,7 @@ struct Begin {
   double lr, wd, log_b1, log_b2;
   unsigned seed;
   int count;
+  const int *linear, *norm;   // status words of the kernels that form gradients with bounded waits
 };
 template <int MAX> struct Indices {
   Begin b;
@@ -402,14 +309,14 @@ template <int MAX> __global__ void __launch_bounds__(MAX) k_adamw_begin(const __
   next_may_start();                                                      // k_adamw
   if ((int)threadIdx.x >= a.b.count) return;
   const int i = a.index[threadIdx.x];
-  const int lost = *reinterpret_cast<volatile int*>(&g_adamw_status);
+  const int lost = *static_cast<const volatile int*>(a.b.linear) | *static_cast<const volatile int*>(a.b.norm);
   const float step = a.b.steps[i] + 1.f;
   const double lr = a.b.lr_dev != nullptr ? (double)*a.b.lr_dev : a.b.lr;
-  if (lost != 0) return;
-  a.b.steps[i] = step;
-  a.b.factors[threadIdx.x] =
-      make_float4((float)(1.0 - lr * a.b.wd), (float)(lr / -expm1((double)step * a.b.log_b1)), (float)(1.0 / sqrt(-expm1((double)step * a.b.log_b2))),
-                  __uint_as_float(mix(a.b.seed + mix((unsigned)step * 0x9E3779B1u + (unsigned)i))));
+  float4 f = make_float4((float)(1.0 - lr * a.b.wd), (float)(lr / -expm1((double)step * a.b.log_b1)), (float)(1.0 / sqrt(-expm1((double)step * a.b.log_b2))),
+                         __uint_as_float(mix(a.b.seed + mix((unsigned)step * 0x9E3779B1u + (unsigned)i))));
+  if (lost != 0) f.z = -1.f;                                             // a wait gave up and has not been reported: the gradients may be what it left
+  else a.b.steps[i] = step;
+  a.b.factors[threadIdx.x] = f;
 }
 
 template <class P, int BITS, bool FLUSH, int MAX>
@@ -420,11 +327,8 @@ int launch(const Step& s, const Begin& b, const spion_adamw_tensor* ts, int coun
   a.s.count = 0;
   ix.b = b;
   ix.b.count = 0;
-  long long chunks = 0, total = 0;
-  for (int i = 0; i < count; ++i) total += ts[i].n;
-  // the ring from sixteen chunks a CTA on; us without / with it: 7.5 million values 26 / 28.7, 15 million 48 / 49, 75 million 257 / 214
-  const bool ring = BITS == 8 && total >= (long long)sm_count() * RING_CTAS * CHUNK * 16;
-  const long long most = (long long)sm_count() * (ring ? RING_CTAS : CTAS);
+  long long chunks = 0;
+  const long long most = (long long)sm_count() * CTAS;
   for (int full = 1; full >= 0; --full)                                  // tensors without values last: they have a count only
     for (int i = 0; i < count; ++i) {
       if ((ts[i].n > 0) != (full == 1)) continue;
@@ -439,19 +343,6 @@ int launch(const Step& s, const Begin& b, const spion_adamw_tensor* ts, int coun
   k_adamw_begin<MAX><<<1, MAX, 0, st>>>(ix);
   SPION_LAUNCH_CHECK();
   const dim3 grid((unsigned)(chunks < most ? chunks : most));
-  if constexpr (BITS == 8) {
-    if (ring) {
-      static std::atomic<uint64_t> ready{0};                               // devices on which the kernel has its shared memory
-      int dev = 0;
-      SPION_CUDA_TRY(cudaGetDevice(&dev));
-      if (dev >= 64 || !(ready.load() >> dev & 1)) {
-        SPION_CUDA_TRY(cudaFuncSetAttribute(k_adamw_ring<P, FLUSH, MAX>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)RingOf<P>::SMEM));
-        if (dev < 64) ready.fetch_or(1ull << dev);
-      }
-      SPION_CUDA_TRY(launch_after(k_adamw_ring<P, FLUSH, MAX>, grid, dim3(CTA + 32), RingOf<P>::SMEM, st, a));
-      return SPION_OK;
-    }
-  }
   if (chunks > 0) SPION_CUDA_TRY(launch_after(k_adamw<P, BITS, FLUSH, MAX>, grid, dim3(CTA), 0, st, a));
   return SPION_OK;
 }
@@ -469,11 +360,6 @@ int launches(const Step& s, const Begin& b, const spion_adamw_tensor* ts, int co
 
 }  // namespace
 
-int* adamw_status_word() {
-  void* word = nullptr;
-  return cudaGetSymbolAddress(&word, g_adamw_status) == cudaSuccess ? static_cast<int*>(word) : nullptr;
-}
-
 extern "C" int spion_adamw_step(const spion_adamw_tensor* host_tensors, int count, int type, int state_bits, void* m, void* v, float* m_scale,
                                 float* v_scale, float* steps, const float* lr_dev, double lr, double beta1, double beta2, double eps,
                                 double weight_decay, double clip_value, unsigned seed, int copy_type, void* workspace, void* cuda_stream) {
@@ -488,13 +374,15 @@ extern "C" int spion_adamw_step(const spion_adamw_tensor* host_tensors, int coun
     if (t.n < 0 || t.at < 0 || t.at % BLOCK || t.index < 0 || (t.n > 0 && (t.p == nullptr || t.g == nullptr))) return SPION_ERR_ARG;
     if (t.copy != nullptr && copy_type != SPION_BF16 && copy_type != SPION_F16) return SPION_ERR_ARG;
   }
+  if (type != SPION_F32 && type != SPION_BF16 && type != SPION_F16) return SPION_ERR_UNSUPPORTED;
+  const int *const linear = linear_status_word(), *const norm = rmsnorm_status_word();
+  if (linear == nullptr || norm == nullptr) return SPION_ERR_CUDA;
   const Step s = {m, v, m_scale, v_scale, static_cast<const float4*>(workspace), (float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2),
                   (float)eps, clip_value >= 0 ? (float)clip_value : -1.f, 0, 0, copy_type};
-  const Begin b = {steps, static_cast<float4*>(workspace), lr_dev, lr, weight_decay, log(beta1), log(beta2), seed, 0};
+  const Begin b = {steps, static_cast<float4*>(workspace), lr_dev, lr, weight_decay, log(beta1), log(beta2), seed, 0, linear, norm};
   const cudaStream_t st = (cudaStream_t)cuda_stream;
   if (type == SPION_F32) return state_bits == 8 ? launches<float, 8>(s, b, host_tensors, count, st) : launches<float, 32>(s, b, host_tensors, count, st);
   if (type == SPION_BF16)
     return state_bits == 8 ? launches<__nv_bfloat16, 8>(s, b, host_tensors, count, st) : launches<__nv_bfloat16, 32>(s, b, host_tensors, count, st);
-  if (type == SPION_F16) return state_bits == 8 ? launches<__half, 8>(s, b, host_tensors, count, st) : launches<__half, 32>(s, b, host_tensors, count, st);
-  return SPION_ERR_UNSUPPORTED;
+  return state_bits == 8 ? launches<__half, 8>(s, b, host_tensors, count, st) : launches<__half, 32>(s, b, host_tensors, count, st);
 }

@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 #include <stdio.h>
+#include <atomic>
 
 #include "../../include/spion_b200.h"
 
@@ -147,11 +148,24 @@ int sm_count();
 
 // linear.cu: status word of the linear layers on the current device, after the work of a stream
 int linear_status(int reset, cudaStream_t st);
-// linear_e4m3.cu, rmsnorm.cu, adamw.cu: where those of the layers on 8-bit operands, of the norm's backward and of the optimizer lie (null: the query failed);
-// reported with the former
+// Where the status words of linear.cu, linear_e4m3.cu and rmsnorm.cu lie on the current device (null: the query failed); reported together
+int* linear_status_word();
 int* linear_e4m3_status_word();
 int* rmsnorm_status_word();
-int* adamw_status_word();
+// ... asked once per device: steps of the optimizer ask each time
+struct StatusWord {
+  std::atomic<int*> at[64] = {};
+  int* on_this_device(const int& symbol) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
+    int* known = dev < 64 ? at[dev].load() : nullptr;
+    if (known != nullptr) return known;
+    void* word = nullptr;
+    if (cudaGetSymbolAddress(&word, symbol) != cudaSuccess) return nullptr;
+    if (dev < 64) at[dev].store(static_cast<int*>(word));
+    return static_cast<int*>(word);
+  }
+};
 
 // Device memory of the contexts, from one pool per device that keeps up to 64 MB of what was given back, beside what is in use: mapping
 // and unmapping two or three megabytes took 2 to 4 ms of every context's life.  Freeing waits for the device, as cudaFree does (where it

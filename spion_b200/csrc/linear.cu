@@ -1605,18 +1605,20 @@ extern "C" int spion_linear_prepare(int fp32) {
   return prepare_wgrad<true, true>();
 }
 
+int* linear_status_word() {
+  static StatusWord word;
+  return word.on_this_device(g_lin_status);
+}
 int linear_status(int reset, cudaStream_t st) {
-  static const char* const whose[] = {"linear layers", "8-bit linear layers", "root-mean-square norm", "optimizer"};
-  void* mine = nullptr;
-  SPION_CUDA_TRY(cudaGetSymbolAddress(&mine, g_lin_status));
-  int* const words[] = {static_cast<int*>(mine), linear_e4m3_status_word(), rmsnorm_status_word(), adamw_status_word()};
-  int v[4] = {0, 0, 0, 0}, rc = SPION_OK;
-  for (int i = 0; i < 4; ++i) {
+  static const char* const whose[] = {"linear layers", "8-bit linear layers", "root-mean-square norm"};
+  int* const words[] = {linear_status_word(), linear_e4m3_status_word(), rmsnorm_status_word()};
+  int v[3] = {0, 0, 0}, rc = SPION_OK;
+  for (int i = 0; i < 3; ++i) {
     if (words[i] == nullptr) return SPION_ERR_CUDA;
     SPION_CUDA_TRY(cudaMemcpyAsync(&v[i], words[i], sizeof(int), cudaMemcpyDeviceToHost, st));
   }
   SPION_CUDA_TRY(cudaStreamSynchronize(st));
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 3; ++i) {
     if (v[i] == 0) continue;
     if (reset) {
       SPION_CUDA_TRY(cudaMemsetAsync(words[i], 0, sizeof(int), st));
@@ -1634,7 +1636,7 @@ extern "C" int spion_linear_status(int reset) {
 }
 
 // One CTA waits, with a limit, on a barrier that nothing arrives on.
-struct StatusWords { int* of[3]; };
+struct StatusWords { int* of[2]; };
 __global__ void k_lin_wait_selftest(long long limit_cycles, const StatusWords others) {
   __shared__ __align__(8) unsigned long long bar_storage;
   const uint32_t bar = smem_u32(&bar_storage);
@@ -1652,7 +1654,7 @@ __global__ void k_lin_wait_selftest(long long limit_cycles, const StatusWords ot
 
 extern "C" int spion_linear_selftest_bounded_wait(long long limit_cycles, void* cuda_stream) {
   if (limit_cycles < 1 || limit_cycles > 2000000000LL) return SPION_ERR_ARG;
-  const StatusWords others = {{linear_e4m3_status_word(), rmsnorm_status_word(), adamw_status_word()}};
+  const StatusWords others = {{linear_e4m3_status_word(), rmsnorm_status_word()}};
   for (int* word : others.of)
     if (word == nullptr) return SPION_ERR_CUDA;
   k_lin_wait_selftest<<<1, 128, 0, (cudaStream_t)cuda_stream>>>(limit_cycles, others);

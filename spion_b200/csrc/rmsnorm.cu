@@ -701,8 +701,8 @@ bool stream_type(int t) { return t == SPION_F32 || t == SPION_BF16 || t == SPION
 }  // namespace
 
 int* rmsnorm_status_word() {
-  void* word = nullptr;
-  return cudaGetSymbolAddress(&word, g_rms_status) == cudaSuccess ? static_cast<int*>(word) : nullptr;
+  static StatusWord word;
+  return word.on_this_device(g_rms_status);
 }
 
 extern "C" {

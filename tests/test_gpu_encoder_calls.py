@@ -153,7 +153,7 @@ def test_inference_mode_and_what_is_refused():
 
 
 def test_the_rings_on_two_streams_at_once():
-    """The kernels that copy ahead: the optimizer's with 8-bit moments, the norm's backward."""
+    """The norm's backward that copies its rows ahead, and the optimizer on many 8-bit moments."""
     from spion_b200.optim import adamw_step
     from spion_b200.rmsnorm import rms_norm
     x, g = torch.randn(4096, 2048, device="cuda", requires_grad=True), torch.rand(2048, device="cuda", requires_grad=True)
