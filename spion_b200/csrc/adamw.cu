@@ -25,7 +25,9 @@ using namespace rows;
 namespace {
 
 constexpr int BLOCK = 256, CTA = 256, CHUNK = CTA / 32 * BLOCK;  // values that share scales; threads; values that a CTA takes at a time, a block per warp
-constexpr int FEW = 64, MOST = 256;                             // tensors of a launch (a table of 512, 24 KB of parameters, cost 100 tensors 10 us on the host)
+// Tensors of a launch, by the table that travels with it: up to 64 tensors with that of 64 12.8 us a call on the host, with that of 256 14.1 (the same on the device); one of
+// 512, 24 KB, cost 100 tensors 10 us more.
+constexpr int FEW = 64, MOST = 256;
 
 struct Tensor {
   void* p;

@@ -9,8 +9,21 @@
 // Statistics are fp32 sums.  The norm of a 16-bit stream is that of the rounded sum, which is what the next layer and the backward see.  The largest
 // |y| is the largest |s w| times rho, rounding included, because rounding keeps the order: sum and maximum take one reduction.
 //
-// Work split: rows of up to 256 values take 8 lanes (a warp has four rows or more), up to 1024 a warp, wider ones a CTA; a row that no register file holds
-// is read twice.  Pieces of eight elements where every row starts on the boundary of such a piece, single elements otherwise (odd widths).  The number of
+// Threads of a row: in the forward 8 lanes up to 256 values, a warp up to 1024, then a CTA of as few threads as hold it in four pieces each; a row that no
+// register file holds is read twice.  The backward keeps twice as much: 8 lanes up to 128 values, a warp up to 512, then a CTA with a thread to a piece behind
+// a ring (two pieces beyond 8192 values).  us for 33.5 million values, bf16 with a residual / fp32 with bf16 branches, and by the next wider split in brackets:
+//   values     forward                             backward
+//      128     46.5 (83.4) / 67.4 (83.8)           47.1 (108) / 73.5 (120)
+//      256     56.5 (70.8) / 67.0 (68.9)           63.6 (157) / 81.0 (182)
+//      512     49.2 (83.7) / 64.3 (64.8)           47.3 (86.2) / 73.6 (106)
+//     1024     57.1 (53.4) / 63.8 (65.1)           52.4 (65.6) / 76.8 (79.6)
+//     2048     44.8 (54.9) / 64.8 (66.7)           46.3 (67.7) / 78.0 (72.9)
+//     4096     44.7 (61.1) / 64.7 (67.9)           46.5 (71.8) / 76.8 (77.9)
+//     8192     46.5 (68.2) / 63.8 (72.0)           47.1 (66.7) / 74.3 (84.0)
+//    16384     50.6 (62.2) / 65.2 (78.1)           51.5 (138) / 148: two rows of fp32 with their residual's gradient do not fit the ring
+// Three forwards of two rows at a time by 8 lanes (16-bit rows up to 64 values) spill 8 to 24 bytes under their bound of four CTAs a multiprocessor.
+//
+// Pieces of eight elements where every row starts on the boundary of such a piece, single elements otherwise (odd widths).  The number of
 // threads of a row is a constant of each kernel, so a piece's place costs no arithmetic.
 //
 // Measured, of a copy's 6.54 TB/s: 32768 x 2048 bf16 + residual to e4m3 75 us (96 %); both directions: 131072 x 64 fp32 with bf16 branches 39 us (92 %), 8192 x

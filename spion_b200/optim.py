@@ -1,4 +1,4 @@
-"""AdamW over many tensors in one launch (csrc/adamw.cu), with moments in 32 or in 8 bits.
+"""AdamW over many tensors at once (csrc/adamw.cu: a launch for the counts and one for the values), with moments in 32 or in 8 bits.
 
 The moments of a set of tensors lie in two arrays, tensor after tensor, each from a multiple of ``BLOCK`` on (``places``); 8-bit moments have a scale per
 ``BLOCK`` values.  ``adamw_step`` is the step on such arrays, ``AdamW`` the optimizer that keeps them.  Beside the update a step can clip the gradients by
@@ -33,7 +33,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, steps, *, scales=None, lr=1e-
     """One step on params (contiguous tensors of one type), in place.  grads: a gradient of the parameter's type and shape each, or None (the tensor and its
     count are left alone).  exp_avg, exp_avg_sq: fp32 arrays of ``places(params)[1]`` values, or float8_e4m3fn and float8_e5m2 with ``scales``, the pair of
     their fp32 scales.  steps: fp32, one count per tensor, raised by the step.  lr: a number, or an fp32 CUDA scalar that is read when the step runs.
-    copies: None, or per parameter a 16-bit tensor that receives it (or None).  ``seed`` and the counts decide how 8-bit moments are rounded."""
+    copies: None, or per parameter a 16-bit tensor that receives it (or None).  ``seed`` and the counts decide how 8-bit moments are rounded.
+    A step after a bounded wait of a kernel gave up changes nothing (``spion_linear_status``)."""
     lr_dev = None
     if isinstance(lr, torch.Tensor):
         lr, lr_dev = (0.0, lr) if lr.is_cuda else (float(lr), None)
@@ -76,11 +77,12 @@ class _Moments:
 
 
 class AdamW(torch.optim.Optimizer):
-    """``torch.optim.AdamW`` on the library's kernel: one launch per parameter group, type and device (256 tensors each).
+    """``torch.optim.AdamW`` on the library's kernels: two launches per parameter group, type and device (256 tensors each).
 
     ``state_bits=8``: moments in 8 bits with a scale per 256 values, 2 bytes a parameter instead of 8, rounded at random (repeatable: ``seed``).
     ``clip_value``: gradients are clipped to [-c, c] as they are read (``torch.nn.utils.clip_grad_value_``; ``.grad`` is left as it is).
-    State dicts have one entry per parameter with torch's names; with 32 bits they are exchangeable with ``torch.optim.AdamW``'s.
+    State dicts have one entry per parameter with torch's names; with 32 bits they are exchangeable with ``torch.optim.AdamW``'s (not those with amsgrad or
+    maximize).  Moments belong to their parameters: groups may be added, removed and moved, not mixed anew.
     A step can be captured in a CUDA graph once a step has been taken; ``lr`` may be an fp32 CUDA scalar, which a replay reads."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *, state_bits: int = 32, clip_value=None, seed: int = 0):
