@@ -356,3 +356,72 @@ def test_gradients_after_a_wait_that_gave_up_are_nan():
     finally:
         assert _lib.lib.spion_linear_status(1) != 0 and _lib.lib.spion_linear_status(0) == 0
     assert all(torch.equal(a, b) for a, b in zip(gradients(), want))
+
+
+class Guarded:
+    """Tensors cut out of larger ones, `off` elements from a boundary, with 64 elements on either side that nothing may change."""
+
+    def __init__(self):
+        self.made = []
+
+    def __call__(self, M, N, dtype, off=0, ld=None):
+        ld = N if ld is None else ld
+        size = torch.empty((), dtype=dtype).element_size()
+        buf = torch.full(((64 + off + max(M, 1) * ld + 64) * size,), 0x5A, dtype=torch.uint8, device="cuda").view(dtype)
+        self.made.append((buf, buf.clone(), off, M, N, ld))
+        return buf[64 + off:].as_strided((M, N), (ld, 1))
+
+    def check(self):
+        for buf, was, off, M, N, ld in self.made:
+            was[64 + off:].as_strided((M, N), (ld, 1)).copy_(buf[64 + off:].as_strided((M, N), (ld, 1)))
+            assert torch.equal(buf.view(torch.uint8), was.view(torch.uint8))
+
+
+CODE = {"fp32": 0, "bf16": 1, "fp16": 2, "e4m3": 3}
+
+
+@pytest.mark.parametrize("M,N", [(1, 1), (3, 8), (5, 64), (37, 72), (130, 120), (9, 250), (300, 256), (7, 512), (150, 520), (11, 1000), (149, 2048), (2, 4096), (5, 4104), (3, 8192), (2, 16384), (3, 16400), (2, 17001)])
+@pytest.mark.parametrize("stream,branch,out", [("fp32", "bf16", "fp16"), ("bf16", "bf16", "bf16"), ("fp32", None, "e4m3"), ("fp16", "fp16", "e4m3"), ("fp32", "fp32", "fp32")])
+def test_nothing_is_written_beside_the_results(M, N, stream, branch, out):
+    """Through the C entries: inputs with rows apart, outputs in the middle of other memory, on and off the boundaries of the wide accesses."""
+    from spion_b200 import _lib
+    from spion_b200.rmsnorm import rms_norm, rms_norm_e4m3
+    st = torch.cuda.current_stream().cuda_stream
+    x, r, w, dy, ds = inputs(M, N, stream, branch, None if out == "e4m3" else out, 5)
+    types = {**T, "e4m3": torch.float8_e4m3fn}
+    if out == "e4m3":
+        want = rms_norm_e4m3(x, w, EPS, res=r)
+        want = (None, *want) if r is None else (want[0], *want[1])
+    else:
+        want = rms_norm(x, w, EPS, res=r, out_dtype=T[out])
+        want = (None, want) if r is None else want
+
+    def p(t):
+        return None if t is None else t.data_ptr()
+
+    for off, apart in ((0, 0), (1, 0), (0, 32), (8, 8), (3, 5)):
+        new = Guarded()
+        X, R = new(M, N, T[stream], off, N + apart).copy_(x), None if r is None else new(M, N, T[branch], 0, N + 2 * apart).copy_(r)
+        S = None if r is None else new(M, N, T[stream], off)
+        Y = new(M, N, types[out], 0 if out == "e4m3" else off, -(-N // 32) * 32 + apart if out == "e4m3" else N + apart)
+        scale, rho = new(1, M, torch.float32) if out == "e4m3" else None, new(1, M, torch.float32)
+        _lib.check(_lib.lib.spion_rmsnorm_forward(p(X), N + apart, CODE[stream], p(R), N + 2 * apart if R is not None else 0, CODE[branch or stream], p(w), 0, p(S), p(Y),
+                                                  Y.stride(0), CODE[out], p(scale), p(rho), M, N, EPS, 1, st))
+        new.check()
+        if S is not None:
+            assert torch.equal(S, want[0])
+        if out == "e4m3":
+            check_rows8(type("Rows", (), {"values": Y, "scales": scale[0]}), normed(x if S is None else S, w), (K(N) / 2 + 8) * U)
+            continue
+        check_forward(x if S is None else S, w, Y)
+        new = Guarded()
+        kept, two = (x if S is None else S), branch == "bf16" and stream == "fp32"
+        Sx, D, Ds = new(M, N, T[stream], off, N + apart).copy_(kept), new(M, N, T[out], off).copy_(dy), new(M, N, T[stream], off).copy_(ds)
+        dx, dr, dw = new(M, N, T[stream], off), new(M, N, T[branch], off) if two else None, new(1, N, torch.float32, off)
+        ws = new(1, int(_lib.lib.spion_rmsnorm_workspace_floats(M, N)), torch.float32)
+        _lib.check(_lib.lib.spion_rmsnorm_backward(p(Sx), N + apart, CODE[stream], p(D), CODE[out], p(Ds), p(w), 0, p(rho), p(dx), p(dr), CODE[branch] if two else 0, p(dw),
+                                                   p(ws), M, N, st))
+        new.check()
+        check_backward(kept, w, dy, ds, dx, dw[0])
+        if two:
+            assert bool(((dr.double() - dx.double()).abs() <= dx.double().abs() * half(dr.dtype) * 1.01 + tiny(dr.dtype)).all())
