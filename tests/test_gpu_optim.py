@@ -548,3 +548,44 @@ def test_small_eps_beside_small_second_moments(eps):
         off = np.abs(p.double().cpu().numpy() - want["p"])
         bound = want["err_p"] + np.abs(want["p"]) * np.minimum(2.0 ** -151 / want["v"], 1)
         assert (off <= bound).all(), (off / bound).max()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_nothing_is_written_beside_the_tensors(dtype, bits):
+    """Parameters, copies and moments in the middle of other memory, on and off the boundaries of the wide accesses; sizes around blocks and chunks; a tensor without a
+    gradient between others: what lies around them, and the places that fill the last block of each, stay."""
+    from spion_b200.optim import adamw_step, places
+    g = torch.Generator(device="cuda").manual_seed(8)
+    for off in (0, 1, 8, 3):
+        sizes = [1, 255, 256, 257, 2047, 2048, 2049, 5000, 70001, 3]
+        spans, at = [], 64 + off
+        for n in sizes:
+            spans.append(slice(at, at + n))
+            at += n + 16 + (off and 1)
+        buf, copy_buf = torch.randn(at + 64, generator=g, device="cuda").to(dtype), torch.randn(at + 64, generator=g, device="cuda").bfloat16()
+        was, copy_was = buf.clone(), copy_buf.clone()
+        ps, cs = [buf[s] for s in spans], [copy_buf[s] for s in spans]
+        gs = [None if i == 5 else torch.randn(n, generator=g, device="cuda").to(dtype) for i, n in enumerate(sizes)]
+        cs[2] = None
+        begins, total = places(ps)
+        m, v = torch.full((total + 512,), 0.5, device="cuda"), torch.full((total + 512,), 0.5, device="cuda")
+        scales = None
+        if bits == 8:
+            m, v = m.to(torch.float8_e4m3fn), v.to(torch.float8_e5m2)
+            scales = torch.full((total // 256 + 2,), 0.25, device="cuda"), torch.full((total // 256 + 2,), 0.25, device="cuda")
+        kept = [t.clone() for t in (m, v, *(scales or ()))]
+        steps = torch.full((len(sizes) + 3,), 4.0, device="cuda")
+        adamw_step(ps, gs, m, v, steps, scales=scales, copies=cs, seed=3, **HYPER)
+        for i, (s, n, b) in enumerate(zip(spans, sizes, begins)):
+            # (a step of lr = 2e-3 is up to half of a bf16's distance from the next one: a few values may all stay)
+            assert (n < 4 or torch.equal(buf[s], was[s]) == (i == 5)) and float(steps[i]) == 4 + (i != 5)
+            assert torch.equal(copy_buf[s], copy_was[s] if i in (2, 5) else buf[s].bfloat16()) or (dtype == torch.float16 and i not in (2, 5))
+            was[s], copy_was[s] = buf[s], copy_buf[s]
+            for t, k in zip((m, v), kept):
+                k.view(torch.uint8 if bits == 8 else torch.float32)[b:b + n] = t.view(torch.uint8 if bits == 8 else torch.float32)[b:b + n]
+            for t, k in zip(scales or (), kept[2:]):
+                k[b // 256:(b + n + 255) // 256] = t[b // 256:(b + n + 255) // 256]
+        raw = lambda t: t.view(torch.uint8)      # noqa: E731
+        assert torch.equal(raw(buf), raw(was)) and torch.equal(raw(copy_buf), raw(copy_was)) and bool((steps[len(sizes):] == 4).all())
+        assert all(torch.equal(raw(t), raw(k)) for t, k in zip((m, v, *(scales or ())), kept))
