@@ -210,3 +210,21 @@ def test_a_module_keeps_its_codes_when_its_type_is_changed():
         assert m.values.dtype == torch.float8_e4m3fn and m.scales.dtype == torch.float32
         m.bias = bias                                                      # (a type change of the bias is the caller's)
         assert torch.equal(m(x), want)
+
+
+@pytest.mark.parametrize("T,K,N", [(5000, 600, 1001), (5001, 2049, 1000), (20001, 513, 300), (5000, 320, 1001), (9999, 512, 515), (20001, 257, 300)])
+def test_pairs_and_their_line_at_odd_sizes(T, K, N):
+    """Tiles of two CTAs that end inside the tokens, the features and a chunk, on both sides of the 512 inner features from which pairs are taken; results on 16-byte
+    boundaries and off them, each with a NaN behind its rows."""
+    from spion_b200.quant import linear_e4m3
+    g = torch.Generator(device="cuda").manual_seed(T + K)
+    x, w = rows8(T, K, g), rows8(N, K, g)
+    bias = torch.randn(N, generator=g, device="cuda").half()
+    for q in (x, w):
+        ld = q.values.stride(0)
+        if ld > K:
+            q.values.as_strided((q.values.shape[0], ld - K), (ld, 1), K).view(torch.uint8).fill_(0x7F)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        y = linear_e4m3(x, w, bias, out_dtype=dtype)
+        check(y, x, w, bias)
+        assert torch.equal(y, linear_e4m3(x, w, bias, out_dtype=dtype))
