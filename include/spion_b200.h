@@ -474,7 +474,7 @@ int spion_linear_prepare(int fp32);
 /* SPION_ERR_TIMEOUT when a bounded wait of these kernels has given up since the last reset (synchronises the device).  Until then
  * every call of them returns without writing its results. */
 int spion_linear_status(int reset);
-/* Failure-path self-test that faults nothing, as spion_selftest_bounded_wait: the status words of the linear layers, of the 8-bit ones and of the norm are set
+/* Failure-path self-test that faults nothing, as spion_selftest_bounded_wait: the status words of the linear layers, of the 8-bit ones, of the norm and of the losses over a vocabulary are set
  * afterwards. */
 int spion_linear_selftest_bounded_wait(long long limit_cycles, void* cuda_stream);
 
@@ -511,7 +511,7 @@ int spion_linear_e4m3(const void* x, long long ldx, const float* x_scale, const 
  * fills the last block of 256 is left alone).  state_bits 32: fp32.  state_bits 8: m in e4m3, v in e5m2, and per block of 256 a scale each (powers of
  * two, [places / 256]); rounded up or down at random, with bits that are a function of seed, step, `index` and the value's place in its tensor.  steps:
  * device array, steps[index] counts the tensor's steps.  lr_dev: device scalar to read the rate from, or NULL: lr.  clip_value < 0: no clipping.  copy:
- * receives p in copy_type (SPION_BF16 or SPION_F16), or NULL.  After a bounded wait of a linear layer or of the norm gave up a step changes nothing, counts
+ * receives p in copy_type (SPION_BF16 or SPION_F16), or NULL.  After a bounded wait of a linear layer, of the norm or of a loss over a vocabulary gave up a step changes nothing, counts
  * included, until spion_linear_status has reported it.  m and v on 32 bytes.  workspace: 16 * min(count, 256) bytes
  * on 16, of the call's stream.  The table is read before the call returns. */
 typedef struct spion_adamw_tensor {
@@ -524,6 +524,44 @@ typedef struct spion_adamw_tensor {
 int spion_adamw_step(const spion_adamw_tensor* host_tensors, int count, int type, int state_bits, void* m, void* v, float* m_scale,
                      float* v_scale, float* steps, const float* lr_dev, double lr, double beta1, double beta2, double eps,
                      double weight_decay, double clip_value, unsigned seed, int copy_type, void* workspace, void* cuda_stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Losses over a vocabulary from the rows before the last layer, without its logits: z = x w^T + bias for T rows x [T, K] and w [V, K].  No teacher: labels [T],
+ * loss_t = lse(z_t) - z_t[label_t]; rows whose label is ignore_index do not count.  With teacher logits [T, k]: labels [T, k], q_t = softmax(teacher_t / temperature)
+ * over the entries whose label is not -1 and whose logit is not -inf, loss_t = sum_j q_tj (ln q_tj - ln softmax(z_t / temperature)[label_tj]); rows without an entry do
+ * not count.  A label outside of [0, V) makes its row's loss NaN, and with it the gradients.  Rows that do not count are not read; their loss and their dx are 0.
+ *   type: of x and w (SPION_F32, SPION_BF16, SPION_F16); row strides ldx (>= 0), ldw (>= K) in elements; w is read in place where its rows are on 16-byte boundaries
+ *   and of 16 bits.  bias [V] fp32 or 16 bits, or NULL.  k: 1 without a teacher, up to 128 with one.  reduction: 0 none (loss [T]), 1 mean over the rows that count (NaN where none
+ *   does), 2 sum (loss: one fp32 number).  The temperature is 1 without a teacher, normally.
+ * spion_vocab_sizes: bytes of `keep` (written by the forward, read by the backward) and of the two workspaces, all on 256-byte boundaries.
+ * The backward takes g [T] (reduction 0) or one number, what arrives at the loss, and writes dx [T, K], dw [V, K] (contiguous, of type `type`, on 32 bytes) and db [V]; each may be
+ * NULL.  Sums have a fixed order.  A bounded wait that gives up is reported by spion_linear_status; losses and gradients are NaN until then. */
+typedef struct spion_vocab_problem {
+  const void* x;
+  const void* w;
+  const void* bias;
+  const void* teacher;
+  const long long* labels;
+  long long ldx, ldw, T, K, V, k, ignore_index;
+  int type, bias_type, teacher_type, reduction;
+  float temperature;
+} spion_vocab_problem;
+int spion_vocab_sizes(const spion_vocab_problem* host_problem, long long* keep_bytes, long long* forward_bytes, long long* backward_bytes);
+int spion_vocab_loss_forward(const spion_vocab_problem* host_problem, float* loss, void* keep, void* workspace, void* cuda_stream);
+int spion_vocab_loss_backward(const spion_vocab_problem* host_problem, const float* g, const void* keep, void* dx, void* dw, void* db, int db_type,
+                              void* workspace, void* cuda_stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Rows of a token table of any size: y[t] = w[ids[t]] * scale, rounded once.  ids [T] int64; w [V, N] with rows ldw (>= N) elements apart, SPION_F32, SPION_BF16 or SPION_F16;
+ * y [T, N] of any of the three.  An id outside of [0, V) gives a row of NaN.
+ * Its gradient dw [V, N] (contiguous, any of the three types) = scale times the sum of the rows g[t] (ldg >= 0 elements apart) with ids[t] = v, in the order of t, in fp32;
+ * zeros for rows without one and for row padding_idx (-1: none); ids outside of the table have none.  workspace: spion_token_rows_workspace_bytes(T, V, N)
+ * bytes on 256. */
+int spion_token_rows_forward(const long long* ids, const void* w, long long ldw, int w_type, void* y, int y_type, float scale, long long T, long long V, long long N,
+                             void* cuda_stream);
+long long spion_token_rows_workspace_bytes(long long T, long long V, long long N);
+int spion_token_rows_backward(const long long* ids, const void* g, long long ldg, int g_type, void* dw, int dw_type, float scale, long long padding_idx, long long T,
+                              long long V, long long N, void* workspace, void* cuda_stream);
 
 #ifdef __cplusplus
 }

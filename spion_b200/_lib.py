@@ -33,6 +33,13 @@ class AdamwTensor(ctypes.Structure):
     _fields_ = [("p", c_void_p), ("g", c_void_p), ("copy", c_void_p), ("n", c_longlong), ("at", c_longlong), ("index", c_int)]
 
 
+class VocabProblem(ctypes.Structure):
+    """spion_vocab_problem: operands of a loss over a vocabulary (see include/spion_b200.h)."""
+    _fields_ = [(n, c_void_p) for n in ("x", "w", "bias", "teacher", "labels")] + \
+        [(n, c_longlong) for n in ("ldx", "ldw", "T", "K", "V", "k", "ignore_index")] + \
+        [(n, c_int) for n in ("type", "bias_type", "teacher_type", "reduction")] + [("temperature", ctypes.c_float)]
+
+
 # name -> (restype, argtypes); every symbol include/spion_b200.h declares
 SIGNATURES = {
     "spion_status_string": (ctypes.c_char_p, [c_int]),
@@ -120,6 +127,12 @@ SIGNATURES = {
                                        c_void_p, c_longlong, c_int, c_void_p]),
     "spion_linear_e4m3": (c_int, [c_void_p, c_longlong, c_void_p] * 2 + [c_void_p, c_int, c_void_p, c_longlong, c_int, c_longlong, c_int, c_int, c_void_p]),
     "spion_adamw_step": (c_int, [ctypes.POINTER(AdamwTensor), c_int, c_int, c_int] + [c_void_p] * 6 + [c_double] * 6 + [ctypes.c_uint, c_int, c_void_p, c_void_p]),
+    "spion_vocab_sizes": (c_int, [ctypes.POINTER(VocabProblem)] + [ctypes.POINTER(c_longlong)] * 3),
+    "spion_vocab_loss_forward": (c_int, [ctypes.POINTER(VocabProblem)] + [c_void_p] * 4),
+    "spion_vocab_loss_backward": (c_int, [ctypes.POINTER(VocabProblem)] + [c_void_p] * 5 + [c_int] + [c_void_p] * 2),
+    "spion_token_rows_forward": (c_int, [c_void_p, c_void_p, c_longlong, c_int, c_void_p, c_int, ctypes.c_float] + [c_longlong] * 3 + [c_void_p]),
+    "spion_token_rows_workspace_bytes": (c_longlong, [c_longlong] * 3),
+    "spion_token_rows_backward": (c_int, [c_void_p, c_void_p, c_longlong, c_int, c_void_p, c_int, ctypes.c_float] + [c_longlong] * 4 + [c_void_p] * 2),
     "spion_static_scratch_capacity": (ctypes.c_size_t, []),
     "spion_attn_forward_static": (c_int, [c_void_p] * 9 + [c_int] * 6 + [c_void_p]),
 }

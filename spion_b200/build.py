@@ -6,7 +6,7 @@ Outputs (git-ignored, but shipped with the working tree):
     spion_b200/lib/libspion_b200.so        all kernels + the C ABI of include/spion_b200.h
     spion_b200/lib/{attn,attn_mask,block_attn,block_attn_mask}.so
                                            shims with the reference's own symbol names
-    spion_b200/lib/_torch_ops.so           autograd nodes of the Python modules (csrc/torch_ops.cpp, torch_encoder_ops.cpp)
+    spion_b200/lib/_torch_ops.so           autograd nodes of the Python modules (csrc/torch_ops.cpp, torch_encoder_ops.cpp, torch_vocab_ops.cpp)
 """
 from __future__ import annotations
 
@@ -76,9 +76,9 @@ def build_torch_ops(main, force: bool = False) -> str:
 
     import torch
     from torch.utils import cpp_extension
-    srcs = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "torch_encoder_ops.cpp")]
+    srcs = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "torch_encoder_ops.cpp", "torch_vocab_ops.cpp")]
     out = os.path.join(LIB, "_torch_ops.so")
-    headers = [os.path.join(os.path.dirname(HERE), "include", "spion_b200.h"), os.path.join(CSRC, "torch_common.h")]
+    headers = [os.path.join(os.path.dirname(HERE), "include", "spion_b200.h"), os.path.join(CSRC, "torch_common.h"), os.path.join(CSRC, "torch_checks.h")]
     if not force and not _newer(srcs + headers + [main], out):
         return out
     inc = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")]

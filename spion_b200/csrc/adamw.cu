@@ -301,7 +301,7 @@ struct Begin {
   double lr, wd, log_b1, log_b2;
   unsigned seed;
   int count;
-  const int *linear, *norm;   // status words of the kernels that form gradients with bounded waits
+  const int *linear, *norm, *vocab;   // status words of the kernels that form gradients with bounded waits
 };
 template <int MAX> struct Indices {
   Begin b;
@@ -311,7 +311,7 @@ template <int MAX> __global__ void __launch_bounds__(MAX) k_adamw_begin(const __
   next_may_start();                                                      // k_adamw
   if ((int)threadIdx.x >= a.b.count) return;
   const int i = a.index[threadIdx.x];
-  const int lost = *static_cast<const volatile int*>(a.b.linear) | *static_cast<const volatile int*>(a.b.norm);
+  const int lost = *static_cast<const volatile int*>(a.b.linear) | *static_cast<const volatile int*>(a.b.norm) | *static_cast<const volatile int*>(a.b.vocab);
   const float step = a.b.steps[i] + 1.f;
   const double lr = a.b.lr_dev != nullptr ? (double)*a.b.lr_dev : a.b.lr;
   float4 f = make_float4((float)(1.0 - lr * a.b.wd), (float)(lr / -expm1((double)step * a.b.log_b1)), (float)(1.0 / sqrt(-expm1((double)step * a.b.log_b2))),
@@ -377,11 +377,11 @@ extern "C" int spion_adamw_step(const spion_adamw_tensor* host_tensors, int coun
     if (t.copy != nullptr && copy_type != SPION_BF16 && copy_type != SPION_F16) return SPION_ERR_ARG;
   }
   if (type != SPION_F32 && type != SPION_BF16 && type != SPION_F16) return SPION_ERR_UNSUPPORTED;
-  const int *const linear = linear_status_word(), *const norm = rmsnorm_status_word();
-  if (linear == nullptr || norm == nullptr) return SPION_ERR_CUDA;
+  const int *const linear = linear_status_word(), *const norm = rmsnorm_status_word(), *const vocab = vocab_status_word();
+  if (linear == nullptr || norm == nullptr || vocab == nullptr) return SPION_ERR_CUDA;
   const Step s = {m, v, m_scale, v_scale, static_cast<const float4*>(workspace), (float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2),
                   (float)eps, clip_value >= 0 ? (float)clip_value : -1.f, 0, 0, copy_type};
-  const Begin b = {steps, static_cast<float4*>(workspace), lr_dev, lr, weight_decay, log(beta1), log(beta2), seed, 0, linear, norm};
+  const Begin b = {steps, static_cast<float4*>(workspace), lr_dev, lr, weight_decay, log(beta1), log(beta2), seed, 0, linear, norm, vocab};
   const cudaStream_t st = (cudaStream_t)cuda_stream;
   if (type == SPION_F32) return state_bits == 8 ? launches<float, 8>(s, b, host_tensors, count, st) : launches<float, 32>(s, b, host_tensors, count, st);
   if (type == SPION_BF16)

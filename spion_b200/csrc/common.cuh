@@ -148,10 +148,11 @@ int sm_count();
 
 // linear.cu: status word of the linear layers on the current device, after the work of a stream
 int linear_status(int reset, cudaStream_t st);
-// Where the status words of linear.cu, linear_e4m3.cu and rmsnorm.cu lie on the current device (null: the query failed); reported together
+// Where the status words of linear.cu, linear_e4m3.cu, rmsnorm.cu and vocab_loss.cu lie on the current device (null: the query failed); reported together
 int* linear_status_word();
 int* linear_e4m3_status_word();
 int* rmsnorm_status_word();
+int* vocab_status_word();
 // ... asked once per device: steps of the optimizer ask each time
 struct StatusWord {
   std::atomic<int*> at[64] = {};

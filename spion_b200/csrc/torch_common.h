@@ -72,8 +72,9 @@ inline SavedVariable save(const Tensor& t) { return SavedVariable(t, false); }
 inline bool recorded() { return at::GradMode::is_enabled(); }
 struct OutsideAutocast { c10::impl::ExcludeDispatchKeyGuard guard{c10::autocast_dispatch_keyset}; };
 
-// torch_encoder_ops.cpp
+// torch_encoder_ops.cpp, torch_vocab_ops.cpp
 void add_encoder_ops(py::module_& m);
+void add_vocab_ops(py::module_& m);
 
 }  // namespace spion_torch
 

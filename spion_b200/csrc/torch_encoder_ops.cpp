@@ -3,68 +3,10 @@
 #include <algorithm>
 #include <mutex>
 
-#include "torch_common.h"
+#include "torch_checks.h"
 
 namespace {
 
-// ------------------------------------------------------------------------------------------------ checks
-[[noreturn]] void refuse(const char* op, const std::string& why) { throw Failure(std::string(op) + ": " + why); }
-std::string shape_of(const Tensor& t) {
-  std::string s = "(";
-  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
-  return s + ")";
-}
-int type_code(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return SPION_F32;
-    case at::kBFloat16: return SPION_BF16;
-    case at::kHalf: return SPION_F16;
-    case at::kFloat8_e4m3fn: return SPION_E4M3;
-    default: return -1;
-  }
-}
-bool stream_type(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
-
-// The kernels work on memory that tracers, function transforms and forward-mode tangents would not see.
-void check_plain(const char* op, const Tensor& t, const char* name) {
-  if (!t.is_cuda()) refuse(op, std::string(name) + " is not a CUDA tensor (there is no CPU path)");
-  if (t.layout() != at::kStrided || torch::jit::tracer::isTracing() || !plain(t))
-    refuse(op, std::string(name) + " is not an ordinary tensor of an ordinary call (tracing, function transforms, forward-mode tangents, tensor subclasses "
-           "and sparse layouts are not served)");
-}
-// ... nor do dispatch modes that hand out tensors without memory
-Tensor made(const char* op, Tensor t) {
-  if (!plain(t)) refuse(op, "a dispatch mode without real tensors is active");
-  return t;
-}
-void same_device(const char* op, const Tensor& t, const Tensor& like, const char* name) {
-  if (t.device() != like.device()) refuse(op, std::string(name) + " is on " + t.device().str() + ", the rows are on " + like.device().str());
-}
-
-// A tensor's rows over its last dimension as the kernels read them: rows a constant step apart, elements next to one another.
-struct Rows {
-  Tensor t;
-  int64_t M = 0, N = 0, ld = 0;
-  explicit Rows(const Tensor& x) {
-    N = x.size(-1);
-    M = N ? x.numel() / N : 0;
-    ld = N;
-    if (x.is_contiguous()) {
-      t = x;
-      return;
-    }
-    t = x.reshape({M, N});               // a view where the strides allow it
-    if (N > 1 && t.stride(1) != 1) t = t.contiguous();
-    if (M > 1) ld = t.stride(0);
-  }
-};
-
-void check_rows(const char* op, const Tensor& x, const char* name) {
-  check_plain(op, x, name);
-  if (!stream_type(x.scalar_type())) refuse(op, std::string(name) + " has type " + c10::toString(x.scalar_type()) + "; fp32, bf16 and fp16 are served");
-  if (x.dim() < 1 || x.size(-1) < 1) refuse(op, std::string(name) + " has shape " + shape_of(x) + ": it needs a last dimension of one element or more");
-  if (x.size(-1) > 0x7fffffff / 2) refuse(op, std::string(name) + " has rows of " + std::to_string(x.size(-1)) + " elements");
-}
 void check_norm(const char* op, const Tensor& x, const Tensor& w, const optional<Tensor>& res) {
   check_rows(op, x, "x");
   check_plain(op, w, "weight");
@@ -79,10 +21,6 @@ void check_norm(const char* op, const Tensor& x, const Tensor& w, const optional
     refuse(op, std::string("res has type ") + c10::toString(res->scalar_type()) + " beside a stream of " + c10::toString(x.scalar_type()) +
            ": it has the stream's type, or 16 bits beside fp32");
 }
-struct Below {                           // what happens inside is not recorded
-  at::AutoDispatchBelowADInplaceOrView below;
-  c10::impl::ExcludeDispatchKeyGuard no_autocast{c10::autocast_dispatch_keyset};
-};
 // Rows of bytes start on 32, a sector of memory: tensor maps ask for 16, which costs them every box's rows a sector more (65536 x 272 to 256: 20.0 us, 65536 x
 // 288: 17.2; 112 and 96 14.7, 11.8).
 int64_t row8_stride(int64_t N) { return (N + 31) / 32 * 32; }

@@ -919,4 +919,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mlp_supported", &mlp_supported);
   m.def("mlp", &mlp);
   add_encoder_ops(m);
+  add_vocab_ops(m);
 }

@@ -1,0 +1,1203 @@
+// Losses over a vocabulary from the rows before the last layer, without its logits:  z = x W^T + b (T rows of K, V rows of W),
+//
+//   loss_t = sum_j q_tj (ln q_tj - z_t[i_tj] / tau + lse_t),   lse_t = ln sum_v exp(z_tv / tau)
+//
+// with one target of weight 1 (cross entropy, tau = 1) or a teacher's k logits, q_t = softmax(logits_t / tau).  Gradients, with g_t what arrives at a row's loss:
+//
+//   G_tv = g_t / tau (softmax(z_t / tau)_v - sum_{j: i_tj = v} q_tj),   dx = G W,  dW = G^T x,  db = sum_t G_t
+//
+//   k_flags, k_gather    which rows count, in order; those rows side by side in the products' type (rows that do not count cost nothing and are never read)
+//   k_gemm<LOGSUM>       z tile by tile in tensor memory; leaves the largest and the sum of exponentials of a row's columns of the tile, and the targets' z
+//   k_finish             lse and loss of each row, and their sum or mean
+//   k_gemm<GRAD>         z again, for a piece of the vocabulary; leaves G in 16 bits
+//   k_gemm<DX>, <DW>     the two products with it;  k_dx, k_dw, k_db join what was summed apart
+//
+// The products are tcgen05 kind::f16, fp32 sums in tensor memory.  A sum there is truncated at every step, so no more than CHAIN steps go to one
+// accumulator where a result has 32 bits; what the accumulators hold is added in fp32 registers.  fp32 operands are three bf16 parts each (8 + 8 + 8 bits, exact) and
+// six products; what is dropped is below 2^-25 of a product.
+//
+// G is rounded to the type that W has, after it was formed in fp32: the products' other operand has those bits, and their results are rounded to them.  G holds g_t
+// over the largest |g_t| (and 2^13 times that in fp16, whose smallest numbers probabilities of a large vocabulary fall below); the factor comes back in fp32.
+// The bias's gradient is summed from G before it is rounded.
+#include <algorithm>
+
+#include "rows.cuh"
+#include "tc_ptx.cuh"
+#include "tc_tiles.cuh"
+
+using namespace tc;
+using namespace rows;
+
+namespace {
+
+// Set by a bounded wait that gave up (see g_lin_status in linear.cu); results after it are NaN until it has been reported.
+__device__ int g_vocab_status;
+
+constexpr float LN2 = 0.6931471805599453f;
+constexpr int MAX_TARGETS = 128;
+constexpr int PAD = 256;                                  // rows and vocabulary columns of scratch come in whole tiles
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float not_a_number() { return __int_as_float(0x7fffffff); }
+
+// ------------------------------------------------------------------------------------------------ which rows count
+// Kept from the forward for the backward, in the order of the rows that count ("slots"); numbers in units of log2
+struct Plan {
+  int* head;                // [0]: rows that count; [1]: CTAs of k_finish that are done
+  int* slot;                // [T] a row's slot, or -1
+  int* row;                 // [Tp] a slot's row
+  float* lse;               // [Tp]
+  int* target;              // [k][Tp]; -1: left out; -2: outside of the vocabulary
+  float* q;                 // [k][Tp] (null: one target of weight 1)
+};
+struct Prep {
+  Plan plan;
+  const long long* labels;  // [T], or [T, k] where there are teacher logits
+  const void* teacher; int teacher_type;                 // [T, k] or null
+  long long ignore;
+  float inv_tau;
+  int T, Tp, V, k;
+  int* counts;              // [chunks of CHUNK rows]
+  float* q;                 // [T, k]
+  const void* bias; int bias_type;
+  float* bias2;             // [Vp] b log2(e) / tau; -inf behind the vocabulary
+  int Vp;
+  float c1;                 // log2(e) / tau
+};
+constexpr int CHUNK = 64;
+
+// A warp: weights of a row's targets.  Returns whether one is there.
+__device__ __forceinline__ bool teacher_weights(const Prep& a, int t, int lane) {
+  const long long at = (long long)t * a.k;
+  float v[MAX_TARGETS / 32];
+  float top = -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < MAX_TARGETS / 32; ++i) {
+    const int j = lane + 32 * i;
+    v[i] = j < a.k && a.labels[at + j] != -1 ? load_any(a.teacher, a.teacher_type, at + j) : -INFINITY;
+    nan |= v[i] != v[i];
+    top = fmaxf(top, v[i]);
+  }
+  top = lane_max<32>(top);
+  const bool any = __any_sync(0xffffffffu, nan) || top != -INFINITY;
+  if (!any) return false;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < MAX_TARGETS / 32; ++i) {
+    v[i] = v[i] == -INFINITY ? 0.f : expf((v[i] - top) * a.inv_tau);
+    sum += v[i];
+  }
+  sum = lane_sum<32>(sum);
+#pragma unroll
+  for (int i = 0; i < MAX_TARGETS / 32; ++i)
+    if (lane + 32 * i < a.k) a.q[at + lane + 32 * i] = v[i] / sum;
+  return true;
+}
+__device__ __forceinline__ void scaled_bias(const Prep& a, int first, int step) {
+  for (int v = first; v < a.Vp; v += step) a.bias2[v] = v >= a.V ? -INFINITY : a.bias != nullptr ? load_any(a.bias, a.bias_type, v) * a.c1 : 0.f;
+}
+// A warp per chunk
+__global__ void __launch_bounds__(256) k_flags(const __grid_constant__ Prep a) {
+  next_may_start();
+  wait_for_kernel_before();
+  const int lane = threadIdx.x & 31, chunks = (a.T + CHUNK - 1) / CHUNK, warps = gridDim.x * 8;
+  for (int c = blockIdx.x * 8 + (threadIdx.x >> 5); c < chunks; c += warps) {
+    int n = 0;
+    if (a.teacher == nullptr) {
+#pragma unroll
+      for (int i = 0; i < CHUNK; i += 32) {
+        const int t = c * CHUNK + i + lane;
+        n += __popc(__ballot_sync(0xffffffffu, t < a.T && a.labels[t] != a.ignore));
+      }
+    } else {
+      for (int t = c * CHUNK; t < min(a.T, (c + 1) * CHUNK); ++t) {
+        const bool counts = teacher_weights(a, t, lane);
+        if (lane == 0) a.plan.slot[t] = counts ? 0 : -1;
+        n += counts;
+      }
+    }
+    if (lane == 0) a.counts[c] = n;
+  }
+  scaled_bias(a, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.plan.head[1] = 0;
+}
+
+// ------------------------------------------------------------------------------------------------ rows in the products' type
+struct Source {
+  const void* p; int type; long long ld;
+  int K, Kp, fast;          // fast: rows on 16-byte boundaries (32 in fp32), whole pieces of 8
+};
+// eight elements of a row to one 16-bit piece, or to three bf16 parts of an fp32 row `plane` elements apart
+template <class T> __device__ __forceinline__ void put_piece(const Source& s, long long row, int c, uint16_t* to, long long plane) {
+  const T* const from = static_cast<const T*>(s.p) + row * s.ld + c;
+  if constexpr (sizeof(T) == 2) {
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (s.fast) {
+      if (c < s.K) w = *reinterpret_cast<const uint4*>(from);
+    } else {
+      uint32_t u[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < s.K) u[i >> 1] |= (uint32_t) * reinterpret_cast<const uint16_t*>(from + i) << (16 * (i & 1));
+      w = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    *reinterpret_cast<uint4*>(to) = w;
+  } else {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = 0.f;
+    if (s.fast) {
+      if (c < s.K) {
+        const float4 u = reinterpret_cast<const float4*>(from)[0], v = reinterpret_cast<const float4*>(from)[1];
+        f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w, f[4] = v.x, f[5] = v.y, f[6] = v.z, f[7] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < s.K) f[i] = from[i];
+    }
+#pragma unroll
+    for (int part = 0; part < 3; ++part) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = pack_bf16(f[2 * i], f[2 * i + 1]);
+        f[2 * i] -= bf16_lo(w[i]), f[2 * i + 1] -= bf16_hi(w[i]);
+      }
+      *reinterpret_cast<uint4*>(to + part * plane) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+// Rows first, first + step, .. below `rows` of a list (null: all of them, zeros from `known` on) to consecutive rows of the scratch
+template <class T> __device__ __forceinline__ void copy_rows(const Source& s, const int* list, int count, long long first, uint16_t* to, long long plane) {
+  const int pieces = s.Kp / 8;
+  for (int i = threadIdx.x; i < count * pieces; i += blockDim.x) {
+    const int r = i / pieces, c = (i - r * pieces) * 8;
+    put_piece<T>(s, list ? list[r] : first + r, c, to + (first + r) * s.Kp + c, plane);
+  }
+}
+
+// A CTA per chunk: its rows that count, to their slots.
+template <class T, bool FIRST> __global__ void __launch_bounds__(256) k_gather(const __grid_constant__ Prep a, const Source s, uint16_t* xs, float* loss_rows, float* zt) {
+  next_may_start();
+  wait_for_kernel_before();
+  __shared__ int list[CHUNK], part[2][8], here;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long plane = (long long)a.Tp * s.Kp;
+  const int pieces = s.Kp / 8;
+  int first, n;
+  if constexpr (FIRST) {
+    const int chunks = (a.T + CHUNK - 1) / CHUNK;
+    int before = 0, all = 0;
+    for (int c = threadIdx.x; c < chunks; c += 256) {
+      const int m = a.counts[c];
+      all += m;
+      if (c < (int)blockIdx.x) before += m;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o), all += __shfl_xor_sync(0xffffffffu, all, o);
+    if (lane == 0) part[0][warp] = before, part[1][warp] = all;
+    __syncthreads();
+    first = n = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) first += part[0][w], n += part[1][w];
+    if (warp == 0) {
+      int at = 0;
+#pragma unroll
+      for (int i = 0; i < CHUNK; i += 32) {
+        const int t = blockIdx.x * CHUNK + i + lane;
+        const bool counts = t < a.T && (a.teacher ? a.plan.slot[t] >= 0 : a.labels[t] != a.ignore);
+        const unsigned who = __ballot_sync(0xffffffffu, counts);
+        const int mine = at + __popc(who & ((1u << lane) - 1));
+        if (t < a.T) {
+          a.plan.slot[t] = counts ? first + mine : -1;
+          if (loss_rows != nullptr && !counts) loss_rows[t] = 0.f;
+        }
+        if (counts) list[mine] = t, a.plan.row[first + mine] = t;
+        at += __popc(who);
+      }
+      if (lane == 0) {
+        here = at;
+        if (blockIdx.x == 0) a.plan.head[0] = n;
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < here * a.k; i += 256) {
+      const int r = i / a.k, j = i - r * a.k;
+      const long long from = (long long)list[r] * a.k + j, to = (long long)j * a.Tp + first + r, v = a.labels[from];
+      const float q = a.teacher ? a.q[from] : 1.f;
+      a.plan.target[to] = a.teacher && (v == -1 || q == 0.f) ? -1 : v < 0 || v >= a.V ? -2 : (int)v;
+      if (a.teacher) a.plan.q[to] = v == -1 ? 0.f : q;
+      zt[to] = not_a_number();                            // of a target that no tile has
+    }
+  } else {
+    n = a.plan.head[0];
+    first = blockIdx.x * CHUNK;
+    if (threadIdx.x < CHUNK && first + (int)threadIdx.x < n) list[threadIdx.x] = a.plan.row[first + threadIdx.x];
+    if (threadIdx.x == 0) here = max(0, min(CHUNK, n - first));
+    __syncthreads();
+  }
+  copy_rows<T>(s, list, here, first, xs, plane);
+  // zeros up to the end of the last tile: what it holds is multiplied with zeros
+  const int zeros = (n + PAD - 1) / PAD * PAD - n;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < zeros * pieces; i += gridDim.x * 256)
+#pragma unroll
+    for (int part_ = 0; part_ < (sizeof(T) == 4 ? 3 : 1); ++part_)
+      *reinterpret_cast<uint4*>(xs + part_ * plane + (long long)n * s.Kp + 8ll * i) = make_uint4(0, 0, 0, 0);
+}
+// W where the products cannot read it as it lies: fp32, or rows off 16 bytes
+template <class T> __global__ void __launch_bounds__(256) k_copy_w(const Source s, int V, int Vp, uint16_t* to) {
+  next_may_start();
+  wait_for_kernel_before();
+  const long long plane = (long long)Vp * s.Kp, pieces = s.Kp / 8, all = (long long)Vp * pieces;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
+    const long long r = i / pieces;
+    const int c = (int)(i - r * pieces) * 8;
+    uint16_t* const at = to + r * s.Kp + c;
+    if (r < V) {
+      put_piece<T>(s, r, c, at, plane);
+    } else {
+#pragma unroll
+      for (int p = 0; p < (sizeof(T) == 4 ? 3 : 1); ++p) *reinterpret_cast<uint4*>(at + p * plane) = make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ the four products
+enum Mode { LOGSUM, GRAD, DX, DW };
+constexpr int BK = 64;                                    // elements of the contraction in a chunk: 128 bytes
+constexpr int EPI = 8, THREADS = 32 * (2 + EPI);
+constexpr int STAGES = 6;
+constexpr uint32_t HALF = 128 * BK * 2, STAGE = 2 * HALF;
+constexpr uint32_t BARS = STAGES * STAGE, SMEM = BARS + 16 * STAGES + 64;
+static_assert(SMEM <= 232448, "shared memory of a multiprocessor");
+
+struct Args {
+  const int* n;                                           // rows that count
+  int products;                                           // 1, or 6 of three parts
+  long long plane_a, plane_b;                             // rows of a part in the maps
+  int M, N, L;                                            // rows of D (0: n), columns of D, contraction (0: n)
+  int col0;                                               // first column of the piece of the vocabulary
+  int chain;                                              // (chunk, product) pairs that one accumulator takes
+  int splits, split_chunks;                               // of the contraction (0: by the number of tiles, at most split_chunks)
+  int fp16;                                               // operands are fp16, else bf16
+  // LOGSUM, GRAD
+  Plan plan; int Tp, k;
+  const float* bias2; float c1;
+  float2* part; int parts;                                // [slots, parts] largest, sum
+  float* zt;                                              // [k][Tp]
+  const float* g; const float* coef;                      // per row or null; coef[1]: 1 / max |g|
+  uint16_t* G; long long ldg;                             // [planes][Tp][ldg]
+  float* colsum;                                          // [Tp / 32][ldg] or null
+  float gscale;                                           // 1, or 2^13 in fp16
+  // DX, DW
+  float* out; long long ldo; int add;                     // fp32 partial sums: [split][rows of whole tiles][ldo]
+  void* dw; int dw_type; long long K; int V;              // DW, one split: the result
+};
+struct Maps { CUtensorMap a, b; };
+
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t in_leader(uint32_t addr) {          // the same place in the pair's first CTA
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ void pair_arrive(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void pair_tma_load_2d(uint32_t smem_dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(smem_dst), "l"((uint64_t)map), "r"(cluster_bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void pair_tmem_alloc(uint32_t smem_slot, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_slot), "r"(ncols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pair_tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// D: 128 rows in the tensor memory of each CTA; A and B: the same places of both CTAs' shared memory, half of the rows in each
+__device__ __forceinline__ void pair_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      :
+      : "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void pair_commit(uint32_t bar) {             // on both CTAs' barriers
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+// the partial products of the split operands, smallest first: (part of A, part of B)
+__device__ __forceinline__ void parts_of(int products, int i, int& a, int& b) {
+  a = b = 0;
+  if (products == 1) return;
+  a = (0x010210 >> (4 * i)) & 3;                          // 0 1 2 0 1 0
+  b = (0x001012 >> (4 * i)) & 3;                          // 2 1 0 1 0 0
+}
+
+// What a launch works on, the same in all its warps and (for DX) in the kernel that joins the sums
+struct Work { int tiles_m, tiles_n, splits, chunks, per; };
+__host__ __device__ __forceinline__ int split_by_tiles(int tiles, int units, int chunks) {
+  const int s = tiles > 0 ? units / tiles : 1;
+  return s < 1 ? 1 : s > chunks ? (chunks < 1 ? 1 : chunks) : s;
+}
+__device__ __forceinline__ Work work_of(const Args& a, int n, int tile_m, int tile_n, int units) {
+  Work w;
+  w.tiles_m = ((a.M ? a.M : n) + tile_m - 1) / tile_m;
+  w.tiles_n = (a.N + tile_n - 1) / tile_n;
+  w.chunks = ((a.L ? a.L : n) + BK - 1) / BK;
+  w.splits = a.splits ? a.splits : split_by_tiles(w.tiles_m * w.tiles_n, units, a.split_chunks);
+  w.per = (w.chunks + w.splits - 1) / w.splits;
+  return w;
+}
+// Tiles in groups of 8 rows of tiles, column by column inside a group: the CTAs that run at a time share their operands in L2.
+__device__ __forceinline__ void item_at(const Work& w, int i, int& s, int& m, int& n, int& c0, int& c1) {
+  const int tiles = w.tiles_m * w.tiles_n;
+  s = i / tiles;
+  i -= s * tiles;
+  const int per = 8 * w.tiles_n, group = i / per, rows_here = min(8, w.tiles_m - 8 * group), j = i - group * per;
+  n = j / rows_here;
+  m = 8 * group + j - n * rows_here;
+  c0 = min(s * w.per, w.chunks), c1 = min(c0 + w.per, w.chunks);
+}
+
+__device__ __forceinline__ void st_v8(void* p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+               "r"(r[6]), "r"(r[7]) : "memory");
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, int fp16) {
+  if (!fp16) return pack_bf16(a, b);
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Targets of a row among the columns c .. c + 31, of those whose bits are set
+template <class F> __device__ __forceinline__ void each_target(const Args& a, const uint32_t (&hits)[MAX_TARGETS / 32], int slot, int c, F f) {
+#pragma unroll
+  for (int w = 0; w < MAX_TARGETS / 32; ++w) {
+    uint32_t h = hits[w];
+    while (h) {
+      const int j = 32 * w + __ffs(h) - 1;
+      h &= h - 1;
+      const int off = a.plan.target[(long long)j * a.Tp + slot] - c;
+      if ((unsigned)off < 32u) f(j, off);
+    }
+  }
+}
+
+// What a thread does with its sums: row `row` of D, columns col .. col + W - 1 (W = BN / 2)
+template <int MODE, int W> __device__ __forceinline__ void epilogue(const Args& a, const Work& w, float (&acc)[W], int n, int s, int row, int col, int tile_m, int part) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (MODE == LOGSUM || MODE == GRAD) {
+    const bool in = row < n;
+    const int slot = in ? row : 0, c = a.col0 + col;      // of the vocabulary
+    uint32_t hits[MAX_TARGETS / 32] = {};
+    if (in)
+#pragma unroll
+      for (int i = 0; i < MAX_TARGETS / 32; ++i)
+        for (int j = 32 * i; j < min(a.k, 32 * i + 32); ++j)
+          if ((unsigned)(a.plan.target[(long long)j * a.Tp + slot] - c) < (unsigned)W) hits[i] |= 1u << (j & 31);
+#pragma unroll
+    for (int g = 0; g < W; g += 4) {
+      const float4 b = *reinterpret_cast<const float4*>(a.bias2 + c + g);
+      acc[g] = fmaf(acc[g], a.c1, b.x), acc[g + 1] = fmaf(acc[g + 1], a.c1, b.y);
+      acc[g + 2] = fmaf(acc[g + 2], a.c1, b.z), acc[g + 3] = fmaf(acc[g + 3], a.c1, b.w);
+    }
+    if constexpr (MODE == LOGSUM) {
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int g = 0; g < W; ++g) top = fmaxf(top, acc[g]);
+#pragma unroll
+      for (int g = 0; g < W; g += 32)
+        each_target(a, hits, slot, c + g, [&](int j, int off) {
+          float z = 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) z = e == off ? acc[g + e] : z;
+          a.zt[(long long)j * a.Tp + slot] = z;
+        });
+      const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int g = 0; g < W; ++g) sum += ex2(acc[g] - from);
+      if (in) a.part[(long long)row * a.parts + part] = make_float2(top, sum);
+    } else {
+      float lse = 0.f, r = 0.f;
+      if (in) {
+        lse = a.plan.lse[slot];
+        r = a.g ? a.g[a.plan.row[slot]] * a.coef[1] : 1.f;
+        r *= a.gscale;
+      }
+#pragma unroll
+      for (int g = 0; g < W; g += 32) {
+        float v[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = in ? ex2(acc[g + e] - lse) * r : 0.f;
+        each_target(a, hits, slot, c + g, [&](int j, int off) {
+          const float q = (a.plan.q ? a.plan.q[(long long)j * a.Tp + slot] : 1.f) * r;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] -= e == off ? q : 0.f;
+        });
+        uint16_t* const to = a.G + (long long)row * a.ldg + col + g;
+        float left[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) left[e] = v[e];
+        const int planes = a.products == 1 ? 1 : 3;
+        for (int p = 0; p < planes; ++p) {
+          uint32_t u[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) u[e] = pack2(left[2 * e], left[2 * e + 1], a.fp16);
+          uint32_t lo[8], hi[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) lo[e] = u[e], hi[e] = u[8 + e];
+          st_v8(to + p * (long long)a.Tp * a.ldg, lo);
+          st_v8(to + p * (long long)a.Tp * a.ldg + 16, hi);
+          if (planes == 1) break;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) left[2 * e] -= bf16_lo(u[e]), left[2 * e + 1] -= bf16_hi(u[e]);
+        }
+        if (a.colsum != nullptr) {                        // over the warp's 32 rows: lane l ends with column l
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < o; ++i) {
+              const bool up = lane & o;
+              const float give = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
+              v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+            }
+          a.colsum[(long long)(row >> 5) * a.ldg + col + g + lane] = v[0];
+        }
+      }
+    }
+  } else {
+    if (MODE == DW && a.dw != nullptr) {
+      const float alpha = a.coef[0];
+      const int v = a.col0 + row;
+      if (v >= a.V) return;
+#pragma unroll
+      for (int g = 0; g < W; g += 8) {
+        if (col + g >= a.K) continue;
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = acc[g + e] * alpha;
+        const long long at = (long long)v * a.K + col + g;
+        if (a.K % 8 == 0) {
+          if (a.dw_type == SPION_F32) Out<float, 8>::store(static_cast<float*>(a.dw) + at, f);
+          else if (a.dw_type == SPION_BF16) Out<__nv_bfloat16, 8>::store(static_cast<__nv_bfloat16*>(a.dw) + at, f);
+          else Out<__half, 8>::store(static_cast<__half*>(a.dw) + at, f);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (col + g + e < a.K) store_any(a.dw, a.dw_type, at + e, f[e]);
+        }
+      }
+      return;
+    }
+    float* const to = a.out + ((long long)s * w.tiles_m * tile_m + row) * a.ldo + col;
+#pragma unroll
+    for (int g = 0; g < W; g += 8) {
+      if (col + g >= a.ldo) continue;
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = acc[g + e];
+      if (a.add) {
+        Piece<float, 8> was;
+        was.load(to + g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] += was.at(e);
+      }
+      Out<float, 8>::store(to + g, f);
+    }
+  }
+}
+
+// Warp 0 loads, warp 1 multiplies, the others take the sums.  Every wait is bounded; whoever gives up reports it and leaves, and so do all that wait for it; the warps
+// that write go on with NaN.  PAIR: two CTAs of a cluster share a tile of 256 x 256, each brings 128 rows of either operand and holds 128 rows of the sums; the first one's warp 1
+// multiplies for both (see k_lin8 in linear_e4m3.cu, whose scheme this is).  Else tiles of 128 x 128.
+// Operands whose contraction runs along memory (K-major: x and W in z, G in dx) come as one box of 128 rows x 64; those whose contraction runs across it (MN-major: W in dx, G and x
+// in dW) as two boxes of 64 rows x 64.
+template <int MODE, bool PAIR> __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Args a, const __grid_constant__ Maps maps) {
+  constexpr int BN = PAIR ? 256 : 128, TILE = PAIR ? 256 : 128, W = BN / 2;
+  constexpr bool A_MN = MODE == DW, B_MN = MODE == DX || MODE == DW;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t sbase = smem_u32(smem_raw);
+  const uint32_t full = sbase + BARS, empty = full + 8 * STAGES, acc_full = empty + 8 * STAGES, acc_empty = acc_full + 16, slot = acc_empty + 16;
+  const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  volatile int& s_abort = *reinterpret_cast<int*>(smem_raw + (slot + 8 - sbase));
+  const int rank = PAIR ? (int)cta_rank() : 0, first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+  if (warp == 0 && lane == 0) {
+    s_abort = *reinterpret_cast<volatile int*>(&g_vocab_status);
+    for (int i = 0; i < STAGES; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(acc_full + 8 * i, 1), mbar_init(acc_empty + 8 * i, PAIR ? 2 * EPI : EPI);
+    fence_barrier_init();
+    fence_proxy_async();
+    tma_prefetch_desc(&maps.a);
+    tma_prefetch_desc(&maps.b);
+  }
+  if (warp == 1) {
+    if (PAIR) {
+      pair_tmem_alloc(slot, 2 * BN);
+    } else {
+      tmem_alloc(slot, 2 * BN);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (PAIR) cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<uint32_t*>(smem_raw + (slot - sbase));
+  wait_for_kernel_before();
+  const int n = *reinterpret_cast<const volatile int*>(a.n);
+  const Work w = work_of(a, n, TILE, BN, step);
+  const int items = w.splits * w.tiles_m * w.tiles_n;
+  const bool aborted = s_abort != 0;
+  if (warp == 0) {
+    if (!aborted && elect_one()) {
+      int st = 0, ph = 1;                                  // a ring that has not been used yet is empty
+      long long fills = 0;
+      bool ok = true;
+      for (int i = first; i < items && ok; i += step) {
+        int s, m, nn, c0, c1;
+        item_at(w, i, s, m, nn, c0, c1);
+        const int ra = m * TILE + rank * 128, rb = nn * BN + rank * 128;
+        for (int c = c0; c < c1 && ok; ++c)
+          for (int p = 0; p < a.products; ++p) {
+            ok = mbar_wait(empty + 8 * st, ph);
+            if (!ok) break;
+            int pa, pb;
+            parts_of(a.products, p, pa, pb);
+            const uint32_t to_a = sbase + st * STAGE, to_b = to_a + HALF;
+            uint32_t bar = full + 8 * st;
+            if (PAIR) {
+              if (rank == 0) mbar_expect_tx(bar, 2 * STAGE);
+              bar = in_leader(bar);
+            } else {
+              mbar_expect_tx(bar, STAGE);
+            }
+            auto load = [&](uint32_t to, const CUtensorMap* map, int x, int y) {
+              if (PAIR) pair_tma_load_2d(to, map, bar, x, y);
+              else tma_load_2d(to, map, bar, x, y);
+            };
+            const int ya = (int)(pa * a.plane_a), yb = (int)(pb * a.plane_b) + (MODE == LOGSUM || MODE == GRAD || MODE == DX ? a.col0 : 0);
+            if (A_MN) {
+              load(to_a, &maps.a, ra, ya + c * BK);
+              load(to_a + HALF / 2, &maps.a, ra + 64, ya + c * BK);
+            } else {
+              load(to_a, &maps.a, c * BK, ya + ra);
+            }
+            if (B_MN) {
+              load(to_b, &maps.b, rb, yb + c * BK);
+              load(to_b + HALF / 2, &maps.b, rb + 64, yb + c * BK);
+            } else {
+              load(to_b, &maps.b, c * BK, yb + rb);
+            }
+            ++fills;
+            if (++st == STAGES) st = 0, ph ^= 1;
+          }
+      }
+      if (!ok) {                                           // the copies under way end first (a pair's are counted in its first CTA), or this gives up again
+        report(&g_vocab_status, ERR_LOAD_WAIT);
+        for (long long j = fills > STAGES ? fills - STAGES : 0; j < fills && rank == 0; ++j)
+          mbar_wait(full + 8 * (int)(j % STAGES), (int)(j / STAGES) & 1);
+      }
+    }
+  } else if (warp == 1) {
+    if (!aborted && rank == 0 && elect_one()) {
+      const uint32_t kind = a.fp16 ? 0u : (1u << 7) | (1u << 10);
+      const uint32_t idesc = (1u << 4) | kind | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24);
+      const uint64_t a0 = make_smem_desc(sbase, A_MN ? HALF / 2 : 16, 1024, LAYOUT_SW128), b0 = make_smem_desc(sbase + HALF, B_MN ? HALF / 2 : 16, 1024, LAYOUT_SW128);
+      constexpr uint32_t step_a = A_MN ? 2048 : 32, step_b = B_MN ? 2048 : 32;
+      int st = 0, ph = 0, buf = 0, acc_ph = 1;
+      bool ok = true;
+      for (int i = first; i < items && ok; i += step) {
+        int s, m, nn, c0, c1;
+        item_at(w, i, s, m, nn, c0, c1);
+        const int all = (c1 - c0) * a.products;
+        for (int done = 0; done < all && ok;) {
+          ok = mbar_wait(acc_empty + 8 * buf, acc_ph);
+          tc_fence_after();
+          const int until = min(all, done + a.chain);
+          for (bool more = false; done < until && ok; ++done) {
+            ok = mbar_wait(full + 8 * st, ph);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k) {
+              const uint64_t ad = desc_advance(a0, st * STAGE + step_a * k), bd = desc_advance(b0, st * STAGE + step_b * k);
+              if (PAIR) pair_mma(tmem + buf * BN, ad, bd, idesc, more);
+              else mma_bf16(tmem + buf * BN, ad, bd, idesc, more);
+              more = true;
+            }
+            if (PAIR) pair_commit(empty + 8 * st);
+            else mma_commit(empty + 8 * st);
+            if (++st == STAGES) st = 0, ph ^= 1;
+          }
+          if (ok) {
+            if (PAIR) pair_commit(acc_full + 8 * buf);
+            else mma_commit(acc_full + 8 * buf);
+          }
+          buf ^= 1;
+          if (buf == 0) acc_ph ^= 1;
+        }
+      }
+      if (!ok) report(&g_vocab_status, ERR_MMA_WAIT);
+    }
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    int buf = 0, ph = 0;
+    bool lost = aborted;
+    float acc[W];
+    for (int i = first; i < items; i += step) {
+      int s, m, nn, c0, c1;
+      item_at(w, i, s, m, nn, c0, c1);
+      const int all = (c1 - c0) * a.products;
+#pragma unroll
+      for (int g = 0; g < W; ++g) acc[g] = 0.f;
+      for (int done = 0; done < all && !lost; done += a.chain) {
+        if (!tc::warp_wait(acc_full + 8 * buf, ph, &g_vocab_status, ERR_MMA2_WAIT)) {
+          lost = true;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + buf * BN + half * W;
+#pragma unroll
+        for (int g = 0; g < W; g += 32) {
+          uint32_t r[32];
+          tmem_ld32(at + g, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) acc[g + e] += __uint_as_float(r[e]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) pair_arrive(in_leader(acc_empty + 8 * buf));
+          else mbar_arrive(acc_empty + 8 * buf);
+        }
+        buf ^= 1;
+        if (buf == 0) ph ^= 1;
+      }
+      if (lost)
+#pragma unroll
+        for (int g = 0; g < W; ++g) acc[g] = not_a_number();
+      epilogue<MODE, W>(a, w, acc, n, s, m * TILE + rank * 128 + q * 32 + lane, nn * BN + half * W, TILE, 2 * nn + half);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (PAIR) cluster_sync();                                // neither CTA's memory goes while the other may signal in it
+  tc_fence_after();
+  if (warp == 1) {
+    if (PAIR) pair_tmem_dealloc(tmem, 2 * BN);
+    else tmem_dealloc(tmem, 2 * BN);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ losses
+struct Finish {
+  Plan plan; int Tp, k;
+  const float2* part; int parts;
+  const float* zt;
+  float* loss;              // [T] (reduction 0) or one number
+  float* slot_loss;         // [Tp]
+  int reduction;            // 0 none, 1 mean, 2 sum
+};
+// A warp per row that counts; the last CTA adds them up, in their order.
+__global__ void __launch_bounds__(256) k_finish(const __grid_constant__ Finish a) {
+  next_may_start();
+  wait_for_kernel_before();
+  __shared__ double sums[256];
+  __shared__ int last;
+  const int lane = threadIdx.x & 31, n = *reinterpret_cast<const volatile int*>(a.plan.head);
+  const bool lost = *reinterpret_cast<volatile int*>(&g_vocab_status) != 0;
+  for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += gridDim.x * 8) {
+    const float2* const p = a.part + (long long)i * a.parts;
+    float top = -INFINITY, sum = 0.f;
+    for (int c = lane; c < a.parts; c += 32) {
+      const float2 v = p[c];
+      const float m = fmaxf(top, v.x), from = m == -INFINITY ? 0.f : m;
+      sum = sum * ex2(top - from) + v.y * ex2(v.x - from);
+      top = m;
+    }
+    const float all = lane_max<32>(top), from = all == -INFINITY ? 0.f : all;
+    sum = lane_sum<32>(sum * ex2(top - from));
+    float lse = from + log2f(sum), loss = 0.f;
+    for (int j = lane; j < a.k; j += 32) {
+      const long long at = (long long)j * a.Tp + i;
+      if (a.plan.target[at] == -1) continue;
+      const float q = a.plan.q ? a.plan.q[at] : 1.f;
+      loss += q * ((a.plan.q ? log2f(q) : 0.f) + (lse - a.zt[at]));
+    }
+    loss = lane_sum<32>(loss) * LN2;
+    if (lost) loss = not_a_number();
+    if (lane == 0) {
+      a.plan.lse[i] = loss != loss ? loss : lse;          // a row without a loss has no gradient either: NaN
+      if (a.reduction == 0) a.loss[a.plan.row[i]] = loss;
+      else a.slot_loss[i] = loss;
+    }
+  }
+  if (a.reduction == 0) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(a.plan.head + 1, 1) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += 256) s += (double)*reinterpret_cast<volatile float*>(a.slot_loss + i);
+  sums[threadIdx.x] = s;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) sums[threadIdx.x] += sums[threadIdx.x + o];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *a.loss = a.reduction == 2 ? (float)sums[0] : n > 0 ? (float)(sums[0] / n) : not_a_number();
+}
+
+// ------------------------------------------------------------------------------------------------ gradients
+// coef[0]: what the products with G are multiplied with; coef[1]: 1 / max |g| where every row has its own g (rounded to a power of two).  The first CTA; the others
+// form the bias in units of log2.
+__global__ void __launch_bounds__(1024) k_coef(const __grid_constant__ Prep a, const float* g, int reduction, float inv_gscale, float* coef) {
+  next_may_start();
+  wait_for_kernel_before();
+  if (blockIdx.x > 0) {
+    scaled_bias(a, (blockIdx.x - 1) * 1024 + threadIdx.x, (gridDim.x - 1) * 1024);
+    return;
+  }
+  __shared__ float part[32];
+  const Plan& plan = a.plan;
+  const float inv_tau = a.inv_tau;
+  const int n = *reinterpret_cast<const volatile int*>(plan.head);
+  float top = 0.f;
+  if (reduction == 0)
+    for (int i = threadIdx.x; i < n; i += 1024) {
+      const float v = fabsf(g[plan.row[i]]);
+      if (v < INFINITY) top = fmaxf(top, v);              // one that is not finite stays its own row's
+    }
+  top = lane_max<32>(top);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    top = lane_max<32>(part[threadIdx.x]);
+    if (threadIdx.x == 0) {
+      if (reduction == 0) {
+        // a power of two: the products by it are exact, and neither it nor its reciprocal leaves the normal numbers
+        const float unit = top > 0.f ? exp2f(fminf(fmaxf(ceilf(log2f(top)), -100.f), 126.f)) : 1.f;
+        coef[0] = unit * inv_tau * inv_gscale, coef[1] = 1.f / unit;
+      } else {
+        coef[0] = n > 0 ? (reduction == 1 ? *g / (float)n : *g) * inv_tau * inv_gscale : 0.f;
+        coef[1] = 1.f;
+      }
+    }
+  }
+}
+// dx of all rows: the sums of the splits, zeros where a row does not count.  Also joins the parts of dW (no slots, rows one behind another).
+struct Join {
+  const int* head; const int* slot;                       // slot null: rows are slots
+  const float* part; long long ldp;                       // [splits][plane rows][ldp]
+  int splits, tile, tiles_n, units, chunks;               // splits 0: as k_gemm<DX> had them
+  long long plane;                                        // rows of a split (splits given)
+  const float* coef;
+  void* out; int type; long long rows, K;
+};
+__global__ void __launch_bounds__(256) k_join(const __grid_constant__ Join a) {
+  next_may_start();
+  wait_for_kernel_before();
+  const int n = *reinterpret_cast<const volatile int*>(a.head);
+  const bool lost = *reinterpret_cast<volatile int*>(&g_vocab_status) != 0;
+  const float alpha = lost ? not_a_number() : a.coef[0];
+  int splits = a.splits;
+  long long plane = a.plane;
+  if (splits == 0) {
+    const int tiles_m = (n + a.tile - 1) / a.tile;
+    splits = split_by_tiles(tiles_m * a.tiles_n, a.units, a.chunks);
+    plane = (long long)tiles_m * a.tile;
+  }
+  const long long pieces = (a.K + 7) / 8, all = a.rows * pieces;
+  const bool whole = a.K % 8 == 0;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
+    const long long r = i / pieces, c = (i - r * pieces) * 8;
+    const long long from = a.slot ? a.slot[r] : r;
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (from >= 0) {
+      for (int s = 0; s < splits; ++s) {
+        Piece<float, 8> p;
+        p.load(a.part + (s * plane + from) * a.ldp + c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] += p.at(e);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] *= alpha;
+    }
+    const long long at = r * a.K + c;
+    if (whole) {
+      if (a.type == SPION_F32) Out<float, 8>::store(static_cast<float*>(a.out) + at, f);
+      else if (a.type == SPION_BF16) Out<__nv_bfloat16, 8>::store(static_cast<__nv_bfloat16*>(a.out) + at, f);
+      else Out<__half, 8>::store(static_cast<__half*>(a.out) + at, f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c + e < a.K) store_any(a.out, a.type, at + e, f[e]);
+    }
+  }
+}
+// db of a piece: 32 columns a CTA, eight shares of the blocks of 32 rows
+__global__ void __launch_bounds__(256) k_db(const int* head, const float* colsum, long long ldg, int columns, const float* coef, void* db, int type) {
+  next_may_start();
+  wait_for_kernel_before();
+  __shared__ float part[8][32];
+  const int n = *reinterpret_cast<const volatile int*>(head), lane = threadIdx.x & 31, share = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (c < columns)
+    for (int b = share; b < (n + 31) / 32; b += 8) s += colsum[b * ldg + c];
+  part[share][lane] = s;
+  __syncthreads();
+  if (share > 0 || c >= columns) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) s += part[i][lane];
+  const bool lost = *reinterpret_cast<volatile int*>(&g_vocab_status) != 0;
+  store_any(db, type, c, lost ? not_a_number() : s * coef[0]);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                            CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+int encoder(Encode* out) {
+  static std::atomic<Encode> known{nullptr};
+  Encode e = known.load();
+  if (e == nullptr) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    SPION_CUDA_TRY(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
+    if (q != cudaDriverEntryPointSuccess || fn == nullptr) return SPION_ERR_CUDA;
+    known.store(e = reinterpret_cast<Encode>(fn));
+  }
+  *out = e;
+  return SPION_OK;
+}
+// boxes of 64 columns x box_rows of a matrix of 16-bit elements
+int map_of(CUtensorMap* m, const void* base, long long cols, long long rows_, long long ld, int box_rows) {
+  Encode encode;
+  const int rc = encoder(&encode);
+  if (rc != SPION_OK) return rc;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows_}, strides[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t box[2] = {BK, (cuuint32_t)box_rows}, step[2] = {1, 1};
+  const CUresult r = encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    fprintf(stderr, "spion_b200: cuTensorMapEncodeTiled failed (%d) rows=%lld cols=%lld\n", (int)r, rows_, cols);
+    return SPION_ERR_CUDA;
+  }
+  return SPION_OK;
+}
+// CTAs (or pairs) of a kernel that the current device holds at a time
+template <int MODE, bool PAIR> int units_of(int* units) {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  SPION_CUDA_TRY(cudaGetDevice(&dev));
+  int n = dev < 64 ? known[dev].load() : 0;
+  if (n == 0) {
+    SPION_CUDA_TRY(cudaFuncSetAttribute(k_gemm<MODE, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
+    if (PAIR) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = 2, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+      cfg.gridDim = dim3(2 * (sm_count() / 2)), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = SMEM, cfg.attrs = at, cfg.numAttrs = 1;
+      SPION_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, k_gemm<MODE, PAIR>, &cfg));
+    } else {
+      n = sm_count();
+    }
+    if (n <= 0) return SPION_ERR_UNSUPPORTED;
+    if (dev < 64) known[dev].store(n);
+  }
+  *units = n;
+  return SPION_OK;
+}
+template <int MODE, bool PAIR> int launch_gemm(const Args& a, const Maps& maps, long long most_items, cudaStream_t st) {
+  int units;
+  const int rc = units_of<MODE, PAIR>(&units);
+  if (rc != SPION_OK) return rc;
+  // DX splits its contraction by the number of units: it always has all of them
+  const int use = a.splits == 0 ? units : (int)std::min<long long>(units, std::max<long long>(most_items, 1));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = 2, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(PAIR ? 2 * use : use), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = SMEM, cfg.stream = st, cfg.attrs = at, cfg.numAttrs = PAIR ? 2 : 1;
+  SPION_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_gemm<MODE, PAIR>, a, maps));
+  return SPION_OK;
+}
+template <int MODE> int launch_gemm(bool pair, const Args& a, const Maps& maps, long long most_items, cudaStream_t st) {
+  return pair ? launch_gemm<MODE, true>(a, maps, most_items, st) : launch_gemm<MODE, false>(a, maps, most_items, st);
+}
+
+constexpr long long up(long long x, long long to) { return (x + to - 1) / to * to; }
+constexpr long long tiles_of(long long x, long long tile) { return (x + tile - 1) / tile; }
+constexpr int CHAIN = 16;                                 // 64 steps of 16
+constexpr int LONG_CHAIN = 64;                            // of a result that is rounded to 16 bits
+
+// Sizes and places of a call
+struct Layout {
+  long long T, Tp, K, Kp, V, Vp, k, ldw;
+  int planes;
+  bool copy_w;
+  bool pair_z, pair_dx, pair_dw;
+  long long Gp;                                           // columns of a piece of the vocabulary
+  int dw_splits;
+  size_t keep;                                            // bytes of the plan
+  size_t xs, w, bias2, part, zt, slot_loss, counts, q, forward;
+  size_t g, dxp, dwp, colsum, coef, backward;
+};
+constexpr long long PIECE_BYTES = 256ll << 20;            // of G
+
+int layout_of(const spion_vocab_problem* p, Layout* l) {
+  if (p == nullptr || p->T < 0 || p->K <= 0 || p->V <= 0 || p->k <= 0) return SPION_ERR_ARG;
+  if (p->type != SPION_F32 && p->type != SPION_BF16 && p->type != SPION_F16) return SPION_ERR_ARG;
+  if (p->k > MAX_TARGETS) return SPION_ERR_UNSUPPORTED;
+  if (!(p->temperature > 0.f) || !(p->temperature < INFINITY) || p->ldx < 0 || p->ldw < p->K) return SPION_ERR_ARG;
+  if (p->reduction < 0 || p->reduction > 2) return SPION_ERR_ARG;
+  *l = Layout();
+  l->T = p->T, l->K = p->K, l->V = p->V, l->k = p->k;
+  l->Tp = up(std::max(p->T, 1ll), PAD), l->Kp = up(p->K, BK), l->Vp = up(p->V, PAD);
+  l->planes = p->type == SPION_F32 ? 3 : 1;
+  // places are 32-bit numbers in the tensor maps' coordinates and in the lists of rows
+  if (p->T > 0x7fffffff / 4 || p->V > 0x7fffffff / 4 || p->K > 0x7fffffff / 4 || l->Tp * l->planes > 0x7fffffff || l->Vp * l->planes > 0x7fffffff) return SPION_ERR_SHAPE;
+  l->copy_w = p->type == SPION_F32 || ((uintptr_t)p->w % 16) != 0 || (p->ldw * 2) % 16 != 0;
+  l->ldw = l->copy_w ? l->Kp : p->ldw;
+  int sms = sm_count();
+  if (sms <= 0) return SPION_ERR_CUDA;
+  const int pairs = sms / 2;
+  // Tiles of pairs where every pair has one, else four times as many small ones.
+  auto pair = [&](long long m, long long n) { return m > 128 && n > 128 && tiles_of(m, 256) * tiles_of(n, 256) >= pairs; };
+  l->pair_z = pair(l->T, l->V);
+  l->Gp = std::min(l->Vp, std::max<long long>(PAD, PIECE_BYTES / (2 * l->planes * l->Tp) / PAD * PAD));
+  l->pair_dx = pair(l->T, l->K);
+  l->pair_dw = pair(l->Gp, l->K);
+  const long long dw_tiles = l->pair_dw ? tiles_of(l->Gp, 256) * tiles_of(l->K, 256) : tiles_of(l->Gp, 128) * tiles_of(l->K, 128);
+  l->dw_splits = l->pair_dw ? 1 : split_by_tiles((int)dw_tiles, sms, (int)std::max<long long>(1, tiles_of(l->T, BK) / 4));
+  size_t at = 0;
+  auto take = [&](long long bytes) {
+    const size_t here = at;
+    at += (size_t)up(std::max(bytes, 0ll), 256);
+    return here;
+  };
+  take(256), take(4 * l->Tp), take(4 * l->Tp), take(4 * l->Tp), take(4 * l->k * l->Tp), take(4 * l->k * l->Tp);
+  l->keep = at;
+  at = 0;
+  l->xs = take(2 * l->planes * l->Tp * l->Kp);
+  l->w = take(l->copy_w ? 2 * l->planes * l->Vp * l->Kp : 0);
+  l->bias2 = take(4 * l->Vp);
+  const size_t both = at;
+  l->part = take(8 * l->Tp * 2 * (l->pair_z ? tiles_of(l->V, 256) : tiles_of(l->V, 128)));
+  l->zt = take(4 * l->k * l->Tp);
+  l->slot_loss = take(4 * l->Tp);
+  l->counts = take(4 * tiles_of(l->T, CHUNK));
+  l->q = take(4 * l->T * l->k);
+  l->forward = at;
+  at = both;
+  l->g = take(2 * l->planes * l->Tp * l->Gp);
+  const long long tile = l->pair_dx ? 256 : 128, tn = tiles_of(l->K, tile);
+  l->dxp = take(4 * std::max(tiles_of(l->T, tile), (l->pair_dx ? pairs : sms) / tn) * tile * l->Kp);
+  l->dwp = take(l->dw_splits > 1 ? 4 * l->dw_splits * up(l->Gp, l->pair_dw ? 256 : 128) * l->Kp : 0);
+  l->colsum = take(4 * (l->Tp / 32) * l->Gp);
+  l->coef = take(256);
+  l->backward = at;
+  return SPION_OK;
+}
+Plan plan_at(const Layout& l, void* keep, bool teacher) {
+  char* c = static_cast<char*>(keep);
+  Plan p;
+  p.head = (int*)c, c += 256;
+  const size_t rows_ = (size_t)up(4 * l.Tp, 256), targets = (size_t)up(4 * l.k * l.Tp, 256);
+  p.slot = (int*)c, c += rows_;
+  p.row = (int*)c, c += rows_;
+  p.lse = (float*)c, c += rows_;
+  p.target = (int*)c, c += targets;
+  p.q = teacher ? (float*)c : nullptr;
+  return p;
+}
+Source source_of(const void* p, int type, long long ld, long long K, long long Kp) {
+  const int piece = type == SPION_F32 ? 32 : 16;
+  return {p, type, ld, (int)K, (int)Kp, K % 8 == 0 && (uintptr_t)p % piece == 0 && ld * type_size(type) % piece == 0};
+}
+int launch_copy_w(const spion_vocab_problem* p, const Layout& l, uint16_t* to, cudaStream_t st) {
+  if (!l.copy_w) return SPION_OK;
+  const Source s = source_of(p->w, p->type, p->ldw, l.K, l.Kp);
+  const dim3 grid((unsigned)std::min<long long>(tiles_of(l.Vp * l.Kp / 8, 256), 8 * sm_count()));
+  if (p->type == SPION_F32) SPION_CUDA_TRY(launch_after(k_copy_w<float>, grid, dim3(256), 0, st, s, (int)l.V, (int)l.Vp, to));
+  else SPION_CUDA_TRY(launch_after(k_copy_w<__half>, grid, dim3(256), 0, st, s, (int)l.V, (int)l.Vp, to));
+  return SPION_OK;
+}
+Prep prep_of(const spion_vocab_problem* p, const Layout& l, void* keep, char* ws) {
+  Prep a = {};
+  a.plan = plan_at(l, keep, p->teacher != nullptr);
+  a.labels = p->labels, a.teacher = p->teacher, a.teacher_type = p->teacher_type, a.ignore = p->ignore_index;
+  a.inv_tau = 1.f / p->temperature;
+  a.T = (int)l.T, a.Tp = (int)l.Tp, a.V = (int)l.V, a.k = (int)l.k, a.Vp = (int)l.Vp;
+  a.counts = (int*)(ws + l.counts), a.q = (float*)(ws + l.q);
+  a.bias = p->bias, a.bias_type = p->bias_type, a.bias2 = (float*)(ws + l.bias2);
+  a.c1 = (float)(1.4426950408889634 / (double)p->temperature);
+  return a;
+}
+template <bool FIRST> int launch_gather(const spion_vocab_problem* p, const Layout& l, const Prep& a, uint16_t* xs, float* loss_rows, float* zt, cudaStream_t st) {
+  const Source s = source_of(p->x, p->type, p->ldx, l.K, l.Kp);
+  const dim3 grid((unsigned)tiles_of(l.T, CHUNK));
+  if (p->type == SPION_F32) SPION_CUDA_TRY(launch_after(k_gather<float, FIRST>, grid, dim3(256), 0, st, a, s, xs, loss_rows, zt));
+  else SPION_CUDA_TRY(launch_after(k_gather<__half, FIRST>, grid, dim3(256), 0, st, a, s, xs, loss_rows, zt));
+  return SPION_OK;
+}
+// What the two passes over z have in common
+int logits_args(const spion_vocab_problem* p, const Layout& l, const Prep& prep, char* ws, Args* a, Maps* maps) {
+  *a = Args();
+  a->n = prep.plan.head;
+  a->products = l.planes == 1 ? 1 : 6;
+  a->plane_a = l.Tp, a->plane_b = l.Vp;
+  a->L = (int)l.K;
+  a->chain = CHAIN;
+  a->splits = 1;
+  a->fp16 = p->type == SPION_F16;
+  a->plan = prep.plan, a->Tp = (int)l.Tp, a->k = (int)l.k;
+  a->bias2 = (const float*)(ws + l.bias2), a->c1 = prep.c1;
+  int rc = map_of(&maps->a, ws + l.xs, l.Kp, l.planes * l.Tp, l.Kp, 128);
+  if (rc == SPION_OK)
+    rc = l.copy_w ? map_of(&maps->b, ws + l.w, l.Kp, l.planes * l.Vp, l.Kp, 128) : map_of(&maps->b, p->w, l.K, l.V, l.ldw, 128);
+  return rc;
+}
+
+int check_problem(const spion_vocab_problem* p, const void* keep, const void* workspace) {
+  if (p->x == nullptr || p->w == nullptr || p->labels == nullptr || keep == nullptr || workspace == nullptr) return SPION_ERR_ARG;
+  if (p->teacher != nullptr && p->teacher_type != SPION_F32 && p->teacher_type != SPION_BF16 && p->teacher_type != SPION_F16) return SPION_ERR_ARG;
+  if (p->teacher == nullptr && p->k != 1) return SPION_ERR_ARG;
+  if (p->bias != nullptr && p->bias_type != SPION_F32 && p->bias_type != SPION_BF16 && p->bias_type != SPION_F16) return SPION_ERR_ARG;
+  if (((uintptr_t)keep | (uintptr_t)workspace) % 256 != 0) return SPION_ERR_ARG;
+  return SPION_OK;
+}
+
+}  // namespace
+
+int* vocab_status_word() {
+  static StatusWord word;
+  return word.on_this_device(g_vocab_status);
+}
+
+extern "C" int spion_vocab_sizes(const spion_vocab_problem* p, long long* keep_bytes, long long* forward_bytes, long long* backward_bytes) {
+  Layout l;
+  const int rc = layout_of(p, &l);
+  if (rc != SPION_OK) return rc;
+  if (keep_bytes) *keep_bytes = (long long)l.keep;
+  if (forward_bytes) *forward_bytes = (long long)l.forward;
+  if (backward_bytes) *backward_bytes = (long long)l.backward;
+  return SPION_OK;
+}
+
+extern "C" int spion_vocab_loss_forward(const spion_vocab_problem* p, float* loss, void* keep, void* workspace, void* cuda_stream) {
+  Layout l;
+  int rc = layout_of(p, &l);
+  if (rc != SPION_OK) return rc;
+  if (l.T == 0) return p->reduction == 0 ? SPION_OK : SPION_ERR_ARG;      // nothing to take a mean of
+  if ((rc = check_problem(p, keep, workspace)) != SPION_OK) return rc;
+  if (loss == nullptr) return SPION_ERR_ARG;
+  const cudaStream_t st = (cudaStream_t)cuda_stream;
+  char* const ws = static_cast<char*>(workspace);
+  const Prep prep = prep_of(p, l, keep, ws);
+  float* const zt = (float*)(ws + l.zt);
+  const long long warps = std::max(tiles_of(l.T, CHUNK), tiles_of(l.Vp, 32 * 8));
+  SPION_CUDA_TRY(launch_after(k_flags, dim3((unsigned)std::min<long long>(tiles_of(warps, 8), 8 * sm_count())), dim3(256), 0, st, prep));
+  if ((rc = launch_gather<true>(p, l, prep, (uint16_t*)(ws + l.xs), p->reduction == 0 ? loss : nullptr, zt, st)) != SPION_OK) return rc;
+  if ((rc = launch_copy_w(p, l, (uint16_t*)(ws + l.w), st)) != SPION_OK) return rc;
+  Args a;
+  Maps maps;
+  if ((rc = logits_args(p, l, prep, ws, &a, &maps)) != SPION_OK) return rc;
+  const int tile = l.pair_z ? 256 : 128;
+  a.N = (int)l.V, a.part = (float2*)(ws + l.part), a.parts = (int)(2 * tiles_of(l.V, tile)), a.zt = zt;
+  if ((rc = launch_gemm<LOGSUM>(l.pair_z, a, maps, tiles_of(l.T, tile) * tiles_of(l.V, tile), st)) != SPION_OK) return rc;
+  const Finish f = {prep.plan, (int)l.Tp, (int)l.k, a.part, a.parts, zt, loss, (float*)(ws + l.slot_loss), p->reduction};
+  SPION_CUDA_TRY(launch_after(k_finish, dim3((unsigned)std::min<long long>(tiles_of(l.T, 8), 4 * sm_count())), dim3(256), 0, st, f));
+  return SPION_OK;
+}
+
+extern "C" int spion_vocab_loss_backward(const spion_vocab_problem* p, const float* g, const void* keep, void* dx, void* dw, void* db, int db_type, void* workspace,
+                                         void* cuda_stream) {
+  Layout l;
+  int rc = layout_of(p, &l);
+  if (rc != SPION_OK) return rc;
+  if (l.T == 0) return SPION_ERR_ARG;
+  if ((rc = check_problem(p, keep, workspace)) != SPION_OK) return rc;
+  if (g == nullptr || (dx == nullptr && dw == nullptr && db == nullptr)) return SPION_ERR_ARG;
+  if (db != nullptr && db_type != SPION_F32 && db_type != SPION_BF16 && db_type != SPION_F16) return SPION_ERR_ARG;
+  if (((uintptr_t)dx | (uintptr_t)dw) % 32 != 0) return SPION_ERR_ARG;
+  const cudaStream_t st = (cudaStream_t)cuda_stream;
+  char* const ws = static_cast<char*>(workspace);
+  const Prep prep = prep_of(p, l, const_cast<void*>(keep), ws);
+  uint16_t *const xs = (uint16_t*)(ws + l.xs), *const G = (uint16_t*)(ws + l.g);
+  float* const coef = (float*)(ws + l.coef);
+  const float gscale = p->type == SPION_F16 ? 8192.f : 1.f;
+  SPION_CUDA_TRY(launch_after(k_coef, dim3(1 + (unsigned)std::min<long long>(tiles_of(l.Vp, 1024), 2 * sm_count())), dim3(1024), 0, st, prep, g, p->reduction, 1.f / gscale, coef));
+  if ((rc = launch_gather<false>(p, l, prep, xs, nullptr, nullptr, st)) != SPION_OK) return rc;
+  if ((rc = launch_copy_w(p, l, (uint16_t*)(ws + l.w), st)) != SPION_OK) return rc;
+  Args z;
+  Maps zm, xm, wm;
+  if ((rc = logits_args(p, l, prep, ws, &z, &zm)) != SPION_OK) return rc;
+  if ((rc = map_of(&xm.a, G, l.Gp, l.planes * l.Tp, l.Gp, 128)) != SPION_OK) return rc;
+  if ((rc = l.copy_w ? map_of(&xm.b, ws + l.w, l.Kp, l.planes * l.Vp, l.Kp, 64) : map_of(&xm.b, p->w, l.K, l.V, l.ldw, 64)) != SPION_OK) return rc;
+  if ((rc = map_of(&wm.a, G, l.Gp, l.planes * l.Tp, l.Gp, 64)) != SPION_OK) return rc;
+  if ((rc = map_of(&wm.b, xs, l.Kp, l.planes * l.Tp, l.Kp, 64)) != SPION_OK) return rc;
+  int dx_units = 0;
+  if ((rc = l.pair_dx ? units_of<DX, true>(&dx_units) : units_of<DX, false>(&dx_units)) != SPION_OK) return rc;
+  const int tz = l.pair_z ? 256 : 128, tx = l.pair_dx ? 256 : 128, tw = l.pair_dw ? 256 : 128;
+  z.g = p->reduction == 0 ? g : nullptr, z.coef = coef, z.G = G, z.ldg = l.Gp, z.gscale = gscale;
+  z.colsum = db != nullptr ? (float*)(ws + l.colsum) : nullptr;
+  int dx_chunks = 0;
+  for (long long c = 0; c < l.V; c += l.Gp) {
+    const long long columns = std::min(l.Gp, l.V - c), padded = up(columns, PAD);
+    z.col0 = (int)c, z.N = (int)padded;
+    if ((rc = launch_gemm<GRAD>(l.pair_z, z, zm, tiles_of(l.T, tz) * tiles_of(padded, tz), st)) != SPION_OK) return rc;
+    Args b = z;
+    b.col0 = (int)c;
+    b.chain = l.planes == 3 ? CHAIN : LONG_CHAIN;
+    if (dx != nullptr) {
+      // every piece's contraction is cut as the first one's: the parts are added piece by piece
+      if (c == 0) dx_chunks = (int)tiles_of(columns, BK);
+      Args d = b;
+      d.N = (int)l.K, d.L = (int)columns, d.splits = 0, d.split_chunks = dx_chunks;
+      d.plane_a = l.Tp, d.plane_b = l.Vp;
+      d.out = (float*)(ws + l.dxp), d.ldo = l.Kp, d.add = c > 0;
+      if ((rc = launch_gemm<DX>(l.pair_dx, d, xm, 0, st)) != SPION_OK) return rc;
+    }
+    if (dw != nullptr) {
+      Args d = b;
+      d.M = (int)padded, d.N = (int)l.K, d.L = 0, d.splits = l.dw_splits;
+      d.plane_a = l.Tp, d.plane_b = l.Tp;
+      d.out = (float*)(ws + l.dwp), d.ldo = l.Kp, d.add = 0;
+      d.dw = l.dw_splits == 1 ? dw : nullptr, d.dw_type = p->type, d.K = l.K, d.V = (int)l.V;
+      if ((rc = launch_gemm<DW>(l.pair_dw, d, wm, tiles_of(padded, tw) * tiles_of(l.K, tw) * l.dw_splits, st)) != SPION_OK) return rc;
+      if (l.dw_splits > 1) {
+        const Join j = {prep.plan.head, nullptr, d.out, l.Kp, l.dw_splits, tw, 0, 0, 0, up(padded, tw), coef,
+                        static_cast<char*>(dw) + c * l.K * type_size(p->type), p->type, columns, l.K};
+        SPION_CUDA_TRY(launch_after(k_join, dim3((unsigned)std::min<long long>(tiles_of(columns * tiles_of(l.K, 8), 256), 8 * sm_count())), dim3(256), 0, st, j));
+      }
+    }
+    if (db != nullptr)
+      SPION_CUDA_TRY(launch_after(k_db, dim3((unsigned)tiles_of(columns, 32)), dim3(256), 0, st, (const int*)prep.plan.head, (const float*)z.colsum, l.Gp, (int)columns,
+                                  (const float*)coef, (void*)(static_cast<char*>(db) + c * type_size(db_type)), db_type));
+  }
+  if (dx != nullptr) {
+    const Join j = {prep.plan.head, prep.plan.slot, (const float*)(ws + l.dxp), l.Kp, 0, tx, (int)tiles_of(l.K, tx), dx_units, dx_chunks, 0, coef, dx, p->type, l.T, l.K};
+    SPION_CUDA_TRY(launch_after(k_join, dim3((unsigned)std::min<long long>(tiles_of(l.T * tiles_of(l.K, 8), 256), 8 * sm_count())), dim3(256), 0, st, j));
+  }
+  return SPION_OK;
+}

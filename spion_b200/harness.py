@@ -3,7 +3,7 @@
 The encoder, task heads and training loop of the reference (models/model_transformer.py,
 models/model_LRA.py, main_conv_ff.py:132-318) are not part of the accelerated path; this file
 is the thin stand-in that lets the end-to-end benchmark configs run: a 2-layer pre-LN encoder
-classifier (single or dual tower) whose attention is ``spion_b200.attention.Attention``, with
+classifier (single or dual tower; or, with ``config["objective"] = "tokens"``, a loss over its vocabulary) whose attention is ``spion_b200.attention.Attention``, with
 the reference's phase structure -- dense warm-up steps that return the per-layer mean
 attention map, pattern discovery, then sparse steps -- and data parallelism from
 ``spion_b200.dp``.
@@ -63,7 +63,16 @@ class Embeddings(nn.Module):
     def __init__(self, config):
         super().__init__()
         Embedding = nn.Embedding
-        if config.get("native") and config.get("fused_embedding_grad", True):
+        if config.get("embedding", "small") not in ("small", "table"):
+            raise ValueError(f"config['embedding'] is {config['embedding']!r}: 'small' and 'table' are served")
+        if config.get("embedding", "small") == "table":             # a vocabulary of any size, rows times config["embedding_scale"]
+            from functools import partial
+
+            from .tokens import ScaledEmbedding
+            Embedding = partial(ScaledEmbedding, scale=config.get("embedding_scale", 1.0))
+        elif config.get("embedding_scale", 1.0) != 1.0:
+            raise ValueError(f"config['embedding_scale'] is {config['embedding_scale']}: other than 1 with config['embedding'] = 'table' only")
+        elif config.get("native") and config.get("fused_embedding_grad", True):
             from .layernorm import TokenEmbedding as Embedding      # same parameter and forward; own weight gradient
         self.tok = Embedding(config["vocab_size"], config["embedding_dim"])
         self.pos = nn.Embedding(config["max_seq_len"], config["embedding_dim"])
@@ -297,6 +306,46 @@ class Classifier(nn.Module):
         return loss, maps
 
 
+class TokenModel(Classifier):
+    """The encoder trained on its own tokens: a loss over the vocabulary at the positions that have a label (others: -100), or against a teacher's largest
+    logits there.  ``config["tied_weights"]``: the last layer has the embedding's table."""
+
+    def __init__(self, config):
+        from .vocab import VocabHead
+        if config.get("dual", False):
+            raise ValueError("config['objective'] = 'tokens': one sequence at a time is served, not pairs")
+        super().__init__(config)
+        self.head = VocabHead(config["transformer_dim"], config["vocab_size"], tied=self.model.embeddings.tok if config.get("tied_weights") else None)
+
+    def token_loss(self, t, label):
+        """label: [B, L] ids, or a teacher's ([B, L, k] ids, -1: none; [B, L, k] logits) at ``config["temperature"]``"""
+        if isinstance(label, (tuple, list)):
+            return self.head.distill(t, *label, temperature=self.config.get("temperature", 1.0))
+        return self.head.loss(t, label)
+
+    def forward(self, ids, label, mat_lst=None, is_attn=False):
+        with torch.autocast(device_type="cuda", dtype=torch.bfloat16, enabled=self.amp):
+            t, maps = self.model(ids, (ids != 0).float(), mat_lst, is_attn)
+            return self.token_loss(t, label), maps
+
+    def scores(self, ids, mat_lst):
+        """What the loss is formed from, [B, L, dim]: the logits of all positions are not kept."""
+        with torch.autocast(device_type="cuda", dtype=torch.bfloat16, enabled=self.amp):
+            return self.model(ids, (ids != 0).float(), mat_lst, False)[0]
+
+
+def make_model(config):
+    """``config["objective"]``: 'class' (default) or 'tokens'."""
+    kinds = {"class": Classifier, "tokens": TokenModel}
+    if config.get("objective", "class") not in kinds:
+        raise ValueError(f"config['objective'] is {config['objective']!r}: 'class' and 'tokens' are served")
+    return kinds[config.get("objective", "class")](config)
+
+
+def _each(f, t):
+    return tuple(f(x) for x in t) if isinstance(t, (tuple, list)) else f(t)
+
+
 class Trainer:
     """dense step(s) -> discover -> sparse steps, with one flat-bucket all-reduce per step."""
 
@@ -306,7 +355,7 @@ class Trainer:
         self.config = config
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
         torch.manual_seed(seed)                      # identical initial weights on every rank
-        self.model = Classifier(config).to(self.device)
+        self.model = make_model(config).to(self.device)
         self.bucket = dp.FlatGradBucket(self.model.parameters())
         # config["optimizer"] = "fused": the library's AdamW (clipping and the copies of the parameters inside), its moments in
         # config["optimizer_state_bits"] bits
@@ -382,7 +431,7 @@ class Trainer:
         return bits == 8
 
     def evaluate(self, ids, label):
-        """Mean loss and share of right answers of one batch in the sparse phase with the weights as they are now, without gradients or dropout.
+        """Mean loss and share of right answers (None for a loss over tokens) of one batch in the sparse phase with the weights as they are now, without gradients or dropout.
         ``config["eval_linear_bits"] = 8``: with the encoder's linear layers on 8-bit operands, quantised by the call; else on none, whatever
         ``Classifier.quantize`` has left.  Synchronises, and raises if a kernel's wait gave up (``check_device_status``)."""
         if self.mat_lst is None:
@@ -393,7 +442,11 @@ class Trainer:
         try:
             with torch.no_grad(), self.model.quantized_as(eight):
                 scores = self.model.scores(ids, self.mat_lst)
-                out = nn.functional.cross_entropy(scores, label), (scores.argmax(-1) == label).float().mean()
+                if isinstance(self.model, TokenModel):
+                    with torch.autocast(device_type="cuda", dtype=torch.bfloat16, enabled=self.model.amp):
+                        out = self.model.token_loss(scores, label), None
+                else:
+                    out = nn.functional.cross_entropy(scores, label), (scores.argmax(-1) == label).float().mean()
             self.check_device_status(attention=False)
             return out
         finally:
@@ -414,9 +467,7 @@ class Trainer:
         if self.mat_lst is None:
             raise RuntimeError("capture the step after discover()")
         multi = dp.world_size() > 1
-        dual = isinstance(ids, (tuple, list))
-        self._g_ids = tuple(t.clone() for t in ids) if dual else ids.clone()
-        self._g_lab = label.clone()
+        self._g_ids, self._g_lab = _each(torch.clone, ids), _each(torch.clone, label)
         cur = torch.cuda.current_stream()
         side = torch.cuda.Stream()
         side.wait_stream(cur)
@@ -444,12 +495,10 @@ class Trainer:
 
     def step_graph(self, ids, label):
         """Replay the captured step on new inputs (copied into the graph's static buffers)."""
-        if isinstance(ids, (tuple, list)):
-            for dst, src in zip(self._g_ids, ids):
+        for to, given in ((self._g_ids, ids), (self._g_lab, label)):
+            pairs = zip(to, given) if isinstance(to, tuple) else ((to, given),)
+            for dst, src in pairs:
                 dst.copy_(src, non_blocking=True)
-        else:
-            self._g_ids.copy_(ids, non_blocking=True)
-        self._g_lab.copy_(label, non_blocking=True)
         ev = None
         if self.allreduce_events is not None:
             ev = [torch.cuda.Event(enable_timing=True) for _ in range(4)]
