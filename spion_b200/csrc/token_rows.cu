@@ -3,13 +3,17 @@
 //   y[t, :] = w[ids[t], :] scale                    dw[v, :] = scale sum_{t: ids[t] = v} g[t, :], in the order of t
 //
 //   k_lookup                 copies and scales
-//   k_digits, k_place        ids with their tokens, sorted by id: a stable radix sort, 9 bits a pass at most
-//   k_runs                   whole pieces of PIECE tokens of one id, summed (a padding token's run is thousands long)
-//   k_rows                   every row of the table: its tokens' gradients, or the sums of its whole pieces and the tokens beside them
+//   k_digits, k_place        ids with their tokens, sorted by id: a stable radix sort, 9 bits a pass at most (k_sort_one: all of it, for few ids)
+//   k_sums                   windows of the sorted order, each summed run by run: runs that lie in a window go to dw, the two that may cross its ends to partial sums; zeros for
+//                            rows of the table without a token
+//   k_join                   the runs that cross windows
 //
-// Bound by memory: g is read once, dw written once; ids, orders and partial sums are 1/16 of g or less from 64 features on.  Every sum is a function of
-// the tokens' order alone: no atomics on floating-point numbers, the same bits on every run.
+// Bound by memory: g is read once, dw written once; ids, orders and partial sums are 1/8 of g or less from 64 features on.  Windows and not rows of the table
+// are what is shared out: tokens are as unequally frequent as words are, and what a window has to load is known before the ids of its runs are looked at.  (By rows, each finding its
+// tokens by a search: 131072 ids of 32000, 1024 bf16 features 105 us, where bytes take 51.)  Every sum is a function of the tokens' order alone: no atomics on floating-point
+// numbers, the same bits on every run.
 #include <algorithm>
+#include <type_traits>
 
 #include "rows.cuh"
 
@@ -18,7 +22,6 @@ using namespace rows;
 namespace {
 
 constexpr int THREADS = 256, WARPS = 8;
-constexpr int PIECE = 64;
 constexpr int MAX_BITS = 9, MAX_BINS = 1 << MAX_BITS;
 
 // ------------------------------------------------------------------------------------------------ lookup
@@ -89,6 +92,39 @@ template <class TW, class TY, int VEC> __global__ void __launch_bounds__(THREADS
   }
 }
 
+// Sixteen features a thread where table and result have the same 16-bit type and rows on 32 bytes: whole sectors
+template <class T> __global__ void __launch_bounds__(THREADS) k_lookup_wide(const __grid_constant__ Lookup a) {
+  next_may_start();
+  wait_for_kernel_before();
+  const int groups = THREADS / a.lanes, group = threadIdx.x / a.lanes, lane = threadIdx.x - group * a.lanes;
+  const long long first = ((long long)blockIdx.x * groups + group) * LOOKUP_ROWS, c = ((long long)blockIdx.y * a.lanes + lane) * 16;
+  if (c >= a.N) return;
+  Piece<float, 8> p[LOOKUP_ROWS];                          // (32 bytes)
+#pragma unroll
+  for (int r = 0; r < LOOKUP_ROWS; ++r) {
+    const long long t = first + r, id = t < a.T ? a.ids[t] : -1;
+    if (id >= 0 && id < a.V) {
+      p[r].load(reinterpret_cast<const float*>(static_cast<const T*>(a.w) + id * a.ldw + c));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[r].w[e] = 0x7fff7fffu;
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < LOOKUP_ROWS; ++r) {
+    if (first + r >= a.T) break;
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      T v[2];
+      *reinterpret_cast<uint32_t*>(v) = p[r].w[e];
+      v[0] = rounded<T>(as_float(v[0]) * a.scale), v[1] = rounded<T>(as_float(v[1]) * a.scale);
+      f[e] = __uint_as_float(*reinterpret_cast<const uint32_t*>(v));
+    }
+    Out<float, 8>::store(reinterpret_cast<float*>(static_cast<T*>(a.y) + (first + r) * a.N + c), f);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ sort
 struct Sort {
   const long long* ids;                                    // the first pass: ids, tokens in order
@@ -114,77 +150,162 @@ __global__ void __launch_bounds__(THREADS) k_digits(const __grid_constant__ Sort
   __syncthreads();
   for (int b = threadIdx.x; b < a.bins; b += THREADS) a.counts[(long long)blockIdx.x * a.bins + b] = count[b];
 }
+// Exclusive sums over the digits of `count`, one to a thread (`bins` at most as many as threads), on top of `base`
+template <int N> __device__ __forceinline__ int scan_digits(int count, int (&shared)[32]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int sum = count;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += v;
+  }
+  if (lane == 31) shared[warp] = sum;
+  __syncthreads();
+  int before = 0;
+#pragma unroll
+  for (int w = 0; w < N; ++w) before += w < warp ? shared[w] : 0;
+  return before + sum - count;
+}
+// 32 keys of a warp, in order: where each goes; `at`: the warp's next place of each digit
+__device__ __forceinline__ int place_of(int* at, uint32_t digit, bool in) {
+  const unsigned same = __match_any_sync(0xffffffffu, in ? digit : 0xffffffffu);
+  const int rank = __popc(same & ((1u << (threadIdx.x & 31)) - 1));
+  int to = 0;
+  if (in) to = at[digit] + rank;
+  __syncwarp();
+  if (in && rank == 0) at[digit] += __popc(same);
+  __syncwarp();
+  return to;
+}
 // Where a CTA's first token of each digit goes is the sum of the counts before it (of the CTAs before it, of smaller digits); a warp takes a stretch of the CTA's
-// tokens, 32 at a time, and lanes with the same digit stay in their order.
-__global__ void __launch_bounds__(THREADS) k_place(const __grid_constant__ Sort a) {
-  __shared__ int at[WARPS][MAX_BINS], digit_first[MAX_BINS], scan[WARPS];
+// tokens, 32 at a time, and lanes with the same digit stay in their order.  Threads take four digits and a share of the CTAs each, sixteen loads under way: one digit and all CTAs
+// after another were 20 of 22 us for 64 CTAs.
+constexpr int PLACE = 512;
+__global__ void __launch_bounds__(PLACE) k_place(const __grid_constant__ Sort a) {
+  constexpr int W = PLACE / 32;
+  __shared__ int at[W][MAX_BINS], shared[32];
+  __shared__ __align__(16) int total[MAX_BINS], first_of[MAX_BINS];
   next_may_start();
   wait_for_kernel_before();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long cta_first = (long long)blockIdx.x * a.per_cta, cta_end = min(a.T, cta_first + a.per_cta);
   const long long first = min(cta_end, cta_first + (long long)warp * a.per_warp), end = min(cta_end, first + a.per_warp);
   for (int b = lane; b < a.bins; b += 32) at[warp][b] = 0;
-  __syncwarp();
-  for (long long i = first + lane; i < end; i += 32) atomicAdd(&at[warp][(key_at(a, i) >> a.shift) & (a.bins - 1)], 1);
+  for (int b = threadIdx.x; b < a.bins; b += PLACE) total[b] = first_of[b] = 0;
   __syncthreads();
-  // each thread two neighbouring digits
-  int before[2] = {0, 0}, all[2] = {0, 0};
+  for (long long i0 = first; i0 < end; i0 += 128) {
+    uint32_t key[4];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int b = 2 * threadIdx.x + e;
-    if (b >= a.bins) continue;
-    if (gridDim.x == 1) {
+    for (int u = 0; u < 4; ++u) key[u] = i0 + 32 * u + lane < end ? key_at(a, i0 + 32 * u + lane) : 0;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) all[e] += at[w][b];
-    } else {
-#pragma unroll 4
-      for (int c = 0; c < (int)gridDim.x; ++c) {
-        const int m = a.counts[(long long)c * a.bins + b];
-        all[e] += m;
-        before[e] += c < (int)blockIdx.x ? m : 0;
-      }
+    for (int u = 0; u < 4; ++u)
+      if (i0 + 32 * u + lane < end) atomicAdd(&at[warp][(key[u] >> a.shift) & (a.bins - 1)], 1);
+  }
+  const int fours = max(1, a.bins / 4), part = threadIdx.x / fours, parts = PLACE / fours, ctas = gridDim.x, each = (ctas + parts - 1) / parts;
+  if (part < parts && a.bins >= 4) {
+    int all[4] = {0, 0, 0, 0}, before[4] = {0, 0, 0, 0};
+    const int4* const counts = reinterpret_cast<const int4*>(a.counts) + (threadIdx.x - part * fours);
+#pragma unroll 16
+    for (int c = part * each; c < min(ctas, (part + 1) * each); ++c) {
+      const int4 m = counts[(long long)c * fours];
+      const int in = c < (int)blockIdx.x ? -1 : 0;
+      all[0] += m.x, all[1] += m.y, all[2] += m.z, all[3] += m.w;
+      before[0] += m.x & in, before[1] += m.y & in, before[2] += m.z & in, before[3] += m.w & in;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int b = 4 * (threadIdx.x - part * fours) + e;
+      if (all[e]) atomicAdd(&total[b], all[e]);
+      if (before[e]) atomicAdd(&first_of[b], before[e]);
+    }
+  } else if (a.bins < 4 && threadIdx.x < a.bins) {
+    for (int c = 0; c < ctas; ++c) {
+      const int m = a.counts[(long long)c * a.bins + threadIdx.x];
+      total[threadIdx.x] += m;
+      first_of[threadIdx.x] += c < (int)blockIdx.x ? m : 0;
     }
   }
-  int sum = all[0] + all[1];                               // exclusive sums over the digits
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, sum, o);
-    if (lane >= o) sum += v;
-  }
-  if (lane == 31) scan[warp] = sum;
   __syncthreads();
-  int base = sum - all[0] - all[1];
-  for (int w = 0; w < warp; ++w) base += scan[w];
+  const int b = threadIdx.x, base = scan_digits<W>(b < a.bins ? total[b] : 0, shared);
+  if (b < a.bins) {
+    int next = base + first_of[b];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int b = 2 * threadIdx.x + e;
-    if (b < a.bins) digit_first[b] = base + before[e];
-    base += all[e];
-  }
-  __syncthreads();
-  for (int b = threadIdx.x; b < a.bins; b += THREADS) {
-    int next = digit_first[b];
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
+    for (int w = 0; w < W; ++w) {
       const int m = at[w][b];
       at[w][b] = next;
       next += m;
     }
   }
   __syncthreads();
-  for (long long i0 = first; i0 < end; i0 += 32) {
-    const long long i = i0 + lane;
-    const bool in = i < end;
-    const uint32_t key = in ? key_at(a, i) : 0, digit = (key >> a.shift) & (a.bins - 1);
-    const uint32_t token = in ? (a.ids != nullptr ? (uint32_t)i : a.token[i]) : 0;
-    const unsigned same = __match_any_sync(0xffffffffu, in ? digit : 0xffffffffu);
-    const int rank = __popc(same & ((1u << lane) - 1));
-    int to = 0;
-    if (in) to = at[warp][digit] + rank;
+  for (long long i0 = first; i0 < end; i0 += 128) {
+    uint32_t key[4], token[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long long i = i0 + 32 * u + lane;
+      key[u] = i < end ? key_at(a, i) : 0;
+      token[u] = i < end ? (a.ids != nullptr ? (uint32_t)i : a.token[i]) : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (i0 + 32 * u >= end) break;
+      const bool in = i0 + 32 * u + lane < end;
+      const int to = place_of(at[warp], (key[u] >> a.shift) & (a.bins - 1), in);
+      if (in) a.key_out[to] = key[u], a.token_out[to] = token[u];
+    }
+  }
+}
+// All passes by one CTA, keys and tokens in shared memory: one launch instead of four for few ids (4099 of 10007: 8.9 us, 24)
+constexpr int ONE = 1024, ONE_MAX = 8192;
+constexpr uint32_t ONE_SMEM = 4 * ONE_MAX * 4 + 32 * MAX_BINS * 4;
+__global__ void __launch_bounds__(ONE) k_sort_one(const __grid_constant__ Sort a, int bits, int passes) {
+  extern __shared__ __align__(16) uint32_t smem[];
+  __shared__ int shared[32];
+  int* const at0 = reinterpret_cast<int*>(smem + 4 * ONE_MAX);
+  next_may_start();
+  wait_for_kernel_before();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, T = (int)a.T, bins = 1 << bits;
+  const int first = min(T, warp * a.per_warp), end = min(T, first + a.per_warp);
+  int* const at = at0 + warp * MAX_BINS;
+  uint32_t key[8], token[8];
+  for (int pass = 0; pass < passes; ++pass) {
+    const uint32_t *const kin = smem + (pass & 1) * ONE_MAX, *const tin = kin + 2 * ONE_MAX;
+    uint32_t *const kout = smem + ((pass + 1) & 1) * ONE_MAX, *const tout = kout + 2 * ONE_MAX;
+    for (int b = lane; b < bins; b += 32) at[b] = 0;
     __syncwarp();
-    if (in && rank == 0) at[warp][digit] += __popc(same);
-    __syncwarp();
-    if (in) a.key_out[to] = key, a.token_out[to] = token;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int i = first + 32 * u + lane;
+      if (i >= end) continue;
+      key[u] = pass == 0 ? key_at(a, i) : kin[i];
+      token[u] = pass == 0 ? (uint32_t)i : tin[i];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (first + 32 * u + lane < end) atomicAdd(&at[(key[u] >> (pass * bits)) & (bins - 1)], 1);
+    __syncthreads();
+    const int b = threadIdx.x;
+    int count = 0;
+    if (b < bins)
+      for (int w = 0; w < 32; ++w) count += at0[w * MAX_BINS + b];
+    int next = scan_digits<32>(count, shared);
+    if (b < bins)
+      for (int w = 0; w < 32; ++w) {
+        const int m = at0[w * MAX_BINS + b];
+        at0[w * MAX_BINS + b] = next;
+        next += m;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (first + 32 * u >= end) break;
+      const bool in = first + 32 * u + lane < end;
+      const int to = place_of(at, (key[u] >> (pass * bits)) & (bins - 1), in);
+      if (in) {
+        if (pass == passes - 1) a.key_out[to] = key[u], a.token_out[to] = token[u];
+        else kout[to] = key[u], tout[to] = token[u];
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -192,65 +313,34 @@ __global__ void __launch_bounds__(THREADS) k_place(const __grid_constant__ Sort 
 struct Sums {
   const uint32_t *key, *token;                             // sorted
   const void* g; long long ldg;
-  float* part;                                             // [pieces][N]
+  float* part;                                             // [windows][2][N]: of the run that a window begins in the middle of; of the one that it ends in the middle of
   void* dw;
   float scale;
   long long T, V, N;
-  int lanes, rows;                                         // rows of the table a CTA
+  int lanes, window;                                       // threads to a chunk of a row; tokens of a window
+  long long windows;
+  unsigned sum_ctas;                                       // CTAs of windows, before those of zeros
 };
-__device__ __forceinline__ void add8(float (&s)[8], const float (&f)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) s[e] += f[e];
-}
-// s += the rows of tokens i0 .. i1 - 1 of the sorted order: four loads under way, added one after another
-template <class TG, int VEC> __device__ __forceinline__ void add_tokens(const Sums& a, long long i0, long long i1, int chunk, int lane, float (&s)[8]) {
-  long long i = i0;
-  for (; i + 4 <= i1; i += 4) {
-    float f[4][8];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) load8<TG, VEC>(static_cast<const TG*>(a.g) + (long long)a.token[i + u] * a.ldg, chunk, lane, a.lanes, a.N, f[u]);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) add8(s, f[u]);
+template <class T, int VEC> struct Raw8 {                  // eight elements as they lie in memory
+  Piece<T, 8> p;
+  __device__ __forceinline__ void load(const T* row, int chunk, int lane, int lanes, long long N) {
+    const long long c = column<8>(chunk, lane, lanes, 0);
+    if (c < N) p.load(row + c);
+    else p.zero();
   }
-  for (; i < i1; ++i) {
-    float f[8];
-    load8<TG, VEC>(static_cast<const TG*>(a.g) + (long long)a.token[i] * a.ldg, chunk, lane, a.lanes, a.N, f);
-    add8(s, f);
-  }
-}
-template <int VEC> __device__ __forceinline__ void add_parts(const Sums& a, long long j0, long long j1, int chunk, int lane, float (&s)[8]) {
-#pragma unroll 4
-  for (long long j = j0; j < j1; ++j) {
-    float f[8];
-    load8<float, VEC>(a.part + j * a.N, chunk, lane, a.lanes, a.N, f);
-    add8(s, f);
-  }
-}
-// The groups' sums, added in their order by the first group
-__device__ __forceinline__ void join_groups(float (*shared)[8], int groups, int group, int lane, int lanes, float (&s)[8]) {
+  __device__ __forceinline__ float at(int e) const { return p.at(e); }
+};
+template <class T> struct Raw8<T, 1> {
+  T v[8];
+  __device__ __forceinline__ void load(const T* row, int chunk, int lane, int lanes, long long N) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) shared[threadIdx.x][e] = s[e];
-  __syncthreads();
-  if (group == 0)
-    for (int k = 1; k < groups; ++k)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] += shared[k * lanes + lane][e];
-  __syncthreads();
-}
-template <class TG, int VEC> __global__ void __launch_bounds__(THREADS) k_runs(const __grid_constant__ Sums a) {
-  __shared__ float shared[THREADS][8];
-  next_may_start();
-  wait_for_kernel_before();
-  const long long first = (long long)blockIdx.x * PIECE;
-  const uint32_t key = a.key[first];
-  if (key >= a.V || a.key[first + PIECE - 1] != key) return;
-  const int groups = THREADS / a.lanes, group = threadIdx.x / a.lanes, lane = threadIdx.x - group * a.lanes, chunk = blockIdx.y;
-  const int each = (PIECE + groups - 1) / groups, i0 = min(PIECE, group * each), i1 = min(PIECE, i0 + each);
-  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  add_tokens<TG, VEC>(a, first + i0, first + i1, chunk, lane, s);
-  join_groups(shared, groups, group, lane, a.lanes, s);
-  if (group == 0) store8<float, VEC>(a.part + (long long)blockIdx.x * a.N, chunk, lane, a.lanes, a.N, s);
-}
+    for (int e = 0; e < 8; ++e) {
+      const long long c = column<1>(chunk, lane, lanes, e);
+      v[e] = c < N ? row[c] : rounded<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ float at(int e) const { return as_float(v[e]); }
+};
 // the first place in the order whose key is v or more
 __device__ __forceinline__ long long lower_bound(const uint32_t* key, long long T, long long v) {
   long long lo = 0, hi = T;
@@ -261,43 +351,140 @@ __device__ __forceinline__ long long lower_bound(const uint32_t* key, long long 
   }
   return lo;
 }
-constexpr int FEW = 32;                                    // tokens that one group adds
-template <class TG, class TD, int VEC> __global__ void __launch_bounds__(THREADS) k_rows(const __grid_constant__ Sums a) {
-  __shared__ float shared[THREADS][8];
-  __shared__ long long start[THREADS + 1];
+constexpr int ZERO_ROWS = 64, DEEP = 8;                    // rows of the table that a CTA looks for tokens of; rows of g under way
+template <class TG, class TD, int VEC> __global__ void __launch_bounds__(THREADS) k_sums(const __grid_constant__ Sums a) {
   next_may_start();
   wait_for_kernel_before();
-  const long long v0 = (long long)blockIdx.x * a.rows;
-  const int rows_here = (int)min((long long)a.rows, a.V - v0);
-  for (int r = threadIdx.x; r <= rows_here; r += THREADS) start[r] = lower_bound(a.key, a.T, v0 + r);
-  __syncthreads();
   const int groups = THREADS / a.lanes, group = threadIdx.x / a.lanes, lane = threadIdx.x - group * a.lanes, chunk = blockIdx.y;
   TD* const dw = static_cast<TD*>(a.dw);
-  for (int r = group; r < rows_here; r += groups) {
-    const long long i0 = start[r], i1 = start[r + 1];
-    if (i1 - i0 > FEW) continue;
-    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    add_tokens<TG, VEC>(a, i0, i1, chunk, lane, s);
+  if (blockIdx.x >= a.sum_ctas) {                          // rows without a token
+    __shared__ long long start[ZERO_ROWS + 1];
+    const long long v0 = (long long)(blockIdx.x - a.sum_ctas) * ZERO_ROWS;
+    const int rows_here = (int)min((long long)ZERO_ROWS, a.V - v0);
+    if ((int)threadIdx.x <= rows_here) start[threadIdx.x] = lower_bound(a.key, a.T, v0 + threadIdx.x);
+    __syncthreads();
+    const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int r = group; r < rows_here; r += groups)
+      if (start[r] == start[r + 1]) store8<TD, VEC>(dw + (v0 + r) * a.N, chunk, lane, a.lanes, a.N, zero);
+    return;
+  }
+  const long long w = (long long)blockIdx.x * groups + group;
+  if (w >= a.windows) return;
+  const long long i0 = w * a.window, i1 = min(a.T, i0 + a.window);
+  uint32_t run = a.key[i0];
+  if (run >= a.V) return;                                  // from here on all are without a gradient
+  bool begun = i0 > 0 && a.key[i0 - 1] == run;             // the run began before this window
+  const bool goes_on = i1 < a.T && a.key[i1] == a.key[i1 - 1];
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto put = [&](bool crosses) {
+    if (run < a.V) {
+      if (begun || crosses) {
+        store8<float, VEC>(a.part + (2 * w + !begun) * a.N, chunk, lane, a.lanes, a.N, s);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] *= a.scale;
+        store8<TD, VEC>(dw + (long long)run * a.N, chunk, lane, a.lanes, a.N, s);
+      }
+    }
+    begun = false;
+  };
+  // No load waits behind a branch: the last token again where a window ends, rows without a gradient too where one begins; ids and tokens a step ahead.
+  uint32_t key[DEEP], token[DEEP];
+#pragma unroll
+  for (int u = 0; u < DEEP; ++u) key[u] = a.key[min(i0 + u, i1 - 1)], token[u] = a.token[min(i0 + u, i1 - 1)];
+  for (long long i = i0; i < i1; i += DEEP) {
+    Raw8<TG, VEC> g[DEEP];
+    uint32_t now[DEEP];
+#pragma unroll
+    for (int u = 0; u < DEEP; ++u) {
+      g[u].load(static_cast<const TG*>(a.g) + (long long)token[u] * a.ldg, chunk, lane, a.lanes, a.N);
+      now[u] = key[u];
+    }
+#pragma unroll
+    for (int u = 0; u < DEEP; ++u) {
+      const long long next = min(i + DEEP + u, i1 - 1);
+      key[u] = a.key[next], token[u] = a.token[next];
+    }
+#pragma unroll
+    for (int u = 0; u < DEEP; ++u) {
+      if (i + u >= i1) break;
+      if (now[u] != run) {
+        put(false);
+        run = now[u];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += g[u].at(e);
+    }
+  }
+  put(goes_on);
+}
+// A group looks at a window: where a run begins in it and goes on, it adds the run's partial sums, or, of many, all groups of the CTA do, a share each.
+constexpr int FEW = 16;
+template <class TD, int VEC> __global__ void __launch_bounds__(THREADS) k_join(const __grid_constant__ Sums a) {
+  __shared__ float shared[THREADS][8];
+  __shared__ long long many[THREADS];                      // per group: windows of a long run, or 0
+  next_may_start();
+  wait_for_kernel_before();
+  const int groups = THREADS / a.lanes, group = threadIdx.x / a.lanes, lane = threadIdx.x - group * a.lanes, chunk = blockIdx.y;
+  TD* const dw = static_cast<TD*>(a.dw);
+  const long long w0 = (long long)blockIdx.x * groups, w = w0 + group;
+  auto add = [&](long long from, long long to, float (&s)[8]) {      // the first sums of windows from .. to - 1
+#pragma unroll 8
+    for (long long j = from; j < to; ++j) {
+      float f[8];
+      load8<float, VEC>(a.part + 2 * j * a.N, chunk, lane, a.lanes, a.N, f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += f[e];
+    }
+  };
+  // windows after w0 + k that the run that begins in window w0 + k and goes on is part of; 0: there is none
+  auto run_of = [&](long long w, uint32_t& run) -> long long {
+    const long long i0 = w * a.window, i1 = i0 + a.window;
+    if (w >= a.windows || i1 >= a.T) return 0;
+    run = a.key[i1 - 1];
+    if (run >= a.V || a.key[i1] != run || (i0 > 0 && a.key[i0 - 1] == run)) return 0;
+    long long lo = 1, hi = a.windows - w;                  // windows of the run: those that begin with its id
+    if (w + FEW + 1 >= a.windows || a.key[(w + FEW + 1) * a.window] != run) hi = min(hi, (long long)FEW + 1);
+    while (lo < hi) {
+      const long long mid = (lo + hi) >> 1;
+      if (a.key[(w + mid) * a.window] == run) lo = mid + 1;
+      else hi = mid;
+    }
+    return lo - 1;
+  };
+  uint32_t run = 0;
+  const long long more = run_of(w, run);
+  if (lane == 0) many[group] = more > FEW ? more : 0;
+  if (more > 0 && more <= FEW) {
+    float s[8];
+    load8<float, VEC>(a.part + (2 * w + 1) * a.N, chunk, lane, a.lanes, a.N, s);
+    add(w + 1, w + 1 + more, s);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[e] *= a.scale;
-    store8<TD, VEC>(dw + (v0 + r) * a.N, chunk, lane, a.lanes, a.N, s);
+    store8<TD, VEC>(dw + (long long)run * a.N, chunk, lane, a.lanes, a.N, s);
   }
-  for (int r = 0; r < rows_here; ++r) {                    // the others by all groups
-    const long long i0 = start[r], i1 = start[r + 1];
-    if (i1 - i0 <= FEW) continue;
-    const long long p0 = (i0 + PIECE - 1) / PIECE, p1 = max(p0, i1 / PIECE);      // whole pieces
-    const long long head = min(i1, p0 * PIECE) - i0, parts = p1 - p0, tail0 = min(i1, p1 * PIECE), all = head + parts + (i1 - tail0);
-    const long long each = (all + groups - 1) / groups, m0 = min(all, group * each), m1 = min(all, m0 + each);
+  __syncthreads();
+  for (int k = 0; k < groups; ++k) {
+    const long long all = many[k];
+    if (all == 0) continue;
+    const long long each = (all + groups - 1) / groups, j0 = min(all, group * each), j1 = min(all, j0 + each);
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (m0 < head) add_tokens<TG, VEC>(a, i0 + m0, i0 + min(m1, head), chunk, lane, s);
-    if (m1 > head && m0 < head + parts) add_parts<VEC>(a, p0 + max(m0 - head, 0ll), p0 + min(m1 - head, parts), chunk, lane, s);
-    if (m1 > head + parts) add_tokens<TG, VEC>(a, tail0 + max(m0 - head - parts, 0ll), tail0 + (m1 - head - parts), chunk, lane, s);
-    join_groups(shared, groups, group, lane, a.lanes, s);
+    if (group == 0) load8<float, VEC>(a.part + (2 * (w0 + k) + 1) * a.N, chunk, lane, a.lanes, a.N, s);
+    add(w0 + k + 1 + j0, w0 + k + 1 + j1, s);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) shared[threadIdx.x][e] = s[e];
+    __syncthreads();
     if (group == 0) {
+      for (int o = 1; o < groups; ++o)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += shared[o * a.lanes + lane][e];
 #pragma unroll
       for (int e = 0; e < 8; ++e) s[e] *= a.scale;
-      store8<TD, VEC>(dw + (v0 + r) * a.N, chunk, lane, a.lanes, a.N, s);
+      store8<TD, VEC>(dw + (long long)a.key[(w0 + k + 1) * a.window] * a.N, chunk, lane, a.lanes, a.N, s);
     }
+    __syncthreads();
   }
 }
 
@@ -314,20 +501,26 @@ int lanes_of(long long N) {
   return 32;
 }
 struct Sizes {
-  long long per_cta, ctas, pieces;
+  long long per_cta, ctas, window, windows;
   int passes, bits;
+  bool one;                                                // the sort by one CTA
   size_t key[2], token[2], counts, part, all;
 };
 Sizes sizes_of(long long T, long long V, long long N) {
   Sizes s = {};
+  s.one = T <= ONE_MAX;
   // counts of all CTAs before it are read by every CTA: 128 of them at most
-  s.per_cta = std::max(2048ll, ((T + 127) / 128 + 255) / 256 * 256);
+  s.per_cta = s.one ? (T + 1023) / 1024 * 1024 : std::max(2048ll, ((T + 127) / 128 + PLACE - 1) / PLACE * PLACE);
   s.ctas = (T + s.per_cta - 1) / s.per_cta;
   int bits = 1;
   while (V >> bits) ++bits;                                // keys 0 .. V
   s.passes = (bits + MAX_BITS - 1) / MAX_BITS;
   s.bits = (bits + s.passes - 1) / s.passes;
-  s.pieces = T / PIECE;
+  // Windows of 64 tokens where that leaves 16 warps to every multiprocessor, down to 16 where it does not.
+  const long long chunks = (N + 255) / 256;
+  s.window = 64;
+  while (s.window > 16 && (T + s.window - 1) / s.window * chunks < 148 * 16) s.window /= 2;
+  s.windows = (T + s.window - 1) / s.window;
   size_t at = 0;
   auto take = [&](long long bytes) {
     const size_t here = at;
@@ -336,24 +529,37 @@ Sizes sizes_of(long long T, long long V, long long N) {
   };
   for (int i = 0; i < 2; ++i) s.key[i] = take(4 * T), s.token[i] = take(4 * T);
   s.counts = take(4 * s.ctas * (1ll << s.bits));
-  s.part = take(4 * s.pieces * N);
+  s.part = take(s.windows > 1 ? 8 * s.windows * N : 0);
   s.all = at;
   return s;
 }
 bool sizes_ok(long long T, long long V, long long N) { return T <= 0x7fffffff - 4096 && V <= 0x7fffffff - 4096 && N <= 0x7fffffff / 4; }
 
-template <class TG, int VEC> int launch_sums(const Sums& a, const Sizes& s, int dw_type, cudaStream_t st) {
+template <class TG, class TD, int VEC> int launch_sums(const Sums& a, cudaStream_t st) {
   const unsigned chunks = (unsigned)((a.N + a.lanes * 8 - 1) / (a.lanes * 8));
-  if (s.pieces > 0) SPION_CUDA_TRY(launch_after(k_runs<TG, VEC>, dim3((unsigned)s.pieces, chunks), dim3(THREADS), 0, st, a));
-  const dim3 grid((unsigned)((a.V + a.rows - 1) / a.rows), chunks);
-  if (dw_type == SPION_F32) SPION_CUDA_TRY(launch_after(k_rows<TG, float, VEC>, grid, dim3(THREADS), 0, st, a));
-  else if (dw_type == SPION_BF16) SPION_CUDA_TRY(launch_after(k_rows<TG, __nv_bfloat16, VEC>, grid, dim3(THREADS), 0, st, a));
-  else SPION_CUDA_TRY(launch_after(k_rows<TG, __half, VEC>, grid, dim3(THREADS), 0, st, a));
+  const unsigned zero_ctas = (unsigned)((a.V + ZERO_ROWS - 1) / ZERO_ROWS);
+  SPION_CUDA_TRY(launch_after(k_sums<TG, TD, VEC>, dim3(a.sum_ctas + zero_ctas, chunks), dim3(THREADS), 0, st, a));
+  if (a.windows > 1) SPION_CUDA_TRY(launch_after(k_join<TD, VEC>, dim3(a.sum_ctas, chunks), dim3(THREADS), 0, st, a));
   return SPION_OK;
+}
+template <class TG, int VEC> int launch_sums(const Sums& a, int dw_type, cudaStream_t st) {
+  if (dw_type == SPION_F32) return launch_sums<TG, float, VEC>(a, st);
+  if (dw_type == SPION_BF16) return launch_sums<TG, __nv_bfloat16, VEC>(a, st);
+  return launch_sums<TG, __half, VEC>(a, st);
 }
 template <class TW, class TY> int launch_lookup(const Lookup& a, bool eight, cudaStream_t st) {
   const int rows_ = THREADS / a.lanes * LOOKUP_ROWS;
   const dim3 grid((unsigned)((a.T + rows_ - 1) / rows_), (unsigned)((a.N + a.lanes * 8 - 1) / (a.lanes * 8)));
+  if constexpr (std::is_same<TW, TY>::value && sizeof(TW) == 2) {
+    if (eight && a.N % 16 == 0 && ((uintptr_t)a.w | (uintptr_t)a.y | (uintptr_t)(a.ldw * 2)) % 32 == 0) {
+      Lookup b = a;
+      while (b.lanes > 4 && 8 * b.lanes >= a.N) b.lanes /= 2;
+      const int rows_16 = THREADS / b.lanes * LOOKUP_ROWS;
+      const dim3 grid16((unsigned)((a.T + rows_16 - 1) / rows_16), (unsigned)((a.N + b.lanes * 16 - 1) / (b.lanes * 16)));
+      SPION_CUDA_TRY(launch_after(k_lookup_wide<TW>, grid16, dim3(THREADS), 0, st, b));
+      return SPION_OK;
+    }
+  }
   if (eight) SPION_CUDA_TRY(launch_after(k_lookup<TW, TY, 8>, grid, dim3(THREADS), 0, st, a));
   else SPION_CUDA_TRY(launch_after(k_lookup<TW, TY, 1>, grid, dim3(THREADS), 0, st, a));
   return SPION_OK;
@@ -400,17 +606,30 @@ extern "C" int spion_token_rows_backward(const long long* ids, const void* g, lo
   char* const ws = static_cast<char*>(workspace);
   uint32_t* const key[2] = {(uint32_t*)(ws + s.key[0]), (uint32_t*)(ws + s.key[1])};
   uint32_t* const token[2] = {(uint32_t*)(ws + s.token[0]), (uint32_t*)(ws + s.token[1])};
-  for (int pass = 0; pass < s.passes; ++pass) {
-    const int in = (pass + 1) & 1, out = pass & 1;
-    const Sort a = {pass == 0 ? ids : nullptr, key[in], token[in], key[out], token[out], (int*)(ws + s.counts), T, V, padding_idx, (int)s.per_cta,
-                    (int)s.per_cta / WARPS, pass * s.bits, 1 << s.bits};
-    if (s.ctas > 1) SPION_CUDA_TRY(launch_after(k_digits, dim3((unsigned)s.ctas), dim3(THREADS), 0, st, a));
-    SPION_CUDA_TRY(launch_after(k_place, dim3((unsigned)s.ctas), dim3(THREADS), 0, st, a));
+  const int last = s.one ? 0 : (s.passes - 1) & 1, lanes = lanes_of(N);
+  if (s.one) {
+    static std::atomic<uint64_t> ready{0};                  // once per device
+    int dev = 0;
+    SPION_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev >= 64 || !(ready.load() >> dev & 1)) {
+      SPION_CUDA_TRY(cudaFuncSetAttribute(k_sort_one, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ONE_SMEM));
+      if (dev < 64) ready.fetch_or(1ull << dev);
+    }
+    const Sort a = {ids, nullptr, nullptr, key[0], token[0], nullptr, T, V, padding_idx, (int)s.per_cta, (int)s.per_cta / 32, 0, 0};
+    SPION_CUDA_TRY(launch_after(k_sort_one, dim3(1), dim3(ONE), ONE_SMEM, st, a, s.bits, s.passes));
+  } else {
+    for (int pass = 0; pass < s.passes; ++pass) {
+      const int in = (pass + 1) & 1, out = pass & 1;
+      const Sort a = {pass == 0 ? ids : nullptr, key[in], token[in], key[out], token[out], (int*)(ws + s.counts), T, V, padding_idx, (int)s.per_cta,
+                      (int)s.per_cta / (PLACE / 32), pass * s.bits, 1 << s.bits};
+      SPION_CUDA_TRY(launch_after(k_digits, dim3((unsigned)s.ctas), dim3(THREADS), 0, st, a));
+      SPION_CUDA_TRY(launch_after(k_place, dim3((unsigned)s.ctas), dim3(PLACE), 0, st, a));
+    }
   }
-  const int last = (s.passes - 1) & 1, lanes = lanes_of(N);
-  const Sums a = {key[last], token[last], g, ldg, (float*)(ws + s.part), dw, scale, T, V, N, lanes, THREADS / lanes * 4};
+  const int groups = THREADS / lanes;
+  const Sums a = {key[last], token[last], g, ldg, (float*)(ws + s.part), dw, scale, T, V, N, lanes, (int)s.window, s.windows, (unsigned)((s.windows + groups - 1) / groups)};
   const bool eight = eights(g, ldg, N, g_type) && eights(dw, N, N, dw_type);
-  if (g_type == SPION_F32) return eight ? launch_sums<float, 8>(a, s, dw_type, st) : launch_sums<float, 1>(a, s, dw_type, st);
-  if (g_type == SPION_BF16) return eight ? launch_sums<__nv_bfloat16, 8>(a, s, dw_type, st) : launch_sums<__nv_bfloat16, 1>(a, s, dw_type, st);
-  return eight ? launch_sums<__half, 8>(a, s, dw_type, st) : launch_sums<__half, 1>(a, s, dw_type, st);
+  if (g_type == SPION_F32) return eight ? launch_sums<float, 8>(a, dw_type, st) : launch_sums<float, 1>(a, dw_type, st);
+  if (g_type == SPION_BF16) return eight ? launch_sums<__nv_bfloat16, 8>(a, dw_type, st) : launch_sums<__nv_bfloat16, 1>(a, dw_type, st);
+  return eight ? launch_sums<__half, 8>(a, dw_type, st) : launch_sums<__half, 1>(a, dw_type, st);
 }
