@@ -21,7 +21,7 @@ using namespace rows;
 
 namespace {
 
-constexpr int THREADS = 256, WARPS = 8;
+constexpr int THREADS = 256;
 constexpr int MAX_BITS = 9, MAX_BINS = 1 << MAX_BITS;
 
 // ------------------------------------------------------------------------------------------------ lookup
@@ -319,7 +319,7 @@ struct Sums {
   long long T, V, N;
   int lanes, window;                                       // threads to a chunk of a row; tokens of a window
   long long windows;
-  unsigned sum_ctas;                                       // CTAs of windows, before those of zeros
+  unsigned sum_ctas, chunks;                               // CTAs of windows, before those of zeros; chunks of a row
 };
 template <class T, int VEC> struct Raw8 {                  // eight elements as they lie in memory
   Piece<T, 8> p;
@@ -351,58 +351,79 @@ __device__ __forceinline__ long long lower_bound(const uint32_t* key, long long 
   }
   return lo;
 }
-constexpr int ZERO_ROWS = 64, DEEP = 8;                    // rows of the table that a CTA looks for tokens of; rows of g under way
-template <class TG, class TD, int VEC> __global__ void __launch_bounds__(THREADS) k_sums(const __grid_constant__ Sums a) {
+constexpr int ZERO_ROWS = 64;                              // rows of the table that a CTA looks for tokens of
+// Rows of g under way: more of them cost more registers than they hide (131072 x 1024 bf16: 4 71 us, 8 88, 16 144, where 96 and 154 registers leave half of the warps)
+constexpr int DEEP = 4;
+// P: pieces of eight features a thread
+template <class TG, class TD, int VEC, int P> __global__ void __launch_bounds__(THREADS) k_sums(const __grid_constant__ Sums a) {
   next_may_start();
   wait_for_kernel_before();
-  const int groups = THREADS / a.lanes, group = threadIdx.x / a.lanes, lane = threadIdx.x - group * a.lanes, chunk = blockIdx.y;
+  const int groups = THREADS / a.lanes, group = threadIdx.x / a.lanes, lane = threadIdx.x - group * a.lanes;
   TD* const dw = static_cast<TD*>(a.dw);
-  if (blockIdx.x >= a.sum_ctas) {                          // rows without a token
-    __shared__ long long start[ZERO_ROWS + 1];
-    const long long v0 = (long long)(blockIdx.x - a.sum_ctas) * ZERO_ROWS;
+  // windows first, the chunks of their rows side by side
+  const unsigned sums = a.sum_ctas * a.chunks, at = blockIdx.x - (blockIdx.x >= sums ? sums : 0), cta = at / a.chunks;
+  const int chunk = (int)(at - cta * a.chunks) * P;
+  if (blockIdx.x >= sums) {                                // rows without a token
+    __shared__ int start[ZERO_ROWS + 1];
+    const long long v0 = (long long)cta * ZERO_ROWS;
     const int rows_here = (int)min((long long)ZERO_ROWS, a.V - v0);
-    if ((int)threadIdx.x <= rows_here) start[threadIdx.x] = lower_bound(a.key, a.T, v0 + threadIdx.x);
+    if ((int)threadIdx.x <= rows_here) start[threadIdx.x] = (int)lower_bound(a.key, a.T, v0 + threadIdx.x);
     __syncthreads();
     const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int r = group; r < rows_here; r += groups)
-      if (start[r] == start[r + 1]) store8<TD, VEC>(dw + (v0 + r) * a.N, chunk, lane, a.lanes, a.N, zero);
+      if (start[r] == start[r + 1])
+#pragma unroll
+        for (int p = 0; p < P; ++p) store8<TD, VEC>(dw + (v0 + r) * a.N, chunk + p, lane, a.lanes, a.N, zero);
     return;
   }
-  const long long w = (long long)blockIdx.x * groups + group;
+  const long long w = (long long)cta * groups + group;
   if (w >= a.windows) return;
-  const long long i0 = w * a.window, i1 = min(a.T, i0 + a.window);
+  const int i0 = (int)(w * a.window), i1 = (int)min(a.T, (long long)i0 + a.window);
+  const uint32_t none = (uint32_t)a.V;
   uint32_t run = a.key[i0];
-  if (run >= a.V) return;                                  // from here on all are without a gradient
+  if (run >= none) return;                                 // from here on all are without a gradient
   bool begun = i0 > 0 && a.key[i0 - 1] == run;             // the run began before this window
   const bool goes_on = i1 < a.T && a.key[i1] == a.key[i1 - 1];
-  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  auto put = [&](bool crosses) {
-    if (run < a.V) {
-      if (begun || crosses) {
-        store8<float, VEC>(a.part + (2 * w + !begun) * a.N, chunk, lane, a.lanes, a.N, s);
-      } else {
+  float s[P][8];
+  auto clear = [&] {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] *= a.scale;
-        store8<TD, VEC>(dw + (long long)run * a.N, chunk, lane, a.lanes, a.N, s);
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[p][e] = 0.f;
+  };
+  auto put = [&](bool crosses) {
+    if (run < none) {
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        if (begun || crosses) {
+          store8<float, VEC>(a.part + (2 * w + !begun) * a.N, chunk + p, lane, a.lanes, a.N, s[p]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[p][e] *= a.scale;
+          store8<TD, VEC>(dw + (long long)run * a.N, chunk + p, lane, a.lanes, a.N, s[p]);
+        }
       }
     }
     begun = false;
   };
+  clear();
   // No load waits behind a branch: the last token again where a window ends, rows without a gradient too where one begins; ids and tokens a step ahead.
   uint32_t key[DEEP], token[DEEP];
 #pragma unroll
   for (int u = 0; u < DEEP; ++u) key[u] = a.key[min(i0 + u, i1 - 1)], token[u] = a.token[min(i0 + u, i1 - 1)];
-  for (long long i = i0; i < i1; i += DEEP) {
-    Raw8<TG, VEC> g[DEEP];
+  for (int i = i0; i < i1; i += DEEP) {
+    Raw8<TG, VEC> g[DEEP][P];
     uint32_t now[DEEP];
 #pragma unroll
     for (int u = 0; u < DEEP; ++u) {
-      g[u].load(static_cast<const TG*>(a.g) + (long long)token[u] * a.ldg, chunk, lane, a.lanes, a.N);
+      const TG* const row = static_cast<const TG*>(a.g) + (long long)token[u] * a.ldg;
+#pragma unroll
+      for (int p = 0; p < P; ++p) g[u][p].load(row, chunk + p, lane, a.lanes, a.N);
       now[u] = key[u];
     }
 #pragma unroll
     for (int u = 0; u < DEEP; ++u) {
-      const long long next = min(i + DEEP + u, i1 - 1);
+      const int next = min(i + DEEP + u, i1 - 1);
       key[u] = a.key[next], token[u] = a.token[next];
     }
 #pragma unroll
@@ -411,11 +432,12 @@ template <class TG, class TD, int VEC> __global__ void __launch_bounds__(THREADS
       if (now[u] != run) {
         put(false);
         run = now[u];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = 0.f;
+        clear();
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] += g[u].at(e);
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[p][e] += g[u][p].at(e);
     }
   }
   put(goes_on);
@@ -441,12 +463,13 @@ template <class TD, int VEC> __global__ void __launch_bounds__(THREADS) k_join(c
   };
   // windows after w0 + k that the run that begins in window w0 + k and goes on is part of; 0: there is none
   auto run_of = [&](long long w, uint32_t& run) -> long long {
-    const long long i0 = w * a.window, i1 = i0 + a.window;
+    const long long i0 = w * a.window, i1 = i0 + a.window, far = (w + FEW + 1) * a.window;
     if (w >= a.windows || i1 >= a.T) return 0;
-    run = a.key[i1 - 1];
-    if (run >= a.V || a.key[i1] != run || (i0 > 0 && a.key[i0 - 1] == run)) return 0;
+    run = a.key[i1 - 1];                                   // (all of the keys at once)
+    const uint32_t next = a.key[i1], before = a.key[max(i0 - 1, 0ll)], far_key = a.key[min(far, a.T - 1)];
+    if (run >= a.V || next != run || (i0 > 0 && before == run)) return 0;
     long long lo = 1, hi = a.windows - w;                  // windows of the run: those that begin with its id
-    if (w + FEW + 1 >= a.windows || a.key[(w + FEW + 1) * a.window] != run) hi = min(hi, (long long)FEW + 1);
+    if (far >= a.T || far_key != run) hi = min(hi, (long long)FEW + 1);
     while (lo < hi) {
       const long long mid = (lo + hi) >> 1;
       if (a.key[(w + mid) * a.window] == run) lo = mid + 1;
@@ -536,10 +559,15 @@ Sizes sizes_of(long long T, long long V, long long N) {
 bool sizes_ok(long long T, long long V, long long N) { return T <= 0x7fffffff - 4096 && V <= 0x7fffffff - 4096 && N <= 0x7fffffff / 4; }
 
 template <class TG, class TD, int VEC> int launch_sums(const Sums& a, cudaStream_t st) {
-  const unsigned chunks = (unsigned)((a.N + a.lanes * 8 - 1) / (a.lanes * 8));
-  const unsigned zero_ctas = (unsigned)((a.V + ZERO_ROWS - 1) / ZERO_ROWS);
-  SPION_CUDA_TRY(launch_after(k_sums<TG, TD, VEC>, dim3(a.sum_ctas + zero_ctas, chunks), dim3(THREADS), 0, st, a));
-  if (a.windows > 1) SPION_CUDA_TRY(launch_after(k_join<TD, VEC>, dim3(a.sum_ctas, chunks), dim3(THREADS), 0, st, a));
+  constexpr int P = VEC == 8 ? 2 : 1;
+  const bool two = P == 2 && a.N > 256;
+  Sums b = a;
+  if (two) b.chunks = (a.chunks + 1) / 2;
+  const long long ctas = ((b.V + ZERO_ROWS - 1) / ZERO_ROWS + b.sum_ctas) * b.chunks;
+  if (ctas > 0x7fffffff) return SPION_ERR_SHAPE;
+  if (two) SPION_CUDA_TRY(launch_after(k_sums<TG, TD, VEC, P>, dim3((unsigned)ctas), dim3(THREADS), 0, st, b));
+  else SPION_CUDA_TRY(launch_after(k_sums<TG, TD, VEC, 1>, dim3((unsigned)ctas), dim3(THREADS), 0, st, b));
+  if (a.windows > 1) SPION_CUDA_TRY(launch_after(k_join<TD, VEC>, dim3(a.sum_ctas, a.chunks), dim3(THREADS), 0, st, a));
   return SPION_OK;
 }
 template <class TG, int VEC> int launch_sums(const Sums& a, int dw_type, cudaStream_t st) {
@@ -627,7 +655,8 @@ extern "C" int spion_token_rows_backward(const long long* ids, const void* g, lo
     }
   }
   const int groups = THREADS / lanes;
-  const Sums a = {key[last], token[last], g, ldg, (float*)(ws + s.part), dw, scale, T, V, N, lanes, (int)s.window, s.windows, (unsigned)((s.windows + groups - 1) / groups)};
+  const Sums a = {key[last], token[last], g, ldg, (float*)(ws + s.part), dw, scale, T, V, N, lanes, (int)s.window, s.windows, (unsigned)((s.windows + groups - 1) / groups),
+                  (unsigned)((N + lanes * 8 - 1) / (lanes * 8))};
   const bool eight = eights(g, ldg, N, g_type) && eights(dw, N, N, dw_type);
   if (g_type == SPION_F32) return eight ? launch_sums<float, 8>(a, dw_type, st) : launch_sums<float, 1>(a, dw_type, st);
   if (g_type == SPION_BF16) return eight ? launch_sums<__nv_bfloat16, 8>(a, dw_type, st) : launch_sums<__nv_bfloat16, 1>(a, dw_type, st);
