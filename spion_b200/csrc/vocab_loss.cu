@@ -6,11 +6,12 @@
 //
 //   G_tv = g_t / tau (softmax(z_t / tau)_v - sum_{j: i_tj = v} q_tj),   dx = G W,  dW = G^T x,  db = sum_t G_t
 //
-//   k_flags, k_gather    which rows count, in order; those rows side by side in the products' type (rows that do not count cost nothing and are never read)
+//   k_flags, k_prepare   which rows count, in order; those rows side by side in the products' type (rows that do not count cost nothing and are never read; where all
+//                        count and lie as the products read them, they stay where they are)
 //   k_gemm<LOGSUM>       z tile by tile in tensor memory; leaves the largest and the sum of exponentials of a row's columns of the tile, and the targets' z
 //   k_finish             lse and loss of each row, and their sum or mean
 //   k_gemm<GRAD>         z again, for a piece of the vocabulary; leaves G in 16 bits
-//   k_gemm<DX>, <DW>     the two products with it;  k_dx, k_dw, k_db join what was summed apart
+//   k_gemm<DX>, <DW>     the two products with it;  k_out joins what was summed apart, and forms db
 //
 // The products are tcgen05 kind::f16, fp32 sums in tensor memory.  A sum there is truncated at every step, so no more than CHAIN steps go to one
 // accumulator where a result has 32 bits; what the accumulators hold is added in fp32 registers.  fp32 operands are three bf16 parts each (8 + 8 + 8 bits, exact) and
@@ -20,6 +21,7 @@
 // over the largest |g_t| (and 2^13 times that in fp16, whose smallest numbers probabilities of a large vocabulary fall below); the factor comes back in fp32.
 // The bias's gradient is summed from G before it is rounded.
 #include <algorithm>
+#include <type_traits>
 
 #include "rows.cuh"
 #include "tc_ptx.cuh"
@@ -54,6 +56,10 @@ struct Plan {
   int* target;              // [k][Tp]; -1: left out; -2: outside of the vocabulary
   float* q;                 // [k][Tp] (null: one target of weight 1)
 };
+struct Source {
+  const void* p; int type; long long ld;
+  int K, Kp, fast;          // fast: rows on 16-byte boundaries (32 in fp32), whole pieces of 8
+};
 struct Prep {
   Plan plan;
   const long long* labels;  // [T], or [T, k] where there are teacher logits
@@ -61,143 +67,202 @@ struct Prep {
   long long ignore;
   float inv_tau;
   int T, Tp, V, k;
-  int* counts;              // [chunks of CHUNK rows]
+  int* counts;              // [chunks of CHUNK rows], or null: each CTA counts for itself
   float* q;                 // [T, k]
   const void* bias; int bias_type;
   float* bias2;             // [Vp] b log2(e) / tau; -inf behind the vocabulary
   int Vp;
   float c1;                 // log2(e) / tau
+  // rows and weights in the products' type
+  Source x, w;
+  uint16_t *xs, *ws;        // ws: or null, w is read as it lies
+  int direct;               // x can be read as it lies, if all rows count
+  float* loss_rows;         // [T] or null: zeros where a row does not count
+  float* zt;                // [k][Tp]
+  unsigned row_ctas, slices, w_ctas;                     // CTAs of rows: chunks x column slices; then those of w, then those of the bias
 };
-constexpr int CHUNK = 64;
+constexpr int CHUNK = 64, SELF = 4096;                    // rows of a chunk; labels (or logits) up to which each CTA counts for itself
 
-// A warp: weights of a row's targets.  Returns whether one is there.
-__device__ __forceinline__ bool teacher_weights(const Prep& a, int t, int lane) {
-  const long long at = (long long)t * a.k;
-  float v[MAX_TARGETS / 32];
-  float top = -INFINITY;
-  bool nan = false;
+// A warp: weights of the targets of eight rows (from t0 on, below `end`).  Bits of those that have one.
+template <int WORDS> __device__ __forceinline__ unsigned teacher_weights(const Prep& a, int t0, int end, int lane) {
+  float v[8][WORDS];
 #pragma unroll
-  for (int i = 0; i < MAX_TARGETS / 32; ++i) {
-    const int j = lane + 32 * i;
-    v[i] = j < a.k && a.labels[at + j] != -1 ? load_any(a.teacher, a.teacher_type, at + j) : -INFINITY;
-    nan |= v[i] != v[i];
-    top = fmaxf(top, v[i]);
+  for (int r = 0; r < 8; ++r)
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      const int j = lane + 32 * i;
+      const long long at = (long long)(t0 + r) * a.k + j;
+      const bool in = t0 + r < end && j < a.k;
+      v[r][i] = in && a.labels[at] != -1 ? load_any(a.teacher, a.teacher_type, at) : -INFINITY;
+    }
+  unsigned found = 0;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    float top = -INFINITY;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) nan |= v[r][i] != v[r][i], top = fmaxf(top, v[r][i]);
+    top = lane_max<32>(top);
+    if (!(__any_sync(0xffffffffu, nan) || top != -INFINITY)) continue;
+    found |= 1u << r;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      v[r][i] = v[r][i] == -INFINITY ? 0.f : expf((v[r][i] - top) * a.inv_tau);
+      sum += v[r][i];
+    }
+    sum = lane_sum<32>(sum);
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i)
+      if (lane + 32 * i < a.k) a.q[(long long)(t0 + r) * a.k + lane + 32 * i] = v[r][i] / sum;
   }
-  top = lane_max<32>(top);
-  const bool any = __any_sync(0xffffffffu, nan) || top != -INFINITY;
-  if (!any) return false;
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < MAX_TARGETS / 32; ++i) {
-    v[i] = v[i] == -INFINITY ? 0.f : expf((v[i] - top) * a.inv_tau);
-    sum += v[i];
-  }
-  sum = lane_sum<32>(sum);
-#pragma unroll
-  for (int i = 0; i < MAX_TARGETS / 32; ++i)
-    if (lane + 32 * i < a.k) a.q[at + lane + 32 * i] = v[i] / sum;
-  return true;
+  return found;
 }
+__device__ __forceinline__ unsigned teacher_weights(const Prep& a, int t0, int end, int lane) {
+  return a.k <= 32 ? teacher_weights<1>(a, t0, end, lane) : teacher_weights<MAX_TARGETS / 32>(a, t0, end, lane);
+}
+__device__ __forceinline__ bool is_entry(const Prep& a, long long at) { return a.labels[at] != -1 && load_any(a.teacher, a.teacher_type, at) != -INFINITY; }
 __device__ __forceinline__ void scaled_bias(const Prep& a, int first, int step) {
   for (int v = first; v < a.Vp; v += step) a.bias2[v] = v >= a.V ? -INFINITY : a.bias != nullptr ? load_any(a.bias, a.bias_type, v) * a.c1 : 0.f;
 }
-// A warp per chunk
+// Rows that count, of each chunk: a warp per chunk, or, with a teacher, a CTA per chunk and eight rows a warp (a warp for all of them, one row after another: 8192 rows of 32
+// logits 98 us)
 __global__ void __launch_bounds__(256) k_flags(const __grid_constant__ Prep a) {
+  __shared__ int part[8];
   next_may_start();
   wait_for_kernel_before();
-  const int lane = threadIdx.x & 31, chunks = (a.T + CHUNK - 1) / CHUNK, warps = gridDim.x * 8;
-  for (int c = blockIdx.x * 8 + (threadIdx.x >> 5); c < chunks; c += warps) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = (a.T + CHUNK - 1) / CHUNK;
+  if (a.teacher == nullptr) {
+    const int c = blockIdx.x * 8 + warp;
+    if (c >= chunks) return;
     int n = 0;
-    if (a.teacher == nullptr) {
 #pragma unroll
-      for (int i = 0; i < CHUNK; i += 32) {
-        const int t = c * CHUNK + i + lane;
-        n += __popc(__ballot_sync(0xffffffffu, t < a.T && a.labels[t] != a.ignore));
-      }
-    } else {
-      for (int t = c * CHUNK; t < min(a.T, (c + 1) * CHUNK); ++t) {
-        const bool counts = teacher_weights(a, t, lane);
-        if (lane == 0) a.plan.slot[t] = counts ? 0 : -1;
-        n += counts;
-      }
+    for (int i = 0; i < CHUNK; i += 32) {
+      const int t = c * CHUNK + i + lane;
+      n += __popc(__ballot_sync(0xffffffffu, t < a.T && a.labels[t] != a.ignore));
     }
     if (lane == 0) a.counts[c] = n;
+    return;
   }
-  scaled_bias(a, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.plan.head[1] = 0;
+  const int t0 = blockIdx.x * CHUNK + 8 * warp;
+  const unsigned found = teacher_weights(a, t0, a.T, lane);
+  if (lane < 8 && t0 + lane < a.T) a.plan.slot[t0 + lane] = found >> lane & 1 ? 0 : -1;
+  if (lane == 0) part[warp] = __popc(found);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int n = 0;
+    for (int w = 0; w < 8; ++w) n += part[w];
+    a.counts[blockIdx.x] = n;
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ rows in the products' type
-struct Source {
-  const void* p; int type; long long ld;
-  int K, Kp, fast;          // fast: rows on 16-byte boundaries (32 in fp32), whole pieces of 8
-};
-// eight elements of a row to one 16-bit piece, or to three bf16 parts of an fp32 row `plane` elements apart
-template <class T> __device__ __forceinline__ void put_piece(const Source& s, long long row, int c, uint16_t* to, long long plane) {
-  const T* const from = static_cast<const T*>(s.p) + row * s.ld + c;
-  if constexpr (sizeof(T) == 2) {
-    uint4 w = make_uint4(0, 0, 0, 0);
+// Eight elements of a row from column c on, zeros behind its end, as they lie in memory
+struct Eight16 {
+  uint4 w;
+  __device__ __forceinline__ void load(const Source& s, long long row, int c) {
+    const __half* const from = static_cast<const __half*>(s.p) + row * s.ld + c;
     if (s.fast) {
-      if (c < s.K) w = *reinterpret_cast<const uint4*>(from);
-    } else {
-      uint32_t u[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + i < s.K) u[i >> 1] |= (uint32_t) * reinterpret_cast<const uint16_t*>(from + i) << (16 * (i & 1));
-      w = make_uint4(u[0], u[1], u[2], u[3]);
+      w = c < s.K ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
+      return;
     }
-    *reinterpret_cast<uint4*>(to) = w;
-  } else {
-    float f[8];
+    uint32_t u[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < s.K) u[i >> 1] |= (uint32_t) * reinterpret_cast<const uint16_t*>(from + i) << (16 * (i & 1));
+    w = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+  __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void store(uint16_t* to, long long) const { *reinterpret_cast<uint4*>(to) = w; }
+};
+struct Eight32 {
+  float f[8];
+  __device__ __forceinline__ void load(const Source& s, long long row, int c) {
+    const float* const from = static_cast<const float*>(s.p) + row * s.ld + c;
+    zero();
+    if (s.fast) {
+      if (c >= s.K) return;
+      const float4 u = reinterpret_cast<const float4*>(from)[0], v = reinterpret_cast<const float4*>(from)[1];
+      f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w, f[4] = v.x, f[5] = v.y, f[6] = v.z, f[7] = v.w;
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < s.K) f[i] = from[i];
+  }
+  __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = 0.f;
-    if (s.fast) {
-      if (c < s.K) {
-        const float4 u = reinterpret_cast<const float4*>(from)[0], v = reinterpret_cast<const float4*>(from)[1];
-        f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w, f[4] = v.x, f[5] = v.y, f[6] = v.z, f[7] = v.w;
-      }
-    } else {
+  }
+  // three bf16 parts, `plane` elements apart
+  __device__ __forceinline__ void store(uint16_t* to, long long plane) const {
+    float left[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + i < s.K) f[i] = from[i];
-    }
+    for (int i = 0; i < 8; ++i) left[i] = f[i];
 #pragma unroll
     for (int part = 0; part < 3; ++part) {
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        w[i] = pack_bf16(f[2 * i], f[2 * i + 1]);
-        f[2 * i] -= bf16_lo(w[i]), f[2 * i + 1] -= bf16_hi(w[i]);
+        w[i] = pack_bf16(left[2 * i], left[2 * i + 1]);
+        left[2 * i] -= bf16_lo(w[i]), left[2 * i + 1] -= bf16_hi(w[i]);
       }
       *reinterpret_cast<uint4*>(to + part * plane) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
-}
-// Rows first, first + step, .. below `rows` of a list (null: all of them, zeros from `known` on) to consecutive rows of the scratch
-template <class T> __device__ __forceinline__ void copy_rows(const Source& s, const int* list, int count, long long first, uint16_t* to, long long plane) {
-  const int pieces = s.Kp / 8;
-  for (int i = threadIdx.x; i < count * pieces; i += blockDim.x) {
-    const int r = i / pieces, c = (i - r * pieces) * 8;
-    put_piece<T>(s, list ? list[r] : first + r, c, to + (first + r) * s.Kp + c, plane);
-  }
-}
-
-// A CTA per chunk: its rows that count, to their slots.
-template <class T, bool FIRST> __global__ void __launch_bounds__(256) k_gather(const __grid_constant__ Prep a, const Source s, uint16_t* xs, float* loss_rows, float* zt) {
+};
+// CTAs of rows: a chunk each, or a slice of its columns.  Its rows that count, to their slots.  FIRST: in the forward, which makes the plan too.
+template <class E, bool FIRST> __global__ void __launch_bounds__(256) k_prepare(const __grid_constant__ Prep a) {
+  constexpr int PARTS = std::is_same<E, Eight32>::value ? 3 : 1;
   next_may_start();
   wait_for_kernel_before();
   __shared__ int list[CHUNK], part[2][8], here;
+  __shared__ unsigned flags[SELF / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (blockIdx.x >= a.row_ctas + a.w_ctas) {
+    scaled_bias(a, (blockIdx.x - a.row_ctas - a.w_ctas) * 256 + threadIdx.x, (gridDim.x - a.row_ctas - a.w_ctas) * 256);
+    return;
+  }
+  if (blockIdx.x >= a.row_ctas) {                          // w, padded
+    const Source& s = a.w;
+    const long long plane = (long long)a.Vp * s.Kp;
+    const unsigned pieces = s.Kp / 8;
+    for (long long r0 = (blockIdx.x - a.row_ctas) * 8ll + warp; r0 < a.Vp; r0 += a.w_ctas * 8ll)
+      for (unsigned c = lane; c < pieces; c += 32) {
+        E e;
+        if (r0 < a.V) e.load(s, r0, 8 * c);
+        else e.zero();
+        e.store(a.ws + r0 * s.Kp + 8 * c, plane);
+      }
+    return;
+  }
+  const Source& s = a.x;
+  const int chunk = blockIdx.x / a.slices, slice = blockIdx.x - chunk * a.slices;
   const long long plane = (long long)a.Tp * s.Kp;
   const int pieces = s.Kp / 8;
   int first, n;
   if constexpr (FIRST) {
     const int chunks = (a.T + CHUNK - 1) / CHUNK;
     int before = 0, all = 0;
-    for (int c = threadIdx.x; c < chunks; c += 256) {
-      const int m = a.counts[c];
-      all += m;
-      if (c < (int)blockIdx.x) before += m;
+    if (a.counts != nullptr) {
+      for (int c = threadIdx.x; c < chunks; c += 256) {
+        const int m = a.counts[c];
+        all += m;
+        if (c < chunk) before += m;
+      }
+    } else {
+      const int words = (a.T + 31) / 32;
+      for (int i = threadIdx.x; i < words; i += 256) flags[i] = 0;
+      __syncthreads();
+      for (int i = threadIdx.x; i < a.T * a.k; i += 256) {
+        const int t = i / a.k;
+        if (a.teacher ? is_entry(a, i) : a.labels[i] != a.ignore) atomicOr(&flags[t >> 5], 1u << (t & 31));
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < words; i += 256) {
+        all += __popc(flags[i]);
+        if (i < chunk * (CHUNK / 32)) before += __popc(flags[i]);
+      }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o), all += __shfl_xor_sync(0xffffffffu, all, o);
@@ -210,62 +275,65 @@ template <class T, bool FIRST> __global__ void __launch_bounds__(256) k_gather(c
       int at = 0;
 #pragma unroll
       for (int i = 0; i < CHUNK; i += 32) {
-        const int t = blockIdx.x * CHUNK + i + lane;
-        const bool counts = t < a.T && (a.teacher ? a.plan.slot[t] >= 0 : a.labels[t] != a.ignore);
+        const int t = chunk * CHUNK + i + lane;
+        const bool counts = t < a.T && (a.counts == nullptr ? flags[t >> 5] >> (t & 31) & 1 : a.teacher ? a.plan.slot[t] != -1 : a.labels[t] != a.ignore);
         const unsigned who = __ballot_sync(0xffffffffu, counts);
         const int mine = at + __popc(who & ((1u << lane) - 1));
-        if (t < a.T) {
+        if (counts) list[mine] = t;
+        if (slice == 0 && t < a.T) {
+          // (other slices of the chunk may read a slot before or after this: that it is -1 or not stays)
           a.plan.slot[t] = counts ? first + mine : -1;
-          if (loss_rows != nullptr && !counts) loss_rows[t] = 0.f;
+          if (a.loss_rows != nullptr && !counts) a.loss_rows[t] = 0.f;
+          if (counts) a.plan.row[first + mine] = t;
         }
-        if (counts) list[mine] = t, a.plan.row[first + mine] = t;
         at += __popc(who);
       }
       if (lane == 0) {
         here = at;
-        if (blockIdx.x == 0) a.plan.head[0] = n;
+        if (blockIdx.x == 0) a.plan.head[0] = n, a.plan.head[1] = 0;
       }
     }
+    if (slice == 0 && a.counts == nullptr && a.teacher != nullptr) teacher_weights(a, chunk * CHUNK + 8 * warp, a.T, lane);
     __syncthreads();
-    for (int i = threadIdx.x; i < here * a.k; i += 256) {
-      const int r = i / a.k, j = i - r * a.k;
-      const long long from = (long long)list[r] * a.k + j, to = (long long)j * a.Tp + first + r, v = a.labels[from];
-      const float q = a.teacher ? a.q[from] : 1.f;
-      a.plan.target[to] = a.teacher && (v == -1 || q == 0.f) ? -1 : v < 0 || v >= a.V ? -2 : (int)v;
-      if (a.teacher) a.plan.q[to] = v == -1 ? 0.f : q;
-      zt[to] = not_a_number();                            // of a target that no tile has
-    }
+    if (slice == 0)
+      for (int i = threadIdx.x; i < here * a.k; i += 256) {
+        const int r = i / a.k, j = i - r * a.k;
+        const long long from = (long long)list[r] * a.k + j, to = (long long)j * a.Tp + first + r, v = a.labels[from];
+        const float q = a.teacher ? a.q[from] : 1.f;
+        a.plan.target[to] = a.teacher && (v == -1 || q == 0.f) ? -1 : v < 0 || v >= a.V ? -2 : (int)v;
+        if (a.teacher) a.plan.q[to] = v == -1 ? 0.f : q;
+        a.zt[to] = not_a_number();                          // of a target that no tile has
+      }
   } else {
     n = a.plan.head[0];
-    first = blockIdx.x * CHUNK;
+    first = chunk * CHUNK;
     if (threadIdx.x < CHUNK && first + (int)threadIdx.x < n) list[threadIdx.x] = a.plan.row[first + threadIdx.x];
     if (threadIdx.x == 0) here = max(0, min(CHUNK, n - first));
     __syncthreads();
   }
-  copy_rows<T>(s, list, here, first, xs, plane);
-  // zeros up to the end of the last tile: what it holds is multiplied with zeros
-  const int zeros = (n + PAD - 1) / PAD * PAD - n;
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < zeros * pieces; i += gridDim.x * 256)
+  if (a.direct && n == a.T) return;
+  const int per = (pieces + a.slices - 1) / a.slices, p0 = slice * per, mine = min(pieces, p0 + per) - p0;
+  if (mine > 0) {
+    const int all = here * mine;
+    for (int i0 = threadIdx.x; i0 < all; i0 += 4 * 256) {
+      E e[4];
 #pragma unroll
-    for (int part_ = 0; part_ < (sizeof(T) == 4 ? 3 : 1); ++part_)
-      *reinterpret_cast<uint4*>(xs + part_ * plane + (long long)n * s.Kp + 8ll * i) = make_uint4(0, 0, 0, 0);
-}
-// W where the products cannot read it as it lies: fp32, or rows off 16 bytes
-template <class T> __global__ void __launch_bounds__(256) k_copy_w(const Source s, int V, int Vp, uint16_t* to) {
-  next_may_start();
-  wait_for_kernel_before();
-  const long long plane = (long long)Vp * s.Kp, pieces = s.Kp / 8, all = (long long)Vp * pieces;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
-    const long long r = i / pieces;
-    const int c = (int)(i - r * pieces) * 8;
-    uint16_t* const at = to + r * s.Kp + c;
-    if (r < V) {
-      put_piece<T>(s, r, c, at, plane);
-    } else {
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + 256 * u, r = i / mine;
+        if (i < all) e[u].load(s, list[r], 8 * (p0 + i - r * mine));
+      }
 #pragma unroll
-      for (int p = 0; p < (sizeof(T) == 4 ? 3 : 1); ++p) *reinterpret_cast<uint4*>(at + p * plane) = make_uint4(0, 0, 0, 0);
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + 256 * u, r = i / mine;
+        if (i < all) e[u].store(a.xs + (long long)(first + r) * s.Kp + 8 * (p0 + i - r * mine), plane);
+      }
     }
   }
+  // zeros up to the end of the last tile: what it holds is multiplied with zeros
+  const int zeros = (n + PAD - 1) / PAD * PAD - n;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < (long long)zeros * pieces; i += a.row_ctas * 256ll)
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) *reinterpret_cast<uint4*>(a.xs + p * plane + (long long)n * s.Kp + 8 * i) = make_uint4(0, 0, 0, 0);
 }
 
 // ------------------------------------------------------------------------------------------------ the four products
@@ -274,9 +342,21 @@ constexpr int BK = 64;                                    // elements of the con
 constexpr int EPI = 8, THREADS = 32 * (2 + EPI);
 constexpr int STAGES = 6;
 constexpr uint32_t HALF = 128 * BK * 2, STAGE = 2 * HALF;
-constexpr uint32_t BARS = STAGES * STAGE, SMEM = BARS + 16 * STAGES + 64;
-static_assert(SMEM <= 232448, "shared memory of a multiprocessor");
+constexpr uint32_t BARS = STAGES * STAGE, STAGED = BARS + 16 * STAGES + 64;      // STAGED: 32 x 32 results a writing warp, rows of 33 (DW)
+template <int MODE> constexpr uint32_t SMEM = MODE == DW ? STAGED + EPI * 32 * 33 * 4 : STAGED;
+static_assert(SMEM<DW> <= 232448, "shared memory of a multiprocessor");
 
+// What the products with G are multiplied with.  Rows with a g each: it comes from k_unit.
+struct Coef {
+  const float* g;                                         // one number, or null
+  const float* unit;                                      // [0]: the largest |g|, rounded to a power of two; [1]: its reciprocal
+  int mean;
+  float scale;                                            // 1 / (tau gscale)
+  __device__ __forceinline__ float alpha(int n) const {
+    if (g == nullptr) return unit[0] * scale;
+    return n > 0 ? (mean ? *g / (float)n : *g) * scale : 0.f;
+  }
+};
 struct Args {
   const int* n;                                           // rows that count
   int products;                                           // 1, or 6 of three parts
@@ -286,12 +366,13 @@ struct Args {
   int chain;                                              // (chunk, product) pairs that one accumulator takes
   int splits, split_chunks;                               // of the contraction (0: by the number of tiles, at most split_chunks)
   int fp16;                                               // operands are fp16, else bf16
+  int direct_rows;                                        // rows of x, where they are read as they lie if all count; else 0
   // LOGSUM, GRAD
   Plan plan; int Tp, k;
   const float* bias2; float c1;
   float2* part; int parts;                                // [slots, parts] largest, sum
   float* zt;                                              // [k][Tp]
-  const float* g; const float* coef;                      // per row or null; coef[1]: 1 / max |g|
+  const float* g; Coef coef;                              // per row or null
   uint16_t* G; long long ldg;                             // [planes][Tp][ldg]
   float* colsum;                                          // [Tp / 32][ldg] or null
   float gscale;                                           // 1, or 2^13 in fp16
@@ -299,7 +380,7 @@ struct Args {
   float* out; long long ldo; int add;                     // fp32 partial sums: [split][rows of whole tiles][ldo]
   void* dw; int dw_type; long long K; int V;              // DW, one split: the result
 };
-struct Maps { CUtensorMap a, b; };
+struct Maps { CUtensorMap a, b, x; };                       // x: the rows as they lie, in place of a (LOGSUM, GRAD) or of b (DW)
 
 __device__ __forceinline__ uint32_t cta_rank() {
   uint32_t r;
@@ -398,7 +479,7 @@ template <class F> __device__ __forceinline__ void each_target(const Args& a, co
 }
 
 // What a thread does with its sums: row `row` of D, columns col .. col + W - 1 (W = BN / 2)
-template <int MODE, int W> __device__ __forceinline__ void epilogue(const Args& a, const Work& w, float (&acc)[W], int n, int s, int row, int col, int tile_m, int part) {
+template <int MODE, int W> __device__ __forceinline__ void epilogue(const Args& a, const Work& w, float (&acc)[W], int n, int s, int row, int col, int tile_m, int part, float* stage) {
   const int lane = threadIdx.x & 31;
   if constexpr (MODE == LOGSUM || MODE == GRAD) {
     const bool in = row < n;
@@ -435,7 +516,7 @@ template <int MODE, int W> __device__ __forceinline__ void epilogue(const Args& 
       float lse = 0.f, r = 0.f;
       if (in) {
         lse = a.plan.lse[slot];
-        r = a.g ? a.g[a.plan.row[slot]] * a.coef[1] : 1.f;
+        r = a.g ? a.g[a.plan.row[slot]] * a.coef.unit[1] : 1.f;
         r *= a.gscale;
       }
 #pragma unroll
@@ -481,25 +562,35 @@ template <int MODE, int W> __device__ __forceinline__ void epilogue(const Args& 
     }
   } else {
     if (MODE == DW && a.dw != nullptr) {
-      const float alpha = a.coef[0];
+      const float alpha = a.coef.alpha(n);
       const int v = a.col0 + row;
-      if (v >= a.V) return;
+      if (a.K % 8 == 0) {
+        if (v >= a.V) return;
 #pragma unroll
-      for (int g = 0; g < W; g += 8) {
-        if (col + g >= a.K) continue;
-        float f[8];
+        for (int g = 0; g < W; g += 8) {
+          if (col + g >= a.K) continue;
+          float f[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = acc[g + e] * alpha;
-        const long long at = (long long)v * a.K + col + g;
-        if (a.K % 8 == 0) {
+          for (int e = 0; e < 8; ++e) f[e] = acc[g + e] * alpha;
+          const long long at = (long long)v * a.K + col + g;
           if (a.dw_type == SPION_F32) Out<float, 8>::store(static_cast<float*>(a.dw) + at, f);
           else if (a.dw_type == SPION_BF16) Out<__nv_bfloat16, 8>::store(static_cast<__nv_bfloat16*>(a.dw) + at, f);
           else Out<__half, 8>::store(static_cast<__half*>(a.dw) + at, f);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (col + g + e < a.K) store_any(a.dw, a.dw_type, at + e, f[e]);
         }
+        return;
+      }
+      // rows that start anywhere: lanes side by side along each (one row a lane: 10007 rows of 770 fp16 126 us, so 31)
+#pragma unroll
+      for (int g = 0; g < W; g += 32) {
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) stage[33 * lane + e] = acc[g + e] * alpha;
+        __syncwarp();
+        const int c = col + g + lane, v0 = v - lane;
+        if (c < a.K)
+#pragma unroll 4
+          for (int r = 0; r < 32; ++r)
+            if (v0 + r < a.V) store_any(a.dw, a.dw_type, (long long)(v0 + r) * a.K + c, stage[33 * r + lane]);
       }
       return;
     }
@@ -543,6 +634,7 @@ template <int MODE, bool PAIR> __global__ void __launch_bounds__(THREADS, 1) k_g
     fence_proxy_async();
     tma_prefetch_desc(&maps.a);
     tma_prefetch_desc(&maps.b);
+    tma_prefetch_desc(&maps.x);
   }
   if (warp == 1) {
     if (PAIR) {
@@ -560,6 +652,8 @@ template <int MODE, bool PAIR> __global__ void __launch_bounds__(THREADS, 1) k_g
   wait_for_kernel_before();
   const int n = *reinterpret_cast<const volatile int*>(a.n);
   const Work w = work_of(a, n, TILE, BN, step);
+  const bool direct = n == a.direct_rows;
+  const CUtensorMap *const map_a = MODE != DW && MODE != DX && direct ? &maps.x : &maps.a, *const map_b = MODE == DW && direct ? &maps.x : &maps.b;
   const int items = w.splits * w.tiles_m * w.tiles_n;
   const bool aborted = s_abort != 0;
   if (warp == 0) {
@@ -591,16 +685,16 @@ template <int MODE, bool PAIR> __global__ void __launch_bounds__(THREADS, 1) k_g
             };
             const int ya = (int)(pa * a.plane_a), yb = (int)(pb * a.plane_b) + (MODE == LOGSUM || MODE == GRAD || MODE == DX ? a.col0 : 0);
             if (A_MN) {
-              load(to_a, &maps.a, ra, ya + c * BK);
-              load(to_a + HALF / 2, &maps.a, ra + 64, ya + c * BK);
+              load(to_a, map_a, ra, ya + c * BK);
+              load(to_a + HALF / 2, map_a, ra + 64, ya + c * BK);
             } else {
-              load(to_a, &maps.a, c * BK, ya + ra);
+              load(to_a, map_a, c * BK, ya + ra);
             }
             if (B_MN) {
-              load(to_b, &maps.b, rb, yb + c * BK);
-              load(to_b + HALF / 2, &maps.b, rb + 64, yb + c * BK);
+              load(to_b, map_b, rb, yb + c * BK);
+              load(to_b + HALF / 2, map_b, rb + 64, yb + c * BK);
             } else {
-              load(to_b, &maps.b, c * BK, yb + rb);
+              load(to_b, map_b, c * BK, yb + rb);
             }
             ++fills;
             if (++st == STAGES) st = 0, ph ^= 1;
@@ -691,7 +785,8 @@ template <int MODE, bool PAIR> __global__ void __launch_bounds__(THREADS, 1) k_g
       if (lost)
 #pragma unroll
         for (int g = 0; g < W; ++g) acc[g] = not_a_number();
-      epilogue<MODE, W>(a, w, acc, n, s, m * TILE + rank * 128 + q * 32 + lane, nn * BN + half * W, TILE, 2 * nn + half);
+      epilogue<MODE, W>(a, w, acc, n, s, m * TILE + rank * 128 + q * 32 + lane, nn * BN + half * W, TILE, 2 * nn + half,
+                        reinterpret_cast<float*>(smem_raw + STAGED) + (warp - 2) * 32 * 33);
     }
   }
   tc_fence_before();
@@ -710,113 +805,124 @@ struct Finish {
   const float2* part; int parts;
   const float* zt;
   float* loss;              // [T] (reduction 0) or one number
-  float* slot_loss;         // [Tp]
+  double* cta_loss;         // [CTAs]
   int reduction;            // 0 none, 1 mean, 2 sum
 };
-// A warp per row that counts; the last CTA adds them up, in their order.
-__global__ void __launch_bounds__(256) k_finish(const __grid_constant__ Finish a) {
+template <int LANES> __device__ __forceinline__ float row_loss(const Finish& a, int i, int lane, bool lost, float& lse) {
+  const float2* const p = a.part + (long long)i * a.parts;
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
+  for (int c = lane; c < a.parts; c += LANES) {
+    const float2 v = p[c];
+    const float m = fmaxf(top, v.x), from = m == -INFINITY ? 0.f : m;
+    sum = sum * ex2(top - from) + v.y * ex2(v.x - from);
+    top = m;
+  }
+  const float all = lane_max<LANES>(top), from = all == -INFINITY ? 0.f : all;
+  sum = lane_sum<LANES>(sum * ex2(top - from));
+  lse = from + log2f(sum);
+  float loss = 0.f;
+  for (int j = lane; j < a.k; j += LANES) {
+    const long long at = (long long)j * a.Tp + i;
+    if (a.plan.target[at] == -1) continue;
+    const float q = a.plan.q ? a.plan.q[at] : 1.f;
+    loss += q * ((a.plan.q ? log2f(q) : 0.f) + (lse - a.zt[at]));
+  }
+  loss = lane_sum<LANES>(loss) * LN2;
+  return lost ? not_a_number() : loss;
+}
+// LANES threads per row that counts (4, 8 or 32: the fewest that leave four partial sums or fewer to each, or 32).  A CTA adds its rows' losses, the last one the CTAs', in
+// their order and in 64 bits.
+template <int LANES> __global__ void __launch_bounds__(256) k_finish(const __grid_constant__ Finish a) {
   next_may_start();
   wait_for_kernel_before();
   __shared__ double sums[256];
   __shared__ int last;
-  const int lane = threadIdx.x & 31, n = *reinterpret_cast<const volatile int*>(a.plan.head);
+  const int lane = threadIdx.x % LANES, n = *reinterpret_cast<const volatile int*>(a.plan.head);
   const bool lost = *reinterpret_cast<volatile int*>(&g_vocab_status) != 0;
-  for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += gridDim.x * 8) {
-    const float2* const p = a.part + (long long)i * a.parts;
-    float top = -INFINITY, sum = 0.f;
-    for (int c = lane; c < a.parts; c += 32) {
-      const float2 v = p[c];
-      const float m = fmaxf(top, v.x), from = m == -INFINITY ? 0.f : m;
-      sum = sum * ex2(top - from) + v.y * ex2(v.x - from);
-      top = m;
-    }
-    const float all = lane_max<32>(top), from = all == -INFINITY ? 0.f : all;
-    sum = lane_sum<32>(sum * ex2(top - from));
-    float lse = from + log2f(sum), loss = 0.f;
-    for (int j = lane; j < a.k; j += 32) {
-      const long long at = (long long)j * a.Tp + i;
-      if (a.plan.target[at] == -1) continue;
-      const float q = a.plan.q ? a.plan.q[at] : 1.f;
-      loss += q * ((a.plan.q ? log2f(q) : 0.f) + (lse - a.zt[at]));
-    }
-    loss = lane_sum<32>(loss) * LN2;
-    if (lost) loss = not_a_number();
-    if (lane == 0) {
-      a.plan.lse[i] = loss != loss ? loss : lse;          // a row without a loss has no gradient either: NaN
+  constexpr int ROWS = 256 / LANES;
+  double s = 0.0;
+  for (int i0 = blockIdx.x * ROWS; i0 < n; i0 += gridDim.x * ROWS) {
+    const int i = i0 + threadIdx.x / LANES;
+    float lse;
+    const float loss = row_loss<LANES>(a, min(i, n - 1), lane, lost, lse);      // (all lanes take part in the sums over lanes)
+    if (lane == 0 && i < n) {
+      a.plan.lse[i] = loss != loss ? loss : lse;            // a row without a loss has no gradient either: NaN
       if (a.reduction == 0) a.loss[a.plan.row[i]] = loss;
-      else a.slot_loss[i] = loss;
+      s += (double)loss;
     }
   }
   if (a.reduction == 0) return;
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(a.plan.head + 1, 1) == (int)gridDim.x - 1;
+  auto add_up = [&] {
+    sums[threadIdx.x] = s;
+    __syncthreads();
+    for (int o = 128; o > 0; o >>= 1) {
+      if ((int)threadIdx.x < o) sums[threadIdx.x] += sums[threadIdx.x + o];
+      __syncthreads();
+    }
+  };
+  add_up();
+  if (threadIdx.x == 0) {
+    a.cta_loss[blockIdx.x] = sums[0];
+    __threadfence();
+    last = atomicAdd(a.plan.head + 1, 1) == (int)gridDim.x - 1;
+  }
   __syncthreads();
   if (!last) return;
   __threadfence();
-  double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += 256) s += (double)*reinterpret_cast<volatile float*>(a.slot_loss + i);
-  sums[threadIdx.x] = s;
-  __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
-    if ((int)threadIdx.x < o) sums[threadIdx.x] += sums[threadIdx.x + o];
-    __syncthreads();
-  }
+  s = 0.0;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += 256) s += *reinterpret_cast<volatile double*>(a.cta_loss + i);
+  add_up();
   if (threadIdx.x == 0) *a.loss = a.reduction == 2 ? (float)sums[0] : n > 0 ? (float)(sums[0] / n) : not_a_number();
 }
 
 // ------------------------------------------------------------------------------------------------ gradients
-// coef[0]: what the products with G are multiplied with; coef[1]: 1 / max |g| where every row has its own g (rounded to a power of two).  The first CTA; the others
-// form the bias in units of log2.
-__global__ void __launch_bounds__(1024) k_coef(const __grid_constant__ Prep a, const float* g, int reduction, float inv_gscale, float* coef) {
+// unit[0]: the largest of the rows' |g|, rounded up to a power of two (products by it are exact, and neither it nor its reciprocal leaves the normal numbers); unit[1]: its reciprocal
+__global__ void __launch_bounds__(1024) k_unit(const Plan plan, const float* g, float* unit) {
   next_may_start();
   wait_for_kernel_before();
-  if (blockIdx.x > 0) {
-    scaled_bias(a, (blockIdx.x - 1) * 1024 + threadIdx.x, (gridDim.x - 1) * 1024);
-    return;
-  }
   __shared__ float part[32];
-  const Plan& plan = a.plan;
-  const float inv_tau = a.inv_tau;
   const int n = *reinterpret_cast<const volatile int*>(plan.head);
   float top = 0.f;
-  if (reduction == 0)
-    for (int i = threadIdx.x; i < n; i += 1024) {
-      const float v = fabsf(g[plan.row[i]]);
-      if (v < INFINITY) top = fmaxf(top, v);              // one that is not finite stays its own row's
-    }
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    const float v = fabsf(g[plan.row[i]]);
+    if (v < INFINITY) top = fmaxf(top, v);                  // one that is not finite stays its own row's
+  }
   top = lane_max<32>(top);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
   __syncthreads();
-  if (threadIdx.x < 32) {
-    top = lane_max<32>(part[threadIdx.x]);
-    if (threadIdx.x == 0) {
-      if (reduction == 0) {
-        // a power of two: the products by it are exact, and neither it nor its reciprocal leaves the normal numbers
-        const float unit = top > 0.f ? exp2f(fminf(fmaxf(ceilf(log2f(top)), -100.f), 126.f)) : 1.f;
-        coef[0] = unit * inv_tau * inv_gscale, coef[1] = 1.f / unit;
-      } else {
-        coef[0] = n > 0 ? (reduction == 1 ? *g / (float)n : *g) * inv_tau * inv_gscale : 0.f;
-        coef[1] = 1.f;
-      }
-    }
-  }
+  if (threadIdx.x >= 32) return;
+  top = lane_max<32>(part[threadIdx.x]);
+  if (threadIdx.x > 0) return;
+  const float u = top > 0.f ? exp2f(fminf(fmaxf(ceilf(log2f(top)), -100.f), 126.f)) : 1.f;
+  unit[0] = u, unit[1] = 1.f / u;
 }
-// dx of all rows: the sums of the splits, zeros where a row does not count.  Also joins the parts of dW (no slots, rows one behind another).
+// What leaves: out[r, :] = alpha (sum over the splits of part[split][r, :]), dx by the rows' slots (zeros for rows without one), dw row by row; db[v] = alpha (sum of G's columns).
 struct Join {
-  const int* head; const int* slot;                       // slot null: rows are slots
+  const int* slot;                                        // or null: rows as they are
   const float* part; long long ldp;                       // [splits][plane rows][ldp]
   int splits, tile, tiles_n, units, chunks;               // splits 0: as k_gemm<DX> had them
   long long plane;                                        // rows of a split (splits given)
-  const float* coef;
   void* out; int type; long long rows, K;
+  unsigned ctas;
 };
-__global__ void __launch_bounds__(256) k_join(const __grid_constant__ Join a) {
-  next_may_start();
-  wait_for_kernel_before();
-  const int n = *reinterpret_cast<const volatile int*>(a.head);
-  const bool lost = *reinterpret_cast<volatile int*>(&g_vocab_status) != 0;
-  const float alpha = lost ? not_a_number() : a.coef[0];
+struct Bias { const float* colsum; long long ldg; int columns; void* db; int type; unsigned ctas; };
+struct Leave { const int* head; Coef coef; Join j[2]; Bias b; };
+
+__device__ __forceinline__ void store8(const Join& a, long long r, long long c, const float (&f)[8]) {
+  const long long at = r * a.K + c;
+  if (a.K % 8 == 0) {
+    if (a.type == SPION_F32) Out<float, 8>::store(static_cast<float*>(a.out) + at, f);
+    else if (a.type == SPION_BF16) Out<__nv_bfloat16, 8>::store(static_cast<__nv_bfloat16*>(a.out) + at, f);
+    else Out<__half, 8>::store(static_cast<__half*>(a.out) + at, f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < a.K) store_any(a.out, a.type, at + e, f[e]);
+  }
+}
+__device__ __forceinline__ void join(const Join& a, unsigned cta, int n, float alpha, float (*shared)[8]) {
   int splits = a.splits;
   long long plane = a.plane;
   if (splits == 0) {
@@ -824,50 +930,66 @@ __global__ void __launch_bounds__(256) k_join(const __grid_constant__ Join a) {
     splits = split_by_tiles(tiles_m * a.tiles_n, a.units, a.chunks);
     plane = (long long)tiles_m * a.tile;
   }
-  const long long pieces = (a.K + 7) / 8, all = a.rows * pieces;
-  const bool whole = a.K % 8 == 0;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
-    const long long r = i / pieces, c = (i - r * pieces) * 8;
-    const long long from = a.slot ? a.slot[r] : r;
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (from >= 0) {
-      for (int s = 0; s < splits; ++s) {
-        Piece<float, 8> p;
-        p.load(a.part + (s * plane + from) * a.ldp + c);
+  const int pieces = (int)((a.K + 7) / 8);
+  // of many splits, eight threads take a share each
+  const int shares = splits >= 8 ? 8 : 1, share = threadIdx.x & (shares - 1), each = (splits + shares - 1) / shares, per = 256 / shares;
+  const long long all = a.rows * pieces, step = (long long)a.ctas * per;
+  for (long long i0 = (long long)cta * per; i0 < all; i0 += step) {
+    const long long i = i0 + threadIdx.x / shares;
+    const long long r = all < 0x7fffffff ? (unsigned)i / (unsigned)pieces : i / pieces, c = (i - r * pieces) * 8;
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, by = alpha;
+    if (i < all) {
+      const long long from = a.slot ? a.slot[r] : r;
+      if (from >= 0)
+#pragma unroll 4
+        for (int s = share * each; s < min(splits, (share + 1) * each); ++s) {
+          Piece<float, 8> p;
+          p.load(a.part + (s * plane + from) * a.ldp + c);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] += p.at(e);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] *= alpha;
+          for (int e = 0; e < 8; ++e) f[e] += p.at(e);
+        }
+      if (from < 0) by = 0.f;                             // whatever arrives at the loss
     }
-    const long long at = r * a.K + c;
-    if (whole) {
-      if (a.type == SPION_F32) Out<float, 8>::store(static_cast<float*>(a.out) + at, f);
-      else if (a.type == SPION_BF16) Out<__nv_bfloat16, 8>::store(static_cast<__nv_bfloat16*>(a.out) + at, f);
-      else Out<__half, 8>::store(static_cast<__half*>(a.out) + at, f);
-    } else {
+    if (shares > 1) {
+      __syncthreads();
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c + e < a.K) store_any(a.out, a.type, at + e, f[e]);
+      for (int e = 0; e < 8; ++e) shared[threadIdx.x][e] = f[e];
+      __syncthreads();
+      if (share == 0)
+        for (int o = 1; o < shares; ++o)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] += shared[threadIdx.x + o][e];
+    }
+    if (i < all && share == 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] *= by;
+      store8(a, r, c, f);
     }
   }
 }
-// db of a piece: 32 columns a CTA, eight shares of the blocks of 32 rows
-__global__ void __launch_bounds__(256) k_db(const int* head, const float* colsum, long long ldg, int columns, const float* coef, void* db, int type) {
+__global__ void __launch_bounds__(256) k_out(const __grid_constant__ Leave a) {
+  __shared__ float shared[256][8];
   next_may_start();
   wait_for_kernel_before();
-  __shared__ float part[8][32];
-  const int n = *reinterpret_cast<const volatile int*>(head), lane = threadIdx.x & 31, share = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-  float s = 0.f;
-  if (c < columns)
-    for (int b = share; b < (n + 31) / 32; b += 8) s += colsum[b * ldg + c];
-  part[share][lane] = s;
-  __syncthreads();
-  if (share > 0 || c >= columns) return;
+  const int n = *reinterpret_cast<const volatile int*>(a.head);
+  const float alpha = *reinterpret_cast<volatile int*>(&g_vocab_status) != 0 ? not_a_number() : a.coef.alpha(n);
+  if (blockIdx.x < a.j[0].ctas) {
+    join(a.j[0], blockIdx.x, n, alpha, shared);
+  } else if (blockIdx.x < a.j[0].ctas + a.j[1].ctas) {
+    join(a.j[1], blockIdx.x - a.j[0].ctas, n, alpha, shared);
+  } else {                                                 // 32 columns a CTA, eight shares of the blocks of 32 rows
+    const int lane = threadIdx.x & 31, share = threadIdx.x >> 5, c = (blockIdx.x - a.j[0].ctas - a.j[1].ctas) * 32 + lane;
+    float s = 0.f;
+    if (c < a.b.columns)
+#pragma unroll 8
+      for (int k = share; k < (n + 31) / 32; k += 8) s += a.b.colsum[k * a.b.ldg + c];
+    shared[threadIdx.x][0] = s;
+    __syncthreads();
+    if (share > 0 || c >= a.b.columns) return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) s += part[i][lane];
-  const bool lost = *reinterpret_cast<volatile int*>(&g_vocab_status) != 0;
-  store_any(db, type, c, lost ? not_a_number() : s * coef[0]);
+    for (int i = 1; i < 8; ++i) s += shared[threadIdx.x + 32 * i][0];
+    store_any(a.b.db, a.b.type, c, s * alpha);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -893,8 +1015,17 @@ int map_of(CUtensorMap* m, const void* base, long long cols, long long rows_, lo
   if (rc != SPION_OK) return rc;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows_}, strides[1] = {(cuuint64_t)ld * 2};
   const cuuint32_t box[2] = {BK, (cuuint32_t)box_rows}, step[2] = {1, 1};
-  const CUresult r = encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto make = [&] {
+    return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = make();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {                  // a thread that has used the device for nothing yet (a first backward): this makes its context current
+    int dev = 0;
+    SPION_CUDA_TRY(cudaGetDevice(&dev));
+    SPION_CUDA_TRY(cudaSetDevice(dev));
+    r = make();
+  }
   if (r != CUDA_SUCCESS) {
     fprintf(stderr, "spion_b200: cuTensorMapEncodeTiled failed (%d) rows=%lld cols=%lld\n", (int)r, rows_, cols);
     return SPION_ERR_CUDA;
@@ -908,13 +1039,13 @@ template <int MODE, bool PAIR> int units_of(int* units) {
   SPION_CUDA_TRY(cudaGetDevice(&dev));
   int n = dev < 64 ? known[dev].load() : 0;
   if (n == 0) {
-    SPION_CUDA_TRY(cudaFuncSetAttribute(k_gemm<MODE, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
+    SPION_CUDA_TRY(cudaFuncSetAttribute(k_gemm<MODE, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM<MODE>));
     if (PAIR) {
       cudaLaunchConfig_t cfg = {};
       cudaLaunchAttribute at[1];
       at[0].id = cudaLaunchAttributeClusterDimension;
       at[0].val.clusterDim.x = 2, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-      cfg.gridDim = dim3(2 * (sm_count() / 2)), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = SMEM, cfg.attrs = at, cfg.numAttrs = 1;
+      cfg.gridDim = dim3(2 * (sm_count() / 2)), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = SMEM<MODE>, cfg.attrs = at, cfg.numAttrs = 1;
       SPION_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, k_gemm<MODE, PAIR>, &cfg));
     } else {
       n = sm_count();
@@ -937,7 +1068,7 @@ template <int MODE, bool PAIR> int launch_gemm(const Args& a, const Maps& maps, 
   at[0].val.programmaticStreamSerializationAllowed = 1;
   at[1].id = cudaLaunchAttributeClusterDimension;
   at[1].val.clusterDim.x = 2, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(PAIR ? 2 * use : use), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = SMEM, cfg.stream = st, cfg.attrs = at, cfg.numAttrs = PAIR ? 2 : 1;
+  cfg.gridDim = dim3(PAIR ? 2 * use : use), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = SMEM<MODE>, cfg.stream = st, cfg.attrs = at, cfg.numAttrs = PAIR ? 2 : 1;
   SPION_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_gemm<MODE, PAIR>, a, maps));
   return SPION_OK;
 }
@@ -954,15 +1085,20 @@ constexpr int LONG_CHAIN = 64;                            // of a result that is
 struct Layout {
   long long T, Tp, K, Kp, V, Vp, k, ldw;
   int planes;
-  bool copy_w;
+  bool copy_w, direct;                                    // w has to be copied; x can be read as it lies
+  bool kept;                                              // the operands' copies stay for the backward
+  bool self;                                              // CTAs count for themselves
   bool pair_z, pair_dx, pair_dw;
   long long Gp;                                           // columns of a piece of the vocabulary
   int dw_splits;
   size_t keep;                                            // bytes of the plan
-  size_t xs, w, bias2, part, zt, slot_loss, counts, q, forward;
-  size_t g, dxp, dwp, colsum, coef, backward;
+  size_t xs, w, bias2;                                    // in the plan (kept) or in both workspaces
+  size_t part, zt, cta_loss, counts, q, forward;
+  size_t g, dxp, dwp, colsum, unit, backward;
 };
 constexpr long long PIECE_BYTES = 256ll << 20;            // of G
+constexpr long long KEPT_BYTES = 64ll << 20;              // of copies that stay: small beside the device, and making them again costs launches and, for small calls, most of the time
+constexpr int FINISH_CTAS = 1024;
 
 int layout_of(const spion_vocab_problem* p, Layout* l) {
   if (p == nullptr || p->T < 0 || p->K <= 0 || p->V <= 0 || p->k <= 0) return SPION_ERR_ARG;
@@ -977,7 +1113,9 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   // places are 32-bit numbers in the tensor maps' coordinates and in the lists of rows
   if (p->T > 0x7fffffff / 4 || p->V > 0x7fffffff / 4 || p->K > 0x7fffffff / 4 || l->Tp * l->planes > 0x7fffffff || l->Vp * l->planes > 0x7fffffff) return SPION_ERR_SHAPE;
   l->copy_w = p->type == SPION_F32 || ((uintptr_t)p->w % 16) != 0 || (p->ldw * 2) % 16 != 0;
+  l->direct = p->type != SPION_F32 && ((uintptr_t)p->x % 16) == 0 && (p->ldx * 2) % 16 == 0 && p->ldx >= p->K;
   l->ldw = l->copy_w ? l->Kp : p->ldw;
+  l->self = p->T * p->k <= SELF;
   int sms = sm_count();
   if (sms <= 0) return SPION_ERR_CUDA;
   const int pairs = sms / 2;
@@ -995,16 +1133,18 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
     at += (size_t)up(std::max(bytes, 0ll), 256);
     return here;
   };
+  const long long xs_bytes = 2 * l->planes * l->Tp * l->Kp, w_bytes = l->copy_w ? 2 * l->planes * l->Vp * l->Kp : 0;
+  l->kept = xs_bytes + w_bytes + 4 * l->Vp <= KEPT_BYTES;
   take(256), take(4 * l->Tp), take(4 * l->Tp), take(4 * l->Tp), take(4 * l->k * l->Tp), take(4 * l->k * l->Tp);
+  auto operands = [&] { l->xs = take(xs_bytes), l->w = take(w_bytes), l->bias2 = take(4 * l->Vp); };
+  if (l->kept) operands();
   l->keep = at;
   at = 0;
-  l->xs = take(2 * l->planes * l->Tp * l->Kp);
-  l->w = take(l->copy_w ? 2 * l->planes * l->Vp * l->Kp : 0);
-  l->bias2 = take(4 * l->Vp);
+  if (!l->kept) operands();
   const size_t both = at;
   l->part = take(8 * l->Tp * 2 * (l->pair_z ? tiles_of(l->V, 256) : tiles_of(l->V, 128)));
   l->zt = take(4 * l->k * l->Tp);
-  l->slot_loss = take(4 * l->Tp);
+  l->cta_loss = take(8 * FINISH_CTAS);
   l->counts = take(4 * tiles_of(l->T, CHUNK));
   l->q = take(4 * l->T * l->k);
   l->forward = at;
@@ -1014,7 +1154,7 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   l->dxp = take(4 * std::max(tiles_of(l->T, tile), (l->pair_dx ? pairs : sms) / tn) * tile * l->Kp);
   l->dwp = take(l->dw_splits > 1 ? 4 * l->dw_splits * up(l->Gp, l->pair_dw ? 256 : 128) * l->Kp : 0);
   l->colsum = take(4 * (l->Tp / 32) * l->Gp);
-  l->coef = take(256);
+  l->unit = take(256);
   l->backward = at;
   return SPION_OK;
 }
@@ -1034,34 +1174,33 @@ Source source_of(const void* p, int type, long long ld, long long K, long long K
   const int piece = type == SPION_F32 ? 32 : 16;
   return {p, type, ld, (int)K, (int)Kp, K % 8 == 0 && (uintptr_t)p % piece == 0 && ld * type_size(type) % piece == 0};
 }
-int launch_copy_w(const spion_vocab_problem* p, const Layout& l, uint16_t* to, cudaStream_t st) {
-  if (!l.copy_w) return SPION_OK;
-  const Source s = source_of(p->w, p->type, p->ldw, l.K, l.Kp);
-  const dim3 grid((unsigned)std::min<long long>(tiles_of(l.Vp * l.Kp / 8, 256), 8 * sm_count()));
-  if (p->type == SPION_F32) SPION_CUDA_TRY(launch_after(k_copy_w<float>, grid, dim3(256), 0, st, s, (int)l.V, (int)l.Vp, to));
-  else SPION_CUDA_TRY(launch_after(k_copy_w<__half>, grid, dim3(256), 0, st, s, (int)l.V, (int)l.Vp, to));
-  return SPION_OK;
-}
 Prep prep_of(const spion_vocab_problem* p, const Layout& l, void* keep, char* ws) {
   Prep a = {};
   a.plan = plan_at(l, keep, p->teacher != nullptr);
   a.labels = p->labels, a.teacher = p->teacher, a.teacher_type = p->teacher_type, a.ignore = p->ignore_index;
   a.inv_tau = 1.f / p->temperature;
   a.T = (int)l.T, a.Tp = (int)l.Tp, a.V = (int)l.V, a.k = (int)l.k, a.Vp = (int)l.Vp;
-  a.counts = (int*)(ws + l.counts), a.q = (float*)(ws + l.q);
-  a.bias = p->bias, a.bias_type = p->bias_type, a.bias2 = (float*)(ws + l.bias2);
   a.c1 = (float)(1.4426950408889634 / (double)p->temperature);
+  char* const operands = l.kept ? static_cast<char*>(keep) : ws;
+  a.bias = p->bias, a.bias_type = p->bias_type, a.bias2 = (float*)(operands + l.bias2);
+  a.x = source_of(p->x, p->type, p->ldx, l.K, l.Kp), a.w = source_of(p->w, p->type, p->ldw, l.K, l.Kp);
+  a.xs = (uint16_t*)(operands + l.xs), a.ws = l.copy_w ? (uint16_t*)(operands + l.w) : nullptr;
+  a.direct = l.direct;
+  const long long chunks = tiles_of(l.T, CHUNK), bytes = l.Kp * (l.planes == 3 ? 4 : 2);
+  // slices of 512 bytes of a row at least, where there are too few chunks to fill the device twice
+  a.slices = (unsigned)std::max<long long>(1, std::min<long long>(bytes / 512, 2 * sm_count() / chunks));
+  a.row_ctas = (unsigned)chunks * a.slices;
+  a.w_ctas = l.copy_w ? (unsigned)std::min<long long>(tiles_of(l.Vp, 8), 8 * sm_count()) : 0;
   return a;
 }
-template <bool FIRST> int launch_gather(const spion_vocab_problem* p, const Layout& l, const Prep& a, uint16_t* xs, float* loss_rows, float* zt, cudaStream_t st) {
-  const Source s = source_of(p->x, p->type, p->ldx, l.K, l.Kp);
-  const dim3 grid((unsigned)tiles_of(l.T, CHUNK));
-  if (p->type == SPION_F32) SPION_CUDA_TRY(launch_after(k_gather<float, FIRST>, grid, dim3(256), 0, st, a, s, xs, loss_rows, zt));
-  else SPION_CUDA_TRY(launch_after(k_gather<__half, FIRST>, grid, dim3(256), 0, st, a, s, xs, loss_rows, zt));
+template <bool FIRST> int launch_prepare(const spion_vocab_problem* p, const Prep& a, cudaStream_t st) {
+  const dim3 grid(a.row_ctas + a.w_ctas + (unsigned)std::min<long long>(tiles_of(a.Vp, 256), 2 * sm_count()));
+  if (p->type == SPION_F32) SPION_CUDA_TRY(launch_after(k_prepare<Eight32, FIRST>, grid, dim3(256), 0, st, a));
+  else SPION_CUDA_TRY(launch_after(k_prepare<Eight16, FIRST>, grid, dim3(256), 0, st, a));
   return SPION_OK;
 }
 // What the two passes over z have in common
-int logits_args(const spion_vocab_problem* p, const Layout& l, const Prep& prep, char* ws, Args* a, Maps* maps) {
+int logits_args(const spion_vocab_problem* p, const Layout& l, const Prep& prep, Args* a, Maps* maps) {
   *a = Args();
   a->n = prep.plan.head;
   a->products = l.planes == 1 ? 1 : 6;
@@ -1070,11 +1209,14 @@ int logits_args(const spion_vocab_problem* p, const Layout& l, const Prep& prep,
   a->chain = CHAIN;
   a->splits = 1;
   a->fp16 = p->type == SPION_F16;
+  a->direct_rows = l.direct ? (int)l.T : 0;
   a->plan = prep.plan, a->Tp = (int)l.Tp, a->k = (int)l.k;
-  a->bias2 = (const float*)(ws + l.bias2), a->c1 = prep.c1;
-  int rc = map_of(&maps->a, ws + l.xs, l.Kp, l.planes * l.Tp, l.Kp, 128);
+  a->bias2 = prep.bias2, a->c1 = prep.c1;
+  int rc = map_of(&maps->a, prep.xs, l.Kp, l.planes * l.Tp, l.Kp, 128);
   if (rc == SPION_OK)
-    rc = l.copy_w ? map_of(&maps->b, ws + l.w, l.Kp, l.planes * l.Vp, l.Kp, 128) : map_of(&maps->b, p->w, l.K, l.V, l.ldw, 128);
+    rc = l.copy_w ? map_of(&maps->b, prep.ws, l.Kp, l.planes * l.Vp, l.Kp, 128) : map_of(&maps->b, p->w, l.K, l.V, l.ldw, 128);
+  maps->x = maps->a;
+  if (rc == SPION_OK && l.direct) rc = map_of(&maps->x, p->x, l.K, l.T, p->ldx, 128);
   return rc;
 }
 
@@ -1113,20 +1255,23 @@ extern "C" int spion_vocab_loss_forward(const spion_vocab_problem* p, float* los
   if (loss == nullptr) return SPION_ERR_ARG;
   const cudaStream_t st = (cudaStream_t)cuda_stream;
   char* const ws = static_cast<char*>(workspace);
-  const Prep prep = prep_of(p, l, keep, ws);
-  float* const zt = (float*)(ws + l.zt);
-  const long long warps = std::max(tiles_of(l.T, CHUNK), tiles_of(l.Vp, 32 * 8));
-  SPION_CUDA_TRY(launch_after(k_flags, dim3((unsigned)std::min<long long>(tiles_of(warps, 8), 8 * sm_count())), dim3(256), 0, st, prep));
-  if ((rc = launch_gather<true>(p, l, prep, (uint16_t*)(ws + l.xs), p->reduction == 0 ? loss : nullptr, zt, st)) != SPION_OK) return rc;
-  if ((rc = launch_copy_w(p, l, (uint16_t*)(ws + l.w), st)) != SPION_OK) return rc;
+  Prep prep = prep_of(p, l, keep, ws);
+  prep.counts = l.self ? nullptr : (int*)(ws + l.counts), prep.q = (float*)(ws + l.q), prep.zt = (float*)(ws + l.zt);
+  prep.loss_rows = p->reduction == 0 ? loss : nullptr;
+  if (!l.self) SPION_CUDA_TRY(launch_after(k_flags, dim3((unsigned)tiles_of(tiles_of(l.T, CHUNK), prep.teacher ? 1 : 8)), dim3(256), 0, st, prep));
+  if ((rc = launch_prepare<true>(p, prep, st)) != SPION_OK) return rc;
   Args a;
   Maps maps;
-  if ((rc = logits_args(p, l, prep, ws, &a, &maps)) != SPION_OK) return rc;
+  if ((rc = logits_args(p, l, prep, &a, &maps)) != SPION_OK) return rc;
   const int tile = l.pair_z ? 256 : 128;
-  a.N = (int)l.V, a.part = (float2*)(ws + l.part), a.parts = (int)(2 * tiles_of(l.V, tile)), a.zt = zt;
+  a.N = (int)l.V, a.part = (float2*)(ws + l.part), a.parts = (int)(2 * tiles_of(l.V, tile)), a.zt = prep.zt;
   if ((rc = launch_gemm<LOGSUM>(l.pair_z, a, maps, tiles_of(l.T, tile) * tiles_of(l.V, tile), st)) != SPION_OK) return rc;
-  const Finish f = {prep.plan, (int)l.Tp, (int)l.k, a.part, a.parts, zt, loss, (float*)(ws + l.slot_loss), p->reduction};
-  SPION_CUDA_TRY(launch_after(k_finish, dim3((unsigned)std::min<long long>(tiles_of(l.T, 8), 4 * sm_count())), dim3(256), 0, st, f));
+  const Finish f = {prep.plan, (int)l.Tp, (int)l.k, a.part, a.parts, prep.zt, loss, (double*)(ws + l.cta_loss), p->reduction};
+  const int lanes = std::max<int>(a.parts, l.k) <= 16 ? 4 : std::max<int>(a.parts, l.k) <= 32 ? 8 : 32;
+  const dim3 grid((unsigned)std::min<long long>(tiles_of(l.T, 256 / lanes), std::min(4 * sm_count(), FINISH_CTAS)));
+  if (lanes == 4) SPION_CUDA_TRY(launch_after(k_finish<4>, grid, dim3(256), 0, st, f));
+  else if (lanes == 8) SPION_CUDA_TRY(launch_after(k_finish<8>, grid, dim3(256), 0, st, f));
+  else SPION_CUDA_TRY(launch_after(k_finish<32>, grid, dim3(256), 0, st, f));
   return SPION_OK;
 }
 
@@ -1143,40 +1288,46 @@ extern "C" int spion_vocab_loss_backward(const spion_vocab_problem* p, const flo
   const cudaStream_t st = (cudaStream_t)cuda_stream;
   char* const ws = static_cast<char*>(workspace);
   const Prep prep = prep_of(p, l, const_cast<void*>(keep), ws);
-  uint16_t *const xs = (uint16_t*)(ws + l.xs), *const G = (uint16_t*)(ws + l.g);
-  float* const coef = (float*)(ws + l.coef);
+  uint16_t* const G = (uint16_t*)(ws + l.g);
+  float* const unit = (float*)(ws + l.unit);
   const float gscale = p->type == SPION_F16 ? 8192.f : 1.f;
-  SPION_CUDA_TRY(launch_after(k_coef, dim3(1 + (unsigned)std::min<long long>(tiles_of(l.Vp, 1024), 2 * sm_count())), dim3(1024), 0, st, prep, g, p->reduction, 1.f / gscale, coef));
-  if ((rc = launch_gather<false>(p, l, prep, xs, nullptr, nullptr, st)) != SPION_OK) return rc;
-  if ((rc = launch_copy_w(p, l, (uint16_t*)(ws + l.w), st)) != SPION_OK) return rc;
+  if (p->reduction == 0) SPION_CUDA_TRY(launch_after(k_unit, dim3(1), dim3(1024), 0, st, prep.plan, g, unit));
+  if (!l.kept && (rc = launch_prepare<false>(p, prep, st)) != SPION_OK) return rc;
   Args z;
   Maps zm, xm, wm;
-  if ((rc = logits_args(p, l, prep, ws, &z, &zm)) != SPION_OK) return rc;
+  if ((rc = logits_args(p, l, prep, &z, &zm)) != SPION_OK) return rc;
   if ((rc = map_of(&xm.a, G, l.Gp, l.planes * l.Tp, l.Gp, 128)) != SPION_OK) return rc;
-  if ((rc = l.copy_w ? map_of(&xm.b, ws + l.w, l.Kp, l.planes * l.Vp, l.Kp, 64) : map_of(&xm.b, p->w, l.K, l.V, l.ldw, 64)) != SPION_OK) return rc;
+  if ((rc = l.copy_w ? map_of(&xm.b, prep.ws, l.Kp, l.planes * l.Vp, l.Kp, 64) : map_of(&xm.b, p->w, l.K, l.V, l.ldw, 64)) != SPION_OK) return rc;
+  xm.x = xm.a;
   if ((rc = map_of(&wm.a, G, l.Gp, l.planes * l.Tp, l.Gp, 64)) != SPION_OK) return rc;
-  if ((rc = map_of(&wm.b, xs, l.Kp, l.planes * l.Tp, l.Kp, 64)) != SPION_OK) return rc;
+  if ((rc = map_of(&wm.b, prep.xs, l.Kp, l.planes * l.Tp, l.Kp, 64)) != SPION_OK) return rc;
+  wm.x = wm.b;
+  if (l.direct && (rc = map_of(&wm.x, p->x, l.K, l.T, p->ldx, 64)) != SPION_OK) return rc;
   int dx_units = 0;
   if ((rc = l.pair_dx ? units_of<DX, true>(&dx_units) : units_of<DX, false>(&dx_units)) != SPION_OK) return rc;
   const int tz = l.pair_z ? 256 : 128, tx = l.pair_dx ? 256 : 128, tw = l.pair_dw ? 256 : 128;
-  z.g = p->reduction == 0 ? g : nullptr, z.coef = coef, z.G = G, z.ldg = l.Gp, z.gscale = gscale;
+  z.g = p->reduction == 0 ? g : nullptr, z.G = G, z.ldg = l.Gp, z.gscale = gscale;
+  z.coef = {p->reduction == 0 ? nullptr : g, unit, p->reduction == 1, prep.inv_tau / gscale};
   z.colsum = db != nullptr ? (float*)(ws + l.colsum) : nullptr;
-  int dx_chunks = 0;
+  const int dx_chunks = (int)tiles_of(std::min(l.Gp, l.V), BK);            // every piece's contraction is cut as the first one's: the parts are added piece by piece
+  const unsigned most = 8 * sm_count();
   for (long long c = 0; c < l.V; c += l.Gp) {
     const long long columns = std::min(l.Gp, l.V - c), padded = up(columns, PAD);
     z.col0 = (int)c, z.N = (int)padded;
     if ((rc = launch_gemm<GRAD>(l.pair_z, z, zm, tiles_of(l.T, tz) * tiles_of(padded, tz), st)) != SPION_OK) return rc;
     Args b = z;
-    b.col0 = (int)c;
     b.chain = l.planes == 3 ? CHAIN : LONG_CHAIN;
+    Leave out = {};
+    out.head = prep.plan.head, out.coef = z.coef;
     if (dx != nullptr) {
-      // every piece's contraction is cut as the first one's: the parts are added piece by piece
-      if (c == 0) dx_chunks = (int)tiles_of(columns, BK);
       Args d = b;
       d.N = (int)l.K, d.L = (int)columns, d.splits = 0, d.split_chunks = dx_chunks;
       d.plane_a = l.Tp, d.plane_b = l.Vp;
       d.out = (float*)(ws + l.dxp), d.ldo = l.Kp, d.add = c > 0;
       if ((rc = launch_gemm<DX>(l.pair_dx, d, xm, 0, st)) != SPION_OK) return rc;
+      if (c + l.Gp >= l.V)
+        out.j[0] = {prep.plan.slot, d.out, l.Kp, 0, tx, (int)tiles_of(l.K, tx), dx_units, dx_chunks, 0, dx, p->type, l.T, l.K,
+                    (unsigned)std::min<long long>(tiles_of(l.T * tiles_of(l.K, 8), 256), most)};
     }
     if (dw != nullptr) {
       Args d = b;
@@ -1185,19 +1336,13 @@ extern "C" int spion_vocab_loss_backward(const spion_vocab_problem* p, const flo
       d.out = (float*)(ws + l.dwp), d.ldo = l.Kp, d.add = 0;
       d.dw = l.dw_splits == 1 ? dw : nullptr, d.dw_type = p->type, d.K = l.K, d.V = (int)l.V;
       if ((rc = launch_gemm<DW>(l.pair_dw, d, wm, tiles_of(padded, tw) * tiles_of(l.K, tw) * l.dw_splits, st)) != SPION_OK) return rc;
-      if (l.dw_splits > 1) {
-        const Join j = {prep.plan.head, nullptr, d.out, l.Kp, l.dw_splits, tw, 0, 0, 0, up(padded, tw), coef,
-                        static_cast<char*>(dw) + c * l.K * type_size(p->type), p->type, columns, l.K};
-        SPION_CUDA_TRY(launch_after(k_join, dim3((unsigned)std::min<long long>(tiles_of(columns * tiles_of(l.K, 8), 256), 8 * sm_count())), dim3(256), 0, st, j));
-      }
+      if (l.dw_splits > 1)
+        out.j[1] = {nullptr, d.out, l.Kp, l.dw_splits, tw, 0, 0, 0, up(padded, tw), static_cast<char*>(dw) + c * l.K * type_size(p->type), p->type, columns, l.K,
+                    (unsigned)std::min<long long>(tiles_of(columns * tiles_of(l.K, 8), l.dw_splits >= 8 ? 32 : 256), most)};
     }
-    if (db != nullptr)
-      SPION_CUDA_TRY(launch_after(k_db, dim3((unsigned)tiles_of(columns, 32)), dim3(256), 0, st, (const int*)prep.plan.head, (const float*)z.colsum, l.Gp, (int)columns,
-                                  (const float*)coef, (void*)(static_cast<char*>(db) + c * type_size(db_type)), db_type));
-  }
-  if (dx != nullptr) {
-    const Join j = {prep.plan.head, prep.plan.slot, (const float*)(ws + l.dxp), l.Kp, 0, tx, (int)tiles_of(l.K, tx), dx_units, dx_chunks, 0, coef, dx, p->type, l.T, l.K};
-    SPION_CUDA_TRY(launch_after(k_join, dim3((unsigned)std::min<long long>(tiles_of(l.T * tiles_of(l.K, 8), 256), 8 * sm_count())), dim3(256), 0, st, j));
+    if (db != nullptr) out.b = {z.colsum, l.Gp, (int)columns, static_cast<char*>(db) + c * type_size(db_type), db_type, (unsigned)tiles_of(columns, 32)};
+    const unsigned ctas = out.j[0].ctas + out.j[1].ctas + out.b.ctas;
+    if (ctas > 0) SPION_CUDA_TRY(launch_after(k_out, dim3(ctas), dim3(256), 0, st, out));
   }
   return SPION_OK;
 }

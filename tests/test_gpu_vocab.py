@@ -218,7 +218,7 @@ def test_strides_offsets_shapes_and_label_types(dtype):
     empty = torch.empty(0, 72, device="cuda", dtype=dtype, requires_grad=True)
     none = torch.empty(0, dtype=torch.long, device="cuda")
     assert linear_cross_entropy(empty, w, none, b, reduction="none").shape == (0,)
-    assert bool(linear_cross_entropy(empty, w, none, b).isnan()) and float(linear_cross_entropy(empty, w, none, b, reduction="sum")) == 0.0
+    assert bool(linear_cross_entropy(empty, w, none, b).isnan()) and bool(linear_cross_entropy(empty, w, none, b, reduction="sum") == 0)
     w2 = w.detach().requires_grad_()
     dw, dx = torch.autograd.grad(linear_cross_entropy(empty, w2, none, b, reduction="sum"), (w2, empty))
     assert bool((dw == 0).all()) and dx.shape == (0, 72)
@@ -375,6 +375,21 @@ def test_captured_replayed_and_on_two_streams():
             c = step(*second, labels2)
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(a, want)) and all(torch.equal(p, q) for p, q in zip(c, want2))
+
+
+def test_a_first_backward_of_a_process():
+    """On the autograd engine's thread, which has not used the device yet."""
+    import os
+    import subprocess
+    import sys
+    code = ("import torch\nfrom spion_b200.vocab import linear_cross_entropy\n"
+            "x = torch.randn(200, 64, device='cuda', requires_grad=True)\nw = torch.randn(300, 64, device='cuda', requires_grad=True)\n"
+            "l = torch.zeros(200, dtype=torch.long, device='cuda')\n"
+            "g = torch.autograd.grad(linear_cross_entropy(x, w, l), (x, w), torch.tensor(1.0, device='cuda'))\n"
+            "torch.cuda.synchronize()\nassert all(bool(t.isfinite().all()) for t in g)\nprint('done')\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
 
 
 def test_autocast_and_the_module():
