@@ -30,6 +30,12 @@
 using namespace tc;
 using namespace rows;
 
+#ifndef SPION_GROUP
+#define SPION_GROUP 8
+#endif
+#ifndef SPION_PIECE
+#define SPION_PIECE 512ll
+#endif
 namespace {
 
 // Set by a bounded wait that gave up (see g_lin_status in linear.cu); results after it are NaN until it has been reported.
@@ -58,7 +64,7 @@ struct Plan {
 };
 struct Source {
   const void* p; int type; long long ld;
-  int K, Kp, fast;          // fast: rows on 16-byte boundaries (32 in fp32), whole pieces of 8
+  int K, Kp, fast;          // 2: rows on 16-byte boundaries, whole pieces of 8; 1: rows of pairs, on boundaries of one; 0: any
 };
 struct Prep {
   Plan plan;
@@ -67,7 +73,7 @@ struct Prep {
   long long ignore;
   float inv_tau;
   int T, Tp, V, k;
-  int* counts;              // [chunks of CHUNK rows], or null: each CTA counts for itself
+  int* counts;              // [chunks], or null: each CTA counts for itself
   float* q;                 // [T, k]
   const void* bias; int bias_type;
   float* bias2;             // [Vp] b log2(e) / tau; -inf behind the vocabulary
@@ -79,9 +85,10 @@ struct Prep {
   int direct;               // x can be read as it lies, if all rows count
   float* loss_rows;         // [T] or null: zeros where a row does not count
   float* zt;                // [k][Tp]
-  unsigned row_ctas, slices, w_ctas;                     // CTAs of rows: chunks x column slices; then those of w, then those of the bias
+  int chunk;                // rows of a CTA, a multiple of 32; of BLOCK where there are more
+  unsigned row_ctas, slices, w_ctas;                     // CTAs of rows: x column slices; then those of w, then those of the bias
 };
-constexpr int CHUNK = 64, SELF = 4096;                    // rows of a chunk; labels (or logits) up to which each CTA counts for itself
+constexpr int BLOCK = 128, SELF = 4096;                   // rows that a CTA lists at a time; labels (or logits) up to which each CTA counts for itself
 
 // A warp: weights of the targets of eight rows (from t0 on, below `end`).  Bits of those that have one.
 template <int WORDS> __device__ __forceinline__ unsigned teacher_weights(const Prep& a, int t0, int end, int lane) {
@@ -131,23 +138,27 @@ __global__ void __launch_bounds__(256) k_flags(const __grid_constant__ Prep a) {
   __shared__ int part[8];
   next_may_start();
   wait_for_kernel_before();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = (a.T + CHUNK - 1) / CHUNK;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = (a.T + a.chunk - 1) / a.chunk;
   if (a.teacher == nullptr) {
     const int c = blockIdx.x * 8 + warp;
     if (c >= chunks) return;
     int n = 0;
-#pragma unroll
-    for (int i = 0; i < CHUNK; i += 32) {
-      const int t = c * CHUNK + i + lane;
+#pragma unroll 4
+    for (int i = 0; i < a.chunk; i += 32) {
+      const long long t = (long long)c * a.chunk + i + lane;
       n += __popc(__ballot_sync(0xffffffffu, t < a.T && a.labels[t] != a.ignore));
     }
     if (lane == 0) a.counts[c] = n;
     return;
   }
-  const int t0 = blockIdx.x * CHUNK + 8 * warp;
-  const unsigned found = teacher_weights(a, t0, a.T, lane);
-  if (lane < 8 && t0 + lane < a.T) a.plan.slot[t0 + lane] = found >> lane & 1 ? 0 : -1;
-  if (lane == 0) part[warp] = __popc(found);
+  int mine = 0;
+  const int first = blockIdx.x * a.chunk, end = min(a.T, first + a.chunk);
+  for (int t0 = first + 8 * warp; t0 < end; t0 += 64) {
+    const unsigned found = teacher_weights(a, t0, end, lane);
+    if (lane < 8 && t0 + lane < end) a.plan.slot[t0 + lane] = found >> lane & 1 ? 0 : -1;
+    mine += __popc(found);
+  }
+  if (lane == 0) part[warp] = mine;
   __syncthreads();
   if (threadIdx.x == 0) {
     int n = 0;
@@ -162,11 +173,18 @@ struct Eight16 {
   uint4 w;
   __device__ __forceinline__ void load(const Source& s, long long row, int c) {
     const __half* const from = static_cast<const __half*>(s.p) + row * s.ld + c;
-    if (s.fast) {
+    if (s.fast == 2) {
       w = c < s.K ? *reinterpret_cast<const uint4*>(from) : make_uint4(0, 0, 0, 0);
       return;
     }
     uint32_t u[4] = {0, 0, 0, 0};
+    if (s.fast == 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + 2 * i < s.K) u[i] = *reinterpret_cast<const uint32_t*>(from + 2 * i);
+      w = make_uint4(u[0], u[1], u[2], u[3]);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (c + i < s.K) u[i >> 1] |= (uint32_t) * reinterpret_cast<const uint16_t*>(from + i) << (16 * (i & 1));
@@ -180,7 +198,16 @@ struct Eight32 {
   __device__ __forceinline__ void load(const Source& s, long long row, int c) {
     const float* const from = static_cast<const float*>(s.p) + row * s.ld + c;
     zero();
-    if (s.fast) {
+    if (s.fast == 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + 2 * i < s.K) {
+          const float2 v = *reinterpret_cast<const float2*>(from + 2 * i);
+          f[2 * i] = v.x, f[2 * i + 1] = v.y;
+        }
+      return;
+    }
+    if (s.fast == 2) {
       if (c >= s.K) return;
       const float4 u = reinterpret_cast<const float4*>(from)[0], v = reinterpret_cast<const float4*>(from)[1];
       f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w, f[4] = v.x, f[5] = v.y, f[6] = v.z, f[7] = v.w;
@@ -216,7 +243,7 @@ template <class E, bool FIRST> __global__ void __launch_bounds__(256) k_prepare(
   constexpr int PARTS = std::is_same<E, Eight32>::value ? 3 : 1;
   next_may_start();
   wait_for_kernel_before();
-  __shared__ int list[CHUNK], part[2][8], here;
+  __shared__ int list[BLOCK], part[2][8], here_;
   __shared__ unsigned flags[SELF / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (blockIdx.x >= a.row_ctas + a.w_ctas) {
@@ -239,12 +266,30 @@ template <class E, bool FIRST> __global__ void __launch_bounds__(256) k_prepare(
   const Source& s = a.x;
   const int chunk = blockIdx.x / a.slices, slice = blockIdx.x - chunk * a.slices;
   const long long plane = (long long)a.Tp * s.Kp;
-  const int pieces = s.Kp / 8;
-  int first, n;
+  const int pieces = s.Kp / 8, per = (pieces + a.slices - 1) / a.slices, p0 = slice * per, mine = max(0, min(pieces, p0 + per) - p0);
+  auto copy = [&](int first, int here) {                   // the listed rows' columns of this slice, four pieces a thread under way
+    const int all = here * mine;
+    for (int i0 = threadIdx.x; i0 < all; i0 += 4 * 256) {
+      E e[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + 256 * u, r = i / mine;
+        if (i < all) e[u].load(s, list[r], 8 * (p0 + i - r * mine));
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + 256 * u, r = i / mine;
+        if (i < all) e[u].store(a.xs + (long long)(first + r) * s.Kp + 8 * (p0 + i - r * mine), plane);
+      }
+    }
+  };
+  const int chunk_end = min(a.T, (chunk + 1) * a.chunk);
+  int n;
   if constexpr (FIRST) {
-    const int chunks = (a.T + CHUNK - 1) / CHUNK;
+    const int chunks = (a.T + a.chunk - 1) / a.chunk;
     int before = 0, all = 0;
     if (a.counts != nullptr) {
+#pragma unroll 4
       for (int c = threadIdx.x; c < chunks; c += 256) {
         const int m = a.counts[c];
         all += m;
@@ -261,72 +306,66 @@ template <class E, bool FIRST> __global__ void __launch_bounds__(256) k_prepare(
       __syncthreads();
       for (int i = threadIdx.x; i < words; i += 256) {
         all += __popc(flags[i]);
-        if (i < chunk * (CHUNK / 32)) before += __popc(flags[i]);
+        if (i < chunk * (a.chunk / 32)) before += __popc(flags[i]);
       }
+      if (slice == 0 && a.teacher != nullptr)
+        for (int t0 = chunk * a.chunk + 8 * warp; t0 < chunk_end; t0 += 64) teacher_weights(a, t0, chunk_end, lane);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o), all += __shfl_xor_sync(0xffffffffu, all, o);
     if (lane == 0) part[0][warp] = before, part[1][warp] = all;
     __syncthreads();
-    first = n = 0;
+    int first = 0;
+    n = 0;
 #pragma unroll
     for (int w = 0; w < 8; ++w) first += part[0][w], n += part[1][w];
-    if (warp == 0) {
-      int at = 0;
-#pragma unroll
-      for (int i = 0; i < CHUNK; i += 32) {
-        const int t = chunk * CHUNK + i + lane;
-        const bool counts = t < a.T && (a.counts == nullptr ? flags[t >> 5] >> (t & 31) & 1 : a.teacher ? a.plan.slot[t] != -1 : a.labels[t] != a.ignore);
-        const unsigned who = __ballot_sync(0xffffffffu, counts);
-        const int mine = at + __popc(who & ((1u << lane) - 1));
-        if (counts) list[mine] = t;
-        if (slice == 0 && t < a.T) {
-          // (other slices of the chunk may read a slot before or after this: that it is -1 or not stays)
-          a.plan.slot[t] = counts ? first + mine : -1;
-          if (a.loss_rows != nullptr && !counts) a.loss_rows[t] = 0.f;
-          if (counts) a.plan.row[first + mine] = t;
+    const bool in_place = a.direct && n == a.T;
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.plan.head[0] = n, a.plan.head[1] = 0;
+    for (int t0 = chunk * a.chunk; t0 < chunk_end; t0 += BLOCK) {
+      const int end = min(chunk_end, t0 + BLOCK);
+      if (warp == 0) {
+        int at = 0;
+        for (int i = t0; i < end; i += 32) {
+          const int t = i + lane;
+          const bool counts = t < end && (a.counts == nullptr ? flags[t >> 5] >> (t & 31) & 1 : a.teacher ? a.plan.slot[t] != -1 : a.labels[t] != a.ignore);
+          const unsigned who = __ballot_sync(0xffffffffu, counts);
+          const int place = at + __popc(who & ((1u << lane) - 1));
+          if (counts) list[place] = t;
+          if (slice == 0 && t < end) {
+            // (other slices of the chunk may read a slot before or after this: that it is -1 or not stays)
+            a.plan.slot[t] = counts ? first + place : -1;
+            if (a.loss_rows != nullptr && !counts) a.loss_rows[t] = 0.f;
+            if (counts) a.plan.row[first + place] = t;
+          }
+          at += __popc(who);
         }
-        at += __popc(who);
+        if (lane == 0) here_ = at;
       }
-      if (lane == 0) {
-        here = at;
-        if (blockIdx.x == 0) a.plan.head[0] = n, a.plan.head[1] = 0;
-      }
+      __syncthreads();
+      const int here = here_;
+      if (slice == 0)
+        for (int i = threadIdx.x; i < here * a.k; i += 256) {
+          const int r = i / a.k, j = i - r * a.k;
+          const long long from = (long long)list[r] * a.k + j, to = (long long)j * a.Tp + first + r, v = a.labels[from];
+          const float q = a.teacher ? a.q[from] : 1.f;
+          a.plan.target[to] = a.teacher && (v == -1 || q == 0.f) ? -1 : v < 0 || v >= a.V ? -2 : (int)v;
+          if (a.teacher) a.plan.q[to] = v == -1 ? 0.f : q;
+          a.zt[to] = not_a_number();                        // of a target that no tile has
+        }
+      if (!in_place) copy(first, here);
+      first += here;
+      __syncthreads();
     }
-    if (slice == 0 && a.counts == nullptr && a.teacher != nullptr) teacher_weights(a, chunk * CHUNK + 8 * warp, a.T, lane);
-    __syncthreads();
-    if (slice == 0)
-      for (int i = threadIdx.x; i < here * a.k; i += 256) {
-        const int r = i / a.k, j = i - r * a.k;
-        const long long from = (long long)list[r] * a.k + j, to = (long long)j * a.Tp + first + r, v = a.labels[from];
-        const float q = a.teacher ? a.q[from] : 1.f;
-        a.plan.target[to] = a.teacher && (v == -1 || q == 0.f) ? -1 : v < 0 || v >= a.V ? -2 : (int)v;
-        if (a.teacher) a.plan.q[to] = v == -1 ? 0.f : q;
-        a.zt[to] = not_a_number();                          // of a target that no tile has
-      }
+    if (in_place) return;
   } else {
     n = a.plan.head[0];
-    first = chunk * CHUNK;
-    if (threadIdx.x < CHUNK && first + (int)threadIdx.x < n) list[threadIdx.x] = a.plan.row[first + threadIdx.x];
-    if (threadIdx.x == 0) here = max(0, min(CHUNK, n - first));
-    __syncthreads();
-  }
-  if (a.direct && n == a.T) return;
-  const int per = (pieces + a.slices - 1) / a.slices, p0 = slice * per, mine = min(pieces, p0 + per) - p0;
-  if (mine > 0) {
-    const int all = here * mine;
-    for (int i0 = threadIdx.x; i0 < all; i0 += 4 * 256) {
-      E e[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = i0 + 256 * u, r = i / mine;
-        if (i < all) e[u].load(s, list[r], 8 * (p0 + i - r * mine));
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = i0 + 256 * u, r = i / mine;
-        if (i < all) e[u].store(a.xs + (long long)(first + r) * s.Kp + 8 * (p0 + i - r * mine), plane);
-      }
+    if (a.direct && n == a.T) return;
+    for (int first = chunk * a.chunk; first < min(n, (chunk + 1) * a.chunk); first += BLOCK) {
+      const int here = min(BLOCK, min(n, (chunk + 1) * a.chunk) - first);
+      for (int i = threadIdx.x; i < here; i += 256) list[i] = a.plan.row[first + i];
+      __syncthreads();
+      copy(first, here);
+      __syncthreads();
     }
   }
   // zeros up to the end of the last tile: what it holds is multiplied with zeros
@@ -339,12 +378,16 @@ template <class E, bool FIRST> __global__ void __launch_bounds__(256) k_prepare(
 // ------------------------------------------------------------------------------------------------ the four products
 enum Mode { LOGSUM, GRAD, DX, DW };
 constexpr int BK = 64;                                    // elements of the contraction in a chunk: 128 bytes
-constexpr int EPI = 8, THREADS = 32 * (2 + EPI);
-constexpr int STAGES = 6;
 constexpr uint32_t HALF = 128 * BK * 2, STAGE = 2 * HALF;
-constexpr uint32_t BARS = STAGES * STAGE, STAGED = BARS + 16 * STAGES + 64;      // STAGED: 32 x 32 results a writing warp, rows of 33 (DW)
-template <int MODE> constexpr uint32_t SMEM = MODE == DW ? STAGED + EPI * 32 * 33 * 4 : STAGED;
-static_assert(SMEM<DW> <= 232448, "shared memory of a multiprocessor");
+// PAIR: two CTAs of a cluster share a tile of 256 x 256; else tiles of 128 x 128.  A thread that writes has 64 columns: what it does with them is a chain of latencies, and four
+// warps a scheduler hide more of each other's than two with 128 columns each do (8192 x 64 to 64000, k_gemm<LOGSUM> 663 us, so SPAN).
+template <int MODE, bool PAIR> struct Shape {
+  static constexpr int BN = PAIR ? 256 : 128, TILE = PAIR ? 256 : 128, W = 64;         // columns and rows of a tile; columns of a writing thread
+  static constexpr int EPI = 4 * BN / W, THREADS = 32 * (2 + EPI), STAGES = 6;
+  static constexpr uint32_t BARS = STAGES * STAGE, STAGED = BARS + 16 * STAGES + 96;   // STAGED: 32 x 16 results a writing warp, rows of 17 (DW)
+  static constexpr uint32_t SMEM = MODE == DW ? STAGED + EPI * 32 * 17 * 4 : STAGED;
+};
+static_assert(Shape<DW, true>::SMEM <= 232448 && Shape<DW, false>::SMEM <= 232448, "shared memory of a multiprocessor");
 
 // What the products with G are multiplied with.  Rows with a g each: it comes from k_unit.
 struct Coef {
@@ -430,9 +473,20 @@ __device__ __forceinline__ void parts_of(int products, int i, int& a, int& b) {
 
 // What a launch works on, the same in all its warps and (for DX) in the kernel that joins the sums
 struct Work { int tiles_m, tiles_n, splits, chunks, per; };
+// Parts of the contraction: the number that leaves the fewest units idle in the last round of tiles, a fiftieth less for each part more (its sums are written and read
+// once more), eight at most and eight rounds.  8192 x 2048 from 16384 columns, 256 tiles on 74 pairs: one part 386 us, two 355.
 __host__ __device__ __forceinline__ int split_by_tiles(int tiles, int units, int chunks) {
-  const int s = tiles > 0 ? units / tiles : 1;
-  return s < 1 ? 1 : s > chunks ? (chunks < 1 ? 1 : chunks) : s;
+  int best = 1, score = 0;
+  for (int s = 1; s <= 8 && tiles > 0 && (s == 1 || (tiles * s <= 8 * units && 4 * s <= chunks)); ++s) {
+    const int rounds = (tiles * s + units - 1) / units, now = (int)(1000ll * tiles * s * (51 - s) / (50ll * rounds * units));
+    if (now > score) best = s, score = now;
+  }
+  return best;
+}
+// ... and of many: as many as there are units for each tile
+__host__ __device__ __forceinline__ int split_by_units(int tiles, int units, int chunks) {
+  const int s = units / (tiles > 0 ? tiles : 1), most = chunks / 4;
+  return s > most ? (most > 0 ? most : 1) : s > 0 ? s : 1;
 }
 __device__ __forceinline__ Work work_of(const Args& a, int n, int tile_m, int tile_n, int units) {
   Work w;
@@ -444,14 +498,15 @@ __device__ __forceinline__ Work work_of(const Args& a, int n, int tile_m, int ti
   return w;
 }
 // Tiles in groups of 8 rows of tiles, column by column inside a group: the CTAs that run at a time share their operands in L2.
-__device__ __forceinline__ void item_at(const Work& w, int i, int& s, int& m, int& n, int& c0, int& c1) {
+template <class Wk> __device__ __forceinline__ void item_at(const Wk& w, int i, int& s, int& m, int& n, int& c0, int& c1) {
   const int tiles = w.tiles_m * w.tiles_n;
   s = i / tiles;
   i -= s * tiles;
-  const int per = 8 * w.tiles_n, group = i / per, rows_here = min(8, w.tiles_m - 8 * group), j = i - group * per;
+  const int per = SPION_GROUP * w.tiles_n, group = i / per, rows_here = min(SPION_GROUP, (int)w.tiles_m - SPION_GROUP * group), j = i - group * per;
   n = j / rows_here;
-  m = 8 * group + j - n * rows_here;
-  c0 = min(s * w.per, w.chunks), c1 = min(c0 + w.per, w.chunks);
+  m = SPION_GROUP * group + j - n * rows_here;
+  const int chunks = w.chunks, share = w.per;
+  c0 = min(s * share, chunks), c1 = min(c0 + share, chunks);
 }
 
 __device__ __forceinline__ void st_v8(void* p, const uint32_t (&r)[8]) {
@@ -464,88 +519,122 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, int fp16) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Targets of a row among the columns c .. c + 31, of those whose bits are set
-template <class F> __device__ __forceinline__ void each_target(const Args& a, const uint32_t (&hits)[MAX_TARGETS / 32], int slot, int c, F f) {
+// What a writing thread knows of its row before the sums are there: it is read while they are formed
+struct Row {
+  bool in;                  // the row counts
+  int slot, found;          // targets among the thread's columns: how many,
+  uint32_t two;             // and of the first two the column and the target, a byte each
+  float lse, r;
+};
+// f(offset, target) of every target among the columns g .. g + 31 of the thread's
+template <class F> __device__ __forceinline__ void each_target(const Args& a, const Row& row, int c, int g, F f) {
 #pragma unroll
-  for (int w = 0; w < MAX_TARGETS / 32; ++w) {
-    uint32_t h = hits[w];
-    while (h) {
-      const int j = 32 * w + __ffs(h) - 1;
-      h &= h - 1;
-      const int off = a.plan.target[(long long)j * a.Tp + slot] - c;
-      if ((unsigned)off < 32u) f(j, off);
+  for (int i = 0; i < 2; ++i) {
+    const int off = (int)(row.two >> (16 * i) & 0xff) - g;
+    if (row.found > i && (unsigned)off < 32u) f(off, (int)(row.two >> (16 * i + 8) & 0xff));
+  }
+  if (row.found > 2) {                                     // seldom: all over again, without those two
+    for (int j = (int)(row.two >> 24) + 1; j < a.k; ++j) {
+      const int off = a.plan.target[(long long)j * a.Tp + row.slot] - c - g;
+      if ((unsigned)off < 32u) f(off, j);
     }
   }
 }
+template <int MODE, int W> __device__ __forceinline__ Row row_of(const Args& a, int n, int row, int c) {
+  Row r = {};
+  if (MODE != LOGSUM && MODE != GRAD) return r;
+  r.in = row < n;
+  r.slot = r.in ? row : 0;
+  r.lse = INFINITY;
+  if (r.in) {
+    const int* const target = a.plan.target + r.slot;
+    for (int j0 = 0; j0 < a.k; j0 += 16) {                 // sixteen loads under way: one after another they are 0.25 us each
+      int t[16];
+#pragma unroll
+      for (int u = 0; u < 16; ++u) t[u] = j0 + u < a.k ? target[(long long)(j0 + u) * a.Tp] : -1;
+#pragma unroll
+      for (int u = 0; u < 16; ++u) {
+        const int off = t[u] - c;
+        if ((unsigned)off < (unsigned)W && t[u] >= 0) {
+          if (r.found < 2) r.two |= (uint32_t)(off | (j0 + u) << 8) << (16 * r.found);
+          ++r.found;
+        }
+      }
+    }
+    if (MODE == GRAD) {
+      r.lse = a.plan.lse[r.slot];
+      r.r = (a.g ? a.g[a.plan.row[r.slot]] * a.coef.unit[1] : 1.f) * a.gscale;
+    }
+  }
+  return r;
+}
 
-// What a thread does with its sums: row `row` of D, columns col .. col + W - 1 (W = BN / 2)
-template <int MODE, int W> __device__ __forceinline__ void epilogue(const Args& a, const Work& w, float (&acc)[W], int n, int s, int row, int col, int tile_m, int part, float* stage) {
+// What a thread does with its sums: row `row` of D, columns col .. col + W - 1
+template <int MODE, int W, bool THREE> __device__ __forceinline__ void epilogue(const Args& a, int out_row, float (&acc)[W / 32][32], const Row& me, int n, int row, int col, int part, float* stage) {
   const int lane = threadIdx.x & 31;
   if constexpr (MODE == LOGSUM || MODE == GRAD) {
-    const bool in = row < n;
-    const int slot = in ? row : 0, c = a.col0 + col;      // of the vocabulary
-    uint32_t hits[MAX_TARGETS / 32] = {};
-    if (in)
-#pragma unroll
-      for (int i = 0; i < MAX_TARGETS / 32; ++i)
-        for (int j = 32 * i; j < min(a.k, 32 * i + 32); ++j)
-          if ((unsigned)(a.plan.target[(long long)j * a.Tp + slot] - c) < (unsigned)W) hits[i] |= 1u << (j & 31);
+    const int slot = me.slot, c = a.col0 + col;           // of the vocabulary
 #pragma unroll
     for (int g = 0; g < W; g += 4) {
       const float4 b = *reinterpret_cast<const float4*>(a.bias2 + c + g);
-      acc[g] = fmaf(acc[g], a.c1, b.x), acc[g + 1] = fmaf(acc[g + 1], a.c1, b.y);
-      acc[g + 2] = fmaf(acc[g + 2], a.c1, b.z), acc[g + 3] = fmaf(acc[g + 3], a.c1, b.w);
+      acc[g / 32][g % 32] = fmaf(acc[g / 32][g % 32], a.c1, b.x), acc[(g + 1) / 32][(g + 1) % 32] = fmaf(acc[(g + 1) / 32][(g + 1) % 32], a.c1, b.y);
+      acc[(g + 2) / 32][(g + 2) % 32] = fmaf(acc[(g + 2) / 32][(g + 2) % 32], a.c1, b.z), acc[(g + 3) / 32][(g + 3) % 32] = fmaf(acc[(g + 3) / 32][(g + 3) % 32], a.c1, b.w);
     }
     if constexpr (MODE == LOGSUM) {
       float top = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int g = 0; g < W; ++g) top = fmaxf(top, acc[g]);
+      for (int g = 0; g < W; ++g) top = fmaxf(top, acc[g / 32][g % 32]);
 #pragma unroll
       for (int g = 0; g < W; g += 32)
-        each_target(a, hits, slot, c + g, [&](int j, int off) {
+        each_target(a, me, c, g, [&](int off, int j) {
           float z = 0.f;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) z = e == off ? acc[g + e] : z;
+          for (int e = 0; e < 32; ++e) z = e == off ? acc[(g + e) / 32][(g + e) % 32] : z;
           a.zt[(long long)j * a.Tp + slot] = z;
         });
       const float from = top == -INFINITY ? 0.f : top;
 #pragma unroll
-      for (int g = 0; g < W; ++g) sum += ex2(acc[g] - from);
-      if (in) a.part[(long long)row * a.parts + part] = make_float2(top, sum);
+      for (int g = 0; g < W; ++g) sum += ex2(acc[g / 32][g % 32] - from);
+      if (me.in) a.part[(long long)row * a.parts + part] = make_float2(top, sum);
     } else {
-      float lse = 0.f, r = 0.f;
-      if (in) {
-        lse = a.plan.lse[slot];
-        r = a.g ? a.g[a.plan.row[slot]] * a.coef.unit[1] : 1.f;
-        r *= a.gscale;
-      }
+      const float lse = me.lse, r = me.r;
 #pragma unroll
       for (int g = 0; g < W; g += 32) {
-        float v[32];
+        float (&v)[32] = acc[g / 32];                      // in place: there is no room for another 32
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = in ? ex2(acc[g + e] - lse) * r : 0.f;
-        each_target(a, hits, slot, c + g, [&](int j, int off) {
+        for (int e = 0; e < 32; ++e) v[e] = ex2(v[e] - lse) * r;      // zeros of rows that do not count: their lse is inf
+        each_target(a, me, c, g, [&](int off, int j) {
           const float q = (a.plan.q ? a.plan.q[(long long)j * a.Tp + slot] : 1.f) * r;
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] -= e == off ? q : 0.f;
         });
         uint16_t* const to = a.G + (long long)row * a.ldg + col + g;
-        float left[32];
+        if constexpr (!THREE) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) left[e] = v[e];
-        const int planes = a.products == 1 ? 1 : 3;
-        for (int p = 0; p < planes; ++p) {
-          uint32_t u[16];
+          for (int h = 0; h < 2; ++h) {
+            uint32_t out[8];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) u[e] = pack2(left[2 * e], left[2 * e + 1], a.fp16);
-          uint32_t lo[8], hi[8];
+            for (int e = 0; e < 8; ++e) out[e] = pack2(v[16 * h + 2 * e], v[16 * h + 2 * e + 1], a.fp16);
+            st_v8(to + 16 * h, out);
+          }
+        } else {                                          // sixteen columns at a time, part by part
+          const long long plane = (long long)a.Tp * a.ldg;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) lo[e] = u[e], hi[e] = u[8 + e];
-          st_v8(to + p * (long long)a.Tp * a.ldg, lo);
-          st_v8(to + p * (long long)a.Tp * a.ldg + 16, hi);
-          if (planes == 1) break;
+          for (int h = 0; h < 2; ++h) {
+            float left[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) left[2 * e] -= bf16_lo(u[e]), left[2 * e + 1] -= bf16_hi(u[e]);
+            for (int e = 0; e < 16; ++e) left[e] = v[16 * h + e];
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+              uint32_t out[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                out[e] = pack_bf16(left[2 * e], left[2 * e + 1]);
+                left[2 * e] -= bf16_lo(out[e]), left[2 * e + 1] -= bf16_hi(out[e]);
+              }
+              st_v8(to + p * plane + 16 * h, out);
+            }
+          }
         }
         if (a.colsum != nullptr) {                        // over the warp's 32 rows: lane l ends with column l
 #pragma unroll
@@ -571,7 +660,7 @@ template <int MODE, int W> __device__ __forceinline__ void epilogue(const Args& 
           if (col + g >= a.K) continue;
           float f[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = acc[g + e] * alpha;
+          for (int e = 0; e < 8; ++e) f[e] = acc[(g + e) / 32][(g + e) % 32] * alpha;
           const long long at = (long long)v * a.K + col + g;
           if (a.dw_type == SPION_F32) Out<float, 8>::store(static_cast<float*>(a.dw) + at, f);
           else if (a.dw_type == SPION_BF16) Out<__nv_bfloat16, 8>::store(static_cast<__nv_bfloat16*>(a.dw) + at, f);
@@ -581,26 +670,26 @@ template <int MODE, int W> __device__ __forceinline__ void epilogue(const Args& 
       }
       // rows that start anywhere: lanes side by side along each (one row a lane: 10007 rows of 770 fp16 126 us, so 31)
 #pragma unroll
-      for (int g = 0; g < W; g += 32) {
+      for (int g = 0; g < W; g += 16) {
         __syncwarp();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) stage[33 * lane + e] = acc[g + e] * alpha;
+        for (int e = 0; e < 16; ++e) stage[17 * lane + e] = acc[(g + e) / 32][(g + e) % 32] * alpha;
         __syncwarp();
-        const int c = col + g + lane, v0 = v - lane;
+        const int c = col + g + (lane & 15), v0 = v - lane;
         if (c < a.K)
 #pragma unroll 4
-          for (int r = 0; r < 32; ++r)
-            if (v0 + r < a.V) store_any(a.dw, a.dw_type, (long long)(v0 + r) * a.K + c, stage[33 * r + lane]);
+          for (int r = lane >> 4; r < 32; r += 2)
+            if (v0 + r < a.V) store_any(a.dw, a.dw_type, (long long)(v0 + r) * a.K + c, stage[17 * r + (lane & 15)]);
       }
       return;
     }
-    float* const to = a.out + ((long long)s * w.tiles_m * tile_m + row) * a.ldo + col;
+    float* const to = a.out + (long long)out_row * a.ldo + col;
 #pragma unroll
     for (int g = 0; g < W; g += 8) {
       if (col + g >= a.ldo) continue;
       float f[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = acc[g + e];
+      for (int e = 0; e < 8; ++e) f[e] = acc[(g + e) / 32][(g + e) % 32];
       if (a.add) {
         Piece<float, 8> was;
         was.load(to + g);
@@ -612,17 +701,19 @@ template <int MODE, int W> __device__ __forceinline__ void epilogue(const Args& 
   }
 }
 
+// THREE: G in three parts (GRAD).
 // Warp 0 loads, warp 1 multiplies, the others take the sums.  Every wait is bounded; whoever gives up reports it and leaves, and so do all that wait for it; the warps
 // that write go on with NaN.  PAIR: two CTAs of a cluster share a tile of 256 x 256, each brings 128 rows of either operand and holds 128 rows of the sums; the first one's warp 1
 // multiplies for both (see k_lin8 in linear_e4m3.cu, whose scheme this is).  Else tiles of 128 x 128.
 // Operands whose contraction runs along memory (K-major: x and W in z, G in dx) come as one box of 128 rows x 64; those whose contraction runs across it (MN-major: W in dx, G and x
 // in dW) as two boxes of 64 rows x 64.
-template <int MODE, bool PAIR> __global__ void __launch_bounds__(THREADS, 1) k_gemm(const __grid_constant__ Args a, const __grid_constant__ Maps maps) {
-  constexpr int BN = PAIR ? 256 : 128, TILE = PAIR ? 256 : 128, W = BN / 2;
+template <int MODE, bool PAIR, bool THREE> __global__ void __launch_bounds__(Shape<MODE, PAIR>::THREADS, 1) k_gemm(const __grid_constant__ Args a, const __grid_constant__ Maps maps) {
+  using C = Shape<MODE, PAIR>;
+  constexpr int BN = C::BN, TILE = C::TILE, W = C::W, STAGES = C::STAGES, EPI = C::EPI;
   constexpr bool A_MN = MODE == DW, B_MN = MODE == DX || MODE == DW;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t sbase = smem_u32(smem_raw);
-  const uint32_t full = sbase + BARS, empty = full + 8 * STAGES, acc_full = empty + 8 * STAGES, acc_empty = acc_full + 16, slot = acc_empty + 16;
+  const uint32_t full = sbase + C::BARS, empty = full + 8 * STAGES, acc_full = empty + 8 * STAGES, acc_empty = acc_full + 16, slot = acc_empty + 16;
   const int warp = warp_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   volatile int& s_abort = *reinterpret_cast<int*>(smem_raw + (slot + 8 - sbase));
   const int rank = PAIR ? (int)cta_rank() : 0, first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
@@ -656,6 +747,10 @@ template <int MODE, bool PAIR> __global__ void __launch_bounds__(THREADS, 1) k_g
   const CUtensorMap *const map_a = MODE != DW && MODE != DX && direct ? &maps.x : &maps.a, *const map_b = MODE == DW && direct ? &maps.x : &maps.b;
   const int items = w.splits * w.tiles_m * w.tiles_n;
   const bool aborted = s_abort != 0;
+  // the writing warps keep it in shared memory: every register beside their sums counts
+  volatile Work& kept = *reinterpret_cast<Work*>(smem_raw + (slot + 16 - sbase));
+  if (threadIdx.x == 0) kept.tiles_m = w.tiles_m, kept.tiles_n = w.tiles_n, kept.splits = w.splits, kept.chunks = w.chunks, kept.per = w.per;
+  __syncthreads();
   if (warp == 0) {
     if (!aborted && elect_one()) {
       int st = 0, ph = 1;                                  // a ring that has not been used yet is empty
@@ -748,31 +843,23 @@ template <int MODE, bool PAIR> __global__ void __launch_bounds__(THREADS, 1) k_g
       if (!ok) report(&g_vocab_status, ERR_MMA_WAIT);
     }
   } else {
-    const int q = warp & 3, half = (warp - 2) >> 2;
+    const int q = warp & 3, share = (warp - 2) >> 2;
     int buf = 0, ph = 0;
     bool lost = aborted;
-    float acc[W];
-    for (int i = first; i < items; i += step) {
+    float acc[W / 32][32];
+    for (int i = first; i < kept.splits * kept.tiles_m * kept.tiles_n; i += step) {
       int s, m, nn, c0, c1;
-      item_at(w, i, s, m, nn, c0, c1);
+      item_at(kept, i, s, m, nn, c0, c1);
       const int all = (c1 - c0) * a.products;
-#pragma unroll
-      for (int g = 0; g < W; ++g) acc[g] = 0.f;
-      for (int done = 0; done < all && !lost; done += a.chain) {
-        if (!tc::warp_wait(acc_full + 8 * buf, ph, &g_vocab_status, ERR_MMA2_WAIT)) {
-          lost = true;
-          break;
-        }
+      const int row = m * TILE + rank * 128 + q * 32 + lane, col = nn * BN + share * W;
+      const Row me = row_of<MODE, W>(a, n, row, a.col0 + col);
+      // the first chain's sums as they come, the others' on top, sixteen at a time: more would not fit beside the sums
+      auto ready = [&] {
+        lost = !tc::warp_wait(acc_full + 8 * buf, ph, &g_vocab_status, ERR_MMA2_WAIT);
         tc_fence_after();
-        const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + buf * BN + half * W;
-#pragma unroll
-        for (int g = 0; g < W; g += 32) {
-          uint32_t r[32];
-          tmem_ld32(at + g, r);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) acc[g + e] += __uint_as_float(r[e]);
-        }
+        return !lost;
+      };
+      auto taken = [&] {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -781,12 +868,36 @@ template <int MODE, bool PAIR> __global__ void __launch_bounds__(THREADS, 1) k_g
         }
         buf ^= 1;
         if (buf == 0) ph ^= 1;
+      };
+      const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + share * W;
+      uint32_t r[W / 32][32];
+      if (all > 0 && !lost && ready()) {
+#pragma unroll
+        for (int g = 0; g < W / 32; ++g) tmem_ld32(from + buf * BN + 32 * g, r[g]);
+        tmem_ld_wait();
+        taken();
+      } else {
+#pragma unroll
+        for (int g = 0; g < W; ++g) r[g / 32][g % 32] = lost ? 0x7fffffffu : 0u;
+      }
+#pragma unroll
+      for (int g = 0; g < W; ++g) acc[g / 32][g % 32] = __uint_as_float(r[g / 32][g % 32]);
+      for (int done = a.chain; done < all && !lost; done += a.chain) {
+        if (!ready()) break;
+#pragma unroll
+        for (int g = 0; g < W; g += 16) {
+          uint32_t t[16];
+          tmem_ld16(from + buf * BN + g, t);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[(g + e) / 32][(g + e) % 32] += __uint_as_float(t[e]);
+        }
+        taken();
       }
       if (lost)
 #pragma unroll
-        for (int g = 0; g < W; ++g) acc[g] = not_a_number();
-      epilogue<MODE, W>(a, w, acc, n, s, m * TILE + rank * 128 + q * 32 + lane, nn * BN + half * W, TILE, 2 * nn + half,
-                        reinterpret_cast<float*>(smem_raw + STAGED) + (warp - 2) * 32 * 33);
+        for (int g = 0; g < W; ++g) acc[g / 32][g % 32] = not_a_number();
+      epilogue<MODE, W, THREE>(a, s * kept.tiles_m * TILE + row, acc, me, n, row, col, nn * (BN / W) + share, reinterpret_cast<float*>(smem_raw + C::STAGED) + (warp - 2) * 32 * 17);
     }
   }
   tc_fence_before();
@@ -916,6 +1027,13 @@ __device__ __forceinline__ void store8(const Join& a, long long r, long long c, 
     if (a.type == SPION_F32) Out<float, 8>::store(static_cast<float*>(a.out) + at, f);
     else if (a.type == SPION_BF16) Out<__nv_bfloat16, 8>::store(static_cast<__nv_bfloat16*>(a.out) + at, f);
     else Out<__half, 8>::store(static_cast<__half*>(a.out) + at, f);
+  } else if (a.K % 2 == 0) {                               // pairs
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      if (c + e >= a.K) break;
+      if (a.type == SPION_F32) *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at + e) = make_float2(f[e], f[e + 1]);
+      else *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + at + e) = pack2(f[e], f[e + 1], a.type == SPION_F16);
+    }
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -931,40 +1049,77 @@ __device__ __forceinline__ void join(const Join& a, unsigned cta, int n, float a
     plane = (long long)tiles_m * a.tile;
   }
   const int pieces = (int)((a.K + 7) / 8);
+  const long long all = a.rows * pieces;
+  auto place = [&](long long i, long long& r, int& c) {
+    r = all < 0x7fffffff ? (unsigned)i / (unsigned)pieces : i / pieces, c = (int)(i - r * pieces) * 8;
+  };
+  if (splits < 8) {                                        // up to four pieces a thread under way
+    const long long step = a.ctas * 256ll;
+    for (long long i0 = cta * 256ll + threadIdx.x; i0 < all; i0 += 4 * step) {
+      float f[4][8];
+      long long r[4], from[4];
+      int c[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const long long i = i0 + u * step;
+        place(min(i, all - 1), r[u], c[u]);
+        from[u] = i >= all ? -1 : a.slot ? a.slot[r[u]] : r[u];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[u][e] = 0.f;
+      for (int s = 0; s < splits; ++s) {
+        Piece<float, 8> p[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (from[u] >= 0) p[u].load(a.part + (s * plane + from[u]) * a.ldp + c[u]);
+          else p[u].zero();
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[u][e] += p[u].at(e);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (i0 + u * step >= all) break;
+        const float by = from[u] < 0 ? 0.f : alpha;        // a row that does not count: zeros, whatever arrives at the loss
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[u][e] *= by;
+        store8(a, r[u], c[u], f[u]);
+      }
+    }
+    return;
+  }
   // of many splits, eight threads take a share each
-  const int shares = splits >= 8 ? 8 : 1, share = threadIdx.x & (shares - 1), each = (splits + shares - 1) / shares, per = 256 / shares;
-  const long long all = a.rows * pieces, step = (long long)a.ctas * per;
-  for (long long i0 = (long long)cta * per; i0 < all; i0 += step) {
-    const long long i = i0 + threadIdx.x / shares;
-    const long long r = all < 0x7fffffff ? (unsigned)i / (unsigned)pieces : i / pieces, c = (i - r * pieces) * 8;
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, by = alpha;
-    if (i < all) {
-      const long long from = a.slot ? a.slot[r] : r;
-      if (from >= 0)
+  const int share = threadIdx.x & 7, each = (splits + 7) / 8;
+  for (long long i0 = cta * 32ll; i0 < all; i0 += a.ctas * 32ll) {
+    const long long i = i0 + threadIdx.x / 8;
+    long long r;
+    int c;
+    place(min(i, all - 1), r, c);
+    const long long from = a.slot ? a.slot[r] : r;
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (from >= 0)
 #pragma unroll 4
-        for (int s = share * each; s < min(splits, (share + 1) * each); ++s) {
-          Piece<float, 8> p;
-          p.load(a.part + (s * plane + from) * a.ldp + c);
+      for (int s = share * each; s < min(splits, (share + 1) * each); ++s) {
+        Piece<float, 8> p;
+        p.load(a.part + (s * plane + from) * a.ldp + c);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] += p.at(e);
-        }
-      if (from < 0) by = 0.f;                             // whatever arrives at the loss
-    }
-    if (shares > 1) {
-      __syncthreads();
+        for (int e = 0; e < 8; ++e) f[e] += p.at(e);
+      }
+    __syncthreads();
 #pragma unroll
-      for (int e = 0; e < 8; ++e) shared[threadIdx.x][e] = f[e];
-      __syncthreads();
-      if (share == 0)
-        for (int o = 1; o < shares; ++o)
+    for (int e = 0; e < 8; ++e) shared[threadIdx.x][e] = f[e];
+    __syncthreads();
+    if (share > 0 || i >= all) continue;
+    for (int o = 1; o < 8; ++o)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] += shared[threadIdx.x + o][e];
-    }
-    if (i < all && share == 0) {
+      for (int e = 0; e < 8; ++e) f[e] += shared[threadIdx.x + o][e];
+    const float by = from < 0 ? 0.f : alpha;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] *= by;
-      store8(a, r, c, f);
-    }
+    for (int e = 0; e < 8; ++e) f[e] *= by;
+    store8(a, r, c, f);
   }
 }
 __global__ void __launch_bounds__(256) k_out(const __grid_constant__ Leave a) {
@@ -1033,20 +1188,20 @@ int map_of(CUtensorMap* m, const void* base, long long cols, long long rows_, lo
   return SPION_OK;
 }
 // CTAs (or pairs) of a kernel that the current device holds at a time
-template <int MODE, bool PAIR> int units_of(int* units) {
+template <int MODE, bool PAIR, bool THREE = false> int units_of(int* units) {
   static std::atomic<int> known[64];
   int dev = 0;
   SPION_CUDA_TRY(cudaGetDevice(&dev));
   int n = dev < 64 ? known[dev].load() : 0;
   if (n == 0) {
-    SPION_CUDA_TRY(cudaFuncSetAttribute(k_gemm<MODE, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM<MODE>));
+    SPION_CUDA_TRY(cudaFuncSetAttribute(k_gemm<MODE, PAIR, THREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<MODE, PAIR>::SMEM));
     if (PAIR) {
       cudaLaunchConfig_t cfg = {};
       cudaLaunchAttribute at[1];
       at[0].id = cudaLaunchAttributeClusterDimension;
       at[0].val.clusterDim.x = 2, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-      cfg.gridDim = dim3(2 * (sm_count() / 2)), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = SMEM<MODE>, cfg.attrs = at, cfg.numAttrs = 1;
-      SPION_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, k_gemm<MODE, PAIR>, &cfg));
+      cfg.gridDim = dim3(2 * (sm_count() / 2)), cfg.blockDim = dim3(Shape<MODE, PAIR>::THREADS), cfg.dynamicSmemBytes = Shape<MODE, PAIR>::SMEM, cfg.attrs = at, cfg.numAttrs = 1;
+      SPION_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, k_gemm<MODE, PAIR, THREE>, &cfg));
     } else {
       n = sm_count();
     }
@@ -1056,9 +1211,9 @@ template <int MODE, bool PAIR> int units_of(int* units) {
   *units = n;
   return SPION_OK;
 }
-template <int MODE, bool PAIR> int launch_gemm(const Args& a, const Maps& maps, long long most_items, cudaStream_t st) {
+template <int MODE, bool PAIR, bool THREE> int launch_gemm(const Args& a, const Maps& maps, long long most_items, cudaStream_t st) {
   int units;
-  const int rc = units_of<MODE, PAIR>(&units);
+  const int rc = units_of<MODE, PAIR, THREE>(&units);
   if (rc != SPION_OK) return rc;
   // DX splits its contraction by the number of units: it always has all of them
   const int use = a.splits == 0 ? units : (int)std::min<long long>(units, std::max<long long>(most_items, 1));
@@ -1068,12 +1223,13 @@ template <int MODE, bool PAIR> int launch_gemm(const Args& a, const Maps& maps, 
   at[0].val.programmaticStreamSerializationAllowed = 1;
   at[1].id = cudaLaunchAttributeClusterDimension;
   at[1].val.clusterDim.x = 2, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(PAIR ? 2 * use : use), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = SMEM<MODE>, cfg.stream = st, cfg.attrs = at, cfg.numAttrs = PAIR ? 2 : 1;
-  SPION_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_gemm<MODE, PAIR>, a, maps));
+  cfg.gridDim = dim3(PAIR ? 2 * use : use), cfg.blockDim = dim3(Shape<MODE, PAIR>::THREADS), cfg.dynamicSmemBytes = Shape<MODE, PAIR>::SMEM, cfg.stream = st, cfg.attrs = at, cfg.numAttrs = PAIR ? 2 : 1;
+  SPION_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_gemm<MODE, PAIR, THREE>, a, maps));
   return SPION_OK;
 }
 template <int MODE> int launch_gemm(bool pair, const Args& a, const Maps& maps, long long most_items, cudaStream_t st) {
-  return pair ? launch_gemm<MODE, true>(a, maps, most_items, st) : launch_gemm<MODE, false>(a, maps, most_items, st);
+  if (MODE == GRAD && a.products > 1) return pair ? launch_gemm<MODE, true, MODE == GRAD>(a, maps, most_items, st) : launch_gemm<MODE, false, MODE == GRAD>(a, maps, most_items, st);
+  return pair ? launch_gemm<MODE, true, false>(a, maps, most_items, st) : launch_gemm<MODE, false, false>(a, maps, most_items, st);
 }
 
 constexpr long long up(long long x, long long to) { return (x + to - 1) / to * to; }
@@ -1088,6 +1244,7 @@ struct Layout {
   bool copy_w, direct;                                    // w has to be copied; x can be read as it lies
   bool kept;                                              // the operands' copies stay for the backward
   bool self;                                              // CTAs count for themselves
+  long long chunk;                                        // rows of a CTA of k_prepare
   bool pair_z, pair_dx, pair_dw;
   long long Gp;                                           // columns of a piece of the vocabulary
   int dw_splits;
@@ -1096,7 +1253,7 @@ struct Layout {
   size_t part, zt, cta_loss, counts, q, forward;
   size_t g, dxp, dwp, colsum, unit, backward;
 };
-constexpr long long PIECE_BYTES = 256ll << 20;            // of G
+constexpr long long PIECE_BYTES = SPION_PIECE << 20;       // of G
 constexpr long long KEPT_BYTES = 64ll << 20;              // of copies that stay: small beside the device, and making them again costs launches and, for small calls, most of the time
 constexpr int FINISH_CTAS = 1024;
 
@@ -1116,6 +1273,8 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   l->direct = p->type != SPION_F32 && ((uintptr_t)p->x % 16) == 0 && (p->ldx * 2) % 16 == 0 && p->ldx >= p->K;
   l->ldw = l->copy_w ? l->Kp : p->ldw;
   l->self = p->T * p->k <= SELF;
+  // every CTA reads the counts of all chunks: 4096 of them at most
+  l->chunk = p->T <= 16384 ? 32 : std::max<long long>(BLOCK, up((p->T + 4095) / 4096, BLOCK));
   int sms = sm_count();
   if (sms <= 0) return SPION_ERR_CUDA;
   const int pairs = sms / 2;
@@ -1126,7 +1285,7 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   l->pair_dx = pair(l->T, l->K);
   l->pair_dw = pair(l->Gp, l->K);
   const long long dw_tiles = l->pair_dw ? tiles_of(l->Gp, 256) * tiles_of(l->K, 256) : tiles_of(l->Gp, 128) * tiles_of(l->K, 128);
-  l->dw_splits = l->pair_dw ? 1 : split_by_tiles((int)dw_tiles, sms, (int)std::max<long long>(1, tiles_of(l->T, BK) / 4));
+  l->dw_splits = l->pair_dw ? 1 : split_by_units((int)std::min<long long>(dw_tiles, 1 << 20), sms, (int)tiles_of(l->T, BK));
   size_t at = 0;
   auto take = [&](long long bytes) {
     const size_t here = at;
@@ -1142,16 +1301,17 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   at = 0;
   if (!l->kept) operands();
   const size_t both = at;
-  l->part = take(8 * l->Tp * 2 * (l->pair_z ? tiles_of(l->V, 256) : tiles_of(l->V, 128)));
+  l->part = take(8 * l->Tp * (l->pair_z ? 4 * tiles_of(l->V, 256) : 2 * tiles_of(l->V, 128)));
   l->zt = take(4 * l->k * l->Tp);
   l->cta_loss = take(8 * FINISH_CTAS);
-  l->counts = take(4 * tiles_of(l->T, CHUNK));
+  l->counts = take(4 * tiles_of(l->T, l->chunk));
   l->q = take(4 * l->T * l->k);
   l->forward = at;
   at = both;
   l->g = take(2 * l->planes * l->Tp * l->Gp);
-  const long long tile = l->pair_dx ? 256 : 128, tn = tiles_of(l->K, tile);
-  l->dxp = take(4 * std::max(tiles_of(l->T, tile), (l->pair_dx ? pairs : sms) / tn) * tile * l->Kp);
+  // (as split_by_tiles cuts them: one part, or eight rounds of tiles at most)
+  const long long tile = l->pair_dx ? 256 : 128, tn = tiles_of(l->K, tile), most_m = 8 * (l->pair_dx ? pairs : sms) / tn;
+  l->dxp = take(4 * std::max(tiles_of(l->T, tile), std::min(most_m, 8 * tiles_of(l->T, tile))) * tile * l->Kp);
   l->dwp = take(l->dw_splits > 1 ? 4 * l->dw_splits * up(l->Gp, l->pair_dw ? 256 : 128) * l->Kp : 0);
   l->colsum = take(4 * (l->Tp / 32) * l->Gp);
   l->unit = take(256);
@@ -1171,8 +1331,9 @@ Plan plan_at(const Layout& l, void* keep, bool teacher) {
   return p;
 }
 Source source_of(const void* p, int type, long long ld, long long K, long long Kp) {
-  const int piece = type == SPION_F32 ? 32 : 16;
-  return {p, type, ld, (int)K, (int)Kp, K % 8 == 0 && (uintptr_t)p % piece == 0 && ld * type_size(type) % piece == 0};
+  const int size = type_size(type);
+  auto on = [&](int bytes) { return (uintptr_t)p % bytes == 0 && ld * size % bytes == 0; };
+  return {p, type, ld, (int)K, (int)Kp, K % 8 == 0 && on(16) ? 2 : K % 2 == 0 && on(2 * size) ? 1 : 0};
 }
 Prep prep_of(const spion_vocab_problem* p, const Layout& l, void* keep, char* ws) {
   Prep a = {};
@@ -1186,9 +1347,10 @@ Prep prep_of(const spion_vocab_problem* p, const Layout& l, void* keep, char* ws
   a.x = source_of(p->x, p->type, p->ldx, l.K, l.Kp), a.w = source_of(p->w, p->type, p->ldw, l.K, l.Kp);
   a.xs = (uint16_t*)(operands + l.xs), a.ws = l.copy_w ? (uint16_t*)(operands + l.w) : nullptr;
   a.direct = l.direct;
-  const long long chunks = tiles_of(l.T, CHUNK), bytes = l.Kp * (l.planes == 3 ? 4 : 2);
-  // slices of 512 bytes of a row at least, where there are too few chunks to fill the device twice
-  a.slices = (unsigned)std::max<long long>(1, std::min<long long>(bytes / 512, 2 * sm_count() / chunks));
+  const long long chunks = tiles_of(l.T, l.chunk);
+  a.chunk = (int)l.chunk;
+  // slices of 64 elements of a row at least, where there are too few chunks to fill the device twice
+  a.slices = (unsigned)std::max<long long>(1, std::min<long long>(l.Kp / 64, 2 * sm_count() / chunks));
   a.row_ctas = (unsigned)chunks * a.slices;
   a.w_ctas = l.copy_w ? (unsigned)std::min<long long>(tiles_of(l.Vp, 8), 8 * sm_count()) : 0;
   return a;
@@ -1258,13 +1420,13 @@ extern "C" int spion_vocab_loss_forward(const spion_vocab_problem* p, float* los
   Prep prep = prep_of(p, l, keep, ws);
   prep.counts = l.self ? nullptr : (int*)(ws + l.counts), prep.q = (float*)(ws + l.q), prep.zt = (float*)(ws + l.zt);
   prep.loss_rows = p->reduction == 0 ? loss : nullptr;
-  if (!l.self) SPION_CUDA_TRY(launch_after(k_flags, dim3((unsigned)tiles_of(tiles_of(l.T, CHUNK), prep.teacher ? 1 : 8)), dim3(256), 0, st, prep));
+  if (!l.self) SPION_CUDA_TRY(launch_after(k_flags, dim3((unsigned)tiles_of(tiles_of(l.T, l.chunk), prep.teacher ? 1 : 8)), dim3(256), 0, st, prep));
   if ((rc = launch_prepare<true>(p, prep, st)) != SPION_OK) return rc;
   Args a;
   Maps maps;
   if ((rc = logits_args(p, l, prep, &a, &maps)) != SPION_OK) return rc;
   const int tile = l.pair_z ? 256 : 128;
-  a.N = (int)l.V, a.part = (float2*)(ws + l.part), a.parts = (int)(2 * tiles_of(l.V, tile)), a.zt = prep.zt;
+  a.N = (int)l.V, a.part = (float2*)(ws + l.part), a.parts = (int)(l.pair_z ? 4 * tiles_of(l.V, 256) : 2 * tiles_of(l.V, 128)), a.zt = prep.zt;
   if ((rc = launch_gemm<LOGSUM>(l.pair_z, a, maps, tiles_of(l.T, tile) * tiles_of(l.V, tile), st)) != SPION_OK) return rc;
   const Finish f = {prep.plan, (int)l.Tp, (int)l.k, a.part, a.parts, prep.zt, loss, (double*)(ws + l.cta_loss), p->reduction};
   const int lanes = std::max<int>(a.parts, l.k) <= 16 ? 4 : std::max<int>(a.parts, l.k) <= 32 ? 8 : 32;
