@@ -519,6 +519,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, int fp16) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// What a kernel is made for, beside its product: what it need not do costs registers that the sums want.
+enum : int { ONE = 1, THREE = 2, COLUMNS = 4 };           // one target a row (LOGSUM, GRAD); G in three parts, sums of G's columns (GRAD)
+
 // What a writing thread knows of its row before the sums are there: it is read while they are formed
 struct Row {
   bool in;                  // the row counts
@@ -527,20 +530,21 @@ struct Row {
   float lse, r;
 };
 // f(offset, target) of every target among the columns g .. g + 31 of the thread's
-template <class F> __device__ __forceinline__ void each_target(const Args& a, const Row& row, int c, int g, F f) {
+template <int OPT, class F> __device__ __forceinline__ void each_target(const Args& a, const Row& row, int c, int g, F f) {
+  constexpr int REMEMBERED = OPT & ONE ? 1 : 2;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < REMEMBERED; ++i) {
     const int off = (int)(row.two >> (16 * i) & 0xff) - g;
     if (row.found > i && (unsigned)off < 32u) f(off, (int)(row.two >> (16 * i + 8) & 0xff));
   }
-  if (row.found > 2) {                                     // seldom: all over again, without those two
+  if (!(OPT & ONE) && row.found > 2) {                     // seldom: all over again, without those two
     for (int j = (int)(row.two >> 24) + 1; j < a.k; ++j) {
       const int off = a.plan.target[(long long)j * a.Tp + row.slot] - c - g;
       if ((unsigned)off < 32u) f(off, j);
     }
   }
 }
-template <int MODE, int W> __device__ __forceinline__ Row row_of(const Args& a, int n, int row, int c) {
+template <int MODE, int W, int OPT> __device__ __forceinline__ Row row_of(const Args& a, int n, int row, int c) {
   Row r = {};
   if (MODE != LOGSUM && MODE != GRAD) return r;
   r.in = row < n;
@@ -548,7 +552,11 @@ template <int MODE, int W> __device__ __forceinline__ Row row_of(const Args& a, 
   r.lse = INFINITY;
   if (r.in) {
     const int* const target = a.plan.target + r.slot;
-    for (int j0 = 0; j0 < a.k; j0 += 16) {                 // sixteen loads under way: one after another they are 0.25 us each
+    if (OPT & ONE) {
+      const int t = target[0], off = t - c;
+      if ((unsigned)off < (unsigned)W && t >= 0) r.two = off, r.found = 1;
+    }
+    for (int j0 = 0; !(OPT & ONE) && j0 < a.k; j0 += 16) {  // sixteen loads under way: one after another they are 0.25 us each
       int t[16];
 #pragma unroll
       for (int u = 0; u < 16; ++u) t[u] = j0 + u < a.k ? target[(long long)(j0 + u) * a.Tp] : -1;
@@ -570,7 +578,7 @@ template <int MODE, int W> __device__ __forceinline__ Row row_of(const Args& a, 
 }
 
 // What a thread does with its sums: row `row` of D, columns col .. col + W - 1
-template <int MODE, int W, bool THREE> __device__ __forceinline__ void epilogue(const Args& a, int out_row, float (&acc)[W / 32][32], const Row& me, int n, int row, int col, int part, float* stage) {
+template <int MODE, int W, int OPT> __device__ __forceinline__ void epilogue(const Args& a, int out_row, float (&acc)[W / 32][32], const Row& me, int n, int row, int col, int part, float* stage) {
   const int lane = threadIdx.x & 31;
   if constexpr (MODE == LOGSUM || MODE == GRAD) {
     const int slot = me.slot, c = a.col0 + col;           // of the vocabulary
@@ -586,7 +594,7 @@ template <int MODE, int W, bool THREE> __device__ __forceinline__ void epilogue(
       for (int g = 0; g < W; ++g) top = fmaxf(top, acc[g / 32][g % 32]);
 #pragma unroll
       for (int g = 0; g < W; g += 32)
-        each_target(a, me, c, g, [&](int off, int j) {
+        each_target<OPT>(a, me, c, g, [&](int off, int j) {
           float z = 0.f;
 #pragma unroll
           for (int e = 0; e < 32; ++e) z = e == off ? acc[(g + e) / 32][(g + e) % 32] : z;
@@ -603,13 +611,13 @@ template <int MODE, int W, bool THREE> __device__ __forceinline__ void epilogue(
         float (&v)[32] = acc[g / 32];                      // in place: there is no room for another 32
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] = ex2(v[e] - lse) * r;      // zeros of rows that do not count: their lse is inf
-        each_target(a, me, c, g, [&](int off, int j) {
+        each_target<OPT>(a, me, c, g, [&](int off, int j) {
           const float q = (a.plan.q ? a.plan.q[(long long)j * a.Tp + slot] : 1.f) * r;
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] -= e == off ? q : 0.f;
         });
         uint16_t* const to = a.G + (long long)row * a.ldg + col + g;
-        if constexpr (!THREE) {
+        if constexpr (!(OPT & THREE)) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t out[8];
@@ -636,7 +644,7 @@ template <int MODE, int W, bool THREE> __device__ __forceinline__ void epilogue(
             }
           }
         }
-        if (a.colsum != nullptr) {                        // over the warp's 32 rows: lane l ends with column l
+        if constexpr ((OPT & COLUMNS) != 0) {             // over the warp's 32 rows: lane l ends with column l
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
@@ -701,13 +709,12 @@ template <int MODE, int W, bool THREE> __device__ __forceinline__ void epilogue(
   }
 }
 
-// THREE: G in three parts (GRAD).
 // Warp 0 loads, warp 1 multiplies, the others take the sums.  Every wait is bounded; whoever gives up reports it and leaves, and so do all that wait for it; the warps
 // that write go on with NaN.  PAIR: two CTAs of a cluster share a tile of 256 x 256, each brings 128 rows of either operand and holds 128 rows of the sums; the first one's warp 1
 // multiplies for both (see k_lin8 in linear_e4m3.cu, whose scheme this is).  Else tiles of 128 x 128.
 // Operands whose contraction runs along memory (K-major: x and W in z, G in dx) come as one box of 128 rows x 64; those whose contraction runs across it (MN-major: W in dx, G and x
 // in dW) as two boxes of 64 rows x 64.
-template <int MODE, bool PAIR, bool THREE> __global__ void __launch_bounds__(Shape<MODE, PAIR>::THREADS, 1) k_gemm(const __grid_constant__ Args a, const __grid_constant__ Maps maps) {
+template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<MODE, PAIR>::THREADS, 1) k_gemm(const __grid_constant__ Args a, const __grid_constant__ Maps maps) {
   using C = Shape<MODE, PAIR>;
   constexpr int BN = C::BN, TILE = C::TILE, W = C::W, STAGES = C::STAGES, EPI = C::EPI;
   constexpr bool A_MN = MODE == DW, B_MN = MODE == DX || MODE == DW;
@@ -852,7 +859,7 @@ template <int MODE, bool PAIR, bool THREE> __global__ void __launch_bounds__(Sha
       item_at(kept, i, s, m, nn, c0, c1);
       const int all = (c1 - c0) * a.products;
       const int row = m * TILE + rank * 128 + q * 32 + lane, col = nn * BN + share * W;
-      const Row me = row_of<MODE, W>(a, n, row, a.col0 + col);
+      const Row me = row_of<MODE, W, OPT>(a, n, row, a.col0 + col);
       // the first chain's sums as they come, the others' on top, sixteen at a time: more would not fit beside the sums
       auto ready = [&] {
         lost = !tc::warp_wait(acc_full + 8 * buf, ph, &g_vocab_status, ERR_MMA2_WAIT);
@@ -897,7 +904,7 @@ template <int MODE, bool PAIR, bool THREE> __global__ void __launch_bounds__(Sha
       if (lost)
 #pragma unroll
         for (int g = 0; g < W; ++g) acc[g / 32][g % 32] = not_a_number();
-      epilogue<MODE, W, THREE>(a, s * kept.tiles_m * TILE + row, acc, me, n, row, col, nn * (BN / W) + share, reinterpret_cast<float*>(smem_raw + C::STAGED) + (warp - 2) * 32 * 17);
+      epilogue<MODE, W, OPT>(a, s * kept.tiles_m * TILE + row, acc, me, n, row, col, nn * (BN / W) + share, reinterpret_cast<float*>(smem_raw + C::STAGED) + (warp - 2) * 32 * 17);
     }
   }
   tc_fence_before();
@@ -1188,20 +1195,20 @@ int map_of(CUtensorMap* m, const void* base, long long cols, long long rows_, lo
   return SPION_OK;
 }
 // CTAs (or pairs) of a kernel that the current device holds at a time
-template <int MODE, bool PAIR, bool THREE = false> int units_of(int* units) {
+template <int MODE, bool PAIR, int OPT = 0> int units_of(int* units) {
   static std::atomic<int> known[64];
   int dev = 0;
   SPION_CUDA_TRY(cudaGetDevice(&dev));
   int n = dev < 64 ? known[dev].load() : 0;
   if (n == 0) {
-    SPION_CUDA_TRY(cudaFuncSetAttribute(k_gemm<MODE, PAIR, THREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<MODE, PAIR>::SMEM));
+    SPION_CUDA_TRY(cudaFuncSetAttribute(k_gemm<MODE, PAIR, OPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<MODE, PAIR>::SMEM));
     if (PAIR) {
       cudaLaunchConfig_t cfg = {};
       cudaLaunchAttribute at[1];
       at[0].id = cudaLaunchAttributeClusterDimension;
       at[0].val.clusterDim.x = 2, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
       cfg.gridDim = dim3(2 * (sm_count() / 2)), cfg.blockDim = dim3(Shape<MODE, PAIR>::THREADS), cfg.dynamicSmemBytes = Shape<MODE, PAIR>::SMEM, cfg.attrs = at, cfg.numAttrs = 1;
-      SPION_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, k_gemm<MODE, PAIR, THREE>, &cfg));
+      SPION_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, k_gemm<MODE, PAIR, OPT>, &cfg));
     } else {
       n = sm_count();
     }
@@ -1211,9 +1218,9 @@ template <int MODE, bool PAIR, bool THREE = false> int units_of(int* units) {
   *units = n;
   return SPION_OK;
 }
-template <int MODE, bool PAIR, bool THREE> int launch_gemm(const Args& a, const Maps& maps, long long most_items, cudaStream_t st) {
+template <int MODE, bool PAIR, int OPT> int launch_gemm(const Args& a, const Maps& maps, long long most_items, cudaStream_t st) {
   int units;
-  const int rc = units_of<MODE, PAIR, THREE>(&units);
+  const int rc = units_of<MODE, PAIR, OPT>(&units);
   if (rc != SPION_OK) return rc;
   // DX splits its contraction by the number of units: it always has all of them
   const int use = a.splits == 0 ? units : (int)std::min<long long>(units, std::max<long long>(most_items, 1));
@@ -1224,12 +1231,26 @@ template <int MODE, bool PAIR, bool THREE> int launch_gemm(const Args& a, const 
   at[1].id = cudaLaunchAttributeClusterDimension;
   at[1].val.clusterDim.x = 2, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.gridDim = dim3(PAIR ? 2 * use : use), cfg.blockDim = dim3(Shape<MODE, PAIR>::THREADS), cfg.dynamicSmemBytes = Shape<MODE, PAIR>::SMEM, cfg.stream = st, cfg.attrs = at, cfg.numAttrs = PAIR ? 2 : 1;
-  SPION_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_gemm<MODE, PAIR, THREE>, a, maps));
+  SPION_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_gemm<MODE, PAIR, OPT>, a, maps));
   return SPION_OK;
 }
+template <int MODE, int OPT> int launch_gemm(bool pair, const Args& a, const Maps& maps, long long most_items, cudaStream_t st) {
+  return pair ? launch_gemm<MODE, true, OPT>(a, maps, most_items, st) : launch_gemm<MODE, false, OPT>(a, maps, most_items, st);
+}
 template <int MODE> int launch_gemm(bool pair, const Args& a, const Maps& maps, long long most_items, cudaStream_t st) {
-  if (MODE == GRAD && a.products > 1) return pair ? launch_gemm<MODE, true, MODE == GRAD>(a, maps, most_items, st) : launch_gemm<MODE, false, MODE == GRAD>(a, maps, most_items, st);
-  return pair ? launch_gemm<MODE, true, false>(a, maps, most_items, st) : launch_gemm<MODE, false, false>(a, maps, most_items, st);
+  if constexpr (MODE == LOGSUM) return a.k == 1 ? launch_gemm<MODE, ONE>(pair, a, maps, most_items, st) : launch_gemm<MODE, 0>(pair, a, maps, most_items, st);
+  if constexpr (MODE == GRAD)
+    switch ((a.k == 1 ? ONE : 0) | (a.products > 1 ? THREE : 0) | (a.colsum != nullptr ? COLUMNS : 0)) {
+      case 0: return launch_gemm<MODE, 0>(pair, a, maps, most_items, st);
+      case 1: return launch_gemm<MODE, 1>(pair, a, maps, most_items, st);
+      case 2: return launch_gemm<MODE, 2>(pair, a, maps, most_items, st);
+      case 3: return launch_gemm<MODE, 3>(pair, a, maps, most_items, st);
+      case 4: return launch_gemm<MODE, 4>(pair, a, maps, most_items, st);
+      case 5: return launch_gemm<MODE, 5>(pair, a, maps, most_items, st);
+      case 6: return launch_gemm<MODE, 6>(pair, a, maps, most_items, st);
+      default: return launch_gemm<MODE, 7>(pair, a, maps, most_items, st);
+    }
+  return launch_gemm<MODE, 0>(pair, a, maps, most_items, st);
 }
 
 constexpr long long up(long long x, long long to) { return (x + to - 1) / to * to; }
