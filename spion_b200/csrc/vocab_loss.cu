@@ -11,7 +11,7 @@
 //   k_gemm<LOGSUM>       z tile by tile in tensor memory; leaves the largest and the sum of exponentials of a row's columns of the tile, and the targets' z
 //   k_finish             lse and loss of each row, and their sum or mean
 //   k_gemm<GRAD>         z again, for a piece of the vocabulary; leaves G in 16 bits
-//   k_gemm<DX>, <DW>     the two products with it;  k_out joins what was summed apart, and forms db
+//   k_gemm<GRADS>        the two products with it;  k_out joins what was summed apart, and forms db
 //
 // The products are tcgen05 kind::f16, fp32 sums in tensor memory.  A sum there is truncated at every step, so no more than CHAIN steps go to one
 // accumulator where a result has 32 bits; what the accumulators hold is added in fp32 registers.  fp32 operands are three bf16 parts each (8 + 8 + 8 bits, exact) and
@@ -243,7 +243,7 @@ template <class E, bool FIRST> __global__ void __launch_bounds__(256) k_prepare(
   constexpr int PARTS = std::is_same<E, Eight32>::value ? 3 : 1;
   next_may_start();
   wait_for_kernel_before();
-  __shared__ int list[BLOCK], part[2][8], here_;
+  __shared__ int list[BLOCK], part[2][8];
   __shared__ unsigned flags[SELF / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (blockIdx.x >= a.row_ctas + a.w_ctas) {
@@ -319,30 +319,31 @@ template <class E, bool FIRST> __global__ void __launch_bounds__(256) k_prepare(
     n = 0;
 #pragma unroll
     for (int w = 0; w < 8; ++w) first += part[0][w], n += part[1][w];
+    __syncthreads();
     const bool in_place = a.direct && n == a.T;
     if (blockIdx.x == 0 && threadIdx.x == 0) a.plan.head[0] = n, a.plan.head[1] = 0;
     for (int t0 = chunk * a.chunk; t0 < chunk_end; t0 += BLOCK) {
       const int end = min(chunk_end, t0 + BLOCK);
-      if (warp == 0) {
-        int at = 0;
-        for (int i = t0; i < end; i += 32) {
-          const int t = i + lane;
-          const bool counts = t < end && (a.counts == nullptr ? flags[t >> 5] >> (t & 31) & 1 : a.teacher ? a.plan.slot[t] != -1 : a.labels[t] != a.ignore);
-          const unsigned who = __ballot_sync(0xffffffffu, counts);
-          const int place = at + __popc(who & ((1u << lane) - 1));
-          if (counts) list[place] = t;
-          if (slice == 0 && t < end) {
-            // (other slices of the chunk may read a slot before or after this: that it is -1 or not stays)
-            a.plan.slot[t] = counts ? first + place : -1;
-            if (a.loss_rows != nullptr && !counts) a.loss_rows[t] = 0.f;
-            if (counts) a.plan.row[first + place] = t;
-          }
-          at += __popc(who);
-        }
-        if (lane == 0) here_ = at;
+      // a warp for every 32 rows; where its first goes, after another barrier
+      const int t = t0 + 32 * warp + lane;
+      const bool counts = warp < BLOCK / 32 && t < end && (a.counts == nullptr ? flags[t >> 5] >> (t & 31) & 1 : a.teacher ? a.plan.slot[t] != -1 : a.labels[t] != a.ignore);
+      const unsigned who = __ballot_sync(0xffffffffu, counts);
+      if (lane == 0) part[0][warp] = __popc(who);
+      __syncthreads();
+      int place = __popc(who & ((1u << lane) - 1)), here = 0;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        if (w < warp) place += part[0][w];
+        here += part[0][w];
+      }
+      if (counts) list[place] = t;
+      if (slice == 0 && warp < BLOCK / 32 && t < end) {
+        // (other slices of the chunk may read a slot before or after this: that it is -1 or not stays)
+        a.plan.slot[t] = counts ? first + place : -1;
+        if (a.loss_rows != nullptr && !counts) a.loss_rows[t] = 0.f;
+        if (counts) a.plan.row[first + place] = t;
       }
       __syncthreads();
-      const int here = here_;
       if (slice == 0)
         for (int i = threadIdx.x; i < here * a.k; i += 256) {
           const int r = i / a.k, j = i - r * a.k;
@@ -376,7 +377,8 @@ template <class E, bool FIRST> __global__ void __launch_bounds__(256) k_prepare(
 }
 
 // ------------------------------------------------------------------------------------------------ the four products
-enum Mode { LOGSUM, GRAD, DX, DW };
+enum Mode { LOGSUM, GRAD, GRADS };                        // GRADS: dx and dW, two products in one launch
+enum : int { DX, DW };                                    // ... and which of them
 constexpr int BK = 64;                                    // elements of the contraction in a chunk: 128 bytes
 constexpr uint32_t HALF = 128 * BK * 2, STAGE = 2 * HALF;
 // PAIR: two CTAs of a cluster share a tile of 256 x 256; else tiles of 128 x 128.  A thread that writes has 64 columns: what it does with them is a chain of latencies, and four
@@ -384,10 +386,10 @@ constexpr uint32_t HALF = 128 * BK * 2, STAGE = 2 * HALF;
 template <int MODE, bool PAIR> struct Shape {
   static constexpr int BN = PAIR ? 256 : 128, TILE = PAIR ? 256 : 128, W = 64;         // columns and rows of a tile; columns of a writing thread
   static constexpr int EPI = 4 * BN / W, THREADS = 32 * (2 + EPI), STAGES = 6;
-  static constexpr uint32_t BARS = STAGES * STAGE, STAGED = BARS + 16 * STAGES + 96;   // STAGED: 32 x 16 results a writing warp, rows of 17 (DW)
-  static constexpr uint32_t SMEM = MODE == DW ? STAGED + EPI * 32 * 17 * 4 : STAGED;
+  static constexpr uint32_t BARS = STAGES * STAGE, STAGED = BARS + 16 * STAGES + 128;   // STAGED: 32 x 16 results a writing warp, rows of 17 (DW)
+  static constexpr uint32_t SMEM = MODE == GRADS ? STAGED + EPI * 32 * 17 * 4 : STAGED;
 };
-static_assert(Shape<DW, true>::SMEM <= 232448 && Shape<DW, false>::SMEM <= 232448, "shared memory of a multiprocessor");
+static_assert(Shape<GRADS, true>::SMEM <= 232448 && Shape<GRADS, false>::SMEM <= 232448, "shared memory of a multiprocessor");
 
 // What the products with G are multiplied with.  Rows with a g each: it comes from k_unit.
 struct Coef {
@@ -400,14 +402,34 @@ struct Coef {
     return n > 0 ? (mean ? *g / (float)n : *g) * scale : 0.f;
   }
 };
+// Parts of dx's contraction.  Alone: the number that leaves the fewest units idle in the last round of tiles, a fiftieth less for each part more (its sums are written and read
+// once more), eight at most and eight rounds; 8192 x 2048 from 16384 columns, 256 tiles on 74 pairs: one part 386 us, two 355.  Beside dW's tiles, which fill what is left: the
+// share of a unit in all chunks, and half of the longest tile.
+struct Parts {
+  int units, chunks;        // of the first piece of the vocabulary: every piece is cut alike
+  int other, other_parts;   // tiles of dW beside it, and the parts of their contraction
+  __host__ __device__ int of(int tiles, int n) const {
+    const long long oc = other ? ((n + BK - 1) / BK + other_parts - 1) / other_parts : 0;
+    int best = 1;
+    long long least = 1ll << 62;
+    for (int s = 1; s <= 8 && tiles > 0 && (s == 1 || ((long long)tiles * s <= 8ll * units && 4 * s <= chunks)); ++s) {
+      const long long c = (chunks + s - 1) / s, longest = c > oc ? c : oc;
+      const long long time = other ? ((long long)tiles * chunks + other * oc) * 2 / units + longest : ((long long)tiles * s + units - 1) / units * c * 2;
+      if (time * (50 + s) < least) best = s, least = time * (50 + s);
+    }
+    return best;
+  }
+};
 struct Args {
+  int on;                                                 // 0: nothing to do (GRADS)
   const int* n;                                           // rows that count
   int products;                                           // 1, or 6 of three parts
   long long plane_a, plane_b;                             // rows of a part in the maps
   int M, N, L;                                            // rows of D (0: n), columns of D, contraction (0: n)
   int col0;                                               // first column of the piece of the vocabulary
   int chain;                                              // (chunk, product) pairs that one accumulator takes
-  int splits, split_chunks;                               // of the contraction (0: by the number of tiles, at most split_chunks)
+  int splits;                                             // of the contraction (0: by `cut`)
+  Parts cut;
   int fp16;                                               // operands are fp16, else bf16
   int direct_rows;                                        // rows of x, where they are read as they lie if all count; else 0
   // LOGSUM, GRAD
@@ -423,7 +445,12 @@ struct Args {
   float* out; long long ldo; int add;                     // fp32 partial sums: [split][rows of whole tiles][ldo]
   void* dw; int dw_type; long long K; int V;              // DW, one split: the result
 };
-struct Maps { CUtensorMap a, b, x; };                       // x: the rows as they lie, in place of a (LOGSUM, GRAD) or of b (DW)
+struct Maps { CUtensorMap a, b, x; };                       // x: the rows as they lie, in place of a (LOGSUM, GRAD) or of b (dW)
+template <int MODE> struct Call {
+  static constexpr int PRODUCTS = MODE == GRADS ? 2 : 1;
+  Args a[PRODUCTS];
+  Maps maps[PRODUCTS];
+};
 
 __device__ __forceinline__ uint32_t cta_rank() {
   uint32_t r;
@@ -473,27 +500,17 @@ __device__ __forceinline__ void parts_of(int products, int i, int& a, int& b) {
 
 // What a launch works on, the same in all its warps and (for DX) in the kernel that joins the sums
 struct Work { int tiles_m, tiles_n, splits, chunks, per; };
-// Parts of the contraction: the number that leaves the fewest units idle in the last round of tiles, a fiftieth less for each part more (its sums are written and read
-// once more), eight at most and eight rounds.  8192 x 2048 from 16384 columns, 256 tiles on 74 pairs: one part 386 us, two 355.
-__host__ __device__ __forceinline__ int split_by_tiles(int tiles, int units, int chunks) {
-  int best = 1, score = 0;
-  for (int s = 1; s <= 8 && tiles > 0 && (s == 1 || (tiles * s <= 8 * units && 4 * s <= chunks)); ++s) {
-    const int rounds = (tiles * s + units - 1) / units, now = (int)(1000ll * tiles * s * (51 - s) / (50ll * rounds * units));
-    if (now > score) best = s, score = now;
-  }
-  return best;
-}
-// ... and of many: as many as there are units for each tile
+// Parts of dW's contraction: as many as there are units for each tile
 __host__ __device__ __forceinline__ int split_by_units(int tiles, int units, int chunks) {
   const int s = units / (tiles > 0 ? tiles : 1), most = chunks / 4;
   return s > most ? (most > 0 ? most : 1) : s > 0 ? s : 1;
 }
-__device__ __forceinline__ Work work_of(const Args& a, int n, int tile_m, int tile_n, int units) {
+__device__ __forceinline__ Work work_of(const Args& a, int n, int tile_m, int tile_n) {
   Work w;
-  w.tiles_m = ((a.M ? a.M : n) + tile_m - 1) / tile_m;
+  w.tiles_m = a.on ? ((a.M ? a.M : n) + tile_m - 1) / tile_m : 0;
   w.tiles_n = (a.N + tile_n - 1) / tile_n;
   w.chunks = ((a.L ? a.L : n) + BK - 1) / BK;
-  w.splits = a.splits ? a.splits : split_by_tiles(w.tiles_m * w.tiles_n, units, a.split_chunks);
+  w.splits = a.splits ? a.splits : a.cut.of(w.tiles_m * w.tiles_n, n);
   w.per = (w.chunks + w.splits - 1) / w.splits;
   return w;
 }
@@ -578,7 +595,7 @@ template <int MODE, int W, int OPT> __device__ __forceinline__ Row row_of(const 
 }
 
 // What a thread does with its sums: row `row` of D, columns col .. col + W - 1
-template <int MODE, int W, int OPT> __device__ __forceinline__ void epilogue(const Args& a, int out_row, float (&acc)[W / 32][32], const Row& me, int n, int row, int col, int part, float* stage) {
+template <int MODE, int W, int OPT, int which> __device__ __forceinline__ void epilogue(const Args& a, int out_row, float (&acc)[W / 32][32], const Row& me, int n, int row, int col, int part, float* stage) {
   const int lane = threadIdx.x & 31;
   if constexpr (MODE == LOGSUM || MODE == GRAD) {
     const int slot = me.slot, c = a.col0 + col;           // of the vocabulary
@@ -658,7 +675,7 @@ template <int MODE, int W, int OPT> __device__ __forceinline__ void epilogue(con
       }
     }
   } else {
-    if (MODE == DW && a.dw != nullptr) {
+    if (MODE == GRADS && which == DW && a.dw != nullptr) {
       const float alpha = a.coef.alpha(n);
       const int v = a.col0 + row;
       if (a.K % 8 == 0) {
@@ -714,10 +731,10 @@ template <int MODE, int W, int OPT> __device__ __forceinline__ void epilogue(con
 // multiplies for both (see k_lin8 in linear_e4m3.cu, whose scheme this is).  Else tiles of 128 x 128.
 // Operands whose contraction runs along memory (K-major: x and W in z, G in dx) come as one box of 128 rows x 64; those whose contraction runs across it (MN-major: W in dx, G and x
 // in dW) as two boxes of 64 rows x 64.
-template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<MODE, PAIR>::THREADS, 1) k_gemm(const __grid_constant__ Args a, const __grid_constant__ Maps maps) {
+template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<MODE, PAIR>::THREADS, 1) k_gemm(const __grid_constant__ Call<MODE> call) {
   using C = Shape<MODE, PAIR>;
   constexpr int BN = C::BN, TILE = C::TILE, W = C::W, STAGES = C::STAGES, EPI = C::EPI;
-  constexpr bool A_MN = MODE == DW, B_MN = MODE == DX || MODE == DW;
+  constexpr bool TWO = MODE == GRADS;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t sbase = smem_u32(smem_raw);
   const uint32_t full = sbase + C::BARS, empty = full + 8 * STAGES, acc_full = empty + 8 * STAGES, acc_empty = acc_full + 16, slot = acc_empty + 16;
@@ -730,9 +747,11 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
     for (int i = 0; i < 2; ++i) mbar_init(acc_full + 8 * i, 1), mbar_init(acc_empty + 8 * i, PAIR ? 2 * EPI : EPI);
     fence_barrier_init();
     fence_proxy_async();
-    tma_prefetch_desc(&maps.a);
-    tma_prefetch_desc(&maps.b);
-    tma_prefetch_desc(&maps.x);
+    for (int i = 0; i < Call<MODE>::PRODUCTS; ++i) {
+      tma_prefetch_desc(&call.maps[i].a);
+      tma_prefetch_desc(&call.maps[i].b);
+      tma_prefetch_desc(&call.maps[i].x);
+    }
   }
   if (warp == 1) {
     if (PAIR) {
@@ -748,15 +767,18 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<uint32_t*>(smem_raw + (slot - sbase));
   wait_for_kernel_before();
-  const int n = *reinterpret_cast<const volatile int*>(a.n);
-  const Work w = work_of(a, n, TILE, BN, step);
-  const bool direct = n == a.direct_rows;
-  const CUtensorMap *const map_a = MODE != DW && MODE != DX && direct ? &maps.x : &maps.a, *const map_b = MODE == DW && direct ? &maps.x : &maps.b;
-  const int items = w.splits * w.tiles_m * w.tiles_n;
+  const int n = *reinterpret_cast<const volatile int*>(call.a[0].n);
+  const Work w0 = work_of(call.a[0], n, TILE, BN), w1 = TWO ? work_of(call.a[Call<MODE>::PRODUCTS - 1], n, TILE, BN) : Work();
+  const bool direct = n == call.a[0].direct_rows;
+  const int items0 = w0.splits * w0.tiles_m * w0.tiles_n, items = items0 + (TWO ? w1.splits * w1.tiles_m * w1.tiles_n : 0);
   const bool aborted = s_abort != 0;
   // the writing warps keep it in shared memory: every register beside their sums counts
-  volatile Work& kept = *reinterpret_cast<Work*>(smem_raw + (slot + 16 - sbase));
-  if (threadIdx.x == 0) kept.tiles_m = w.tiles_m, kept.tiles_n = w.tiles_n, kept.splits = w.splits, kept.chunks = w.chunks, kept.per = w.per;
+  volatile Work* const kept = reinterpret_cast<Work*>(smem_raw + (slot + 16 - sbase));
+  if (threadIdx.x < (TWO ? 2 : 1)) {
+    const Work& w = threadIdx.x ? w1 : w0;
+    volatile Work& k = kept[threadIdx.x];
+    k.tiles_m = w.tiles_m, k.tiles_n = w.tiles_n, k.splits = w.splits, k.chunks = w.chunks, k.per = w.per;
+  }
   __syncthreads();
   if (warp == 0) {
     if (!aborted && elect_one()) {
@@ -765,8 +787,13 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
       bool ok = true;
       for (int i = first; i < items && ok; i += step) {
         int s, m, nn, c0, c1;
-        item_at(w, i, s, m, nn, c0, c1);
-        const int ra = m * TILE + rank * 128, rb = nn * BN + rank * 128;
+        const int which = TWO && i >= items0;
+        const Args& a = call.a[which];
+        const Maps& maps = call.maps[which];
+        const bool a_mn = TWO && which == DW, b_mn = TWO;
+        const CUtensorMap *const map_a = !TWO && direct ? &maps.x : &maps.a, *const map_b = a_mn && direct ? &maps.x : &maps.b;
+        item_at(which ? w1 : w0, i - (which ? items0 : 0), s, m, nn, c0, c1);
+        const int ra = m * TILE + rank * 128, rb = nn * BN + rank * 128, b0 = a_mn ? 0 : a.col0;
         for (int c = c0; c < c1 && ok; ++c)
           for (int p = 0; p < a.products; ++p) {
             ok = mbar_wait(empty + 8 * st, ph);
@@ -785,14 +812,14 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
               if (PAIR) pair_tma_load_2d(to, map, bar, x, y);
               else tma_load_2d(to, map, bar, x, y);
             };
-            const int ya = (int)(pa * a.plane_a), yb = (int)(pb * a.plane_b) + (MODE == LOGSUM || MODE == GRAD || MODE == DX ? a.col0 : 0);
-            if (A_MN) {
+            const int ya = (int)(pa * a.plane_a), yb = (int)(pb * a.plane_b) + b0;
+            if (a_mn) {
               load(to_a, map_a, ra, ya + c * BK);
               load(to_a + HALF / 2, map_a, ra + 64, ya + c * BK);
             } else {
               load(to_a, map_a, c * BK, ya + ra);
             }
-            if (B_MN) {
+            if (b_mn) {
               load(to_b, map_b, rb, yb + c * BK);
               load(to_b + HALF / 2, map_b, rb + 64, yb + c * BK);
             } else {
@@ -810,16 +837,18 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
     }
   } else if (warp == 1) {
     if (!aborted && rank == 0 && elect_one()) {
-      const uint32_t kind = a.fp16 ? 0u : (1u << 7) | (1u << 10);
-      const uint32_t idesc = (1u << 4) | kind | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24);
-      const uint64_t a0 = make_smem_desc(sbase, A_MN ? HALF / 2 : 16, 1024, LAYOUT_SW128), b0 = make_smem_desc(sbase + HALF, B_MN ? HALF / 2 : 16, 1024, LAYOUT_SW128);
-      constexpr uint32_t step_a = A_MN ? 2048 : 32, step_b = B_MN ? 2048 : 32;
+      const uint32_t kind = call.a[0].fp16 ? 0u : (1u << 7) | (1u << 10);
+      const uint32_t shape = (1u << 4) | kind | ((uint32_t)TWO << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24);
+      const uint64_t b0 = make_smem_desc(sbase + HALF, TWO ? HALF / 2 : 16, 1024, LAYOUT_SW128);
+      constexpr uint32_t step_b = TWO ? 2048 : 32;
       int st = 0, ph = 0, buf = 0, acc_ph = 1;
       bool ok = true;
-      for (int i = first; i < items && ok; i += step) {
-        int s, m, nn, c0, c1;
-        item_at(w, i, s, m, nn, c0, c1);
-        const int all = (c1 - c0) * a.products;
+      // A_MN at compile time: descriptors that depend on a branch do not stay in uniform registers
+      auto multiply = [&](auto a_mn, const Args& a, int all) {
+        constexpr bool A_MN = decltype(a_mn)::value;
+        constexpr uint32_t step_a = A_MN ? 2048 : 32;
+        const uint32_t idesc = shape | ((uint32_t)A_MN << 15);
+        const uint64_t a0 = make_smem_desc(sbase, A_MN ? HALF / 2 : 16, 1024, LAYOUT_SW128);
         for (int done = 0; done < all && ok;) {
           ok = mbar_wait(acc_empty + 8 * buf, acc_ph);
           tc_fence_after();
@@ -846,6 +875,14 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
           buf ^= 1;
           if (buf == 0) acc_ph ^= 1;
         }
+      };
+      for (int i = first; i < items && ok; i += step) {
+        int s, m, nn, c0, c1;
+        const int which = TWO && i >= items0;
+        item_at(which ? w1 : w0, i - (which ? items0 : 0), s, m, nn, c0, c1);
+        const int all = (c1 - c0) * call.a[0].products;
+        if (TWO && which == DW) multiply(std::integral_constant<bool, TWO>(), call.a[Call<MODE>::PRODUCTS - 1], all);
+        else multiply(std::integral_constant<bool, false>(), call.a[0], all);
       }
       if (!ok) report(&g_vocab_status, ERR_MMA_WAIT);
     }
@@ -854,9 +891,15 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
     int buf = 0, ph = 0;
     bool lost = aborted;
     float acc[W / 32][32];
-    for (int i = first; i < kept.splits * kept.tiles_m * kept.tiles_n; i += step) {
-      int s, m, nn, c0, c1;
-      item_at(kept, i, s, m, nn, c0, c1);
+    for (int i = first;; i += step) {
+      int s, m, nn, c0, c1, which = 0, at = i;
+      const int before = kept[0].splits * kept[0].tiles_m * kept[0].tiles_n;
+      if (i >= before) {
+        if (!TWO || i >= before + kept[1].splits * kept[1].tiles_m * kept[1].tiles_n) break;
+        which = 1, at = i - before;
+      }
+      const Args& a = call.a[which];
+      item_at(kept[which], at, s, m, nn, c0, c1);
       const int all = (c1 - c0) * a.products;
       const int row = m * TILE + rank * 128 + q * 32 + lane, col = nn * BN + share * W;
       const Row me = row_of<MODE, W, OPT>(a, n, row, a.col0 + col);
@@ -904,7 +947,10 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
       if (lost)
 #pragma unroll
         for (int g = 0; g < W; ++g) acc[g / 32][g % 32] = not_a_number();
-      epilogue<MODE, W, OPT>(a, s * kept.tiles_m * TILE + row, acc, me, n, row, col, nn * (BN / W) + share, reinterpret_cast<float*>(smem_raw + C::STAGED) + (warp - 2) * 32 * 17);
+      float* const stage = reinterpret_cast<float*>(smem_raw + C::STAGED) + (warp - 2) * 32 * 17;
+      const int out_row = s * kept[which].tiles_m * TILE + row, part = nn * (BN / W) + share;
+      if (TWO && which == DW) epilogue<MODE, W, OPT, DW>(call.a[Call<MODE>::PRODUCTS - 1], out_row, acc, me, n, row, col, part, stage);
+      else epilogue<MODE, W, OPT, DX>(call.a[0], out_row, acc, me, n, row, col, part, stage);
     }
   }
   tc_fence_before();
@@ -1020,12 +1066,13 @@ __global__ void __launch_bounds__(1024) k_unit(const Plan plan, const float* g, 
 struct Join {
   const int* slot;                                        // or null: rows as they are
   const float* part; long long ldp;                       // [splits][plane rows][ldp]
-  int splits, tile, tiles_n, units, chunks;               // splits 0: as k_gemm<DX> had them
+  int splits, tile, tiles_n;                              // splits 0: as k_gemm<GRADS> had them
+  Parts cut;
   long long plane;                                        // rows of a split (splits given)
   void* out; int type; long long rows, K;
   unsigned ctas;
 };
-struct Bias { const float* colsum; long long ldg; int columns; void* db; int type; unsigned ctas; };
+struct Bias { const float* colsum; long long ldg; int columns; void* db; int type; int wide; unsigned ctas; };
 struct Leave { const int* head; Coef coef; Join j[2]; Bias b; };
 
 __device__ __forceinline__ void store8(const Join& a, long long r, long long c, const float (&f)[8]) {
@@ -1052,7 +1099,7 @@ __device__ __forceinline__ void join(const Join& a, unsigned cta, int n, float a
   long long plane = a.plane;
   if (splits == 0) {
     const int tiles_m = (n + a.tile - 1) / a.tile;
-    splits = split_by_tiles(tiles_m * a.tiles_n, a.units, a.chunks);
+    splits = a.cut.of(tiles_m * a.tiles_n, n);
     plane = (long long)tiles_m * a.tile;
   }
   const int pieces = (int)((a.K + 7) / 8);
@@ -1060,8 +1107,34 @@ __device__ __forceinline__ void join(const Join& a, unsigned cta, int n, float a
   auto place = [&](long long i, long long& r, int& c) {
     r = all < 0x7fffffff ? (unsigned)i / (unsigned)pieces : i / pieces, c = (int)(i - r * pieces) * 8;
   };
-  if (splits < 8) {                                        // up to four pieces a thread under way
-    const long long step = a.ctas * 256ll;
+  const long long step = a.ctas * 256ll;
+  if (splits <= 8 && all <= step) {                        // a piece a thread: four of its parts under way
+    const long long i = cta * 256ll + threadIdx.x;
+    if (i >= all) return;
+    long long r;
+    int c;
+    place(i, r, c);
+    const long long from = a.slot ? a.slot[r] : r;
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (from >= 0)
+      for (int s = 0; s < splits; s += 4) {
+        Piece<float, 8> p[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (s + u < splits) p[u].load(a.part + ((s + u) * plane + from) * a.ldp + c);
+          else p[u].zero();
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] += p[u].at(e);
+      }
+    const float by = from < 0 ? 0.f : alpha;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= by;
+    store8(a, r, c, f);
+    return;
+  }
+  if (splits <= 8) {                                       // up to four pieces a thread under way
     for (long long i0 = cta * 256ll + threadIdx.x; i0 < all; i0 += 4 * step) {
       float f[4][8];
       long long r[4], from[4];
@@ -1098,10 +1171,10 @@ __device__ __forceinline__ void join(const Join& a, unsigned cta, int n, float a
     }
     return;
   }
-  // of many splits, eight threads take a share each
-  const int share = threadIdx.x & 7, each = (splits + 7) / 8;
+  // of many splits, the eight warps take a share each
+  const int lane = threadIdx.x & 31, share = threadIdx.x >> 5, each = (splits + 7) / 8;
   for (long long i0 = cta * 32ll; i0 < all; i0 += a.ctas * 32ll) {
-    const long long i = i0 + threadIdx.x / 8;
+    const long long i = i0 + lane;
     long long r;
     int c;
     place(min(i, all - 1), r, c);
@@ -1122,7 +1195,7 @@ __device__ __forceinline__ void join(const Join& a, unsigned cta, int n, float a
     if (share > 0 || i >= all) continue;
     for (int o = 1; o < 8; ++o)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] += shared[threadIdx.x + o][e];
+      for (int e = 0; e < 8; ++e) f[e] += shared[lane + 32 * o][e];
     const float by = from < 0 ? 0.f : alpha;
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] *= by;
@@ -1135,22 +1208,26 @@ __global__ void __launch_bounds__(256) k_out(const __grid_constant__ Leave a) {
   wait_for_kernel_before();
   const int n = *reinterpret_cast<const volatile int*>(a.head);
   const float alpha = *reinterpret_cast<volatile int*>(&g_vocab_status) != 0 ? not_a_number() : a.coef.alpha(n);
-  if (blockIdx.x < a.j[0].ctas) {
-    join(a.j[0], blockIdx.x, n, alpha, shared);
-  } else if (blockIdx.x < a.j[0].ctas + a.j[1].ctas) {
-    join(a.j[1], blockIdx.x - a.j[0].ctas, n, alpha, shared);
-  } else {                                                 // 32 columns a CTA, eight shares of the blocks of 32 rows
-    const int lane = threadIdx.x & 31, share = threadIdx.x >> 5, c = (blockIdx.x - a.j[0].ctas - a.j[1].ctas) * 32 + lane;
-    float s = 0.f;
+  // the long chains of sums first: db (32 columns a CTA and eight shares of the blocks of 32 rows; of many blocks 8 columns and 32 shares); dw; dx
+  if (blockIdx.x < a.b.ctas) {
+    const int wide = a.b.wide, lane = threadIdx.x & (wide - 1), shares = 256 / wide, share = threadIdx.x / wide, c = blockIdx.x * wide + lane;
+    float *const flat = &shared[0][0], s = 0.f;
     if (c < a.b.columns)
 #pragma unroll 8
-      for (int k = share; k < (n + 31) / 32; k += 8) s += a.b.colsum[k * a.b.ldg + c];
-    shared[threadIdx.x][0] = s;
+      for (int k = share; k < (n + 31) / 32; k += shares) s += a.b.colsum[k * a.b.ldg + c];
+    if (wide == 8) {
+      s += __shfl_xor_sync(0xffffffffu, s, 8);
+      s += __shfl_xor_sync(0xffffffffu, s, 16);
+    }
+    if ((threadIdx.x & 31) < wide) flat[threadIdx.x] = s;
     __syncthreads();
-    if (share > 0 || c >= a.b.columns) return;
-#pragma unroll
-    for (int i = 1; i < 8; ++i) s += shared[threadIdx.x + 32 * i][0];
+    if (threadIdx.x >= wide || c >= a.b.columns) return;
+    for (int i = 1; i < 8; ++i) s += flat[32 * i + threadIdx.x];
     store_any(a.b.db, a.b.type, c, s * alpha);
+  } else if (blockIdx.x < a.b.ctas + a.j[1].ctas) {
+    join(a.j[1], blockIdx.x - a.b.ctas, n, alpha, shared);
+  } else {
+    join(a.j[0], blockIdx.x - a.b.ctas - a.j[1].ctas, n, alpha, shared);
   }
 }
 
@@ -1218,12 +1295,12 @@ template <int MODE, bool PAIR, int OPT = 0> int units_of(int* units) {
   *units = n;
   return SPION_OK;
 }
-template <int MODE, bool PAIR, int OPT> int launch_gemm(const Args& a, const Maps& maps, long long most_items, cudaStream_t st) {
+template <int MODE, bool PAIR, int OPT> int launch_gemm(const Call<MODE>& call, long long most_items, cudaStream_t st) {
   int units;
   const int rc = units_of<MODE, PAIR, OPT>(&units);
   if (rc != SPION_OK) return rc;
-  // DX splits its contraction by the number of units: it always has all of them
-  const int use = a.splits == 0 ? units : (int)std::min<long long>(units, std::max<long long>(most_items, 1));
+  // dx splits its contraction by the number of units: it always has all of them
+  const int use = MODE == GRADS ? units : (int)std::min<long long>(units, std::max<long long>(most_items, 1));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1231,28 +1308,28 @@ template <int MODE, bool PAIR, int OPT> int launch_gemm(const Args& a, const Map
   at[1].id = cudaLaunchAttributeClusterDimension;
   at[1].val.clusterDim.x = 2, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.gridDim = dim3(PAIR ? 2 * use : use), cfg.blockDim = dim3(Shape<MODE, PAIR>::THREADS), cfg.dynamicSmemBytes = Shape<MODE, PAIR>::SMEM, cfg.stream = st, cfg.attrs = at, cfg.numAttrs = PAIR ? 2 : 1;
-  SPION_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_gemm<MODE, PAIR, OPT>, a, maps));
+  SPION_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_gemm<MODE, PAIR, OPT>, call));
   return SPION_OK;
 }
-template <int MODE, int OPT> int launch_gemm(bool pair, const Args& a, const Maps& maps, long long most_items, cudaStream_t st) {
-  return pair ? launch_gemm<MODE, true, OPT>(a, maps, most_items, st) : launch_gemm<MODE, false, OPT>(a, maps, most_items, st);
+template <int MODE, int OPT> int launch_gemm(bool pair, const Call<MODE>& call, long long most_items, cudaStream_t st) {
+  return pair ? launch_gemm<MODE, true, OPT>(call, most_items, st) : launch_gemm<MODE, false, OPT>(call, most_items, st);
 }
-template <int MODE> int launch_gemm(bool pair, const Args& a, const Maps& maps, long long most_items, cudaStream_t st) {
-  if constexpr (MODE == LOGSUM) return a.k == 1 ? launch_gemm<MODE, ONE>(pair, a, maps, most_items, st) : launch_gemm<MODE, 0>(pair, a, maps, most_items, st);
-  if constexpr (MODE == GRAD)
-    switch ((a.k == 1 ? ONE : 0) | (a.products > 1 ? THREE : 0) | (a.colsum != nullptr ? COLUMNS : 0)) {
-      case 0: return launch_gemm<MODE, 0>(pair, a, maps, most_items, st);
-      case 1: return launch_gemm<MODE, 1>(pair, a, maps, most_items, st);
-      case 2: return launch_gemm<MODE, 2>(pair, a, maps, most_items, st);
-      case 3: return launch_gemm<MODE, 3>(pair, a, maps, most_items, st);
-      case 4: return launch_gemm<MODE, 4>(pair, a, maps, most_items, st);
-      case 5: return launch_gemm<MODE, 5>(pair, a, maps, most_items, st);
-      case 6: return launch_gemm<MODE, 6>(pair, a, maps, most_items, st);
-      default: return launch_gemm<MODE, 7>(pair, a, maps, most_items, st);
-    }
-  return launch_gemm<MODE, 0>(pair, a, maps, most_items, st);
+int launch_logsum(bool pair, const Call<LOGSUM>& call, long long most_items, cudaStream_t st) {
+  return call.a[0].k == 1 ? launch_gemm<LOGSUM, ONE>(pair, call, most_items, st) : launch_gemm<LOGSUM, 0>(pair, call, most_items, st);
 }
-
+int launch_grad(bool pair, const Call<GRAD>& call, long long most_items, cudaStream_t st) {
+  const Args& a = call.a[0];
+  switch ((a.k == 1 ? ONE : 0) | (a.products > 1 ? THREE : 0) | (a.colsum != nullptr ? COLUMNS : 0)) {
+    case 0: return launch_gemm<GRAD, 0>(pair, call, most_items, st);
+    case 1: return launch_gemm<GRAD, 1>(pair, call, most_items, st);
+    case 2: return launch_gemm<GRAD, 2>(pair, call, most_items, st);
+    case 3: return launch_gemm<GRAD, 3>(pair, call, most_items, st);
+    case 4: return launch_gemm<GRAD, 4>(pair, call, most_items, st);
+    case 5: return launch_gemm<GRAD, 5>(pair, call, most_items, st);
+    case 6: return launch_gemm<GRAD, 6>(pair, call, most_items, st);
+    default: return launch_gemm<GRAD, 7>(pair, call, most_items, st);
+  }
+}
 constexpr long long up(long long x, long long to) { return (x + to - 1) / to * to; }
 constexpr long long tiles_of(long long x, long long tile) { return (x + tile - 1) / tile; }
 constexpr int CHAIN = 16;                                 // 64 steps of 16
@@ -1266,9 +1343,9 @@ struct Layout {
   bool kept;                                              // the operands' copies stay for the backward
   bool self;                                              // CTAs count for themselves
   long long chunk;                                        // rows of a CTA of k_prepare
-  bool pair_z, pair_dx, pair_dw;
+  bool pair_z, pair_g;                                    // tiles of pairs of CTAs: in z; in dx and dW
   long long Gp;                                           // columns of a piece of the vocabulary
-  int dw_splits;
+  int tile_g, dw_splits;
   size_t keep;                                            // bytes of the plan
   size_t xs, w, bias2;                                    // in the plan (kept) or in both workspaces
   size_t part, zt, cta_loss, counts, q, forward;
@@ -1300,13 +1377,12 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   if (sms <= 0) return SPION_ERR_CUDA;
   const int pairs = sms / 2;
   // Tiles of pairs where every pair has one, else four times as many small ones.
-  auto pair = [&](long long m, long long n) { return m > 128 && n > 128 && tiles_of(m, 256) * tiles_of(n, 256) >= pairs; };
-  l->pair_z = pair(l->T, l->V);
+  auto tiles = [](long long m, long long n) { return m > 128 && n > 128 ? tiles_of(m, 256) * tiles_of(n, 256) : 0; };
+  l->pair_z = tiles(l->T, l->V) >= pairs;
   l->Gp = std::min(l->Vp, std::max<long long>(PAD, PIECE_BYTES / (2 * l->planes * l->Tp) / PAD * PAD));
-  l->pair_dx = pair(l->T, l->K);
-  l->pair_dw = pair(l->Gp, l->K);
-  const long long dw_tiles = l->pair_dw ? tiles_of(l->Gp, 256) * tiles_of(l->K, 256) : tiles_of(l->Gp, 128) * tiles_of(l->K, 128);
-  l->dw_splits = l->pair_dw ? 1 : split_by_units((int)std::min<long long>(dw_tiles, 1 << 20), sms, (int)tiles_of(l->T, BK));
+  l->pair_g = tiles(l->T, l->K) > 0 && tiles(l->T, l->K) + tiles(l->Gp, l->K) >= pairs;
+  l->tile_g = l->pair_g ? 256 : 128;
+  l->dw_splits = split_by_units((int)std::min<long long>(tiles_of(l->Gp, l->tile_g) * tiles_of(l->K, l->tile_g), 1 << 20), l->pair_g ? pairs : sms, (int)tiles_of(l->T, BK));
   size_t at = 0;
   auto take = [&](long long bytes) {
     const size_t here = at;
@@ -1330,10 +1406,10 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   l->forward = at;
   at = both;
   l->g = take(2 * l->planes * l->Tp * l->Gp);
-  // (as split_by_tiles cuts them: one part, or eight rounds of tiles at most)
-  const long long tile = l->pair_dx ? 256 : 128, tn = tiles_of(l->K, tile), most_m = 8 * (l->pair_dx ? pairs : sms) / tn;
+  // (as Parts cuts them: one part, or eight rounds of tiles at most)
+  const long long tile = l->tile_g, tn = tiles_of(l->K, tile), most_m = 8 * (l->pair_g ? pairs : sms) / tn;
   l->dxp = take(4 * std::max(tiles_of(l->T, tile), std::min(most_m, 8 * tiles_of(l->T, tile))) * tile * l->Kp);
-  l->dwp = take(l->dw_splits > 1 ? 4 * l->dw_splits * up(l->Gp, l->pair_dw ? 256 : 128) * l->Kp : 0);
+  l->dwp = take(l->dw_splits > 1 ? 4 * l->dw_splits * up(l->Gp, l->tile_g) * l->Kp : 0);
   l->colsum = take(4 * (l->Tp / 32) * l->Gp);
   l->unit = take(256);
   l->backward = at;
@@ -1385,6 +1461,7 @@ template <bool FIRST> int launch_prepare(const spion_vocab_problem* p, const Pre
 // What the two passes over z have in common
 int logits_args(const spion_vocab_problem* p, const Layout& l, const Prep& prep, Args* a, Maps* maps) {
   *a = Args();
+  a->on = 1;
   a->n = prep.plan.head;
   a->products = l.planes == 1 ? 1 : 6;
   a->plane_a = l.Tp, a->plane_b = l.Vp;
@@ -1443,12 +1520,12 @@ extern "C" int spion_vocab_loss_forward(const spion_vocab_problem* p, float* los
   prep.loss_rows = p->reduction == 0 ? loss : nullptr;
   if (!l.self) SPION_CUDA_TRY(launch_after(k_flags, dim3((unsigned)tiles_of(tiles_of(l.T, l.chunk), prep.teacher ? 1 : 8)), dim3(256), 0, st, prep));
   if ((rc = launch_prepare<true>(p, prep, st)) != SPION_OK) return rc;
-  Args a;
-  Maps maps;
-  if ((rc = logits_args(p, l, prep, &a, &maps)) != SPION_OK) return rc;
+  Call<LOGSUM> call;
+  Args& a = call.a[0];
+  if ((rc = logits_args(p, l, prep, &a, &call.maps[0])) != SPION_OK) return rc;
   const int tile = l.pair_z ? 256 : 128;
   a.N = (int)l.V, a.part = (float2*)(ws + l.part), a.parts = (int)(l.pair_z ? 4 * tiles_of(l.V, 256) : 2 * tiles_of(l.V, 128)), a.zt = prep.zt;
-  if ((rc = launch_gemm<LOGSUM>(l.pair_z, a, maps, tiles_of(l.T, tile) * tiles_of(l.V, tile), st)) != SPION_OK) return rc;
+  if ((rc = launch_logsum(l.pair_z, call, tiles_of(l.T, tile) * tiles_of(l.V, tile), st)) != SPION_OK) return rc;
   const Finish f = {prep.plan, (int)l.Tp, (int)l.k, a.part, a.parts, prep.zt, loss, (double*)(ws + l.cta_loss), p->reduction};
   const int lanes = std::max<int>(a.parts, l.k) <= 16 ? 4 : std::max<int>(a.parts, l.k) <= 32 ? 8 : 32;
   const dim3 grid((unsigned)std::min<long long>(tiles_of(l.T, 256 / lanes), std::min(4 * sm_count(), FINISH_CTAS)));
@@ -1476,9 +1553,11 @@ extern "C" int spion_vocab_loss_backward(const spion_vocab_problem* p, const flo
   const float gscale = p->type == SPION_F16 ? 8192.f : 1.f;
   if (p->reduction == 0) SPION_CUDA_TRY(launch_after(k_unit, dim3(1), dim3(1024), 0, st, prep.plan, g, unit));
   if (!l.kept && (rc = launch_prepare<false>(p, prep, st)) != SPION_OK) return rc;
-  Args z;
-  Maps zm, xm, wm;
-  if ((rc = logits_args(p, l, prep, &z, &zm)) != SPION_OK) return rc;
+  Call<GRAD> grad;
+  Call<GRADS> grads;
+  Args& z = grad.a[0];
+  Maps &xm = grads.maps[DX], &wm = grads.maps[DW];
+  if ((rc = logits_args(p, l, prep, &z, &grad.maps[0])) != SPION_OK) return rc;
   if ((rc = map_of(&xm.a, G, l.Gp, l.planes * l.Tp, l.Gp, 128)) != SPION_OK) return rc;
   if ((rc = l.copy_w ? map_of(&xm.b, prep.ws, l.Kp, l.planes * l.Vp, l.Kp, 64) : map_of(&xm.b, p->w, l.K, l.V, l.ldw, 64)) != SPION_OK) return rc;
   xm.x = xm.a;
@@ -1487,8 +1566,8 @@ extern "C" int spion_vocab_loss_backward(const spion_vocab_problem* p, const flo
   wm.x = wm.b;
   if (l.direct && (rc = map_of(&wm.x, p->x, l.K, l.T, p->ldx, 64)) != SPION_OK) return rc;
   int dx_units = 0;
-  if ((rc = l.pair_dx ? units_of<DX, true>(&dx_units) : units_of<DX, false>(&dx_units)) != SPION_OK) return rc;
-  const int tz = l.pair_z ? 256 : 128, tx = l.pair_dx ? 256 : 128, tw = l.pair_dw ? 256 : 128;
+  if ((rc = l.pair_g ? units_of<GRADS, true>(&dx_units) : units_of<GRADS, false>(&dx_units)) != SPION_OK) return rc;
+  const int tz = l.pair_z ? 256 : 128, tg = l.tile_g;
   z.g = p->reduction == 0 ? g : nullptr, z.G = G, z.ldg = l.Gp, z.gscale = gscale;
   z.coef = {p->reduction == 0 ? nullptr : g, unit, p->reduction == 1, prep.inv_tau / gscale};
   z.colsum = db != nullptr ? (float*)(ws + l.colsum) : nullptr;
@@ -1497,33 +1576,32 @@ extern "C" int spion_vocab_loss_backward(const spion_vocab_problem* p, const flo
   for (long long c = 0; c < l.V; c += l.Gp) {
     const long long columns = std::min(l.Gp, l.V - c), padded = up(columns, PAD);
     z.col0 = (int)c, z.N = (int)padded;
-    if ((rc = launch_gemm<GRAD>(l.pair_z, z, zm, tiles_of(l.T, tz) * tiles_of(padded, tz), st)) != SPION_OK) return rc;
+    if ((rc = launch_grad(l.pair_z, grad, tiles_of(l.T, tz) * tiles_of(padded, tz), st)) != SPION_OK) return rc;
     Args b = z;
     b.chain = l.planes == 3 ? CHAIN : LONG_CHAIN;
     Leave out = {};
     out.head = prep.plan.head, out.coef = z.coef;
-    if (dx != nullptr) {
-      Args d = b;
-      d.N = (int)l.K, d.L = (int)columns, d.splits = 0, d.split_chunks = dx_chunks;
-      d.plane_a = l.Tp, d.plane_b = l.Vp;
-      d.out = (float*)(ws + l.dxp), d.ldo = l.Kp, d.add = c > 0;
-      if ((rc = launch_gemm<DX>(l.pair_dx, d, xm, 0, st)) != SPION_OK) return rc;
-      if (c + l.Gp >= l.V)
-        out.j[0] = {prep.plan.slot, d.out, l.Kp, 0, tx, (int)tiles_of(l.K, tx), dx_units, dx_chunks, 0, dx, p->type, l.T, l.K,
-                    (unsigned)std::min<long long>(tiles_of(l.T * tiles_of(l.K, 8), 256), most)};
-    }
-    if (dw != nullptr) {
-      Args d = b;
-      d.M = (int)padded, d.N = (int)l.K, d.L = 0, d.splits = l.dw_splits;
-      d.plane_a = l.Tp, d.plane_b = l.Tp;
-      d.out = (float*)(ws + l.dwp), d.ldo = l.Kp, d.add = 0;
-      d.dw = l.dw_splits == 1 ? dw : nullptr, d.dw_type = p->type, d.K = l.K, d.V = (int)l.V;
-      if ((rc = launch_gemm<DW>(l.pair_dw, d, wm, tiles_of(padded, tw) * tiles_of(l.K, tw) * l.dw_splits, st)) != SPION_OK) return rc;
-      if (l.dw_splits > 1)
-        out.j[1] = {nullptr, d.out, l.Kp, l.dw_splits, tw, 0, 0, 0, up(padded, tw), static_cast<char*>(dw) + c * l.K * type_size(p->type), p->type, columns, l.K,
-                    (unsigned)std::min<long long>(tiles_of(columns * tiles_of(l.K, 8), l.dw_splits >= 8 ? 32 : 256), most)};
-    }
-    if (db != nullptr) out.b = {z.colsum, l.Gp, (int)columns, static_cast<char*>(db) + c * type_size(db_type), db_type, (unsigned)tiles_of(columns, 32)};
+    Args &d = grads.a[DX], &e = grads.a[DW];
+    d = e = b;
+    d.on = dx != nullptr, e.on = dw != nullptr;
+    const bool together = dx != nullptr && dw != nullptr;
+    d.N = (int)l.K, d.L = (int)columns, d.splits = 0;
+    d.cut = {dx_units, dx_chunks, together ? (int)(tiles_of(up(std::min(l.Gp, l.V), PAD), tg) * tiles_of(l.K, tg) * l.dw_splits) : 0, l.dw_splits};
+    d.plane_a = l.Tp, d.plane_b = l.Vp;
+    d.out = (float*)(ws + l.dxp), d.ldo = l.Kp, d.add = c > 0;
+    e.M = (int)padded, e.N = (int)l.K, e.L = 0, e.splits = l.dw_splits;
+    e.plane_a = l.Tp, e.plane_b = l.Tp;
+    e.out = (float*)(ws + l.dwp), e.ldo = l.Kp, e.add = 0;
+    e.dw = l.dw_splits == 1 ? dw : nullptr, e.dw_type = p->type, e.K = l.K, e.V = (int)l.V;
+    if ((dx != nullptr || dw != nullptr) && (rc = launch_gemm<GRADS, 0>(l.pair_g, grads, 0, st)) != SPION_OK) return rc;
+    if (dx != nullptr && c + l.Gp >= l.V)
+      out.j[0] = {prep.plan.slot, d.out, l.Kp, 0, tg, (int)tiles_of(l.K, tg), d.cut, 0, dx, p->type, l.T, l.K,
+                  (unsigned)std::min<long long>(tiles_of(l.T * tiles_of(l.K, 8), 256), most)};
+    if (dw != nullptr && l.dw_splits > 1)
+      out.j[1] = {nullptr, e.out, l.Kp, l.dw_splits, tg, 0, {}, up(padded, tg), static_cast<char*>(dw) + c * l.K * type_size(p->type), p->type, columns, l.K,
+                  (unsigned)std::min<long long>(tiles_of(columns * tiles_of(l.K, 8), l.dw_splits >= 8 ? 32 : 256), most)};
+    if (db != nullptr) out.b = {z.colsum, l.Gp, (int)columns, static_cast<char*>(db) + c * type_size(db_type), db_type, l.T > 16384 ? 8 : 32,
+                                 (unsigned)tiles_of(columns, l.T > 16384 ? 8 : 32)};
     const unsigned ctas = out.j[0].ctas + out.j[1].ctas + out.b.ctas;
     if (ctas > 0) SPION_CUDA_TRY(launch_after(k_out, dim3(ctas), dim3(256), 0, st, out));
   }
