@@ -17,8 +17,8 @@
 // accumulator where a result has 32 bits; what the accumulators hold is added in fp32 registers.  fp32 operands are three bf16 parts each (8 + 8 + 8 bits, exact) and
 // six products; what is dropped is below 2^-25 of a product.
 //
-// G is rounded to the type that W has, after it was formed in fp32: the products' other operand has those bits, and their results are rounded to them.  G holds g_t
-// over the largest |g_t| (and 2^13 times that in fp16, whose smallest numbers probabilities of a large vocabulary fall below); the factor comes back in fp32.
+// G is rounded to the type that W has, after it was formed in fp32: the products' other operand has those bits, and their results are rounded to them.  In fp16, whose
+// smallest numbers probabilities of a large vocabulary fall below, G holds 2^13 g_t over the largest |g_t|; the factor comes back in fp32.
 // The bias's gradient is summed from G before it is rounded.
 #include <algorithm>
 #include <type_traits>
@@ -30,12 +30,6 @@
 using namespace tc;
 using namespace rows;
 
-#ifndef SPION_GROUP
-#define SPION_GROUP 8
-#endif
-#ifndef SPION_PIECE
-#define SPION_PIECE 512ll
-#endif
 namespace {
 
 // Set by a bounded wait that gave up (see g_lin_status in linear.cu); results after it are NaN until it has been reported.
@@ -391,14 +385,14 @@ template <int MODE, bool PAIR> struct Shape {
 };
 static_assert(Shape<GRADS, true>::SMEM <= 232448 && Shape<GRADS, false>::SMEM <= 232448, "shared memory of a multiprocessor");
 
-// What the products with G are multiplied with.  Rows with a g each: it comes from k_unit.
+// What the products with G are multiplied with.
 struct Coef {
   const float* g;                                         // one number, or null
-  const float* unit;                                      // [0]: the largest |g|, rounded to a power of two; [1]: its reciprocal
+  const float* unit;                                      // fp16: [0]: the largest |g|, rounded to a power of two; [1]: its reciprocal; else null
   int mean;
   float scale;                                            // 1 / (tau gscale)
   __device__ __forceinline__ float alpha(int n) const {
-    if (g == nullptr) return unit[0] * scale;
+    if (g == nullptr) return unit ? unit[0] * scale : scale;
     return n > 0 ? (mean ? *g / (float)n : *g) * scale : 0.f;
   }
 };
@@ -426,6 +420,7 @@ struct Args {
   int products;                                           // 1, or 6 of three parts
   long long plane_a, plane_b;                             // rows of a part in the maps
   int M, N, L;                                            // rows of D (0: n), columns of D, contraction (0: n)
+  int row0, most;                                         // first slot and slots of a launch (0: all)
   int col0;                                               // first column of the piece of the vocabulary
   int chain;                                              // (chunk, product) pairs that one accumulator takes
   int splits;                                             // of the contraction (0: by `cut`)
@@ -507,21 +502,24 @@ __host__ __device__ __forceinline__ int split_by_units(int tiles, int units, int
 }
 __device__ __forceinline__ Work work_of(const Args& a, int n, int tile_m, int tile_n) {
   Work w;
-  w.tiles_m = a.on ? ((a.M ? a.M : n) + tile_m - 1) / tile_m : 0;
+  const int rows_ = a.M ? a.M : a.most ? min(a.most, max(0, n - a.row0)) : n;
+  w.tiles_m = a.on ? (rows_ + tile_m - 1) / tile_m : 0;
   w.tiles_n = (a.N + tile_n - 1) / tile_n;
   w.chunks = ((a.L ? a.L : n) + BK - 1) / BK;
   w.splits = a.splits ? a.splits : a.cut.of(w.tiles_m * w.tiles_n, n);
   w.per = (w.chunks + w.splits - 1) / w.splits;
   return w;
 }
-// Tiles in groups of 8 rows of tiles, column by column inside a group: the CTAs that run at a time share their operands in L2.
+// Tiles in groups of 8 rows of tiles, column by column inside a group: the CTAs that run at a time share their operands in L2 (8192 x 4096 to 128000, forward and
+// backward: groups of 4 28.5 ms, 8 and 16 27.3).
+constexpr int GROUP = 8;
 template <class Wk> __device__ __forceinline__ void item_at(const Wk& w, int i, int& s, int& m, int& n, int& c0, int& c1) {
   const int tiles = w.tiles_m * w.tiles_n;
   s = i / tiles;
   i -= s * tiles;
-  const int per = SPION_GROUP * w.tiles_n, group = i / per, rows_here = min(SPION_GROUP, (int)w.tiles_m - SPION_GROUP * group), j = i - group * per;
+  const int per = GROUP * w.tiles_n, group = i / per, rows_here = min(GROUP, (int)w.tiles_m - GROUP * group), j = i - group * per;
   n = j / rows_here;
-  m = SPION_GROUP * group + j - n * rows_here;
+  m = GROUP * group + j - n * rows_here;
   const int chunks = w.chunks, share = w.per;
   c0 = min(s * share, chunks), c1 = min(c0 + share, chunks);
 }
@@ -588,7 +586,7 @@ template <int MODE, int W, int OPT> __device__ __forceinline__ Row row_of(const 
     }
     if (MODE == GRAD) {
       r.lse = a.plan.lse[r.slot];
-      r.r = (a.g ? a.g[a.plan.row[r.slot]] * a.coef.unit[1] : 1.f) * a.gscale;
+      r.r = (a.g ? a.g[a.plan.row[r.slot]] * (a.coef.unit ? a.coef.unit[1] : 1.f) : 1.f) * a.gscale;
     }
   }
   return r;
@@ -620,7 +618,7 @@ template <int MODE, int W, int OPT, int which> __device__ __forceinline__ void e
       const float from = top == -INFINITY ? 0.f : top;
 #pragma unroll
       for (int g = 0; g < W; ++g) sum += ex2(acc[g / 32][g % 32] - from);
-      if (me.in) a.part[(long long)row * a.parts + part] = make_float2(top, sum);
+      if (me.in) a.part[(long long)(row - a.row0) * a.parts + part] = make_float2(top, sum);
     } else {
       const float lse = me.lse, r = me.r;
 #pragma unroll
@@ -793,7 +791,7 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
         const bool a_mn = TWO && which == DW, b_mn = TWO;
         const CUtensorMap *const map_a = !TWO && direct ? &maps.x : &maps.a, *const map_b = a_mn && direct ? &maps.x : &maps.b;
         item_at(which ? w1 : w0, i - (which ? items0 : 0), s, m, nn, c0, c1);
-        const int ra = m * TILE + rank * 128, rb = nn * BN + rank * 128, b0 = a_mn ? 0 : a.col0;
+        const int ra = m * TILE + rank * 128 + (MODE == LOGSUM ? a.row0 : 0), rb = nn * BN + rank * 128, b0 = a_mn ? 0 : a.col0;
         for (int c = c0; c < c1 && ok; ++c)
           for (int p = 0; p < a.products; ++p) {
             ok = mbar_wait(empty + 8 * st, ph);
@@ -901,7 +899,7 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
       const Args& a = call.a[which];
       item_at(kept[which], at, s, m, nn, c0, c1);
       const int all = (c1 - c0) * a.products;
-      const int row = m * TILE + rank * 128 + q * 32 + lane, col = nn * BN + share * W;
+      const int row = (MODE == LOGSUM ? a.row0 : 0) + m * TILE + rank * 128 + q * 32 + lane, col = nn * BN + share * W;
       const Row me = row_of<MODE, W, OPT>(a, n, row, a.col0 + col);
       // the first chain's sums as they come, the others' on top, sixteen at a time: more would not fit beside the sums
       auto ready = [&] {
@@ -969,11 +967,13 @@ struct Finish {
   const float2* part; int parts;
   const float* zt;
   float* loss;              // [T] (reduction 0) or one number
-  double* cta_loss;         // [CTAs]
+  double* cta_loss;         // [launches][CTAs]
   int reduction;            // 0 none, 1 mean, 2 sum
+  int row0, most;           // slots of this launch
+  int launch, launches;
 };
 template <int LANES> __device__ __forceinline__ float row_loss(const Finish& a, int i, int lane, bool lost, float& lse) {
-  const float2* const p = a.part + (long long)i * a.parts;
+  const float2* const p = a.part + (long long)(i - a.row0) * a.parts;
   float top = -INFINITY, sum = 0.f;
 #pragma unroll 4
   for (int c = lane; c < a.parts; c += LANES) {
@@ -1006,11 +1006,12 @@ template <int LANES> __global__ void __launch_bounds__(256) k_finish(const __gri
   const bool lost = *reinterpret_cast<volatile int*>(&g_vocab_status) != 0;
   constexpr int ROWS = 256 / LANES;
   double s = 0.0;
-  for (int i0 = blockIdx.x * ROWS; i0 < n; i0 += gridDim.x * ROWS) {
+  const int end = min(n, a.row0 + a.most);
+  for (int i0 = a.row0 + blockIdx.x * ROWS; i0 < end; i0 += gridDim.x * ROWS) {
     const int i = i0 + threadIdx.x / LANES;
     float lse;
-    const float loss = row_loss<LANES>(a, min(i, n - 1), lane, lost, lse);      // (all lanes take part in the sums over lanes)
-    if (lane == 0 && i < n) {
+    const float loss = row_loss<LANES>(a, min(i, end - 1), lane, lost, lse);      // (all lanes take part in the sums over lanes)
+    if (lane == 0 && i < end) {
       a.plan.lse[i] = loss != loss ? loss : lse;            // a row without a loss has no gradient either: NaN
       if (a.reduction == 0) a.loss[a.plan.row[i]] = loss;
       s += (double)loss;
@@ -1027,15 +1028,15 @@ template <int LANES> __global__ void __launch_bounds__(256) k_finish(const __gri
   };
   add_up();
   if (threadIdx.x == 0) {
-    a.cta_loss[blockIdx.x] = sums[0];
+    a.cta_loss[a.launch * gridDim.x + blockIdx.x] = sums[0];
     __threadfence();
-    last = atomicAdd(a.plan.head + 1, 1) == (int)gridDim.x - 1;
+    last = atomicAdd(a.plan.head + 1, 1) == (int)gridDim.x * a.launches - 1;
   }
   __syncthreads();
   if (!last) return;
   __threadfence();
   s = 0.0;
-  for (int i = threadIdx.x; i < (int)gridDim.x; i += 256) s += *reinterpret_cast<volatile double*>(a.cta_loss + i);
+  for (int i = threadIdx.x; i < (int)gridDim.x * a.launches; i += 256) s += *reinterpret_cast<volatile double*>(a.cta_loss + i);
   add_up();
   if (threadIdx.x == 0) *a.loss = a.reduction == 2 ? (float)sums[0] : n > 0 ? (float)(sums[0] / n) : not_a_number();
 }
@@ -1048,7 +1049,7 @@ __global__ void __launch_bounds__(1024) k_unit(const Plan plan, const float* g, 
   __shared__ float part[32];
   const int n = *reinterpret_cast<const volatile int*>(plan.head);
   float top = 0.f;
-#pragma unroll 4
+#pragma unroll 8
   for (int i = threadIdx.x; i < n; i += 1024) {
     const float v = fabsf(g[plan.row[i]]);
     if (v < INFINITY) top = fmaxf(top, v);                  // one that is not finite stays its own row's
@@ -1337,11 +1338,12 @@ constexpr int LONG_CHAIN = 64;                            // of a result that is
 
 // Sizes and places of a call
 struct Layout {
-  long long T, Tp, K, Kp, V, Vp, k, ldw;
+  long long T, Tp, K, Kp, V, Vp, k, ldw, parts;           // parts: partial sums of a row
   int planes;
   bool copy_w, direct;                                    // w has to be copied; x can be read as it lies
   bool kept;                                              // the operands' copies stay for the backward
   bool self;                                              // CTAs count for themselves
+  long long rows, launches;                               // slots of a pass over z in the forward, and how many there are
   long long chunk;                                        // rows of a CTA of k_prepare
   bool pair_z, pair_g;                                    // tiles of pairs of CTAs: in z; in dx and dW
   long long Gp;                                           // columns of a piece of the vocabulary
@@ -1351,8 +1353,9 @@ struct Layout {
   size_t part, zt, cta_loss, counts, q, forward;
   size_t g, dxp, dwp, colsum, unit, backward;
 };
-constexpr long long PIECE_BYTES = SPION_PIECE << 20;       // of G
+constexpr long long PIECE_BYTES = 512ll << 20;              // of G: half of it costs 16384 x 1024 to 50021, 2458 rows that count, 1240 us -> 1430, and 8192 x 4096 to 128000 nothing
 constexpr long long KEPT_BYTES = 64ll << 20;              // of copies that stay: small beside the device, and making them again costs launches and, for small calls, most of the time
+constexpr long long PART_BYTES = 256ll << 20;             // of the partial sums of a pass over z: a sixteenth of 16-bit logits, where there are no more than these
 constexpr int FINISH_CTAS = 1024;
 
 int layout_of(const spion_vocab_problem* p, Layout* l) {
@@ -1379,9 +1382,14 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   // Tiles of pairs where every pair has one, else four times as many small ones.
   auto tiles = [](long long m, long long n) { return m > 128 && n > 128 ? tiles_of(m, 256) * tiles_of(n, 256) : 0; };
   l->pair_z = tiles(l->T, l->V) >= pairs;
+  l->parts = l->pair_z ? 4 * tiles_of(l->V, 256) : 2 * tiles_of(l->V, 128);
+  l->rows = std::min(l->Tp, std::max<long long>(PAD, PART_BYTES / (8 * l->parts) / PAD * PAD));
+  l->launches = tiles_of(l->Tp, l->rows);
   l->Gp = std::min(l->Vp, std::max<long long>(PAD, PIECE_BYTES / (2 * l->planes * l->Tp) / PAD * PAD));
   l->pair_g = tiles(l->T, l->K) > 0 && tiles(l->T, l->K) + tiles(l->Gp, l->K) >= pairs;
   l->tile_g = l->pair_g ? 256 : 128;
+  // tiles are counted in 32 bits, eight parts of dx's contraction among them
+  if (tiles_of(l->T, 128) * tiles_of(l->V, 128) > 0x7fffffff || (8 * tiles_of(l->T, 128) + 2 * tiles_of(l->Gp, 128)) * tiles_of(l->K, 128) > 0x7fffffff) return SPION_ERR_SHAPE;
   l->dw_splits = split_by_units((int)std::min<long long>(tiles_of(l->Gp, l->tile_g) * tiles_of(l->K, l->tile_g), 1 << 20), l->pair_g ? pairs : sms, (int)tiles_of(l->T, BK));
   size_t at = 0;
   auto take = [&](long long bytes) {
@@ -1398,9 +1406,9 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   at = 0;
   if (!l->kept) operands();
   const size_t both = at;
-  l->part = take(8 * l->Tp * (l->pair_z ? 4 * tiles_of(l->V, 256) : 2 * tiles_of(l->V, 128)));
+  l->part = take(8 * l->rows * l->parts);
   l->zt = take(4 * l->k * l->Tp);
-  l->cta_loss = take(8 * FINISH_CTAS);
+  l->cta_loss = take(8 * FINISH_CTAS * l->launches);
   l->counts = take(4 * tiles_of(l->T, l->chunk));
   l->q = take(4 * l->T * l->k);
   l->forward = at;
@@ -1524,14 +1532,17 @@ extern "C" int spion_vocab_loss_forward(const spion_vocab_problem* p, float* los
   Args& a = call.a[0];
   if ((rc = logits_args(p, l, prep, &a, &call.maps[0])) != SPION_OK) return rc;
   const int tile = l.pair_z ? 256 : 128;
-  a.N = (int)l.V, a.part = (float2*)(ws + l.part), a.parts = (int)(l.pair_z ? 4 * tiles_of(l.V, 256) : 2 * tiles_of(l.V, 128)), a.zt = prep.zt;
-  if ((rc = launch_logsum(l.pair_z, call, tiles_of(l.T, tile) * tiles_of(l.V, tile), st)) != SPION_OK) return rc;
-  const Finish f = {prep.plan, (int)l.Tp, (int)l.k, a.part, a.parts, prep.zt, loss, (double*)(ws + l.cta_loss), p->reduction};
+  a.N = (int)l.V, a.part = (float2*)(ws + l.part), a.parts = (int)l.parts, a.zt = prep.zt;
   const int lanes = std::max<int>(a.parts, l.k) <= 16 ? 4 : std::max<int>(a.parts, l.k) <= 32 ? 8 : 32;
-  const dim3 grid((unsigned)std::min<long long>(tiles_of(l.T, 256 / lanes), std::min(4 * sm_count(), FINISH_CTAS)));
-  if (lanes == 4) SPION_CUDA_TRY(launch_after(k_finish<4>, grid, dim3(256), 0, st, f));
-  else if (lanes == 8) SPION_CUDA_TRY(launch_after(k_finish<8>, grid, dim3(256), 0, st, f));
-  else SPION_CUDA_TRY(launch_after(k_finish<32>, grid, dim3(256), 0, st, f));
+  const dim3 grid((unsigned)std::min<long long>(tiles_of(std::min(l.T, l.rows), 256 / lanes), std::min(4 * sm_count(), FINISH_CTAS)));
+  for (int pass = 0; pass < l.launches; ++pass) {
+    a.row0 = (int)(pass * l.rows), a.most = (int)l.rows;
+    if ((rc = launch_logsum(l.pair_z, call, tiles_of(std::min(l.T, l.rows), tile) * tiles_of(l.V, tile), st)) != SPION_OK) return rc;
+    const Finish f = {prep.plan, (int)l.Tp, (int)l.k, a.part, a.parts, prep.zt, loss, (double*)(ws + l.cta_loss), p->reduction, a.row0, a.most, pass, (int)l.launches};
+    if (lanes == 4) SPION_CUDA_TRY(launch_after(k_finish<4>, grid, dim3(256), 0, st, f));
+    else if (lanes == 8) SPION_CUDA_TRY(launch_after(k_finish<8>, grid, dim3(256), 0, st, f));
+    else SPION_CUDA_TRY(launch_after(k_finish<32>, grid, dim3(256), 0, st, f));
+  }
   return SPION_OK;
 }
 
@@ -1551,7 +1562,8 @@ extern "C" int spion_vocab_loss_backward(const spion_vocab_problem* p, const flo
   uint16_t* const G = (uint16_t*)(ws + l.g);
   float* const unit = (float*)(ws + l.unit);
   const float gscale = p->type == SPION_F16 ? 8192.f : 1.f;
-  if (p->reduction == 0) SPION_CUDA_TRY(launch_after(k_unit, dim3(1), dim3(1024), 0, st, prep.plan, g, unit));
+  const bool by_unit = p->reduction == 0 && p->type == SPION_F16;
+  if (by_unit) SPION_CUDA_TRY(launch_after(k_unit, dim3(1), dim3(1024), 0, st, prep.plan, g, unit));
   if (!l.kept && (rc = launch_prepare<false>(p, prep, st)) != SPION_OK) return rc;
   Call<GRAD> grad;
   Call<GRADS> grads;
@@ -1569,7 +1581,7 @@ extern "C" int spion_vocab_loss_backward(const spion_vocab_problem* p, const flo
   if ((rc = l.pair_g ? units_of<GRADS, true>(&dx_units) : units_of<GRADS, false>(&dx_units)) != SPION_OK) return rc;
   const int tz = l.pair_z ? 256 : 128, tg = l.tile_g;
   z.g = p->reduction == 0 ? g : nullptr, z.G = G, z.ldg = l.Gp, z.gscale = gscale;
-  z.coef = {p->reduction == 0 ? nullptr : g, unit, p->reduction == 1, prep.inv_tau / gscale};
+  z.coef = {p->reduction == 0 ? nullptr : g, by_unit ? unit : nullptr, p->reduction == 1, prep.inv_tau / gscale};
   z.colsum = db != nullptr ? (float*)(ws + l.colsum) : nullptr;
   const int dx_chunks = (int)tiles_of(std::min(l.Gp, l.V), BK);            // every piece's contraction is cut as the first one's: the parts are added piece by piece
   const unsigned most = 8 * sm_count();

@@ -180,6 +180,36 @@ def test_distillation(dtype, k, tau, reduction):
     check(lambda x, w, b: distill_top_logits(x, w, idx, teacher, b, tau, reduction), x, w, b, rows, idx[rows].clamp_min(0), q, tau, reduction, g)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_targets_side_by_side_and_many_times_the_same(dtype):
+    """More targets among a thread's 64 columns than it remembers."""
+    from spion_b200.vocab import distill_top_logits
+    T, V, k = 140, 500, 40
+    x, w, b, _, g = inputs(T, 64, V, dtype, seed=9)
+    idx = torch.randint(0, V - k, (T, 1), generator=g, device="cuda") + torch.arange(k, device="cuda")
+    idx[:40] = idx[:40, :1]                                # one id, forty times
+    idx[40:60, ::3] = 77
+    teacher = torch.randn(T, k, generator=g, device="cuda")
+    q = torch.softmax(teacher.double(), 1)
+    rows = torch.arange(T, device="cuda")
+    check(lambda x, w, b: distill_top_logits(x, w, idx, teacher, b), x, w, b, rows, idx, q, 1.0, "mean", g)
+    check(lambda x, w, b: distill_top_logits(x, w, idx, teacher, b, reduction="none"), x, w, None, rows, idx, q, 1.0, "none", g)
+
+
+def test_more_rows_than_one_pass_takes():
+    """Partial sums are kept for a part of the rows at a time; a row's are its own."""
+    from spion_b200.vocab import linear_cross_entropy
+    x, w, b, labels, g = inputs(40000, 16, 64000, torch.bfloat16)
+    for kept in (1.0, 0.9):
+        labels[torch.rand(40000, generator=g, device="cuda") >= kept] = -100
+        each = linear_cross_entropy(x, w, labels, b, reduction="none")
+        parts = torch.cat([linear_cross_entropy(x[i:i + 20000], w, labels[i:i + 20000], b, reduction="none") for i in (0, 20000)])
+        assert torch.equal(each, parts)
+        mean, n = each.double().sum() / (labels >= 0).sum(), int((labels >= 0).sum())
+        assert abs(float(linear_cross_entropy(x, w, labels, b)) - float(mean)) <= 2.0 ** -23 * float(mean)
+        assert abs(float(linear_cross_entropy(x, w, labels, b, reduction="sum")) - float(mean) * n) <= 2.0 ** -23 * float(mean) * n
+
+
 def test_one_entry_of_weight_one_is_the_cross_entropy():
     from spion_b200.vocab import distill_top_logits, linear_cross_entropy
     x, w, b, labels, g = inputs(100, 64, 500, torch.bfloat16)
@@ -387,6 +417,25 @@ def test_a_first_backward_of_a_process():
             "l = torch.zeros(200, dtype=torch.long, device='cuda')\n"
             "g = torch.autograd.grad(linear_cross_entropy(x, w, l), (x, w), torch.tensor(1.0, device='cuda'))\n"
             "torch.cuda.synchronize()\nassert all(bool(t.isfinite().all()) for t in g)\nprint('done')\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
+
+
+def test_a_first_call_under_a_capture():
+    """The first use of the operators in a process, kernels not loaded yet."""
+    import os
+    import subprocess
+    import sys
+    code = ("import torch\nfrom spion_b200.vocab import linear_cross_entropy\nfrom spion_b200.tokens import embed_tokens\n"
+            "ids = torch.arange(200, device='cuda') % 50\ntable = torch.randn(50, 64, device='cuda', requires_grad=True)\n"
+            "w = torch.randn(300, 64, device='cuda', requires_grad=True)\none = torch.ones((), device='cuda')\n"
+            "s = torch.cuda.Stream()\ns.wait_stream(torch.cuda.current_stream())\ng = torch.cuda.CUDAGraph()\n"
+            "with torch.cuda.stream(s):\n  with torch.cuda.graph(g, stream=s):\n"
+            "    loss = linear_cross_entropy(embed_tokens(ids, table), w, ids)\n    grads = torch.autograd.grad(loss, (table, w), one)\n"
+            "torch.cuda.synchronize()\ng.replay()\ntorch.cuda.synchronize()\n"
+            "want = torch.autograd.grad(linear_cross_entropy(embed_tokens(ids, table), w, ids), (table, w))\n"
+            "assert all(torch.equal(a, b) for a, b in zip(grads, want))\nprint('done')\n")
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
