@@ -533,7 +533,7 @@ Sizes sizes_of(long long T, long long V, long long N) {
   Sizes s = {};
   s.one = T <= ONE_MAX;
   // counts of all CTAs before it are read by every CTA: 128 of them at most
-  s.per_cta = s.one ? (T + 1023) / 1024 * 1024 : std::max(2048ll, ((T + 127) / 128 + PLACE - 1) / PLACE * PLACE);
+  s.per_cta = s.one ? (T + 1023) / 1024 * 1024 : std::max(1024ll, ((T + 127) / 128 + PLACE - 1) / PLACE * PLACE);
   s.ctas = (T + s.per_cta - 1) / s.per_cta;
   int bits = 1;
   while (V >> bits) ++bits;                                // keys 0 .. V
