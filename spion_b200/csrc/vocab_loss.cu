@@ -376,7 +376,7 @@ enum : int { DX, DW };                                    // ... and which of th
 constexpr int BK = 64;                                    // elements of the contraction in a chunk: 128 bytes
 constexpr uint32_t HALF = 128 * BK * 2, STAGE = 2 * HALF;
 // PAIR: two CTAs of a cluster share a tile of 256 x 256; else tiles of 128 x 128.  A thread that writes has 64 columns: what it does with them is a chain of latencies, and four
-// warps a scheduler hide more of each other's than two with 128 columns each do (8192 x 64 to 64000, k_gemm<LOGSUM> 663 us, so SPAN).
+// warps a scheduler hide more of each other's than two with 128 columns each do (8192 x 64 to 64000: k_gemm<LOGSUM> 663 us, so 462; k_gemm<GRAD> 911, 698).
 template <int MODE, bool PAIR> struct Shape {
   static constexpr int BN = PAIR ? 256 : 128, TILE = PAIR ? 256 : 128, W = 64;         // columns and rows of a tile; columns of a writing thread
   static constexpr int EPI = 4 * BN / W, THREADS = 32 * (2 + EPI), STAGES = 6;
@@ -402,14 +402,16 @@ struct Coef {
 struct Parts {
   int units, chunks;        // of the first piece of the vocabulary: every piece is cut alike
   int other, other_parts;   // tiles of dW beside it, and the parts of their contraction
-  __host__ __device__ int of(int tiles, int n) const {
-    const long long oc = other ? ((n + BK - 1) / BK + other_parts - 1) / other_parts : 0;
+  __device__ int of(int tiles, int n) const {
+    if (tiles <= 0 || tiles > 8 * units) return 1;
+    const int oc = other ? ((n + BK - 1) / BK + other_parts - 1) / other_parts : 0;
     int best = 1;
-    long long least = 1ll << 62;
-    for (int s = 1; s <= 8 && tiles > 0 && (s == 1 || ((long long)tiles * s <= 8ll * units && 4 * s <= chunks)); ++s) {
-      const long long c = (chunks + s - 1) / s, longest = c > oc ? c : oc;
-      const long long time = other ? ((long long)tiles * chunks + other * oc) * 2 / units + longest : ((long long)tiles * s + units - 1) / units * c * 2;
-      if (time * (50 + s) < least) best = s, least = time * (50 + s);
+    long long least = 0;
+    for (int s = 1; s <= 8 && (s == 1 || (tiles * s <= 8 * units && 4 * s <= chunks)); ++s) {
+      const int c = (chunks + s - 1) / s, rounds = (tiles * s + units - 1) / units;
+      const long long longest = c > oc ? c : oc;          // times in chunks of a tile, times twice the units
+      const long long time = (other ? 2 * ((long long)tiles * chunks + (long long)other * oc) + longest * units : 2ll * rounds * c * units) * (50 + s);
+      if (s == 1 || time < least) best = s, least = time;
     }
     return best;
   }
@@ -727,6 +729,7 @@ template <int MODE, int W, int OPT, int which> __device__ __forceinline__ void e
 // Warp 0 loads, warp 1 multiplies, the others take the sums.  Every wait is bounded; whoever gives up reports it and leaves, and so do all that wait for it; the warps
 // that write go on with NaN.  PAIR: two CTAs of a cluster share a tile of 256 x 256, each brings 128 rows of either operand and holds 128 rows of the sums; the first one's warp 1
 // multiplies for both (see k_lin8 in linear_e4m3.cu, whose scheme this is).  Else tiles of 128 x 128.
+// 8192 x 2048 to 32000, bf16: z and its log sums 660 us (1.63 PFLOP/s, the tensor pipe 93 % busy), z and G 705 - 740, dx and dW 1480 (1.45 PFLOP/s, at the power cap).
 // Operands whose contraction runs along memory (K-major: x and W in z, G in dx) come as one box of 128 rows x 64; those whose contraction runs across it (MN-major: W in dx, G and x
 // in dW) as two boxes of 64 rows x 64.
 template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<MODE, PAIR>::THREADS, 1) k_gemm(const __grid_constant__ Call<MODE> call) {

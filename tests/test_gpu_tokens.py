@@ -60,6 +60,22 @@ def test_sizes(T, V, N, dtype):
     check(ids, w, 1.7)
 
 
+@pytest.mark.parametrize("seed", range(24))
+def test_drawn_calls(seed):
+    """Sizes, types, frequencies, strides and padding at random."""
+    import random
+    rng = random.Random(seed)
+    T, V, N = (int(2 ** rng.uniform(0, m)) for m in (16, 14, 9))
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    w = torch.randn(V, N, generator=g, device="cuda").to(rng.choice(TYPES))
+    if rng.random() < 0.3:
+        w = torch.nn.functional.pad(w, (1, 2))[:, 1:1 + N]
+    skew = rng.choice([0.0, 1.0, 4.0])                     # how unequally frequent ids are
+    ids = (torch.rand(T, generator=g, device="cuda") ** (1 + skew) * V).long().clamp(max=V - 1)
+    ids = ids if rng.random() < 0.5 else ids.sort().values
+    check(ids, w, rng.choice([1.0, 0.1, 7.0]), rng.choice([None, rng.randrange(V)]), rng.choice([None, *TYPES]), seed)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("N", [5, 64, 520])
 def test_runs_of_every_length(N, dtype):

@@ -95,7 +95,10 @@ def check(call, x, w, b, rows, idx, q, tau, reduction, g):
     close(grads[1], *o["dw"], "dw")
     assert grads[0].dtype == x.dtype and grads[1].dtype == w.dtype
     if b is not None:
-        close(grads[2], *o["db"], "db")
+        want, bound = o["db"]
+        rounding = 0.0 if b.dtype == torch.float32 else want.abs() * torch.finfo(b.dtype).eps / 2 + (2.0 ** -25 if b.dtype == torch.float16 else 0.0)
+        close(grads[2], want, bound + rounding, "db")
+        assert grads[2].dtype == b.dtype
     return loss, grads
 
 
@@ -124,6 +127,41 @@ def test_every_kind_of_tile(T, K, V, dtype):
     labelled(x, w, b, labels, g, "sum")
     labels[torch.rand(T, generator=g, device="cuda") < 0.85] = -100
     labelled(x, w, b, labels, g, "mean")
+
+
+@pytest.mark.parametrize("seed", range(36))
+def test_drawn_calls(seed):
+    """Sizes, types, masks, targets, strides and reductions at random."""
+    import random
+
+    from spion_b200.vocab import distill_top_logits
+    rng = random.Random(seed)
+    dtype = rng.choice(TYPES)
+    T, K, V = (int(2 ** rng.uniform(0, m)) for m in (10.5, 10.5, 12.5))
+    if rng.random() < 0.25:
+        T, K, V = T * 4, min(K * 3, 3000), V * 2           # on both sides of the tiles of pairs
+    x, w, b, labels, g = inputs(T, K, V, dtype, seed=seed, bias=rng.random() < 0.6)
+    if rng.random() < 0.3:
+        pad = rng.choice([1, 3, 8])
+        x = torch.nn.functional.pad(x, (pad, pad))[:, pad:pad + K]
+        w = torch.nn.functional.pad(w, (0, pad))[:, :K]
+    if b is not None and rng.random() < 0.4:
+        b = b.to(rng.choice([torch.bfloat16, torch.float16]))
+    reduction, kept = rng.choice(["mean", "sum", "none"]), rng.choice([1.0, 1.0, 0.7, 0.1])
+    labels[torch.rand(T, generator=g, device="cuda") >= kept] = -100
+    labels[rng.randrange(T)] = rng.randrange(V)
+    if rng.random() < 0.5:
+        labelled(x, w, b, labels, g, reduction)
+        return
+    k, tau = int(2 ** rng.uniform(0, 7)), rng.choice([1.0, 2.0, 0.8])
+    idx = torch.randint(-1, V, (T, k), generator=g, device="cuda")
+    idx[labels < 0] = -1
+    idx[(idx >= 0).any(1).logical_not() & (labels >= 0), 0] = 0
+    teacher = (2 * torch.randn(T, k, generator=g, device="cuda")).to(rng.choice(TYPES))
+    there = idx >= 0
+    rows = there.any(1).nonzero().squeeze(1)
+    q = torch.softmax(torch.where(there, teacher.double(), -float("inf"))[rows] / tau, 1)
+    check(lambda x, w, b: distill_top_logits(x, w, idx, teacher, b, tau, reduction), x, w, b, rows, idx[rows].clamp_min(0), q, tau, reduction, g)
 
 
 @pytest.mark.parametrize("dtype", TYPES)

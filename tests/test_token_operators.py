@@ -25,6 +25,8 @@ def test_modules_refuse_what_they_do_not_serve():
         with pytest.raises(ValueError, match="not served"):
             ScaledEmbedding(10, 8, **kw)
     assert ScaledEmbedding(10, 8, max_norm=None, sparse=False).scale == 1.0
+    made = ScaledEmbedding.from_pretrained(torch.ones(4, 8), padding_idx=1)
+    assert type(made) is ScaledEmbedding and not made.weight.requires_grad and made.padding_idx == 1
     table = ScaledEmbedding(10, 8)
     assert VocabHead(8, 10, tied=table).weight is table.weight
     with pytest.raises(ValueError, match="tied"):
