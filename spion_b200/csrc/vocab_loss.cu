@@ -1138,34 +1138,34 @@ __device__ __forceinline__ void join(const Join& a, unsigned cta, int n, float a
     store8(a, r, c, f);
     return;
   }
-  if (splits <= 8) {                                       // up to four pieces a thread under way
-    for (long long i0 = cta * 256ll + threadIdx.x; i0 < all; i0 += 4 * step) {
-      float f[4][8];
-      long long r[4], from[4];
-      int c[4];
+  if (splits <= 8) {                                       // two pieces a thread under way
+    for (long long i0 = cta * 256ll + threadIdx.x; i0 < all; i0 += 2 * step) {
+      float f[2][8];
+      long long r[2], from[2];
+      int c[2];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < 2; ++u) {
         const long long i = i0 + u * step;
         place(min(i, all - 1), r[u], c[u]);
         from[u] = i >= all ? -1 : a.slot ? a.slot[r[u]] : r[u];
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[u][e] = 0.f;
       for (int s = 0; s < splits; ++s) {
-        Piece<float, 8> p[4];
+        Piece<float, 8> p[2];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 2; ++u)
           if (from[u] >= 0) p[u].load(a.part + (s * plane + from[u]) * a.ldp + c[u]);
           else p[u].zero();
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int e = 0; e < 8; ++e) f[u][e] += p[u].at(e);
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < 2; ++u) {
         if (i0 + u * step >= all) break;
         const float by = from[u] < 0 ? 0.f : alpha;        // a row that does not count: zeros, whatever arrives at the loss
 #pragma unroll
@@ -1206,7 +1206,7 @@ __device__ __forceinline__ void join(const Join& a, unsigned cta, int n, float a
     store8(a, r, c, f);
   }
 }
-__global__ void __launch_bounds__(256) k_out(const __grid_constant__ Leave a) {
+__global__ void __launch_bounds__(256, 3) k_out(const __grid_constant__ Leave a) {
   __shared__ float shared[256][8];
   next_may_start();
   wait_for_kernel_before();
@@ -1389,6 +1389,7 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   l->rows = std::min(l->Tp, std::max<long long>(PAD, PART_BYTES / (8 * l->parts) / PAD * PAD));
   l->launches = tiles_of(l->Tp, l->rows);
   l->Gp = std::min(l->Vp, std::max<long long>(PAD, PIECE_BYTES / (2 * l->planes * l->Tp) / PAD * PAD));
+  l->Gp = up(tiles_of(l->Vp, tiles_of(l->Vp, l->Gp)), PAD);               // pieces of one size
   l->pair_g = tiles(l->T, l->K) > 0 && tiles(l->T, l->K) + tiles(l->Gp, l->K) >= pairs;
   l->tile_g = l->pair_g ? 256 : 128;
   // tiles are counted in 32 bits, eight parts of dx's contraction among them
