@@ -52,7 +52,8 @@ def check(ids, w, scale=1.0, padding=None, out_dtype=None, seed=0):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("T,V,N", [(1, 1, 1), (1, 32000, 4096), (3, 2, 7), (31, 511, 8), (64, 512, 33), (2048, 513, 64), (2049, 1000, 72), (5000, 300000, 16), (4099, 10007, 769),
-                                   (70000, 100, 32), (300000, 5000, 24), (9000, 1, 260)])
+                                   (70000, 100, 32), (300000, 5000, 24), (9000, 1, 260), (8192, 300, 16),
+                                   (8193, 300, 16), (5000, 262143, 4), (9000, 262144, 4), (10, 50, 20000), (100, 2000000, 3), (131073, 70, 1)])
 def test_sizes(T, V, N, dtype):
     g = torch.Generator(device="cuda").manual_seed(T + V + N)
     w = torch.randn(V, N, generator=g, device="cuda").to(dtype)

@@ -119,7 +119,31 @@ def test_sizes(T, K, V, dtype):
     labelled(x, w, None, labels, g, "none")
 
 
-# (1100, 2064, 5000): pairs of CTAs in all products; (17000, 64, 9000): pieces of the vocabulary; (3000, 64, 256): the contraction of dW shared out; (40, 200, 33000): that of dx
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,K,V", [(70, 5000, 300), (3, 8, 300000), (70000, 1, 2), (4097, 20, 130), (16385, 8, 40)])
+def test_long_in_one_direction(T, K, V, dtype):
+    x, w, b, labels, g = inputs(T, K, V, dtype)
+    labels[torch.rand(T, generator=g, device="cuda") < 0.1] = -100
+    labels[0] = 0
+    labelled(x, w, b, labels, g, "mean")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_logits_an_ignored_id_of_the_vocabulary_and_one_tensor_as_both_operands(dtype):
+    from spion_b200.vocab import linear_cross_entropy
+    x, w, b, labels, g = inputs(200, 64, 300, dtype, size=30.0)
+    labelled(x, w, b, labels, g, "none")
+    labels[::2] = 3
+    labelled(x, w, b, labels, g, "mean", ignore=3)
+    table = w.detach()[:90].clone().requires_grad_()
+    own = torch.arange(90, device="cuda").flip(0)
+    both, = torch.autograd.grad(linear_cross_entropy(table, table, own, reduction="sum"), table)
+    rows, cols = table.detach().clone().requires_grad_(), table.detach().clone().requires_grad_()
+    dx, dw = torch.autograd.grad(linear_cross_entropy(rows, cols, own, reduction="sum"), (rows, cols))
+    torch.testing.assert_close(both, dx + dw)
+
+
+# (2600, 2064, 5000): pairs of CTAs in all products; (17000, 64, 9000): pieces of the vocabulary; (3000, 64, 256): the contraction of dW shared out; (40, 200, 33000): that of dx
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("T,K,V", [(2600, 2064, 5000), (17000, 64, 9000), (3000, 64, 256), (40, 200, 33000), (7000, 300, 1100)])
 def test_every_kind_of_tile(T, K, V, dtype):
