@@ -70,7 +70,7 @@ struct Prep {
   int* counts;              // [chunks], or null: each CTA counts for itself
   float* q;                 // [T, k]
   const void* bias; int bias_type;
-  float* bias2;             // [Vp] b log2(e) / tau; -inf behind the vocabulary
+  float* bias2;             // [Vp + PAD] b log2(e) / tau; -inf behind the vocabulary
   int Vp;
   float c1;                 // log2(e) / tau
   // rows and weights in the products' type
@@ -124,7 +124,7 @@ __device__ __forceinline__ unsigned teacher_weights(const Prep& a, int t0, int e
 }
 __device__ __forceinline__ bool is_entry(const Prep& a, long long at) { return a.labels[at] != -1 && load_any(a.teacher, a.teacher_type, at) != -INFINITY; }
 __device__ __forceinline__ void scaled_bias(const Prep& a, int first, int step) {
-  for (int v = first; v < a.Vp; v += step) a.bias2[v] = v >= a.V ? -INFINITY : a.bias != nullptr ? load_any(a.bias, a.bias_type, v) * a.c1 : 0.f;
+  for (int v = first; v < a.Vp + PAD; v += step) a.bias2[v] = v >= a.V ? -INFINITY : a.bias != nullptr ? load_any(a.bias, a.bias_type, v) * a.c1 : 0.f;
 }
 // Rows that count, of each chunk: a warp per chunk, or, with a teacher, a CTA per chunk and eight rows a warp (a warp for all of them, one row after another: 8192 rows of 32
 // logits 98 us)
@@ -374,16 +374,21 @@ template <class E, bool FIRST> __global__ void __launch_bounds__(256) k_prepare(
 enum Mode { LOGSUM, GRAD, GRADS };                        // GRADS: dx and dW, two products in one launch
 enum : int { DX, DW };                                    // ... and which of them
 constexpr int BK = 64;                                    // elements of the contraction in a chunk: 128 bytes
-constexpr uint32_t HALF = 128 * BK * 2, STAGE = 2 * HALF;
-// PAIR: two CTAs of a cluster share a tile of 256 x 256; else tiles of 128 x 128.  A thread that writes has 64 columns: what it does with them is a chain of latencies, and four
-// warps a scheduler hide more of each other's than two with 128 columns each do (8192 x 64 to 64000: k_gemm<LOGSUM> 663 us, so 462; k_gemm<GRAD> 911, 698).
-template <int MODE, bool PAIR> struct Shape {
-  static constexpr int BN = PAIR ? 256 : 128, TILE = PAIR ? 256 : 128, W = 64;         // columns and rows of a tile; columns of a writing thread
-  static constexpr int EPI = 4 * BN / W, THREADS = 32 * (2 + EPI), STAGES = 6;
+constexpr uint32_t HALF = 128 * BK * 2;
+// What a kernel is made for, beside its product: what it need not do costs registers that the sums want.
+enum : int { ONE = 1, THREE = 2, COLUMNS = 4, WIDE = 8 };  // one target a row (LOGSUM, GRAD); G in three parts, sums of G's columns (GRAD); wide tiles (LOGSUM)
+// PAIR: two CTAs of a cluster share a tile of 256 x 256; else tiles of 128 x 128, or (WIDE) 128 rows of as many columns as leave one tile to each multiprocessor: few rows, where
+// the weights are all there is to read (16 x 2048 to 32000: 250 tiles of 128 43 us alone, 143 of 224 38).  A thread that writes has 64 columns: what it does with them
+// is a chain of latencies, and four warps a scheduler hide more of each other's than two with 128 columns each do (8192 x 64 to 64000: k_gemm<LOGSUM> 663 us, so 462; k_gemm<GRAD> 911, 698).
+template <int MODE, bool PAIR, int OPT> struct Shape {
+  static constexpr bool LARGE = PAIR || (OPT & WIDE);
+  static constexpr int BN = LARGE ? 256 : 128, TILE = PAIR ? 256 : 128, W = 64;        // columns (at most) and rows of a tile; columns of a writing thread
+  static constexpr int EPI = 4 * BN / W, THREADS = 32 * (2 + EPI), STAGES = OPT & WIDE ? 4 : 6;
+  static constexpr uint32_t STAGE = (OPT & WIDE ? 3 : 2) * HALF;                       // of A, and of B
   static constexpr uint32_t BARS = STAGES * STAGE, STAGED = BARS + 16 * STAGES + 128;   // STAGED: 32 x 16 results a writing warp, rows of 17 (DW)
   static constexpr uint32_t SMEM = MODE == GRADS ? STAGED + EPI * 32 * 17 * 4 : STAGED;
 };
-static_assert(Shape<GRADS, true>::SMEM <= 232448 && Shape<GRADS, false>::SMEM <= 232448, "shared memory of a multiprocessor");
+static_assert(Shape<GRADS, true, 0>::SMEM <= 232448 && Shape<GRADS, false, 0>::SMEM <= 232448 && Shape<LOGSUM, false, WIDE>::SMEM <= 232448, "shared memory of a multiprocessor");
 
 // What the products with G are multiplied with.
 struct Coef {
@@ -423,6 +428,7 @@ struct Args {
   long long plane_a, plane_b;                             // rows of a part in the maps
   int M, N, L;                                            // rows of D (0: n), columns of D, contraction (0: n)
   int row0, most;                                         // first slot and slots of a launch (0: all)
+  int bn;                                                 // WIDE: columns of a tile, a multiple of 32
   int col0;                                               // first column of the piece of the vocabulary
   int chain;                                              // (chunk, product) pairs that one accumulator takes
   int splits;                                             // of the contraction (0: by `cut`)
@@ -536,13 +542,11 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, int fp16) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// What a kernel is made for, beside its product: what it need not do costs registers that the sums want.
-enum : int { ONE = 1, THREE = 2, COLUMNS = 4 };           // one target a row (LOGSUM, GRAD); G in three parts, sums of G's columns (GRAD)
-
 // What a writing thread knows of its row before the sums are there: it is read while they are formed
 struct Row {
   bool in;                  // the row counts
   int slot, found;          // targets among the thread's columns: how many,
+  int width;                // of the thread's columns, those of its tile
   uint32_t two;             // and of the first two the column and the target, a byte each
   float lse, r;
 };
@@ -557,13 +561,14 @@ template <int OPT, class F> __device__ __forceinline__ void each_target(const Ar
   if (!(OPT & ONE) && row.found > 2) {                     // seldom: all over again, without those two
     for (int j = (int)(row.two >> 24) + 1; j < a.k; ++j) {
       const int off = a.plan.target[(long long)j * a.Tp + row.slot] - c - g;
-      if ((unsigned)off < 32u) f(off, j);
+      if ((unsigned)off < 32u && g + off < row.width) f(off, j);
     }
   }
 }
-template <int MODE, int W, int OPT> __device__ __forceinline__ Row row_of(const Args& a, int n, int row, int c) {
+template <int MODE, int W, int OPT> __device__ __forceinline__ Row row_of(const Args& a, int n, int row, int c, int width) {
   Row r = {};
   if (MODE != LOGSUM && MODE != GRAD) return r;
+  r.width = width;
   r.in = row < n;
   r.slot = r.in ? row : 0;
   r.lse = INFINITY;
@@ -571,7 +576,7 @@ template <int MODE, int W, int OPT> __device__ __forceinline__ Row row_of(const 
     const int* const target = a.plan.target + r.slot;
     if (OPT & ONE) {
       const int t = target[0], off = t - c;
-      if ((unsigned)off < (unsigned)W && t >= 0) r.two = off, r.found = 1;
+      if (off >= 0 && off < width && t >= 0) r.two = off, r.found = 1;
     }
     for (int j0 = 0; !(OPT & ONE) && j0 < a.k; j0 += 16) {  // sixteen loads under way: one after another they are 0.25 us each
       int t[16];
@@ -580,7 +585,7 @@ template <int MODE, int W, int OPT> __device__ __forceinline__ Row row_of(const 
 #pragma unroll
       for (int u = 0; u < 16; ++u) {
         const int off = t[u] - c;
-        if ((unsigned)off < (unsigned)W && t[u] >= 0) {
+        if (off >= 0 && off < width && t[u] >= 0) {
           if (r.found < 2) r.two |= (uint32_t)(off | (j0 + u) << 8) << (16 * r.found);
           ++r.found;
         }
@@ -595,7 +600,7 @@ template <int MODE, int W, int OPT> __device__ __forceinline__ Row row_of(const 
 }
 
 // What a thread does with its sums: row `row` of D, columns col .. col + W - 1
-template <int MODE, int W, int OPT, int which> __device__ __forceinline__ void epilogue(const Args& a, int out_row, float (&acc)[W / 32][32], const Row& me, int n, int row, int col, int part, float* stage) {
+template <int MODE, int W, int OPT, int which> __device__ __forceinline__ void epilogue(const Args& a, int out_row, float (&acc)[W / 32][32], const Row& me, int n, int row, int col, int part, int width, float* stage) {
   const int lane = threadIdx.x & 31;
   if constexpr (MODE == LOGSUM || MODE == GRAD) {
     const int slot = me.slot, c = a.col0 + col;           // of the vocabulary
@@ -607,6 +612,13 @@ template <int MODE, int W, int OPT, int which> __device__ __forceinline__ void e
     }
     if constexpr (MODE == LOGSUM) {
       float top = -INFINITY, sum = 0.f;
+      if constexpr ((OPT & WIDE) != 0) {                  // columns of the next tile, or of none
+#pragma unroll
+        for (int g = 0; g < W; g += 32)
+          if (g >= width)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) acc[g / 32][e] = -INFINITY;
+      }
 #pragma unroll
       for (int g = 0; g < W; ++g) top = fmaxf(top, acc[g / 32][g % 32]);
 #pragma unroll
@@ -732,9 +744,10 @@ template <int MODE, int W, int OPT, int which> __device__ __forceinline__ void e
 // 8192 x 2048 to 32000, bf16: z and its log sums 660 us (1.63 PFLOP/s, the tensor pipe 93 % busy), z and G 705 - 740, dx and dW 1480 (1.45 PFLOP/s, at the power cap).
 // Operands whose contraction runs along memory (K-major: x and W in z, G in dx) come as one box of 128 rows x 64; those whose contraction runs across it (MN-major: W in dx, G and x
 // in dW) as two boxes of 64 rows x 64.
-template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<MODE, PAIR>::THREADS, 1) k_gemm(const __grid_constant__ Call<MODE> call) {
-  using C = Shape<MODE, PAIR>;
+template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<MODE, PAIR, OPT>::THREADS, 1) k_gemm(const __grid_constant__ Call<MODE> call) {
+  using C = Shape<MODE, PAIR, OPT>;
   constexpr int BN = C::BN, TILE = C::TILE, W = C::W, STAGES = C::STAGES, EPI = C::EPI;
+  constexpr uint32_t STAGE = C::STAGE;
   constexpr bool TWO = MODE == GRADS;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t sbase = smem_u32(smem_raw);
@@ -769,7 +782,8 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
   const uint32_t tmem = *reinterpret_cast<uint32_t*>(smem_raw + (slot - sbase));
   wait_for_kernel_before();
   const int n = *reinterpret_cast<const volatile int*>(call.a[0].n);
-  const Work w0 = work_of(call.a[0], n, TILE, BN), w1 = TWO ? work_of(call.a[Call<MODE>::PRODUCTS - 1], n, TILE, BN) : Work();
+  const int bn = OPT & WIDE ? call.a[0].bn : BN;
+  const Work w0 = work_of(call.a[0], n, TILE, bn), w1 = TWO ? work_of(call.a[Call<MODE>::PRODUCTS - 1], n, TILE, BN) : Work();
   const bool direct = n == call.a[0].direct_rows;
   const int items0 = w0.splits * w0.tiles_m * w0.tiles_n, items = items0 + (TWO ? w1.splits * w1.tiles_m * w1.tiles_n : 0);
   const bool aborted = s_abort != 0;
@@ -794,7 +808,7 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
         const bool a_mn = TWO && which == DW, b_mn = TWO;
         const CUtensorMap *const map_a = !TWO && direct ? &maps.x : &maps.a, *const map_b = a_mn && direct ? &maps.x : &maps.b;
         item_at(which ? w1 : w0, i - (which ? items0 : 0), s, m, nn, c0, c1);
-        const int ra = m * TILE + rank * 128 + (MODE == LOGSUM ? a.row0 : 0), rb = nn * BN + rank * 128, b0 = a_mn ? 0 : a.col0;
+        const int ra = m * TILE + rank * 128 + (MODE == LOGSUM ? a.row0 : 0), rb = nn * bn + rank * 128, b0 = a_mn ? 0 : a.col0;
         for (int c = c0; c < c1 && ok; ++c)
           for (int p = 0; p < a.products; ++p) {
             ok = mbar_wait(empty + 8 * st, ph);
@@ -807,7 +821,7 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
               if (rank == 0) mbar_expect_tx(bar, 2 * STAGE);
               bar = in_leader(bar);
             } else {
-              mbar_expect_tx(bar, STAGE);
+              mbar_expect_tx(bar, OPT & WIDE ? HALF + bn * BK * 2 : STAGE);
             }
             auto load = [&](uint32_t to, const CUtensorMap* map, int x, int y) {
               if (PAIR) pair_tma_load_2d(to, map, bar, x, y);
@@ -839,7 +853,7 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
   } else if (warp == 1) {
     if (!aborted && rank == 0 && elect_one()) {
       const uint32_t kind = call.a[0].fp16 ? 0u : (1u << 7) | (1u << 10);
-      const uint32_t shape = (1u << 4) | kind | ((uint32_t)TWO << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24);
+      const uint32_t shape = (1u << 4) | kind | ((uint32_t)TWO << 16) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(TILE >> 4) << 24);
       const uint64_t b0 = make_smem_desc(sbase + HALF, TWO ? HALF / 2 : 16, 1024, LAYOUT_SW128);
       constexpr uint32_t step_b = TWO ? 2048 : 32;
       int st = 0, ph = 0, buf = 0, acc_ph = 1;
@@ -902,8 +916,8 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
       const Args& a = call.a[which];
       item_at(kept[which], at, s, m, nn, c0, c1);
       const int all = (c1 - c0) * a.products;
-      const int row = (MODE == LOGSUM ? a.row0 : 0) + m * TILE + rank * 128 + q * 32 + lane, col = nn * BN + share * W;
-      const Row me = row_of<MODE, W, OPT>(a, n, row, a.col0 + col);
+      const int row = (MODE == LOGSUM ? a.row0 : 0) + m * TILE + rank * 128 + q * 32 + lane, col = nn * bn + share * W, width = OPT & WIDE ? min(W, bn - share * W) : W;
+      const Row me = row_of<MODE, W, OPT>(a, n, row, a.col0 + col, width);
       // the first chain's sums as they come, the others' on top, sixteen at a time: more would not fit beside the sums
       auto ready = [&] {
         lost = !tc::warp_wait(acc_full + 8 * buf, ph, &g_vocab_status, ERR_MMA2_WAIT);
@@ -950,8 +964,8 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
         for (int g = 0; g < W; ++g) acc[g / 32][g % 32] = not_a_number();
       float* const stage = reinterpret_cast<float*>(smem_raw + C::STAGED) + (warp - 2) * 32 * 17;
       const int out_row = s * kept[which].tiles_m * TILE + row, part = nn * (BN / W) + share;
-      if (TWO && which == DW) epilogue<MODE, W, OPT, DW>(call.a[Call<MODE>::PRODUCTS - 1], out_row, acc, me, n, row, col, part, stage);
-      else epilogue<MODE, W, OPT, DX>(call.a[0], out_row, acc, me, n, row, col, part, stage);
+      if (TWO && which == DW) epilogue<MODE, W, OPT, DW>(call.a[Call<MODE>::PRODUCTS - 1], out_row, acc, me, n, row, col, part, width, stage);
+      else epilogue<MODE, W, OPT, DX>(call.a[0], out_row, acc, me, n, row, col, part, width, stage);
     }
   }
   tc_fence_before();
@@ -1282,13 +1296,13 @@ template <int MODE, bool PAIR, int OPT = 0> int units_of(int* units) {
   SPION_CUDA_TRY(cudaGetDevice(&dev));
   int n = dev < 64 ? known[dev].load() : 0;
   if (n == 0) {
-    SPION_CUDA_TRY(cudaFuncSetAttribute(k_gemm<MODE, PAIR, OPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<MODE, PAIR>::SMEM));
+    SPION_CUDA_TRY(cudaFuncSetAttribute(k_gemm<MODE, PAIR, OPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<MODE, PAIR, OPT>::SMEM));
     if (PAIR) {
       cudaLaunchConfig_t cfg = {};
       cudaLaunchAttribute at[1];
       at[0].id = cudaLaunchAttributeClusterDimension;
       at[0].val.clusterDim.x = 2, at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-      cfg.gridDim = dim3(2 * (sm_count() / 2)), cfg.blockDim = dim3(Shape<MODE, PAIR>::THREADS), cfg.dynamicSmemBytes = Shape<MODE, PAIR>::SMEM, cfg.attrs = at, cfg.numAttrs = 1;
+      cfg.gridDim = dim3(2 * (sm_count() / 2)), cfg.blockDim = dim3(Shape<MODE, PAIR, OPT>::THREADS), cfg.dynamicSmemBytes = Shape<MODE, PAIR, OPT>::SMEM, cfg.attrs = at, cfg.numAttrs = 1;
       SPION_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, k_gemm<MODE, PAIR, OPT>, &cfg));
     } else {
       n = sm_count();
@@ -1311,7 +1325,7 @@ template <int MODE, bool PAIR, int OPT> int launch_gemm(const Call<MODE>& call, 
   at[0].val.programmaticStreamSerializationAllowed = 1;
   at[1].id = cudaLaunchAttributeClusterDimension;
   at[1].val.clusterDim.x = 2, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(PAIR ? 2 * use : use), cfg.blockDim = dim3(Shape<MODE, PAIR>::THREADS), cfg.dynamicSmemBytes = Shape<MODE, PAIR>::SMEM, cfg.stream = st, cfg.attrs = at, cfg.numAttrs = PAIR ? 2 : 1;
+  cfg.gridDim = dim3(PAIR ? 2 * use : use), cfg.blockDim = dim3(Shape<MODE, PAIR, OPT>::THREADS), cfg.dynamicSmemBytes = Shape<MODE, PAIR, OPT>::SMEM, cfg.stream = st, cfg.attrs = at, cfg.numAttrs = PAIR ? 2 : 1;
   SPION_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_gemm<MODE, PAIR, OPT>, call));
   return SPION_OK;
 }
@@ -1319,6 +1333,8 @@ template <int MODE, int OPT> int launch_gemm(bool pair, const Call<MODE>& call, 
   return pair ? launch_gemm<MODE, true, OPT>(call, most_items, st) : launch_gemm<MODE, false, OPT>(call, most_items, st);
 }
 int launch_logsum(bool pair, const Call<LOGSUM>& call, long long most_items, cudaStream_t st) {
+  if (call.a[0].bn)
+    return call.a[0].k == 1 ? launch_gemm<LOGSUM, false, ONE | WIDE>(call, most_items, st) : launch_gemm<LOGSUM, false, WIDE>(call, most_items, st);
   return call.a[0].k == 1 ? launch_gemm<LOGSUM, ONE>(pair, call, most_items, st) : launch_gemm<LOGSUM, 0>(pair, call, most_items, st);
 }
 int launch_grad(bool pair, const Call<GRAD>& call, long long most_items, cudaStream_t st) {
@@ -1348,6 +1364,7 @@ struct Layout {
   bool self;                                              // CTAs count for themselves
   long long rows, launches;                               // slots of a pass over z in the forward, and how many there are
   long long chunk;                                        // rows of a CTA of k_prepare
+  int wide;                                               // columns of a wide tile of the forward's z, or 0
   bool pair_z, pair_g;                                    // tiles of pairs of CTAs: in z; in dx and dW
   long long Gp;                                           // columns of a piece of the vocabulary
   int tile_g, dw_splits;
@@ -1385,7 +1402,12 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   // Tiles of pairs where every pair has one, else four times as many small ones.
   auto tiles = [](long long m, long long n) { return m > 128 && n > 128 ? tiles_of(m, 256) * tiles_of(n, 256) : 0; };
   l->pair_z = tiles(l->T, l->V) >= pairs;
-  l->parts = l->pair_z ? 4 * tiles_of(l->V, 256) : 2 * tiles_of(l->V, 128);
+  // Wide tiles for few rows, where they keep fifteen of sixteen multiprocessors: as few rounds of them as can be, of one size.  One row of 1024, wide / tiles of 128: to 19200 (120 tiles
+  // of 160) 18.1 us / 15.6, 32000 (143 of 224) 20.5 / 21.8, 37888 (148 of 256) 19.8 / 23.3, 50000 (261 of 192) 35.6 / 33.0, 128000 (572 of 224) 62.8 / 71.8; 128 rows: 12.7 / 13.2 to
+  // 32000, 50.7 / 50.0 to 128000.
+  const long long rounds = tiles_of(l->V, 256ll * sms), columns = up(tiles_of(l->V, sms * rounds), 32);
+  l->wide = l->T <= 64 && columns > 128 && 16 * tiles_of(l->V, columns) >= 15 * rounds * sms ? (int)columns : 0;
+  l->parts = l->wide ? 4 * tiles_of(l->V, l->wide) : l->pair_z ? 4 * tiles_of(l->V, 256) : 2 * tiles_of(l->V, 128);
   l->rows = std::min(l->Tp, std::max<long long>(PAD, PART_BYTES / (8 * l->parts) / PAD * PAD));
   l->launches = tiles_of(l->Tp, l->rows);
   l->Gp = std::min(l->Vp, std::max<long long>(PAD, PIECE_BYTES / (2 * l->planes * l->Tp) / PAD * PAD));
@@ -1402,9 +1424,9 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
     return here;
   };
   const long long xs_bytes = 2 * l->planes * l->Tp * l->Kp, w_bytes = l->copy_w ? 2 * l->planes * l->Vp * l->Kp : 0;
-  l->kept = xs_bytes + w_bytes + 4 * l->Vp <= KEPT_BYTES;
+  l->kept = xs_bytes + w_bytes + 4 * (l->Vp + PAD) <= KEPT_BYTES;
   take(256), take(4 * l->Tp), take(4 * l->Tp), take(4 * l->Tp), take(4 * l->k * l->Tp), take(4 * l->k * l->Tp);
-  auto operands = [&] { l->xs = take(xs_bytes), l->w = take(w_bytes), l->bias2 = take(4 * l->Vp); };
+  auto operands = [&] { l->xs = take(xs_bytes), l->w = take(w_bytes), l->bias2 = take(4 * (l->Vp + PAD)); };
   if (l->kept) operands();
   l->keep = at;
   at = 0;
@@ -1536,12 +1558,16 @@ extern "C" int spion_vocab_loss_forward(const spion_vocab_problem* p, float* los
   Args& a = call.a[0];
   if ((rc = logits_args(p, l, prep, &a, &call.maps[0])) != SPION_OK) return rc;
   const int tile = l.pair_z ? 256 : 128;
+  if (l.wide) {
+    a.bn = l.wide;
+    if ((rc = l.copy_w ? map_of(&call.maps[0].b, prep.ws, l.Kp, l.planes * l.Vp, l.Kp, l.wide) : map_of(&call.maps[0].b, p->w, l.K, l.V, l.ldw, l.wide)) != SPION_OK) return rc;
+  }
   a.N = (int)l.V, a.part = (float2*)(ws + l.part), a.parts = (int)l.parts, a.zt = prep.zt;
   const int lanes = std::max<int>(a.parts, l.k) <= 16 ? 4 : std::max<int>(a.parts, l.k) <= 32 ? 8 : 32;
   const dim3 grid((unsigned)std::min<long long>(tiles_of(std::min(l.T, l.rows), 256 / lanes), std::min(4 * sm_count(), FINISH_CTAS)));
   for (int pass = 0; pass < l.launches; ++pass) {
     a.row0 = (int)(pass * l.rows), a.most = (int)l.rows;
-    if ((rc = launch_logsum(l.pair_z, call, tiles_of(std::min(l.T, l.rows), tile) * tiles_of(l.V, tile), st)) != SPION_OK) return rc;
+    if ((rc = launch_logsum(l.pair_z, call, tiles_of(std::min(l.T, l.rows), tile) * tiles_of(l.V, l.wide ? l.wide : tile), st)) != SPION_OK) return rc;
     const Finish f = {prep.plan, (int)l.Tp, (int)l.k, a.part, a.parts, prep.zt, loss, (double*)(ws + l.cta_loss), p->reduction, a.row0, a.most, pass, (int)l.launches};
     if (lanes == 4) SPION_CUDA_TRY(launch_after(k_finish<4>, grid, dim3(256), 0, st, f));
     else if (lanes == 8) SPION_CUDA_TRY(launch_after(k_finish<8>, grid, dim3(256), 0, st, f));

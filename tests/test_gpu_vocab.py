@@ -272,6 +272,21 @@ def test_more_rows_than_one_pass_takes():
         assert abs(float(linear_cross_entropy(x, w, labels, b, reduction="sum")) - float(mean) * n) <= 2.0 ** -23 * float(mean) * n
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,K,V", [(1, 64, 20000), (16, 200, 32000), (64, 72, 37888), (64, 64, 37700), (33, 8, 37889), (5, 1100, 32001), (2, 24, 128000)])
+def test_few_rows_and_a_large_vocabulary(T, K, V, dtype):
+    """Tiles as wide as the vocabulary asks for, targets on both sides of their ends."""
+    from spion_b200.vocab import distill_top_logits
+    x, w, b, labels, g = inputs(T, K, V, dtype)
+    labels[-1] = V - 1
+    labelled(x, w, b, labels, g, "none")
+    idx = (torch.randint(0, V // 32, (T, 30), generator=g, device="cuda") * 32 + torch.arange(-15, 15, device="cuda") % 4).clamp(0, V - 1)
+    idx[:, 5:] = (idx[:, :1] + torch.arange(25, device="cuda")).clamp(0, V - 1)
+    teacher = torch.randn(T, 30, generator=g, device="cuda")
+    rows = torch.arange(T, device="cuda")
+    check(lambda x, w, b: distill_top_logits(x, w, idx, teacher, b, 1.3), x, w, None, rows, idx, torch.softmax(teacher.double() / 1.3, 1), 1.3, "mean", g)
+
+
 def test_one_entry_of_weight_one_is_the_cross_entropy():
     from spion_b200.vocab import distill_top_logits, linear_cross_entropy
     x, w, b, labels, g = inputs(100, 64, 500, torch.bfloat16)
