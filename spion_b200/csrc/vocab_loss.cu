@@ -12,10 +12,11 @@
 //   k_finish             lse and loss of each row, and their sum or mean
 //   k_gemm<GRAD>         z again, for a piece of the vocabulary; leaves G in 16 bits
 //   k_gemm<GRADS>        the two products with it;  k_out joins what was summed apart, and forms db
+//   k_few_*              in place of these three, and of the operands' copies, up to sixteen rows of fp32 on the ordinary units
 //
 // The products are tcgen05 kind::f16, fp32 sums in tensor memory.  A sum there is truncated at every step, so no more than CHAIN steps go to one
 // accumulator where a result has 32 bits; what the accumulators hold is added in fp32 registers.  fp32 operands are three bf16 parts each (8 + 8 + 8 bits, exact) and
-// six products; what is dropped is below 2^-25 of a product.
+// six products (few rows: as they are); what is dropped is below 2^-25 of a product.
 //
 // G is rounded to the type that W has, after it was formed in fp32: the products' other operand has those bits, and their results are rounded to them.  In fp16, whose
 // smallest numbers probabilities of a large vocabulary fall below, G holds 2^13 g_t over the largest |g_t|; the factor comes back in fp32.
@@ -77,6 +78,7 @@ struct Prep {
   Source x, w;
   uint16_t *xs, *ws;        // ws: or null, w is read as it lies
   int direct;               // x can be read as it lies, if all rows count
+  int few;                  // x and w are read as they lie, whatever counts
   float* loss_rows;         // [T] or null: zeros where a row does not count
   float* zt;                // [k][Tp]
   int chunk;                // rows of a CTA, a multiple of 32; of BLOCK where there are more
@@ -314,7 +316,7 @@ template <class E, bool FIRST> __global__ void __launch_bounds__(256) k_prepare(
 #pragma unroll
     for (int w = 0; w < 8; ++w) first += part[0][w], n += part[1][w];
     __syncthreads();
-    const bool in_place = a.direct && n == a.T;
+    const bool in_place = a.few || (a.direct && n == a.T);
     if (blockIdx.x == 0 && threadIdx.x == 0) a.plan.head[0] = n, a.plan.head[1] = 0;
     for (int t0 = chunk * a.chunk; t0 < chunk_end; t0 += BLOCK) {
       const int end = min(chunk_end, t0 + BLOCK);
@@ -354,7 +356,7 @@ template <class E, bool FIRST> __global__ void __launch_bounds__(256) k_prepare(
     if (in_place) return;
   } else {
     n = a.plan.head[0];
-    if (a.direct && n == a.T) return;
+    if (a.few || (a.direct && n == a.T)) return;
     for (int first = chunk * a.chunk; first < min(n, (chunk + 1) * a.chunk); first += BLOCK) {
       const int here = min(BLOCK, min(n, (chunk + 1) * a.chunk) - first);
       for (int i = threadIdx.x; i < here; i += 256) list[i] = a.plan.row[first + i];
@@ -1249,6 +1251,268 @@ __global__ void __launch_bounds__(256, 3) k_out(const __grid_constant__ Leave a)
   }
 }
 
+// ------------------------------------------------------------------------------------------------ few rows of fp32
+// Up to FEW rows bring so little arithmetic to each weight that the weights' bytes bound the call, and three parts of them in bf16 would be written once and read three times:
+// fp32 sums on the ordinary units, w read as it lies, once in the forward and twice in the backward.
+// NT rows at most (8 or 16).  In z a warp takes FOUR rows of w with all rows of x, which wait in shared memory in pieces of FEW_K elements: lanes along the contraction, 4 NT sums a
+// lane, which one transposing sum over the lanes leaves to lane i (r NT + t).  In dx and dW a thread takes E columns and keeps x and dx of them in registers; G comes row by row.
+// Forward and backward, us a call, by tiles / here (2048 to 32000: w read three times and dW written at the measured copy rate take 160): one row 620 / 255, eight 620 / 268, sixteen
+// 621 / 409, which shared memory's reads of x bound, so seventeen and more stay with the tiles (32 rows 623); sixteen of 770 to 50021, in single elements, 541 / 468; two of 2656 to
+// 427 131 / 86; eight of 16 to 50021 187 / 82.
+constexpr int FEW = 16, FOUR = 4, FEW_ROWS = 64;
+constexpr long long FEW_WEIGHTS = 1 << 16;                // below, launches take the time (a forward of 16 x 64 to 400: 16 us by tiles, 13 here) and a row alone keeps the loss it has among many
+template <int NT> constexpr int FEW_K = NT == 8 ? 1280 : 512;
+struct Few {
+  Plan plan; int Tp, k;
+  const float* x; long long ldx;
+  const float* w; long long ldw;
+  const float* bias2; float c1;
+  int V, K;
+  float2* part; int parts;                                // z: [slots, parts] largest, sum
+  float* zt;
+  const float* g; Coef coef;
+  float* G;                                               // [V][NT]
+  float* sums; float *dx, *dw;                            // [parts of V][NT][K]; results or null
+  void* db; int db_type;
+  int columns, groups;                                    // threads along a row of w, and rows side by side
+  int per, all_parts;                                     // rows of w of a CTA; parts of dx
+  int T;
+};
+template <int NT, int E, bool BACK> __global__ void __launch_bounds__(256, 2) k_few_z(const __grid_constant__ Few a) {
+  constexpr int UNROLL = NT == 8 ? 2 : 1, VALUES = FOUR * NT / 32, TARGETS = MAX_TARGETS + 4;       // (rows of targets on different banks)
+  __shared__ __align__(16) float xs[NT * FEW_K<NT>];
+  __shared__ __align__(16) int targets[NT * TARGETS];
+  __shared__ float2 tops[8][NT];
+  next_may_start();
+  wait_for_kernel_before();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane % NT;
+  const int n = *reinterpret_cast<const volatile int*>(a.plan.head);
+  if (n == 0) return;                                     // G is not read either
+  const int k4 = (a.k + 3) / 4 * 4;
+  for (int i = threadIdx.x; i < NT * k4; i += 256) {
+    const int r = i / k4, j = i - r * k4;
+    targets[r * TARGETS + j] = r < n && j < a.k ? a.plan.target[(long long)j * a.Tp + r] : -1;
+  }
+  const bool in = t < n;
+  float top = -INFINITY, sum = 0.f, lse = 0.f, by = 0.f;
+  if (BACK && in) {
+    lse = a.plan.lse[t];
+    by = a.g ? a.g[a.plan.row[t]] : 1.f;
+  }
+  const int pieces = (a.K + FEW_K<NT> - 1) / FEW_K<NT>, piece = ((a.K + pieces - 1) / pieces + 31) / 32 * 32;
+  auto bring = [&](int k0, int len) {
+    for (int r = warp; r < NT; r += 8) {
+      const float* const from = r < n ? a.x + a.plan.row[r] * a.ldx + k0 : nullptr;
+#pragma unroll 8
+      for (int i = lane; i < len; i += 32) xs[r * piece + i] = from ? from[i] : 0.f;
+    }
+  };
+  if (pieces == 1) bring(0, a.K);
+  __syncthreads();
+  for (long long v0 = blockIdx.x * 8ll * FOUR; v0 < a.V; v0 += gridDim.x * 8ll * FOUR) {
+    float acc[FOUR * NT];
+#pragma unroll
+    for (int i = 0; i < FOUR * NT; ++i) acc[i] = 0.f;
+    const float* from[FOUR];
+#pragma unroll
+    for (int r = 0; r < FOUR; ++r) from[r] = a.w + min(v0 + warp * FOUR + r, a.V - 1ll) * a.ldw;
+    for (int k0 = 0; k0 < a.K; k0 += piece) {
+      const int len = min(piece, a.K - k0);
+      if (pieces > 1) {
+        __syncthreads();
+        bring(k0, len);
+        __syncthreads();
+      }
+#pragma unroll UNROLL
+      for (int c = lane * E; c < len; c += 32 * E) {
+        float w[FOUR][E];
+#pragma unroll
+        for (int r = 0; r < FOUR; ++r)
+          if constexpr (E == 4) {
+            const float4 f = __ldcs(reinterpret_cast<const float4*>(from[r] + k0 + c));
+            w[r][0] = f.x, w[r][1] = f.y, w[r][2] = f.z, w[r][3] = f.w;
+          } else {
+            w[r][0] = __ldcs(from[r] + k0 + c);
+          }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          float f[E];
+          if constexpr (E == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(xs + i * piece + c);
+            f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+          } else {
+            f[0] = xs[i * piece + c];
+          }
+#pragma unroll
+          for (int r = 0; r < FOUR; ++r)
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[r * NT + i] = fmaf(w[r][e], f[e], acc[r * NT + i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < VALUES; ++h) {
+      float (&mine)[32] = *reinterpret_cast<float (*)[32]>(acc + 32 * h);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+          const bool up = lane & o;
+          const float give = up ? mine[i] : mine[i + o], keep = up ? mine[i + o] : mine[i];
+          mine[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+      const long long v = v0 + warp * FOUR + (32 * h + lane) / NT;
+      if (v >= a.V) continue;
+      float z = in ? fmaf(mine[0], a.c1, a.bias2[v]) : 0.f;
+      if (BACK) z = in ? ex2(z - lse) * by : 0.f;
+      if (in) {
+        const int4* const list = reinterpret_cast<const int4*>(targets + t * TARGETS);
+        for (int j = 0; j < a.k; j += 4) {
+          const int4 four = list[j / 4];
+          if (four.x != v && four.y != v && four.z != v && four.w != v) continue;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if ((e == 0 ? four.x : e == 1 ? four.y : e == 2 ? four.z : four.w) != v) continue;
+            const long long at = (long long)(j + e) * a.Tp + t;
+            if (BACK) z -= (a.plan.q ? a.plan.q[at] : 1.f) * by;
+            else a.zt[at] = z;
+          }
+        }
+      }
+      if (BACK) {
+        a.G[v * NT + t] = z;
+      } else if (in) {
+        const float m = fmaxf(top, z), least = m == -INFINITY ? 0.f : m;
+        sum = sum * ex2(top - least) + ex2(z - least);
+        top = m;
+      }
+    }
+  }
+  if (BACK) return;
+  auto merge = [&](float m2, float s2) {
+    const float m = fmaxf(top, m2), least = m == -INFINITY ? 0.f : m;
+    sum = sum * ex2(top - least) + s2 * ex2(m2 - least);
+    top = m;
+  };
+#pragma unroll
+  for (int o = 16; o >= NT; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, top, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
+    merge(m2, s2);
+  }
+  if (lane < NT) tops[warp][lane] = make_float2(top, sum);
+  __syncthreads();
+  if (warp > 0 || lane >= n) return;
+  for (int i = 1; i < 8; ++i) merge(tops[i][lane].x, tops[i][lane].y);
+  a.part[(long long)lane * a.parts + blockIdx.x] = make_float2(top, sum);
+}
+template <int NT, int E> __global__ void __launch_bounds__(256, 2) k_few_out(const __grid_constant__ Few a) {
+  __shared__ __align__(16) float G[FEW_ROWS * NT], each[256 * NT * E];
+  next_may_start();
+  wait_for_kernel_before();
+  const int n = *reinterpret_cast<const volatile int*>(a.plan.head);
+  const float alpha = *reinterpret_cast<volatile int*>(&g_vocab_status) != 0 ? not_a_number() : a.coef.alpha(n);
+  const int group = threadIdx.x / a.columns, c = (blockIdx.x * a.columns + threadIdx.x - group * a.columns) * E;
+  const bool on = c < a.K, take = on && a.dx != nullptr && n > 0, give = on && a.dw != nullptr;
+  float x[NT][E], dx[NT][E];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const float* const from = a.x + (t < n ? a.plan.row[t] : 0) * a.ldx + c;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[t][e] = give && t < n ? from[e] : 0.f, dx[t][e] = 0.f;
+  }
+  const long long begin = (long long)blockIdx.y * a.per, end = min(begin + a.per, (long long)a.V);
+  for (long long v0 = begin; v0 < end; v0 += FEW_ROWS) {
+    const int here = (int)min((long long)FEW_ROWS, end - v0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < FEW_ROWS * NT; i += blockDim.x) G[i] = n > 0 && i < here * NT ? a.G[v0 * NT + i] : 0.f;
+    __syncthreads();
+    if (a.db != nullptr && blockIdx.x == 0)
+      for (int i = threadIdx.x; i < here; i += blockDim.x) {
+        float s = 0.f;
+        for (int t = 0; t < NT; ++t) s += G[i * NT + t];
+        store_any(a.db, a.db_type, v0 + i, s * alpha);
+      }
+    constexpr int U = NT == 8 ? 4 : 8;                    // 8 to 2048 x 32000: eight 292 us for 278; 16: four 446 for 421
+    for (int i0 = group; i0 < here; i0 += U * a.groups) {
+      float w[U][E];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * a.groups;
+        const float* const from = a.w + (v0 + i) * a.ldw + c;
+#pragma unroll
+        for (int e = 0; e < E; ++e) w[u][e] = 0.f;
+        if (!take || i >= here) continue;
+        if constexpr (E == 4) {
+          const float4 f = __ldcs(reinterpret_cast<const float4*>(from));
+          w[u][0] = f.x, w[u][1] = f.y, w[u][2] = f.z, w[u][3] = f.w;
+        } else if constexpr (E == 2) {
+          const float2 f = __ldcs(reinterpret_cast<const float2*>(from));
+          w[u][0] = f.x, w[u][1] = f.y;
+        } else {
+          w[u][0] = __ldcs(from);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * a.groups;
+        if (i >= here) break;
+        float f[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = 0.f;
+#pragma unroll
+        for (int t = 0; t < NT; t += 4) {
+          const float4 q = *reinterpret_cast<const float4*>(G + i * NT + t);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            dx[t][e] = fmaf(q.x, w[u][e], dx[t][e]), dx[t + 1][e] = fmaf(q.y, w[u][e], dx[t + 1][e]);
+            dx[t + 2][e] = fmaf(q.z, w[u][e], dx[t + 2][e]), dx[t + 3][e] = fmaf(q.w, w[u][e], dx[t + 3][e]);
+            f[e] = fmaf(q.x, x[t][e], fmaf(q.y, x[t + 1][e], fmaf(q.z, x[t + 2][e], fmaf(q.w, x[t + 3][e], f[e]))));
+          }
+        }
+        if (!give) continue;
+        float* const to = a.dw + (v0 + i) * a.K + c;
+        if constexpr (E == 4) __stcs(reinterpret_cast<float4*>(to), make_float4(f[0] * alpha, f[1] * alpha, f[2] * alpha, f[3] * alpha));
+        else if constexpr (E == 2) __stcs(reinterpret_cast<float2*>(to), make_float2(f[0] * alpha, f[1] * alpha));
+        else __stcs(to, f[0] * alpha);
+      }
+    }
+  }
+  if (a.dx == nullptr || n == 0) return;
+  // the groups' sums in their order
+  const int span = a.columns * E, first = blockIdx.x * span;
+  if (group < a.groups)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < E; ++e) each[(group * NT + t) * span + c - first + e] = dx[t][e];
+  __syncthreads();
+  for (int o = threadIdx.x; o < n * span; o += blockDim.x) {
+    float s = 0.f;
+    for (int g = 0; g < a.groups; ++g) s += each[g * NT * span + o];
+    const int t = o / span, k = first + o - t * span;
+    if (k < a.K) a.sums[((long long)blockIdx.y * NT + t) * a.K + k] = s;
+  }
+}
+// dx: 32 columns of a row and eight shares of the parts a CTA
+template <int NT> __global__ void __launch_bounds__(256) k_few_join(const __grid_constant__ Few a) {
+  __shared__ float shares[8][32];
+  next_may_start();
+  wait_for_kernel_before();
+  const int n = *reinterpret_cast<const volatile int*>(a.plan.head), lane = threadIdx.x & 31, share = threadIdx.x >> 5;
+  const float alpha = *reinterpret_cast<volatile int*>(&g_vocab_status) != 0 ? not_a_number() : a.coef.alpha(n);
+  const long long c = blockIdx.x * 32ll + lane;
+  const int t = blockIdx.y, slot = a.plan.slot[t];
+  float s = 0.f;
+  if (slot >= 0 && c < a.K)
+#pragma unroll 8
+    for (int p = share; p < a.all_parts; p += 8) s += a.sums[((long long)p * NT + slot) * a.K + c];
+  shares[share][lane] = s;
+  __syncthreads();
+  if (share > 0 || c >= a.K) return;
+  for (int i = 1; i < 8; ++i) s += shares[i][lane];
+  a.dx[(long long)t * a.K + c] = slot < 0 ? 0.f : s * alpha;
+}
+
 // ------------------------------------------------------------------------------------------------ host
 using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -1360,6 +1624,7 @@ struct Layout {
   long long T, Tp, K, Kp, V, Vp, k, ldw, parts;           // parts: partial sums of a row
   int planes;
   bool copy_w, direct;                                    // w has to be copied; x can be read as it lies
+  int few, few_vector, few_columns, few_groups, few_chunks, few_parts, few_per;      // rows of fp32 that k_few_* take, 8 or 16 (0: none), and their grid
   bool kept;                                              // the operands' copies stay for the backward
   bool self;                                              // CTAs count for themselves
   long long rows, launches;                               // slots of a pass over z in the forward, and how many there are
@@ -1390,7 +1655,8 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   l->planes = p->type == SPION_F32 ? 3 : 1;
   // places are 32-bit numbers in the tensor maps' coordinates and in the lists of rows
   if (p->T > 0x7fffffff / 4 || p->V > 0x7fffffff / 4 || p->K > 0x7fffffff / 4 || l->Tp * l->planes > 0x7fffffff || l->Vp * l->planes > 0x7fffffff) return SPION_ERR_SHAPE;
-  l->copy_w = p->type == SPION_F32 || ((uintptr_t)p->w % 16) != 0 || (p->ldw * 2) % 16 != 0;
+  l->few = p->type == SPION_F32 && p->T <= FEW && p->V * p->K >= FEW_WEIGHTS ? p->T <= 8 ? 8 : 16 : 0;
+  l->copy_w = !l->few && (p->type == SPION_F32 || ((uintptr_t)p->w % 16) != 0 || (p->ldw * 2) % 16 != 0);
   l->direct = p->type != SPION_F32 && ((uintptr_t)p->x % 16) == 0 && (p->ldx * 2) % 16 == 0 && p->ldx >= p->K;
   l->ldw = l->copy_w ? l->Kp : p->ldw;
   l->self = p->T * p->k <= SELF;
@@ -1406,7 +1672,7 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   // of 160) 18.1 us / 15.6, 32000 (143 of 224) 20.5 / 21.8, 37888 (148 of 256) 19.8 / 23.3, 50000 (261 of 192) 35.6 / 33.0, 128000 (572 of 224) 62.8 / 71.8; 128 rows: 12.7 / 13.2 to
   // 32000, 50.7 / 50.0 to 128000.
   const long long rounds = tiles_of(l->V, 256ll * sms), columns = up(tiles_of(l->V, sms * rounds), 32);
-  l->wide = l->T <= 64 && columns > 128 && 16 * tiles_of(l->V, columns) >= 15 * rounds * sms ? (int)columns : 0;
+  l->wide = !l->few && l->T <= 64 && columns > 128 && 16 * tiles_of(l->V, columns) >= 15 * rounds * sms ? (int)columns : 0;
   l->parts = l->wide ? 4 * tiles_of(l->V, l->wide) : l->pair_z ? 4 * tiles_of(l->V, 256) : 2 * tiles_of(l->V, 128);
   l->rows = std::min(l->Tp, std::max<long long>(PAD, PART_BYTES / (8 * l->parts) / PAD * PAD));
   l->launches = tiles_of(l->Tp, l->rows);
@@ -1423,7 +1689,18 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
     at += (size_t)up(std::max(bytes, 0ll), 256);
     return here;
   };
-  const long long xs_bytes = 2 * l->planes * l->Tp * l->Kp, w_bytes = l->copy_w ? 2 * l->planes * l->Vp * l->Kp : 0;
+  if (l->few) {
+    l->parts = std::min<long long>(tiles_of(l->V, 8 * FOUR), 2 * sms);
+    l->rows = l->Tp, l->launches = 1;
+    l->few_vector = l->K % 4 == 0 && (uintptr_t)p->w % 16 == 0 && p->ldw % 4 == 0;
+    const long long along = tiles_of(l->K, l->few_vector ? 32 / l->few : 1);
+    l->few_chunks = (int)tiles_of(along, 256);
+    l->few_columns = (int)tiles_of(along, l->few_chunks);
+    l->few_groups = 256 / l->few_columns;
+    l->few_per = (int)up(tiles_of(l->V, std::max<long long>(1, 2 * sms / l->few_chunks)), 16);
+    l->few_parts = (int)tiles_of(l->V, l->few_per);
+  }
+  const long long xs_bytes = l->few ? 0 : 2 * l->planes * l->Tp * l->Kp, w_bytes = l->copy_w ? 2 * l->planes * l->Vp * l->Kp : 0;
   l->kept = xs_bytes + w_bytes + 4 * (l->Vp + PAD) <= KEPT_BYTES;
   take(256), take(4 * l->Tp), take(4 * l->Tp), take(4 * l->Tp), take(4 * l->k * l->Tp), take(4 * l->k * l->Tp);
   auto operands = [&] { l->xs = take(xs_bytes), l->w = take(w_bytes), l->bias2 = take(4 * (l->Vp + PAD)); };
@@ -1439,6 +1716,12 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   l->q = take(4 * l->T * l->k);
   l->forward = at;
   at = both;
+  if (l->few) {
+    l->g = take(4 * l->few * l->V);
+    l->dxp = take(4ll * l->few_parts * l->few * l->K);
+    l->backward = at;
+    return SPION_OK;
+  }
   l->g = take(2 * l->planes * l->Tp * l->Gp);
   // (as Parts cuts them: one part, or eight rounds of tiles at most)
   const long long tile = l->tile_g, tn = tiles_of(l->K, tile), most_m = 8 * (l->pair_g ? pairs : sms) / tn;
@@ -1477,11 +1760,11 @@ Prep prep_of(const spion_vocab_problem* p, const Layout& l, void* keep, char* ws
   a.bias = p->bias, a.bias_type = p->bias_type, a.bias2 = (float*)(operands + l.bias2);
   a.x = source_of(p->x, p->type, p->ldx, l.K, l.Kp), a.w = source_of(p->w, p->type, p->ldw, l.K, l.Kp);
   a.xs = (uint16_t*)(operands + l.xs), a.ws = l.copy_w ? (uint16_t*)(operands + l.w) : nullptr;
-  a.direct = l.direct;
+  a.direct = l.direct, a.few = l.few;
   const long long chunks = tiles_of(l.T, l.chunk);
   a.chunk = (int)l.chunk;
   // slices of 64 elements of a row at least, where there are too few chunks to fill the device twice
-  a.slices = (unsigned)std::max<long long>(1, std::min<long long>(l.Kp / 64, 2 * sm_count() / chunks));
+  a.slices = l.few ? 1 : (unsigned)std::max<long long>(1, std::min<long long>(l.Kp / 64, 2 * sm_count() / chunks));
   a.row_ctas = (unsigned)chunks * a.slices;
   a.w_ctas = l.copy_w ? (unsigned)std::min<long long>(tiles_of(l.Vp, 8), 8 * sm_count()) : 0;
   return a;
@@ -1512,6 +1795,31 @@ int logits_args(const spion_vocab_problem* p, const Layout& l, const Prep& prep,
   maps->x = maps->a;
   if (rc == SPION_OK && l.direct) rc = map_of(&maps->x, p->x, l.K, l.T, p->ldx, 128);
   return rc;
+}
+
+Few few_of(const spion_vocab_problem* p, const Layout& l, const Prep& prep) {
+  Few f = {};
+  f.plan = prep.plan, f.Tp = (int)l.Tp, f.k = (int)l.k, f.T = (int)l.T;
+  f.x = static_cast<const float*>(p->x), f.ldx = p->ldx, f.w = static_cast<const float*>(p->w), f.ldw = p->ldw;
+  f.bias2 = prep.bias2, f.c1 = prep.c1, f.V = (int)l.V, f.K = (int)l.K;
+  f.parts = (int)l.parts, f.zt = prep.zt;
+  f.columns = l.few_columns, f.groups = l.few_groups, f.per = l.few_per, f.all_parts = l.few_parts;
+  return f;
+}
+template <bool BACK> int few_z(const Layout& l, const Few& f, cudaStream_t st) {
+  const dim3 grid((unsigned)l.parts);
+  if (l.few == 8) SPION_CUDA_TRY(launch_after(l.few_vector ? k_few_z<8, 4, BACK> : k_few_z<8, 1, BACK>, grid, dim3(256), 0, st, f));
+  else SPION_CUDA_TRY(launch_after(l.few_vector ? k_few_z<16, 4, BACK> : k_few_z<16, 1, BACK>, grid, dim3(256), 0, st, f));
+  return SPION_OK;
+}
+int few_backward(const Layout& l, const Few& f, cudaStream_t st) {
+  const int rc = few_z<true>(l, f, st);
+  if (rc != SPION_OK) return rc;
+  const dim3 grid(l.few_chunks, l.few_parts), block(l.few_columns * l.few_groups), join((unsigned)tiles_of(l.K, 32), (unsigned)l.T);
+  if (l.few == 8) SPION_CUDA_TRY(launch_after(l.few_vector ? k_few_out<8, 4> : k_few_out<8, 1>, grid, block, 0, st, f));
+  else SPION_CUDA_TRY(launch_after(l.few_vector ? k_few_out<16, 2> : k_few_out<16, 1>, grid, block, 0, st, f));
+  if (f.dx != nullptr) SPION_CUDA_TRY(launch_after(l.few == 8 ? k_few_join<8> : k_few_join<16>, join, dim3(256), 0, st, f));
+  return SPION_OK;
 }
 
 int check_problem(const spion_vocab_problem* p, const void* keep, const void* workspace) {
@@ -1556,7 +1864,9 @@ extern "C" int spion_vocab_loss_forward(const spion_vocab_problem* p, float* los
   if ((rc = launch_prepare<true>(p, prep, st)) != SPION_OK) return rc;
   Call<LOGSUM> call;
   Args& a = call.a[0];
-  if ((rc = logits_args(p, l, prep, &a, &call.maps[0])) != SPION_OK) return rc;
+  Few few;
+  if (l.few) few = few_of(p, l, prep), few.part = (float2*)(ws + l.part);
+  if (!l.few && (rc = logits_args(p, l, prep, &a, &call.maps[0])) != SPION_OK) return rc;
   const int tile = l.pair_z ? 256 : 128;
   if (l.wide) {
     a.bn = l.wide;
@@ -1567,7 +1877,7 @@ extern "C" int spion_vocab_loss_forward(const spion_vocab_problem* p, float* los
   const dim3 grid((unsigned)std::min<long long>(tiles_of(std::min(l.T, l.rows), 256 / lanes), std::min(4 * sm_count(), FINISH_CTAS)));
   for (int pass = 0; pass < l.launches; ++pass) {
     a.row0 = (int)(pass * l.rows), a.most = (int)l.rows;
-    if ((rc = launch_logsum(l.pair_z, call, tiles_of(std::min(l.T, l.rows), tile) * tiles_of(l.V, l.wide ? l.wide : tile), st)) != SPION_OK) return rc;
+    if ((rc = l.few ? few_z<false>(l, few, st) : launch_logsum(l.pair_z, call, tiles_of(std::min(l.T, l.rows), tile) * tiles_of(l.V, l.wide ? l.wide : tile), st)) != SPION_OK) return rc;
     const Finish f = {prep.plan, (int)l.Tp, (int)l.k, a.part, a.parts, prep.zt, loss, (double*)(ws + l.cta_loss), p->reduction, a.row0, a.most, pass, (int)l.launches};
     if (lanes == 4) SPION_CUDA_TRY(launch_after(k_finish<4>, grid, dim3(256), 0, st, f));
     else if (lanes == 8) SPION_CUDA_TRY(launch_after(k_finish<8>, grid, dim3(256), 0, st, f));
@@ -1595,6 +1905,13 @@ extern "C" int spion_vocab_loss_backward(const spion_vocab_problem* p, const flo
   const bool by_unit = p->reduction == 0 && p->type == SPION_F16;
   if (by_unit) SPION_CUDA_TRY(launch_after(k_unit, dim3(1), dim3(1024), 0, st, prep.plan, g, unit));
   if (!l.kept && (rc = launch_prepare<false>(p, prep, st)) != SPION_OK) return rc;
+  const Coef coef = {p->reduction == 0 ? nullptr : g, by_unit ? unit : nullptr, p->reduction == 1, prep.inv_tau / gscale};
+  if (l.few) {
+    Few few = few_of(p, l, prep);
+    few.g = p->reduction == 0 ? g : nullptr, few.coef = coef;
+    few.G = (float*)(ws + l.g), few.sums = (float*)(ws + l.dxp), few.dx = static_cast<float*>(dx), few.dw = static_cast<float*>(dw), few.db = db, few.db_type = db_type;
+    return few_backward(l, few, st);
+  }
   Call<GRAD> grad;
   Call<GRADS> grads;
   Args& z = grad.a[0];
@@ -1611,7 +1928,7 @@ extern "C" int spion_vocab_loss_backward(const spion_vocab_problem* p, const flo
   if ((rc = l.pair_g ? units_of<GRADS, true>(&dx_units) : units_of<GRADS, false>(&dx_units)) != SPION_OK) return rc;
   const int tz = l.pair_z ? 256 : 128, tg = l.tile_g;
   z.g = p->reduction == 0 ? g : nullptr, z.G = G, z.ldg = l.Gp, z.gscale = gscale;
-  z.coef = {p->reduction == 0 ? nullptr : g, by_unit ? unit : nullptr, p->reduction == 1, prep.inv_tau / gscale};
+  z.coef = coef;
   z.colsum = db != nullptr ? (float*)(ws + l.colsum) : nullptr;
   const int dx_chunks = (int)tiles_of(std::min(l.Gp, l.V), BK);            // every piece's contraction is cut as the first one's: the parts are added piece by piece
   const unsigned most = 8 * sm_count();

@@ -549,3 +549,103 @@ def test_refusals():
                  lambda: distill_top_logits(x, w, labels[:, None].repeat(1, 129), torch.zeros(10, 129, device="cuda"))):
         with pytest.raises(SpionError):
             call()
+
+
+@pytest.mark.parametrize("T", [1, 2, 3, 8, 9, 15, 16, 17])
+@pytest.mark.parametrize("K,V", [(1, 1048581), (7, 150001), (64, 20000), (130, 9001), (1276, 900), (1284, 1000), (2656, 427), (1030, 4099), (4100, 300), (40000, 31), (16, 70001), (17, 5003), (3, 40001)])
+def test_few_rows_of_fp32_and_many_weights(T, K, V):
+    """A sum over the contraction or the vocabulary takes K / 32 or V / 148 numbers one after another at most, each rounded to half a step: below the bounds of the accumulators."""
+    x, w, b, labels, g = inputs(T, K, V, torch.float32, seed=5, bias=V != 900)
+    labels[T // 2] = labels[0]
+    labelled(x, w, b, labels, g, "none")
+
+
+@pytest.mark.parametrize("T", [4, 16])
+@pytest.mark.parametrize("k", [1, 5, 128])
+def test_few_rows_of_fp32_and_a_teacher(T, k):
+    from spion_b200.vocab import distill_top_logits
+    V = 4099
+    x, w, b, _, g = inputs(T, 300, V, torch.float32, seed=k)
+    idx = torch.rand(T, V, generator=g, device="cuda").argsort(1)[:, :k].contiguous()
+    teacher = 2 * torch.randn(T, k, generator=g, device="cuda")
+    idx[1] = -1
+    if k > 1:
+        idx[0, 1] = idx[0, 0]
+        idx[2, k // 2:] = -1
+    rows = (idx >= 0).any(1).nonzero().squeeze(1)
+    q = torch.softmax(torch.where(idx >= 0, teacher.double() / 2, -float("inf"))[rows], 1)
+    check(lambda x, w, b: distill_top_logits(x, w, idx, teacher, b, 2.0, "sum"), x, w, b, rows, idx[rows].clamp_min(0), q, 2.0, "sum", g)
+
+
+@pytest.mark.parametrize("T", [5, 12])
+def test_few_rows_of_fp32_strides_masks_and_what_is_not_finite(T):
+    from spion_b200.vocab import linear_cross_entropy
+    x, w, b, labels, g = inputs(T, 204, 11000, torch.float32, seed=9)
+    labels[1::3] = -100
+    labels[2] = -100
+
+    def grads(x, w, b, labels, reduction="mean"):
+        x, w, b = (t.detach().requires_grad_() for t in (x, w, b))
+        loss = linear_cross_entropy(x, w, labels, b, reduction=reduction)
+        return [loss.detach(), *torch.autograd.grad(loss, (x, w, b))]
+
+    for a in ((x[:, 1:201], w[:, 1:201]), (x[:, :200], w[:, 4:204]), (x[:1, :200].expand(T, 200), w[::2, :200])):
+        labelled(*a, b[:a[1].shape[0]], torch.where(labels < 0, labels, labels % a[1].shape[0]), g)
+    want = grads(x, w, b, labels)
+    bad = x.clone()
+    bad[1] = float("nan")                                  # a row that does not count
+    for a, e in zip(grads(bad, w, b, labels), want):
+        assert torch.equal(a, e)
+    assert bool((want[1][1] == 0).all())
+    bad[0, 3] = float("inf")                               # one that does
+    got = grads(bad, w, b, labels)
+    assert bool(got[0].isnan()) and bool(got[1][0].isnan().all()) and bool(got[1][3].isfinite().all()) and bool((got[1][1] == 0).all())
+    masked = b.clone()
+    masked[10000:] = -float("inf")                         # entries that no row can have: as if they were not there (their exponentials are zeros)
+    inside = torch.where(labels < 0, labels, labels % 10000)
+    loss, dx, dw, db = grads(x, w, masked, inside)
+    assert bool((dw[10000:] == 0).all()) and bool((db[10000:] == 0).all()) and bool(dx.isfinite().all())
+    labelled(x, w[:10000], b[:10000], inside, g)
+    close(loss, *(t.double() for t in (grads(x, w[:10000], b[:10000], inside)[0], torch.tensor(2.0 ** -18))), "masked entries")
+    outside = labels.clone()
+    outside[0] = 11000
+    assert bool(grads(x, w, b, outside)[0].isnan())
+    outside[:] = -100                                      # no row counts
+    loss, dx, dw, db = grads(x, w, b, outside, "sum")
+    assert bool(loss == 0) and not any(bool(t.any()) for t in (dx, dw, db))
+    assert bool(grads(x, w, b, outside)[0].isnan())
+
+
+def test_few_rows_of_fp32_some_gradients_and_a_captured_call():
+    from spion_b200.vocab import linear_cross_entropy
+    x, w, b, labels, g = inputs(6, 256, 5000, torch.float32, seed=4)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    want = torch.autograd.grad(linear_cross_entropy(leaves[0], leaves[1], labels, leaves[2]), leaves)
+    for i, t in enumerate((x, w, b)):
+        one = [x, w, b]
+        one[i] = t.detach().requires_grad_()
+        got, = torch.autograd.grad(linear_cross_entropy(one[0], one[1], labels, one[2]), one[i])
+        assert torch.equal(got, want[i])
+    del leaves, one
+    stream = torch.cuda.Stream()
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    with torch.cuda.stream(stream):
+        for _ in range(2):
+            torch.autograd.grad(linear_cross_entropy(leaves[0], leaves[1], labels, leaves[2]), leaves)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = torch.autograd.grad(linear_cross_entropy(leaves[0], leaves[1], labels, leaves[2]), leaves)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, e in zip(got, want):
+        assert torch.equal(a, e)
+    with torch.no_grad():
+        x2 = torch.randn_like(x)
+        leaves[0].copy_(x2)
+    graph.replay()
+    torch.cuda.synchronize()
+    fresh = [t.detach().requires_grad_() for t in (x2, w, b)]
+    for a, e in zip(got, torch.autograd.grad(linear_cross_entropy(fresh[0], fresh[1], labels, fresh[2]), fresh)):
+        assert torch.equal(a, e)
