@@ -54,6 +54,7 @@ struct Plan {
   int* slot;                // [T] a row's slot, or -1
   int* row;                 // [Tp] a slot's row
   float* lse;               // [Tp]
+  float* less;              // [Tp], one target: its probability less 1.  From the loss: where the row is sure of its target, p - 1 would keep the rounding of p alone
   int* target;              // [k][Tp]; -1: left out; -2: outside of the vocabulary
   float* q;                 // [k][Tp] (null: one target of weight 1)
 };
@@ -550,7 +551,7 @@ struct Row {
   int slot, found;          // targets among the thread's columns: how many,
   int width;                // of the thread's columns, those of its tile
   uint32_t two;             // and of the first two the column and the target, a byte each
-  float lse, r;
+  float lse, r, less;       // less: ONE, GRAD
 };
 // f(offset, target) of every target among the columns g .. g + 31 of the thread's
 template <int OPT, class F> __device__ __forceinline__ void each_target(const Args& a, const Row& row, int c, int g, F f) {
@@ -595,6 +596,7 @@ template <int MODE, int W, int OPT> __device__ __forceinline__ Row row_of(const 
     }
     if (MODE == GRAD) {
       r.lse = a.plan.lse[r.slot];
+      if (OPT & ONE) r.less = a.plan.less[r.slot];
       r.r = (a.g ? a.g[a.plan.row[r.slot]] * (a.coef.unit ? a.coef.unit[1] : 1.f) : 1.f) * a.gscale;
     }
   }
@@ -613,7 +615,7 @@ template <int MODE, int W, int OPT, int which> __device__ __forceinline__ void e
       acc[(g + 2) / 32][(g + 2) % 32] = fmaf(acc[(g + 2) / 32][(g + 2) % 32], a.c1, b.z), acc[(g + 3) / 32][(g + 3) % 32] = fmaf(acc[(g + 3) / 32][(g + 3) % 32], a.c1, b.w);
     }
     if constexpr (MODE == LOGSUM) {
-      float top = -INFINITY, sum = 0.f;
+      float top = -INFINITY, sum[4] = {0.f, 0.f, 0.f, 0.f};
       if constexpr ((OPT & WIDE) != 0) {                  // columns of the next tile, or of none
 #pragma unroll
         for (int g = 0; g < W; g += 32)
@@ -633,8 +635,8 @@ template <int MODE, int W, int OPT, int which> __device__ __forceinline__ void e
         });
       const float from = top == -INFINITY ? 0.f : top;
 #pragma unroll
-      for (int g = 0; g < W; ++g) sum += ex2(acc[g / 32][g % 32] - from);
-      if (me.in) a.part[(long long)(row - a.row0) * a.parts + part] = make_float2(top, sum);
+      for (int g = 0; g < W; ++g) sum[g % 4] += ex2(acc[g / 32][g % 32] - from);
+      if (me.in) a.part[(long long)(row - a.row0) * a.parts + part] = make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
     } else {
       const float lse = me.lse, r = me.r;
 #pragma unroll
@@ -643,9 +645,15 @@ template <int MODE, int W, int OPT, int which> __device__ __forceinline__ void e
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] = ex2(v[e] - lse) * r;      // zeros of rows that do not count: their lse is inf
         each_target<OPT>(a, me, c, g, [&](int off, int j) {
-          const float q = (a.plan.q ? a.plan.q[(long long)j * a.Tp + slot] : 1.f) * r;
+          if constexpr ((OPT & ONE) != 0) {
+            const float less = me.less * r;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] -= e == off ? q : 0.f;
+            for (int e = 0; e < 32; ++e) v[e] = e == off ? less : v[e];
+          } else {
+            const float q = (a.plan.q ? a.plan.q[(long long)j * a.Tp + slot] : 1.f) * r;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] -= e == off ? q : 0.f;
+          }
         });
         uint16_t* const to = a.G + (long long)row * a.ldg + col + g;
         if constexpr (!(OPT & THREE)) {
@@ -1003,13 +1011,14 @@ template <int LANES> __device__ __forceinline__ float row_loss(const Finish& a, 
   }
   const float all = lane_max<LANES>(top), from = all == -INFINITY ? 0.f : all;
   sum = lane_sum<LANES>(sum * ex2(top - from));
-  lse = from + log2f(sum);
+  const float rest = log2f(sum);
+  lse = from + rest;
   float loss = 0.f;
   for (int j = lane; j < a.k; j += LANES) {
     const long long at = (long long)j * a.Tp + i;
     if (a.plan.target[at] == -1) continue;
     const float q = a.plan.q ? a.plan.q[at] : 1.f;
-    loss += q * ((a.plan.q ? log2f(q) : 0.f) + (lse - a.zt[at]));
+    loss += q * ((a.plan.q ? log2f(q) : 0.f) + ((from - a.zt[at]) + rest));       // (lse is rounded: a sure row's loss is as small as that)
   }
   loss = lane_sum<LANES>(loss) * LN2;
   return lost ? not_a_number() : loss;
@@ -1032,6 +1041,7 @@ template <int LANES> __global__ void __launch_bounds__(256) k_finish(const __gri
     const float loss = row_loss<LANES>(a, min(i, end - 1), lane, lost, lse);      // (all lanes take part in the sums over lanes)
     if (lane == 0 && i < end) {
       a.plan.lse[i] = loss != loss ? loss : lse;            // a row without a loss has no gradient either: NaN
+      if (a.k == 1) a.plan.less[i] = expm1f(-loss);
       if (a.reduction == 0) a.loss[a.plan.row[i]] = loss;
       s += (double)loss;
     }
@@ -1374,7 +1384,7 @@ template <int NT, int E, bool BACK> __global__ void __launch_bounds__(256, 2) k_
           for (int e = 0; e < 4; ++e) {
             if ((e == 0 ? four.x : e == 1 ? four.y : e == 2 ? four.z : four.w) != v) continue;
             const long long at = (long long)(j + e) * a.Tp + t;
-            if (BACK) z -= (a.plan.q ? a.plan.q[at] : 1.f) * by;
+            if (BACK) z = a.k == 1 ? a.plan.less[t] * by : z - (a.plan.q ? a.plan.q[at] : 1.f) * by;
             else a.zt[at] = z;
           }
         }
@@ -1702,7 +1712,7 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   }
   const long long xs_bytes = l->few ? 0 : 2 * l->planes * l->Tp * l->Kp, w_bytes = l->copy_w ? 2 * l->planes * l->Vp * l->Kp : 0;
   l->kept = xs_bytes + w_bytes + 4 * (l->Vp + PAD) <= KEPT_BYTES;
-  take(256), take(4 * l->Tp), take(4 * l->Tp), take(4 * l->Tp), take(4 * l->k * l->Tp), take(4 * l->k * l->Tp);
+  take(256), take(4 * l->Tp), take(4 * l->Tp), take(4 * l->Tp), take(4 * l->Tp), take(4 * l->k * l->Tp), take(4 * l->k * l->Tp);
   auto operands = [&] { l->xs = take(xs_bytes), l->w = take(w_bytes), l->bias2 = take(4 * (l->Vp + PAD)); };
   if (l->kept) operands();
   l->keep = at;
@@ -1740,6 +1750,7 @@ Plan plan_at(const Layout& l, void* keep, bool teacher) {
   p.slot = (int*)c, c += rows_;
   p.row = (int*)c, c += rows_;
   p.lse = (float*)c, c += rows_;
+  p.less = (float*)c, c += rows_;
   p.target = (int*)c, c += targets;
   p.q = teacher ? (float*)c : nullptr;
   return p;

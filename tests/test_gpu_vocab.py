@@ -649,3 +649,30 @@ def test_few_rows_of_fp32_some_gradients_and_a_captured_call():
     fresh = [t.detach().requires_grad_() for t in (x2, w, b)]
     for a, e in zip(got, torch.autograd.grad(linear_cross_entropy(fresh[0], fresh[1], labels, fresh[2]), fresh)):
         assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,K,V", [(1, 64, 200), (5, 64, 200), (150, 64, 200), (3, 400, 200), (1, 64, 20000)])
+def test_rows_that_are_sure_of_their_target(T, K, V, dtype):
+    """Large logits, and losses far below 1: 1 - p and -ln p keep the accuracy of what is left.  Of a row's sum, 1 and little more, each of fewer than 40 additions and the logarithm
+    round by U at most (16 of a thread's numbers, 3 of its four sums, 16 of the parts, 5 over lanes): 48 U; the others' exponentials bring twice a logit's error."""
+    from spion_b200.vocab import distill_top_logits, linear_cross_entropy
+    x, w, _, _, g = inputs(T, K, V, dtype, seed=11, size=0.2)
+    b = torch.full((V,), 300.0, device="cuda")
+    b[3] = 300 + 7 + math.log(V)
+    labels = torch.full((T,), 3, device="cuda")
+    leaf = b.detach().requires_grad_()
+    loss = linear_cross_entropy(x, w, labels, leaf, reduction="none")
+    db, = torch.autograd.grad(loss, leaf, torch.ones_like(loss))
+    z = x.double() @ w.double().t() + b.double()
+    S = x.double().abs() @ w.double().abs().t() + b.double()
+    steps = (6 if dtype == torch.float32 else 1) * (-(-K // 64)) * 4
+    delta = (S * U * (2 * min(steps, 64) + steps / 64 + 24)).amax(1)
+    others = torch.logsumexp(z[:, torch.arange(V, device="cuda") != 3], 1)
+    want = torch.log1p(torch.exp(others - z[:, 3]))
+    bound = 2 * delta * want + 48 * U
+    assert float(want.max()) < 2e-3
+    close(loss.detach(), want, bound, "loss")
+    close(db[3], torch.expm1(-want).sum(), bound.sum() + 2 * T * U * float(want.max()), "db")
+    two = torch.tensor([[3, -1]], device="cuda").expand(T, 2).contiguous()
+    close(distill_top_logits(x, w, two, torch.zeros(T, 2, device="cuda"), b, reduction="none"), want, bound, "one entry of two")
