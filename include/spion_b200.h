@@ -534,6 +534,10 @@ int spion_adamw_step(const spion_adamw_tensor* host_tensors, int count, int type
  *   and of 16 bits.  bias [V] fp32 or 16 bits, or NULL.  k: 1 without a teacher, up to 128 with one.  reduction: 0 none (loss [T]), 1 mean over the rows that count (NaN where none
  *   does), 2 sum (loss: one fp32 number).  The temperature is 1 without a teacher, normally.
  * spion_vocab_sizes: bytes of `keep` (written by the forward, read by the backward) and of the two workspaces, all on 256-byte boundaries.
+ * What `keep` holds follows from how the forward could read x and w.  The backward is given the forward's problem again: sizes, types, k, ignore_index, reduction, temperature, a teacher or
+ * none, and the same values of x, w and bias.  layout 0: x and w lie where they lay, with the same strides.  layout as spion_vocab_layout (> 0, or an error) gave it for the
+ * forward's problem: x, w and bias may lie anywhere, in rows of other strides; what `keep` lacks of them is made again in the workspace.  The forward takes no notice of it.  Sizes of a
+ * backward's workspace are those of the problem that the backward gets; those of `keep`, of the problem that the forward got.
  * The backward takes g [T] (reduction 0) or one number, what arrives at the loss, and writes dx [T, K], dw [V, K] (contiguous, of type `type`, on 32 bytes) and db [V]; each may be
  * NULL.  Sums have a fixed order.  A bounded wait that gives up is reported by spion_linear_status; losses and gradients are NaN until then. */
 typedef struct spion_vocab_problem {
@@ -545,7 +549,9 @@ typedef struct spion_vocab_problem {
   long long ldx, ldw, T, K, V, k, ignore_index;
   int type, bias_type, teacher_type, reduction;
   float temperature;
+  int layout;
 } spion_vocab_problem;
+int spion_vocab_layout(const spion_vocab_problem* host_problem);
 int spion_vocab_sizes(const spion_vocab_problem* host_problem, long long* keep_bytes, long long* forward_bytes, long long* backward_bytes);
 int spion_vocab_loss_forward(const spion_vocab_problem* host_problem, float* loss, void* keep, void* workspace, void* cuda_stream);
 int spion_vocab_loss_backward(const spion_vocab_problem* host_problem, const float* g, const void* keep, void* dx, void* dw, void* db, int db_type,

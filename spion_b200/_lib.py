@@ -37,7 +37,7 @@ class VocabProblem(ctypes.Structure):
     """spion_vocab_problem: operands of a loss over a vocabulary (see include/spion_b200.h)."""
     _fields_ = [(n, c_void_p) for n in ("x", "w", "bias", "teacher", "labels")] + \
         [(n, c_longlong) for n in ("ldx", "ldw", "T", "K", "V", "k", "ignore_index")] + \
-        [(n, c_int) for n in ("type", "bias_type", "teacher_type", "reduction")] + [("temperature", ctypes.c_float)]
+        [(n, c_int) for n in ("type", "bias_type", "teacher_type", "reduction")] + [("temperature", ctypes.c_float), ("layout", c_int)]
 
 
 # name -> (restype, argtypes); every symbol include/spion_b200.h declares
@@ -127,6 +127,7 @@ SIGNATURES = {
                                        c_void_p, c_longlong, c_int, c_void_p]),
     "spion_linear_e4m3": (c_int, [c_void_p, c_longlong, c_void_p] * 2 + [c_void_p, c_int, c_void_p, c_longlong, c_int, c_longlong, c_int, c_int, c_void_p]),
     "spion_adamw_step": (c_int, [ctypes.POINTER(AdamwTensor), c_int, c_int, c_int] + [c_void_p] * 6 + [c_double] * 6 + [ctypes.c_uint, c_int, c_void_p, c_void_p]),
+    "spion_vocab_layout": (c_int, [ctypes.POINTER(VocabProblem)]),
     "spion_vocab_sizes": (c_int, [ctypes.POINTER(VocabProblem)] + [ctypes.POINTER(c_longlong)] * 3),
     "spion_vocab_loss_forward": (c_int, [ctypes.POINTER(VocabProblem)] + [c_void_p] * 4),
     "spion_vocab_loss_backward": (c_int, [ctypes.POINTER(VocabProblem)] + [c_void_p] * 5 + [c_int] + [c_void_p] * 2),

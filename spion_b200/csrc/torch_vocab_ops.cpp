@@ -117,6 +117,7 @@ struct Problem {
   int64_t ignore = -100;
   int reduction = 1;
   double tau = 1;
+  int layout = 0;                        // how the forward read its operands
 };
 // The operands as the kernels read them, and what keeps their memory
 struct Operands {
@@ -137,19 +138,34 @@ struct Operands {
     c.teacher_type = teacher.defined() ? type_code(teacher.scalar_type()) : SPION_F32;
     c.reduction = a.reduction;
     c.temperature = (float)a.tau;
+    c.layout = a.layout;
+  }
+};
+// What came back of a tensor that was saved: hooks may hand out another one, laid out otherwise, but its values have to be the same
+struct Saved {
+  SavedVariable v;
+  std::vector<int64_t> sizes;
+  at::ScalarType type = at::kFloat;
+  c10::Device device = at::kCPU;
+  void operator=(const Tensor& t) { v = save(t), sizes = t.sizes().vec(), type = t.scalar_type(), device = t.device(); }
+  Tensor unpack(const char* node, const char* name) const {
+    const Tensor t = v.unpack();
+    if (t.defined() && (t.sizes() != at::IntArrayRef(sizes) || t.scalar_type() != type || t.device() != device || t.layout() != at::kStrided))
+      refuse(node, std::string("a hook on saved tensors gave ") + name + " back with shape " + shape_of(t) + " and type " + c10::toString(t.scalar_type()) + " on " +
+             t.device().str() + "; it was saved with another");
+    return t;
   }
 };
 
 struct VocabLossNode : public Node {
-  SavedVariable x, w, bias, labels, teacher;
+  Saved x, w, bias, labels, teacher;
   Tensor keep;
   Problem rest;                          // without its tensors
-  std::string who;
   bool released = false;
   std::string name() const override { return "VocabLossBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    x.reset_data(); w.reset_data(); bias.reset_data(); labels.reset_data(); teacher.reset_data();
+    for (Saved* s : {&x, &w, &bias, &labels, &teacher}) s->v.reset_data();
     keep.reset();
     released = true;
   }
@@ -164,7 +180,8 @@ struct VocabLossNode : public Node {
     const bool want_x = task_should_compute_output(0), want_w = task_should_compute_output(1), want_b = num_outputs() > 2 && task_should_compute_output(2);
     if (!grads[0].defined() || !(want_x || want_w || want_b)) return out;
     Problem a = rest;
-    a.x = x.unpack(), a.w = w.unpack(), a.bias = bias.unpack(), a.labels = labels.unpack(), a.teacher = teacher.unpack();
+    const char* me = "VocabLossBackward";
+    a.x = x.unpack(me, "x"), a.w = w.unpack(me, "weight"), a.bias = bias.unpack(me, "bias"), a.labels = labels.unpack(me, "labels"), a.teacher = teacher.unpack(me, "teacher_logits");
     c10::cuda::CUDAGuard guard(a.x.device());
     if (recorded()) return by_operators(a, grads[0], want_x, want_w, want_b);
     if (a.x.numel() == 0) {
@@ -269,6 +286,8 @@ Tensor vocab_loss(const char* op, const Tensor& x, const Tensor& w, const Tensor
       const int rc = spion_vocab_sizes(&o.c, &keeps, &bytes, nullptr);
       if (rc == SPION_ERR_SHAPE) refuse(op, "x has shape " + shape_of(x) + ", weight " + shape_of(w) + ": too large");
       check(rc, "spion_vocab_sizes");
+      a.layout = spion_vocab_layout(&o.c);
+      check(std::min(a.layout, 0), "spion_vocab_layout");
       keep = at::empty({(int64_t)keeps}, x.options().dtype(at::kByte));
       const Tensor ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
       check(spion_vocab_loss_forward(&o.c, (float*)p(loss), p256(keep), p256(ws), stream_of(x)), "spion_vocab_loss_forward");
@@ -278,11 +297,11 @@ Tensor vocab_loss(const char* op, const Tensor& x, const Tensor& w, const Tensor
     auto node = std::shared_ptr<VocabLossNode>(new VocabLossNode(), torch::autograd::deleteNode);
     node->set_next_edges(bias.has_value() ? torch::autograd::collect_next_edges(x, w, *bias) : torch::autograd::collect_next_edges(x, w));
     torch::autograd::set_history(loss, node);
-    node->rest.ignore = ignore, node->rest.reduction = reduction, node->rest.tau = tau;
+    node->rest.ignore = ignore, node->rest.reduction = reduction, node->rest.tau = tau, node->rest.layout = a.layout;
     node->keep = keep;
-    node->x = save(x), node->w = save(w), node->labels = save(a.labels);
-    if (bias.has_value()) node->bias = save(*bias);
-    if (teacher.has_value()) node->teacher = save(*teacher);
+    node->x = x, node->w = w, node->labels = a.labels;
+    if (bias.has_value()) node->bias = *bias;
+    if (teacher.has_value()) node->teacher = *teacher;
   }
   return loss;
 }

@@ -1635,7 +1635,8 @@ struct Layout {
   int planes;
   bool copy_w, direct;                                    // w has to be copied; x can be read as it lies
   int few, few_vector, few_columns, few_groups, few_chunks, few_parts, few_per;      // rows of fp32 that k_few_* take, 8 or 16 (0: none), and their grid
-  bool kept;                                              // the operands' copies stay for the backward
+  bool kept;                                              // the operands' copies stay for the backward (in the backward: and serve it)
+  int given;                                              // how the forward read its operands, as problems carry it
   bool self;                                              // CTAs count for themselves
   long long rows, launches;                               // slots of a pass over z in the forward, and how many there are
   long long chunk;                                        // rows of a CTA of k_prepare
@@ -1652,9 +1653,11 @@ constexpr long long PIECE_BYTES = 512ll << 20;              // of G: half of it 
 constexpr long long KEPT_BYTES = 64ll << 20;              // of copies that stay: small beside the device, and making them again costs launches and, for small calls, most of the time
 constexpr long long PART_BYTES = 256ll << 20;             // of the partial sums of a pass over z: a sixteenth of 16-bit logits, where there are no more than these
 constexpr int FINISH_CTAS = 1024;
+// How a forward read its operands: with this alone the backward knows what `keep` holds, wherever its own operands lie (tensors saved for a backward may come back as copies)
+enum : int { KNOWN = 1, COPIED_W = 2, DIRECT_X = 4 };
 
 int layout_of(const spion_vocab_problem* p, Layout* l) {
-  if (p == nullptr || p->T < 0 || p->K <= 0 || p->V <= 0 || p->k <= 0) return SPION_ERR_ARG;
+  if (p == nullptr || p->layout < 0 || p->layout > (KNOWN | COPIED_W | DIRECT_X) || (p->layout != 0 && !(p->layout & KNOWN)) || p->T < 0 || p->K <= 0 || p->V <= 0 || p->k <= 0) return SPION_ERR_ARG;
   if (p->type != SPION_F32 && p->type != SPION_BF16 && p->type != SPION_F16) return SPION_ERR_ARG;
   if (p->k > MAX_TARGETS) return SPION_ERR_UNSUPPORTED;
   if (!(p->temperature > 0.f) || !(p->temperature < INFINITY) || p->ldx < 0 || p->ldw < p->K) return SPION_ERR_ARG;
@@ -1668,7 +1671,9 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   l->few = p->type == SPION_F32 && p->T <= FEW && p->V * p->K >= FEW_WEIGHTS ? p->T <= 8 ? 8 : 16 : 0;
   l->copy_w = !l->few && (p->type == SPION_F32 || ((uintptr_t)p->w % 16) != 0 || (p->ldw * 2) % 16 != 0);
   l->direct = p->type != SPION_F32 && ((uintptr_t)p->x % 16) == 0 && (p->ldx * 2) % 16 == 0 && p->ldx >= p->K;
-  l->ldw = l->copy_w ? l->Kp : p->ldw;
+  l->given = p->layout ? p->layout : KNOWN | (l->copy_w ? COPIED_W : 0) | (l->direct ? DIRECT_X : 0);
+  const bool copied_w = l->given & COPIED_W, direct_x = l->given & DIRECT_X;
+  if (p->type == SPION_F32 && (direct_x || copied_w == (l->few != 0))) return SPION_ERR_ARG;
   l->self = p->T * p->k <= SELF;
   // every CTA reads the counts of all chunks: 4096 of them at most
   l->chunk = p->T <= 16384 ? 32 : std::max<long long>(BLOCK, up((p->T + 4095) / 4096, BLOCK));
@@ -1710,14 +1715,18 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
     l->few_per = (int)up(tiles_of(l->V, std::max<long long>(1, 2 * sms / l->few_chunks)), 16);
     l->few_parts = (int)tiles_of(l->V, l->few_per);
   }
-  const long long xs_bytes = l->few ? 0 : 2 * l->planes * l->Tp * l->Kp, w_bytes = l->copy_w ? 2 * l->planes * l->Vp * l->Kp : 0;
-  l->kept = xs_bytes + w_bytes + 4 * (l->Vp + PAD) <= KEPT_BYTES;
+  const long long xs_bytes = l->few ? 0 : 2 * l->planes * l->Tp * l->Kp, ws_bytes = 2 * l->planes * l->Vp * l->Kp;
+  l->kept = xs_bytes + (copied_w ? ws_bytes : 0) + 4 * (l->Vp + PAD) <= KEPT_BYTES;
   take(256), take(4 * l->Tp), take(4 * l->Tp), take(4 * l->Tp), take(4 * l->Tp), take(4 * l->k * l->Tp), take(4 * l->k * l->Tp);
-  auto operands = [&] { l->xs = take(xs_bytes), l->w = take(w_bytes), l->bias2 = take(4 * (l->Vp + PAD)); };
-  if (l->kept) operands();
+  auto operands = [&](bool copy) { l->xs = take(xs_bytes), l->w = take(copy ? ws_bytes : 0), l->bias2 = take(4 * (l->Vp + PAD)); };
+  if (l->kept) operands(copied_w);
   l->keep = at;
+  // What the forward kept serves where the operands that it read in place can be read in place again (x: if all rows count; a copy of x is kept if not).  Else both are made anew.
+  l->kept = l->kept && (copied_w || !l->copy_w) && (!direct_x || l->direct);
+  if (l->kept) l->copy_w = copied_w, l->direct = direct_x;
+  l->ldw = l->copy_w ? l->Kp : p->ldw;
   at = 0;
-  if (!l->kept) operands();
+  if (!l->kept) operands(l->copy_w);
   const size_t both = at;
   l->part = take(8 * l->rows * l->parts);
   l->zt = take(4 * l->k * l->Tp);
@@ -1849,6 +1858,14 @@ int* vocab_status_word() {
   return word.on_this_device(g_vocab_status);
 }
 
+extern "C" int spion_vocab_layout(const spion_vocab_problem* p) {
+  Layout l;
+  spion_vocab_problem forward;
+  if (p != nullptr) forward = *p, forward.layout = 0;
+  const int rc = layout_of(p != nullptr ? &forward : nullptr, &l);
+  return rc == SPION_OK ? l.given : rc;
+}
+
 extern "C" int spion_vocab_sizes(const spion_vocab_problem* p, long long* keep_bytes, long long* forward_bytes, long long* backward_bytes) {
   Layout l;
   const int rc = layout_of(p, &l);
@@ -1859,8 +1876,11 @@ extern "C" int spion_vocab_sizes(const spion_vocab_problem* p, long long* keep_b
   return SPION_OK;
 }
 
-extern "C" int spion_vocab_loss_forward(const spion_vocab_problem* p, float* loss, void* keep, void* workspace, void* cuda_stream) {
+extern "C" int spion_vocab_loss_forward(const spion_vocab_problem* problem, float* loss, void* keep, void* workspace, void* cuda_stream) {
   Layout l;
+  spion_vocab_problem own;                                 // with a layout of its own
+  if (problem != nullptr) own = *problem, own.layout = 0;
+  const spion_vocab_problem* const p = problem != nullptr ? &own : nullptr;
   int rc = layout_of(p, &l);
   if (rc != SPION_OK) return rc;
   if (l.T == 0) return p->reduction == 0 ? SPION_OK : SPION_ERR_ARG;      // nothing to take a mean of
