@@ -21,9 +21,25 @@ bool needs_gradient(std::initializer_list<Tensor> ts) {
 }
 void* p256(const Tensor& t) { return t.data_ptr(); }      // (the allocator's blocks begin on 512 bytes)
 
+// What came back of a tensor that was saved: hooks may hand out another one, laid out otherwise, but its values have to be the same
+struct Saved {
+  SavedVariable v;
+  std::vector<int64_t> sizes;
+  at::ScalarType type = at::kFloat;
+  c10::Device device = at::kCPU;
+  void operator=(const Tensor& t) { v = save(t), sizes = t.sizes().vec(), type = t.scalar_type(), device = t.device(); }
+  Tensor unpack(const char* node, const char* name) const {
+    const Tensor t = v.unpack();
+    if (t.defined() && (t.sizes() != at::IntArrayRef(sizes) || t.scalar_type() != type || t.device() != device || t.layout() != at::kStrided))
+      refuse(node, std::string("a hook on saved tensors gave ") + name + " back with shape " + shape_of(t) + " and type " + c10::toString(t.scalar_type()) + " on " +
+             t.device().str() + "; it was saved with another");
+    return t;
+  }
+};
+
 // ------------------------------------------------------------------------------------------------ rows of a table
 struct TokenRowsNode : public Node {
-  SavedVariable ids;
+  Saved ids;
   std::vector<int64_t> table;
   at::ScalarType type = at::kFloat;
   c10::TensorOptions options;
@@ -33,7 +49,7 @@ struct TokenRowsNode : public Node {
   std::string name() const override { return "TokenRowsBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    ids.reset_data();
+    ids.v.reset_data();
     released = true;
   }
   variable_list apply(variable_list&& grads) override {
@@ -44,7 +60,7 @@ struct TokenRowsNode : public Node {
     TORCH_CHECK(!released, "Trying to backward through the graph a second time (the saved tensors have been freed)");
     variable_list out(1);
     if (!grads[0].defined() || !task_should_compute_output(0)) return out;
-    const Tensor i = ids.unpack();
+    const Tensor i = ids.unpack("TokenRowsBackward", "ids").contiguous();      // (a hook may have spread them out)
     const int64_t V = table[0], N = table[1];
     c10::cuda::CUDAGuard guard(i.device());
     if (recorded()) {                    // by torch operators: the gradient of what arrives is part of a graph
@@ -106,7 +122,7 @@ Tensor token_rows(const Tensor& ids, const Tensor& w, double scale, const option
     node->scale = scale;
     node->padding = pad;
     torch::autograd::set_history(y, node);
-    node->ids = save(i);
+    node->ids = i;
   }
   return y;
 }
@@ -139,21 +155,6 @@ struct Operands {
     c.reduction = a.reduction;
     c.temperature = (float)a.tau;
     c.layout = a.layout;
-  }
-};
-// What came back of a tensor that was saved: hooks may hand out another one, laid out otherwise, but its values have to be the same
-struct Saved {
-  SavedVariable v;
-  std::vector<int64_t> sizes;
-  at::ScalarType type = at::kFloat;
-  c10::Device device = at::kCPU;
-  void operator=(const Tensor& t) { v = save(t), sizes = t.sizes().vec(), type = t.scalar_type(), device = t.device(); }
-  Tensor unpack(const char* node, const char* name) const {
-    const Tensor t = v.unpack();
-    if (t.defined() && (t.sizes() != at::IntArrayRef(sizes) || t.scalar_type() != type || t.device() != device || t.layout() != at::kStrided))
-      refuse(node, std::string("a hook on saved tensors gave ") + name + " back with shape " + shape_of(t) + " and type " + c10::toString(t.scalar_type()) + " on " +
-             t.device().str() + "; it was saved with another");
-    return t;
   }
 };
 
