@@ -11,6 +11,8 @@ import torch
 from torch import nn
 
 from . import _ops
+from ._lib import SpionError
+from .attention import untouched
 
 
 def _operands(x, weight):
@@ -35,7 +37,8 @@ def distill_top_logits(x, weight, indices, teacher_logits, bias=None, temperatur
 
 
 class VocabHead(nn.Linear):
-    """``nn.Linear(features, vocabulary)`` whose losses are formed without its logits.  ``tied``: an embedding whose weight is this layer's too."""
+    """``nn.Linear(features, vocabulary)`` whose losses are formed without its logits.  ``tied``: an embedding whose weight is this layer's too.  Losses call no forward of the
+    layer: they are refused where it has hooks (those of older weight normalisations and of pruning form the weight) or a forward of its own."""
 
     def __init__(self, features: int, vocabulary: int, bias: bool = True, tied=None):
         super().__init__(features, vocabulary, bias=bias)
@@ -44,8 +47,15 @@ class VocabHead(nn.Linear):
                 raise ValueError(f"VocabHead: the tied table has shape {tuple(tied.weight.shape)}, the layer {(vocabulary, features)}")
             self.weight = tied.weight
 
+    def _weights(self):
+        if not untouched(self, (type(self),)):
+            raise SpionError("VocabHead: a loss calls no forward of the layer, whose hooks or own forward would be passed over")
+        return self.weight, self.bias
+
     def loss(self, x, labels, ignore_index: int = -100, reduction: str = "mean"):
-        return linear_cross_entropy(x, self.weight, labels, self.bias, ignore_index, reduction)
+        weight, bias = self._weights()
+        return linear_cross_entropy(x, weight, labels, bias, ignore_index, reduction)
 
     def distill(self, x, indices, teacher_logits, temperature: float = 1.0, reduction: str = "mean"):
-        return distill_top_logits(x, self.weight, indices, teacher_logits, self.bias, temperature, reduction)
+        weight, bias = self._weights()
+        return distill_top_logits(x, weight, indices, teacher_logits, bias, temperature, reduction)
