@@ -6,7 +6,8 @@ mask list four times so that scatter hands each replica a copy (:299).  Here eve
 its replica and its shard of the batch; the only exchanges are
 
 * one all-reduce per step over a single flat gradient bucket (<= ~1.6 MB for the LRA
-  encoders: latency-bound on NVLink, so one call, not one per parameter), and
+  encoders: latency-bound on NVLink, so one call, not one per parameter); before it, where
+  ranks' losses are means over unequal numbers of labels, one of those numbers, and
 * one broadcast of each layer's ``nb x nb`` byte mask when the pattern is discovered (rank 0
   discovers from its shard's map, as the reference uses replica 0's, main_conv_ff.py:255).
 
@@ -150,13 +151,25 @@ class FlatGradBucket:
         finally:
             self._attach()
 
-    def allreduce_mean(self, async_op: bool = False):
-        """Average gradients over ranks.  With async_op the handle is returned (wait before the optimizer)."""
+    def allreduce_mean(self, async_op: bool = False, share=None):
+        """Average gradients over ranks.  With async_op the handle is returned (wait before the optimizer).  share: what each rank's count for
+        (``share_of``), where the ranks' losses are means over unequal numbers; else all count alike."""
         if not dist.is_initialized() or dist.get_world_size() == 1:
             return None
-        self.flat.div_(dist.get_world_size())
+        if share is None:
+            self.flat.div_(dist.get_world_size())
+        else:
+            self.flat.mul_(share)
         work = dist.all_reduce(self.flat, op=dist.ReduceOp.SUM, async_op=async_op)
         return work
+
+
+def share_of(count: torch.Tensor) -> torch.Tensor:
+    """This rank's part of all ranks' ``count`` (an integer scalar on its device; 0 where no rank has any), without waiting for the device."""
+    total = count.clone()
+    if dist.is_initialized() and dist.get_world_size() > 1:
+        dist.all_reduce(total, op=dist.ReduceOp.SUM)
+    return count / total.clamp_min(1)
 
 
 def broadcast_mask(mat: torch.Tensor, src: int = 0) -> torch.Tensor:

@@ -271,6 +271,11 @@ class Classifier(nn.Module):
             for layer, (linear8, mlp8) in zip(encoder.layers, kept):
                 layer.mha.linear8, layer.mlp8 = linear8, mlp8
 
+    @staticmethod
+    def counted(label):
+        """How many terms the loss is the mean of, on the labels' device; None: as many on every rank."""
+        return None
+
     def scores(self, ids, mat_lst):
         """Class scores of single- or dual-tower inputs in the sparse phase, without a loss."""
         with torch.autocast(device_type="cuda", dtype=torch.bfloat16, enabled=self.amp):
@@ -328,6 +333,13 @@ class TokenModel(Classifier):
             t, maps = self.model(ids, (ids != 0).float(), mat_lst, is_attn)
             return self.token_loss(t, label), maps
 
+    @staticmethod
+    def counted(label):
+        """Positions that have a label, or a teacher's entry."""
+        if isinstance(label, (tuple, list)):
+            return ((label[0] != -1) & (label[1] != -float("inf"))).any(-1).sum()
+        return (label != -100).sum()
+
     def scores(self, ids, mat_lst):
         """What the loss is formed from, [B, L, dim]: the logits of all positions are not kept."""
         with torch.autocast(device_type="cuda", dtype=torch.bfloat16, enabled=self.amp):
@@ -347,7 +359,8 @@ def _each(f, t):
 
 
 class Trainer:
-    """dense step(s) -> discover -> sparse steps, with one flat-bucket all-reduce per step."""
+    """dense step(s) -> discover -> sparse steps, with one flat-bucket all-reduce per step.  Steps return the loss of this rank's own batch; with
+    several ranks its gradients are those of the mean over all of their batches."""
 
     status_every = 256               # steps after which a wait that gave up in a kernel ends the run
 
@@ -409,14 +422,19 @@ class Trainer:
         if self.allreduce_events is not None:
             e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
             e0.record()
-            self.bucket.allreduce_mean()
+            self._average(label)
             e1.record()
             self.allreduce_events.append((e0, e1))
         else:
-            self.bucket.allreduce_mean()
+            self._average(label)
         self._update()
         self._taken()
         return loss.detach(), maps
+
+    def _average(self, label):
+        """The gradients become those of the mean over all ranks' labels."""
+        count = self.model.counted(label) if dp.world_size() > 1 else None
+        self.bucket.allreduce_mean(share=None if count is None else dp.share_of(count))
 
     def _update(self):
         if not self.fused_opt:
@@ -507,7 +525,7 @@ class Trainer:
         if ev:
             ev[1].record()
         if self._graph_opt is not None:
-            self.bucket.allreduce_mean()                      # eager, between the two replays
+            self._average(self._g_lab)                        # eager, between the two replays
             if ev:
                 ev[2].record()
             self._graph_opt.replay()
