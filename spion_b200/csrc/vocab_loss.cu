@@ -54,7 +54,7 @@ struct Plan {
   int* slot;                // [T] a row's slot, or -1
   int* row;                 // [Tp] a slot's row
   float* lse;               // [Tp]
-  float* less;              // [Tp], one target: its probability less 1.  From the loss: where the row is sure of its target, p - 1 would keep the rounding of p alone
+  float* less;              // [Tp] of a target of weight 1, if the row has one: its probability less 1.  From its own -ln p: where the row is sure of it, p - 1 would keep the rounding of p alone
   int* target;              // [k][Tp]; -1: left out; -2: outside of the vocabulary
   float* q;                 // [k][Tp] (null: one target of weight 1)
 };
@@ -551,7 +551,7 @@ struct Row {
   int slot, found;          // targets among the thread's columns: how many,
   int width;                // of the thread's columns, those of its tile
   uint32_t two;             // and of the first two the column and the target, a byte each
-  float lse, r, less;       // less: ONE, GRAD
+  float lse, r, less;       // less: ONE, GRAD (others read it where they need it)
 };
 // f(offset, target) of every target among the columns g .. g + 31 of the thread's
 template <int OPT, class F> __device__ __forceinline__ void each_target(const Args& a, const Row& row, int c, int g, F f) {
@@ -650,7 +650,13 @@ template <int MODE, int W, int OPT, int which> __device__ __forceinline__ void e
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = e == off ? less : v[e];
           } else {
-            const float q = (a.plan.q ? a.plan.q[(long long)j * a.Tp + slot] : 1.f) * r;
+            float q = a.plan.q[(long long)j * a.Tp + slot];
+            if (q == 1.f) {                               // in place of p, not beside it (others of the row weigh less than its rounding)
+              q = -a.plan.less[slot];
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = e == off ? 0.f : v[e];
+            }
+            q *= r;
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] -= e == off ? q : 0.f;
           }
@@ -999,7 +1005,7 @@ struct Finish {
   int row0, most;           // slots of this launch
   int launch, launches;
 };
-template <int LANES> __device__ __forceinline__ float row_loss(const Finish& a, int i, int lane, bool lost, float& lse) {
+template <int LANES> __device__ __forceinline__ float row_loss(const Finish& a, int i, int lane, bool lost, float& lse, float& sure) {
   const float2* const p = a.part + (long long)(i - a.row0) * a.parts;
   float top = -INFINITY, sum = 0.f;
 #pragma unroll 4
@@ -1014,13 +1020,16 @@ template <int LANES> __device__ __forceinline__ float row_loss(const Finish& a, 
   const float rest = log2f(sum);
   lse = from + rest;
   float loss = 0.f;
+  sure = -INFINITY;
   for (int j = lane; j < a.k; j += LANES) {
     const long long at = (long long)j * a.Tp + i;
     if (a.plan.target[at] == -1) continue;
-    const float q = a.plan.q ? a.plan.q[at] : 1.f;
-    loss += q * ((a.plan.q ? log2f(q) : 0.f) + ((from - a.zt[at]) + rest));       // (lse is rounded: a sure row's loss is as small as that)
+    const float q = a.plan.q ? a.plan.q[at] : 1.f, one = (from - a.zt[at]) + rest;       // (lse is rounded: a sure row's loss is as small as that)
+    loss += q * ((a.plan.q ? log2f(q) : 0.f) + one);
+    if (q == 1.f) sure = one;
   }
   loss = lane_sum<LANES>(loss) * LN2;
+  sure = lane_max<LANES>(sure) * LN2;                       // -ln p of a target of weight 1
   return lost ? not_a_number() : loss;
 }
 // LANES threads per row that counts (4, 8 or 32: the fewest that leave four partial sums or fewer to each, or 32).  A CTA adds its rows' losses, the last one the CTAs', in
@@ -1037,11 +1046,11 @@ template <int LANES> __global__ void __launch_bounds__(256) k_finish(const __gri
   const int end = min(n, a.row0 + a.most);
   for (int i0 = a.row0 + blockIdx.x * ROWS; i0 < end; i0 += gridDim.x * ROWS) {
     const int i = i0 + threadIdx.x / LANES;
-    float lse;
-    const float loss = row_loss<LANES>(a, min(i, end - 1), lane, lost, lse);      // (all lanes take part in the sums over lanes)
+    float lse, sure;
+    const float loss = row_loss<LANES>(a, min(i, end - 1), lane, lost, lse, sure);      // (all lanes take part in the sums over lanes)
     if (lane == 0 && i < end) {
       a.plan.lse[i] = loss != loss ? loss : lse;            // a row without a loss has no gradient either: NaN
-      if (a.k == 1) a.plan.less[i] = expm1f(-loss);
+      a.plan.less[i] = loss != loss ? loss : expm1f(-sure);
       if (a.reduction == 0) a.loss[a.plan.row[i]] = loss;
       s += (double)loss;
     }
@@ -1384,8 +1393,12 @@ template <int NT, int E, bool BACK> __global__ void __launch_bounds__(256, 2) k_
           for (int e = 0; e < 4; ++e) {
             if ((e == 0 ? four.x : e == 1 ? four.y : e == 2 ? four.z : four.w) != v) continue;
             const long long at = (long long)(j + e) * a.Tp + t;
-            if (BACK) z = a.k == 1 ? a.plan.less[t] * by : z - (a.plan.q ? a.plan.q[at] : 1.f) * by;
-            else a.zt[at] = z;
+            if (BACK) {
+              const float q = a.plan.q ? a.plan.q[at] : 1.f;
+              z = q == 1.f ? a.plan.less[t] * by : z - q * by;
+            } else {
+              a.zt[at] = z;
+            }
           }
         }
       }
