@@ -8,9 +8,10 @@
 //                            rows of the table without a token
 //   k_join                   the runs that cross windows
 //
-// Bound by memory: g is read once, dw written once; ids, orders and partial sums are 1/8 of g or less from 64 features on.  Windows and not rows of the table
+// Bound by memory: g is read once, dw written once.  Beside them the workspace has 16 bytes a token for two orders and two fp32 rows a window, N / 8 bytes a token in windows of 64 (N / 4, N / 2
+// in windows of 32, 16): in windows of 64 an eighth of g for 128 features of 16 bits, a tenth for 64 of fp32, a fifth for 64 of 16 bits.  Sorting moves 30 bytes a token a pass, which the L2 cache keeps.  Windows and not rows of the table
 // are what is shared out: tokens are as unequally frequent as words are, and what a window has to load is known before the ids of its runs are looked at (131072 ids of 32000,
-// 1024 bf16 features: by rows, each finding its tokens by a search, 105 us; by windows 71, 4.3 TB/s, and 10 to join; the lookup 52, 5.2 TB/s with what the caches keep).  Every sum is a function of the tokens' order alone: no atomics on floating-point
+// 1024 bf16 features: by rows, each finding its tokens by a search, 105 us; by windows 71, 4.3 TB/s, and 10 to join, 17 with cold caches; the lookup 52, 5.2 TB/s with what the caches keep).  Every sum is a function of the tokens' order alone: no atomics on floating-point
 // numbers, the same bits on every run.
 #include <algorithm>
 #include <type_traits>
@@ -540,7 +541,8 @@ Sizes sizes_of(long long T, long long V, long long N) {
   while (V >> bits) ++bits;                                // keys 0 .. V
   s.passes = (bits + MAX_BITS - 1) / MAX_BITS;
   s.bits = (bits + s.passes - 1) / s.passes;
-  // Windows of 64 tokens where that leaves 16 warps to every multiprocessor, down to 16 where it does not.
+  // Windows of 64 tokens where that leaves 16 warps to every multiprocessor (of 148, whatever the device has: sums and workspaces are a function of the sizes alone), down to 16 where
+  // it does not.
   const long long chunks = (N + 255) / 256;
   s.window = 64;
   while (s.window > 16 && (T + s.window - 1) / s.window * chunks < 148 * 16) s.window /= 2;

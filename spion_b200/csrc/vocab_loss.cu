@@ -14,12 +14,14 @@
 //   k_gemm<GRADS>        the two products with it;  k_out joins what was summed apart, and forms db
 //   k_few_*              in place of these three, and of the operands' copies, up to sixteen rows of fp32 on the ordinary units
 //
-// The products are tcgen05 kind::f16, fp32 sums in tensor memory.  A sum there is truncated at every step, so no more than CHAIN steps go to one
-// accumulator where a result has 32 bits; what the accumulators hold is added in fp32 registers.  fp32 operands are three bf16 parts each (8 + 8 + 8 bits, exact) and
+// The products are tcgen05 kind::f16, fp32 sums in tensor memory.  A sum there is truncated at every step, 2^-23 of it at most, so no more than 64 steps (CHAIN) go to one
+// accumulator where a result has 32 bits, and 256 (LONG_CHAIN) where it is rounded to 16; what the accumulators hold is added in fp32 registers.  fp32 operands are three bf16 parts each (8 + 8 + 8 bits, exact) and
 // six products (few rows: as they are); what is dropped is below 2^-25 of a product.
 //
-// G is rounded to the type that W has, after it was formed in fp32: the products' other operand has those bits, and their results are rounded to them.  In fp16, whose
-// smallest numbers probabilities of a large vocabulary fall below, G holds 2^13 g_t over the largest |g_t|; the factor comes back in fp32.
+// G is rounded to the type that W has, after it was formed in fp32: the products' other operand has those bits, and their results are rounded to them.  It shows in the results: dx and dW
+// of a few products a row are as far from exact ones by G's rounding as by their own (8192 x 2048 to 32000 against 32 logits, bf16: 2.3e-3 of the norm, 1.7e-3 with G in fp32); two parts of G would
+// double both products.  In fp16, whose smallest numbers probabilities of a large vocabulary fall below, G holds 2^13 g_t over the largest |g_t|, rounded up to a power of two; the
+// factor comes back in fp32.  A probability p of a row whose g is a part r of the largest keeps all its bits while p r >= 2^-26, and is 0 below 2^-38.
 // The bias's gradient is summed from G before it is rounded.
 #include <algorithm>
 #include <type_traits>
@@ -54,7 +56,8 @@ struct Plan {
   int* slot;                // [T] a row's slot, or -1
   int* row;                 // [Tp] a slot's row
   float* lse;               // [Tp]
-  float* less;              // [Tp] of a target of weight 1, if the row has one: its probability less 1.  From its own -ln p: where the row is sure of it, p - 1 would keep the rounding of p alone
+  float* less;              // [Tp] of a target of weight 1, if the row has one: its probability less 1.  From its own -ln p, the rounding of whose sum and logarithm
+                            // does not grow with the logits: p - 1, with p from a log of the sum as large as they are, would keep that one's rounding alone where the row is sure of it
   int* target;              // [k][Tp]; -1: left out; -2: outside of the vocabulary
   float* q;                 // [k][Tp] (null: one target of weight 1)
 };
@@ -1024,7 +1027,7 @@ template <int LANES> __device__ __forceinline__ float row_loss(const Finish& a, 
   for (int j = lane; j < a.k; j += LANES) {
     const long long at = (long long)j * a.Tp + i;
     if (a.plan.target[at] == -1) continue;
-    const float q = a.plan.q ? a.plan.q[at] : 1.f, one = (from - a.zt[at]) + rest;       // (lse is rounded: a sure row's loss is as small as that)
+    const float q = a.plan.q ? a.plan.q[at] : 1.f, one = (from - a.zt[at]) + rest;       // (lse is rounded, to 2^-24 of itself; this to that of the numbers added up)
     loss += q * ((a.plan.q ? log2f(q) : 0.f) + one);
     if (q == 1.f) sure = one;
   }
@@ -1275,8 +1278,8 @@ __global__ void __launch_bounds__(256, 3) k_out(const __grid_constant__ Leave a)
 // fp32 sums on the ordinary units, w read as it lies, once in the forward and twice in the backward.
 // NT rows at most (8 or 16).  In z a warp takes FOUR rows of w with all rows of x, which wait in shared memory in pieces of FEW_K elements: lanes along the contraction, 4 NT sums a
 // lane, which one transposing sum over the lanes leaves to lane i (r NT + t).  In dx and dW a thread takes E columns and keeps x and dx of them in registers; G comes row by row.
-// Forward and backward, us a call, by tiles / here (2048 to 32000: w read three times and dW written at the measured copy rate take 160): one row 620 / 255, eight 620 / 268, sixteen
-// 621 / 409, which shared memory's reads of x bound, so seventeen and more stay with the tiles (32 rows 623); sixteen of 770 to 50021, in single elements, 541 / 468; two of 2656 to
+// Forward and backward, us a call, by tiles / here (2048 to 32000: w read three times and dW written at the measured copy rate take 160): one row 620 / 268, eight 620 / 283, sixteen
+// 621 / 410, which shared memory's reads of x bound, so seventeen and more stay with the tiles (32 rows 623); sixteen of 770 to 50021, in single elements, 541 / 468; two of 2656 to
 // 427 131 / 86; eight of 16 to 50021 187 / 82.
 constexpr int FEW = 16, FOUR = 4, FEW_ROWS = 64;
 constexpr long long FEW_WEIGHTS = 1 << 16;                // below, launches take the time (a forward of 16 x 64 to 400: 16 us by tiles, 13 here) and a row alone keeps the loss it has among many
@@ -1640,7 +1643,7 @@ int launch_grad(bool pair, const Call<GRAD>& call, long long most_items, cudaStr
 constexpr long long up(long long x, long long to) { return (x + to - 1) / to * to; }
 constexpr long long tiles_of(long long x, long long tile) { return (x + tile - 1) / tile; }
 constexpr int CHAIN = 16;                                 // 64 steps of 16
-constexpr int LONG_CHAIN = 64;                            // of a result that is rounded to 16 bits
+constexpr int LONG_CHAIN = 64;                            // of a result that is rounded to 16 bits: 256 truncations are 2^-15 of the sum at worst, a sixteenth of fp16's half step
 
 // Sizes and places of a call
 struct Layout {
