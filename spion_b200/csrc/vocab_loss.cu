@@ -14,8 +14,8 @@
 //   k_gemm<GRADS>        the two products with it;  k_out joins what was summed apart, and forms db
 //   k_few_*              in place of these three, and of the operands' copies, up to sixteen rows of fp32 on the ordinary units
 //
-// The products are tcgen05 kind::f16, fp32 sums in tensor memory.  A sum there is truncated at every step, 2^-23 of it at most, so no more than 64 steps (CHAIN) go to one
-// accumulator where a result has 32 bits, and 256 (LONG_CHAIN) where it is rounded to 16; what the accumulators hold is added in fp32 registers.  fp32 operands are three bf16 parts each (8 + 8 + 8 bits, exact) and
+// The products are tcgen05 kind::f16, fp32 sums in tensor memory.  A sum there is truncated at every step, by some 2^-23 of it and always towards zero, so few steps go to one
+// accumulator where a result has 32 bits (chain_of); what the accumulators hold is added in fp32 registers.  fp32 operands are three bf16 parts each (8 + 8 + 8 bits, exact) and
 // six products (few rows: as they are); what is dropped is below 2^-25 of a product.
 //
 // G is rounded to the type that W has, after it was formed in fp32: the products' other operand has those bits, and their results are rounded to them.  It shows in the results: dx and dW
@@ -436,7 +436,7 @@ struct Args {
   int row0, most;                                         // first slot and slots of a launch (0: all)
   int bn;                                                 // WIDE: columns of a tile, a multiple of 32
   int col0;                                               // first column of the piece of the vocabulary
-  int chain;                                              // (chunk, product) pairs that one accumulator takes
+  int chain;                                              // (chunk, product) pairs that one accumulator takes, a multiple of `products`
   int splits;                                             // of the contraction (0: by `cut`)
   Parts cut;
   int fp16;                                               // operands are fp16, else bf16
@@ -828,8 +828,10 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
         const CUtensorMap *const map_a = !TWO && direct ? &maps.x : &maps.a, *const map_b = a_mn && direct ? &maps.x : &maps.b;
         item_at(which ? w1 : w0, i - (which ? items0 : 0), s, m, nn, c0, c1);
         const int ra = m * TILE + rank * 128 + (MODE == LOGSUM ? a.row0 : 0), rb = nn * bn + rank * 128, b0 = a_mn ? 0 : a.col0;
-        for (int c = c0; c < c1 && ok; ++c)
-          for (int p = 0; p < a.products; ++p) {
+        // of an accumulator's chunks the small products first: what is added is truncated beside the sum so far
+        const int most = a.chain / a.products;
+        for (int from = c0; from < c1 && ok; from += most)
+          for (int p = 0, c = from; p < a.products && ok;) {
             ok = mbar_wait(empty + 8 * st, ph);
             if (!ok) break;
             int pa, pb;
@@ -861,6 +863,7 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
             }
             ++fills;
             if (++st == STAGES) st = 0, ph ^= 1;
+            if (++c == min(from + most, c1)) c = from, ++p;
           }
       }
       if (!ok) {                                           // the copies under way end first (a pair's are counted in its first CTA), or this gives up again
@@ -1642,8 +1645,11 @@ int launch_grad(bool pair, const Call<GRAD>& call, long long most_items, cudaStr
 }
 constexpr long long up(long long x, long long to) { return (x + to - 1) / to * to; }
 constexpr long long tiles_of(long long x, long long tile) { return (x + tile - 1) / tile; }
-constexpr int CHAIN = 16;                                 // 64 steps of 16
-constexpr int LONG_CHAIN = 64;                            // of a result that is rounded to 16 bits: 256 truncations are 2^-15 of the sum at worst, a sixteenth of fp16's half step
+// (chunk, product) pairs, of four steps each, that one accumulator takes; a multiple of the products.  fp32: two chunks, whose ten small products go first: 8 steps of 48 count (one after another,
+// 16 pairs, 64 steps: dW of 45754 x 1829 to 29 1.4e-6 of the norm off, so 0.25e-6, and the plain form 0.67e-6; 19652 x 320 to 35829 forward and backward 11.7 ms, with one chunk 12.6, with 16 pairs 11.4).  16 bits: z in small tiles 16
+// steps (3012 x 2464 to 2 in fp16, a small loss: 1.7e-6 of it off, so 0.5e-6, at the same time); in tiles of pairs 64, which keep the multiplying warp busy while the others form exponentials (32 steps: 8192 x
+// 2048 to 32000 4 % slower, 16 steps 20 %).  dx and dW that are rounded to 16 bits: 256 steps, 2^-15 of the sum at worst, a sixteenth of fp16's half step.
+int chain_of(int planes, bool pair, bool rounded) { return planes == 3 ? 12 : rounded ? 64 : pair ? 16 : 4; }
 
 // Sizes and places of a call
 struct Layout {
@@ -1819,7 +1825,7 @@ int logits_args(const spion_vocab_problem* p, const Layout& l, const Prep& prep,
   a->products = l.planes == 1 ? 1 : 6;
   a->plane_a = l.Tp, a->plane_b = l.Vp;
   a->L = (int)l.K;
-  a->chain = CHAIN;
+  a->chain = chain_of(l.planes, l.pair_z, false);
   a->splits = 1;
   a->fp16 = p->type == SPION_F16;
   a->direct_rows = l.direct ? (int)l.T : 0;
@@ -1984,7 +1990,7 @@ extern "C" int spion_vocab_loss_backward(const spion_vocab_problem* p, const flo
     z.col0 = (int)c, z.N = (int)padded;
     if ((rc = launch_grad(l.pair_z, grad, tiles_of(l.T, tz) * tiles_of(padded, tz), st)) != SPION_OK) return rc;
     Args b = z;
-    b.chain = l.planes == 3 ? CHAIN : LONG_CHAIN;
+    b.chain = chain_of(l.planes, l.pair_g, true);
     Leave out = {};
     out.head = prep.plan.head, out.coef = z.coef;
     Args &d = grads.a[DX], &e = grads.a[DW];
