@@ -19,8 +19,8 @@
 // six products (few rows: as they are); what is dropped is below 2^-25 of a product.
 //
 // G is rounded to the type that W has, after it was formed in fp32: the products' other operand has those bits, and their results are rounded to them.  It shows in the results: dx and dW
-// of a few products a row are as far from exact ones by G's rounding as by their own (8192 x 2048 to 32000 against 32 logits, bf16: 2.3e-3 of the norm, 1.7e-3 with G in fp32); two parts of G would
-// double both products.  In fp16, whose smallest numbers probabilities of a large vocabulary fall below, G holds 2^13 g_t over the largest |g_t|, rounded up to a power of two; the
+// of many rows are as far from exact ones by G's rounding as by their own (8192 x 2048 to 32000 against 32 logits, bf16: 2.3e-3 of the norm, 1.7e-3 with G in fp32); two parts of G, which few rows and
+// small calls have (see layout_of), would double both products.  In fp16, whose smallest numbers probabilities of a large vocabulary fall below, G holds 2^13 g_t over the largest |g_t|, rounded up to a power of two; the
 // factor comes back in fp32.  A probability p of a row whose g is a part r of the largest keeps all its bits while p r >= 2^-26, and is 0 below 2^-38.
 // The bias's gradient is summed from G before it is rounded.
 #include <algorithm>
@@ -382,7 +382,7 @@ enum : int { DX, DW };                                    // ... and which of th
 constexpr int BK = 64;                                    // elements of the contraction in a chunk: 128 bytes
 constexpr uint32_t HALF = 128 * BK * 2;
 // What a kernel is made for, beside its product: what it need not do costs registers that the sums want.
-enum : int { ONE = 1, THREE = 2, COLUMNS = 4, WIDE = 8 };  // one target a row (LOGSUM, GRAD); G in three parts, sums of G's columns (GRAD); wide tiles (LOGSUM)
+enum : int { ONE = 1, THREE = 2, COLUMNS = 4, WIDE = 8, TWO = 16 };  // one target a row (LOGSUM, GRAD); G in three or two parts, sums of G's columns (GRAD); wide tiles (LOGSUM)
 // PAIR: two CTAs of a cluster share a tile of 256 x 256; else tiles of 128 x 128, or (WIDE) 128 rows of as many columns as leave one tile to each multiprocessor: few rows, where
 // the weights are all there is to read (16 x 2048 to 32000: 250 tiles of 128 43 us alone, 143 of 224 38).  A thread that writes has 64 columns: what it does with them
 // is a chain of latencies, and four warps a scheduler hide more of each other's than two with 128 columns each do (8192 x 64 to 64000: k_gemm<LOGSUM> 663 us, so 462; k_gemm<GRAD> 911, 698).
@@ -409,16 +409,17 @@ struct Coef {
 };
 // Parts of dx's contraction.  Alone: the number that leaves the fewest units idle in the last round of tiles, a fiftieth less for each part more (its sums are written and read
 // once more), eight at most and eight rounds; 8192 x 2048 from 16384 columns, 256 tiles on 74 pairs: one part 386 us, two 355.  Beside dW's tiles, which fill what is left: the
-// share of a unit in all chunks, and half of the longest tile.
+// share of a unit in all chunks, and half of the longest tile.  G in two parts: up to 32 where there are a few tiles only (71 x 2 to 63111 130 us by eight, 99).
 struct Parts {
   int units, chunks;        // of the first piece of the vocabulary: every piece is cut alike
   int other, other_parts;   // tiles of dW beside it, and the parts of their contraction
+  int alone;                // parts of a tile that is nearly alone (units for four times as many), or 8
   __device__ int of(int tiles, int n) const {
     if (tiles <= 0 || tiles > 8 * units) return 1;
     const int oc = other ? ((n + BK - 1) / BK + other_parts - 1) / other_parts : 0;
     int best = 1;
     long long least = 0;
-    for (int s = 1; s <= 8 && (s == 1 || (tiles * s <= 8 * units && 4 * s <= chunks)); ++s) {
+    for (int s = 1; (s <= 8 || (s <= alone && 4 * tiles * s <= units)) && (s == 1 || (tiles * s <= 8 * units && 4 * s <= chunks)); ++s) {
       const int c = (chunks + s - 1) / s, rounds = (tiles * s + units - 1) / units;
       const long long longest = c > oc ? c : oc;          // times in chunks of a tile, times twice the units
       const long long time = (other ? 2 * ((long long)tiles * chunks + (long long)other * oc) + longest * units : 2ll * rounds * c * units) * (50 + s);
@@ -430,7 +431,7 @@ struct Parts {
 struct Args {
   int on;                                                 // 0: nothing to do (GRADS)
   const int* n;                                           // rows that count
-  int products;                                           // 1, or 6 of three parts
+  int products;                                           // 1; 2 of G's two parts; 6 of three parts
   long long plane_a, plane_b;                             // rows of a part in the maps
   int M, N, L;                                            // rows of D (0: n), columns of D, contraction (0: n)
   int row0, most;                                         // first slot and slots of a launch (0: all)
@@ -499,10 +500,13 @@ __device__ __forceinline__ void pair_mma(uint32_t d_tmem, uint64_t adesc, uint64
 __device__ __forceinline__ void pair_commit(uint32_t bar) {             // on both CTAs' barriers
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
-// the partial products of the split operands, smallest first: (part of A, part of B)
+// the partial products of the split operands, smallest first: (part of A, part of B); two: of A alone
 __device__ __forceinline__ void parts_of(int products, int i, int& a, int& b) {
   a = b = 0;
-  if (products == 1) return;
+  if (products <= 2) {
+    a = products - 1 - i;
+    return;
+  }
   a = (0x010210 >> (4 * i)) & 3;                          // 0 1 2 0 1 0
   b = (0x001012 >> (4 * i)) & 3;                          // 2 1 0 1 0 0
 }
@@ -665,7 +669,7 @@ template <int MODE, int W, int OPT, int which> __device__ __forceinline__ void e
           }
         });
         uint16_t* const to = a.G + (long long)row * a.ldg + col + g;
-        if constexpr (!(OPT & THREE)) {
+        if constexpr (!(OPT & (THREE | TWO))) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t out[8];
@@ -681,12 +685,17 @@ template <int MODE, int W, int OPT, int which> __device__ __forceinline__ void e
 #pragma unroll
             for (int e = 0; e < 16; ++e) left[e] = v[16 * h + e];
 #pragma unroll
-            for (int p = 0; p < 3; ++p) {
+            for (int p = 0; p < (OPT & THREE ? 3 : 2); ++p) {
               uint32_t out[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
-                out[e] = pack_bf16(left[2 * e], left[2 * e + 1]);
-                left[2 * e] -= bf16_lo(out[e]), left[2 * e + 1] -= bf16_hi(out[e]);
+                out[e] = pack2(left[2 * e], left[2 * e + 1], OPT & TWO ? a.fp16 : 0);
+                if (OPT & TWO && a.fp16) {
+                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&out[e]));
+                  left[2 * e] -= f.x, left[2 * e + 1] -= f.y;
+                } else {
+                  left[2 * e] -= bf16_lo(out[e]), left[2 * e + 1] -= bf16_hi(out[e]);
+                }
               }
               st_v8(to + p * plane + 16 * h, out);
             }
@@ -828,8 +837,8 @@ template <int MODE, bool PAIR, int OPT> __global__ void __launch_bounds__(Shape<
         const CUtensorMap *const map_a = !TWO && direct ? &maps.x : &maps.a, *const map_b = a_mn && direct ? &maps.x : &maps.b;
         item_at(which ? w1 : w0, i - (which ? items0 : 0), s, m, nn, c0, c1);
         const int ra = m * TILE + rank * 128 + (MODE == LOGSUM ? a.row0 : 0), rb = nn * bn + rank * 128, b0 = a_mn ? 0 : a.col0;
-        // of an accumulator's chunks the small products first: what is added is truncated beside the sum so far
-        const int most = a.chain / a.products;
+        // of an accumulator's chunks the small products first: what is added is truncated beside the sum so far (two parts of G: chunk by chunk, whose weights the L2 cache still has)
+        const int most = a.products > 2 ? a.chain / a.products : 1;
         for (int from = c0; from < c1 && ok; from += most)
           for (int p = 0, c = from; p < a.products && ok;) {
             ok = mbar_wait(empty + 8 * st, ph);
@@ -1630,8 +1639,14 @@ int launch_logsum(bool pair, const Call<LOGSUM>& call, long long most_items, cud
     return call.a[0].k == 1 ? launch_gemm<LOGSUM, false, ONE | WIDE>(call, most_items, st) : launch_gemm<LOGSUM, false, WIDE>(call, most_items, st);
   return call.a[0].k == 1 ? launch_gemm<LOGSUM, ONE>(pair, call, most_items, st) : launch_gemm<LOGSUM, 0>(pair, call, most_items, st);
 }
-int launch_grad(bool pair, const Call<GRAD>& call, long long most_items, cudaStream_t st) {
+int launch_grad(bool pair, bool two, const Call<GRAD>& call, long long most_items, cudaStream_t st) {
   const Args& a = call.a[0];
+  if (two) switch ((a.k == 1 ? ONE : 0) | (a.colsum != nullptr ? COLUMNS : 0)) {
+    case 0: return launch_gemm<GRAD, false, TWO>(call, most_items, st);
+    case ONE: return launch_gemm<GRAD, false, TWO | ONE>(call, most_items, st);
+    case COLUMNS: return launch_gemm<GRAD, false, TWO | COLUMNS>(call, most_items, st);
+    default: return launch_gemm<GRAD, false, TWO | ONE | COLUMNS>(call, most_items, st);
+  }
   switch ((a.k == 1 ? ONE : 0) | (a.products > 1 ? THREE : 0) | (a.colsum != nullptr ? COLUMNS : 0)) {
     case 0: return launch_gemm<GRAD, 0>(pair, call, most_items, st);
     case 1: return launch_gemm<GRAD, 1>(pair, call, most_items, st);
@@ -1654,7 +1669,7 @@ int chain_of(int planes, bool pair, bool rounded) { return planes == 3 ? 12 : ro
 // Sizes and places of a call
 struct Layout {
   long long T, Tp, K, Kp, V, Vp, k, ldw, parts;           // parts: partial sums of a row
-  int planes;
+  int planes, gparts;                                     // parts of the operands; of G
   bool copy_w, direct;                                    // w has to be copied; x can be read as it lies
   int few, few_vector, few_columns, few_groups, few_chunks, few_parts, few_per;      // rows of fp32 that k_few_* take, 8 or 16 (0: none), and their grid
   bool kept;                                              // the operands' copies stay for the backward (in the backward: and serve it)
@@ -1671,6 +1686,7 @@ struct Layout {
   size_t part, zt, cta_loss, counts, q, forward;
   size_t g, dxp, dwp, colsum, unit, backward;
 };
+constexpr long long FEW_ROWS_G = 64, LITTLE_G = 1 << 23, LITTLE_WORK = 1 << 28;       // rows, logits and products whose G has two parts
 constexpr long long PIECE_BYTES = 512ll << 20;              // of G: half of it costs 16384 x 1024 to 50021, 2458 rows that count, 1240 us -> 1430, and 8192 x 4096 to 128000 nothing
 constexpr long long KEPT_BYTES = 64ll << 20;              // of copies that stay: small beside the device, and making them again costs launches and, for small calls, most of the time
 constexpr long long PART_BYTES = 256ll << 20;             // of the partial sums of a pass over z: a sixteenth of 16-bit logits, where there are no more than these
@@ -1713,7 +1729,12 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
   l->parts = l->wide ? 4 * tiles_of(l->V, l->wide) : l->pair_z ? 4 * tiles_of(l->V, 256) : 2 * tiles_of(l->V, 128);
   l->rows = std::min(l->Tp, std::max<long long>(PAD, PART_BYTES / (8 * l->parts) / PAD * PAD));
   l->launches = tiles_of(l->Tp, l->rows);
-  l->Gp = std::min(l->Vp, std::max<long long>(PAD, PIECE_BYTES / (2 * l->planes * l->Tp) / PAD * PAD));
+  // G beside 16-bit operands: a row's gradient hangs on its target's entry, mostly, whose rounding is then the whole row's, up to twice that of the results; in the mean of many rows both are alike,
+  // of few rows it is as it comes (one row of 1304 to 4 in fp16: 3.3e-4 of the norm off, in fp32 products 2.1e-4; 2 rows of 32 to 9704 in bf16 3.7e-3, 2.2e-3).  So few rows, and calls
+  // of little work, where launches take the time, have G in two parts.  us forward and backward, one part / two: 16 x 2048 to 32000 195 / 215, 64 x 1024 to 50000 175 / 203, 64 x 2048 to 32000 185 / 205;
+  // 2000 x 128 to 1000 89 / 87, 8192 x 32 to 1000 92 / 91, 71 x 2 to 63111 97 / 99; 128 x 4096 to 128000, which keeps one, 1190 / 1390.
+  l->gparts = l->planes == 3 ? 3 : !l->pair_z && ((l->T <= FEW_ROWS_G && 2 * l->T <= l->K) || (l->T * l->V <= LITTLE_G && l->T * l->V * l->K <= LITTLE_WORK)) ? 2 : 1;
+  l->Gp = std::min(l->Vp, std::max<long long>(PAD, PIECE_BYTES / (2 * l->gparts * l->Tp) / PAD * PAD));
   l->Gp = up(tiles_of(l->Vp, tiles_of(l->Vp, l->Gp)), PAD);               // pieces of one size
   l->pair_g = tiles(l->T, l->K) > 0 && tiles(l->T, l->K) + tiles(l->Gp, l->K) >= pairs;
   l->tile_g = l->pair_g ? 256 : 128;
@@ -1763,10 +1784,10 @@ int layout_of(const spion_vocab_problem* p, Layout* l) {
     l->backward = at;
     return SPION_OK;
   }
-  l->g = take(2 * l->planes * l->Tp * l->Gp);
-  // (as Parts cuts them: one part, or eight rounds of tiles at most)
+  l->g = take(2 * l->gparts * l->Tp * l->Gp);
+  // (as Parts cuts them: one part, or eight rounds of tiles at most, in so many parts)
   const long long tile = l->tile_g, tn = tiles_of(l->K, tile), most_m = 8 * (l->pair_g ? pairs : sms) / tn;
-  l->dxp = take(4 * std::max(tiles_of(l->T, tile), std::min(most_m, 8 * tiles_of(l->T, tile))) * tile * l->Kp);
+  l->dxp = take(4 * std::max(tiles_of(l->T, tile), std::min(most_m, (l->gparts == 2 ? 32 : 8) * tiles_of(l->T, tile))) * tile * l->Kp);
   l->dwp = take(l->dw_splits > 1 ? 4 * l->dw_splits * up(l->Gp, l->tile_g) * l->Kp : 0);
   l->colsum = take(4 * (l->Tp / 32) * l->Gp);
   l->unit = take(256);
@@ -1970,10 +1991,10 @@ extern "C" int spion_vocab_loss_backward(const spion_vocab_problem* p, const flo
   Args& z = grad.a[0];
   Maps &xm = grads.maps[DX], &wm = grads.maps[DW];
   if ((rc = logits_args(p, l, prep, &z, &grad.maps[0])) != SPION_OK) return rc;
-  if ((rc = map_of(&xm.a, G, l.Gp, l.planes * l.Tp, l.Gp, 128)) != SPION_OK) return rc;
+  if ((rc = map_of(&xm.a, G, l.Gp, l.gparts * l.Tp, l.Gp, 128)) != SPION_OK) return rc;
   if ((rc = l.copy_w ? map_of(&xm.b, prep.ws, l.Kp, l.planes * l.Vp, l.Kp, 64) : map_of(&xm.b, p->w, l.K, l.V, l.ldw, 64)) != SPION_OK) return rc;
   xm.x = xm.a;
-  if ((rc = map_of(&wm.a, G, l.Gp, l.planes * l.Tp, l.Gp, 64)) != SPION_OK) return rc;
+  if ((rc = map_of(&wm.a, G, l.Gp, l.gparts * l.Tp, l.Gp, 64)) != SPION_OK) return rc;
   if ((rc = map_of(&wm.b, prep.xs, l.Kp, l.planes * l.Tp, l.Kp, 64)) != SPION_OK) return rc;
   wm.x = wm.b;
   if (l.direct && (rc = map_of(&wm.x, p->x, l.K, l.T, p->ldx, 64)) != SPION_OK) return rc;
@@ -1988,9 +2009,9 @@ extern "C" int spion_vocab_loss_backward(const spion_vocab_problem* p, const flo
   for (long long c = 0; c < l.V; c += l.Gp) {
     const long long columns = std::min(l.Gp, l.V - c), padded = up(columns, PAD);
     z.col0 = (int)c, z.N = (int)padded;
-    if ((rc = launch_grad(l.pair_z, grad, tiles_of(l.T, tz) * tiles_of(padded, tz), st)) != SPION_OK) return rc;
+    if ((rc = launch_grad(l.pair_z, l.gparts == 2, grad, tiles_of(l.T, tz) * tiles_of(padded, tz), st)) != SPION_OK) return rc;
     Args b = z;
-    b.chain = chain_of(l.planes, l.pair_g, true);
+    b.chain = chain_of(l.planes, l.pair_g, true), b.products = l.gparts == 2 ? 2 : z.products;
     Leave out = {};
     out.head = prep.plan.head, out.coef = z.coef;
     Args &d = grads.a[DX], &e = grads.a[DW];
@@ -1998,7 +2019,7 @@ extern "C" int spion_vocab_loss_backward(const spion_vocab_problem* p, const flo
     d.on = dx != nullptr, e.on = dw != nullptr;
     const bool together = dx != nullptr && dw != nullptr;
     d.N = (int)l.K, d.L = (int)columns, d.splits = 0;
-    d.cut = {dx_units, dx_chunks, together ? (int)(tiles_of(up(std::min(l.Gp, l.V), PAD), tg) * tiles_of(l.K, tg) * l.dw_splits) : 0, l.dw_splits};
+    d.cut = {dx_units, dx_chunks, together ? (int)(tiles_of(up(std::min(l.Gp, l.V), PAD), tg) * tiles_of(l.K, tg) * l.dw_splits) : 0, l.dw_splits, l.gparts == 2 ? 32 : 8};
     d.plane_a = l.Tp, d.plane_b = l.Vp;
     d.out = (float*)(ws + l.dxp), d.ldo = l.Kp, d.add = c > 0;
     e.M = (int)padded, e.N = (int)l.K, e.L = 0, e.splits = l.dw_splits;

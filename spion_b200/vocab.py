@@ -2,8 +2,8 @@
 largest logits.  Rows that do not count cost nothing.
 
 x [.., features] and weight [vocabulary, features] have one type, fp32, bf16 or fp16; under ``torch.autocast`` both are converted to its type.  bias [vocabulary] is fp32 or
-16 bits.  The products are exact to fp32's rounding for fp32 operands; for 16-bit ones the gradient of the logits is rounded to the operands' type before it is multiplied
-(fp16: in units of 2^-13 of the largest |gradient| that arrives at a row, so probabilities below 2^-26 over a row's part of that lose bits in the row's dx, and below 2^-38 all of them).
+16 bits.  The products are exact to fp32's rounding for fp32 operands; for 16-bit ones the gradient of the logits is rounded to the operands' type before it is multiplied, to twice its bits
+where rows or work are few (fp16: in units of 2^-13 of the largest |gradient| that arrives at a row, so probabilities below 2^-26 over a row's part of that lose bits in the row's dx, and below 2^-38 all of them).
 Under autocast fp32 weights are converted by torch in each call, and their gradient back.
 Losses are fp32.  ``reduction``: "mean" over the rows that count (NaN, with gradients of zero, where none does), "sum", or "none" (0 where a row does not count).
 """

@@ -52,3 +52,26 @@ def test_gradients_of_fp32(T, K, V):
         bound = (9 + (length / 128 / 2) ** 0.5 / 2 + 4) * U
         off = float((p.double() - q).norm() / q.norm())
         assert off <= bound, (off / U, bound / U)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,K,V", [(1, 64, 50), (1, 1304, 4), (2, 32, 9704), (6, 29, 2760), (11, 2, 63111), (40, 256, 30000), (64, 128, 20000), (300, 16, 5)])
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_gradients_of_few_rows_are_rounded_once(T, K, V, dtype, reduction):
+    """A row's gradient hangs on its target's entry of G, whose rounding to 16 bits would be the whole row's: up to twice the result's own.  With twice the bits, 2^-16 or less of an entry, the
+    result is as far off as its own rounding makes it; next to a tie that may be the other way, of no more than a part 2^-16 / (half a step) of the numbers: a tenth covers it."""
+    from spion_b200.vocab import linear_cross_entropy
+    for seed in range(8):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        x = torch.randn(T, K, generator=g, device="cuda").to(dtype).requires_grad_()
+        w = (torch.randn(V, K, generator=g, device="cuda") / K ** 0.5).to(dtype).requires_grad_()
+        b = torch.zeros(V, device="cuda")
+        b[0] = torch.log(torch.tensor(float(V))) + torch.randn((), generator=g, device="cuda")      # a likely entry, and the label: its probability is a half or so
+        labels = torch.zeros(T, dtype=torch.long, device="cuda")
+        given = torch.randn(T, generator=g, device="cuda") if reduction == "none" else torch.ones((), device="cuda")
+        got = torch.autograd.grad(linear_cross_entropy(x, w, labels, b, reduction=reduction), (x, w), given)
+        a, c = x.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+        want = torch.autograd.grad(torch.nn.functional.cross_entropy(a @ c.t() + b.double(), labels, reduction=reduction), (a, c), given.double())
+        for p, q in zip(got, want):
+            own = float((q.to(dtype).double() - q).norm())
+            assert float((p.double() - q).norm()) <= 1.1 * own + 2.0 ** -15 * float(q.norm()), (seed, float((p.double() - q).norm()) / own)
