@@ -50,7 +50,7 @@ class VocabHead(nn.Linear):
             self.weight = tied.weight
 
     def _weights(self):
-        if not untouched(self, (type(self),)):
+        if not untouched(self, (type(self),)) or type(self).forward is not nn.Linear.forward:
             raise SpionError("VocabHead: a loss calls no forward of the layer, whose hooks or own forward would be passed over")
         return self.weight, self.bias
 

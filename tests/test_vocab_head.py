@@ -34,6 +34,23 @@ def test_a_layer_with_hooks_has_no_loss(hook):
                 call()
 
 
+def test_a_class_with_a_forward_of_its_own_has_no_loss():
+    class Scaled(VocabHead):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    class Named(VocabHead):
+        pass
+
+    for call in calls_on_cpu(Scaled(8, 10)):
+        with pytest.raises(SpionError, match="forward"):
+            call()
+    for head in (Named(8, 10), nn.utils.parametrizations.weight_norm(Named(8, 10))):
+        for call in calls_on_cpu(head):
+            with pytest.raises(SpionError, match="CUDA"):
+                call()
+
+
 @pytest.mark.gpu
 def test_weights_that_are_formed_by_parametrisations_are_served():
     """These change the attribute, not the forward."""
